@@ -1,0 +1,476 @@
+// Layer norm over rows on gfx950: forward, and backward with the weight's and bias's gradients.
+//
+//   y = w (x - m) r + b,  m = mean x,  r = 1 / sqrt(mean (x - m)^2 + epsilon)
+//   with xh = (x - m) r and c = dy w:  dx = r (c - mean c - xh mean(c xh)),
+//   dw = sum over rows of dy xh,  db = sum over rows of dy.
+//
+// Bound by memory: x is read once and kept in registers between the statistics (the variance about
+// the mean, not a difference of squares) and the result.  G threads share a row, E columns each, the
+// fewest that hold it: eight rows a wave at width 64, one at 512, a whole workgroup at 8192.  Rows
+// wider than 32768 are read again for each pass.  The backward's workgroups walk over rows with the
+// column sums in registers and write one partial row each, added up in a fixed order by a second launch.
+#include <math.h>
+
+#include <algorithm>
+
+#include "gdn2_common.h"
+#include "gdn2_status.h"
+
+namespace gdn2 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kPartials = 512;  // workgroups of the backward (fixed: the sums' order)
+
+struct LnArgs {
+    View x, dy;
+    int64_t T, H, rows;   // row r = (b, t, h)
+    int W;
+    float epsilon;
+    const float *weight, *bias;
+    void *y;              // y or dx, dense
+    float *mean, *inverse;
+    float *part_w, *part_b;
+};
+
+// N adjacent elements as floats.
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T *p, int64_t s, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = Elem<T>::load(p, 0);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    } else {
+        const float4 q = *reinterpret_cast<const float4 *>(p);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T *p, const float (&v)[N]) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) Elem<T>::store(e, i, v[i]);
+    __builtin_memcpy(__builtin_assume_aligned(p, N * sizeof(T)), e, sizeof e);
+}
+
+// Sums over the G threads of a row, in every one of them.
+template <int G, int K>
+__device__ __forceinline__ void row_sum(float (&x)[K], float *red) {
+#pragma unroll
+    for (int d = 1; d < (G < 64 ? G : 64); d *= 2)
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], d);
+    if constexpr (G > 64) {
+        constexpr int WAVES = G / 64;
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[k * WAVES + wave] = x[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            x[k] = red[k * WAVES];
+            for (int i = 1; i < WAVES; ++i) x[k] += red[k * WAVES + i];
+        }
+    }
+}
+
+__device__ __forceinline__ int64_t row_at(const View &x, const LnArgs &p, int64_t r) {
+    const uint32_t n = (uint32_t)r, H = (uint32_t)p.H, T = (uint32_t)p.T;
+    const uint32_t bt = n / H, h = n % H;
+    return (int64_t)(bt / T) * x.s0 + (int64_t)(bt % T) * x.s1 + (int64_t)h * x.s2;
+}
+
+// Columns of thread l, piece j: N adjacent ones from N (l + j G).
+template <typename T, int N, int G, int E>
+struct Row {
+    static constexpr int P = E / N;
+    float v[P][N];
+    __device__ __forceinline__ void load(const void *base, int64_t at, int64_t s, int l, int W) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int c = N * (l + j * G);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[j][e] = 0.f;
+            if (c < W) load_n<T, N>(reinterpret_cast<const T *>(base) + at + c * (N == 1 ? s : 1), s, v[j]);
+        }
+    }
+};
+
+template <typename T, int N, int G, int E>
+__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel(LnArgs p) {
+    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
+    __shared__ float red[2 * (G > 64 ? G / 64 : 1)];
+    const int l = threadIdx.x % G;
+    const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
+    const bool on = r < p.rows;  // the row's threads stay for its sums
+    typedef Row<T, N, G, E> R;
+    R x{};
+    if (on) x.load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < R::P; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[0] += x.v[j][e];
+    row_sum<G, 1>(s, red);
+    const float m = s[0] / p.W;
+    s[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < R::P; ++j)
+        if (N * (l + j * G) < p.W)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                x.v[j][e] -= m;
+                s[0] = fmaf(x.v[j][e], x.v[j][e], s[0]);
+            }
+    row_sum<G, 1>(s, red);
+    const float inv = 1.f / sqrtf(s[0] / p.W + p.epsilon);
+    if (!on) return;
+    if (l == 0) {
+        if (p.mean) p.mean[r] = m;
+        if (p.inverse) p.inverse[r] = inv;
+    }
+    T *y = reinterpret_cast<T *>(p.y) + r * p.W;
+#pragma unroll
+    for (int j = 0; j < R::P; ++j) {
+        const int c = N * (l + j * G);
+        if (c >= p.W) continue;
+        float o[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            o[e] = fmaf(x.v[j][e] * inv, p.weight[c + e], p.bias ? p.bias[c + e] : 0.f);
+        store_n<T, N>(y + c, o);
+    }
+}
+
+template <typename T, int N, int G, int E>
+__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kernel(LnArgs p) {
+    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
+    __shared__ float red[2 * (G > 64 ? G / 64 : 1)];
+    __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
+    const int l = threadIdx.x % G, g = threadIdx.x / G;
+    typedef Row<T, N, G, E> R;
+    float w[R::P][N], dw[R::P][N], db[R::P][N];
+#pragma unroll
+    for (int j = 0; j < R::P; ++j) {
+        const int c = N * (l + j * G);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[j][e] = c < p.W ? p.weight[c + e] : 0.f, dw[j][e] = db[j][e] = 0.f;
+    }
+    // Every group of the workgroup makes the same number of turns: row_sum has barriers.
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t r = r0 + g;
+        const bool on = r < p.rows;
+        R x{}, dy{};
+        float m = 0.f, inv = 0.f;
+        if (on) {
+            x.load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
+            dy.load(p.dy.data, row_at(p.dy, p, r), p.dy.s3, l, p.W);
+            m = p.mean[r], inv = p.inverse[r];
+        }
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < R::P; ++j)
+            if (on && N * (l + j * G) < p.W)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float xh = (x.v[j][e] - m) * inv, d = dy.v[j][e];
+                    dw[j][e] = fmaf(d, xh, dw[j][e]);
+                    db[j][e] += d;
+                    const float c = d * w[j][e];
+                    s[0] += c;
+                    s[1] = fmaf(c, xh, s[1]);
+                    x.v[j][e] = xh, dy.v[j][e] = c;
+                }
+        row_sum<G, 2>(s, red);
+        if (!on || !p.y) continue;
+        const float a = s[0] / p.W, c2 = s[1] / p.W;
+        T *dx = reinterpret_cast<T *>(p.y) + r * p.W;
+#pragma unroll
+        for (int j = 0; j < R::P; ++j) {
+            const int c = N * (l + j * G);
+            if (c >= p.W) continue;
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = inv * ((dy.v[j][e] - a) - x.v[j][e] * c2);
+            store_n<T, N>(dx + c, o);
+        }
+    }
+    // The workgroup's column sums, over its groups in order.
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float *part = k ? p.part_b : p.part_w;
+        if (!part) continue;
+        part += (int64_t)blockIdx.x * p.W;
+        if constexpr (ROWS == 1) {
+#pragma unroll
+            for (int j = 0; j < R::P; ++j)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int c = N * (l + j * G) + e;
+                    if (c < p.W) part[c] = k ? db[j][e] : dw[j][e];
+                }
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < R::P; ++j)
+#pragma unroll
+                for (int e = 0; e < N; ++e) cols[g * G * E + N * (l + j * G) + e] = k ? db[j][e] : dw[j][e];
+            __syncthreads();
+            for (int c = threadIdx.x; c < p.W; c += THREADS) {
+                float t = cols[c];
+                for (int i = 1; i < ROWS; ++i) t += cols[i * G * E + c];
+                part[c] = t;
+            }
+        }
+    }
+}
+
+// Rows of any width: one workgroup of 1024, the row read again for each pass.
+constexpr int kLong = 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(kLong) ln_forward_long(LnArgs p) {
+    __shared__ float red[kLong / 64];
+    const int64_t r = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(p.x.data) + row_at(p.x, p, r);
+    float s[1] = {0.f};
+    for (int64_t c = threadIdx.x; c < p.W; c += kLong) s[0] += Elem<T>::load(x, c * p.x.s3);
+    row_sum<kLong, 1>(s, red);
+    const float m = s[0] / p.W;
+    s[0] = 0.f;
+    for (int64_t c = threadIdx.x; c < p.W; c += kLong) {
+        const float d = Elem<T>::load(x, c * p.x.s3) - m;
+        s[0] = fmaf(d, d, s[0]);
+    }
+    row_sum<kLong, 1>(s, red);
+    const float inv = 1.f / sqrtf(s[0] / p.W + p.epsilon);
+    if (threadIdx.x == 0) {
+        if (p.mean) p.mean[r] = m;
+        if (p.inverse) p.inverse[r] = inv;
+    }
+    for (int64_t c = threadIdx.x; c < p.W; c += kLong)
+        Elem<T>::store(p.y, r * p.W + c, fmaf((Elem<T>::load(x, c * p.x.s3) - m) * inv, p.weight[c],
+                                              p.bias ? p.bias[c] : 0.f));
+}
+
+// dx of one row a workgroup.
+template <typename T>
+__global__ void __launch_bounds__(kLong) ln_backward_long(LnArgs p) {
+    __shared__ float red[2 * kLong / 64];
+    const int64_t r = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(p.x.data) + row_at(p.x, p, r);
+    const T *dy = reinterpret_cast<const T *>(p.dy.data) + row_at(p.dy, p, r);
+    const float m = p.mean[r], inv = p.inverse[r];
+    float s[2] = {0.f, 0.f};
+    for (int64_t c = threadIdx.x; c < p.W; c += kLong) {
+        const float d = Elem<T>::load(dy, c * p.dy.s3) * p.weight[c];
+        s[0] += d;
+        s[1] = fmaf(d, (Elem<T>::load(x, c * p.x.s3) - m) * inv, s[1]);
+    }
+    row_sum<kLong, 2>(s, red);
+    const float a = s[0] / p.W, b = s[1] / p.W;
+    for (int64_t c = threadIdx.x; c < p.W; c += kLong) {
+        const float d = Elem<T>::load(dy, c * p.dy.s3) * p.weight[c];
+        const float xh = (Elem<T>::load(x, c * p.x.s3) - m) * inv;
+        Elem<T>::store(p.y, r * p.W + c, inv * ((d - a) - xh * b));
+    }
+}
+
+// Column sums of wide rows: 256 columns and every gridDim.y-th row a workgroup.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ln_columns_long(LnArgs p) {
+    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (c >= p.W) return;
+    float dw = 0.f, db = 0.f;
+    for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
+        const float d = Elem<T>::load(p.dy.data, row_at(p.dy, p, r) + c * p.dy.s3);
+        const float x = Elem<T>::load(p.x.data, row_at(p.x, p, r) + c * p.x.s3);
+        dw = fmaf(d, (x - p.mean[r]) * p.inverse[r], dw);
+        db += d;
+    }
+    if (p.part_w) p.part_w[(int64_t)blockIdx.y * p.W + c] = dw;
+    if (p.part_b) p.part_b[(int64_t)blockIdx.y * p.W + c] = db;
+}
+
+// Partial rows -> dweight (blockIdx.y 0) and dbias (1): 64 columns a workgroup, sixteen waves over
+// the partials, then the waves in order.
+__global__ void __launch_bounds__(1024) ln_sum_kernel(const float *pw, const float *pb, int64_t W,
+                                                      int64_t n, float *dw, float *db) {
+    __shared__ float red[16][64];
+    const float *part = blockIdx.y ? pb : pw;
+    float *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (c < W)
+#pragma unroll 8
+        for (int64_t k = wave; k < n; k += 16) s += part[k * W + c];
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < W) {
+        float t = red[0][lane];
+        for (int i = 1; i < 16; ++i) t += red[i][lane];
+        out[c] = t;
+    }
+}
+
+constexpr int64_t kWide = 32768;  // wider rows do not fit the registers of one workgroup
+
+int64_t row_threads(int64_t W) {  // at most, as launch_width has them
+    return W <= 1024 ? 64 : W <= 8192 ? 256 : 1024;
+}
+
+int check_ln(const gdn2_rows_shape *s, const gdn2_view *x, const float *weight) {
+    if (!s) return fail(GDN2_ERR_ARGUMENT, "shape is null");
+    if (s->batch < 0 || s->time < 0 || s->heads < 0 || s->width < 1)
+        return fail(GDN2_ERR_SHAPE, "width must be >= 1 and the row axes >= 0");
+    const int64_t lim = (int64_t)1 << 31;
+    if (s->batch >= lim || s->time >= lim || s->heads >= lim || s->width >= lim ||
+        (s->batch && s->time && s->heads > (lim / 2) / s->batch / s->time))
+        return fail(GDN2_ERR_SHAPE, "at most 2^30 rows, and widths below 2^31");
+    const int64_t rows = s->batch * s->time * s->heads;
+    if (rows >= ((int64_t)1 << 32) / row_threads(s->width))  // threads of one launch
+        return fail(GDN2_ERR_SHAPE, "too many rows: at most 2^26 of up to 1024 columns, 2^24 of up to "
+                                    "8192 and 2^22 of wider ones");
+    GDN2_TRY(check_view(x, "x", -1, rows == 0));
+    if (!weight) return fail(GDN2_ERR_ARGUMENT, "weight is null");
+    return GDN2_OK;
+}
+
+// Whether every row is a run of 16-byte pieces.
+bool vec_rows(const gdn2_view *v, int64_t W) {
+    const int64_t es = v->dtype == GDN2_BF16 ? 2 : 4;
+    if (v->stride[3] != 1 || ((uintptr_t)v->data & 15) || W * es % 16) return false;
+    for (int d = 0; d < 3; ++d)
+        if (v->stride[d] * es % 16) return false;
+    return true;
+}
+
+template <typename T, int N, int G, int E, bool BWD>
+void launch_one(const LnArgs &a, int64_t partials, hipStream_t st) {
+    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
+    const int64_t groups = (a.rows + ROWS - 1) / ROWS;
+    if constexpr (BWD)
+        hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
+    else
+        hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E>), dim3((unsigned)groups), dim3(THREADS), 0, st, a);
+}
+
+// Threads a row by its width, eight columns each while they fit a wave, more beyond.
+template <typename T, int N, bool BWD>
+void launch_width(const LnArgs &a, int64_t partials, hipStream_t st) {
+    if (a.W <= 64) launch_one<T, N, 8, 8, BWD>(a, partials, st);
+    else if (a.W <= 128) launch_one<T, N, 16, 8, BWD>(a, partials, st);
+    else if (a.W <= 256) launch_one<T, N, 32, 8, BWD>(a, partials, st);
+    else if (a.W <= 512) launch_one<T, N, 64, 8, BWD>(a, partials, st);
+    else if (a.W <= 1024) launch_one<T, N, 64, 16, BWD>(a, partials, st);
+    else if (a.W <= 2048) launch_one<T, N, 256, 8, BWD>(a, partials, st);
+    else if (a.W <= 8192) launch_one<T, N, 256, 32, BWD>(a, partials, st);
+    else launch_one<T, N, 1024, 32, BWD>(a, partials, st);
+}
+
+template <bool BWD>
+void launch_ln(const LnArgs &a, int dtype, bool vec, int64_t partials, hipStream_t st) {
+    const bool bf = dtype == GDN2_BF16;
+    if (vec && bf) launch_width<bf16_t, 8, BWD>(a, partials, st);
+    else if (vec) launch_width<float, 4, BWD>(a, partials, st);
+    else if (bf) launch_width<bf16_t, 1, BWD>(a, partials, st);
+    else launch_width<float, 1, BWD>(a, partials, st);
+}
+
+int64_t partial_rows(int64_t rows) { return std::max<int64_t>(1, std::min(rows, kPartials)); }
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon, const gdn2_view *x,
+                            const float *weight, const float *bias, void *y, float *mean,
+                            float *inverse, void *stream) {
+    GDN2_TRY(check_ln(shape, x, weight));
+    LnArgs a{};
+    a.rows = shape->batch * shape->time * shape->heads;
+    if (a.rows == 0) return ok();
+    if (!y) return fail(GDN2_ERR_ARGUMENT, "y is null");
+    a.x = make_view(x);
+    a.T = shape->time, a.H = shape->heads, a.W = (int)shape->width;
+    a.epsilon = epsilon;
+    a.weight = weight, a.bias = bias;
+    a.y = y, a.mean = mean, a.inverse = inverse;
+    hipStream_t st = (hipStream_t)stream;
+    if (a.W > kWide) {
+        if (x->dtype == GDN2_BF16)
+            hipLaunchKernelGGL((ln_forward_long<bf16_t>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
+        else hipLaunchKernelGGL((ln_forward_long<float>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
+    } else {
+        launch_ln<false>(a, x->dtype, vec_rows(x, a.W) && ((uintptr_t)y & 15) == 0, 0, st);
+    }
+    return launch_status(hipGetLastError(), "gdn2_layer_norm_forward");
+}
+
+size_t gdn2_layer_norm_workspace_bytes(int64_t rows, int64_t width) {
+    if (rows < 0 || width < 1) return 0;
+    return (size_t)(2 * 4 * partial_rows(rows) * width);
+}
+
+int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, const float *weight,
+                             const float *mean, const float *inverse, const gdn2_view *dy, void *dx,
+                             float *dweight, float *dbias, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+    GDN2_TRY(check_ln(shape, x, weight));
+    LnArgs a{};
+    a.rows = shape->batch * shape->time * shape->heads;
+    GDN2_TRY(check_view(dy, "dy", x->dtype, a.rows == 0));
+    if (a.rows && (!mean || !inverse)) return fail(GDN2_ERR_ARGUMENT, "mean and inverse must be non-null");
+    a.W = (int)shape->width;
+    const int64_t n = partial_rows(a.rows);
+    const bool params = dweight || dbias;
+    if (params) {
+        if (!workspace || workspace_bytes < gdn2_layer_norm_workspace_bytes(a.rows, a.W))
+            return fail(GDN2_ERR_WORKSPACE, "workspace is too small: %zu bytes needed",
+                        gdn2_layer_norm_workspace_bytes(a.rows, a.W));
+        if ((uintptr_t)workspace & 15) return fail(GDN2_ERR_ARGUMENT, "workspace must be 16-byte aligned");
+    }
+    a.x = make_view(x), a.dy = make_view(dy);
+    a.T = shape->time, a.H = shape->heads;
+    a.weight = weight;
+    a.mean = const_cast<float *>(mean), a.inverse = const_cast<float *>(inverse);
+    a.y = dx;
+    if (params) {
+        float *ws = (float *)workspace;
+        a.part_w = dweight ? ws : nullptr;
+        a.part_b = dbias ? ws + n * a.W : nullptr;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const bool bf = x->dtype == GDN2_BF16;
+    if (a.rows && a.W > kWide) {
+        if (dx) {
+            if (bf) hipLaunchKernelGGL((ln_backward_long<bf16_t>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
+            else hipLaunchKernelGGL((ln_backward_long<float>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
+        }
+        if (params) {
+            const dim3 grid((unsigned)((a.W + (int64_t)kThreads - 1) / kThreads), (unsigned)n);
+            if (bf) hipLaunchKernelGGL((ln_columns_long<bf16_t>), grid, dim3(kThreads), 0, st, a);
+            else hipLaunchKernelGGL((ln_columns_long<float>), grid, dim3(kThreads), 0, st, a);
+        }
+    } else if (a.rows && (dx || params)) {
+        launch_ln<true>(a, x->dtype,
+                        vec_rows(x, a.W) && vec_rows(dy, a.W) && ((uintptr_t)dx & 15) == 0, n, st);
+    }
+    if (params)
+        hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((a.W + 63) / 64), 2), dim3(1024), 0, st,
+                           a.part_w, a.part_b, a.W, a.rows ? n : 0, dweight, dbias);
+    return launch_status(hipGetLastError(), "gdn2_layer_norm_backward");
+}
+
+}  // extern "C"

@@ -497,7 +497,14 @@ from .train_ops import (FusedAdamW, adamw_update, cross_entropy_rows,  # noqa: E
                         linear_cross_entropy)
 from .hola_ops import HolaReadOutput, hola_read, hola_schedule  # noqa: E402
 from . import lm_ops  # noqa: E402
+from .linear_ops import (layer_norm, layer_norm_backward, layer_norm_forward,  # noqa: E402
+                         linear_attention, linear_attention_backward, linear_attention_forward,
+                         linear_attention_step, q8_values, swiglu_q8, swiglu_q8_backward,
+                         swiglu_q8_forward)
 
 __all__ += ["causal_conv", "l2_norm", "rms_norm", "decay", "cross_entropy_rows",
             "linear_cross_entropy", "adamw_update", "FusedAdamW", "HolaReadOutput", "hola_read",
-            "hola_schedule", "lm_ops"]
+            "hola_schedule", "lm_ops", "linear_attention", "linear_attention_forward",
+            "linear_attention_backward", "linear_attention_step", "layer_norm",
+            "layer_norm_forward", "layer_norm_backward", "swiglu_q8", "swiglu_q8_forward",
+            "swiglu_q8_backward", "q8_values"]

@@ -522,6 +522,85 @@ GDN2_API int gdn2_hola_backward(const gdn2_hola_shape *shape, const gdn2_view *q
                                 float *dk, float *dv, float *dsink, void *workspace,
                                 size_t workspace_bytes, void *stream);
 
+/* ---- Linear attention with a decay for each head ----------------------------- */
+/* No counterpart in the reference: the scalar-gate scan without its erase term.
+ * Per (batch, head) and valid token:
+ *   S = exp(g) S (S zeroed first when reset[t] != 0),  S += k v^T,  out = S^T q.
+ * Padding tokens (valid == 0) emit zero output and keep the state; what q, k, v,
+ * g and d_output hold there is not used.  q, k: [B,T,H,keys], v: [B,T,H,values],
+ * F32 or BF16 (one dtype); g F32 [B,T,H] of any sign (stride 0 for one decay a
+ * head; -inf empties the state like a reset); valid, reset F32 [B,T], views or
+ * NULL (all valid, no reset); initial F32 [B,H,keys,values], a view or NULL.
+ * Any element strides; rows of 16-byte aligned unit-stride channels are read
+ * fastest.  batch * heads * ceil(time / 32) is at most 2^21.  A value that is not
+ * finite reaches the tokens that see it and no others.
+ *
+ * output is dense in q's dtype, final_state F32 dense.  The checkpoint (16-byte
+ * aligned, sized by the query for the dtype) holds start states of segments of
+ * the sequence for the backward; the forward needs it also where none follows. */
+GDN2_API size_t gdn2_linear_checkpoint_bytes(const gdn2_shape *shape, int32_t dtype);
+GDN2_API int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
+                              const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
+                              const gdn2_view *reset, const gdn2_view *initial, void *output,
+                              float *final_state, void *checkpoint, size_t checkpoint_bytes,
+                              void *stream);
+
+/* VJP.  d_output ([B,T,H,values], q's dtype, strided); d_final_state F32 dense or
+ * NULL (zero).  dq, dk, dv dense in q's dtype; dg [B,T,H] and its sums over batch
+ * and time dg_heads [H], d_initial [B,H,keys,values], F32 dense; any of them may
+ * be NULL, and what only it needs is then not computed.  dg is 0 at padding, at
+ * resets and where exp(g) is 0. */
+GDN2_API size_t gdn2_linear_workspace_bytes(const gdn2_shape *shape, int32_t dtype);
+GDN2_API int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
+                                  const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
+                                  const gdn2_view *reset, const gdn2_view *initial,
+                                  const void *checkpoint, size_t checkpoint_bytes,
+                                  const gdn2_view *d_output, const float *d_final_state, void *dq,
+                                  void *dk, void *dv, float *dg, float *dg_heads,
+                                  float *d_initial, void *workspace, size_t workspace_bytes,
+                                  void *stream);
+
+/* One token (time == 1) on a carried state [B,H,keys,values], F32 dense, updated
+ * in place; output dense in q's dtype. */
+GDN2_API int gdn2_linear_step(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
+                              const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
+                              const gdn2_view *reset, float *state, void *output, void *stream);
+
+/* ---- Layer norm ---------------------------------------------------------------- */
+/* No counterpart in the reference, whose norms are l2 and RMS.  Rows of
+ * [batch, time, heads, width] (x and dy F32 or BF16 views of one dtype, any
+ * strides; an empty row axis is allowed):
+ *   y = weight (x - mean) inverse + bias,  inverse = 1/sqrt(var + epsilon)
+ * with var the mean square about the mean.  weight, bias [width] F32 (bias may be
+ * NULL); y and dx dense in x's dtype; mean, inverse [rows] F32 (the forward takes
+ * NULL where no backward follows).  dx, dweight, dbias may each be NULL.  dweight
+ * and dbias are summed in a fixed order through the workspace. */
+GDN2_API int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon,
+                                     const gdn2_view *x, const float *weight, const float *bias,
+                                     void *y, float *mean, float *inverse, void *stream);
+GDN2_API size_t gdn2_layer_norm_workspace_bytes(int64_t rows, int64_t width);
+GDN2_API int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x,
+                                      const float *weight, const float *mean, const float *inverse,
+                                      const gdn2_view *dy, void *dx, float *dweight, float *dbias,
+                                      void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- SwiGLU that keeps its input in 8 bits -------------------------------------- */
+/* No counterpart in the reference.  h [rows, 2 width] = [gate | up] -> a [rows,
+ * width] = silu(gate) up, rounded once, and what the backward reads instead of h:
+ * codes [rows, 2 width] and, for each block of 32 columns of a half (the last may
+ * be short), one exponent: exponents [rows, 2 ceil(width / 32)], e + 127.  2^e is
+ * the smallest power of two with max |h| <= 127 2^e in the block (e >= -126), a
+ * code is h 2^-e to the nearest whole number, ties to even, and the kept value is
+ * code 2^e.  A block with a value that is not finite has exponent 255 and reads
+ * back as NaN.  The backward takes the VJP at the kept values: dh [rows, 2 width],
+ * and a at the kept values again (may be NULL).  Dense, F32 or BF16 (one dtype);
+ * widths that are a multiple of 8 in 16-byte aligned buffers run fastest. */
+GDN2_API int gdn2_swiglu_q8_forward(int64_t rows, int64_t width, int32_t dtype, const void *h,
+                                    void *a, int8_t *codes, uint8_t *exponents, void *stream);
+GDN2_API int gdn2_swiglu_q8_backward(int64_t rows, int64_t width, int32_t dtype,
+                                     const int8_t *codes, const uint8_t *exponents,
+                                     const void *da, void *dh, void *a, void *stream);
+
 /* Measurement hook.  No counterpart in the reference: it serves benchmarks
  * that need the duration of each kernel of the chunked paths, measured on the
  * stream the kernels run on.  After gdn2_stage_timing(1), every chunked
