@@ -29,7 +29,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kCols = 64;       // columns of c (and of the state) that a workgroup owns
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
-constexpr int kWalks = 3;       // walks of one launch (dq, dv, dk)
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
 // order() reads a row in the order in which two accumulator tiles hold their 32 rows.
@@ -96,48 +95,51 @@ __device__ __forceinline__ Split3 split3(const float (&x)[8]) {
     return s;
 }
 
-// One walk over the chunks: see the head of the file.
+// One walk over the chunks: see the head of the file.  Tensor views are [B, T, H, channels].
 struct Walk {
-    View a, b, c;
-    const void *dot_x;      // optional: dot_t = sum over columns of row_t (a_t S) dot_x_t
-    int64_t dx0, dx1, dx2, dx3;
-    int a_vec, b_vec, c_vec;
-    int ka, vc;             // widths of a and b, and of c and out
-    int rev;                // 1: from the last chunk to the first
-    const float *init;      // start state of a segment, or null (zero)
-    int64_t i_bh, i_seg, i_row, i_col;
-    const float *first;     // start state of the walk's first segment where init has none for it
-    int64_t f_b, f_h, f_row, f_col;
-    float *fin;             // state after the walk's last segment, or null
-    int64_t n_bh, n_row, n_col;
+    View a, b, c, d;        // d: see DOT
+    View g, valid, reset;   // valid.data, reset.data may be null
+    View first;             // state before the walk, [B, H, ka, vc] (data may be null: zero)
+    const float *starts;    // states before every segment, or null: taken from first by a prewalk
+    int64_t s_bh;
+    int s_row, s_col;
+    float *starts_out;      // the prewalk's states before every segment, or null
+    float *fin;             // state after the walk, [B H, ka, vc], or null
     void *out;              // dense [B, T, H, vc], or null
-    float *dots;            // [slices, BH, T]
-    float *dot_sums;        // [slices, BH, chunks]
-    const float *edge;      // with dots of a reversed walk: the forward's state at the segment's start
-    int64_t e_bh, e_seg, e_row, e_col;
-    const float *edge_first;
-    int64_t ef_b, ef_h, ef_row, ef_col;
-    float *edges;           // [slices, BH, segments]: <edge, state at the walk's end of the segment>
-    float *seg_state;       // carry walk: state that the segment adds, [BH, segments, ka, vc]
-    float *seg_decay;       // [BH, segments]
-    int slices;
+    float *dots, *dot_sums; // [slices, B H, T], [slices, B H, chunks]: see DOT
+    float *pairs;           // [slices, B H, T]
+    View edge_first;        // with DOT of a reversed walk: the other direction's states, as above
+    const float *edge;
+    float *edges;           // [slices, B H, segments]: <edge, state after the walk's segment>
+    float *totals;          // [B H, chunks]: decay of each chunk, or null
+    float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
+    float *seg_decay;       // [B H, segments]
+    int64_t T;
+    int H;
+    int ka, vc;             // widths of a and b, and of c, d and out
+    int chunks, seg_chunks, segments, slices;
 };
 
-struct WalkArgs {
-    Walk w[kWalks];
-    int walks;
-    int64_t B, T, H;
-    View g, valid, reset;   // valid.data, reset.data may be null
-    float *totals;          // [BH, chunks]: decay of each chunk, written by the first reversed walk
-    int chunks, seg_chunks, segments;
-    int first_seg;          // carry walk: the first segment that it covers
-    int per_group;          // workgroups of one (batch, head, segment)
-};
+// DPP moves of 64 bits; lanes without a source read 0.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)dpp<CTRL, ROWS>((int)(uint32_t)u);
+    const uint32_t hi = (uint32_t)dpp<CTRL, ROWS>((int)(uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// One step of a scan that stops at a new segment: adds the source lane's sum if its segment is ours.
+// A lane without a source reads 0 for both, and adds 0.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ void seg_step(double &G, int seg1) {
+    const double y = dpp64<CTRL, ROWS>(G);
+    if (dpp<CTRL, ROWS>(seg1) == seg1) G += y;
+}
 
 // Gates of one chunk, from one wave (lane = token).
 template <int C>
 struct GateTile {
-    float hi[C], lo[C];     // sum of g log2(e) up to each token: hi + lo, both float32
+    float hi[C], lo[C];     // sum of g log2(e) in the token's segment: hi + lo, both float32
     float row[C], col[C];   // factor of the start state and of the token's update (0: none of it)
     float step[C];          // exp(g), 0 at a cut, 1 at padding
     int seg[C];             // cuts up to the token; -1 at padding
@@ -149,7 +151,7 @@ struct GateIn {
 };
 
 template <int C>
-__device__ __forceinline__ GateIn gate_load(const WalkArgs &p, int64_t b, int64_t h, int64_t chunk) {
+__device__ __forceinline__ GateIn gate_load(const Walk &p, int64_t b, int64_t h, int64_t chunk) {
     const int l = lane_id();
     const int64_t t = chunk * C + l;
     GateIn x{0.f, 0.f, 0.f};
@@ -161,92 +163,93 @@ __device__ __forceinline__ GateIn gate_load(const WalkArgs &p, int64_t b, int64_
     return x;
 }
 
-template <int C>
-__device__ __forceinline__ void gate_store(const GateIn &x, int rev, GateTile<C> *o) {
+template <int C, bool REV>
+__device__ __forceinline__ void gate_store(const GateIn &x, GateTile<C> *o) {
     const int l = lane_id();
     const bool val = x.valid != 0.f;
     float g = val ? x.g : 0.f;
     const bool cut = val && (x.reset != 0.f || g < kCut);
     if (cut) g = 0.f;
-    int seg = cut;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int z = __shfl_up(seg, d);
-        if (l >= d) seg += z;
-    }
+    const int seg = wave_scan_add((int)cut);
     // The sums are taken in 64 bits, since differences of float32 sums over a chunk would lose digits,
     // and start again at a cut, so that a gate that is not finite ends there.
     double G = (double)g * 1.4426950408889634;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double y = __shfl_up(G, d);
-        const int z = __shfl_up(seg, d);
-        if (l >= d && z == seg) G += y;
-    }
+    seg_step<0x111>(G, seg + 1);
+    seg_step<0x112>(G, seg + 1);
+    seg_step<0x114>(G, seg + 1);
+    seg_step<0x118>(G, seg + 1);
+    seg_step<0x142, 0xA>(G, seg + 1);
+    seg_step<0x143, 0xC>(G, seg + 1);
     const double last = __shfl(G, 63);
-    const int end = __shfl(seg, 63);
+    const int end = __builtin_amdgcn_readlane(seg, 63);
     if (l < C) {
-        const float gam = seg == 0 && val ? exp2f((float)G) : 0.f;
-        const float lam = seg == end && val ? exp2f((float)(last - G)) : 0.f;
+        const float gam = seg == 0 && val ? __builtin_amdgcn_exp2f((float)G) : 0.f;
+        const float lam = seg == end && val ? __builtin_amdgcn_exp2f((float)(last - G)) : 0.f;
         o->hi[l] = (float)G;
         o->lo[l] = (float)(G - (double)(float)G);
-        o->row[l] = rev ? lam : gam;
-        o->col[l] = rev ? gam : lam;
-        o->step[l] = cut ? 0.f : val ? expf(g) : 1.f;
+        o->row[l] = REV ? lam : gam;
+        o->col[l] = REV ? gam : lam;
+        o->step[l] = cut ? 0.f : val ? __builtin_amdgcn_exp2f(g * 1.44269504f) : 1.f;
         o->seg[l] = val ? seg : -1;
-        if (l == 0) o->tot = end == 0 ? exp2f((float)last) : 0.f;
+        if (l == 0) o->tot = end == 0 ? __builtin_amdgcn_exp2f((float)last) : 0.f;
     }
 }
 
-// 16 bytes of one row of a sequence tensor; zero beyond its width, past the end and at padding.
-template <typename T>
-__device__ __forceinline__ uint4 load_piece(const View &x, int vec, int64_t b, int64_t t, int64_t h,
-                                            int c0, int width, bool on) {
-    constexpr int N = Mat<T>::N;
-    if (!on || c0 >= width) return make_uint4(0, 0, 0, 0);
-    const T *p = reinterpret_cast<const T *>(x.data) + b * x.s0 + t * x.s1 + h * x.s2;
-    if (vec && c0 + N <= width) return *reinterpret_cast<const uint4 *>(p + c0);
-    T e[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = c0 + i < width ? p[(int64_t)(c0 + i) * x.s3] : T(0);
-    uint4 r;
-    __builtin_memcpy(&r, e, 16);
-    return r;
-}
-
-// A tile of C rows and W columns on its way from memory to LDS.
-template <typename T, int W>
+// A tile of C rows and W columns on its way from memory to LDS: 16 bytes a thread and turn, the rows
+// of a (batch, head) at base.  VEC: unit channel stride, 16-byte aligned rows, whole pieces, and
+// offsets inside a chunk below 2^31 bytes.
+template <typename T, int W, bool VEC>
 struct Staged {
-    static constexpr int N = Mat<T>::N, C = Mat<T>::C, PIECES = C * W / N / kThreads;
+    static constexpr int N = Mat<T>::N, C = Mat<T>::C, PER = W / N, ROWS = kThreads / PER,
+                         PIECES = C / ROWS;
     uint4 r[PIECES];
-    __device__ __forceinline__ void load(const View &x, int vec, const WalkArgs &p, int64_t b,
-                                         int64_t h, int64_t chunk, int c0, int width) {
+    __device__ __forceinline__ void load(const View &x, int64_t b, int64_t h, int64_t t0, int64_t T_,
+                                         int c0, int width) {
+        const int row = threadIdx.x / PER, c = threadIdx.x % PER * N;
+        const T *base = reinterpret_cast<const T *>(x.data) + b * x.s0 + h * x.s2 + t0 * x.s1;
+        const int left = (int)min(T_ - t0, (int64_t)C);
+        if constexpr (VEC) {
+            const char *p = reinterpret_cast<const char *>(base + c0);
+            const uint32_t step = (uint32_t)x.s1 * (uint32_t)sizeof(T);
+            const uint32_t off = (uint32_t)row * step + (uint32_t)c * (uint32_t)sizeof(T);
+            const bool in = c0 + c < width;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int n = threadIdx.x + i * kThreads;
-            const int64_t t = chunk * C + n / (W / N);
-            const bool on = t < p.T && (!p.valid.data || ld4<float>(p.valid, b, t, 0, 0) != 0.f);
-            r[i] = load_piece<T>(x, vec, b, t, h, c0 + n % (W / N) * N, width, on);
+            for (int i = 0; i < PIECES; ++i) {
+                r[i] = make_uint4(0, 0, 0, 0);
+                if (in && row + i * ROWS < left)
+                    r[i] = *reinterpret_cast<const uint4 *>(p + (off + (uint32_t)(i * ROWS) * step));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                T e[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    e[j] = row + i * ROWS < left && c0 + c + j < width
+                               ? base[(int64_t)(row + i * ROWS) * x.s1 + (int64_t)(c0 + c + j) * x.s3] : T(0);
+                __builtin_memcpy(&r[i], e, 16);
+            }
         }
     }
+    // Rows of padding become zero: what they hold is not used.
     template <int LD>
-    __device__ __forceinline__ void store(T *tile) const {
+    __device__ __forceinline__ void store(T *tile, const int *seg) const {
+        const int row = threadIdx.x / PER, c = threadIdx.x % PER * N;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int n = threadIdx.x + i * kThreads;
-            *reinterpret_cast<uint4 *>(tile + n / (W / N) * LD + n % (W / N) * N) = r[i];
-        }
+        for (int i = 0; i < PIECES; ++i)
+            *reinterpret_cast<uint4 *>(tile + (row + i * ROWS) * LD + c) =
+                seg[row + i * ROWS] >= 0 ? r[i] : make_uint4(0, 0, 0, 0);
     }
 };
 
 // Four consecutive columns of the output at token t.
-template <typename T>
+template <typename T, bool VEC>
 __device__ __forceinline__ void store4(T *out, int64_t row, int col, int width, const f32x4 &x) {
     T *p = out + row * width + col;
     T e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i]);
-    if (width % 4 == 0) {
+    if (VEC) {
         if (col < width) __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), e, sizeof e);
     } else {
 #pragma unroll
@@ -256,11 +259,11 @@ __device__ __forceinline__ void store4(T *out, int64_t row, int col, int width, 
 }
 
 // Gam of the pair (out token t, source token s), 0 where s is not seen from t.
-template <int C>
-__device__ __forceinline__ float pair_decay(const GateTile<C> &gt, int rev, int t, int s) {
+template <int C, bool REV>
+__device__ __forceinline__ float pair_decay(const GateTile<C> &gt, int t, int s) {
     const float d = (gt.hi[t] - gt.hi[s]) + (gt.lo[t] - gt.lo[s]);
-    const bool on = gt.seg[t] == gt.seg[s] && (rev ? s >= t : s <= t);
-    return on ? exp2f(rev ? -d : d) : 0.f;
+    const bool on = gt.seg[t] == gt.seg[s] && (REV ? s >= t : s <= t);
+    return on ? __builtin_amdgcn_exp2f(REV ? -d : d) : 0.f;
 }
 
 // Sum over the four 16-lane groups of a wave.
@@ -269,94 +272,247 @@ __device__ __forceinline__ float groups_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-template <typename T, int KP>
+template <typename T, int KP, bool OUT, bool DOT>
 struct WalkLds {
     static constexpr int C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = kCols + Mat<T>::PAD,
                          LDP = C + Mat<T>::PAD;
-    T a[C * LDA], b[C * LDA], c[C * LDC], p[C * LDP];
-    GateTile<C> gate;
+    T b[C * LDA], c[C * LDC];
+    T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
+    GateTile<C> gate[2];
     float red[4][C];
+    float rows[3][C], cols[3][C], diag[C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
-// One workgroup: a segment's chunks in the walk's order, kCols columns of the state.  Each of the four
-// waves owns 16 columns, so its part of the state stays in its accumulators, where the state is at
-// once the product's operand of the next chunk: neither it nor its update passes through LDS.
-// CARRY: only the state that the segment adds and its decay.
-template <typename T, int KP, bool CARRY>
-__global__ void __launch_bounds__(kThreads, 2) linear_walk(WalkArgs p) {
-    typedef Mat<T> M;
-    typedef WalkLds<T, KP> L;
-    constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDA = L::LDA, LDC = L::LDC,
-                  LDP = L::LDP, BT = RB / 16;  // BT: accumulator tiles of one fragment
-    __shared__ __align__(16) L lds;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
-
-    // Workgroups of one group share their inputs: they take neighbouring numbers on one XCD.
-    const unsigned total = gridDim.x, xcd = blockIdx.x % 8;
-    const unsigned whole = total / 8, rest = total % 8;
-    unsigned id = xcd * whole + min(xcd, rest) + blockIdx.x / 8;
-    int sub = id % p.per_group;
-    id /= p.per_group;
-    const int segs = p.segments - (CARRY ? 1 : 0);
-    int seg = id % segs;
-    const int64_t bh = id / segs, b = bh / p.H, h = bh % p.H;
-    int wi = 0;
-    while (sub >= p.w[wi].slices) sub -= p.w[wi].slices, ++wi;
-    const Walk &w = p.w[wi];
-    const int rev = w.rev, col0 = sub * kCols;
-    if (CARRY) seg += p.first_seg;
-
-    const int c_lo = seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
-    const int64_t BH = p.B * p.H;
-
-    f32x4 S[KT];
+// State of one wave: 16 columns, accumulator tiles of 16 rows.
+template <int KT>
+struct State {
+    f32x4 t[KT];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int m = 0; m < KT; ++m) S[m] = zero4();
-    const bool walk_first = rev ? seg == p.segments - 1 : seg == 0;
-    if (!CARRY) {
-        const float *src = walk_first ? w.first : w.init;
-        if (src) {
-            src += walk_first ? b * w.f_b + h * w.f_h : bh * w.i_bh + seg * w.i_seg;
-            const int64_t rs = walk_first ? w.f_row : w.i_row, cs = walk_first ? w.f_col : w.i_col;
-            const int v = col0 + 16 * wave + n16;
+        for (int m = 0; m < KT; ++m) t[m] = zero4();
+    }
+    // Rows and columns of src at strides below 2^22 (32-bit offsets: 64 addresses would spill).
+    __device__ __forceinline__ void load(const float *src, int rs, int cs, int v, int ka, int vc) {
+        const int g4 = 4 * (lane_id() >> 4);
+        if (v >= vc) return;
+#pragma unroll
+        for (int m = 0; m < KT; ++m) {
+            const int k = 16 * m + g4;
+            const uint32_t at = (uint32_t)(k * rs + v * cs);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + i < ka) t[m][i] = src[at + (uint32_t)(i * rs)];
+        }
+    }
+    // Dense rows of vc columns.
+    __device__ __forceinline__ void store(float *dst, int v, int ka, int vc) const {
+        const int g4 = 4 * (lane_id() >> 4);
+        if (v >= vc) return;
+#pragma unroll
+        for (int m = 0; m < KT; ++m) {
+            const int k = 16 * m + g4;
+            const uint32_t at = (uint32_t)(k * vc + v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + i < ka) dst[at + (uint32_t)(i * vc)] = t[m][i];
+        }
+    }
+};
+
+// What the chunk adds to the state, apart from the state: col_s b_s c_s^T over its tokens.  Whether
+// that is finite tells whether b and c are.
+template <typename T, int KP>
+__device__ __forceinline__ bool update(State<KP / 16> &U, const typename Mat<T>::Frag (&cf)[Mat<T>::C / Mat<T>::RB],
+                                       const T *b, const float *col) {
+    typedef Mat<T> M;
+    constexpr int KT = KP / 16, RB = M::RB, LDA = KP + M::PAD;
+    U.zero();
+#pragma unroll
+    for (int r = 0; r < M::C / RB; ++r) {
+        const float *f = col + r * RB + (RB / 4) * (lane_id() >> 4);
+        if constexpr (sizeof(T) == 2) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(cf[r][e]) * f[e];
+            const Split3 s3 = split3(x);
+#pragma unroll
+            for (int m = 0; m < KT; ++m) {
+                const typename M::Frag y = M::template across<LDA>(b, r * RB, 16 * m);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) M::mma(U.t[m], y, s3.t[q]);
+            }
+        } else {
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = cf[r][e] * f[e];
+#pragma unroll
+            for (int m = 0; m < KT; ++m) M::mma(U.t[m], M::template across<LDA>(b, r * RB, 16 * m), x);
+        }
+    }
+    float z = 0.f;
+#pragma unroll
+    for (int m = 0; m < KT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z = fmaf(U.t[m][i], 0.f, z);
+    return !__any(z != 0.f);  // z is 0 or NaN
+}
+
+// A chunk whose b or c holds a value that is not finite, token by token: a product over masked tokens
+// would spread the value to tokens that do not see it.
+template <typename T, int KP, bool REV, bool OUT>
+__device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const T *b, const T *c,
+                                                      const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
+                                                      T *out, int64_t stride, int tokens) {
+    constexpr int KT = KP / 16, C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = kCols + Mat<T>::PAD;
+    const int g4 = 4 * (lane_id() >> 4);
+#pragma unroll 1
+    for (int n = 0; n < C; ++n) {
+        const int t = REV ? C - 1 - n : n;
+        if (t >= tokens) continue;
+        const float f = gate.step[t];
+        float o = 0.f;
+        if (gate.seg[t] >= 0) {
+            const float x = Elem<T>::load(c, t * LDC + v % kCols);
 #pragma unroll
             for (int m = 0; m < KT; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int k = 16 * m + g4 + i;
-                    if (k < w.ka && v < w.vc) S[m][i] = src[k * rs + v * cs];
+                    if (k >= ka) continue;  // 0 there, whatever x is
+                    if (!REV) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
+                    S.t[m][i] += Elem<T>::load(b, t * LDA + k) * x;
+                    if (OUT) o += Elem<T>::load(a, t * LDA + k) * S.t[m][i];
+                    if (REV) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
                 }
+            o = groups_sum(o);
+        }
+        if (OUT && out && lane_id() < 16 && v < vc) Elem<T>::store(out, t * stride + v, o);
+    }
+}
+
+// One workgroup: a segment's chunks in the walk's order (REV: from the last to the first), kCols columns
+// of the state.  Each of the four waves owns 16 columns, so its part of the state stays in its
+// accumulators, where the state is at once the product's operand of the next chunk: neither it nor its
+// update passes through LDS.  The next chunk's tiles and gates are on their way while one is worked on.
+// Without `starts` a segment's start state is walked to from the sequence's start (prewalk: b and c alone).
+// OUT = false: only the state that the segment adds and its decay (carry).
+// DOT: dot_t = sum over columns of row_t (a_t S) d_t, and in the forward direction also the pair sums
+//   pairs_t = sum_{u >= t, s < t, both in the chunk} Gam_us (a_u.b_s)(d_u.c_s),
+// which with (a, b, c, d) = (do, v, k, q) is the part of the gate's gradient inside the chunk; over the
+// slices of c and d it adds up.
+template <typename T, int KP, bool VEC, bool REV, bool OUT, bool DOT>
+__global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
+    typedef Mat<T> M;
+    typedef WalkLds<T, KP, OUT, DOT> L;
+    constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDA = L::LDA, LDC = L::LDC,
+                  LDP = L::LDP, BT = RB / 16;  // BT: accumulator tiles of one fragment
+    constexpr bool PAIRS = DOT && !REV;
+    __shared__ __align__(16) L lds;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
+
+    // Workgroups that share inputs take neighbouring numbers on one XCD; the longest prewalk first.
+    const unsigned total = gridDim.x, xcd = blockIdx.x % 8, whole = total / 8, rest = total % 8;
+    unsigned id = xcd * whole + min(xcd, rest) + blockIdx.x / 8;
+    const int slice = id % p.slices;
+    id /= p.slices;
+    const int segs = p.segments - (OUT ? 0 : 1);
+    const int nth = OUT ? segs - 1 - (int)(id % segs) : (int)(id % segs);  // in the walk's order
+    const int bh = id / segs;
+    const int64_t b = bh / p.H, h = bh % p.H, BH = (int64_t)gridDim.x / segs / p.slices;
+    const int seg = REV ? p.segments - 1 - nth : nth;
+    const int col0 = slice * kCols, v = col0 + 16 * wave + n16;
+    const int c_lo = seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
+
+    State<KT> S;
+    S.zero();
+    int n = c_hi - c_lo;   // chunks to walk, the last `out` of them with results
+    const int out = OUT ? n : 0;
+    if (OUT) {
+        if (nth > 0 && p.starts) {
+            S.load(p.starts + bh * p.s_bh + seg * (int64_t)p.ka * p.vc, p.s_row, p.s_col, v, p.ka, p.vc);
+        } else {
+            if (p.first.data)
+                S.load(reinterpret_cast<const float *>(p.first.data) + b * p.first.s0 + h * p.first.s1,
+                       (int)p.first.s2, (int)p.first.s3, v, p.ka, p.vc);
+            n = REV ? p.chunks - c_lo : c_hi;
         }
     }
     float decay = 1.f;
+    int ci = REV ? c_lo + n - 1 : c_hi - n;
 
-    Staged<T, KP> sa, sb;
-    Staged<T, kCols> sc;
+    Staged<T, KP, VEC> sa, sb;
+    Staged<T, kCols, VEC> sc, sd;
     GateIn gi{};
-    const auto fetch = [&](int ci) {
-        if (!CARRY) sa.load(w.a, w.a_vec, p, b, h, ci, 0, w.ka);
-        sb.load(w.b, w.b_vec, p, b, h, ci, 0, w.ka);
-        sc.load(w.c, w.c_vec, p, b, h, ci, col0, w.vc);
-        if (wave == 0) gi = gate_load<C>(p, b, h, ci);
+    const auto fetch = [&](int chunk, bool full) {
+        const int64_t t0 = (int64_t)chunk * C;
+        sb.load(p.b, b, h, t0, p.T, 0, p.ka);
+        sc.load(p.c, b, h, t0, p.T, col0, p.vc);
+        if (OUT && full) {
+            sa.load(p.a, b, h, t0, p.T, 0, p.ka);
+            if (DOT) sd.load(p.d, b, h, t0, p.T, col0, p.vc);
+        }
+        if (wave == 0) gi = gate_load<C>(p, b, h, chunk);
     };
-    fetch(rev ? c_hi - 1 : c_lo);
+    fetch(ci, n <= out);
+    if (wave == 0) gate_store<C, REV>(gi, &lds.gate[n & 1]);
+    __syncthreads();
 
-    for (int n = c_lo; n < c_hi; ++n) {
-        const int ci = rev ? c_lo + c_hi - 1 - n : n;
-        __syncthreads();  // the last chunk's tiles are read
-        if (!CARRY) sa.template store<LDA>(lds.a);
-        sb.template store<LDA>(lds.b);
-        sc.template store<LDC>(lds.c);
-        if (wave == 0) gate_store<C>(gi, rev, &lds.gate);
-        if (n + 1 < c_hi) fetch(rev ? ci - 1 : ci + 1);
+    // The chunk's update from the tiles in LDS, and whether it is finite.
+    const auto add = [&](typename M::Frag (&cf)[C / RB], State<KT> &U, const GateTile<C> &gate) {
+#pragma unroll
+        for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
+        decay *= gate.tot;
+        return update<T, KP>(U, cf, lds.b, gate.col);
+    };
+    const auto advance = [&](const State<KT> &U, float tot) {
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S.t[m][i] = (tot == 0.f ? 0.f : S.t[m][i] * tot) + U.t[m][i];
+    };
+
+    for (; n > out; --n, ci += REV ? -1 : 1) {
+        const GateTile<C> &gate = lds.gate[n & 1];
+        sb.template store<LDA>(lds.b, gate.seg);
+        sc.template store<LDC>(lds.c, gate.seg);
+        if (n > 1) fetch(REV ? ci - 1 : ci + 1, n - 1 <= out);
+        __syncthreads();
+        typename M::Frag cf[C / RB];
+        State<KT> U;
+        if (__builtin_expect(add(cf, U, gate), 1))
+            advance(U, gate.tot);
+        else
+            walk_tokens<T, KP, REV, false>(S, lds.b, lds.b, lds.c, gate, p.ka, v, p.vc, nullptr, 0,
+                                           (int)min(p.T - (int64_t)ci * C, (int64_t)C));
+        if (n > 1 && wave == 0) gate_store<C, REV>(gi, &lds.gate[(n - 1) & 1]);
+        __syncthreads();  // the chunk's tiles are read, the next one's gates written
+    }
+    if (!OUT) {
+        S.store(p.seg_state + ((int64_t)bh * p.segments + seg) * p.ka * p.vc, v, p.ka, p.vc);
+        if (threadIdx.x == 0 && slice == 0) p.seg_decay[(int64_t)bh * p.segments + seg] = decay;
+        return;
+    }
+    if (p.starts_out && nth > 0)
+        S.store(p.starts_out + bh * p.s_bh + seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
+
+    for (; n > 0; --n, ci += REV ? -1 : 1) {
+        const GateTile<C> &gate = lds.gate[n & 1];
+        sa.template store<LDA>(lds.a, gate.seg);
+        sb.template store<LDA>(lds.b, gate.seg);
+        sc.template store<LDC>(lds.c, gate.seg);
+        if (DOT) sd.template store<LDC>(lds.d, gate.seg);
+        if (n > 1) fetch(REV ? ci - 1 : ci + 1, true);
         __syncthreads();
 
         f32x4 acc[TT];
-        if (!CARRY) {
-            // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows.
-            for (int n2 = wave; n2 < TT * TT; n2 += 4) {
-                const int tj = n2 / TT, si = n2 % TT;
-                if (rev ? si / BT < tj / BT : si / BT > tj / BT) continue;
+        {
+            // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: three a
+            // wave in bf16, one in float32.
+#pragma unroll
+            for (int m = 0; m < (TT == 4 ? 3 : 1); ++m) {
+                int tj = m == 0 ? wave >> 1 : m + 1, si = m == 0 ? wave & 1 : wave;
+                if (TT == 2 && si > tj) continue;  // a block of 16 sources that no row sees
+                if (REV) tj = TT - 1 - tj, si = TT - 1 - si;
                 f32x4 x = zero4();
 #pragma unroll
                 for (int r = 0; r < KP; r += RB)
@@ -365,10 +521,40 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(WalkArgs p) {
                 T e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float f = pair_decay<C>(lds.gate, rev, t, s + i);
-                    Elem<T>::store(e, i, f == 0.f ? 0.f : x[i] * f);
+                    const float f = pair_decay<C, REV>(gate, t, s + i);
+                    x[i] = f == 0.f ? 0.f : x[i] * f;
+                    Elem<T>::store(e, i, x[i]);
                 }
                 __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
+                if (PAIRS && si <= tj) {
+                    f32x4 y = zero4();
+#pragma unroll
+                    for (int r = 0; r < kCols; r += RB)
+                        M::mma(y, M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        y[i] = x[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
+                    if (si < tj) {
+                        const float sum = groups_sum((y[0] + y[1]) + (y[2] + y[3]));
+                        if (lane < 16) lds.rows[si][t] = sum;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float c = row16_sum(y[i]);
+                            if (n16 == i) lds.cols[tj - 1][s + i] = c;
+                        }
+                    } else {
+                        // sums over s before each of the lane's four tokens, over the groups in order
+                        const float q = (y[0] + y[1]) + (y[2] + y[3]);
+                        const float q1 = __shfl_up(q, 16), q2 = __shfl_up(q, 32), q3 = __shfl_up(q, 48);
+                        float pre = (g4 > 0 ? q1 : 0.f) + (g4 > 4 ? q2 : 0.f) + (g4 > 8 ? q3 : 0.f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float c = row16_sum(n16 >= g4 + i ? pre : 0.f);
+                            if (n16 == i) lds.diag[s + i] = c;
+                            pre += y[i];
+                        }
+                    }
+                }
             }
             // acc[j]: rows = the wave's columns, column = token 16 j + n16; the state's part.
 #pragma unroll
@@ -376,185 +562,130 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(WalkArgs p) {
 #pragma unroll
             for (int r = 0; r < KP / RB; ++r) {
                 if constexpr (sizeof(T) == 2) {
-                    const f32x4 u = S[2 * r], v = S[2 * r + 1];
-                    const Split3 s3 = split3({u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+                    const f32x4 u = S.t[2 * r], w = S.t[2 * r + 1];
+                    const Split3 s3 = split3({u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]});
 #pragma unroll
                     for (int j = 0; j < TT; ++j) {
                         const typename M::Frag x = M::order(lds.a + 16 * j * LDA, LDA, r * RB);
-                        M::mma(acc[j], s3.t[0], x);
-                        if (w.dot_x) {
-                            M::mma(acc[j], s3.t[1], x);
-                            M::mma(acc[j], s3.t[2], x);
-                        }
+#pragma unroll
+                        for (int q = 0; q < (DOT ? 3 : 1); ++q) M::mma(acc[j], s3.t[q], x);
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < TT; ++j)
-                        M::mma(acc[j], S[r], M::order(lds.a + 16 * j * LDA, LDA, r * RB));
+                        M::mma(acc[j], S.t[r], M::order(lds.a + 16 * j * LDA, LDA, r * RB));
                 }
             }
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
-                const float f = lds.gate.row[16 * j + n16];
+                const float f = gate.row[16 * j + n16];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[j][i] = f == 0.f ? 0.f : acc[j][i] * f;
-                if (w.dot_x) {
-                    const int64_t t = (int64_t)ci * C + 16 * j + n16;
-                    float d = 0.f;
+                if (DOT) {
+                    const T *d = lds.d + (16 * j + n16) * LDC + 16 * wave + g4;
+                    float x = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int v = col0 + 16 * wave + g4 + i;
-                        if (f != 0.f && v < w.vc)
-                            d += acc[j][i] * Elem<T>::load(w.dot_x, b * w.dx0 + t * w.dx1 + h * w.dx2 + v * w.dx3);
-                    }
-                    d = groups_sum(d);
-                    if (lane < 16) lds.red[wave][16 * j + n16] = d;
+                    for (int i = 0; i < 4; ++i) x += acc[j][i] * Elem<T>::load(d, i);
+                    x = groups_sum(f == 0.f ? 0.f : x);
+                    if (lane < 16) lds.red[wave][16 * j + n16] = x;
                 }
             }
             __syncthreads();
-            if (w.dot_x && wave == 0) {
-                const int64_t t = (int64_t)ci * C + lane;
+            if (DOT && wave == 1) {
+                const int64_t t = (int64_t)ci * C + lane, at = (int64_t)slice * BH + bh;
                 float d = 0.f;
                 if (lane < C) d = (lds.red[0][lane] + lds.red[1][lane]) + (lds.red[2][lane] + lds.red[3][lane]);
-                if (lane < C && t < p.T) w.dots[(sub * BH + bh) * p.T + t] = d;
+                if (lane < C && t < p.T) p.dots[at * p.T + t] = d;
                 const float sum = wave_sum(d);
-                if (lane == 0) w.dot_sums[(sub * BH + bh) * p.chunks + ci] = sum;
+                if (lane == 0) p.dot_sums[at * p.chunks + ci] = sum;
             }
-        }
-        if (p.totals && wi == 0 && sub == 0 && threadIdx.x == 0) p.totals[bh * p.chunks + ci] = lds.gate.tot;
-
-        // The update, apart from the state: it tells whether b or c held a value that is not finite.
-        typename M::Frag cf[C / RB];
-#pragma unroll
-        for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
-        f32x4 U[KT];
-#pragma unroll
-        for (int m = 0; m < KT; ++m) U[m] = zero4();
-#pragma unroll
-        for (int r = 0; r < C / RB; ++r) {
-            const float *f = lds.gate.col + r * RB + (RB / 4) * (lane >> 4);
-            if constexpr (sizeof(T) == 2) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(cf[r][e]) * f[e];
-                const Split3 s3 = split3(x);
-#pragma unroll
-                for (int m = 0; m < KT; ++m) {
-                    const typename M::Frag y = M::template across<LDA>(lds.b, r * RB, 16 * m);
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) M::mma(U[m], y, s3.t[q]);
+            if (PAIRS && wave == 2) {
+                // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t
+                // of the tile over the tiles below, whole tiles below and to the left, and its own tile.
+                const int64_t t = (int64_t)ci * C + lane;
+                const int j = lane / 16;
+                float left = 0.f, below = 0.f, x = 0.f;
+                float r0 = 0.f, r1 = 0.f;
+                if (lane < C) {
+                    if (j > 0) left = r0 = lds.rows[0][lane];
+                    if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
+                    if (TT == 4 && j > 2) left += lds.rows[2][lane];
+                    if (TT > 1 && j < 1) below += lds.cols[0][lane];
+                    if (TT == 4 && j < 2) below += lds.cols[1][lane];
+                    if (TT == 4 && j < 3) below += lds.cols[2][lane];
+                    x = lds.diag[lane];
                 }
-            } else {
-                f32x4 x;
+                if (TT == 4) {
+                    const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
+                    const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
+                    x += j == 1 ? f1 : j == 2 ? f2 : 0.f;
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = cf[r][e] * f[e];
+                for (int d = 1; d < 16; d *= 2) {
+                    const float y = __shfl_down(left, d);
+                    if (n16 + d < 16) left += y;
+                }
+                float pre = __shfl_up(below, 1);
+                if (n16 == 0) pre = 0.f;
 #pragma unroll
-                for (int m = 0; m < KT; ++m)
-                    M::mma(U[m], M::template across<LDA>(lds.b, r * RB, 16 * m), x);
+                for (int d = 1; d < 16; d *= 2) {
+                    const float y = __shfl_up(pre, d);
+                    if (n16 >= d) pre += y;
+                }
+                if (lane < C && t < p.T) p.pairs[((int64_t)slice * BH + bh) * p.T + t] = (left + pre) + x;
             }
+            if (p.totals && slice == 0 && threadIdx.x == 0) p.totals[(int64_t)bh * p.chunks + ci] = gate.tot;
         }
-        float z = 0.f;
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z = fmaf(U[m][i], 0.f, z);
-        const float tot = lds.gate.tot;
-        decay *= tot;
 
-        if (!__any(z != 0.f)) {  // z is 0 or NaN
-            if (!CARRY) {
+        typename M::Frag cf[C / RB];
+        State<KT> U;
+        const bool fine = add(cf, U, gate);
+        T *o = reinterpret_cast<T *>(p.out);
+        const int64_t row0 = (b * p.T + (int64_t)ci * C) * p.H + h;
+        if (__builtin_expect(fine, 1)) {
+            if (o) {
+                const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
 #pragma unroll
                 for (int j = 0; j < TT; ++j) {
 #pragma unroll
-                    for (int r = 0; r < C / RB; ++r) {
-                        if (rev ? r < j / BT : r > j / BT) continue;
-                        M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
-                    }
-                    const int64_t t = (int64_t)ci * C + 16 * j + n16;
-                    if (w.out && t < p.T)
-                        store4<T>(reinterpret_cast<T *>(w.out), (b * p.T + t) * p.H + h,
-                                  col0 + 16 * wave + g4, w.vc, acc[j]);
+                    for (int r = 0; r < C / RB; ++r)
+                        if (REV ? r >= j / BT : r <= j / BT)
+                            M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
+                    const int t = 16 * j + n16;
+                    if (t < left)
+                        store4<T, VEC>(o, row0 + (int64_t)t * p.H, col0 + 16 * wave + g4, p.vc, acc[j]);
                 }
             }
-#pragma unroll
-            for (int m = 0; m < KT; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[m][i] = (tot == 0.f ? 0.f : S[m][i] * tot) + U[m][i];
+            advance(U, gate.tot);
         } else {
-            // A product over masked tokens would spread the value to tokens that do not see it: the
-            // wave takes this chunk token by token.
-            for (int n2 = 0; n2 < C; ++n2) {
-                const int tl = rev ? C - 1 - n2 : n2;
-                const int64_t t = (int64_t)ci * C + tl;
-                if (t >= p.T) continue;
-                const bool val = lds.gate.seg[tl] >= 0;
-                const float f = lds.gate.step[tl];
-                float o = 0.f;
-                if (val) {
-                    const float x = Elem<T>::load(lds.c, tl * LDC + 16 * wave + n16);
-#pragma unroll
-                    for (int m = 0; m < KT; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int k = 16 * m + g4 + i;
-                            if (k >= w.ka) continue;  // 0 there, whatever x is
-                            if (!rev) S[m][i] = f == 0.f ? 0.f : S[m][i] * f;
-                            S[m][i] += Elem<T>::load(lds.b, tl * LDA + k) * x;
-                            if (!CARRY) o += Elem<T>::load(lds.a, tl * LDA + k) * S[m][i];
-                            if (rev) S[m][i] = f == 0.f ? 0.f : S[m][i] * f;
-                        }
-                    o = groups_sum(o);
-                }
-                const int v = col0 + 16 * wave + n16;
-                if (!CARRY && w.out && lane < 16 && v < w.vc)
-                    Elem<T>::store(w.out, ((b * p.T + t) * p.H + h) * w.vc + v, o);
-            }
+            T *at = o ? o + row0 * p.vc : nullptr;
+            walk_tokens<T, KP, REV, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc, at, (int64_t)p.H * p.vc,
+                                         (int)min(p.T - (int64_t)ci * C, (int64_t)C));
         }
+        if (n > 1 && wave == 0) gate_store<C, REV>(gi, &lds.gate[(n - 1) & 1]);
+        __syncthreads();  // the chunk's tiles are read, the next one's gates written
     }
 
-    const int v = col0 + 16 * wave + n16;
-    if (CARRY) {
-        float *dst = w.seg_state + (bh * p.segments + seg) * w.ka * w.vc;
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = 16 * m + g4 + i;
-                if (k < w.ka && v < w.vc) dst[(int64_t)k * w.vc + v] = S[m][i];
-            }
-        if (threadIdx.x == 0 && sub == 0) w.seg_decay[bh * p.segments + seg] = decay;
-        return;
-    }
-    if (w.fin && (rev ? seg == 0 : seg == p.segments - 1)) {
-        float *dst = w.fin + bh * w.n_bh;
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = 16 * m + g4 + i;
-                if (k < w.ka && v < w.vc) dst[k * w.n_row + v * w.n_col] = S[m][i];
-            }
-    }
-    if (w.edges) {
-        const float *e = seg == 0 ? w.edge_first : w.edge;
+    if (p.fin && nth == p.segments - 1) S.store(p.fin + (int64_t)bh * p.ka * p.vc, v, p.ka, p.vc);
+    if (DOT && REV) {
+        // seg > 0 has the other direction's start state at hand, the first segment its initial state.
+        State<KT> e;
+        e.zero();
+        if (seg > 0)
+            e.load(p.edge + ((int64_t)bh * p.segments + seg) * p.ka * p.vc, p.vc, 1, v, p.ka, p.vc);
+        else if (p.edge_first.data)
+            e.load(reinterpret_cast<const float *>(p.edge_first.data) + b * p.edge_first.s0 + h * p.edge_first.s1,
+                   (int)p.edge_first.s2, (int)p.edge_first.s3, v, p.ka, p.vc);
         float d = 0.f;
-        if (e) {
-            e += seg == 0 ? b * w.ef_b + h * w.ef_h : bh * w.e_bh + seg * w.e_seg;
-            const int64_t rs = seg == 0 ? w.ef_row : w.e_row, cs = seg == 0 ? w.ef_col : w.e_col;
 #pragma unroll
-            for (int m = 0; m < KT; ++m)
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = 16 * m + g4 + i;
-                    if (k < w.ka && v < w.vc) d += S[m][i] * e[k * rs + v * cs];
-                }
-        }
-        d = wave_sum(d);
-        __syncthreads();  // wave 0 has read the last chunk's sums
+            for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
+        d = wave_sum(v < p.vc ? d : 0.f);
         if (lane == 0) lds.red[wave][0] = d;
         __syncthreads();
         if (threadIdx.x == 0)
-            w.edges[(sub * BH + bh) * p.segments + seg] =
+            p.edges[((int64_t)slice * BH + bh) * p.segments + seg] =
                 (lds.red[0][0] + lds.red[1][0]) + (lds.red[2][0] + lds.red[3][0]);
     }
 }
@@ -590,100 +721,39 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
 // ---- the gate's gradient -------------------------------------------------------------------------
 
 struct GateGradArgs {
-    WalkArgs w;           // g, masks, sizes
-    View q, k, v, d_o;
-    int q_vec, k_vec, v_vec, o_vec;
-    int K, V;
-    const float *x, *y;           // dots of the dq and dv walks
+    Walk w;                       // g, masks, sizes
+    const float *x, *y, *pairs;   // dots of the dq and dv walks, pair sums of the dq walk
     const float *x_sums, *y_sums; // per chunk
-    const float *edges;
-    const float *totals;
+    const float *edges, *totals;
+    int64_t BH;
     int x_slices, y_slices;
     float *dg;                    // dense [B, T, H]
 };
 
-// One workgroup a chunk: W by matrix products in 64-wide slabs of the channels, prefix sums along
-// its rows, and the parts of pairs that reach out of the chunk:
-//   dg_t = sum_{u>=t, s<t inside} W_us + sum_{u>=t} x_u + sum_{s<t} y_s + E,
-// E the pairs around the whole chunk: edge products at the segment's start, then chunk by chunk.
-template <typename T>
+// One wave a chunk: the pair sums inside it, and the pairs that reach out of it:
+//   dg_t = pairs_t + sum_{u>=t} x_u + sum_{s<t} y_s + E,
+// E the pairs around the whole chunk: the edge product at the segment's start, then chunk by chunk,
+// from the last chunk with a cut in it if there is one.
+template <int C>
 __global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
-    typedef Mat<T> M;
-    constexpr int C = M::C, TT = C / 16, RB = M::RB, LD = kCols + M::PAD, LDW = C + 1;
-    constexpr int MINE = (TT * (TT + 1) / 2 + 3) / 4;
-    __shared__ __align__(16) T xs[C * LD], ys[C * LD];
-    __shared__ float W[C * LDW], red[4][64];
-    __shared__ GateTile<C> gate;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
-    const int ci = blockIdx.x % p.w.chunks;
-    const int64_t bh = blockIdx.x / p.w.chunks, b = bh / p.w.H, h = bh % p.w.H;
-    const int64_t BH = p.w.B * p.w.H;
-    GateIn gi{};
-    if (wave == 0) {
-        gi = gate_load<C>(p.w, b, h, ci);
-        gate_store<C>(gi, 0, &gate);
-    }
-    for (int i = threadIdx.x; i < C * LDW; i += kThreads) W[i] = 0.f;
-    f32x4 qk[MINE], ov[MINE];
-#pragma unroll
-    for (int m = 0; m < MINE; ++m) qk[m] = zero4(), ov[m] = zero4();
-    const int kslabs = (p.K + kCols - 1) / kCols, slabs = kslabs + (p.V + kCols - 1) / kCols;
-    for (int s = 0; s < slabs; ++s) {
-        Staged<T, kCols> a, c;
-        const bool first = s < kslabs;
-        const int c0 = (first ? s : s - kslabs) * kCols;
-        a.load(first ? p.q : p.d_o, first ? p.q_vec : p.o_vec, p.w, b, h, ci, c0, first ? p.K : p.V);
-        c.load(first ? p.k : p.v, first ? p.k_vec : p.v_vec, p.w, b, h, ci, c0, first ? p.K : p.V);
-        __syncthreads();
-        a.template store<LD>(xs);
-        c.template store<LD>(ys);
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < MINE; ++m) {
-            int n = wave + 4 * m, tj = 0;
-            if (n >= TT * (TT + 1) / 2) continue;
-            while (n > tj) n -= ++tj;  // the lower tiles (tj, si <= tj), row by row
-            f32x4 acc = first ? qk[m] : ov[m];
-#pragma unroll
-            for (int r = 0; r < kCols; r += RB)
-                M::mma(acc, M::row(ys + 16 * n * LD, LD, r), M::row(xs + 16 * tj * LD, LD, r));
-            if (first) qk[m] = acc;
-            else ov[m] = acc;
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MINE; ++m) {
-        int n = wave + 4 * m, tj = 0;
-        if (n >= TT * (TT + 1) / 2) continue;
-        while (n > tj) n -= ++tj;
-        const int t = 16 * tj + n16, s = 16 * n + g4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float f = s + i < t ? pair_decay<C>(gate, 0, t, s + i) : 0.f;
-            W[t * LDW + s + i] = f == 0.f ? 0.f : f * qk[m][i] * ov[m][i];
-        }
-    }
-    __syncthreads();
-    // lane t of a wave: sum over its rows u >= t of the row's sum before t.
-    float r = 0.f;
-    for (int u = wave; u < C; u += 4) {
-        const float x = lane < C ? W[u * LDW + lane] : 0.f;
-        const float y = __shfl_up(x, 1);
-        const float pre = wave_scan_add(lane == 0 ? 0.f : y);
-        if (u >= lane) r += pre;
-    }
-    red[wave][lane] = r;
-    __syncthreads();
-    if (wave != 0) return;
+    const int lane = lane_id(), wave = threadIdx.x >> 6;
+    const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + wave;
+    if (id >= p.BH * p.w.chunks) return;
+    const int ci = id % p.w.chunks;
+    const int64_t bh = id / p.w.chunks, b = bh / p.w.H, h = bh % p.w.H;
     const int64_t t = (int64_t)ci * C + lane;
     const bool in = lane < C && t < p.w.T;
-    float x = 0.f, y = 0.f;
+    const GateIn gi = gate_load<C>(p.w, b, h, ci);
+    const bool val = in && gi.valid != 0.f && gi.reset == 0.f && !(gi.g < kCut);
+    float dg = 0.f, x = 0.f, y = 0.f;
     if (in) {
-        for (int s = 0; s < p.x_slices; ++s) x += p.x[(s * BH + bh) * p.w.T + t];
-        for (int s = 0; s < p.y_slices; ++s) y += p.y[(s * BH + bh) * p.w.T + t];
+        for (int s = 0; s < p.x_slices; ++s) {
+            x += p.x[(s * p.BH + bh) * p.w.T + t];
+            dg += p.pairs[(s * p.BH + bh) * p.w.T + t];
+        }
+        for (int s = 0; s < p.y_slices; ++s) y += p.y[(s * p.BH + bh) * p.w.T + t];
     }
-    float dg = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    // sum of x over u >= t, and of y over s < t; scans that add only what belongs to them
+    // sum of x over u >= t, and of y over s < t: scans that add only what belongs to them
     float sx = x, sy = __shfl_up(y, 1);
     if (lane == 0) sy = 0.f;
 #pragma unroll
@@ -692,9 +762,8 @@ __global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
         if (lane + d < 64) sx += a;
         if (lane >= d) sy += c;
     }
-    // E: from the segment's start, or from the last chunk before this one with a cut in it.
     float E = 0.f;
-    if (gate.tot != 0.f) {
+    if (p.totals[bh * p.w.chunks + ci] != 0.f) {
         const int seg = ci / p.w.seg_chunks, c_lo = seg * p.w.seg_chunks;
         int from = c_lo;  // first chunk whose sums count in full
         bool cut = false;
@@ -705,18 +774,17 @@ __global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
         }
         for (int c = from + lane; c < ci; c += 64) {
             float d = 0.f;
-            for (int s = 0; s < p.y_slices; ++s) d += p.y_sums[(s * BH + bh) * p.w.chunks + c];
+            for (int s = 0; s < p.y_slices; ++s) d += p.y_sums[(s * p.BH + bh) * p.w.chunks + c];
             if (!(cut && c == from))
-                for (int s = 0; s < p.x_slices; ++s) d -= p.x_sums[(s * BH + bh) * p.w.chunks + c];
+                for (int s = 0; s < p.x_slices; ++s) d -= p.x_sums[(s * p.BH + bh) * p.w.chunks + c];
             E += d;
         }
         if (lane == 0 && !cut)
-            for (int s = 0; s < p.y_slices; ++s) E += p.edges[(s * BH + bh) * p.w.segments + seg];
+            for (int s = 0; s < p.y_slices; ++s) E += p.edges[(s * p.BH + bh) * p.w.segments + seg];
         E = wave_sum(E);
         E -= wave_sum(x);
     }
     if (!in) return;
-    const bool val = gate.seg[lane] >= 0 && gate.step[lane] != 0.f;
     dg += sx + sy + E;
     p.dg[(b * p.w.T + t) * p.w.H + h] = val ? dg : 0.f;
 }
@@ -826,6 +894,7 @@ struct Plan {
     int C, chunks, seg_chunks, segments;
     int64_t BH, KV;
     int kslices, vslices;
+    bool prewalk;  // start states are walked to, instead of carried by a launch of their own
 };
 
 constexpr int64_t kWantGroups = 512;  // workgroups that fill the card
@@ -845,11 +914,12 @@ Plan plan(const gdn2_shape *s, int dtype) {
     want = std::max<int64_t>(1, std::min<int64_t>(want, p.chunks / 2));
     p.seg_chunks = (int)((p.chunks + want - 1) / want);
     p.segments = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
+    p.prewalk = p.chunks <= 8;
     return p;
 }
 
 struct Layout {
-    size_t state, decay, x, y, x_sums, y_sums, edges, totals, dinit, bytes;
+    size_t state, decay, x, y, pairs, x_sums, y_sums, edges, totals, dg, bytes;
 };
 
 // Checkpoint: the start states of the segments, and their decays.
@@ -868,15 +938,16 @@ Layout workspace_layout(const Plan &p, int64_t T) {
         n += round16(4 * floats);
         return at;
     };
-    l.state = take(p.segments > 1 ? p.BH * p.segments * p.KV : 0);
+    l.state = take(p.segments > 1 && !p.prewalk ? p.BH * p.segments * p.KV : 0);
     l.decay = take(p.BH * p.segments);
     l.x = take(p.kslices * p.BH * T);
     l.y = take(p.vslices * p.BH * T);
+    l.pairs = take(p.kslices * p.BH * T);
     l.x_sums = take((int64_t)p.kslices * p.BH * p.chunks);
     l.y_sums = take((int64_t)p.vslices * p.BH * p.chunks);
     l.edges = take((int64_t)p.vslices * p.BH * p.segments);
     l.totals = take(p.BH * p.chunks);
-    l.dinit = take(p.BH * T);
+    l.dg = take(p.BH * T);
     l.bytes = n;
     return l;
 }
@@ -889,7 +960,7 @@ int check_linear(const gdn2_shape *s, int dtype) {
         return fail(GDN2_ERR_SHAPE, "key and value widths must be 1..128");
     if (dtype != GDN2_F32 && dtype != GDN2_BF16)
         return fail(GDN2_ERR_DTYPE, "dtype must be F32 or BF16");
-    // A launch has at most 2^24 workgroups of 256 threads: 6 for a chunk of 32 or 64 tokens.
+    // A launch has at most 2^24 workgroups of 256 threads: two for a segment of 32 or 64 tokens.
     const int64_t lim = (int64_t)1 << 21;
     if (s->batch > lim || s->heads > lim || s->batch * s->heads > lim || s->time > 32 * lim ||
         (s->time + 31) / 32 > lim / (s->batch * s->heads))
@@ -897,13 +968,13 @@ int check_linear(const gdn2_shape *s, int dtype) {
     return GDN2_OK;
 }
 
-// 16-byte pieces of every row: unit channel stride, aligned rows.
-int vec_rows(const gdn2_view *v) {
+// Whether rows are read in 16-byte pieces: unit channel stride, aligned rows, whole pieces.
+bool vec_rows(const gdn2_view *v, int64_t width) {
     const int64_t es = v->dtype == GDN2_BF16 ? 2 : 4;
-    if (v->stride[3] != 1 || ((uintptr_t)v->data & 15)) return 0;
+    if (v->stride[3] != 1 || ((uintptr_t)v->data & 15) || width * es % 16) return false;
     for (int d = 0; d < 3; ++d)
-        if (v->stride[d] * es % 16) return 0;
-    return 1;
+        if (v->stride[d] * es % 16) return false;
+    return v->stride[1] * es * 64 < ((int64_t)1 << 31);
 }
 
 int check_inputs(const gdn2_shape *s, const gdn2_view *q, const gdn2_view *k, const gdn2_view *v,
@@ -918,75 +989,69 @@ int check_inputs(const gdn2_shape *s, const gdn2_view *q, const gdn2_view *k, co
     return GDN2_OK;
 }
 
-WalkArgs walk_args(const gdn2_shape *s, const Plan &p, const gdn2_view *g, const gdn2_view *valid,
-                   const gdn2_view *reset) {
-    WalkArgs a{};
-    a.B = s->batch;
-    a.T = s->time;
-    a.H = s->heads;
-    a.g = make_view(g);
-    a.valid = make_view(valid);
-    a.reset = make_view(reset);
-    a.chunks = p.chunks;
-    a.seg_chunks = p.seg_chunks;
-    a.segments = p.segments;
-    return a;
-}
-
-Walk make_walk(const gdn2_view *a, const gdn2_view *b, const gdn2_view *c, int64_t ka, int64_t vc, int rev) {
+Walk base_walk(const gdn2_shape *s, const Plan &p, const gdn2_view *g, const gdn2_view *valid,
+               const gdn2_view *reset) {
     Walk w{};
-    if (a) w.a = make_view(a), w.a_vec = vec_rows(a);
-    w.b = make_view(b), w.b_vec = vec_rows(b);
-    w.c = make_view(c), w.c_vec = vec_rows(c);
-    w.ka = (int)ka;
-    w.vc = (int)vc;
-    w.rev = rev;
-    w.slices = (int)((vc + kCols - 1) / kCols);
+    w.T = s->time;
+    w.H = (int)s->heads;
+    w.g = make_view(g);
+    w.valid = make_view(valid);
+    w.reset = make_view(reset);
+    w.chunks = p.chunks;
+    w.seg_chunks = p.seg_chunks;
+    w.segments = p.segments;
     return w;
 }
 
-// The start state x [B, H, K, V] of a walk over that state, or over its transpose.
-void set_first(Walk *w, const View &x, bool transposed) {
-    w->first = (const float *)x.data, w->f_b = x.s0, w->f_h = x.s1;
-    w->f_row = transposed ? x.s3 : x.s2, w->f_col = transposed ? x.s2 : x.s3;
+View transposed(const View &x) { return View{x.data, x.s0, x.s1, x.s3, x.s2}; }
+
+void set_triple(Walk *w, const gdn2_view *a, const gdn2_view *b, const gdn2_view *c, int64_t ka, int64_t vc) {
+    w->a = make_view(a), w->b = make_view(b), w->c = make_view(c);
+    w->ka = (int)ka;
+    w->vc = (int)vc;
+    w->slices = (int)((vc + kCols - 1) / kCols);
 }
 
-template <typename T, bool CARRY>
-void launch_walk(const WalkArgs &a, const Plan &p, int64_t ka, hipStream_t st) {
-    const int64_t segs = p.segments - (CARRY ? 1 : 0);
-    const dim3 grid((unsigned)(p.BH * segs * a.per_group)), block(kThreads);
-    if (ka <= 64) hipLaunchKernelGGL((linear_walk<T, 64, CARRY>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((linear_walk<T, 128, CARRY>), grid, block, 0, st, a);
+template <typename T, bool VEC, bool REV, bool OUT, bool DOT>
+void launch_walk(const Walk &w, const dim3 &grid, hipStream_t st) {
+    const dim3 block(kThreads);
+    if (w.ka <= 64) hipLaunchKernelGGL((linear_walk<T, 64, VEC, REV, OUT, DOT>), grid, block, 0, st, w);
+    else hipLaunchKernelGGL((linear_walk<T, 128, VEC, REV, OUT, DOT>), grid, block, 0, st, w);
 }
 
-template <bool CARRY>
-hipError_t run_walk(WalkArgs a, const Plan &p, int dtype, hipStream_t st) {
-    a.per_group = 0;
-    int64_t ka = 0;
-    for (int i = 0; i < a.walks; ++i) a.per_group += a.w[i].slices, ka = std::max<int64_t>(ka, a.w[i].ka);
-    if (dtype == GDN2_BF16) launch_walk<bf16_t, CARRY>(a, p, ka, st);
-    else launch_walk<float, CARRY>(a, p, ka, st);
+template <bool REV, bool OUT, bool DOT>
+hipError_t run_walk(const Walk &w, const Plan &p, int dtype, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)(p.BH * (p.segments - (OUT ? 0 : 1)) * w.slices));
+    const bool bf = dtype == GDN2_BF16;
+    if (bf && vec) launch_walk<bf16_t, true, REV, OUT, DOT>(w, grid, st);
+    else if (bf) launch_walk<bf16_t, false, REV, OUT, DOT>(w, grid, st);
+    else if (vec) launch_walk<float, true, REV, OUT, DOT>(w, grid, st);
+    else launch_walk<float, false, REV, OUT, DOT>(w, grid, st);
     return hipGetLastError();
 }
 
-// Start states of every segment of a walk over (b, c), from `first` ([B, H, K, V], data may be null).
-hipError_t run_carry(const WalkArgs &base, const Plan &p, const gdn2_view *b, const gdn2_view *c,
-                     int64_t K, int64_t V, int rev, const View &first, float *state,
-                     float *decay, int dtype, hipStream_t st) {
-    WalkArgs a = base;
-    a.w[0] = make_walk(nullptr, b, c, K, V, rev);
-    a.w[0].seg_state = state;
-    a.w[0].seg_decay = decay;
-    a.walks = 1;
-    a.first_seg = rev ? 1 : 0;
-    a.totals = nullptr;
-    hipError_t e = run_walk<true>(a, p, dtype, st);
+// Start states of every segment of a walk over (b, c) into `state`, from `first`.
+template <bool REV>
+hipError_t run_carry(Walk w, const Plan &p, const gdn2_view *b, const gdn2_view *c, int64_t K, int64_t V,
+                     const View &first, float *state, float *decay, int dtype, bool vec, hipStream_t st) {
+    set_triple(&w, nullptr, b, c, K, V);
+    w.seg_state = state;
+    w.seg_decay = decay;
+    hipError_t e = run_walk<REV, false, false>(w, p, dtype, vec, st);
     if (e != hipSuccess) return e;
-    const JoinArgs j{state,    decay,    (const float *)first.data, first.s0, first.s1, first.s2,
-                     first.s3, base.H, K * V, V, p.segments, rev};
+    const JoinArgs j{state, decay, (const float *)first.data, first.s0, first.s1, first.s2, first.s3,
+                     w.H, K * V, V, p.segments, REV};
     hipLaunchKernelGGL(linear_join, dim3((unsigned)((K * V + kThreads - 1) / kThreads), (unsigned)p.BH),
                        dim3(kThreads), 0, st, j);
     return hipGetLastError();
+}
+
+// Rows and columns of a state view at strides that 32-bit offsets reach.
+int check_state(const gdn2_view *v, const char *name) {
+    GDN2_TRY(check_view(v, name, GDN2_F32, true));
+    if (v->data && (v->stride[2] >= (1 << 22) || v->stride[3] >= (1 << 22)))
+        return fail(GDN2_ERR_SHAPE, "%s: the key and value strides must be below 2^22", name);
+    return GDN2_OK;
 }
 
 int check_buffer(const void *buf, size_t bytes, size_t need, const char *name) {
@@ -1013,7 +1078,7 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
                      const gdn2_view *reset, const gdn2_view *initial, void *output,
                      float *final_state, void *checkpoint, size_t checkpoint_bytes, void *stream) {
     GDN2_TRY(check_inputs(shape, q, k, v, g, valid, reset));
-    if (initial) GDN2_TRY(check_view(initial, "initial", GDN2_F32, true));
+    if (initial) GDN2_TRY(check_state(initial, "initial"));
     if (!output || !final_state)
         return fail(GDN2_ERR_ARGUMENT, "output and final_state must be non-null");
     const Plan p = plan(shape, q->dtype);
@@ -1021,22 +1086,23 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, l.bytes, "checkpoint"));
     if (initial && !initial->data) initial = nullptr;
     const int64_t K = shape->keys, V = shape->values;
+    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V);
     hipStream_t st = (hipStream_t)stream;
-    WalkArgs a = walk_args(shape, p, g, valid, reset);
+    Walk w = base_walk(shape, p, g, valid, reset);
     const View first = make_view(initial);
     float *state = (float *)checkpoint, *decay = (float *)((char *)checkpoint + l.decay);
-    if (p.segments > 1) {
-        const hipError_t e = run_carry(a, p, k, v, K, V, 0, first, state, decay, q->dtype, st);
+    if (p.segments > 1 && !p.prewalk) {
+        const hipError_t e = run_carry<false>(w, p, k, v, K, V, first, state, decay, q->dtype, vec, st);
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_scan");
+        w.starts = state;
     }
-    Walk &w = a.w[0];
-    w = make_walk(q, k, v, K, V, 0);
-    a.walks = 1;
-    set_first(&w, first, false);
-    w.init = state, w.i_bh = p.segments * p.KV, w.i_seg = p.KV, w.i_row = V, w.i_col = 1;
-    w.fin = final_state, w.n_bh = p.KV, w.n_row = V, w.n_col = 1;
+    if (p.segments > 1 && p.prewalk) w.starts_out = state;
+    set_triple(&w, q, k, v, K, V);
+    w.first = first;
+    w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
+    w.fin = final_state;
     w.out = output;
-    return launch_status(run_walk<false>(a, p, q->dtype, st), "gdn2_linear_scan");
+    return launch_status(run_walk<false, true, false>(w, p, q->dtype, vec, st), "gdn2_linear_scan");
 }
 
 size_t gdn2_linear_workspace_bytes(const gdn2_shape *shape, int32_t dtype) {
@@ -1052,84 +1118,84 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
                          float *dg_heads, float *d_initial, void *workspace, size_t workspace_bytes,
                          void *stream) {
     GDN2_TRY(check_inputs(shape, q, k, v, g, valid, reset));
-    if (initial) GDN2_TRY(check_view(initial, "initial", GDN2_F32, true));
+    if (initial) GDN2_TRY(check_state(initial, "initial"));
     GDN2_TRY(check_view(d_output, "d_output", q->dtype, false));
     const Plan p = plan(shape, q->dtype);
     const Layout lc = checkpoint_layout(p), l = workspace_layout(p, shape->time);
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, lc.bytes, "checkpoint"));
     GDN2_TRY(check_buffer(workspace, workspace_bytes, l.bytes, "workspace"));
     if (initial && !initial->data) initial = nullptr;
-    const int64_t K = shape->keys, V = shape->values, BH = p.BH;
+    const int64_t K = shape->keys, V = shape->values;
     const int dtype = q->dtype;
     const bool gates = dg || dg_heads;
+    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V) && vec_rows(d_output, V);
     hipStream_t st = (hipStream_t)stream;
-    const WalkArgs base = walk_args(shape, p, g, valid, reset);
+    const Walk base = base_walk(shape, p, g, valid, reset);
     const auto at = [&](size_t off) { return (float *)((char *)workspace + off); };
-    const float *states = (const float *)checkpoint;  // [BH, segments, K, V]
+    const float *states = (const float *)checkpoint;  // [B H, segments, K, V]
     const View first = make_view(initial), d_final{d_final_state, shape->heads * p.KV, p.KV, V, 1};
-    float *adj = at(l.state);
+    const bool many = p.segments > 1;
+    float *adj = nullptr;
     hipError_t e = hipSuccess;
-    if (p.segments > 1) {
-        e = run_carry(base, p, q, d_output, K, V, 1, d_final, adj, at(l.decay), dtype, st);
+    if (many && !p.prewalk) {
+        adj = at(l.state);
+        e = run_carry<true>(base, p, q, d_output, K, V, d_final, adj, at(l.decay), dtype, vec, st);
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
     }
-    const int64_t sb = p.segments * p.KV;
-    Walk wq = make_walk(d_output, v, k, V, K, 0);  // state transposed: rows V, columns K
-    wq.out = dq;
-    wq.init = states, wq.i_bh = sb, wq.i_seg = p.KV, wq.i_row = 1, wq.i_col = V;
-    set_first(&wq, first, true);
-    Walk wv = make_walk(k, q, d_output, K, V, 1);
-    wv.out = dv;
-    wv.init = adj, wv.i_bh = sb, wv.i_seg = p.KV, wv.i_row = V, wv.i_col = 1;
-    set_first(&wv, d_final, false);
-    wv.fin = d_initial, wv.n_bh = p.KV, wv.n_row = V, wv.n_col = 1;
-    Walk wk = make_walk(v, d_output, q, V, K, 1);
-    wk.out = dk;
-    wk.init = adj, wk.i_bh = sb, wk.i_seg = p.KV, wk.i_row = 1, wk.i_col = V;
-    set_first(&wk, d_final, true);
-    if (gates) {
-        wq.dot_x = q->data, wq.dx0 = q->stride[0], wq.dx1 = q->stride[1], wq.dx2 = q->stride[2],
-        wq.dx3 = q->stride[3];
-        wq.dots = at(l.x), wq.dot_sums = at(l.x_sums);
-        wv.dot_x = v->data, wv.dx0 = v->stride[0], wv.dx1 = v->stride[1], wv.dx2 = v->stride[2],
-        wv.dx3 = v->stride[3];
-        wv.dots = at(l.y), wv.dot_sums = at(l.y_sums);
-        wv.edges = at(l.edges);
-        wv.edge = states, wv.e_bh = sb, wv.e_seg = p.KV, wv.e_row = V, wv.e_col = 1;
-        wv.edge_first = (const float *)first.data, wv.ef_b = first.s0, wv.ef_h = first.s1,
-        wv.ef_row = first.s2, wv.ef_col = first.s3;
-    }
-    const bool one = (K <= 64) == (V <= 64);  // one launch covers all three
-    for (int n = 0; n < 2; ++n) {
-        WalkArgs a = base;
-        if (n == 0) {
-            if (dv || gates || d_initial) {
-                if (gates) a.totals = at(l.totals);
-                a.w[a.walks++] = wv;
-            }
-            if (!one && a.walks == 0) continue;
+    if (dv || gates || d_initial) {
+        Walk w = base;
+        set_triple(&w, k, q, d_output, K, V);
+        w.out = dv;
+        w.first = d_final;
+        w.starts = adj, w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
+        w.fin = d_initial;
+        if (gates) {
+            w.d = make_view(v);
+            w.dots = at(l.y), w.dot_sums = at(l.y_sums);
+            w.edges = at(l.edges), w.edge = states, w.edge_first = first;
+            w.totals = at(l.totals);
+            e = run_walk<true, true, true>(w, p, dtype, vec, st);
+        } else {
+            e = run_walk<true, true, false>(w, p, dtype, vec, st);
         }
-        if (n == 1 || one) {
-            if (dq || gates) a.w[a.walks++] = wq;
-            if (dk) a.w[a.walks++] = wk;
-        }
-        if (a.walks) e = run_walk<false>(a, p, dtype, st);
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
-        if (one) break;
+    }
+    if (dk) {
+        Walk w = base;
+        set_triple(&w, v, d_output, q, V, K);  // the state transposed: rows V, columns K
+        w.out = dk;
+        w.first = transposed(d_final);
+        w.starts = adj, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
+        e = run_walk<true, true, false>(w, p, dtype, vec, st);
+        if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
+    }
+    if (dq || gates) {
+        Walk w = base;
+        set_triple(&w, d_output, v, k, V, K);
+        w.out = dq;
+        w.first = transposed(first);
+        w.starts = many ? states : nullptr, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
+        if (gates) {
+            w.d = make_view(q);
+            w.dots = at(l.x), w.dot_sums = at(l.x_sums), w.pairs = at(l.pairs);
+            e = run_walk<false, true, true>(w, p, dtype, vec, st);
+        } else {
+            e = run_walk<false, true, false>(w, p, dtype, vec, st);
+        }
+        if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
     }
     if (!gates) return ok();
     GateGradArgs ga{};
     ga.w = base;
-    ga.q = make_view(q), ga.k = make_view(k), ga.v = make_view(v), ga.d_o = make_view(d_output);
-    ga.q_vec = vec_rows(q), ga.k_vec = vec_rows(k), ga.v_vec = vec_rows(v), ga.o_vec = vec_rows(d_output);
-    ga.K = (int)K, ga.V = (int)V;
-    ga.x = at(l.x), ga.y = at(l.y), ga.x_sums = at(l.x_sums), ga.y_sums = at(l.y_sums);
+    ga.x = at(l.x), ga.y = at(l.y), ga.pairs = at(l.pairs);
+    ga.x_sums = at(l.x_sums), ga.y_sums = at(l.y_sums);
     ga.edges = at(l.edges), ga.totals = at(l.totals);
+    ga.BH = p.BH;
     ga.x_slices = p.kslices, ga.y_slices = p.vslices;
-    ga.dg = dg ? dg : at(l.dinit);
-    const dim3 grid((unsigned)(BH * p.chunks)), block(kThreads);
-    if (dtype == GDN2_BF16) hipLaunchKernelGGL((linear_gate<bf16_t>), grid, block, 0, st, ga);
-    else hipLaunchKernelGGL((linear_gate<float>), grid, block, 0, st, ga);
+    ga.dg = dg ? dg : at(l.dg);
+    const dim3 grid((unsigned)((p.BH * p.chunks + kThreads / 64 - 1) / (kThreads / 64))), block(kThreads);
+    if (dtype == GDN2_BF16) hipLaunchKernelGGL((linear_gate<Mat<bf16_t>::C>), grid, block, 0, st, ga);
+    else hipLaunchKernelGGL((linear_gate<Mat<float>::C>), grid, block, 0, st, ga);
     if (dg_heads)
         hipLaunchKernelGGL(linear_head_sum, dim3((unsigned)shape->heads), dim3(1024), 0, st, ga.dg,
                            shape->batch * shape->time, shape->heads, dg_heads);
