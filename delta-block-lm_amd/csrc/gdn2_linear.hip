@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCols = 64;       // columns of c (and of the state) that a workgroup owns
+constexpr int kGates = 8;       // chunks whose gates are made at a time, two by each wave
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
@@ -195,50 +196,57 @@ __device__ __forceinline__ void gate_store(const GateIn &x, GateTile<C> *o) {
     }
 }
 
-// A tile of C rows and W columns on its way from memory to LDS: 16 bytes a thread and turn, the rows
-// of a (batch, head) at base.  VEC: unit channel stride, 16-byte aligned rows, whole pieces, and
-// offsets inside a chunk below 2^31 bytes.
+// A tile of C rows and W columns on its way from memory to LDS: 16 bytes a thread and turn.  Rows past
+// the end and columns past the width read others in their place, and become zero on the way to LDS,
+// as do the rows of padding: what they hold is not used.  VEC: unit channel stride, 16-byte aligned
+// rows, whole pieces, and offsets inside a chunk below 2^31 bytes.
 template <typename T, int W, bool VEC>
 struct Staged {
     static constexpr int N = Mat<T>::N, C = Mat<T>::C, PER = W / N, ROWS = kThreads / PER,
                          PIECES = C / ROWS;
     uint4 r[PIECES];
-    __device__ __forceinline__ void load(const View &x, int64_t b, int64_t h, int64_t t0, int64_t T_,
-                                         int c0, int width) {
+    // base: row 0 of the (batch, head), column 0 of the tile; width: columns there are from it on
+    __device__ __forceinline__ void load(const T *base, int64_t s1, int64_t s3, int64_t t0, int left, int width) {
         const int row = threadIdx.x / PER, c = threadIdx.x % PER * N;
-        const T *base = reinterpret_cast<const T *>(x.data) + b * x.s0 + h * x.s2 + t0 * x.s1;
-        const int left = (int)min(T_ - t0, (int64_t)C);
+        base += t0 * s1;
         if constexpr (VEC) {
-            const char *p = reinterpret_cast<const char *>(base + c0);
-            const uint32_t step = (uint32_t)x.s1 * (uint32_t)sizeof(T);
-            const uint32_t off = (uint32_t)row * step + (uint32_t)c * (uint32_t)sizeof(T);
-            const bool in = c0 + c < width;
+            const char *p = reinterpret_cast<const char *>(base);
+            const uint32_t step = (uint32_t)s1 * (uint32_t)sizeof(T);
+            const uint32_t col = (uint32_t)(c < width ? c : 0) * (uint32_t)sizeof(T);
+            if (left >= C) {
+                const uint32_t off = (uint32_t)row * step + col;
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                r[i] = make_uint4(0, 0, 0, 0);
-                if (in && row + i * ROWS < left)
+                for (int i = 0; i < PIECES; ++i)
                     r[i] = *reinterpret_cast<const uint4 *>(p + (off + (uint32_t)(i * ROWS) * step));
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    r[i] = *reinterpret_cast<const uint4 *>(p + ((uint32_t)min(row + i * ROWS, left - 1) * step + col));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
+                const T *q = base + (int64_t)min(row + i * ROWS, left - 1) * s1;
                 T e[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    e[j] = row + i * ROWS < left && c0 + c + j < width
-                               ? base[(int64_t)(row + i * ROWS) * x.s1 + (int64_t)(c0 + c + j) * x.s3] : T(0);
+                for (int j = 0; j < N; ++j) e[j] = c + j < width ? q[(int64_t)(c + j) * s3] : T(0);
                 __builtin_memcpy(&r[i], e, 16);
             }
         }
     }
-    // Rows of padding become zero: what they hold is not used.
     template <int LD>
-    __device__ __forceinline__ void store(T *tile, const int *seg) const {
+    __device__ __forceinline__ void store(T *tile, const int *seg, bool masks, int width) const {
         const int row = threadIdx.x / PER, c = threadIdx.x % PER * N;
+        T *p = tile + row * LD + c;
+        if (!masks) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4 *>(p + i * ROWS * LD) = r[i];
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
-            *reinterpret_cast<uint4 *>(tile + (row + i * ROWS) * LD + c) =
-                seg[row + i * ROWS] >= 0 ? r[i] : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(p + i * ROWS * LD) =
+                seg[row + i * ROWS] >= 0 && c < width ? r[i] : make_uint4(0, 0, 0, 0);
     }
 };
 
@@ -258,12 +266,31 @@ __device__ __forceinline__ void store4(T *out, int64_t row, int col, int width, 
     }
 }
 
-// Gam of the pair (out token t, source token s), 0 where s is not seen from t.
-template <int C, bool REV>
-__device__ __forceinline__ float pair_decay(const GateTile<C> &gt, int t, int s) {
-    const float d = (gt.hi[t] - gt.hi[s]) + (gt.lo[t] - gt.lo[s]);
-    const bool on = gt.seg[t] == gt.seg[s] && (REV ? s >= t : s <= t);
-    return on ? __builtin_amdgcn_exp2f(REV ? -d : d) : 0.f;
+// Gam of the pairs of out token t with the sources s .. s + 3, 0 for those that t does not see.  EXACT
+// adds the sums' lower parts; without them a decay is off by 2^-24 of the sum since the last cut, at
+// most 2^-11 where the pair still counts, which a bf16 weight does not show.
+template <int C, bool REV, bool EXACT>
+__device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s) {
+    const float ht = gt.hi[t];
+    const int st = gt.seg[t];
+    const f32x4 hs = *reinterpret_cast<const f32x4 *>(gt.hi + s);
+    const int4 ss = *reinterpret_cast<const int4 *>(gt.seg + s);
+    const int seg[4] = {ss.x, ss.y, ss.z, ss.w};
+    f32x4 f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = REV ? hs[i] - ht : ht - hs[i];
+    if (EXACT) {
+        const float lt = gt.lo[t];
+        const f32x4 ls = *reinterpret_cast<const f32x4 *>(gt.lo + s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] += REV ? ls[i] - lt : lt - ls[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool on = seg[i] == st && (REV ? s + i >= t : s + i <= t);
+        f[i] = __builtin_amdgcn_exp2f(on ? f[i] : -1000.f);
+    }
+    return f;
 }
 
 // Sum over the four 16-lane groups of a wave.
@@ -278,7 +305,7 @@ struct WalkLds {
                          LDP = C + Mat<T>::PAD;
     T b[C * LDA], c[C * LDC];
     T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
-    GateTile<C> gate[2];
+    GateTile<C> gate[kGates];
     float red[4][C];
     float rows[3][C], cols[3][C], diag[C];  // parts of the pair sums, by tiles of 16 tokens
 };
@@ -291,38 +318,52 @@ struct State {
 #pragma unroll
         for (int m = 0; m < KT; ++m) t[m] = zero4();
     }
+    // Whether no value of the wave's part is infinite or NaN.
+    __device__ __forceinline__ bool finite() const {
+        float z = 0.f;
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z = fmaf(t[m][i], 0.f, z);
+        return !__any(z != 0.f);  // z is 0 or NaN
+    }
     // Rows and columns of src at strides below 2^22 (32-bit offsets: 64 addresses would spill).
     __device__ __forceinline__ void load(const float *src, int rs, int cs, int v, int ka, int vc) {
         const int g4 = 4 * (lane_id() >> 4);
-        if (v >= vc) return;
+        const uint32_t col = (uint32_t)(min(v, vc - 1) * cs);
 #pragma unroll
-        for (int m = 0; m < KT; ++m) {
-            const int k = 16 * m + g4;
-            const uint32_t at = (uint32_t)(k * rs + v * cs);
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (k + i < ka) t[m][i] = src[at + (uint32_t)(i * rs)];
-        }
+            for (int i = 0; i < 4; ++i) {
+                const int k = 16 * m + g4 + i;
+                const float x = src[col + (uint32_t)(min(k, ka - 1) * rs)];
+                t[m][i] = k < ka && v < vc ? x : 0.f;
+            }
     }
     // Dense rows of vc columns.
     __device__ __forceinline__ void store(float *dst, int v, int ka, int vc) const {
         const int g4 = 4 * (lane_id() >> 4);
         if (v >= vc) return;
+        dst += g4 * vc + v;
+        if (ka == 16 * KT) {
 #pragma unroll
-        for (int m = 0; m < KT; ++m) {
-            const int k = 16 * m + g4;
-            const uint32_t at = (uint32_t)(k * vc + v);
+            for (int m = 0; m < KT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dst[(uint32_t)((16 * m + i) * vc)] = t[m][i];
+            return;
+        }
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (k + i < ka) dst[at + (uint32_t)(i * vc)] = t[m][i];
-        }
+                if (16 * m + g4 + i < ka) dst[(uint32_t)((16 * m + i) * vc)] = t[m][i];
     }
 };
 
-// What the chunk adds to the state, apart from the state: col_s b_s c_s^T over its tokens.  Whether
-// that is finite tells whether b and c are.
+// The state after the chunk, tot S + sum_s col_s b_s c_s^T, and whether all of it is finite.
 template <typename T, int KP>
-__device__ __forceinline__ bool update(State<KP / 16> &U, const typename Mat<T>::Frag (&cf)[Mat<T>::C / Mat<T>::RB],
+__device__ __forceinline__ bool update(State<KP / 16> &U, const State<KP / 16> &S, float tot,
+                                       const typename Mat<T>::Frag (&cf)[Mat<T>::C / Mat<T>::RB],
                                        const T *b, const float *col) {
     typedef Mat<T> M;
     constexpr int KT = KP / 16, RB = M::RB, LDA = KP + M::PAD;
@@ -330,35 +371,40 @@ __device__ __forceinline__ bool update(State<KP / 16> &U, const typename Mat<T>:
 #pragma unroll
     for (int r = 0; r < M::C / RB; ++r) {
         const float *f = col + r * RB + (RB / 4) * (lane_id() >> 4);
-        if constexpr (sizeof(T) == 2) {
-            float x[8];
+        // Four tiles one after the other: a product waits for none of the others.
+        Split3 s3;
+        float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(cf[r][e]) * f[e];
-            const Split3 s3 = split3(x);
+        for (int e = 0; e < RB / 4; ++e) x[e] = static_cast<float>(cf[r][e]) * f[e];
+        if constexpr (sizeof(T) == 2) s3 = split3(x);
 #pragma unroll
-            for (int m = 0; m < KT; ++m) {
-                const typename M::Frag y = M::template across<LDA>(b, r * RB, 16 * m);
+        for (int m0 = 0; m0 < KT; m0 += 4) {
+            typename M::Frag y[4];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) M::mma(U.t[m], y, s3.t[q]);
+            for (int m = 0; m < 4; ++m) y[m] = M::template across<LDA>(b, r * RB, 16 * (m0 + m));
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) M::mma(U.t[m0 + m], y[m], s3.t[q]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+                        U.t[m0 + m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[m][e], x[e], U.t[m0 + m], 0, 0, 0);
             }
-        } else {
-            f32x4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = cf[r][e] * f[e];
-#pragma unroll
-            for (int m = 0; m < KT; ++m) M::mma(U.t[m], M::template across<LDA>(b, r * RB, 16 * m), x);
         }
     }
-    float z = 0.f;
 #pragma unroll
     for (int m = 0; m < KT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z = fmaf(U.t[m][i], 0.f, z);
-    return !__any(z != 0.f);  // z is 0 or NaN
+        for (int i = 0; i < 4; ++i) U.t[m][i] = fmaf(tot, S.t[m][i], U.t[m][i]);
+    return U.finite();
 }
 
-// A chunk whose b or c holds a value that is not finite, token by token: a product over masked tokens
-// would spread the value to tokens that do not see it.
+// A chunk token by token, taken where the state before or after it is not finite: products over masked
+// tokens, and with factors that are 0, would spread such a value to tokens that do not see it.
 template <typename T, int KP, bool REV, bool OUT>
 __device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const T *b, const T *c,
                                                       const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
@@ -423,69 +469,92 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
     const int col0 = slice * kCols, v = col0 + 16 * wave + n16;
     const int c_lo = seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
 
-    State<KT> S;
-    S.zero();
     int n = c_hi - c_lo;   // chunks to walk, the last `out` of them with results
     const int out = OUT ? n : 0;
-    if (OUT) {
-        if (nth > 0 && p.starts) {
-            S.load(p.starts + bh * p.s_bh + seg * (int64_t)p.ka * p.vc, p.s_row, p.s_col, v, p.ka, p.vc);
-        } else {
-            if (p.first.data)
-                S.load(reinterpret_cast<const float *>(p.first.data) + b * p.first.s0 + h * p.first.s1,
-                       (int)p.first.s2, (int)p.first.s3, v, p.ka, p.vc);
-            n = REV ? p.chunks - c_lo : c_hi;
-        }
-    }
+    const bool walked = OUT && !(nth > 0 && p.starts);  // from the sequence's start
+    if (walked) n = REV ? p.chunks - c_lo : c_hi;
     float decay = 1.f;
     int ci = REV ? c_lo + n - 1 : c_hi - n;
 
     Staged<T, KP, VEC> sa, sb;
     Staged<T, kCols, VEC> sc, sd;
-    GateIn gi{};
+    const auto base = [&](const View &x, int c0) {
+        return reinterpret_cast<const T *>(x.data) + b * x.s0 + h * x.s2 + c0 * x.s3;
+    };
+    const T *pa = base(p.a, 0), *pb = base(p.b, 0), *pc = base(p.c, col0), *pd = base(p.d, col0);
+    const int wide = p.vc - col0;  // columns of c and d
     const auto fetch = [&](int chunk, bool full) {
         const int64_t t0 = (int64_t)chunk * C;
-        sb.load(p.b, b, h, t0, p.T, 0, p.ka);
-        sc.load(p.c, b, h, t0, p.T, col0, p.vc);
+        const int left = (int)min(p.T - t0, (int64_t)C);
+        sb.load(pb, p.b.s1, p.b.s3, t0, left, p.ka);
+        sc.load(pc, p.c.s1, p.c.s3, t0, left, wide);
         if (OUT && full) {
-            sa.load(p.a, b, h, t0, p.T, 0, p.ka);
-            if (DOT) sd.load(p.d, b, h, t0, p.T, col0, p.vc);
+            sa.load(pa, p.a.s1, p.a.s3, t0, left, p.ka);
+            if (DOT) sd.load(pd, p.d.s1, p.d.s3, t0, left, wide);
         }
-        if (wave == 0) gi = gate_load<C>(p, b, h, chunk);
+    };
+    // The gates of the next kGates chunks of the walk.
+    const auto gates = [&]() {
+        GateIn x[kGates / 4];
+#pragma unroll
+        for (int i = 0; i < kGates / 4; ++i)
+            if (wave + 4 * i < n) x[i] = gate_load<C>(p, b, h, ci + (REV ? -1 : 1) * (wave + 4 * i));
+#pragma unroll
+        for (int i = 0; i < kGates / 4; ++i)
+            if (wave + 4 * i < n) gate_store<C, REV>(x[i], &lds.gate[wave + 4 * i]);
     };
     fetch(ci, n <= out);
-    if (wave == 0) gate_store<C, REV>(gi, &lds.gate[n & 1]);
+    State<KT> S;
+    S.zero();
+    if (OUT) {
+        const float *src = reinterpret_cast<const float *>(p.first.data);
+        int rs = (int)p.first.s2, cs = (int)p.first.s3;
+        int64_t at = b * p.first.s0 + h * p.first.s1;
+        if (!walked) {
+            src = p.starts, rs = p.s_row, cs = p.s_col;
+            at = bh * p.s_bh + seg * (int64_t)p.ka * p.vc;
+        }
+        if (src) S.load(src + at, rs, cs, v, p.ka, p.vc);
+    }
+    int gi = 0;  // the chunk's place among the gates in LDS
+    gates();
     __syncthreads();
 
-    // The chunk's update from the tiles in LDS, and whether it is finite.
-    const auto add = [&](typename M::Frag (&cf)[C / RB], State<KT> &U, const GateTile<C> &gate) {
+    const bool masks = p.valid.data || p.T % C || p.ka < KP || wide < kCols;
+    bool fine = S.finite();  // the state is: held at the start of every chunk that is taken by products
+    const auto across_c = [&](typename M::Frag (&cf)[C / RB]) {
 #pragma unroll
         for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
-        decay *= gate.tot;
-        return update<T, KP>(U, cf, lds.b, gate.col);
     };
-    const auto advance = [&](const State<KT> &U, float tot) {
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S.t[m][i] = (tot == 0.f ? 0.f : S.t[m][i] * tot) + U.t[m][i];
+
+    const auto next_gates = [&]() {
+        --n, ci += REV ? -1 : 1;  // as seen from the next chunk
+        gates();
+        ++n, ci -= REV ? -1 : 1;
+        gi = 0;
+        __syncthreads();
     };
 
     for (; n > out; --n, ci += REV ? -1 : 1) {
-        const GateTile<C> &gate = lds.gate[n & 1];
-        sb.template store<LDA>(lds.b, gate.seg);
-        sc.template store<LDC>(lds.c, gate.seg);
+        const GateTile<C> &gate = lds.gate[gi];
+        sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
+        sc.template store<LDC>(lds.c, gate.seg, masks, wide);
         if (n > 1) fetch(REV ? ci - 1 : ci + 1, n - 1 <= out);
         __syncthreads();
         typename M::Frag cf[C / RB];
+        across_c(cf);
         State<KT> U;
-        if (__builtin_expect(add(cf, U, gate), 1))
-            advance(U, gate.tot);
-        else
+        const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
+        decay *= gate.tot;
+        if (__builtin_expect(fine && next, 1)) {
+            S = U;
+        } else {
             walk_tokens<T, KP, REV, false>(S, lds.b, lds.b, lds.c, gate, p.ka, v, p.vc, nullptr, 0,
                                            (int)min(p.T - (int64_t)ci * C, (int64_t)C));
-        if (n > 1 && wave == 0) gate_store<C, REV>(gi, &lds.gate[(n - 1) & 1]);
-        __syncthreads();  // the chunk's tiles are read, the next one's gates written
+            fine = S.finite();
+        }
+        __syncthreads();  // the chunk's tiles are read
+        if (++gi == kGates && n > 1) next_gates();
     }
     if (!OUT) {
         S.store(p.seg_state + ((int64_t)bh * p.segments + seg) * p.ka * p.vc, v, p.ka, p.vc);
@@ -496,11 +565,11 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
         S.store(p.starts_out + bh * p.s_bh + seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
 
     for (; n > 0; --n, ci += REV ? -1 : 1) {
-        const GateTile<C> &gate = lds.gate[n & 1];
-        sa.template store<LDA>(lds.a, gate.seg);
-        sb.template store<LDA>(lds.b, gate.seg);
-        sc.template store<LDC>(lds.c, gate.seg);
-        if (DOT) sd.template store<LDC>(lds.d, gate.seg);
+        const GateTile<C> &gate = lds.gate[gi];
+        sa.template store<LDA>(lds.a, gate.seg, masks, p.ka);
+        sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
+        sc.template store<LDC>(lds.c, gate.seg, masks, wide);
+        if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, wide);
         if (n > 1) fetch(REV ? ci - 1 : ci + 1, true);
         __syncthreads();
 
@@ -518,13 +587,10 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
                 for (int r = 0; r < KP; r += RB)
                     M::mma(x, M::row(lds.b + 16 * si * LDA, LDA, r), M::row(lds.a + 16 * tj * LDA, LDA, r));
                 const int t = 16 * tj + n16, s = 16 * si + g4;
+                const f32x4 f = pair_decays<C, REV, DOT || sizeof(T) == 4>(gate, t, s);
                 T e[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = pair_decay<C, REV>(gate, t, s + i);
-                    x[i] = f == 0.f ? 0.f : x[i] * f;
-                    Elem<T>::store(e, i, x[i]);
-                }
+                for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
                 __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
                 if (PAIRS && si <= tj) {
                     f32x4 y = zero4();
@@ -533,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
                         M::mma(y, M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        y[i] = x[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
+                        y[i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
                     if (si < tj) {
                         const float sum = groups_sum((y[0] + y[1]) + (y[2] + y[3]));
                         if (lane < 16) lds.rows[si][t] = sum;
@@ -580,13 +646,13 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
             for (int j = 0; j < TT; ++j) {
                 const float f = gate.row[16 * j + n16];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = f == 0.f ? 0.f : acc[j][i] * f;
+                for (int i = 0; i < 4; ++i) acc[j][i] *= f;
                 if (DOT) {
                     const T *d = lds.d + (16 * j + n16) * LDC + 16 * wave + g4;
                     float x = 0.f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x += acc[j][i] * Elem<T>::load(d, i);
-                    x = groups_sum(f == 0.f ? 0.f : x);
+                    x = groups_sum(f == 0.f ? 0.f : x);  // also where the state is not finite
                     if (lane < 16) lds.red[wave][16 * j + n16] = x;
                 }
             }
@@ -638,11 +704,12 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
         }
 
         typename M::Frag cf[C / RB];
+        across_c(cf);
         State<KT> U;
-        const bool fine = add(cf, U, gate);
+        const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
         T *o = reinterpret_cast<T *>(p.out);
         const int64_t row0 = (b * p.T + (int64_t)ci * C) * p.H + h;
-        if (__builtin_expect(fine, 1)) {
+        if (__builtin_expect(fine && next, 1)) {
             if (o) {
                 const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
 #pragma unroll
@@ -656,14 +723,15 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
                         store4<T, VEC>(o, row0 + (int64_t)t * p.H, col0 + 16 * wave + g4, p.vc, acc[j]);
                 }
             }
-            advance(U, gate.tot);
+            S = U;
         } else {
             T *at = o ? o + row0 * p.vc : nullptr;
             walk_tokens<T, KP, REV, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc, at, (int64_t)p.H * p.vc,
                                          (int)min(p.T - (int64_t)ci * C, (int64_t)C));
+            fine = S.finite();
         }
-        if (n > 1 && wave == 0) gate_store<C, REV>(gi, &lds.gate[(n - 1) & 1]);
-        __syncthreads();  // the chunk's tiles are read, the next one's gates written
+        __syncthreads();  // the chunk's tiles are read
+        if (++gi == kGates && n > 1) next_gates();
     }
 
     if (p.fin && nth == p.segments - 1) S.store(p.fin + (int64_t)bh * p.ka * p.vc, v, p.ka, p.vc);
