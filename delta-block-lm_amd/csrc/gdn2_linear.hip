@@ -153,21 +153,16 @@ struct GateIn {
 
 template <int C>
 __device__ __forceinline__ GateIn gate_load(const Walk &p, int64_t b, int64_t h, int64_t chunk) {
-    const int l = lane_id();
-    const int64_t t = chunk * C + l;
-    GateIn x{0.f, 0.f, 0.f};
-    if (l < C && t < p.T) {
-        x.valid = p.valid.data ? ld4<float>(p.valid, b, t, 0, 0) : 1.f;
-        x.reset = p.reset.data ? ld4<float>(p.reset, b, t, 0, 0) : 0.f;
-        x.g = ld4<float>(p.g, b, t, h, 0);
-    }
-    return x;
+    const int64_t t = min(chunk * C + lane_id(), p.T - 1);
+    const auto at = [&](const View &x) { return reinterpret_cast<const float *>(x.data) + b * x.s0 + t * x.s1; };
+    const float *g = at(p.g) + h * p.g.s2;
+    return GateIn{*g, p.valid.data ? *at(p.valid) : 1.f, p.reset.data ? *at(p.reset) : 0.f};
 }
 
 template <int C, bool REV>
-__device__ __forceinline__ void gate_store(const GateIn &x, GateTile<C> *o) {
+__device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C> *o) {
     const int l = lane_id();
-    const bool val = x.valid != 0.f;
+    const bool val = l < left && l < C && x.valid != 0.f;
     float g = val ? x.g : 0.f;
     const bool cut = val && (x.reset != 0.f || g < kCut);
     if (cut) g = 0.f;
@@ -310,6 +305,10 @@ struct WalkLds {
     float rows[3][C], cols[3][C], diag[C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
+// Holds a loaded value where it is: the compiler otherwise moves each load under the condition that
+// selects it, one after the other, and waits for every one.
+__device__ __forceinline__ void keep(float &x) { asm volatile("" : "+v"(x)); }
+
 // State of one wave: 16 columns, accumulator tiles of 16 rows.
 template <int KT>
 struct State {
@@ -334,10 +333,14 @@ struct State {
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
+            for (int i = 0; i < 4; ++i) t[m][i] = src[col + (uint32_t)(min(16 * m + g4 + i, ka - 1) * rs)];
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int k = 16 * m + g4 + i;
-                const float x = src[col + (uint32_t)(min(k, ka - 1) * rs)];
-                t[m][i] = k < ka && v < vc ? x : 0.f;
+                float x = t[m][i];
+                keep(x);
+                t[m][i] = 16 * m + g4 + i < ka && v < vc ? x : 0.f;
             }
     }
     // Dense rows of vc columns.
@@ -495,13 +498,10 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
     };
     // The gates of the next kGates chunks of the walk.
     const auto gates = [&]() {
-        GateIn x[kGates / 4];
-#pragma unroll
-        for (int i = 0; i < kGates / 4; ++i)
-            if (wave + 4 * i < n) x[i] = gate_load<C>(p, b, h, ci + (REV ? -1 : 1) * (wave + 4 * i));
-#pragma unroll
-        for (int i = 0; i < kGates / 4; ++i)
-            if (wave + 4 * i < n) gate_store<C, REV>(x[i], &lds.gate[wave + 4 * i]);
+        for (int i = wave; i < min(n, kGates); i += 4) {
+            const int64_t at = ci + (REV ? -i : i);
+            gate_store<C, REV>(gate_load<C>(p, b, h, at), (int)min(p.T - at * C, (int64_t)C), &lds.gate[i]);
+        }
     };
     fetch(ci, n <= out);
     State<KT> S;
