@@ -35,7 +35,7 @@ struct LnArgs {
 
 // N adjacent elements as floats.
 template <typename T, int N>
-__device__ __forceinline__ void load_n(const T *p, int64_t s, float (&v)[N]) {
+__device__ __forceinline__ void load_n(const T *p, float (&v)[N]) {
     if constexpr (N == 1) {
         v[0] = Elem<T>::load(p, 0);
     } else if constexpr (sizeof(T) == 2) {
@@ -45,8 +45,11 @@ __device__ __forceinline__ void load_n(const T *p, int64_t s, float (&v)[N]) {
         for (int j = 0; j < 4; ++j)
             v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
     } else {
-        const float4 q = *reinterpret_cast<const float4 *>(p);
-        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(p + j);
+            v[j] = q.x, v[j + 1] = q.y, v[j + 2] = q.z, v[j + 3] = q.w;
+        }
     }
 }
 template <typename T, int N>
@@ -57,13 +60,36 @@ __device__ __forceinline__ void store_n(T *p, const float (&v)[N]) {
     __builtin_memcpy(__builtin_assume_aligned(p, N * sizeof(T)), e, sizeof e);
 }
 
-// Sums over the G threads of a row, in every one of them.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float readlane_f(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Sums over the G threads of a row, in every one of them: lane moves inside 16 lanes, K sums at a time
+// so that one's waits are the others' work.
 template <int G, int K>
 __device__ __forceinline__ void row_sum(float (&x)[K], float *red) {
+    static_assert(G >= 8, "");
 #pragma unroll
-    for (int d = 1; d < (G < 64 ? G : 64); d *= 2)
+    for (int k = 0; k < K; ++k) x[k] += dpp_f<0xB1>(x[k]);
 #pragma unroll
-        for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], d);
+    for (int k = 0; k < K; ++k) x[k] += dpp_f<0x4E>(x[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] += dpp_f<0x141>(x[k]);
+    if constexpr (G >= 16)
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k] += dpp_f<0x140>(x[k]);
+    if constexpr (G == 32)
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k] += __shfl_xor(x[k], 16);
+    if constexpr (G >= 64)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            x[k] = (readlane_f(x[k], 0) + readlane_f(x[k], 16)) + (readlane_f(x[k], 32) + readlane_f(x[k], 48));
     if constexpr (G > 64) {
         constexpr int WAVES = G / 64;
         const int wave = threadIdx.x >> 6;
@@ -97,108 +123,143 @@ struct Row {
             const int c = N * (l + j * G);
 #pragma unroll
             for (int e = 0; e < N; ++e) v[j][e] = 0.f;
-            if (c < W) load_n<T, N>(reinterpret_cast<const T *>(base) + at + c * (N == 1 ? s : 1), s, v[j]);
+            if (c < W) load_n<T, N>(reinterpret_cast<const T *>(base) + at + c * (N == 1 ? s : 1), v[j]);
         }
     }
 };
 
-template <typename T, int N, int G, int E>
+// R rows a group at once, their loads and sums side by side.
+template <typename T, int N, int G, int E, int R>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel(LnArgs p) {
     constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
-    __shared__ float red[2 * (G > 64 ? G / 64 : 1)];
+    __shared__ float red[R * (G > 64 ? G / 64 : 1)];
+    typedef Row<T, N, G, E> X;
     const int l = threadIdx.x % G;
-    const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
-    const bool on = r < p.rows;  // the row's threads stay for its sums
-    typedef Row<T, N, G, E> R;
-    R x{};
-    if (on) x.load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
-    float s[1] = {0.f};
+    const int64_t r0 = ((int64_t)blockIdx.x * ROWS + threadIdx.x / G) * R;
+    X x[R];
 #pragma unroll
-    for (int j = 0; j < R::P; ++j)
+    for (int i = 0; i < R; ++i)  // rows past the end read the last one again
+        x[i].load(p.x.data, row_at(p.x, p, min(r0 + i, p.rows - 1)), p.x.s3, l, p.W);
+    float w[X::P][N], b[X::P][N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[0] += x.v[j][e];
-    row_sum<G, 1>(s, red);
-    const float m = s[0] / p.W;
-    s[0] = 0.f;
-#pragma unroll
-    for (int j = 0; j < R::P; ++j)
-        if (N * (l + j * G) < p.W)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                x.v[j][e] -= m;
-                s[0] = fmaf(x.v[j][e], x.v[j][e], s[0]);
-            }
-    row_sum<G, 1>(s, red);
-    const float inv = 1.f / sqrtf(s[0] / p.W + p.epsilon);
-    if (!on) return;
-    if (l == 0) {
-        if (p.mean) p.mean[r] = m;
-        if (p.inverse) p.inverse[r] = inv;
-    }
-    T *y = reinterpret_cast<T *>(p.y) + r * p.W;
-#pragma unroll
-    for (int j = 0; j < R::P; ++j) {
-        const int c = N * (l + j * G);
-        if (c >= p.W) continue;
-        float o[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            o[e] = fmaf(x.v[j][e] * inv, p.weight[c + e], p.bias ? p.bias[c + e] : 0.f);
-        store_n<T, N>(y + c, o);
-    }
-}
-
-template <typename T, int N, int G, int E>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kernel(LnArgs p) {
-    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
-    __shared__ float red[2 * (G > 64 ? G / 64 : 1)];
-    __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
-    const int l = threadIdx.x % G, g = threadIdx.x / G;
-    typedef Row<T, N, G, E> R;
-    float w[R::P][N], dw[R::P][N], db[R::P][N];
-#pragma unroll
-    for (int j = 0; j < R::P; ++j) {
+    for (int j = 0; j < X::P; ++j) {
         const int c = N * (l + j * G);
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[j][e] = c < p.W ? p.weight[c + e] : 0.f, dw[j][e] = db[j][e] = 0.f;
-    }
-    // Every group of the workgroup makes the same number of turns: row_sum has barriers.
-    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t r = r0 + g;
-        const bool on = r < p.rows;
-        R x{}, dy{};
-        float m = 0.f, inv = 0.f;
-        if (on) {
-            x.load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
-            dy.load(p.dy.data, row_at(p.dy, p, r), p.dy.s3, l, p.W);
-            m = p.mean[r], inv = p.inverse[r];
+        for (int e = 0; e < N; ++e) w[j][e] = b[j][e] = 0.f;
+        if (c < p.W) {
+            load_n<float, N>(p.weight + c, w[j]);
+            if (p.bias) load_n<float, N>(p.bias + c, b[j]);
         }
-        float s[2] = {0.f, 0.f};
+    }
+    float m[R], s[R];
 #pragma unroll
-        for (int j = 0; j < R::P; ++j)
-            if (on && N * (l + j * G) < p.W)
+    for (int i = 0; i < R; ++i) {
+        m[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < X::P; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) m[i] += x[i].v[j][e];
+    }
+    row_sum<G, R>(m, red);
+    const float W = (float)p.W;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        m[i] /= W;
+        s[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < X::P; ++j)
+            if (N * (l + j * G) < p.W)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const float xh = (x.v[j][e] - m) * inv, d = dy.v[j][e];
-                    dw[j][e] = fmaf(d, xh, dw[j][e]);
-                    db[j][e] += d;
-                    const float c = d * w[j][e];
-                    s[0] += c;
-                    s[1] = fmaf(c, xh, s[1]);
-                    x.v[j][e] = xh, dy.v[j][e] = c;
+                    x[i].v[j][e] -= m[i];
+                    s[i] = fmaf(x[i].v[j][e], x[i].v[j][e], s[i]);
                 }
-        row_sum<G, 2>(s, red);
-        if (!on || !p.y) continue;
-        const float a = s[0] / p.W, c2 = s[1] / p.W;
-        T *dx = reinterpret_cast<T *>(p.y) + r * p.W;
+    }
+    row_sum<G, R>(s, red);
 #pragma unroll
-        for (int j = 0; j < R::P; ++j) {
+    for (int i = 0; i < R; ++i) {
+        const int64_t r = r0 + i;
+        if (r >= p.rows) break;
+        const float inv = 1.f / sqrtf(s[i] / W + p.epsilon);
+        if (l == 0) {
+            if (p.mean) p.mean[r] = m[i];
+            if (p.inverse) p.inverse[r] = inv;
+        }
+        T *y = reinterpret_cast<T *>(p.y) + r * p.W;
+#pragma unroll
+        for (int j = 0; j < X::P; ++j) {
             const int c = N * (l + j * G);
             if (c >= p.W) continue;
             float o[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = inv * ((dy.v[j][e] - a) - x.v[j][e] * c2);
-            store_n<T, N>(dx + c, o);
+            for (int e = 0; e < N; ++e) o[e] = fmaf(x[i].v[j][e] * inv, w[j][e], b[j][e]);
+            store_n<T, N>(y + c, o);
+        }
+    }
+}
+
+template <typename T, int N, int G, int E, int R>
+__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kernel(LnArgs p) {
+    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
+    __shared__ float red[2 * R * (G > 64 ? G / 64 : 1)];
+    __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
+    const int l = threadIdx.x % G, g = threadIdx.x / G;
+    typedef Row<T, N, G, E> X;
+    float w[X::P][N], dw[X::P][N], db[X::P][N];
+#pragma unroll
+    for (int j = 0; j < X::P; ++j) {
+        const int c = N * (l + j * G);
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[j][e] = dw[j][e] = db[j][e] = 0.f;
+        if (c < p.W) load_n<float, N>(p.weight + c, w[j]);
+    }
+    const float W = (float)p.W;
+    // Every group of the workgroup makes the same number of turns: row_sum has barriers.
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS * R; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS * R) {
+        X x[R], dy[R];
+        float m[R], inv[R], s[2 * R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = min(r0 + g * R + i, p.rows - 1);
+            x[i].load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
+            dy[i].load(p.dy.data, row_at(p.dy, p, r), p.dy.s3, l, p.W);
+            m[i] = p.mean[r], inv[i] = p.inverse[r];
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            s[2 * i] = s[2 * i + 1] = 0.f;
+            const bool on = r0 + g * R + i < p.rows;  // the others add nothing
+#pragma unroll
+            for (int j = 0; j < X::P; ++j)
+                if (on && N * (l + j * G) < p.W)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const float xh = (x[i].v[j][e] - m[i]) * inv[i], d = dy[i].v[j][e];
+                        dw[j][e] = fmaf(d, xh, dw[j][e]);
+                        db[j][e] += d;
+                        const float c = d * w[j][e];
+                        s[2 * i] += c;
+                        s[2 * i + 1] = fmaf(c, xh, s[2 * i + 1]);
+                        x[i].v[j][e] = xh, dy[i].v[j][e] = c;
+                    }
+        }
+        row_sum<G, 2 * R>(s, red);
+        if (!p.y) continue;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = r0 + g * R + i;
+            if (r >= p.rows) break;
+            const float a = s[2 * i] / W, c2 = s[2 * i + 1] / W;
+            T *dx = reinterpret_cast<T *>(p.y) + r * p.W;
+#pragma unroll
+            for (int j = 0; j < X::P; ++j) {
+                const int c = N * (l + j * G);
+                if (c >= p.W) continue;
+                float o[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] = inv[i] * ((dy[i].v[j][e] - a) - x[i].v[j][e] * c2);
+                store_n<T, N>(dx + c, o);
+            }
         }
     }
     // The workgroup's column sums, over its groups in order.
@@ -209,7 +270,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kerne
         part += (int64_t)blockIdx.x * p.W;
         if constexpr (ROWS == 1) {
 #pragma unroll
-            for (int j = 0; j < R::P; ++j)
+            for (int j = 0; j < X::P; ++j)
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     const int c = N * (l + j * G) + e;
@@ -218,7 +279,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kerne
         } else {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < R::P; ++j)
+            for (int j = 0; j < X::P; ++j)
 #pragma unroll
                 for (int e = 0; e < N; ++e) cols[g * G * E + N * (l + j * G) + e] = k ? db[j][e] : dw[j][e];
             __syncthreads();
@@ -298,25 +359,26 @@ __global__ void __launch_bounds__(kThreads) ln_columns_long(LnArgs p) {
     if (p.part_b) p.part_b[(int64_t)blockIdx.y * p.W + c] = db;
 }
 
-// Partial rows -> dweight (blockIdx.y 0) and dbias (1): 64 columns a workgroup, sixteen waves over
-// the partials, then the waves in order.
+// Partial rows -> dweight (blockIdx.y 0) and dbias (1): 16 columns a workgroup, 64 threads of each over
+// the partials, then those in order.
 __global__ void __launch_bounds__(1024) ln_sum_kernel(const float *pw, const float *pb, int64_t W,
                                                       int64_t n, float *dw, float *db) {
-    __shared__ float red[16][64];
+    __shared__ float red[64][17];
     const float *part = blockIdx.y ? pb : pw;
     float *out = blockIdx.y ? db : dw;
     if (!out) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int col = threadIdx.x & 15, k0 = threadIdx.x >> 4;
+    const int64_t c = (int64_t)blockIdx.x * 16 + col;
     float s = 0.f;
     if (c < W)
 #pragma unroll 8
-        for (int64_t k = wave; k < n; k += 16) s += part[k * W + c];
-    red[wave][lane] = s;
+        for (int64_t k = k0; k < n; k += 64) s += part[k * W + c];
+    red[k0][col] = s;
     __syncthreads();
-    if (wave == 0 && c < W) {
-        float t = red[0][lane];
-        for (int i = 1; i < 16; ++i) t += red[i][lane];
+    if (threadIdx.x < 16 && c < W) {
+        float t = red[0][col];
+#pragma unroll
+        for (int i = 1; i < 64; ++i) t += red[i][col];
         out[c] = t;
     }
 }
@@ -344,6 +406,8 @@ int check_ln(const gdn2_rows_shape *s, const gdn2_view *x, const float *weight) 
     return GDN2_OK;
 }
 
+bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 // Whether every row is a run of 16-byte pieces.
 bool vec_rows(const gdn2_view *v, int64_t W) {
     const int64_t es = v->dtype == GDN2_BF16 ? 2 : 4;
@@ -353,14 +417,27 @@ bool vec_rows(const gdn2_view *v, int64_t W) {
     return true;
 }
 
+// Rows at once: four (two in the backward) where that leaves eight waves for each of the 256 units.
 template <typename T, int N, int G, int E, bool BWD>
 void launch_one(const LnArgs &a, int64_t partials, hipStream_t st) {
-    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
-    const int64_t groups = (a.rows + ROWS - 1) / ROWS;
-    if constexpr (BWD)
-        hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
-    else
-        hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E>), dim3((unsigned)groups), dim3(THREADS), 0, st, a);
+    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G, R = BWD ? 2 : 4;
+    const auto groups = [&](int r) { return (unsigned)((a.rows + ROWS * r - 1) / (ROWS * r)); };
+    const bool many = G <= 64 && a.rows * G >= (int64_t)R * 2048 * 64;
+    if constexpr (BWD) {
+        if constexpr (G <= 64 && E <= 8)
+            if (many) {
+                hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E, R>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
+                return;
+            }
+        hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E, 1>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
+    } else {
+        if constexpr (G <= 64 && E <= 8)
+            if (many) {
+                hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E, R>), dim3(groups(R)), dim3(THREADS), 0, st, a);
+                return;
+            }
+        hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E, 1>), dim3(groups(1)), dim3(THREADS), 0, st, a);
+    }
 }
 
 // Threads a row by its width, eight columns each while they fit a wave, more beyond.
@@ -413,7 +490,8 @@ int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon, const g
             hipLaunchKernelGGL((ln_forward_long<bf16_t>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
         else hipLaunchKernelGGL((ln_forward_long<float>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
     } else {
-        launch_ln<false>(a, x->dtype, vec_rows(x, a.W) && ((uintptr_t)y & 15) == 0, 0, st);
+        launch_ln<false>(a, x->dtype, vec_rows(x, a.W) && aligned(y) && aligned(weight) && aligned(bias), 0,
+                         st);
     }
     return launch_status(hipGetLastError(), "gdn2_layer_norm_forward");
 }
@@ -465,10 +543,10 @@ int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, c
         }
     } else if (a.rows && (dx || params)) {
         launch_ln<true>(a, x->dtype,
-                        vec_rows(x, a.W) && vec_rows(dy, a.W) && ((uintptr_t)dx & 15) == 0, n, st);
+                        vec_rows(x, a.W) && vec_rows(dy, a.W) && aligned(dx) && aligned(weight), n, st);
     }
     if (params)
-        hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((a.W + 63) / 64), 2), dim3(1024), 0, st,
+        hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((a.W + (int64_t)15) / 16), 2), dim3(1024), 0, st,
                            a.part_w, a.part_b, a.W, a.rows ? n : 0, dweight, dbias);
     return launch_status(hipGetLastError(), "gdn2_layer_norm_backward");
 }

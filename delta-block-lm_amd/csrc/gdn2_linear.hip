@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
     gates();
     __syncthreads();
 
-    const bool masks = p.valid.data || p.T % C || p.ka < KP || wide < kCols;
+    const bool odd = p.valid.data || p.ka < KP || wide < kCols;
     bool fine = S.finite();  // the state is: held at the start of every chunk that is taken by products
     const auto across_c = [&](typename M::Frag (&cf)[C / RB]) {
 #pragma unroll
@@ -537,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
 
     for (; n > out; --n, ci += REV ? -1 : 1) {
         const GateTile<C> &gate = lds.gate[gi];
+        const bool masks = odd || p.T - (int64_t)ci * C < C;
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
         sc.template store<LDC>(lds.c, gate.seg, masks, wide);
         if (n > 1) fetch(REV ? ci - 1 : ci + 1, n - 1 <= out);
@@ -566,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
 
     for (; n > 0; --n, ci += REV ? -1 : 1) {
         const GateTile<C> &gate = lds.gate[gi];
+        const bool masks = odd || p.T - (int64_t)ci * C < C;
         sa.template store<LDA>(lds.a, gate.seg, masks, p.ka);
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
         sc.template store<LDC>(lds.c, gate.seg, masks, wide);

@@ -155,16 +155,14 @@ SIGNATURES = {
     "gdn2_lm_swiglu_forward": (_I, [_L, _L, _P, _P, _P]),
     "gdn2_lm_swiglu_backward": (_I, [_L, _L, _P, _P, _P, _P]),
     "gdn2_linear_checkpoint_bytes": (_Z, [_S, ctypes.c_int32]),
-    "gdn2_linear_scan": (_I, [_S] + [_V] * 7 + [_P, _F, _P, _Z, _P]),
+    # Shapes and views of these go as packed bytes, hence as plain pointers.
+    "gdn2_linear_scan": (_I, [_P] * 8 + [_P, _F, _P, _Z, _P]),
     "gdn2_linear_workspace_bytes": (_Z, [_S, ctypes.c_int32]),
-    "gdn2_linear_backward": (_I, [_S] + [_V] * 7 + [_P, _Z, _V, _F] + [_P] * 3 + [_F] * 3
-                             + [_P, _Z, _P]),
-    "gdn2_linear_step": (_I, [_S] + [_V] * 6 + [_F, _P, _P]),
-    "gdn2_layer_norm_forward": (_I, [ctypes.POINTER(Gdn2RowsShape), ctypes.c_float, _V, _F, _F, _P,
-                                     _F, _F, _P]),
+    "gdn2_linear_backward": (_I, [_P] * 8 + [_P, _Z, _P, _F] + [_P] * 3 + [_F] * 3 + [_P, _Z, _P]),
+    "gdn2_linear_step": (_I, [_P] * 7 + [_F, _P, _P]),
+    "gdn2_layer_norm_forward": (_I, [_P, ctypes.c_float, _P, _F, _F, _P, _F, _F, _P]),
     "gdn2_layer_norm_workspace_bytes": (_Z, [_L, _L]),
-    "gdn2_layer_norm_backward": (_I, [ctypes.POINTER(Gdn2RowsShape), _V, _F, _F, _F, _V, _P, _F, _F,
-                                      _P, _Z, _P]),
+    "gdn2_layer_norm_backward": (_I, [_P, _P, _F, _F, _F, _P, _P, _F, _F, _P, _Z, _P]),
     "gdn2_swiglu_q8_forward": (_I, [_L, _L, ctypes.c_int32] + [_P] * 5),
     "gdn2_swiglu_q8_backward": (_I, [_L, _L, ctypes.c_int32] + [_P] * 6),
     "gdn2_stage_timing": (_I, [_I]),
