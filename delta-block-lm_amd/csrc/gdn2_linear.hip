@@ -10,11 +10,13 @@
 //   dq_t = sum_{s<=t} Gam_ts (do_t.v_s) k_s + gam_t S0 do_t      the forward on  (do, v, k)
 //   dv_s = sum_{t>=s} Gam_ts (k_s.q_t) do_t + lam_s R^T k_s      time reversed on (k, q, do)
 //   dk_s = sum_{t>=s} Gam_ts (v_s.do_t) q_t + lam_s R v_s        time reversed on (v, do, q)
-// so one kernel, linear_walk, computes all four from a triple (a, b, c) and a direction:
-//   out_t = sum_s Gam (a_t.b_s) c_s + row_t (a_t S),   S' = tot S + sum_s col_s b_s c_s^T.
-// The gate's gradient is a sum over the pairs that span a token, dg_t = sum_{u>=t,s<t} W_us with
-// W_us = Gam_us (q_u.k_s)(do_u.v_s), cut at the chunk's bounds (linear_gate).  Nothing is subtracted
-// over more than one segment, so it keeps float32 accuracy for long memories.
+// The forward and dq are one walk over the chunks in order (linear_walk), from a triple (a, b, c):
+//   out_t = sum_s Gam (a_t.b_s) c_s + row_t (a_t S),   S' = tot S + sum_s col_s b_s c_s^T;
+// dv and dk share a walk in the other direction (linear_back), with the pairs' decays and the adjoint
+// state of both.  The gate's gradient is a sum over the pairs that span a token,
+//   dg_t = sum_{u>=t,s<t} W_us,  W_us = Gam_us (q_u.k_s)(do_u.v_s),
+// cut at the chunk's bounds (linear_gate): the walks give its parts.  Nothing is subtracted over more
+// than one segment, so it keeps float32 accuracy for long memories.
 #include <math.h>
 
 #include <algorithm>
@@ -27,8 +29,8 @@ namespace gdn2 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCols = 64;       // columns of c (and of the state) that a workgroup owns
-constexpr int kGates = 8;       // chunks whose gates are made at a time, two by each wave
+constexpr int kGates = 8;       // chunks whose gates are made at a time
+constexpr int kFew = 4;         // sequences of up to so many tokens are taken token by token
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
@@ -96,29 +98,40 @@ __device__ __forceinline__ Split3 split3(const float (&x)[8]) {
     return s;
 }
 
-// One walk over the chunks: see the head of the file.  Tensor views are [B, T, H, channels].
+// The chunks, gates and states of a walk.  Tensor views are [B, T, H, channels].
 struct Walk {
-    View a, b, c, d;        // d: see DOT
     View g, valid, reset;   // valid.data, reset.data may be null
-    View first;             // state before the walk, [B, H, ka, vc] (data may be null: zero)
+    View first;             // state before the walk, [B, H, rows, columns] (data may be null: zero)
     const float *starts;    // states before every segment, or null: taken from first by a prewalk
     int64_t s_bh;
     int s_row, s_col;
     float *starts_out;      // the prewalk's states before every segment, or null
-    float *fin;             // state after the walk, [B H, ka, vc], or null
-    void *out;              // dense [B, T, H, vc], or null
-    float *dots, *dot_sums; // [slices, B H, T], [slices, B H, chunks]: see DOT
-    float *pairs;           // [slices, B H, T]
-    View edge_first;        // with DOT of a reversed walk: the other direction's states, as above
-    const float *edge;
-    float *edges;           // [slices, B H, segments]: <edge, state after the walk's segment>
-    float *totals;          // [B H, chunks]: decay of each chunk, or null
-    float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
-    float *seg_decay;       // [B H, segments]
+    float *fin;             // state after the walk, [B H, rows, columns], or null
+    float *dots, *dot_sums; // [B H, T], [B H, chunks]: see DOT
     int64_t T;
     int H;
+    int chunks, seg_chunks, segments;
+};
+
+// A walk in order: see the head of the file.
+struct Forward : Walk {
+    View a, b, c, d;        // d: see DOT
     int ka, vc;             // widths of a and b, and of c, d and out
-    int chunks, seg_chunks, segments, slices;
+    void *out;              // dense [B, T, H, vc], or null
+    float *pairs;           // [B H, T]: see DOT
+    float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
+    float *seg_decay;       // [B H, segments]
+};
+
+// The walk of dv and dk in the other direction, over the adjoint state [K, V].
+struct Back : Walk {
+    View q, k, v, o;        // o: the output's gradient
+    int K, V;
+    void *dk, *dv;          // dense, or null
+    View edge_first;        // with DOT: the forward's states, its first one
+    const float *edge;      // and those before the other segments
+    float *edges;           // [B H, segments]: <forward state, adjoint> at each segment's start
+    float *totals;          // [B H, chunks]: decay of each chunk
 };
 
 // DPP moves of 64 bits; lanes without a source read 0.
@@ -139,7 +152,7 @@ __device__ __forceinline__ void seg_step(double &G, int seg1) {
 
 // Gates of one chunk, from one wave (lane = token).
 template <int C>
-struct GateTile {
+struct alignas(16) GateTile {
     float hi[C], lo[C];     // sum of g log2(e) in the token's segment: hi + lo, both float32
     float row[C], col[C];   // factor of the start state and of the token's update (0: none of it)
     float step[C];          // exp(g), 0 at a cut, 1 at padding
@@ -195,9 +208,9 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
 // the end and columns past the width read others in their place, and become zero on the way to LDS,
 // as do the rows of padding: what they hold is not used.  VEC: unit channel stride, 16-byte aligned
 // rows, whole pieces, and offsets inside a chunk below 2^31 bytes.
-template <typename T, int W, bool VEC>
+template <typename T, int W, int THREADS, bool VEC>
 struct Staged {
-    static constexpr int N = Mat<T>::N, C = Mat<T>::C, PER = W / N, ROWS = kThreads / PER,
+    static constexpr int N = Mat<T>::N, C = Mat<T>::C, PER = W / N, ROWS = THREADS / PER,
                          PIECES = C / ROWS;
     uint4 r[PIECES];
     // base: row 0 of the (batch, head), column 0 of the tile; width: columns there are from it on
@@ -294,15 +307,27 @@ __device__ __forceinline__ float groups_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-template <typename T, int KP, bool OUT, bool DOT>
+template <typename T, int KP, int CP, bool OUT, bool DOT>
 struct WalkLds {
-    static constexpr int C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = kCols + Mat<T>::PAD,
+    static constexpr int C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = CP + Mat<T>::PAD,
                          LDP = C + Mat<T>::PAD;
     T b[C * LDA], c[C * LDC];
     T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
     GateTile<C> gate[kGates];
-    float red[4][C];
+    float red[CP / 16][C];
     float rows[3][C], cols[3][C], diag[C];  // parts of the pair sums, by tiles of 16 tokens
+};
+
+template <typename T, int KP, int VP>
+struct BackLds {
+    static constexpr int C = Mat<T>::C, LDK = KP + Mat<T>::PAD, LDV = VP + Mat<T>::PAD,
+                         LDP = C + Mat<T>::PAD, NW = (KP > VP ? KP : VP) / 16;
+    T q[C * LDK], k[C * LDK], v[C * LDV], o[C * LDV];
+    T pk[C * LDP], pv[C * LDP];  // Gam k.q and Gam v.do; the token-by-token form keeps float sums in pk
+    T D[VP * LDK];               // the adjoint state transposed, [value][key]
+    GateTile<C> gate[kGates];
+    float red[NW][C];
+    int bad[2];                  // whether any wave's state is not finite, in turn for even and odd chunks
 };
 
 // Holds a loaded value where it is: the compiler otherwise moves each load under the condition that
@@ -406,13 +431,63 @@ __device__ __forceinline__ bool update(State<KP / 16> &U, const State<KP / 16> &
     return U.finite();
 }
 
+// acc[j] += (row t of x) S for the tokens t of tile j: rows = the wave's columns, column = t.  THREE
+// terms of the state give float32 accuracy; with one, the state is rounded to bf16, as the result is.
+template <typename T, int KP, bool THREE>
+__device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const State<KP / 16> &S, const T *x, int ld) {
+    typedef Mat<T> M;
+#pragma unroll
+    for (int r = 0; r < KP / M::RB; ++r) {
+        if constexpr (sizeof(T) == 2) {
+            const f32x4 u = S.t[2 * r], w = S.t[2 * r + 1];
+            const Split3 s3 = split3({u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]});
+            typename M::Frag y[M::C / 16];
+#pragma unroll
+            for (int j = 0; j < M::C / 16; ++j) y[j] = M::order(x + 16 * j * ld, ld, r * M::RB);
+#pragma unroll
+            for (int q = 0; q < (THREE ? 3 : 1); ++q)
+#pragma unroll
+                for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], s3.t[q], y[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], S.t[r], M::order(x + 16 * j * ld, ld, r * M::RB));
+        }
+    }
+}
+
+// The wave's part of a dot product per token: its four columns of d against acc, summed over the groups.
+template <typename T>
+__device__ __forceinline__ void dot_rows(const f32x4 &acc, float f, const T *d, float *red) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x += acc[i] * Elem<T>::load(d, i);
+    x = groups_sum(f == 0.f ? 0.f : x);  // also where the state is not finite
+    if (lane_id() < 16) red[lane_id()] = x;
+}
+
+// A chunk's dot products from the waves' parts, and their sum (one wave).
+template <int C, int NW, int ALL>
+__device__ __forceinline__ void store_dots(const float (&red)[ALL][C], const Walk &p, int64_t bh, int ci) {
+    const int lane = lane_id();
+    const int64_t t = (int64_t)ci * C + lane;
+    float d = 0.f;
+    if (lane < C) {
+        d = red[0][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) d += red[w][lane];
+    }
+    if (lane < C && t < p.T) p.dots[bh * p.T + t] = d;
+    const float sum = wave_sum(d);
+    if (lane == 0) p.dot_sums[bh * p.chunks + ci] = sum;
+}
+
 // A chunk token by token, taken where the state before or after it is not finite: products over masked
 // tokens, and with factors that are 0, would spread such a value to tokens that do not see it.
-template <typename T, int KP, bool REV, bool OUT>
+template <typename T, int KP, int LDC, bool REV, bool OUT>
 __device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const T *b, const T *c,
-                                                      const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
-                                                      T *out, int64_t stride, int tokens) {
-    constexpr int KT = KP / 16, C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = kCols + Mat<T>::PAD;
+                                            const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
+                                            T *out, int64_t stride, int tokens) {
+    constexpr int KT = KP / 16, C = Mat<T>::C, LDA = KP + Mat<T>::PAD;
     const int g4 = 4 * (lane_id() >> 4);
 #pragma unroll 1
     for (int n = 0; n < C; ++n) {
@@ -421,7 +496,7 @@ __device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const
         const float f = gate.step[t];
         float o = 0.f;
         if (gate.seg[t] >= 0) {
-            const float x = Elem<T>::load(c, t * LDC + v % kCols);
+            const float x = Elem<T>::load(c, t * LDC + v);
 #pragma unroll
             for (int m = 0; m < KT; ++m)
 #pragma unroll
@@ -439,98 +514,112 @@ __device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const
     }
 }
 
-// One workgroup: a segment's chunks in the walk's order (REV: from the last to the first), kCols columns
-// of the state.  Each of the four waves owns 16 columns, so its part of the state stays in its
-// accumulators, where the state is at once the product's operand of the next chunk: neither it nor its
-// update passes through LDS.  The next chunk's tiles and gates are on their way while one is worked on.
-// Without `starts` a segment's start state is walked to from the sequence's start (prewalk: b and c alone).
-// OUT = false: only the state that the segment adds and its decay (carry).
-// DOT: dot_t = sum over columns of row_t (a_t S) d_t, and in the forward direction also the pair sums
+// A workgroup's place: segments that share a (batch, head) take neighbouring numbers on one XCD, the
+// longest prewalk first.
+struct Place {
+    int64_t b, h;
+    int bh, seg, nth;  // nth: the segment's place in the walk's order
+};
+__device__ __forceinline__ Place place(const Walk &p, int segs, bool rev, bool longest_first) {
+    const unsigned total = gridDim.x, xcd = blockIdx.x % 8, whole = total / 8, rest = total % 8;
+    const unsigned id = xcd * whole + min(xcd, rest) + blockIdx.x / 8;
+    Place r;
+    r.bh = id / segs;
+    r.nth = longest_first ? segs - 1 - (int)(id % segs) : (int)(id % segs);
+    r.b = r.bh / p.H, r.h = r.bh % p.H;
+    r.seg = rev ? p.segments - 1 - r.nth : r.nth;
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ const T *head_rows(const View &x, const Place &at) {
+    return reinterpret_cast<const T *>(x.data) + at.b * x.s0 + at.h * x.s2;
+}
+
+// The state before a walk's segment: at hand (stored), or the walk's first.
+template <int KT>
+__device__ __forceinline__ void start_state(State<KT> &S, const Walk &p, const Place &at, bool stored, int v,
+                                            int ka, int vc) {
+    const float *src = reinterpret_cast<const float *>(p.first.data);
+    int rs = (int)p.first.s2, cs = (int)p.first.s3;
+    int64_t off = at.b * p.first.s0 + at.h * p.first.s1;
+    if (stored) {
+        src = p.starts, rs = p.s_row, cs = p.s_col;
+        off = at.bh * p.s_bh + at.seg * (int64_t)ka * vc;
+    }
+    if (src) S.load(src + off, rs, cs, v, ka, vc);
+}
+
+// Gates of the next chunks of a walk with n left, from chunk ci on.
+template <int C, bool REV, int NW>
+__device__ __forceinline__ void make_gates(const Walk &p, const Place &at, int ci, int n, GateTile<C> *gate) {
+    for (int i = threadIdx.x >> 6; i < min(n, kGates); i += NW) {
+        const int64_t c = ci + (REV ? -i : i);
+        gate_store<C, REV>(gate_load<C>(p, at.b, at.h, c), (int)min(p.T - c * C, (int64_t)C), &gate[i]);
+    }
+}
+
+// One workgroup: a segment's chunks in the walk's order.  Each wave owns 16 columns of the state, so its
+// part stays in its accumulators, where it is at once the product's operand of the next chunk: neither
+// the state nor its update passes through LDS.  The next chunk's tiles are on their way while one is
+// worked on.  Without `starts` a segment's start state is walked to from the sequence's start (prewalk: b
+// and c alone).  OUT = false: only the state that the segment adds and its decay (carry; REV: from the
+// last chunk to the first).
+// DOT: dot_t = sum over columns of row_t (a_t S) d_t, and the pair sums
 //   pairs_t = sum_{u >= t, s < t, both in the chunk} Gam_us (a_u.b_s)(d_u.c_s),
-// which with (a, b, c, d) = (do, v, k, q) is the part of the gate's gradient inside the chunk; over the
-// slices of c and d it adds up.
-template <typename T, int KP, bool VEC, bool REV, bool OUT, bool DOT>
-__global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
+// which with (a, b, c, d) = (do, v, k, q) is the part of the gate's gradient inside the chunk.
+template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
+__global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward p) {
+    static_assert(!(OUT && REV), "");
     typedef Mat<T> M;
-    typedef WalkLds<T, KP, OUT, DOT> L;
+    typedef WalkLds<T, KP, CP, OUT, DOT> L;
     constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDA = L::LDA, LDC = L::LDC,
                   LDP = L::LDP, BT = RB / 16;  // BT: accumulator tiles of one fragment
-    constexpr bool PAIRS = DOT && !REV;
-    __shared__ __align__(16) L lds;
+    constexpr int NW = CP / 16;
+    __shared__ L lds;
     const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
-
-    // Workgroups that share inputs take neighbouring numbers on one XCD; the longest prewalk first.
-    const unsigned total = gridDim.x, xcd = blockIdx.x % 8, whole = total / 8, rest = total % 8;
-    unsigned id = xcd * whole + min(xcd, rest) + blockIdx.x / 8;
-    const int slice = id % p.slices;
-    id /= p.slices;
+    const int v = 16 * wave + n16;
     const int segs = p.segments - (OUT ? 0 : 1);
-    const int nth = OUT ? segs - 1 - (int)(id % segs) : (int)(id % segs);  // in the walk's order
-    const int bh = id / segs;
-    const int64_t b = bh / p.H, h = bh % p.H, BH = (int64_t)gridDim.x / segs / p.slices;
-    const int seg = REV ? p.segments - 1 - nth : nth;
-    const int col0 = slice * kCols, v = col0 + 16 * wave + n16;
-    const int c_lo = seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
+    const Place at = place(p, segs, REV, OUT);
+    const int c_lo = at.seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
 
     int n = c_hi - c_lo;   // chunks to walk, the last `out` of them with results
     const int out = OUT ? n : 0;
-    const bool walked = OUT && !(nth > 0 && p.starts);  // from the sequence's start
-    if (walked) n = REV ? p.chunks - c_lo : c_hi;
+    const bool walked = OUT && !(at.nth > 0 && p.starts);  // from the sequence's start
+    if (walked) n = c_hi;
     float decay = 1.f;
     int ci = REV ? c_lo + n - 1 : c_hi - n;
 
-    Staged<T, KP, VEC> sa, sb;
-    Staged<T, kCols, VEC> sc, sd;
-    const auto base = [&](const View &x, int c0) {
-        return reinterpret_cast<const T *>(x.data) + b * x.s0 + h * x.s2 + c0 * x.s3;
-    };
-    const T *pa = base(p.a, 0), *pb = base(p.b, 0), *pc = base(p.c, col0), *pd = base(p.d, col0);
-    const int wide = p.vc - col0;  // columns of c and d
+    Staged<T, KP, 64 * NW, VEC> sa, sb;
+    Staged<T, CP, 64 * NW, VEC> sc, sd;
+    const T *pa = head_rows<T>(p.a, at), *pb = head_rows<T>(p.b, at);
+    const T *pc = head_rows<T>(p.c, at), *pd = head_rows<T>(p.d, at);
     const auto fetch = [&](int chunk, bool full) {
         const int64_t t0 = (int64_t)chunk * C;
         const int left = (int)min(p.T - t0, (int64_t)C);
         sb.load(pb, p.b.s1, p.b.s3, t0, left, p.ka);
-        sc.load(pc, p.c.s1, p.c.s3, t0, left, wide);
+        sc.load(pc, p.c.s1, p.c.s3, t0, left, p.vc);
         if (OUT && full) {
             sa.load(pa, p.a.s1, p.a.s3, t0, left, p.ka);
-            if (DOT) sd.load(pd, p.d.s1, p.d.s3, t0, left, wide);
-        }
-    };
-    // The gates of the next kGates chunks of the walk.
-    const auto gates = [&]() {
-        for (int i = wave; i < min(n, kGates); i += 4) {
-            const int64_t at = ci + (REV ? -i : i);
-            gate_store<C, REV>(gate_load<C>(p, b, h, at), (int)min(p.T - at * C, (int64_t)C), &lds.gate[i]);
+            if (DOT) sd.load(pd, p.d.s1, p.d.s3, t0, left, p.vc);
         }
     };
     fetch(ci, n <= out);
     State<KT> S;
     S.zero();
-    if (OUT) {
-        const float *src = reinterpret_cast<const float *>(p.first.data);
-        int rs = (int)p.first.s2, cs = (int)p.first.s3;
-        int64_t at = b * p.first.s0 + h * p.first.s1;
-        if (!walked) {
-            src = p.starts, rs = p.s_row, cs = p.s_col;
-            at = bh * p.s_bh + seg * (int64_t)p.ka * p.vc;
-        }
-        if (src) S.load(src + at, rs, cs, v, p.ka, p.vc);
-    }
+    if (OUT) start_state(S, p, at, !walked, v, p.ka, p.vc);
     int gi = 0;  // the chunk's place among the gates in LDS
-    gates();
+    make_gates<C, REV, NW>(p, at, ci, n, lds.gate);
     __syncthreads();
 
-    const bool odd = p.valid.data || p.ka < KP || wide < kCols;
-    bool fine = S.finite();  // the state is: held at the start of every chunk that is taken by products
+    const bool odd = p.valid.data || p.ka < KP || p.vc < CP;
+    bool fine = S.finite() && p.T > kFew;  // products take a chunk only where the state before it is finite
     const auto across_c = [&](typename M::Frag (&cf)[C / RB]) {
 #pragma unroll
         for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
     };
-
     const auto next_gates = [&]() {
-        --n, ci += REV ? -1 : 1;  // as seen from the next chunk
-        gates();
-        ++n, ci -= REV ? -1 : 1;
+        make_gates<C, REV, NW>(p, at, REV ? ci - 1 : ci + 1, n - 1, lds.gate);
         gi = 0;
         __syncthreads();
     };
@@ -539,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
         const GateTile<C> &gate = lds.gate[gi];
         const bool masks = odd || p.T - (int64_t)ci * C < C;
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
-        sc.template store<LDC>(lds.c, gate.seg, masks, wide);
+        sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
         if (n > 1) fetch(REV ? ci - 1 : ci + 1, n - 1 <= out);
         __syncthreads();
         typename M::Frag cf[C / RB];
@@ -550,159 +639,130 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
         if (__builtin_expect(fine && next, 1)) {
             S = U;
         } else {
-            walk_tokens<T, KP, REV, false>(S, lds.b, lds.b, lds.c, gate, p.ka, v, p.vc, nullptr, 0,
-                                           (int)min(p.T - (int64_t)ci * C, (int64_t)C));
+            walk_tokens<T, KP, LDC, REV, false>(S, lds.b, lds.b, lds.c, gate, p.ka, v, p.vc, nullptr, 0,
+                                                (int)min(p.T - (int64_t)ci * C, (int64_t)C));
             fine = S.finite();
         }
         __syncthreads();  // the chunk's tiles are read
         if (++gi == kGates && n > 1) next_gates();
     }
     if (!OUT) {
-        S.store(p.seg_state + ((int64_t)bh * p.segments + seg) * p.ka * p.vc, v, p.ka, p.vc);
-        if (threadIdx.x == 0 && slice == 0) p.seg_decay[(int64_t)bh * p.segments + seg] = decay;
+        S.store(p.seg_state + ((int64_t)at.bh * p.segments + at.seg) * p.ka * p.vc, v, p.ka, p.vc);
+        if (threadIdx.x == 0) p.seg_decay[(int64_t)at.bh * p.segments + at.seg] = decay;
         return;
     }
-    if (p.starts_out && nth > 0)
-        S.store(p.starts_out + bh * p.s_bh + seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
+    if (p.starts_out && at.nth > 0)
+        S.store(p.starts_out + at.bh * p.s_bh + at.seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
 
-    for (; n > 0; --n, ci += REV ? -1 : 1) {
+    for (; n > 0; --n, ++ci) {
         const GateTile<C> &gate = lds.gate[gi];
         const bool masks = odd || p.T - (int64_t)ci * C < C;
         sa.template store<LDA>(lds.a, gate.seg, masks, p.ka);
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
-        sc.template store<LDC>(lds.c, gate.seg, masks, wide);
-        if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, wide);
-        if (n > 1) fetch(REV ? ci - 1 : ci + 1, true);
+        sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
+        if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, p.vc);
+        if (n > 1) fetch(ci + 1, true);
         __syncthreads();
 
-        f32x4 acc[TT];
-        {
-            // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: three a
-            // wave in bf16, one in float32.
+        // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: twelve in
+        // bf16, three in float32.
 #pragma unroll
-            for (int m = 0; m < (TT == 4 ? 3 : 1); ++m) {
-                int tj = m == 0 ? wave >> 1 : m + 1, si = m == 0 ? wave & 1 : wave;
-                if (TT == 2 && si > tj) continue;  // a block of 16 sources that no row sees
-                if (REV) tj = TT - 1 - tj, si = TT - 1 - si;
-                f32x4 x = zero4();
-#pragma unroll
-                for (int r = 0; r < KP; r += RB)
-                    M::mma(x, M::row(lds.b + 16 * si * LDA, LDA, r), M::row(lds.a + 16 * tj * LDA, LDA, r));
-                const int t = 16 * tj + n16, s = 16 * si + g4;
-                const f32x4 f = pair_decays<C, REV, DOT || sizeof(T) == 4>(gate, t, s);
-                T e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
-                __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
-                if (PAIRS && si <= tj) {
-                    f32x4 y = zero4();
-#pragma unroll
-                    for (int r = 0; r < kCols; r += RB)
-                        M::mma(y, M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        y[i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
-                    if (si < tj) {
-                        const float sum = groups_sum((y[0] + y[1]) + (y[2] + y[3]));
-                        if (lane < 16) lds.rows[si][t] = sum;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float c = row16_sum(y[i]);
-                            if (n16 == i) lds.cols[tj - 1][s + i] = c;
-                        }
-                    } else {
-                        // sums over s before each of the lane's four tokens, over the groups in order
-                        const float q = (y[0] + y[1]) + (y[2] + y[3]);
-                        const float q1 = __shfl_up(q, 16), q2 = __shfl_up(q, 32), q3 = __shfl_up(q, 48);
-                        float pre = (g4 > 0 ? q1 : 0.f) + (g4 > 4 ? q2 : 0.f) + (g4 > 8 ? q3 : 0.f);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float c = row16_sum(n16 >= g4 + i ? pre : 0.f);
-                            if (n16 == i) lds.diag[s + i] = c;
-                            pre += y[i];
-                        }
-                    }
-                }
+        for (int m = 0; m < (TT == 4 ? 12 / NW + (12 % NW > 0) : 1); ++m) {
+            const int id = wave + m * NW;
+            int tj, si;
+            if (TT == 4) {
+                if (12 % NW && id >= 12) continue;
+                tj = id < 4 ? id >> 1 : id < 8 ? 2 : 3, si = id < 4 ? id & 1 : id & 3;
+            } else {
+                tj = id >> 1, si = id & 1;
+                if (id >= 4 || si > tj) continue;  // a block of 16 sources that no row sees
             }
-            // acc[j]: rows = the wave's columns, column = token 16 j + n16; the state's part.
+            f32x4 x = zero4();
 #pragma unroll
-            for (int j = 0; j < TT; ++j) acc[j] = zero4();
+            for (int r = 0; r < KP; r += RB)
+                M::mma(x, M::row(lds.b + 16 * si * LDA, LDA, r), M::row(lds.a + 16 * tj * LDA, LDA, r));
+            const int t = 16 * tj + n16, s = 16 * si + g4;
+            const f32x4 f = pair_decays<C, false, DOT || sizeof(T) == 4>(gate, t, s);
+            T e[4];
 #pragma unroll
-            for (int r = 0; r < KP / RB; ++r) {
-                if constexpr (sizeof(T) == 2) {
-                    const f32x4 u = S.t[2 * r], w = S.t[2 * r + 1];
-                    const Split3 s3 = split3({u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]});
+            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
+            __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
+            if (DOT && si <= tj) {
+                f32x4 y = zero4();
 #pragma unroll
-                    for (int j = 0; j < TT; ++j) {
-                        const typename M::Frag x = M::order(lds.a + 16 * j * LDA, LDA, r * RB);
+                for (int r = 0; r < CP; r += RB)
+                    M::mma(y, M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
 #pragma unroll
-                        for (int q = 0; q < (DOT ? 3 : 1); ++q) M::mma(acc[j], s3.t[q], x);
+                for (int i = 0; i < 4; ++i) y[i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
+                if (si < tj) {
+                    const float sum = groups_sum((y[0] + y[1]) + (y[2] + y[3]));
+                    if (lane < 16) lds.rows[si][t] = sum;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float c = row16_sum(y[i]);
+                        if (n16 == i) lds.cols[tj - 1][s + i] = c;
                     }
                 } else {
+                    // sums over s before each of the lane's four tokens, over the groups in order
+                    const float q = (y[0] + y[1]) + (y[2] + y[3]);
+                    const float q1 = __shfl_up(q, 16), q2 = __shfl_up(q, 32), q3 = __shfl_up(q, 48);
+                    float pre = (g4 > 0 ? q1 : 0.f) + (g4 > 4 ? q2 : 0.f) + (g4 > 8 ? q3 : 0.f);
 #pragma unroll
-                    for (int j = 0; j < TT; ++j)
-                        M::mma(acc[j], S.t[r], M::order(lds.a + 16 * j * LDA, LDA, r * RB));
+                    for (int i = 0; i < 4; ++i) {
+                        const float c = row16_sum(n16 >= g4 + i ? pre : 0.f);
+                        if (n16 == i) lds.diag[s + i] = c;
+                        pre += y[i];
+                    }
                 }
             }
+        }
+        // acc[j]: rows = the wave's columns, column = token 16 j + n16; the state's part.
+        f32x4 acc[TT];
 #pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                const float f = gate.row[16 * j + n16];
+        for (int j = 0; j < TT; ++j) acc[j] = zero4();
+        state_rows<T, KP, DOT>(acc, S, lds.a, LDA);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] *= f;
-                if (DOT) {
-                    const T *d = lds.d + (16 * j + n16) * LDC + 16 * wave + g4;
-                    float x = 0.f;
+        for (int j = 0; j < TT; ++j) {
+            const float f = gate.row[16 * j + n16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x += acc[j][i] * Elem<T>::load(d, i);
-                    x = groups_sum(f == 0.f ? 0.f : x);  // also where the state is not finite
-                    if (lane < 16) lds.red[wave][16 * j + n16] = x;
-                }
+            for (int i = 0; i < 4; ++i) acc[j][i] *= f;
+            if (DOT) dot_rows<T>(acc[j], f, lds.d + (16 * j + n16) * LDC + 16 * wave + g4, &lds.red[wave][16 * j]);
+        }
+        __syncthreads();
+        if (DOT && wave == 1) store_dots<C, NW>(lds.red, p, at.bh, ci);
+        if (DOT && wave == 2) {
+            // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t of the
+            // tile over the tiles below, whole tiles below and to the left, and its own tile.
+            const int64_t t = (int64_t)ci * C + lane;
+            const int j = lane / 16;
+            float left = 0.f, below = 0.f, x = 0.f, r0 = 0.f, r1 = 0.f;
+            if (lane < C) {
+                if (j > 0) left = r0 = lds.rows[0][lane];
+                if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
+                if (TT == 4 && j > 2) left += lds.rows[2][lane];
+                if (j < 1) below += lds.cols[0][lane];
+                if (TT == 4 && j < 2) below += lds.cols[1][lane];
+                if (TT == 4 && j < 3) below += lds.cols[2][lane];
+                x = lds.diag[lane];
             }
-            __syncthreads();
-            if (DOT && wave == 1) {
-                const int64_t t = (int64_t)ci * C + lane, at = (int64_t)slice * BH + bh;
-                float d = 0.f;
-                if (lane < C) d = (lds.red[0][lane] + lds.red[1][lane]) + (lds.red[2][lane] + lds.red[3][lane]);
-                if (lane < C && t < p.T) p.dots[at * p.T + t] = d;
-                const float sum = wave_sum(d);
-                if (lane == 0) p.dot_sums[at * p.chunks + ci] = sum;
+            if (TT == 4) {
+                const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
+                const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
+                x += j == 1 ? f1 : j == 2 ? f2 : 0.f;
             }
-            if (PAIRS && wave == 2) {
-                // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t
-                // of the tile over the tiles below, whole tiles below and to the left, and its own tile.
-                const int64_t t = (int64_t)ci * C + lane;
-                const int j = lane / 16;
-                float left = 0.f, below = 0.f, x = 0.f;
-                float r0 = 0.f, r1 = 0.f;
-                if (lane < C) {
-                    if (j > 0) left = r0 = lds.rows[0][lane];
-                    if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
-                    if (TT == 4 && j > 2) left += lds.rows[2][lane];
-                    if (TT > 1 && j < 1) below += lds.cols[0][lane];
-                    if (TT == 4 && j < 2) below += lds.cols[1][lane];
-                    if (TT == 4 && j < 3) below += lds.cols[2][lane];
-                    x = lds.diag[lane];
-                }
-                if (TT == 4) {
-                    const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
-                    const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
-                    x += j == 1 ? f1 : j == 2 ? f2 : 0.f;
-                }
 #pragma unroll
-                for (int d = 1; d < 16; d *= 2) {
-                    const float y = __shfl_down(left, d);
-                    if (n16 + d < 16) left += y;
-                }
-                float pre = __shfl_up(below, 1);
-                if (n16 == 0) pre = 0.f;
-#pragma unroll
-                for (int d = 1; d < 16; d *= 2) {
-                    const float y = __shfl_up(pre, d);
-                    if (n16 >= d) pre += y;
-                }
-                if (lane < C && t < p.T) p.pairs[((int64_t)slice * BH + bh) * p.T + t] = (left + pre) + x;
+            for (int d = 1; d < 16; d *= 2) {
+                const float y = __shfl_down(left, d);
+                if (n16 + d < 16) left += y;
             }
-            if (p.totals && slice == 0 && threadIdx.x == 0) p.totals[(int64_t)bh * p.chunks + ci] = gate.tot;
+            float pre = __shfl_up(below, 1);
+            if (n16 == 0) pre = 0.f;
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) {
+                const float y = __shfl_up(pre, d);
+                if (n16 >= d) pre += y;
+            }
+            if (lane < C && t < p.T) p.pairs[(int64_t)at.bh * p.T + t] = (left + pre) + x;
         }
 
         typename M::Frag cf[C / RB];
@@ -710,53 +770,297 @@ __global__ void __launch_bounds__(kThreads, 2) linear_walk(Walk p) {
         State<KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
         T *o = reinterpret_cast<T *>(p.out);
-        const int64_t row0 = (b * p.T + (int64_t)ci * C) * p.H + h;
+        const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
+        const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
         if (__builtin_expect(fine && next, 1)) {
             if (o) {
-                const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
 #pragma unroll
                 for (int j = 0; j < TT; ++j) {
 #pragma unroll
-                    for (int r = 0; r < C / RB; ++r)
-                        if (REV ? r >= j / BT : r <= j / BT)
-                            M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
+                    for (int r = 0; r <= j / BT; ++r)
+                        M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
                     const int t = 16 * j + n16;
                     if (t < left)
-                        store4<T, VEC>(o, row0 + (int64_t)t * p.H, col0 + 16 * wave + g4, p.vc, acc[j]);
+                        store4<T, VEC>(o, row0 + (int64_t)t * p.H, 16 * wave + g4, p.vc, acc[j]);
                 }
             }
             S = U;
         } else {
-            T *at = o ? o + row0 * p.vc : nullptr;
-            walk_tokens<T, KP, REV, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc, at, (int64_t)p.H * p.vc,
-                                         (int)min(p.T - (int64_t)ci * C, (int64_t)C));
+            walk_tokens<T, KP, LDC, false, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc,
+                                                 o ? o + row0 * p.vc : nullptr, (int64_t)p.H * p.vc, left);
+            fine = S.finite();
+        }
+        __syncthreads();  // the chunk's tiles are read
+        if (++gi == kGates && n > 1) next_gates();
+    }
+    if (p.fin && at.nth == p.segments - 1) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
+}
+
+// dv and dk, from the last chunk to the first.  A wave owns 16 value columns of the adjoint state [K, V]
+// and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once
+// a chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for
+// dk read three of the four tensors again, and took its pairs' decays and the state's update a second
+// time.)  DOT: dot_s = row_s k_s^T S v_s, and the products with the forward's states at segment starts.
+template <typename T, int KP, int VP, bool VEC, bool DOT>
+__global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
+    typedef Mat<T> M;
+    typedef BackLds<T, KP, VP> L;
+    constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDK = L::LDK, LDV = L::LDV,
+                  LDP = L::LDP, BT = RB / 16, NW = L::NW, THREADS = 64 * NW;
+    __shared__ L lds;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int v = 16 * wave + n16;
+    const bool own_v = 16 * wave < VP, own_k = 16 * wave < KP;
+    const Place at = place(p, p.segments, true, true);
+    const int c_lo = at.seg * p.seg_chunks, c_hi = min(p.chunks, c_lo + p.seg_chunks);
+    int n = c_hi - c_lo;
+    const int out = n;
+    const bool walked = !(at.nth > 0 && p.starts);
+    if (walked) n = p.chunks - c_lo;
+    int ci = c_lo + n - 1;
+
+    Staged<T, KP, THREADS, VEC> sq, sk;
+    Staged<T, VP, THREADS, VEC> sv, so;
+    const T *pq = head_rows<T>(p.q, at), *pk = head_rows<T>(p.k, at);
+    const T *pv = head_rows<T>(p.v, at), *po = head_rows<T>(p.o, at);
+    const auto fetch = [&](int chunk, bool full) {
+        const int64_t t0 = (int64_t)chunk * C;
+        const int left = (int)min(p.T - t0, (int64_t)C);
+        sq.load(pq, p.q.s1, p.q.s3, t0, left, p.K);
+        so.load(po, p.o.s1, p.o.s3, t0, left, p.V);
+        if (full) {
+            sk.load(pk, p.k.s1, p.k.s3, t0, left, p.K);
+            sv.load(pv, p.v.s1, p.v.s3, t0, left, p.V);
+        }
+    };
+    fetch(ci, n <= out);
+    State<KT> S;
+    S.zero();
+    if (own_v) start_state(S, p, at, !walked, v, p.K, p.V);
+    int gi = 0;
+    make_gates<C, true, NW>(p, at, ci, n, lds.gate);
+    if (threadIdx.x < 2) lds.bad[threadIdx.x] = 0;
+    __syncthreads();
+
+    const bool odd = p.valid.data || p.K < KP || p.V < VP;
+    bool fine = S.finite() && p.T > kFew;
+    const auto across_o = [&](typename M::Frag (&of)[C / RB]) {
+#pragma unroll
+        for (int r = 0; r < C / RB; ++r) of[r] = M::template across<LDV>(lds.o, r * RB, 16 * wave);
+    };
+    const auto next_gates = [&]() {
+        make_gates<C, true, NW>(p, at, ci - 1, n - 1, lds.gate);
+        gi = 0;
+        __syncthreads();
+    };
+
+    for (; n > out; --n, --ci) {
+        const GateTile<C> &gate = lds.gate[gi];
+        const bool masks = odd || p.T - (int64_t)ci * C < C;
+        sq.template store<LDK>(lds.q, gate.seg, masks, p.K);
+        so.template store<LDV>(lds.o, gate.seg, masks, p.V);
+        fetch(ci - 1, n - 1 <= out);
+        __syncthreads();
+        if (own_v) {
+            typename M::Frag of[C / RB];
+            across_o(of);
+            State<KT> U;
+            const bool next = update<T, KP>(U, S, gate.tot, of, lds.q, gate.col);
+            if (__builtin_expect(fine && next, 1)) {
+                S = U;
+            } else {
+                walk_tokens<T, KP, LDV, true, false>(S, lds.q, lds.q, lds.o, gate, p.K, v, p.V, nullptr, 0,
+                                                     (int)min(p.T - (int64_t)ci * C, (int64_t)C));
+                fine = S.finite();
+            }
+        }
+        __syncthreads();
+        if (++gi == kGates) next_gates();
+    }
+
+    for (; n > 0; --n, --ci) {
+        const GateTile<C> &gate = lds.gate[gi];
+        const bool masks = odd || p.T - (int64_t)ci * C < C;
+        sq.template store<LDK>(lds.q, gate.seg, masks, p.K);
+        sk.template store<LDK>(lds.k, gate.seg, masks, p.K);
+        sv.template store<LDV>(lds.v, gate.seg, masks, p.V);
+        so.template store<LDV>(lds.o, gate.seg, masks, p.V);
+        if (own_v) {
+#pragma unroll
+            for (int m = 0; m < KT; ++m) {
+                T e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, S.t[m][i]);
+                __builtin_memcpy(__builtin_assume_aligned(lds.D + v * LDK + 16 * m + g4, 4 * sizeof(T)), e, sizeof e);
+            }
+        }
+        if (n > 1) fetch(ci - 1, true);
+        __syncthreads();
+
+        // For out token s and source t >= s: pk = Gam k_s.q_t, pv = Gam v_s.do_t, by tiles as in linear_walk
+        // but from the other end.
+#pragma unroll
+        for (int m = 0; m < (TT == 4 ? 12 / NW + (12 % NW > 0) : 1); ++m) {
+            const int id = wave + m * NW;
+            int sj, ti;
+            if (TT == 4) {
+                if (12 % NW && id >= 12) continue;
+                sj = id < 4 ? id >> 1 : id < 8 ? 2 : 3, ti = id < 4 ? id & 1 : id & 3;
+            } else {
+                sj = id >> 1, ti = id & 1;
+                if (id >= 4 || ti > sj) continue;
+            }
+            sj = TT - 1 - sj, ti = TT - 1 - ti;
+            f32x4 x = zero4(), y = zero4();
+#pragma unroll
+            for (int r = 0; r < KP; r += RB)
+                M::mma(x, M::row(lds.q + 16 * ti * LDK, LDK, r), M::row(lds.k + 16 * sj * LDK, LDK, r));
+#pragma unroll
+            for (int r = 0; r < VP; r += RB)
+                M::mma(y, M::row(lds.o + 16 * ti * LDV, LDV, r), M::row(lds.v + 16 * sj * LDV, LDV, r));
+            const int s = 16 * sj + n16, t = 16 * ti + g4;
+            const f32x4 f = pair_decays<C, true, sizeof(T) == 4>(gate, s, t);
+            T e[4], g[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] * f[i]), Elem<T>::store(g, i, y[i] * f[i]);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pk + s * LDP + t, 4 * sizeof(T)), e, sizeof e);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pv + s * LDP + t, 4 * sizeof(T)), g, sizeof g);
+        }
+        // The state's parts: rows = the wave's columns, column = token 16 j + n16.
+        f32x4 av[TT], ak[TT];
+#pragma unroll
+        for (int j = 0; j < TT; ++j) av[j] = ak[j] = zero4();
+        State<KT> U;
+        U.zero();
+        typename M::Frag of[C / RB];
+        bool good = fine;
+        if (own_v) {
+            state_rows<T, KP, DOT>(av, S, lds.k, LDK);
+            across_o(of);
+            good = update<T, KP>(U, S, gate.tot, of, lds.q, gate.col) && fine;
+        }
+        if (own_k) {
+#pragma unroll
+            for (int r = 0; r < VP; r += RB) {
+                const typename M::Frag x = M::template across<LDK>(lds.D, r, 16 * wave);
+#pragma unroll
+                for (int j = 0; j < TT; ++j) M::mma(ak[j], x, M::row(lds.v + 16 * j * LDV, LDV, r));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+            const float f = gate.row[16 * j + n16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) av[j][i] *= f, ak[j][i] *= f;
+            if (DOT && own_v)
+                dot_rows<T>(av[j], f, lds.v + (16 * j + n16) * LDV + 16 * wave + g4, &lds.red[wave][16 * j]);
+        }
+        if (!good && lane == 0) lds.bad[n & 1] = 1;
+        __syncthreads();
+        const bool bad = lds.bad[n & 1] != 0;
+        if (threadIdx.x == 0) lds.bad[(n & 1) ^ 1] = 0;
+        if (DOT && wave == 1) store_dots<C, VP / 16>(lds.red, p, at.bh, ci);
+        if (DOT && threadIdx.x == 0) p.totals[(int64_t)at.bh * p.chunks + ci] = gate.tot;
+        const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
+        const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
+        T *dv = reinterpret_cast<T *>(p.dv), *dk = reinterpret_cast<T *>(p.dk);
+        if (__builtin_expect(!bad, 1)) {
+            if (dv && own_v) {
+#pragma unroll
+                for (int j = 0; j < TT; ++j) {
+#pragma unroll
+                    for (int r = j / BT; r < C / RB; ++r)
+                        M::mma(av[j], of[r], M::row(lds.pk + 16 * j * LDP, LDP, r * RB));
+                    const int t = 16 * j + n16;
+                    if (t < left) store4<T, VEC>(dv, row0 + (int64_t)t * p.H, 16 * wave + g4, p.V, av[j]);
+                }
+            }
+            if (dk && own_k) {
+                typename M::Frag qf[C / RB];
+#pragma unroll
+                for (int r = 0; r < C / RB; ++r) qf[r] = M::template across<LDK>(lds.q, r * RB, 16 * wave);
+#pragma unroll
+                for (int j = 0; j < TT; ++j) {
+#pragma unroll
+                    for (int r = j / BT; r < C / RB; ++r)
+                        M::mma(ak[j], qf[r], M::row(lds.pv + 16 * j * LDP, LDP, r * RB));
+                    const int t = 16 * j + n16;
+                    if (t < left) store4<T, VEC>(dk, row0 + (int64_t)t * p.H, 16 * wave + g4, p.K, ak[j]);
+                }
+            }
+            S = U;
+        } else {
+            // Token by token, all waves together: see walk_tokens.
+            float *part = reinterpret_cast<float *>(lds.pk);  // [NW][KP]: dk's sums over a wave's columns
+            static_assert(sizeof(lds.pk) >= sizeof(float) * NW * KP, "");
+#pragma unroll 1
+            for (int t = left - 1; t >= 0; --t) {
+                const bool on = gate.seg[t] >= 0;
+                const float f = gate.step[t];
+                float o = 0.f;
+                __syncthreads();  // the last token's sums are read
+                if (on && own_v) {
+                    const float x = Elem<T>::load(lds.o, t * LDV + v);
+                    const float y = v < p.V ? Elem<T>::load(lds.v, t * LDV + v) : 0.f;
+#pragma unroll
+                    for (int m = 0; m < KT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = 16 * m + g4 + i;
+                            if (k < p.K) {
+                                S.t[m][i] += Elem<T>::load(lds.q, t * LDK + k) * x;
+                                o += Elem<T>::load(lds.k, t * LDK + k) * S.t[m][i];
+                            }
+                            const float d = row16_sum(v < p.V ? S.t[m][i] * y : 0.f);
+                            if (n16 == 0) part[wave * KP + k] = d;
+                            if (k < p.K) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
+                        }
+                    o = groups_sum(o);
+                }
+                __syncthreads();
+                const int64_t row = row0 + (int64_t)t * p.H;
+                if (dv && own_v && lane < 16 && v < p.V) Elem<T>::store(dv, row * p.V + v, o);
+                if (dk && (int)threadIdx.x < p.K) {
+                    float d = 0.f;
+                    if (on)
+                        for (int w = 0; w < VP / 16; ++w) d += part[w * KP + threadIdx.x];
+                    Elem<T>::store(dk, row * p.K + threadIdx.x, d);
+                }
+            }
             fine = S.finite();
         }
         __syncthreads();  // the chunk's tiles are read
         if (++gi == kGates && n > 1) next_gates();
     }
 
-    if (p.fin && nth == p.segments - 1) S.store(p.fin + (int64_t)bh * p.ka * p.vc, v, p.ka, p.vc);
-    if (DOT && REV) {
-        // seg > 0 has the other direction's start state at hand, the first segment its initial state.
-        State<KT> e;
-        e.zero();
-        if (seg > 0)
-            e.load(p.edge + ((int64_t)bh * p.segments + seg) * p.ka * p.vc, p.vc, 1, v, p.ka, p.vc);
-        else if (p.edge_first.data)
-            e.load(reinterpret_cast<const float *>(p.edge_first.data) + b * p.edge_first.s0 + h * p.edge_first.s1,
-                   (int)p.edge_first.s2, (int)p.edge_first.s3, v, p.ka, p.vc);
+    if (p.fin && own_v && at.seg == 0) S.store(p.fin + (int64_t)at.bh * p.K * p.V, v, p.K, p.V);
+    if (DOT) {
         float d = 0.f;
+        if (own_v) {
+            const float *src = reinterpret_cast<const float *>(p.edge_first.data);
+            int rs = (int)p.edge_first.s2, cs = (int)p.edge_first.s3;
+            int64_t off = at.b * p.edge_first.s0 + at.h * p.edge_first.s1;
+            if (at.seg > 0) {
+                src = p.edge, rs = p.V, cs = 1;
+                off = ((int64_t)at.bh * p.segments + at.seg) * p.K * p.V;
+            }
+            if (src) {
+                State<KT> e;
+                e.load(src + off, rs, cs, v, p.K, p.V);
 #pragma unroll
-        for (int m = 0; m < KT; ++m)
+                for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
-        d = wave_sum(v < p.vc ? d : 0.f);
-        if (lane == 0) lds.red[wave][0] = d;
+                    for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
+                d = wave_sum(v < p.V ? d : 0.f);
+            }
+            if (lane == 0) lds.red[wave][0] = d;
+        }
         __syncthreads();
-        if (threadIdx.x == 0)
-            p.edges[((int64_t)slice * BH + bh) * p.segments + seg] =
-                (lds.red[0][0] + lds.red[1][0]) + (lds.red[2][0] + lds.red[3][0]);
+        if (threadIdx.x == 0) {
+            d = lds.red[0][0];
+            for (int w = 1; w < VP / 16; ++w) d += lds.red[w][0];
+            p.edges[(int64_t)at.bh * p.segments + at.seg] = d;
+        }
     }
 }
 
@@ -796,7 +1100,6 @@ struct GateGradArgs {
     const float *x_sums, *y_sums; // per chunk
     const float *edges, *totals;
     int64_t BH;
-    int x_slices, y_slices;
     float *dg;                    // dense [B, T, H]
 };
 
@@ -817,11 +1120,9 @@ __global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
     const bool val = in && gi.valid != 0.f && gi.reset == 0.f && !(gi.g < kCut);
     float dg = 0.f, x = 0.f, y = 0.f;
     if (in) {
-        for (int s = 0; s < p.x_slices; ++s) {
-            x += p.x[(s * p.BH + bh) * p.w.T + t];
-            dg += p.pairs[(s * p.BH + bh) * p.w.T + t];
-        }
-        for (int s = 0; s < p.y_slices; ++s) y += p.y[(s * p.BH + bh) * p.w.T + t];
+        x = p.x[bh * p.w.T + t];
+        y = p.y[bh * p.w.T + t];
+        dg = p.pairs[bh * p.w.T + t];
     }
     // sum of x over u >= t, and of y over s < t: scans that add only what belongs to them
     float sx = x, sy = __shfl_up(y, 1);
@@ -842,15 +1143,9 @@ __global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
             const unsigned long long m = __ballot(c < ci && p.totals[bh * p.w.chunks + min(c, ci)] == 0.f);
             if (m) from = c0 + 63 - __clzll(m), cut = true;
         }
-        for (int c = from + lane; c < ci; c += 64) {
-            float d = 0.f;
-            for (int s = 0; s < p.y_slices; ++s) d += p.y_sums[(s * p.BH + bh) * p.w.chunks + c];
-            if (!(cut && c == from))
-                for (int s = 0; s < p.x_slices; ++s) d -= p.x_sums[(s * p.BH + bh) * p.w.chunks + c];
-            E += d;
-        }
-        if (lane == 0 && !cut)
-            for (int s = 0; s < p.y_slices; ++s) E += p.edges[(s * p.BH + bh) * p.w.segments + seg];
+        for (int c = from + lane; c < ci; c += 64)
+            E += p.y_sums[bh * p.w.chunks + c] - (cut && c == from ? 0.f : p.x_sums[bh * p.w.chunks + c]);
+        if (lane == 0 && !cut) E += p.edges[bh * p.w.segments + seg];
         E = wave_sum(E);
         E -= wave_sum(x);
     }
@@ -963,7 +1258,6 @@ __global__ void __launch_bounds__(kThreads) linear_step(StepArgs p) {
 struct Plan {
     int C, chunks, seg_chunks, segments;
     int64_t BH, KV;
-    int kslices, vslices;
     bool prewalk;  // start states are walked to, instead of carried by a launch of their own
 };
 
@@ -977,10 +1271,9 @@ Plan plan(const gdn2_shape *s, int dtype) {
     p.chunks = (int)((s->time + p.C - 1) / p.C);
     p.BH = s->batch * s->heads;
     p.KV = s->keys * s->values;
-    p.kslices = (int)((s->keys + kCols - 1) / kCols);
-    p.vslices = (int)((s->values + kCols - 1) / kCols);
-    // Segments of at least two chunks, as many as fill the card.
-    int64_t want = kWantGroups / std::max<int64_t>(1, p.BH * p.vslices);
+    // Segments of at least two chunks, as many as fill the card, and of at most 16 (the gate's gradient adds
+    // up what happens in a segment).
+    int64_t want = std::max<int64_t>(kWantGroups / p.BH, (p.chunks + 15) / 16);
     want = std::max<int64_t>(1, std::min<int64_t>(want, p.chunks / 2));
     p.seg_chunks = (int)((p.chunks + want - 1) / want);
     p.segments = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
@@ -1010,12 +1303,12 @@ Layout workspace_layout(const Plan &p, int64_t T) {
     };
     l.state = take(p.segments > 1 && !p.prewalk ? p.BH * p.segments * p.KV : 0);
     l.decay = take(p.BH * p.segments);
-    l.x = take(p.kslices * p.BH * T);
-    l.y = take(p.vslices * p.BH * T);
-    l.pairs = take(p.kslices * p.BH * T);
-    l.x_sums = take((int64_t)p.kslices * p.BH * p.chunks);
-    l.y_sums = take((int64_t)p.vslices * p.BH * p.chunks);
-    l.edges = take((int64_t)p.vslices * p.BH * p.segments);
+    l.x = take(p.BH * T);
+    l.y = take(p.BH * T);
+    l.pairs = take(p.BH * T);
+    l.x_sums = take(p.BH * p.chunks);
+    l.y_sums = take(p.BH * p.chunks);
+    l.edges = take(p.BH * p.segments);
     l.totals = take(p.BH * p.chunks);
     l.dg = take(p.BH * T);
     l.bytes = n;
@@ -1030,7 +1323,7 @@ int check_linear(const gdn2_shape *s, int dtype) {
         return fail(GDN2_ERR_SHAPE, "key and value widths must be 1..128");
     if (dtype != GDN2_F32 && dtype != GDN2_BF16)
         return fail(GDN2_ERR_DTYPE, "dtype must be F32 or BF16");
-    // A launch has at most 2^24 workgroups of 256 threads: two for a segment of 32 or 64 tokens.
+    // A launch has below 2^32 threads: at most 512 for a chunk of 32 or 64 tokens.
     const int64_t lim = (int64_t)1 << 21;
     if (s->batch > lim || s->heads > lim || s->batch * s->heads > lim || s->time > 32 * lim ||
         (s->time + 31) / 32 > lim / (s->batch * s->heads))
@@ -1059,9 +1352,10 @@ int check_inputs(const gdn2_shape *s, const gdn2_view *q, const gdn2_view *k, co
     return GDN2_OK;
 }
 
-Walk base_walk(const gdn2_shape *s, const Plan &p, const gdn2_view *g, const gdn2_view *valid,
+template <typename W>
+W base_walk(const gdn2_shape *s, const Plan &p, const gdn2_view *g, const gdn2_view *valid,
                const gdn2_view *reset) {
-    Walk w{};
+    W w{};
     w.T = s->time;
     w.H = (int)s->heads;
     w.g = make_view(g);
@@ -1075,34 +1369,61 @@ Walk base_walk(const gdn2_shape *s, const Plan &p, const gdn2_view *g, const gdn
 
 View transposed(const View &x) { return View{x.data, x.s0, x.s1, x.s3, x.s2}; }
 
-void set_triple(Walk *w, const gdn2_view *a, const gdn2_view *b, const gdn2_view *c, int64_t ka, int64_t vc) {
+void set_triple(Forward *w, const gdn2_view *a, const gdn2_view *b, const gdn2_view *c, int64_t ka, int64_t vc) {
     w->a = make_view(a), w->b = make_view(b), w->c = make_view(c);
     w->ka = (int)ka;
     w->vc = (int)vc;
-    w->slices = (int)((vc + kCols - 1) / kCols);
 }
 
-template <typename T, bool VEC, bool REV, bool OUT, bool DOT>
-void launch_walk(const Walk &w, const dim3 &grid, hipStream_t st) {
-    const dim3 block(kThreads);
-    if (w.ka <= 64) hipLaunchKernelGGL((linear_walk<T, 64, VEC, REV, OUT, DOT>), grid, block, 0, st, w);
-    else hipLaunchKernelGGL((linear_walk<T, 128, VEC, REV, OUT, DOT>), grid, block, 0, st, w);
+template <typename T, int KP, int CP, bool REV, bool OUT, bool DOT>
+void launch_walk(const Forward &w, bool vec, unsigned grid, hipStream_t st) {
+    const dim3 block(4 * CP);
+    if (vec) hipLaunchKernelGGL((linear_walk<T, KP, CP, true, REV, OUT, DOT>), dim3(grid), block, 0, st, w);
+    else hipLaunchKernelGGL((linear_walk<T, KP, CP, false, REV, OUT, DOT>), dim3(grid), block, 0, st, w);
+}
+
+template <typename T, bool REV, bool OUT, bool DOT>
+void size_walk(const Forward &w, bool vec, unsigned grid, hipStream_t st) {
+    if (w.ka <= 64 && w.vc <= 64) launch_walk<T, 64, 64, REV, OUT, DOT>(w, vec, grid, st);
+    else if (w.ka <= 64) launch_walk<T, 64, 128, REV, OUT, DOT>(w, vec, grid, st);
+    else if (w.vc <= 64) launch_walk<T, 128, 64, REV, OUT, DOT>(w, vec, grid, st);
+    else launch_walk<T, 128, 128, REV, OUT, DOT>(w, vec, grid, st);
 }
 
 template <bool REV, bool OUT, bool DOT>
-hipError_t run_walk(const Walk &w, const Plan &p, int dtype, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)(p.BH * (p.segments - (OUT ? 0 : 1)) * w.slices));
-    const bool bf = dtype == GDN2_BF16;
-    if (bf && vec) launch_walk<bf16_t, true, REV, OUT, DOT>(w, grid, st);
-    else if (bf) launch_walk<bf16_t, false, REV, OUT, DOT>(w, grid, st);
-    else if (vec) launch_walk<float, true, REV, OUT, DOT>(w, grid, st);
-    else launch_walk<float, false, REV, OUT, DOT>(w, grid, st);
+hipError_t run_walk(const Forward &w, const Plan &p, int dtype, bool vec, hipStream_t st) {
+    const unsigned grid = (unsigned)(p.BH * (p.segments - (OUT ? 0 : 1)));
+    if (dtype == GDN2_BF16) size_walk<bf16_t, REV, OUT, DOT>(w, vec, grid, st);
+    else size_walk<float, REV, OUT, DOT>(w, vec, grid, st);
+    return hipGetLastError();
+}
+
+template <typename T, int KP, int VP, bool DOT>
+void launch_back(const Back &w, bool vec, unsigned grid, hipStream_t st) {
+    const dim3 block(4 * std::max(KP, VP));
+    if (vec) hipLaunchKernelGGL((linear_back<T, KP, VP, true, DOT>), dim3(grid), block, 0, st, w);
+    else hipLaunchKernelGGL((linear_back<T, KP, VP, false, DOT>), dim3(grid), block, 0, st, w);
+}
+
+template <typename T, bool DOT>
+void size_back(const Back &w, bool vec, unsigned grid, hipStream_t st) {
+    if (w.K <= 64 && w.V <= 64) launch_back<T, 64, 64, DOT>(w, vec, grid, st);
+    else if (w.K <= 64) launch_back<T, 64, 128, DOT>(w, vec, grid, st);
+    else if (w.V <= 64) launch_back<T, 128, 64, DOT>(w, vec, grid, st);
+    else launch_back<T, 128, 128, DOT>(w, vec, grid, st);
+}
+
+template <bool DOT>
+hipError_t run_back(const Back &w, const Plan &p, int dtype, bool vec, hipStream_t st) {
+    const unsigned grid = (unsigned)(p.BH * p.segments);
+    if (dtype == GDN2_BF16) size_back<bf16_t, DOT>(w, vec, grid, st);
+    else size_back<float, DOT>(w, vec, grid, st);
     return hipGetLastError();
 }
 
 // Start states of every segment of a walk over (b, c) into `state`, from `first`.
 template <bool REV>
-hipError_t run_carry(Walk w, const Plan &p, const gdn2_view *b, const gdn2_view *c, int64_t K, int64_t V,
+hipError_t run_carry(Forward w, const Plan &p, const gdn2_view *b, const gdn2_view *c, int64_t K, int64_t V,
                      const View &first, float *state, float *decay, int dtype, bool vec, hipStream_t st) {
     set_triple(&w, nullptr, b, c, K, V);
     w.seg_state = state;
@@ -1158,7 +1479,7 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
     const int64_t K = shape->keys, V = shape->values;
     const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V);
     hipStream_t st = (hipStream_t)stream;
-    Walk w = base_walk(shape, p, g, valid, reset);
+    Forward w = base_walk<Forward>(shape, p, g, valid, reset);
     const View first = make_view(initial);
     float *state = (float *)checkpoint, *decay = (float *)((char *)checkpoint + l.decay);
     if (p.segments > 1 && !p.prewalk) {
@@ -1200,48 +1521,39 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     const bool gates = dg || dg_heads;
     const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V) && vec_rows(d_output, V);
     hipStream_t st = (hipStream_t)stream;
-    const Walk base = base_walk(shape, p, g, valid, reset);
+    const Forward base = base_walk<Forward>(shape, p, g, valid, reset);
     const auto at = [&](size_t off) { return (float *)((char *)workspace + off); };
     const float *states = (const float *)checkpoint;  // [B H, segments, K, V]
     const View first = make_view(initial), d_final{d_final_state, shape->heads * p.KV, p.KV, V, 1};
     const bool many = p.segments > 1;
-    float *adj = nullptr;
     hipError_t e = hipSuccess;
-    if (many && !p.prewalk) {
-        adj = at(l.state);
-        e = run_carry<true>(base, p, q, d_output, K, V, d_final, adj, at(l.decay), dtype, vec, st);
-        if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
-    }
-    if (dv || gates || d_initial) {
-        Walk w = base;
-        set_triple(&w, k, q, d_output, K, V);
-        w.out = dv;
+    if (dk || dv || gates || d_initial) {
+        Back w = base_walk<Back>(shape, p, g, valid, reset);
+        if (many && !p.prewalk) {
+            float *adj = at(l.state);
+            e = run_carry<true>(base, p, q, d_output, K, V, d_final, adj, at(l.decay), dtype, vec, st);
+            if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
+            w.starts = adj;
+        }
+        w.q = make_view(q), w.k = make_view(k), w.v = make_view(v), w.o = make_view(d_output);
+        w.K = (int)K, w.V = (int)V;
+        w.dk = dk, w.dv = dv;
         w.first = d_final;
-        w.starts = adj, w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
+        w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
         w.fin = d_initial;
         if (gates) {
-            w.d = make_view(v);
             w.dots = at(l.y), w.dot_sums = at(l.y_sums);
             w.edges = at(l.edges), w.edge = states, w.edge_first = first;
             w.totals = at(l.totals);
-            e = run_walk<true, true, true>(w, p, dtype, vec, st);
+            e = run_back<true>(w, p, dtype, vec, st);
         } else {
-            e = run_walk<true, true, false>(w, p, dtype, vec, st);
+            e = run_back<false>(w, p, dtype, vec, st);
         }
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
     }
-    if (dk) {
-        Walk w = base;
-        set_triple(&w, v, d_output, q, V, K);  // the state transposed: rows V, columns K
-        w.out = dk;
-        w.first = transposed(d_final);
-        w.starts = adj, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
-        e = run_walk<true, true, false>(w, p, dtype, vec, st);
-        if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
-    }
     if (dq || gates) {
-        Walk w = base;
-        set_triple(&w, d_output, v, k, V, K);
+        Forward w = base;
+        set_triple(&w, d_output, v, k, V, K);  // the state transposed: rows V, columns K
         w.out = dq;
         w.first = transposed(first);
         w.starts = many ? states : nullptr, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
@@ -1261,7 +1573,6 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     ga.x_sums = at(l.x_sums), ga.y_sums = at(l.y_sums);
     ga.edges = at(l.edges), ga.totals = at(l.totals);
     ga.BH = p.BH;
-    ga.x_slices = p.kslices, ga.y_slices = p.vslices;
     ga.dg = dg ? dg : at(l.dg);
     const dim3 grid((unsigned)((p.BH * p.chunks + kThreads / 64 - 1) / (kThreads / 64))), block(kThreads);
     if (dtype == GDN2_BF16) hipLaunchKernelGGL((linear_gate<Mat<bf16_t>::C>), grid, block, 0, st, ga);
