@@ -204,6 +204,9 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
     }
 }
 
+// Waits for the wave's memory operations (vmcnt(0), the other counters free).
+__device__ __forceinline__ void no_loads_left() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // A tile of C rows and W columns on its way from memory to LDS: 16 bytes a thread and turn.  Rows past
 // the end and columns past the width read others in their place, and become zero on the way to LDS,
 // as do the rows of padding: what they hold is not used.  VEC: unit channel stride, 16-byte aligned
@@ -258,19 +261,41 @@ struct Staged {
     }
 };
 
-// Four consecutive columns of the output at token t.
-template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T *out, int64_t row, int col, int width, const f32x4 &x) {
-    T *p = out + row * width + col;
-    T e[4];
+// A chunk's rows of a dense output, from tiles whose rows are four columns from col on and whose columns
+// are the tokens 16 j + n16; out is at the chunk's first row, stride the elements between two rows.
+//
+// Whole chunks of whole columns are stored without conditions.  Otherwise the compiler cannot count the
+// stores behind the next chunk's loads, and the wait for those loads becomes one for the stores too (a
+// tenth of a step); on the other way it is told that none are left.
+template <typename T, int TT, bool VEC>
+__device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int width, int left, bool whole,
+                                           const f32x4 (&x)[TT]) {
+    const int n16 = lane_id() & 15;
+    T *p = out + n16 * stride + col;
+    if (VEC && whole && left >= 16 * TT) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i]);
-    if (VEC) {
-        if (col < width) __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), e, sizeof e);
-    } else {
+        for (int j = 0; j < TT; ++j) {
+            T e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (col + i < width) p[i] = e[i];
+            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[j][i]);
+            __builtin_memcpy(__builtin_assume_aligned(p + 16 * j * stride, 4 * sizeof(T)), e, sizeof e);
+        }
+        return;
+    }
+    no_loads_left();
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[j][i]);
+        if (16 * j + n16 >= left) continue;
+        if (VEC) {
+            if (col < width) __builtin_memcpy(__builtin_assume_aligned(p + 16 * j * stride, 4 * sizeof(T)), e, sizeof e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < width) p[16 * j * stride + i] = e[i];
+        }
     }
 }
 
@@ -315,7 +340,7 @@ struct WalkLds {
     T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
     GateTile<C> gate[kGates];
     float red[CP / 16][C];
-    float rows[3][C], cols[3][C], diag[C];  // parts of the pair sums, by tiles of 16 tokens
+    float rows[C / 16][C], cols[C / 16][C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
 template <typename T, int KP, int VP>
@@ -455,14 +480,36 @@ __device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const S
     }
 }
 
-// The wave's part of a dot product per token: its four columns of d against acc, summed over the groups.
-template <typename T>
-__device__ __forceinline__ void dot_rows(const f32x4 &acc, float f, const T *d, float *red) {
-    float x = 0.f;
+// The value of the lane's 16-lane group (or of the lane's place in it) among four.
+__device__ __forceinline__ float pick(int i, float a, float b, float c, float d) {
+    return i < 2 ? (i == 0 ? a : b) : (i == 2 ? c : d);
+}
+
+// The wave's part of a dot product per token: its columns of d against acc, summed over the groups; the
+// tiles side by side, so that the lane moves of one are the waits of the others.  f: row factors; a row
+// with factor 0 gives 0, also where the state is not finite.
+template <typename T, int TT>
+__device__ __forceinline__ void dot_rows(const f32x4 (&acc)[TT], const float (&f)[TT], const T *d, int ld, float *red) {
+    const int lane = lane_id(), n16 = lane & 15, g4 = 4 * (lane >> 4);
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x += acc[i] * Elem<T>::load(d, i);
-    x = groups_sum(f == 0.f ? 0.f : x);  // also where the state is not finite
-    if (lane_id() < 16) red[lane_id()] = x;
+    for (int j = 0; j < TT; ++j) {
+        T e[4];
+        __builtin_memcpy(e, __builtin_assume_aligned(d + (16 * j + n16) * ld + g4, 4 * sizeof(T)), sizeof e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j] += acc[j][i] * Elem<T>::load(e, i);
+        x[j] = f[j] == 0.f ? 0.f : x[j];
+    }
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < TT; ++j) y[j] = __shfl_xor(x[j], 16);
+#pragma unroll
+    for (int j = 0; j < TT; ++j) x[j] += y[j];
+#pragma unroll
+    for (int j = 0; j < TT; ++j) y[j] = __shfl_xor(x[j], 32);
+#pragma unroll
+    for (int j = 0; j < TT; ++j) x[j] += y[j];
+    if (lane < 16 * TT) red[lane] = pick(lane >> 4, x[0], x[1], x[2], x[3]);
 }
 
 // A chunk's dot products from the waves' parts, and their sum (one wave).
@@ -666,16 +713,19 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward 
 
         // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: twelve in
         // bf16, three in float32.
+        constexpr int MINE = TT == 4 ? (12 + NW - 1) / NW : 1;
+        f32x4 y[MINE];
+        int tjs[MINE], sis[MINE];
 #pragma unroll
-        for (int m = 0; m < (TT == 4 ? 12 / NW + (12 % NW > 0) : 1); ++m) {
+        for (int m = 0; m < MINE; ++m) {
             const int id = wave + m * NW;
-            int tj, si;
-            if (TT == 4) {
-                if (12 % NW && id >= 12) continue;
-                tj = id < 4 ? id >> 1 : id < 8 ? 2 : 3, si = id < 4 ? id & 1 : id & 3;
-            } else {
-                tj = id >> 1, si = id & 1;
-                if (id >= 4 || si > tj) continue;  // a block of 16 sources that no row sees
+            int tj = id >> 1, si = id & 1;
+            if (TT == 4 && id >= 4) tj = id < 8 ? 2 : 3, si = id & 3;
+            tjs[m] = tj, sis[m] = si;
+            // none: a wave without a tile, or a block of 16 sources that no row sees
+            if ((TT == 4 && 12 % NW && id >= 12) || (TT == 2 && (id >= 4 || si > tj))) {
+                tjs[m] = -1;
+                continue;
             }
             f32x4 x = zero4();
 #pragma unroll
@@ -687,33 +737,39 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward 
 #pragma unroll
             for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
             __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
-            if (DOT && si <= tj) {
-                f32x4 y = zero4();
+            if (DOT) {
+                y[m] = zero4();
 #pragma unroll
                 for (int r = 0; r < CP; r += RB)
-                    M::mma(y, M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
+                    M::mma(y[m], M::row(lds.c + 16 * si * LDC, LDC, r), M::row(lds.d + 16 * tj * LDC, LDC, r));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[i];
-                if (si < tj) {
-                    const float sum = groups_sum((y[0] + y[1]) + (y[2] + y[3]));
-                    if (lane < 16) lds.rows[si][t] = sum;
+                for (int i = 0; i < 4; ++i) y[m][i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[m][i];
+            }
+        }
+        if (DOT) {
+            // By tiles: the sums over s for each row, and over the rows for each s; of a tile on the diagonal, for
+            // each of its tokens, the sum over the rows from it on and the s before it.  All tiles of the wave
+            // side by side.
+            float q[MINE], a[MINE], b[MINE], c[MINE];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float c = row16_sum(y[i]);
-                        if (n16 == i) lds.cols[tj - 1][s + i] = c;
-                    }
-                } else {
-                    // sums over s before each of the lane's four tokens, over the groups in order
-                    const float q = (y[0] + y[1]) + (y[2] + y[3]);
-                    const float q1 = __shfl_up(q, 16), q2 = __shfl_up(q, 32), q3 = __shfl_up(q, 48);
-                    float pre = (g4 > 0 ? q1 : 0.f) + (g4 > 4 ? q2 : 0.f) + (g4 > 8 ? q3 : 0.f);
+            for (int m = 0; m < MINE; ++m) q[m] = (y[m][0] + y[m][1]) + (y[m][2] + y[m][3]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float c = row16_sum(n16 >= g4 + i ? pre : 0.f);
-                        if (n16 == i) lds.diag[s + i] = c;
-                        pre += y[i];
-                    }
+            for (int m = 0; m < MINE; ++m)
+                a[m] = __shfl_up(q[m], 16), b[m] = __shfl_up(q[m], 32), c[m] = __shfl_up(q[m], 48);
+#pragma unroll
+            for (int m = 0; m < MINE; ++m) {
+                const float pre = (g4 > 0 ? a[m] : 0.f) + (g4 > 4 ? b[m] : 0.f) + (g4 > 8 ? c[m] : 0.f);
+                const bool diag = tjs[m] == sis[m];
+                float z[4], before = pre;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    z[i] = row16_sum(diag ? (n16 >= g4 + i ? before : 0.f) : y[m][i]);
+                    before += y[m][i];
                 }
+                if (tjs[m] < 0 || sis[m] > tjs[m]) continue;
+                const int s = 16 * sis[m] + g4;
+                if (n16 < 4) lds.cols[tjs[m]][s + n16] = pick(n16, z[0], z[1], z[2], z[3]);
+                if (lane >= 48) lds.rows[sis[m]][16 * tjs[m] + n16] = pre + q[m];  // the last group: all s
             }
         }
         // acc[j]: rows = the wave's columns, column = token 16 j + n16; the state's part.
@@ -721,13 +777,14 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward 
 #pragma unroll
         for (int j = 0; j < TT; ++j) acc[j] = zero4();
         state_rows<T, KP, DOT>(acc, S, lds.a, LDA);
+        float f[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            const float f = gate.row[16 * j + n16];
+            f[j] = gate.row[16 * j + n16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] *= f;
-            if (DOT) dot_rows<T>(acc[j], f, lds.d + (16 * j + n16) * LDC + 16 * wave + g4, &lds.red[wave][16 * j]);
+            for (int i = 0; i < 4; ++i) acc[j][i] *= f[j];
         }
+        if (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
         if (DOT && wave == 1) store_dots<C, NW>(lds.red, p, at.bh, ci);
         if (DOT && wave == 2) {
@@ -740,10 +797,10 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward 
                 if (j > 0) left = r0 = lds.rows[0][lane];
                 if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
                 if (TT == 4 && j > 2) left += lds.rows[2][lane];
-                if (j < 1) below += lds.cols[0][lane];
-                if (TT == 4 && j < 2) below += lds.cols[1][lane];
-                if (TT == 4 && j < 3) below += lds.cols[2][lane];
-                x = lds.diag[lane];
+                if (j < 1) below += lds.cols[1][lane];
+                if (TT == 4 && j < 2) below += lds.cols[2][lane];
+                if (TT == 4 && j < 3) below += lds.cols[3][lane];
+                x = lds.cols[j][lane];
             }
             if (TT == 4) {
                 const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
@@ -773,19 +830,19 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward 
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
         const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
         if (__builtin_expect(fine && next, 1)) {
-            if (o) {
 #pragma unroll
-                for (int j = 0; j < TT; ++j) {
+            for (int j = 0; j < TT; ++j)
 #pragma unroll
-                    for (int r = 0; r <= j / BT; ++r)
-                        M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
-                    const int t = 16 * j + n16;
-                    if (t < left)
-                        store4<T, VEC>(o, row0 + (int64_t)t * p.H, 16 * wave + g4, p.vc, acc[j]);
-                }
-            }
+                for (int r = 0; r <= j / BT; ++r)
+                    M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
+            if (o)
+                store_rows<T, TT, VEC>(o + row0 * p.vc, (int64_t)p.H * p.vc, 16 * wave + g4, p.vc, left,
+                                       p.vc == CP, acc);
+            else
+                no_loads_left();
             S = U;
         } else {
+            no_loads_left();
             walk_tokens<T, KP, LDC, false, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc,
                                                  o ? o + row0 * p.vc : nullptr, (int64_t)p.H * p.vc, left);
             fine = S.finite();
@@ -947,14 +1004,14 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 for (int j = 0; j < TT; ++j) M::mma(ak[j], x, M::row(lds.v + 16 * j * LDV, LDV, r));
             }
         }
+        float f[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            const float f = gate.row[16 * j + n16];
+            f[j] = gate.row[16 * j + n16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) av[j][i] *= f, ak[j][i] *= f;
-            if (DOT && own_v)
-                dot_rows<T>(av[j], f, lds.v + (16 * j + n16) * LDV + 16 * wave + g4, &lds.red[wave][16 * j]);
+            for (int i = 0; i < 4; ++i) av[j][i] *= f[j], ak[j][i] *= f[j];
         }
+        if (DOT && own_v) dot_rows<T, TT>(av, f, lds.v + 16 * wave, LDV, lds.red[wave]);
         if (!good && lane == 0) lds.bad[n & 1] = 1;
         __syncthreads();
         const bool bad = lds.bad[n & 1] != 0;
@@ -967,29 +1024,30 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         if (__builtin_expect(!bad, 1)) {
             if (dv && own_v) {
 #pragma unroll
-                for (int j = 0; j < TT; ++j) {
+                for (int j = 0; j < TT; ++j)
 #pragma unroll
                     for (int r = j / BT; r < C / RB; ++r)
                         M::mma(av[j], of[r], M::row(lds.pk + 16 * j * LDP, LDP, r * RB));
-                    const int t = 16 * j + n16;
-                    if (t < left) store4<T, VEC>(dv, row0 + (int64_t)t * p.H, 16 * wave + g4, p.V, av[j]);
-                }
+                store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, p.V == VP, av);
+            } else {
+                no_loads_left();
             }
             if (dk && own_k) {
                 typename M::Frag qf[C / RB];
 #pragma unroll
                 for (int r = 0; r < C / RB; ++r) qf[r] = M::template across<LDK>(lds.q, r * RB, 16 * wave);
 #pragma unroll
-                for (int j = 0; j < TT; ++j) {
+                for (int j = 0; j < TT; ++j)
 #pragma unroll
                     for (int r = j / BT; r < C / RB; ++r)
                         M::mma(ak[j], qf[r], M::row(lds.pv + 16 * j * LDP, LDP, r * RB));
-                    const int t = 16 * j + n16;
-                    if (t < left) store4<T, VEC>(dk, row0 + (int64_t)t * p.H, 16 * wave + g4, p.K, ak[j]);
-                }
+                store_rows<T, TT, VEC>(dk + row0 * p.K, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, ak);
+            } else {
+                no_loads_left();
             }
             S = U;
         } else {
+            no_loads_left();
             // Token by token, all waves together: see walk_tokens.
             float *part = reinterpret_cast<float *>(lds.pk);  // [NW][KP]: dk's sums over a wave's columns
             static_assert(sizeof(lds.pk) >= sizeof(float) * NW * KP, "");
@@ -1083,13 +1141,25 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
     float x = 0.f;
     if (p.first)
         x = p.first[bh / p.H * p.f_b + bh % p.H * p.f_h + i / p.V * p.f_row + i % p.V * p.f_col];
-    for (int n = 0; n + 1 < p.segments; ++n) {
-        const int s = p.rev ? p.segments - 1 - n : n;
-        const float add = st[s * p.KV];
-        st[s * p.KV] = x;
-        x = (d[s] == 0.f ? 0.f : d[s] * x) + add;
+    // Eight segments' additions are read at a time: each store would hold back the next load.
+    constexpr int N = 8;
+    const int step = p.rev ? -1 : 1;
+    int s = p.rev ? p.segments - 1 : 0;
+    for (int n = p.segments; n > 0; n -= N, s += step * N) {
+        float add[N], f[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int at = s + step * min(k, max(n - 2, 0));  // the last segment adds nothing that is needed
+            add[k] = st[at * p.KV];
+            f[k] = d[at];
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (k >= n) break;
+            st[(s + step * k) * p.KV] = x;
+            x = (f[k] == 0.f ? 0.f : f[k] * x) + add[k];
+        }
     }
-    st[(p.rev ? 0 : p.segments - 1) * p.KV] = x;
 }
 
 // ---- the gate's gradient -------------------------------------------------------------------------
