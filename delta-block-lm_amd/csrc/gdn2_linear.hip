@@ -616,7 +616,7 @@ __device__ __forceinline__ void make_gates(const Walk &p, const Place &at, int c
 //   pairs_t = sum_{u >= t, s < t, both in the chunk} Gam_us (a_u.b_s)(d_u.c_s),
 // which with (a, b, c, d) = (do, v, k, q) is the part of the gate's gradient inside the chunk.
 template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
-__global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : 1) linear_walk(Forward p) {
+__global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_walk(Forward p) {
     static_assert(!(OUT && REV), "");
     typedef Mat<T> M;
     typedef WalkLds<T, KP, CP, OUT, DOT> L;
