@@ -15,8 +15,11 @@
 // dv and dk share a walk in the other direction (linear_back), with the pairs' decays and the adjoint
 // state of both.  The gate's gradient is a sum over the pairs that span a token,
 //   dg_t = sum_{u>=t,s<t} W_us,  W_us = Gam_us (q_u.k_s)(do_u.v_s),
-// cut at the chunk's bounds (linear_gate): the walks give its parts.  Nothing is subtracted over more
-// than one segment, so it keeps float32 accuracy for long memories.
+// cut at the chunk's bounds, with x_u = gam_u q_u^T S0 do_u, y_s = lam_s k_s^T R v_s and E = gam <S0, R>:
+//   dg_t = sum_{u>=t,s<t inside the chunk} W_us + sum_{u>=t} x_u + sum_{s<t} y_s + E.
+// linear_back gives y and the products <S0, R> at segment starts; the dq walk has the rest and steps
+// E from chunk to chunk (less x, plus y; 0 at a cut).  Nothing is subtracted over more than one segment,
+// so it keeps float32 accuracy for long memories.
 #include <math.h>
 
 #include <algorithm>
@@ -107,7 +110,6 @@ struct Walk {
     int s_row, s_col;
     float *starts_out;      // the prewalk's states before every segment, or null
     float *fin;             // state after the walk, [B H, rows, columns], or null
-    float *dots, *dot_sums; // [B H, T], [B H, chunks]: see DOT
     int64_t T;
     int H;
     int chunks, seg_chunks, segments;
@@ -118,7 +120,8 @@ struct Forward : Walk {
     View a, b, c, d;        // d: see DOT
     int ka, vc;             // widths of a and b, and of c, d and out
     void *out;              // dense [B, T, H, vc], or null
-    float *pairs;           // [B H, T]: see DOT
+    const float *y, *edges; // [B H, T], [B H, segments], from linear_back
+    float *dg;              // dense [B, T, H]
     float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
     float *seg_decay;       // [B H, segments]
 };
@@ -130,8 +133,8 @@ struct Back : Walk {
     void *dk, *dv;          // dense, or null
     View edge_first;        // with DOT: the forward's states, its first one
     const float *edge;      // and those before the other segments
+    float *y;               // [B H, T]: see DOT
     float *edges;           // [B H, segments]: <forward state, adjoint> at each segment's start
-    float *totals;          // [B H, chunks]: decay of each chunk
 };
 
 // DPP moves of 64 bits; lanes without a source read 0.
@@ -326,6 +329,14 @@ __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s
     return f;
 }
 
+// Inclusive sums over the lanes of each 16-lane group.
+__device__ __forceinline__ void row_scan(float &x) {
+    x += dpp<0x111>(x);
+    x += dpp<0x112>(x);
+    x += dpp<0x114>(x);
+    x += dpp<0x118>(x);
+}
+
 // Sum over the four 16-lane groups of a wave.
 __device__ __forceinline__ float groups_sum(float x) {
     x += __shfl_xor(x, 16);
@@ -512,20 +523,17 @@ __device__ __forceinline__ void dot_rows(const f32x4 (&acc)[TT], const float (&f
     if (lane < 16 * TT) red[lane] = pick(lane >> 4, x[0], x[1], x[2], x[3]);
 }
 
-// A chunk's dot products from the waves' parts, and their sum (one wave).
+// A token's dot product from the waves' parts (one wave, lane = token; 0 past the chunk).
 template <int C, int NW, int ALL>
-__device__ __forceinline__ void store_dots(const float (&red)[ALL][C], const Walk &p, int64_t bh, int ci) {
+__device__ __forceinline__ float sum_dots(const float (&red)[ALL][C]) {
     const int lane = lane_id();
-    const int64_t t = (int64_t)ci * C + lane;
     float d = 0.f;
     if (lane < C) {
         d = red[0][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) d += red[w][lane];
     }
-    if (lane < C && t < p.T) p.dots[bh * p.T + t] = d;
-    const float sum = wave_sum(d);
-    if (lane == 0) p.dot_sums[bh * p.chunks + ci] = sum;
+    return d;
 }
 
 // A chunk token by token, taken where the state before or after it is not finite: products over masked
@@ -612,11 +620,10 @@ __device__ __forceinline__ void make_gates(const Walk &p, const Place &at, int c
 // worked on.  Without `starts` a segment's start state is walked to from the sequence's start (prewalk: b
 // and c alone).  OUT = false: only the state that the segment adds and its decay (carry; REV: from the
 // last chunk to the first).
-// DOT: dot_t = sum over columns of row_t (a_t S) d_t, and the pair sums
-//   pairs_t = sum_{u >= t, s < t, both in the chunk} Gam_us (a_u.b_s)(d_u.c_s),
-// which with (a, b, c, d) = (do, v, k, q) is the part of the gate's gradient inside the chunk.
+// DOT: the gate's gradient too, with (a, b, c, d) = (do, v, k, q): the products of the state's part with d
+// are its x, and W_us = Gam_us (a_u.b_s)(d_u.c_s).
 template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
-__global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_walk(Forward p) {
+__global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_walk(Forward p) {
     static_assert(!(OUT && REV), "");
     typedef Mat<T> M;
     typedef WalkLds<T, KP, CP, OUT, DOT> L;
@@ -701,6 +708,7 @@ __global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_wa
     if (p.starts_out && at.nth > 0)
         S.store(p.starts_out + at.bh * p.s_bh + at.seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
 
+    float edge = DOT ? p.edges[at.bh * p.segments + at.seg] : 0.f;  // <S0, R> at the chunk's start
     for (; n > 0; --n, ++ci) {
         const GateTile<C> &gate = lds.gate[gi];
         const bool masks = odd || p.T - (int64_t)ci * C < C;
@@ -709,6 +717,9 @@ __global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_wa
         sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
         if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, p.vc);
         if (n > 1) fetch(ci + 1, true);
+        const int64_t token = (int64_t)ci * C + lane;
+        float y_now = 0.f;  // of this chunk, for the wave that adds up dg
+        if (DOT && wave == 2) y_now = p.y[at.bh * p.T + min(token, p.T - 1)];
         __syncthreads();
 
         // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: twelve in
@@ -786,13 +797,11 @@ __global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_wa
         }
         if (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
-        if (DOT && wave == 1) store_dots<C, NW>(lds.red, p, at.bh, ci);
         if (DOT && wave == 2) {
             // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t of the
             // tile over the tiles below, whole tiles below and to the left, and its own tile.
-            const int64_t t = (int64_t)ci * C + lane;
             const int j = lane / 16;
-            float left = 0.f, below = 0.f, x = 0.f, r0 = 0.f, r1 = 0.f;
+            float left = 0.f, below = 0.f, dg = 0.f, r0 = 0.f, r1 = 0.f;
             if (lane < C) {
                 if (j > 0) left = r0 = lds.rows[0][lane];
                 if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
@@ -800,26 +809,30 @@ __global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_wa
                 if (j < 1) below += lds.cols[1][lane];
                 if (TT == 4 && j < 2) below += lds.cols[2][lane];
                 if (TT == 4 && j < 3) below += lds.cols[3][lane];
-                x = lds.cols[j][lane];
+                dg = lds.cols[j][lane];
             }
             if (TT == 4) {
                 const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
                 const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
-                x += j == 1 ? f1 : j == 2 ? f2 : 0.f;
+                dg += j == 1 ? f1 : j == 2 ? f2 : 0.f;
             }
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) {
-                const float y = __shfl_down(left, d);
-                if (n16 + d < 16) left += y;
-            }
-            float pre = __shfl_up(below, 1);
-            if (n16 == 0) pre = 0.f;
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) {
-                const float y = __shfl_up(pre, d);
-                if (n16 >= d) pre += y;
-            }
-            if (lane < C && t < p.T) p.pairs[(int64_t)at.bh * p.T + t] = (left + pre) + x;
+            // Sums from a lane to the end are sums up to it with the lanes turned round: scans add only what
+            // belongs to them, so that a value that is not finite stays with the tokens that see it.
+            const bool in = lane < C && token < p.T;
+            const float x = sum_dots<C, NW>(lds.red), y = in ? y_now : 0.f;
+            const int turned = lane ^ 15;
+            float up = __shfl(left, turned);
+            row_scan(up);
+            float before = __shfl_up(below, 1), y_before = __shfl_up(y, 1);
+            if (n16 == 0) before = 0.f;
+            row_scan(before);
+            const float x_on = wave_scan_add(__shfl(x, 63 - lane));
+            const float y_sum = wave_scan_add(lane == 0 ? 0.f : y_before);
+            const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(x);
+            dg += (__shfl(up, turned) + before) + (__shfl(x_on, 63 - lane) + y_sum) + E;
+            edge = E + wave_sum(y);
+            const bool on = in && gate.seg[lane] >= 0 && gate.step[lane] != 0.f;
+            if (in) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
         }
 
         typename M::Frag cf[C / RB];
@@ -857,7 +870,7 @@ __global__ void __launch_bounds__(4 * CP, !OUT ? 4 : CP == 64 ? 2 : 1) linear_wa
 // and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once
 // a chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for
 // dk read three of the four tensors again, and took its pairs' decays and the state's update a second
-// time.)  DOT: dot_s = row_s k_s^T S v_s, and the products with the forward's states at segment starts.
+// time.)  DOT: y_s = row_s k_s^T S v_s, and the products with the forward's states at segment starts.
 template <typename T, int KP, int VP, bool VEC, bool DOT>
 __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
     typedef Mat<T> M;
@@ -1016,8 +1029,11 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         __syncthreads();
         const bool bad = lds.bad[n & 1] != 0;
         if (threadIdx.x == 0) lds.bad[(n & 1) ^ 1] = 0;
-        if (DOT && wave == 1) store_dots<C, VP / 16>(lds.red, p, at.bh, ci);
-        if (DOT && threadIdx.x == 0) p.totals[(int64_t)at.bh * p.chunks + ci] = gate.tot;
+        if (DOT && wave == 1) {
+            const int64_t t = (int64_t)ci * C + lane;
+            const float y = sum_dots<C, VP / 16>(lds.red);
+            if (lane < C && t < p.T) p.y[at.bh * p.T + t] = y;
+        }
         const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
         T *dv = reinterpret_cast<T *>(p.dv), *dk = reinterpret_cast<T *>(p.dk);
@@ -1162,68 +1178,6 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
     }
 }
 
-// ---- the gate's gradient -------------------------------------------------------------------------
-
-struct GateGradArgs {
-    Walk w;                       // g, masks, sizes
-    const float *x, *y, *pairs;   // dots of the dq and dv walks, pair sums of the dq walk
-    const float *x_sums, *y_sums; // per chunk
-    const float *edges, *totals;
-    int64_t BH;
-    float *dg;                    // dense [B, T, H]
-};
-
-// One wave a chunk: the pair sums inside it, and the pairs that reach out of it:
-//   dg_t = pairs_t + sum_{u>=t} x_u + sum_{s<t} y_s + E,
-// E the pairs around the whole chunk: the edge product at the segment's start, then chunk by chunk,
-// from the last chunk with a cut in it if there is one.
-template <int C>
-__global__ void __launch_bounds__(kThreads) linear_gate(GateGradArgs p) {
-    const int lane = lane_id(), wave = threadIdx.x >> 6;
-    const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + wave;
-    if (id >= p.BH * p.w.chunks) return;
-    const int ci = id % p.w.chunks;
-    const int64_t bh = id / p.w.chunks, b = bh / p.w.H, h = bh % p.w.H;
-    const int64_t t = (int64_t)ci * C + lane;
-    const bool in = lane < C && t < p.w.T;
-    const GateIn gi = gate_load<C>(p.w, b, h, ci);
-    const bool val = in && gi.valid != 0.f && gi.reset == 0.f && !(gi.g < kCut);
-    float dg = 0.f, x = 0.f, y = 0.f;
-    if (in) {
-        x = p.x[bh * p.w.T + t];
-        y = p.y[bh * p.w.T + t];
-        dg = p.pairs[bh * p.w.T + t];
-    }
-    // sum of x over u >= t, and of y over s < t: scans that add only what belongs to them
-    float sx = x, sy = __shfl_up(y, 1);
-    if (lane == 0) sy = 0.f;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const float a = __shfl_down(sx, d), c = __shfl_up(sy, d);
-        if (lane + d < 64) sx += a;
-        if (lane >= d) sy += c;
-    }
-    float E = 0.f;
-    if (p.totals[bh * p.w.chunks + ci] != 0.f) {
-        const int seg = ci / p.w.seg_chunks, c_lo = seg * p.w.seg_chunks;
-        int from = c_lo;  // first chunk whose sums count in full
-        bool cut = false;
-        for (int c0 = c_lo; c0 < ci; c0 += 64) {
-            const int c = c0 + lane;
-            const unsigned long long m = __ballot(c < ci && p.totals[bh * p.w.chunks + min(c, ci)] == 0.f);
-            if (m) from = c0 + 63 - __clzll(m), cut = true;
-        }
-        for (int c = from + lane; c < ci; c += 64)
-            E += p.y_sums[bh * p.w.chunks + c] - (cut && c == from ? 0.f : p.x_sums[bh * p.w.chunks + c]);
-        if (lane == 0 && !cut) E += p.edges[bh * p.w.segments + seg];
-        E = wave_sum(E);
-        E -= wave_sum(x);
-    }
-    if (!in) return;
-    dg += sx + sy + E;
-    p.dg[(b * p.w.T + t) * p.w.H + h] = val ? dg : 0.f;
-}
-
 // out[h] = sum over b, t of x[b, t, h]: one workgroup a head, a fixed order.
 __global__ void __launch_bounds__(1024) linear_head_sum(const float *x, int64_t rows, int64_t H, float *out) {
     __shared__ float red[16];
@@ -1352,7 +1306,7 @@ Plan plan(const gdn2_shape *s, int dtype) {
 }
 
 struct Layout {
-    size_t state, decay, x, y, pairs, x_sums, y_sums, edges, totals, dg, bytes;
+    size_t state, decay, y, edges, dg, bytes;
 };
 
 // Checkpoint: the start states of the segments, and their decays.
@@ -1373,13 +1327,8 @@ Layout workspace_layout(const Plan &p, int64_t T) {
     };
     l.state = take(p.segments > 1 && !p.prewalk ? p.BH * p.segments * p.KV : 0);
     l.decay = take(p.BH * p.segments);
-    l.x = take(p.BH * T);
     l.y = take(p.BH * T);
-    l.pairs = take(p.BH * T);
-    l.x_sums = take(p.BH * p.chunks);
-    l.y_sums = take(p.BH * p.chunks);
     l.edges = take(p.BH * p.segments);
-    l.totals = take(p.BH * p.chunks);
     l.dg = take(p.BH * T);
     l.bytes = n;
     return l;
@@ -1612,9 +1561,8 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
         w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
         w.fin = d_initial;
         if (gates) {
-            w.dots = at(l.y), w.dot_sums = at(l.y_sums);
-            w.edges = at(l.edges), w.edge = states, w.edge_first = first;
-            w.totals = at(l.totals);
+            w.y = at(l.y), w.edges = at(l.edges);
+            w.edge = states, w.edge_first = first;
             e = run_back<true>(w, p, dtype, vec, st);
         } else {
             e = run_back<false>(w, p, dtype, vec, st);
@@ -1629,26 +1577,17 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
         w.starts = many ? states : nullptr, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
         if (gates) {
             w.d = make_view(q);
-            w.dots = at(l.x), w.dot_sums = at(l.x_sums), w.pairs = at(l.pairs);
+            w.y = at(l.y), w.edges = at(l.edges);
+            w.dg = dg ? dg : at(l.dg);
             e = run_walk<false, true, true>(w, p, dtype, vec, st);
         } else {
             e = run_walk<false, true, false>(w, p, dtype, vec, st);
         }
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
     }
-    if (!gates) return ok();
-    GateGradArgs ga{};
-    ga.w = base;
-    ga.x = at(l.x), ga.y = at(l.y), ga.pairs = at(l.pairs);
-    ga.x_sums = at(l.x_sums), ga.y_sums = at(l.y_sums);
-    ga.edges = at(l.edges), ga.totals = at(l.totals);
-    ga.BH = p.BH;
-    ga.dg = dg ? dg : at(l.dg);
-    const dim3 grid((unsigned)((p.BH * p.chunks + kThreads / 64 - 1) / (kThreads / 64))), block(kThreads);
-    if (dtype == GDN2_BF16) hipLaunchKernelGGL((linear_gate<Mat<bf16_t>::C>), grid, block, 0, st, ga);
-    else hipLaunchKernelGGL((linear_gate<Mat<float>::C>), grid, block, 0, st, ga);
     if (dg_heads)
-        hipLaunchKernelGGL(linear_head_sum, dim3((unsigned)shape->heads), dim3(1024), 0, st, ga.dg,
+        hipLaunchKernelGGL(linear_head_sum, dim3((unsigned)shape->heads), dim3(1024), 0, st,
+                           dg ? dg : at(l.dg),
                            shape->batch * shape->time, shape->heads, dg_heads);
     return launch_status(hipGetLastError(), "gdn2_linear_backward");
 }
