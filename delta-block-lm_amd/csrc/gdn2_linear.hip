@@ -387,7 +387,8 @@ struct State {
             for (int i = 0; i < 4; ++i) z = fmaf(t[m][i], 0.f, z);
         return !__any(z != 0.f);  // z is 0 or NaN
     }
-    // Rows and columns of src at strides below 2^22 (32-bit offsets: 64 addresses would spill).
+    // Rows and columns of src at strides below 2^22 (32-bit offsets: 64 addresses would spill).  The loads
+    // are only issued; settle() waits for them and zeroes what lies outside the state.
     __device__ __forceinline__ void load(const float *src, int rs, int cs, int v, int ka, int vc) {
         const int g4 = 4 * (lane_id() >> 4);
         const uint32_t col = (uint32_t)(min(v, vc - 1) * cs);
@@ -395,6 +396,9 @@ struct State {
         for (int m = 0; m < KT; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) t[m][i] = src[col + (uint32_t)(min(16 * m + g4 + i, ka - 1) * rs)];
+    }
+    __device__ __forceinline__ void settle(int v, int ka, int vc) {
+        const int g4 = 4 * (lane_id() >> 4);
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
@@ -607,12 +611,27 @@ __device__ __forceinline__ void start_state(State<KT> &S, const Walk &p, const P
 
 // Gates of the next chunks of a walk with n left, from chunk ci on.
 template <int C, bool REV, int NW>
-__device__ __forceinline__ void make_gates(const Walk &p, const Place &at, int ci, int n, GateTile<C> *gate) {
-    for (int i = threadIdx.x >> 6; i < min(n, kGates); i += NW) {
-        const int64_t c = ci + (REV ? -i : i);
-        gate_store<C, REV>(gate_load<C>(p, at.b, at.h, c), (int)min(p.T - c * C, (int64_t)C), &gate[i]);
+struct MakeGates {
+    static constexpr int EACH = kGates / NW;  // chunks of each wave
+    GateIn x[EACH];
+    int ci, n;
+    __device__ __forceinline__ void load(const Walk &p, const Place &at, int chunk, int left) {
+        ci = chunk, n = left;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int k = min((int)(threadIdx.x >> 6) + i * NW, n - 1);
+            x[i] = gate_load<C>(p, at.b, at.h, ci + (REV ? -k : k));
+        }
     }
-}
+    __device__ __forceinline__ void store(const Walk &p, GateTile<C> *gate) const {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int k = (int)(threadIdx.x >> 6) + i * NW;
+            const int64_t c = ci + (REV ? -k : k);
+            if (k < n) gate_store<C, REV>(x[i], (int)min(p.T - c * C, (int64_t)C), &gate[k]);
+        }
+    }
+};
 
 // One workgroup: a segment's chunks in the walk's order.  Each wave owns 16 columns of the state, so its
 // part stays in its accumulators, where it is at once the product's operand of the next chunk: neither
@@ -658,12 +677,16 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             if (DOT) sd.load(pd, p.d.s1, p.d.s3, t0, left, p.vc);
         }
     };
-    fetch(ci, n <= out);
+    // All first loads are on their way before the first is waited for.
+    MakeGates<C, REV, NW> gates;
+    gates.load(p, at, ci, n);
     State<KT> S;
     S.zero();
     if (OUT) start_state(S, p, at, !walked, v, p.ka, p.vc);
+    fetch(ci, n <= out);
     int gi = 0;  // the chunk's place among the gates in LDS
-    make_gates<C, REV, NW>(p, at, ci, n, lds.gate);
+    gates.store(p, lds.gate);
+    S.settle(v, p.ka, p.vc);
     __syncthreads();
 
     const bool odd = p.valid.data || p.ka < KP || p.vc < CP;
@@ -673,7 +696,8 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
     };
     const auto next_gates = [&]() {
-        make_gates<C, REV, NW>(p, at, REV ? ci - 1 : ci + 1, n - 1, lds.gate);
+        gates.load(p, at, REV ? ci - 1 : ci + 1, n - 1);
+        gates.store(p, lds.gate);
         gi = 0;
         __syncthreads();
     };
@@ -719,7 +743,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         if (n > 1) fetch(ci + 1, true);
         const int64_t token = (int64_t)ci * C + lane;
         float y_now = 0.f;  // of this chunk, for the wave that adds up dg
-        if (DOT && wave == 2) y_now = p.y[at.bh * p.T + min(token, p.T - 1)];
+        if (DOT && wave == 1) y_now = p.y[at.bh * p.T + min(token, p.T - 1)];
         __syncthreads();
 
         // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: twelve in
@@ -797,7 +821,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         }
         if (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
-        if (DOT && wave == 2) {
+        if (DOT && wave == 1) {
             // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t of the
             // tile over the tiles below, whole tiles below and to the left, and its own tile.
             const int j = lane / 16;
@@ -903,12 +927,15 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             sv.load(pv, p.v.s1, p.v.s3, t0, left, p.V);
         }
     };
-    fetch(ci, n <= out);
+    MakeGates<C, true, NW> gates;
+    gates.load(p, at, ci, n);
     State<KT> S;
     S.zero();
     if (own_v) start_state(S, p, at, !walked, v, p.K, p.V);
+    fetch(ci, n <= out);
     int gi = 0;
-    make_gates<C, true, NW>(p, at, ci, n, lds.gate);
+    gates.store(p, lds.gate);
+    S.settle(v, p.K, p.V);
     if (threadIdx.x < 2) lds.bad[threadIdx.x] = 0;
     __syncthreads();
 
@@ -919,7 +946,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         for (int r = 0; r < C / RB; ++r) of[r] = M::template across<LDV>(lds.o, r * RB, 16 * wave);
     };
     const auto next_gates = [&]() {
-        make_gates<C, true, NW>(p, at, ci - 1, n - 1, lds.gate);
+        gates.load(p, at, ci - 1, n - 1);
+        gates.store(p, lds.gate);
         gi = 0;
         __syncthreads();
     };
@@ -1121,6 +1149,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             if (src) {
                 State<KT> e;
                 e.load(src + off, rs, cs, v, p.K, p.V);
+                e.settle(v, p.K, p.V);
 #pragma unroll
                 for (int m = 0; m < KT; ++m)
 #pragma unroll
