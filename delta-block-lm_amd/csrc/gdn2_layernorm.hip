@@ -391,10 +391,10 @@ int64_t row_threads(int64_t W) {  // at most, as launch_width has them
 
 int check_ln(const gdn2_rows_shape *s, const gdn2_view *x, const float *weight) {
     if (!s) return fail(GDN2_ERR_ARGUMENT, "shape is null");
-    if (s->batch < 0 || s->time < 0 || s->heads < 0 || s->width < 1)
-        return fail(GDN2_ERR_SHAPE, "width must be >= 1 and the row axes >= 0");
+    if (s->batch < 0 || s->time < 0 || s->heads < 0 || s->width < 1 || s->width > (1 << 25))
+        return fail(GDN2_ERR_SHAPE, "width must be 1..2^25 and the row axes >= 0");
     const int64_t lim = (int64_t)1 << 31;
-    if (s->batch >= lim || s->time >= lim || s->heads >= lim || s->width >= lim ||
+    if (s->batch >= lim || s->time >= lim || s->heads >= lim ||
         (s->batch && s->time && s->heads > (lim / 2) / s->batch / s->time))
         return fail(GDN2_ERR_SHAPE, "at most 2^30 rows, and widths below 2^31");
     const int64_t rows = s->batch * s->time * s->heads;

@@ -1179,7 +1179,8 @@ struct JoinArgs {
 };
 
 __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
-    const int64_t bh = blockIdx.y, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const unsigned blocks = (unsigned)((p.KV + kThreads - 1) / kThreads);
+    const int64_t bh = blockIdx.x / blocks, i = (int64_t)(blockIdx.x % blocks) * kThreads + threadIdx.x;
     if (i >= p.KV) return;
     float *st = p.state + bh * p.segments * p.KV + i;
     const float *d = p.decay + bh * p.segments;
@@ -1480,7 +1481,7 @@ hipError_t run_carry(Forward w, const Plan &p, const gdn2_view *b, const gdn2_vi
     if (e != hipSuccess) return e;
     const JoinArgs j{state, decay, (const float *)first.data, first.s0, first.s1, first.s2, first.s3,
                      w.H, K * V, V, p.segments, REV};
-    hipLaunchKernelGGL(linear_join, dim3((unsigned)((K * V + kThreads - 1) / kThreads), (unsigned)p.BH),
+    hipLaunchKernelGGL(linear_join, dim3((unsigned)((K * V + kThreads - 1) / kThreads * p.BH)),
                        dim3(kThreads), 0, st, j);
     return hipGetLastError();
 }

@@ -170,6 +170,18 @@ def test_gradient_is_that_of_differences(dk):
         assert abs((loss(*p) - loss(*m)) / (2 * h) - terms.sum()) <= 2e-3 * np.abs(terms).sum()
 
 
+def test_more_than_32_bits_of_values(dk):
+    x = torch.randn((1, 4096), device="cuda").to(torch.bfloat16).repeat(1 << 20, 1)  # 2^32 values
+    x[-1] = torch.randn(4096, device="cuda").to(torch.bfloat16)
+    w, b = torch.rand(4096, device="cuda"), torch.rand(4096, device="cuda")
+    y, mean, inv = dk.layer_norm_forward(x, w, b)
+    tail, m, i = dk.layer_norm_forward(x[-2:].clone(), w, b)
+    assert torch.equal(y[-2:], tail) and torch.equal(mean[-2:], m) and torch.equal(inv[-2:], i)
+    dx, _, _ = dk.layer_norm_backward(x, w, mean, inv, y)
+    dt, _, _ = dk.layer_norm_backward(x[-2:].clone(), w, m, i, tail)
+    assert torch.equal(dx[-2:], dt)
+
+
 def test_runs_are_equal_bit_for_bit(dk):
     x, w, b, dy = inputs(7, (3000, 512), torch.bfloat16)
     for a, c in zip(run(dk, x, w, b, dy, 1e-5, torch.bfloat16), run(dk, x, w, b, dy, 1e-5, torch.bfloat16)):

@@ -254,6 +254,37 @@ def test_a_value_that_is_not_finite_stays_with_those_that_see_it(dk, name, dtype
         assert np.isnan(got["out"][after]).any(-1).all()
 
 
+def test_rows_more_than_32_bits_apart(dk):
+    """Tokens 65536 elements apart, so that the last ones lie beyond 2^32 elements: the same results as
+    from a copy."""
+    T, far = 66000, 1 << 16
+    buf = torch.empty((T * far,), dtype=torch.bfloat16, device="cuda")
+    x = [buf[64 * i:].as_strided((1, T, 1, 32), (0, far, 64, 1)) for i in range(3)]
+    for t in x:
+        t.copy_(torch.randn(t.shape, device="cuda"))
+    dense = [t.contiguous() for t in x]
+    g = -torch.rand((1, T, 1), device="cuda")
+    a = dk.linear_attention_forward(*x, g)
+    b = dk.linear_attention_forward(*dense, g)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    da = dk.linear_attention_backward(*x, g, None, None, None, a[2], x[1])
+    db = dk.linear_attention_backward(*dense, g, None, None, None, b[2], dense[1])
+    for i, (p, q) in enumerate(zip(da[:4], db[:4])):
+        assert torch.equal(p, q), i
+
+
+def test_more_sequences_than_a_grid_axis_holds(dk):
+    """65600 heads in two segments each: the same as a few of them alone."""
+    B, T, H = 4100, 17 * 32, 16
+    q = torch.randn((1, T, 1, 4), device="cuda").expand(B, T, H, 4)
+    g = torch.linspace(-0.5, -0.01, H, device="cuda")
+    out, fin, _ = dk.linear_attention_forward(q, q, q, g)
+    few, few_fin, _ = dk.linear_attention_forward(q[:1], q[:1], q[:1], g)
+    for b in (0, 1, 4095, 4096, 4099):
+        assert torch.allclose(fin[b], few_fin[0], rtol=1e-5, atol=1e-5), b
+        assert torch.allclose(out[b], few[0], rtol=1e-5, atol=1e-4), b
+
+
 def test_runs_are_equal_bit_for_bit(dk):
     p = problem(12, 2, 700, 2, 64, 64, torch.bfloat16, initial=True, final=True)
     a, b = run(dk, p, torch.bfloat16), run(dk, p, torch.bfloat16)

@@ -112,6 +112,18 @@ def test_no_rows(dk):
     assert a.shape == again.shape == (0, 32) and dh.shape == (0, 64) and exps.shape == (0, 2)
 
 
+def test_more_than_32_bits_of_values(dk):
+    rows, M = (1 << 17) + 3, 1 << 14  # 2^32 and more values of h
+    h = torch.randn((1, 2 * M), device="cuda").to(torch.bfloat16).repeat(rows, 1)
+    h[-1] = torch.randn(2 * M, device="cuda").to(torch.bfloat16)
+    a, codes, exps = dk.swiglu_q8_forward(h)
+    ta, tc, te = dk.swiglu_q8_forward(h[-2:].clone())
+    assert torch.equal(a[-2:], ta) and torch.equal(codes[-2:], tc) and torch.equal(exps[-2:], te)
+    dh, again = dk.swiglu_q8_backward(codes, exps, a)
+    td, tg = dk.swiglu_q8_backward(tc, te, ta)
+    assert torch.equal(dh[-2:], td) and torch.equal(again[-2:], tg)
+
+
 def test_buffers_off_16_bytes(dk):
     h, da = inputs(3, 20, 64, torch.bfloat16)
 
