@@ -58,7 +58,7 @@ def _call(fn: str, device, *args):
         rc = f(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with on_device(device):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         check(fn, rc)
 
@@ -72,11 +72,11 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _same_device(like: torch.Tensor, **tensors) -> None:
-    dev = like.device
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must live on {dev} (got {t.device})")
+def _same_device(like: torch.Tensor, names: str, *tensors) -> None:
+    idx = like.get_device()
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"{names.split()[i]} must live on {like.device} (got {t.device})")
 
 
 def _wants_grad(*tensors) -> bool:
@@ -89,15 +89,18 @@ def _wants_grad(*tensors) -> bool:
 def _attention_inputs(q, k, v, g, valid, reset, state=None, state_name="initial"):
     """Checked inputs: (dtype code, sizes, views of q, k, v, g, valid, reset and what they look at)."""
     code = _dtype(q, "q")
-    if q.dim() != 4 or v.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4 or v.dim() != 4:
         raise ValueError("q must be [batch, time, head, key] and v [batch, time, head, value]")
-    B, T, H, K = q.shape
+    B, T, H, K = shape
     V = v.shape[3]
-    if k.shape != q.shape or v.shape[:3] != q.shape[:3]:
+    if k.shape != shape or v.shape != (B, T, H, V):
         raise ValueError("q, k, v must share [batch, time, head], and q and k the key width")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError("q, k and v must have one dtype")
-    if g.shape != (B, T, H) and g.shape != (H,):
+    gs = g.shape
+    if gs != (B, T, H) and gs != (H,):
         raise ValueError(f"g must have shape {(B, T, H)} or {(H,)} (got {tuple(g.shape)})")
     if valid is not None and valid.shape != (B, T):
         raise ValueError(f"valid must be [batch, time] (got {tuple(valid.shape)})")
@@ -106,8 +109,13 @@ def _attention_inputs(q, k, v, g, valid, reset, state=None, state_name="initial"
     if state is not None and state.shape != (B, H, K, V):
         raise ValueError(f"{state_name} must be [batch, head, key, value] (got "
                          f"{tuple(state.shape)})")
-    _same_device(q, k=k, v=v, g=g, valid=valid, reset=reset, **{state_name: state})
-    g, valid, reset = (m if m is None or m.dtype == F32 else m.to(F32) for m in (g, valid, reset))
+    _same_device(q, "k v g valid reset " + state_name, k, v, g, valid, reset, state)
+    if g.dtype != F32:
+        g = g.float()
+    if valid is not None and valid.dtype != F32:
+        valid = valid.float()
+    if reset is not None and reset.dtype != F32:
+        reset = reset.float()
     gv = _view(g) if g.dim() == 3 else _VIEW(g.data_ptr(), GDN2_F32, 0, 0, 0, g.stride(0), 0)
     views = (_view(q), _view(k), _view(v), gv, _view(valid), _view(reset))
     return code, (B, T, H, K, V), views, (g, valid, reset)
@@ -152,7 +160,7 @@ def linear_attention_backward(q, k, v, g, valid, reset, initial, checkpoint, d_o
         raise ValueError(f"d_output must have shape {tuple(v.shape)} (got {tuple(d_output.shape)})")
     if d_final_state is not None and d_final_state.shape != (B, H, K, V):
         raise ValueError("d_final_state must be [batch, head, key, value]")
-    _same_device(q, d_output=d_output, d_final_state=d_final_state, checkpoint=checkpoint)
+    _same_device(q, "d_output d_final_state checkpoint", d_output, d_final_state, checkpoint)
     if d_output.dtype != q.dtype:
         d_output = d_output.to(q.dtype)
     if d_final_state is not None:
@@ -250,12 +258,11 @@ def _ln_inputs(x, weight, bias):
     W = x.shape[-1] if x.dim() else 0
     if W < 1:
         raise ValueError("x must be [..., W] with W >= 1")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None and name == "bias":
-            continue
-        if t.dtype != F32 or t.shape != (W,):
-            raise ValueError(f"{name} must be float32 [{W}] (got {t.dtype} {tuple(t.shape)})")
-    _same_device(x, weight=weight, bias=bias)
+    for t in (weight, bias):
+        if t is not None and (t.dtype != F32 or t.shape != (W,)):
+            raise ValueError(f"{'weight' if t is weight else 'bias'} must be float32 [{W}] (got "
+                             f"{t.dtype} {tuple(t.shape)})")
+    _same_device(x, "weight bias", weight, bias)
     return weight.contiguous(), None if bias is None else bias.contiguous()
 
 
@@ -293,7 +300,7 @@ def layer_norm_backward(x, weight, mean, inverse, dy, want_bias: bool = True,
     for name, t in (("mean", mean), ("inverse", inverse)):
         if t.dtype != F32 or t.numel() != rows or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 [{rows}]")
-    _same_device(x, mean=mean, inverse=inverse, dy=dy)
+    _same_device(x, "mean inverse dy", mean, inverse, dy)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
     dw = torch.empty((W,), dtype=F32, device=dev) if want_weight else None
     db = torch.empty((W,), dtype=F32, device=dev) if want_bias else None
@@ -366,7 +373,7 @@ def swiglu_q8_backward(codes: torch.Tensor, exponents: torch.Tensor, da: torch.T
     _dense(da, "da", da.dtype, da.shape)
     _dense(codes, "codes", torch.int8, (rows, 2 * M))
     _dense(exponents, "exponents", torch.uint8, (rows, 2 * -(-M // Q8_BLOCK)))
-    _same_device(da, codes=codes, exponents=exponents)
+    _same_device(da, "codes exponents", codes, exponents)
     dh = torch.empty((rows, 2 * M), dtype=da.dtype, device=da.device)
     a = torch.empty((rows, M), dtype=da.dtype, device=da.device) if want_a else None
     _call("gdn2_swiglu_q8_backward", da.device, rows, M, code, codes.data_ptr(),
