@@ -20,7 +20,6 @@ namespace gdn2 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kPartials = 512;  // workgroups of the backward (fixed: the sums' order)
 
 struct LnArgs {
     View x, dy;
@@ -33,31 +32,39 @@ struct LnArgs {
     float *part_w, *part_b;
 };
 
-// N adjacent elements as floats.
-template <typename T, int N>
-__device__ __forceinline__ void load_n(const T *p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = Elem<T>::load(p, 0);
-    } else if constexpr (sizeof(T) == 2) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+// The elements of 16 bytes.
+template <typename T> constexpr int kPiece = 16 / (int)sizeof(T);
+
+// N adjacent elements as floats.  ALIGNED: whole pieces at 16-byte addresses.  Otherwise `left` of them are
+// there (the rest is 0), s elements apart; side by side they are read as one piece wherever it lies.
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void load_n(const T *p, int64_t s, int left, float (&v)[N]) {
+    T e[N];
+    if (ALIGNED) {
+        __builtin_memcpy(e, __builtin_assume_aligned(p, 16), sizeof e);
+    } else if (s == 1 && left >= N) {
+        __builtin_memcpy(e, p, sizeof e);
     } else {
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const float4 q = *reinterpret_cast<const float4 *>(p + j);
-            v[j] = q.x, v[j + 1] = q.y, v[j + 2] = q.z, v[j + 3] = q.w;
-        }
+        for (int i = 0; i < N; ++i) e[i] = i < left ? p[i * s] : T(0);
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Elem<T>::load(e, i);
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_n(T *p, const float (&v)[N]) {
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void store_n(T *p, int left, const float (&v)[N]) {
     T e[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) Elem<T>::store(e, i, v[i]);
-    __builtin_memcpy(__builtin_assume_aligned(p, N * sizeof(T)), e, sizeof e);
+    if (ALIGNED) {
+        __builtin_memcpy(__builtin_assume_aligned(p, 16), e, sizeof e);
+    } else if (left >= N) {
+        __builtin_memcpy(p, e, sizeof e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) p[i] = e[i];
+    }
 }
 
 template <int CTRL>
@@ -113,9 +120,9 @@ __device__ __forceinline__ int64_t row_at(const View &x, const LnArgs &p, int64_
 }
 
 // Columns of thread l, piece j: N adjacent ones from N (l + j G).
-template <typename T, int N, int G, int E>
+template <typename T, int G, int E, bool ALIGNED>
 struct Row {
-    static constexpr int P = E / N;
+    static constexpr int N = kPiece<T>, P = E / N;
     float v[P][N];
     __device__ __forceinline__ void load(const void *base, int64_t at, int64_t s, int l, int W) {
 #pragma unroll
@@ -123,34 +130,37 @@ struct Row {
             const int c = N * (l + j * G);
 #pragma unroll
             for (int e = 0; e < N; ++e) v[j][e] = 0.f;
-            if (c < W) load_n<T, N>(reinterpret_cast<const T *>(base) + at + c * (N == 1 ? s : 1), v[j]);
+            if (c < W) load_n<T, N, ALIGNED>(reinterpret_cast<const T *>(base) + at + c * (ALIGNED ? 1 : s), s, W - c, v[j]);
+        }
+    }
+    // The columns of a parameter.
+    __device__ __forceinline__ void params(const float *w, int l, int W) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int c = N * (l + j * G);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[j][e] = 0.f;
+            if (c < W) load_n<float, N, ALIGNED>(w + c, 1, W - c, v[j]);
         }
     }
 };
 
 // R rows a group at once, their loads and sums side by side.
-template <typename T, int N, int G, int E, int R>
+template <typename T, int G, int E, int R, bool ALIGNED>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel(LnArgs p) {
     constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
     __shared__ float red[R * (G > 64 ? G / 64 : 1)];
-    typedef Row<T, N, G, E> X;
+    typedef Row<T, G, E, ALIGNED> X;
+    constexpr int N = X::N;
     const int l = threadIdx.x % G;
     const int64_t r0 = ((int64_t)blockIdx.x * ROWS + threadIdx.x / G) * R;
     X x[R];
 #pragma unroll
     for (int i = 0; i < R; ++i)  // rows past the end read the last one again
         x[i].load(p.x.data, row_at(p.x, p, min(r0 + i, p.rows - 1)), p.x.s3, l, p.W);
-    float w[X::P][N], b[X::P][N];
-#pragma unroll
-    for (int j = 0; j < X::P; ++j) {
-        const int c = N * (l + j * G);
-#pragma unroll
-        for (int e = 0; e < N; ++e) w[j][e] = b[j][e] = 0.f;
-        if (c < p.W) {
-            load_n<float, N>(p.weight + c, w[j]);
-            if (p.bias) load_n<float, N>(p.bias + c, b[j]);
-        }
-    }
+    X w{}, b{};
+    w.params(p.weight, l, p.W);
+    if (p.bias) b.params(p.bias, l, p.W);
     float m[R], s[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -172,7 +182,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
                     x[i].v[j][e] -= m[i];
-                    s[i] = fmaf(x[i].v[j][e], x[i].v[j][e], s[i]);
+                    if (ALIGNED || N * (l + j * G) + e < p.W) s[i] = fmaf(x[i].v[j][e], x[i].v[j][e], s[i]);
                 }
     }
     row_sum<G, R>(s, red);
@@ -192,27 +202,27 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel
             if (c >= p.W) continue;
             float o[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = fmaf(x[i].v[j][e] * inv, w[j][e], b[j][e]);
-            store_n<T, N>(y + c, o);
+            for (int e = 0; e < N; ++e) o[e] = fmaf(x[i].v[j][e] * inv, w.v[j][e], b.v[j][e]);
+            store_n<T, N, ALIGNED>(y + c, p.W - c, o);
         }
     }
 }
 
-template <typename T, int N, int G, int E, int R>
+template <typename T, int G, int E, int R, bool ALIGNED>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kernel(LnArgs p) {
     constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
     __shared__ float red[2 * R * (G > 64 ? G / 64 : 1)];
     __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
-    typedef Row<T, N, G, E> X;
-    float w[X::P][N], dw[X::P][N], db[X::P][N];
+    typedef Row<T, G, E, ALIGNED> X;
+    constexpr int N = X::N;
+    X w;
+    w.params(p.weight, l, p.W);
+    float dw[X::P][N], db[X::P][N];
 #pragma unroll
-    for (int j = 0; j < X::P; ++j) {
-        const int c = N * (l + j * G);
+    for (int j = 0; j < X::P; ++j)
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[j][e] = dw[j][e] = db[j][e] = 0.f;
-        if (c < p.W) load_n<float, N>(p.weight + c, w[j]);
-    }
+        for (int e = 0; e < N; ++e) dw[j][e] = db[j][e] = 0.f;
     const float W = (float)p.W;
     // Every group of the workgroup makes the same number of turns: row_sum has barriers.
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS * R; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS * R) {
@@ -237,7 +247,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kerne
                         const float xh = (x[i].v[j][e] - m[i]) * inv[i], d = dy[i].v[j][e];
                         dw[j][e] = fmaf(d, xh, dw[j][e]);
                         db[j][e] += d;
-                        const float c = d * w[j][e];
+                        const float c = d * w.v[j][e];
                         s[2 * i] += c;
                         s[2 * i + 1] = fmaf(c, xh, s[2 * i + 1]);
                         x[i].v[j][e] = xh, dy[i].v[j][e] = c;
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kerne
                 float o[N];
 #pragma unroll
                 for (int e = 0; e < N; ++e) o[e] = inv[i] * ((dy[i].v[j][e] - a) - x[i].v[j][e] * c2);
-                store_n<T, N>(dx + c, o);
+                store_n<T, N, ALIGNED>(dx + c, p.W - c, o);
             }
         }
     }
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(1024) ln_sum_kernel(const float *pw, const flo
 constexpr int64_t kWide = 32768;  // wider rows do not fit the registers of one workgroup
 
 int64_t row_threads(int64_t W) {  // at most, as launch_width has them
-    return W <= 1024 ? 64 : W <= 8192 ? 256 : 1024;
+    return W <= 1024 ? 64 : W <= 4096 ? 256 : W <= 8192 ? 512 : 1024;
 }
 
 int check_ln(const gdn2_rows_shape *s, const gdn2_view *x, const float *weight) {
@@ -399,8 +409,8 @@ int check_ln(const gdn2_rows_shape *s, const gdn2_view *x, const float *weight) 
         return fail(GDN2_ERR_SHAPE, "at most 2^30 rows, and widths below 2^31");
     const int64_t rows = s->batch * s->time * s->heads;
     if (rows >= ((int64_t)1 << 32) / row_threads(s->width))  // threads of one launch
-        return fail(GDN2_ERR_SHAPE, "too many rows: at most 2^26 of up to 1024 columns, 2^24 of up to "
-                                    "8192 and 2^22 of wider ones");
+        return fail(GDN2_ERR_SHAPE, "too many rows: below 2^26 of up to 1024 columns, 2^24 of up to "
+                                    "4096, 2^23 of up to 8192 and 2^22 of wider ones");
     GDN2_TRY(check_view(x, "x", -1, rows == 0));
     if (!weight) return fail(GDN2_ERR_ARGUMENT, "weight is null");
     return GDN2_OK;
@@ -417,52 +427,56 @@ bool vec_rows(const gdn2_view *v, int64_t W) {
     return true;
 }
 
-// Rows at once: four (two in the backward) where that leaves eight waves for each of the 256 units.
-template <typename T, int N, int G, int E, bool BWD>
+// Rows at once: four (two in the backward) where that leaves eight waves for each of the 256 units and
+// a thread has eight columns (with 16, 65536 rows of 1024 took 140 us in place of 127 backward).
+template <typename T, int G, int E, bool BWD, bool ALIGNED>
 void launch_one(const LnArgs &a, int64_t partials, hipStream_t st) {
     constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G, R = BWD ? 2 : 4;
     const auto groups = [&](int r) { return (unsigned)((a.rows + ROWS * r - 1) / (ROWS * r)); };
-    const bool many = G <= 64 && a.rows * G >= (int64_t)R * 2048 * 64;
-    if constexpr (BWD) {
-        if constexpr (G <= 64 && E <= 8)
-            if (many) {
-                hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E, R>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
-                return;
-            }
-        hipLaunchKernelGGL((ln_backward_kernel<T, N, G, E, 1>), dim3((unsigned)partials), dim3(THREADS), 0, st, a);
-    } else {
-        if constexpr (G <= 64 && E <= 8)
-            if (many) {
-                hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E, R>), dim3(groups(R)), dim3(THREADS), 0, st, a);
-                return;
-            }
-        hipLaunchKernelGGL((ln_forward_kernel<T, N, G, E, 1>), dim3(groups(1)), dim3(THREADS), 0, st, a);
-    }
+    const bool many = a.rows * G >= (int64_t)R * 2048 * 64;
+    const dim3 block(THREADS);
+    if constexpr (G <= 64 && E <= 8)
+        if (many) {
+            if constexpr (BWD)
+                hipLaunchKernelGGL((ln_backward_kernel<T, G, E, R, ALIGNED>), dim3((unsigned)partials), block, 0, st, a);
+            else
+                hipLaunchKernelGGL((ln_forward_kernel<T, G, E, R, ALIGNED>), dim3(groups(R)), block, 0, st, a);
+            return;
+        }
+    if constexpr (BWD)
+        hipLaunchKernelGGL((ln_backward_kernel<T, G, E, 1, ALIGNED>), dim3((unsigned)partials), block, 0, st, a);
+    else
+        hipLaunchKernelGGL((ln_forward_kernel<T, G, E, 1, ALIGNED>), dim3(groups(1)), block, 0, st, a);
 }
 
-// Threads a row by its width, eight columns each while they fit a wave, more beyond.
-template <typename T, int N, bool BWD>
+// Threads a row by its width: eight columns each while they fit a wave, 16 up to 8192 columns.
+template <typename T, bool BWD, bool ALIGNED>
 void launch_width(const LnArgs &a, int64_t partials, hipStream_t st) {
-    if (a.W <= 64) launch_one<T, N, 8, 8, BWD>(a, partials, st);
-    else if (a.W <= 128) launch_one<T, N, 16, 8, BWD>(a, partials, st);
-    else if (a.W <= 256) launch_one<T, N, 32, 8, BWD>(a, partials, st);
-    else if (a.W <= 512) launch_one<T, N, 64, 8, BWD>(a, partials, st);
-    else if (a.W <= 1024) launch_one<T, N, 64, 16, BWD>(a, partials, st);
-    else if (a.W <= 2048) launch_one<T, N, 256, 8, BWD>(a, partials, st);
-    else if (a.W <= 8192) launch_one<T, N, 256, 32, BWD>(a, partials, st);
-    else launch_one<T, N, 1024, 32, BWD>(a, partials, st);
+    if (a.W <= 64) launch_one<T, 8, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 128) launch_one<T, 16, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 256) launch_one<T, 32, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 512) launch_one<T, 64, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 1024) launch_one<T, 64, 16, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 2048) launch_one<T, 256, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 4096) launch_one<T, 256, 16, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 8192) launch_one<T, 512, 16, BWD, ALIGNED>(a, partials, st);
+    else launch_one<T, 1024, 32, BWD, ALIGNED>(a, partials, st);
 }
 
 template <bool BWD>
 void launch_ln(const LnArgs &a, int dtype, bool vec, int64_t partials, hipStream_t st) {
     const bool bf = dtype == GDN2_BF16;
-    if (vec && bf) launch_width<bf16_t, 8, BWD>(a, partials, st);
-    else if (vec) launch_width<float, 4, BWD>(a, partials, st);
-    else if (bf) launch_width<bf16_t, 1, BWD>(a, partials, st);
-    else launch_width<float, 1, BWD>(a, partials, st);
+    if (vec && bf) launch_width<bf16_t, BWD, true>(a, partials, st);
+    else if (vec) launch_width<float, BWD, true>(a, partials, st);
+    else if (bf) launch_width<bf16_t, BWD, false>(a, partials, st);
+    else launch_width<float, BWD, false>(a, partials, st);
 }
 
-int64_t partial_rows(int64_t rows) { return std::max<int64_t>(1, std::min(rows, kPartials)); }
+// Workgroups of the backward, each of which writes a row of column sums: by the sizes alone, as the order
+// of the sums goes by them.  Many rows are walked by more; the sums of wide rows weigh as much as the rows.
+int64_t partial_rows(int64_t rows, int64_t W) {
+    return std::max<int64_t>(1, std::min<int64_t>(rows, W > 8192 ? 256 : rows >= 32768 ? 1024 : 512));
+}
 
 }  // namespace
 }  // namespace gdn2
@@ -498,7 +512,7 @@ int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon, const g
 
 size_t gdn2_layer_norm_workspace_bytes(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1) return 0;
-    return (size_t)(2 * 4 * partial_rows(rows) * width);
+    return (size_t)(2 * 4 * partial_rows(rows, width) * width);
 }
 
 int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, const float *weight,
@@ -511,7 +525,7 @@ int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, c
     GDN2_TRY(check_view(dy, "dy", x->dtype, a.rows == 0));
     if (a.rows && (!mean || !inverse)) return fail(GDN2_ERR_ARGUMENT, "mean and inverse must be non-null");
     a.W = (int)shape->width;
-    const int64_t n = partial_rows(a.rows);
+    const int64_t n = partial_rows(a.rows, a.W);
     const bool params = dweight || dbias;
     if (params) {
         if (!workspace || workspace_bytes < gdn2_layer_norm_workspace_bytes(a.rows, a.W))

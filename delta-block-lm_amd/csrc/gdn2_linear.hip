@@ -241,6 +241,10 @@ struct Staged {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const T *q = base + (int64_t)min(row + i * ROWS, left - 1) * s1;
+                if (s3 == 1 && c + N <= width) {  // a whole piece, wherever it lies
+                    __builtin_memcpy(&r[i], q + c, 16);
+                    continue;
+                }
                 T e[N];
 #pragma unroll
                 for (int j = 0; j < N; ++j) e[j] = c + j < width ? q[(int64_t)(c + j) * s3] : T(0);

@@ -62,8 +62,15 @@ __device__ __forceinline__ void load8(const T *p, uint32_t c, uint32_t M, int ve
         }
         return;
     }
+    T e[8];
+    if (c + 8 <= M) {  // a whole piece, wherever it lies
+        __builtin_memcpy(e, p + c, sizeof e);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < M ? Elem<T>::load(p, c + i) : 0.f;
+        for (int i = 0; i < 8; ++i) e[i] = c + i < M ? p[c + i] : T(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(e, i);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T *p, uint32_t c, uint32_t M, int vec, const float (&v)[8]) {
@@ -72,6 +79,10 @@ __device__ __forceinline__ void store8(T *p, uint32_t c, uint32_t M, int vec, co
     for (int i = 0; i < 8; ++i) Elem<T>::store(e, i, v[i]);
     if (vec) {
         __builtin_memcpy(__builtin_assume_aligned(p + c, 16), e, sizeof e);
+        return;
+    }
+    if (c + 8 <= M) {
+        __builtin_memcpy(p + c, e, sizeof e);
         return;
     }
 #pragma unroll
@@ -107,6 +118,10 @@ __device__ __forceinline__ void put_codes(int8_t *p, uint32_t c, uint32_t M, int
         *reinterpret_cast<uint2 *>(p + c) = make_uint2(w[0], w[1]);
         return;
     }
+    if (c + 8 <= M) {
+        __builtin_memcpy(p + c, w, sizeof w);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (c + i < M) p[c + i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
@@ -114,11 +129,12 @@ __device__ __forceinline__ void put_codes(int8_t *p, uint32_t c, uint32_t M, int
 __device__ __forceinline__ void get_values(const int8_t *p, uint32_t c, uint32_t M, int vec, int ex,
                                            float (&v)[8]) {
     const float s = ex == kNan ? __builtin_nanf("") : power(ex);
-    if (vec) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p + c);
+    if (vec || c + 8 <= M) {
+        uint32_t w[2];
+        if (vec) __builtin_memcpy(w, __builtin_assume_aligned(p + c, 8), sizeof w);
+        else __builtin_memcpy(w, p + c, sizeof w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i % 4))) * s;
+        for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * s;
         return;
     }
 #pragma unroll

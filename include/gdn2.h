@@ -575,7 +575,8 @@ GDN2_API int gdn2_linear_step(const gdn2_shape *shape, const gdn2_view *q, const
  * NULL); y and dx dense in x's dtype; mean, inverse [rows] F32 (the forward takes
  * NULL where no backward follows).  dx, dweight, dbias may each be NULL.  dweight
  * and dbias are summed in a fixed order through the workspace.  Widths up to 2^25;
- * up to 2^26 rows of up to 1024 columns, 2^24 of up to 8192, 2^22 of wider ones. */
+ * below 2^26 rows of up to 1024 columns, 2^24 of up to 4096, 2^23 of up to 8192 and
+ * 2^22 of wider ones. */
 GDN2_API int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon,
                                      const gdn2_view *x, const float *weight, const float *bias,
                                      void *y, float *mean, float *inverse, void *stream);
