@@ -6,9 +6,10 @@
 //
 // Bound by memory: x is read once and kept in registers between the statistics (the variance about
 // the mean, not a difference of squares) and the result.  G threads share a row, E columns each, the
-// fewest that hold it: eight rows a wave at width 64, one at 512, a whole workgroup at 8192.  Rows
+// fewest that hold it: eight rows a wave at width 64, one at 512, a workgroup of 512 at 8192.  Rows
 // wider than 32768 are read again for each pass.  The backward's workgroups walk over rows with the
-// column sums in registers and write one partial row each, added up in a fixed order by a second launch.
+// column sums in registers and write one partial row each, added up in a fixed order by a second launch;
+// rows wider than 8192 are read again for their column sums.
 #include <math.h>
 
 #include <algorithm>
@@ -32,14 +33,17 @@ struct LnArgs {
     float *part_w, *part_b;
 };
 
+// Threads of a workgroup whose rows have G each: a row of more than one wave has a workgroup of its own.
+template <int G> constexpr int kGroup = G > 64 ? G : kThreads;
+
 // The elements of 16 bytes.
 template <typename T> constexpr int kPiece = 16 / (int)sizeof(T);
 
-// N adjacent elements as floats.  ALIGNED: whole pieces at 16-byte addresses.  Otherwise `left` of them are
-// there (the rest is 0), s elements apart; side by side they are read as one piece wherever it lies.
+// N adjacent elements, as they are or as floats.  ALIGNED: whole pieces at 16-byte addresses.  Otherwise
+// `left` of them are there (the rest is 0), s elements apart; side by side they are read as one piece
+// wherever it lies.
 template <typename T, int N, bool ALIGNED>
-__device__ __forceinline__ void load_n(const T *p, int64_t s, int left, float (&v)[N]) {
-    T e[N];
+__device__ __forceinline__ void fetch_n(const T *p, int64_t s, int left, T (&e)[N]) {
     if (ALIGNED) {
         __builtin_memcpy(e, __builtin_assume_aligned(p, 16), sizeof e);
     } else if (s == 1 && left >= N) {
@@ -48,6 +52,11 @@ __device__ __forceinline__ void load_n(const T *p, int64_t s, int left, float (&
 #pragma unroll
         for (int i = 0; i < N; ++i) e[i] = i < left ? p[i * s] : T(0);
     }
+}
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ void load_n(const T *p, int64_t s, int left, float (&v)[N]) {
+    T e[N];
+    fetch_n<T, N, ALIGNED>(p, s, left, e);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = Elem<T>::load(e, i);
 }
@@ -119,99 +128,105 @@ __device__ __forceinline__ int64_t row_at(const View &x, const LnArgs &p, int64_
     return (int64_t)(bt / T) * x.s0 + (int64_t)(bt % T) * x.s1 + (int64_t)h * x.s2;
 }
 
-// Columns of thread l, piece j: N adjacent ones from N (l + j G).
+// Columns of thread l, piece j: N adjacent ones from N (l + j G).  Pieces past the width read the row's first
+// one in their place and become zero afterwards: under a condition each load would wait for the one before.
 template <typename T, int G, int E, bool ALIGNED>
 struct Row {
     static constexpr int N = kPiece<T>, P = E / N;
+    typedef T Raw[P][N];
     float v[P][N];
-    __device__ __forceinline__ void load(const void *base, int64_t at, int64_t s, int l, int W) {
+    static __device__ __forceinline__ void fetch(Raw &r, const void *base, int64_t at, int64_t s, int l, int W) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const int c = N * (l + j * G);
+            const int c = N * (l + j * G), k = c < W ? c : 0;
+            fetch_n<T, N, ALIGNED>(reinterpret_cast<const T *>(base) + at + k * (ALIGNED ? 1 : s), s, W - k, r[j]);
+        }
+    }
+    __device__ __forceinline__ void take(const Raw &r, bool on, int l, int W) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[j][e] = 0.f;
-            if (c < W) load_n<T, N, ALIGNED>(reinterpret_cast<const T *>(base) + at + c * (ALIGNED ? 1 : s), s, W - c, v[j]);
+        for (int j = 0; j < P; ++j) {
+            uint4 q;
+            __builtin_memcpy(&q, r[j], 16);
+            if (!(on && N * (l + j * G) < W)) q = make_uint4(0, 0, 0, 0);
+            T e[N];
+            __builtin_memcpy(e, &q, 16);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[j][i] = Elem<T>::load(e, i);
         }
     }
     // The columns of a parameter.
     __device__ __forceinline__ void params(const float *w, int l, int W) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            const int c = N * (l + j * G);
+            const int c = N * (l + j * G), k = c < W ? c : 0;
+            load_n<float, N, ALIGNED>(w + k, 1, W - k, v[j]);
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[j][e] = 0.f;
-            if (c < W) load_n<float, N, ALIGNED>(w + c, 1, W - c, v[j]);
+            for (int e = 0; e < N; ++e) v[j][e] = c < W ? v[j][e] : 0.f;
         }
     }
 };
 
-// R rows a group at once, their loads and sums side by side.
-template <typename T, int G, int E, int R, bool ALIGNED>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_forward_kernel(LnArgs p) {
-    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
-    __shared__ float red[R * (G > 64 ? G / 64 : 1)];
+// One row a group of G threads.  Bound by memory: bf16 rows read and written, 8192 of 512 columns 5.6 us
+// (3.0 TB/s, much of it the launch), 65536 of 512 23 us (5.8 TB/s), of 1024 42 us (6.4 TB/s); 65536 f32 rows
+// of 64 7.2 us (4.7 TB/s).
+template <typename T, int G, int E, bool ALIGNED>
+__global__ void __launch_bounds__(kGroup<G>) ln_forward_kernel(LnArgs p) {
+    constexpr int THREADS = kGroup<G>, ROWS = THREADS / G;
+    __shared__ float red[G > 64 ? G / 64 : 1];
     typedef Row<T, G, E, ALIGNED> X;
     constexpr int N = X::N;
     const int l = threadIdx.x % G;
-    const int64_t r0 = ((int64_t)blockIdx.x * ROWS + threadIdx.x / G) * R;
-    X x[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i)  // rows past the end read the last one again
-        x[i].load(p.x.data, row_at(p.x, p, min(r0 + i, p.rows - 1)), p.x.s3, l, p.W);
-    X w{}, b{};
+    const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
+    typename X::Raw raw;  // a row past the end reads the last one again: row_sum has barriers
+    X::fetch(raw, p.x.data, row_at(p.x, p, min(r, p.rows - 1)), p.x.s3, l, p.W);
+    X x, w{}, b{};
     w.params(p.weight, l, p.W);
     if (p.bias) b.params(p.bias, l, p.W);
-    float m[R], s[R];
+    x.take(raw, true, l, p.W);
+    float s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        m[i] = 0.f;
+    for (int j = 0; j < X::P; ++j)
 #pragma unroll
-        for (int j = 0; j < X::P; ++j)
+        for (int e = 0; e < N; ++e) s[0] += x.v[j][e];
+    row_sum<G, 1>(s, red);
+    const float W = (float)p.W, m = s[0] / W;
+    s[0] = 0.f;
 #pragma unroll
-            for (int e = 0; e < N; ++e) m[i] += x[i].v[j][e];
+    for (int j = 0; j < X::P; ++j)
+        if (N * (l + j * G) < p.W)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                x.v[j][e] -= m;
+                if (ALIGNED || N * (l + j * G) + e < p.W) s[0] = fmaf(x.v[j][e], x.v[j][e], s[0]);
+            }
+    row_sum<G, 1>(s, red);
+    if (r >= p.rows) return;
+    const float inv = 1.f / sqrtf(s[0] / W + p.epsilon);
+    if (l == 0) {
+        if (p.mean) p.mean[r] = m;
+        if (p.inverse) p.inverse[r] = inv;
     }
-    row_sum<G, R>(m, red);
-    const float W = (float)p.W;
+    T *y = reinterpret_cast<T *>(p.y) + r * p.W;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        m[i] /= W;
-        s[i] = 0.f;
+    for (int j = 0; j < X::P; ++j) {
+        const int c = N * (l + j * G);
+        if (c >= p.W) continue;
+        float o[N];
 #pragma unroll
-        for (int j = 0; j < X::P; ++j)
-            if (N * (l + j * G) < p.W)
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    x[i].v[j][e] -= m[i];
-                    if (ALIGNED || N * (l + j * G) + e < p.W) s[i] = fmaf(x[i].v[j][e], x[i].v[j][e], s[i]);
-                }
-    }
-    row_sum<G, R>(s, red);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t r = r0 + i;
-        if (r >= p.rows) break;
-        const float inv = 1.f / sqrtf(s[i] / W + p.epsilon);
-        if (l == 0) {
-            if (p.mean) p.mean[r] = m[i];
-            if (p.inverse) p.inverse[r] = inv;
-        }
-        T *y = reinterpret_cast<T *>(p.y) + r * p.W;
-#pragma unroll
-        for (int j = 0; j < X::P; ++j) {
-            const int c = N * (l + j * G);
-            if (c >= p.W) continue;
-            float o[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = fmaf(x[i].v[j][e] * inv, w.v[j][e], b.v[j][e]);
-            store_n<T, N, ALIGNED>(y + c, p.W - c, o);
-        }
+        for (int e = 0; e < N; ++e) o[e] = fmaf(x.v[j][e] * inv, w.v[j][e], b.v[j][e]);
+        store_n<T, N, ALIGNED>(y + c, p.W - c, o);
     }
 }
 
-template <typename T, int G, int E, int R, bool ALIGNED>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kernel(LnArgs p) {
-    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G;
-    __shared__ float red[2 * R * (G > 64 ? G / 64 : 1)];
+// dx, and for rows up to 8192 the column sums of the workgroup's rows.  Wider ones leave no registers for
+// the sums (2000 bf16 rows of 32768 columns: 336 us with them, 165 with ln_columns).  Bound by memory: bf16
+// rows, x and dy read and dx written, with ln_sum_kernel: 8192 of 512 columns 11.4 us (2.2 TB/s, much of it
+// the launches), 65536 of 512 37 us (5.5 TB/s), of 1024 81 us (5.0 TB/s); 65536 f32 rows of 64 14 us.
+template <typename T, int G, int E, bool ALIGNED>
+__global__ void __launch_bounds__(kGroup<G>) ln_backward_kernel(LnArgs p) {
+    constexpr int THREADS = kGroup<G>, ROWS = THREADS / G;
+    constexpr bool SUMS = G <= 512, AHEAD = SUMS && ALIGNED;
+    __shared__ float red[2 * (G > 64 ? G / 64 : 1)];
     __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
     typedef Row<T, G, E, ALIGNED> X;
@@ -224,54 +239,55 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) ln_backward_kerne
 #pragma unroll
         for (int e = 0; e < N; ++e) dw[j][e] = db[j][e] = 0.f;
     const float W = (float)p.W;
-    // Every group of the workgroup makes the same number of turns: row_sum has barriers.
-    for (int64_t r0 = (int64_t)blockIdx.x * ROWS * R; r0 < p.rows; r0 += (int64_t)gridDim.x * ROWS * R) {
-        X x[R], dy[R];
-        float m[R], inv[R], s[2 * R];
+    // Every group of the workgroup makes the same number of turns: row_sum has barriers.  The next row is on
+    // its way while one is worked on (not for rows off 16 bytes, whose loads have branches: 65536 bf16 rows of
+    // 999 took 177 us instead of 124); past the end the last row is read again and adds nothing.
+    typename X::Raw rx, rdy;
+    float rm, rinv;
+    const auto fetch = [&](int64_t r) {
+        r = min(r, p.rows - 1);
+        X::fetch(rx, p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
+        X::fetch(rdy, p.dy.data, row_at(p.dy, p, r), p.dy.s3, l, p.W);
+        rm = p.mean[r], rinv = p.inverse[r];
+    };
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t r = (int64_t)blockIdx.x * ROWS + g;
+    if (AHEAD) fetch(r);
+    for (; r - g < p.rows; r += step) {
+        const bool on = r < p.rows;
+        if (!AHEAD) fetch(r);
+        X x, dy;
+        x.take(rx, on, l, p.W);
+        dy.take(rdy, on, l, p.W);
+        const float m = on ? rm : 0.f, inv = on ? rinv : 0.f;
+        if (AHEAD) fetch(r + step);
+        float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int64_t r = min(r0 + g * R + i, p.rows - 1);
-            x[i].load(p.x.data, row_at(p.x, p, r), p.x.s3, l, p.W);
-            dy[i].load(p.dy.data, row_at(p.dy, p, r), p.dy.s3, l, p.W);
-            m[i] = p.mean[r], inv[i] = p.inverse[r];
-        }
+        for (int j = 0; j < X::P; ++j)
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            s[2 * i] = s[2 * i + 1] = 0.f;
-            const bool on = r0 + g * R + i < p.rows;  // the others add nothing
-#pragma unroll
-            for (int j = 0; j < X::P; ++j)
-                if (on && N * (l + j * G) < p.W)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float xh = (x[i].v[j][e] - m[i]) * inv[i], d = dy[i].v[j][e];
-                        dw[j][e] = fmaf(d, xh, dw[j][e]);
-                        db[j][e] += d;
-                        const float c = d * w.v[j][e];
-                        s[2 * i] += c;
-                        s[2 * i + 1] = fmaf(c, xh, s[2 * i + 1]);
-                        x[i].v[j][e] = xh, dy[i].v[j][e] = c;
-                    }
-        }
-        row_sum<G, 2 * R>(s, red);
-        if (!p.y) continue;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int64_t r = r0 + g * R + i;
-            if (r >= p.rows) break;
-            const float a = s[2 * i] / W, c2 = s[2 * i + 1] / W;
-            T *dx = reinterpret_cast<T *>(p.y) + r * p.W;
-#pragma unroll
-            for (int j = 0; j < X::P; ++j) {
-                const int c = N * (l + j * G);
-                if (c >= p.W) continue;
-                float o[N];
-#pragma unroll
-                for (int e = 0; e < N; ++e) o[e] = inv[i] * ((dy[i].v[j][e] - a) - x[i].v[j][e] * c2);
-                store_n<T, N, ALIGNED>(dx + c, p.W - c, o);
+            for (int e = 0; e < N; ++e) {
+                const float xh = (x.v[j][e] - m) * inv, d = dy.v[j][e];
+                if (SUMS) dw[j][e] = fmaf(d, xh, dw[j][e]), db[j][e] += d;
+                const float c = d * w.v[j][e];
+                s[0] += c;
+                s[1] = fmaf(c, xh, s[1]);
+                x.v[j][e] = xh, dy.v[j][e] = c;
             }
+        row_sum<G, 2>(s, red);
+        if (!p.y || !on) continue;
+        const float a = s[0] / W, c2 = s[1] / W;
+        T *dx = reinterpret_cast<T *>(p.y) + r * p.W;
+#pragma unroll
+        for (int j = 0; j < X::P; ++j) {
+            const int c = N * (l + j * G);
+            if (c >= p.W) continue;
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = inv * ((dy.v[j][e] - a) - x.v[j][e] * c2);
+            store_n<T, N, ALIGNED>(dx + c, p.W - c, o);
         }
     }
+    if constexpr (!SUMS) return;
     // The workgroup's column sums, over its groups in order.
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -353,20 +369,32 @@ __global__ void __launch_bounds__(kLong) ln_backward_long(LnArgs p) {
     }
 }
 
-// Column sums of wide rows: 256 columns and every gridDim.y-th row a workgroup.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) ln_columns_long(LnArgs p) {
-    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+// Column sums of wide rows: a piece of columns a thread and every gridDim.y-th row.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) ln_columns(LnArgs p) {
+    constexpr int N = kPiece<T>;
+    const int64_t c = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * N;
     if (c >= p.W) return;
-    float dw = 0.f, db = 0.f;
+    const int left = (int)(p.W - c);
+    float dw[N], db[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) dw[e] = db[e] = 0.f;
+#pragma unroll 2
     for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
-        const float d = Elem<T>::load(p.dy.data, row_at(p.dy, p, r) + c * p.dy.s3);
-        const float x = Elem<T>::load(p.x.data, row_at(p.x, p, r) + c * p.x.s3);
-        dw = fmaf(d, (x - p.mean[r]) * p.inverse[r], dw);
-        db += d;
+        float x[N], d[N];
+        load_n<T, N, ALIGNED>(reinterpret_cast<const T *>(p.x.data) + row_at(p.x, p, r) + c * p.x.s3, p.x.s3, left, x);
+        load_n<T, N, ALIGNED>(reinterpret_cast<const T *>(p.dy.data) + row_at(p.dy, p, r) + c * p.dy.s3, p.dy.s3, left, d);
+        const float m = p.mean[r], inv = p.inverse[r];
+#pragma unroll
+        for (int e = 0; e < N; ++e) dw[e] = fmaf(d[e], (x[e] - m) * inv, dw[e]), db[e] += d[e];
     }
-    if (p.part_w) p.part_w[(int64_t)blockIdx.y * p.W + c] = dw;
-    if (p.part_b) p.part_b[(int64_t)blockIdx.y * p.W + c] = db;
+    const int64_t at = (int64_t)blockIdx.y * p.W + c;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (e >= left) break;
+        if (p.part_w) p.part_w[at + e] = dw[e];
+        if (p.part_b) p.part_b[at + e] = db[e];
+    }
 }
 
 // Partial rows -> dweight (blockIdx.y 0) and dbias (1): 16 columns a workgroup, 64 threads of each over
@@ -393,9 +421,10 @@ __global__ void __launch_bounds__(1024) ln_sum_kernel(const float *pw, const flo
     }
 }
 
-constexpr int64_t kWide = 32768;  // wider rows do not fit the registers of one workgroup
+constexpr int64_t kWide = 32768;  // wider rows do not fit the registers of one workgroup,
+constexpr int64_t kSums = 8192;   // nor wider ones than this their column sums too
 
-int64_t row_threads(int64_t W) {  // at most, as launch_width has them
+int64_t row_threads(int64_t W) {  // at most, where a row has a group of its own in the grid
     return W <= 1024 ? 64 : W <= 4096 ? 256 : W <= 8192 ? 512 : 1024;
 }
 
@@ -427,40 +456,43 @@ bool vec_rows(const gdn2_view *v, int64_t W) {
     return true;
 }
 
-// Rows at once: four (two in the backward) where that leaves eight waves for each of the 256 units and
-// a thread has eight columns (with 16, 65536 rows of 1024 took 140 us in place of 127 backward).
 template <typename T, int G, int E, bool BWD, bool ALIGNED>
 void launch_one(const LnArgs &a, int64_t partials, hipStream_t st) {
-    constexpr int THREADS = G > kThreads ? G : kThreads, ROWS = THREADS / G, R = BWD ? 2 : 4;
-    const auto groups = [&](int r) { return (unsigned)((a.rows + ROWS * r - 1) / (ROWS * r)); };
-    const bool many = a.rows * G >= (int64_t)R * 2048 * 64;
-    const dim3 block(THREADS);
-    if constexpr (G <= 64 && E <= 8)
-        if (many) {
-            if constexpr (BWD)
-                hipLaunchKernelGGL((ln_backward_kernel<T, G, E, R, ALIGNED>), dim3((unsigned)partials), block, 0, st, a);
-            else
-                hipLaunchKernelGGL((ln_forward_kernel<T, G, E, R, ALIGNED>), dim3(groups(R)), block, 0, st, a);
-            return;
-        }
-    if constexpr (BWD)
-        hipLaunchKernelGGL((ln_backward_kernel<T, G, E, 1, ALIGNED>), dim3((unsigned)partials), block, 0, st, a);
-    else
-        hipLaunchKernelGGL((ln_forward_kernel<T, G, E, 1, ALIGNED>), dim3(groups(1)), block, 0, st, a);
+    constexpr int THREADS = kGroup<G>, ROWS = THREADS / G;
+    const dim3 block(THREADS), every((unsigned)((a.rows + ROWS - 1) / ROWS));
+    if constexpr (!BWD) {
+        hipLaunchKernelGGL((ln_forward_kernel<T, G, E, ALIGNED>), every, block, 0, st, a);
+    } else if constexpr (G <= 512) {
+        hipLaunchKernelGGL((ln_backward_kernel<T, G, E, ALIGNED>), dim3((unsigned)partials), block, 0, st, a);
+    } else if (a.y) {
+        hipLaunchKernelGGL((ln_backward_kernel<T, G, E, ALIGNED>), every, block, 0, st, a);
+    }
 }
 
-// Threads a row by its width: eight columns each while they fit a wave, 16 up to 8192 columns.
+// Threads a row by its width: 8 columns a thread up to 512 (the forward 16 from 257 on), 16 up to 8192 (the
+// backward 8 from 1025 to 2048).  bf16 forward and backward with the one and the other: 65536 rows of 512 25 and
+// 37 us with 64 x 8, 22 and 39 with 32 x 16; of 1024 41 and 82 with 64 x 16, 48 and 129 with 128 x 8; 20000 of
+// 2048 26 and 61 with 128 x 16, 30 and 52 with 256 x 8; 16384 of 4096 46 and 88 with 256 x 16, 55 and 88 with
+// 512 x 8.
 template <typename T, bool BWD, bool ALIGNED>
 void launch_width(const LnArgs &a, int64_t partials, hipStream_t st) {
     if (a.W <= 64) launch_one<T, 8, 8, BWD, ALIGNED>(a, partials, st);
     else if (a.W <= 128) launch_one<T, 16, 8, BWD, ALIGNED>(a, partials, st);
     else if (a.W <= 256) launch_one<T, 32, 8, BWD, ALIGNED>(a, partials, st);
-    else if (a.W <= 512) launch_one<T, 64, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 512) launch_one<T, BWD ? 64 : 32, BWD ? 8 : 16, BWD, ALIGNED>(a, partials, st);
     else if (a.W <= 1024) launch_one<T, 64, 16, BWD, ALIGNED>(a, partials, st);
-    else if (a.W <= 2048) launch_one<T, 256, 8, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= 2048) launch_one<T, BWD ? 256 : 128, BWD ? 8 : 16, BWD, ALIGNED>(a, partials, st);
     else if (a.W <= 4096) launch_one<T, 256, 16, BWD, ALIGNED>(a, partials, st);
-    else if (a.W <= 8192) launch_one<T, 512, 16, BWD, ALIGNED>(a, partials, st);
+    else if (a.W <= kSums) launch_one<T, 512, 16, BWD, ALIGNED>(a, partials, st);
     else launch_one<T, 1024, 32, BWD, ALIGNED>(a, partials, st);
+}
+
+template <typename T>
+void launch_columns(const LnArgs &a, bool vec, int64_t partials, hipStream_t st) {
+    const int64_t each = kThreads * kPiece<T>;
+    const dim3 grid((unsigned)((a.W + each - 1) / each), (unsigned)partials);
+    if (vec) hipLaunchKernelGGL((ln_columns<T, true>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((ln_columns<T, false>), grid, dim3(kThreads), 0, st, a);
 }
 
 template <bool BWD>
@@ -473,9 +505,12 @@ void launch_ln(const LnArgs &a, int dtype, bool vec, int64_t partials, hipStream
 }
 
 // Workgroups of the backward, each of which writes a row of column sums: by the sizes alone, as the order
-// of the sums goes by them.  Many rows are walked by more; the sums of wide rows weigh as much as the rows.
+// of the sums goes by them.  512 (1024: 65536 bf16 rows of 1024 88 us in place of 81, 8192 of 8192 130 in place
+// of 100); 1024 for many rows of widths whose rows start off 16 bytes, which have no row ahead on its way
+// (65536 of 999 118 us, with 512 174); of wide rows fewer, whose sums would weigh as much as they (2000 of
+// 32768 165 us, with 128 178).
 int64_t partial_rows(int64_t rows, int64_t W) {
-    return std::max<int64_t>(1, std::min<int64_t>(rows, W > 8192 ? 256 : rows >= 32768 ? 1024 : 512));
+    return std::max<int64_t>(1, std::min<int64_t>(rows, W > kSums ? 64 : rows >= 32768 && W % 8 ? 1024 : 512));
 }
 
 }  // namespace
@@ -544,20 +579,18 @@ int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, c
         a.part_b = dbias ? ws + n * a.W : nullptr;
     }
     hipStream_t st = (hipStream_t)stream;
-    const bool bf = x->dtype == GDN2_BF16;
+    const bool bf = x->dtype == GDN2_BF16, vec = vec_rows(x, a.W) && vec_rows(dy, a.W);
     if (a.rows && a.W > kWide) {
         if (dx) {
             if (bf) hipLaunchKernelGGL((ln_backward_long<bf16_t>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
             else hipLaunchKernelGGL((ln_backward_long<float>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
         }
-        if (params) {
-            const dim3 grid((unsigned)((a.W + (int64_t)kThreads - 1) / kThreads), (unsigned)n);
-            if (bf) hipLaunchKernelGGL((ln_columns_long<bf16_t>), grid, dim3(kThreads), 0, st, a);
-            else hipLaunchKernelGGL((ln_columns_long<float>), grid, dim3(kThreads), 0, st, a);
-        }
     } else if (a.rows && (dx || params)) {
-        launch_ln<true>(a, x->dtype,
-                        vec_rows(x, a.W) && vec_rows(dy, a.W) && aligned(dx) && aligned(weight), n, st);
+        launch_ln<true>(a, x->dtype, vec && aligned(dx) && aligned(weight), n, st);
+    }
+    if (a.rows && params && a.W > kSums) {
+        if (bf) launch_columns<bf16_t>(a, vec, n, st);
+        else launch_columns<float>(a, vec, n, st);
     }
     if (params)
         hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((a.W + (int64_t)15) / 16), 2), dim3(1024), 0, st,
