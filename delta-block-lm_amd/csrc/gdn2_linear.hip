@@ -109,6 +109,7 @@ struct Walk {
     int64_t s_bh;
     int s_row, s_col;
     float *starts_out;      // the prewalk's states before every segment, or null
+    float *kept;            // states before every chunk and after the last, [B H, chunks + 1] kept forms, or null
     float *fin;             // state after the walk, [B H, rows, columns], or null
     int64_t T;
     int H;
@@ -130,7 +131,8 @@ struct Forward : Walk {
 struct Back : Walk {
     View q, k, v, o;        // o: the output's gradient
     int K, V;
-    void *dk, *dv;          // dense, or null
+    void *dq, *dk, *dv;     // dense, or null (dq: all in one)
+    float *dg;              // dense [B, T, H], or null (all in one)
     View edge_first;        // with DOT: the forward's states, its first one
     const float *edge;      // and those before the other segments
     float *y;               // [B H, T]: see DOT
@@ -358,7 +360,7 @@ struct WalkLds {
     float rows[C / 16][C], cols[C / 16][C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
-template <typename T, int KP, int VP>
+template <typename T, int KP, int VP, bool ALL>
 struct BackLds {
     static constexpr int C = Mat<T>::C, LDK = KP + Mat<T>::PAD, LDV = VP + Mat<T>::PAD,
                          LDP = C + Mat<T>::PAD, NW = (KP > VP ? KP : VP) / 16;
@@ -366,13 +368,17 @@ struct BackLds {
     T pk[C * LDP], pv[C * LDP];  // Gam k.q and Gam v.do; the token-by-token form keeps float sums in pk
     T D[VP * LDK];               // the adjoint state transposed, [value][key]
     GateTile<C> gate[kGates];
-    float red[NW][C];
+    float red[NW][C], red_q[ALL ? NW : 1][C];
+    float rows[ALL ? C / 16 : 1][C], cols[ALL ? C / 16 : 1][C];  // parts of the pair sums, as in WalkLds
     int bad[2];                  // whether any wave's state is not finite, in turn for even and odd chunks
 };
 
 // Holds a loaded value where it is: the compiler otherwise moves each load under the condition that
 // selects it, one after the other, and waits for every one.
 __device__ __forceinline__ void keep(float &x) { asm volatile("" : "+v"(x)); }
+
+__host__ __device__ inline int up16(int n) { return (n + 15) & ~15; }
+__host__ __device__ inline int64_t kept_size(int rows, int cols) { return (int64_t)up16(rows) * up16(cols); }
 
 // State of one wave: 16 columns, accumulator tiles of 16 rows.
 template <int KT>
@@ -411,6 +417,33 @@ struct State {
                 keep(x);
                 t[m][i] = 16 * m + g4 + i < ka && v < vc ? x : 0.f;
             }
+    }
+    // The kept form of a whole state: [columns][rows], both rounded up to 16.
+    __device__ __forceinline__ void keep_at(float *dst, int v, int rows, int cols) const {
+        if ((v & ~15) >= cols) return;
+        dst += v * rows + 4 * (lane_id() >> 4);
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+            if (16 * m < rows) *reinterpret_cast<f32x4 *>(dst + 16 * m) = t[m];
+    }
+    // A kept state as it was (the loads are only issued), or its transpose: columns and rows change places.
+    __device__ __forceinline__ void load_kept(const float *src, int v, int rows, int cols) {
+        zero();
+        if ((v & ~15) >= cols) return;
+        src += v * rows + 4 * (lane_id() >> 4);
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+            if (16 * m < rows) t[m] = *reinterpret_cast<const f32x4 *>(src + 16 * m);
+    }
+    __device__ __forceinline__ void load_transposed(const float *src, int v, int rows, int cols) {
+        zero();
+        if ((v & ~15) >= cols) return;
+        src += 4 * (lane_id() >> 4) * cols + v;
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+            if (16 * m < rows)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[m][i] = src[(uint32_t)((16 * m + i) * cols)];
     }
     // Dense rows of vc columns.
     __device__ __forceinline__ void store(float *dst, int v, int ka, int vc) const {
@@ -542,6 +575,46 @@ __device__ __forceinline__ float sum_dots(const float (&red)[ALL][C]) {
         for (int w = 1; w < NW; ++w) d += red[w][lane];
     }
     return d;
+}
+
+// The pair sums of a chunk from the parts by tiles, rows[si][t] (over the s of tile si, t of a later tile) and
+// cols[tj][s] (over the t of tile tj; of a tile on the diagonal the sums themselves), and the sums of x from
+// each token on and of y before it (one wave, lane = token): dg but for E.
+//
+// Sums from a lane to the end are sums up to it with the lanes turned round: scans add only what belongs to
+// them, so that a value that is not finite stays with the tokens that see it.
+template <int C>
+__device__ __forceinline__ float gate_sums(const float (&rows)[C / 16][C], const float (&cols)[C / 16][C], float x, float y) {
+    constexpr int TT = C / 16;
+    const int lane = lane_id(), n16 = lane & 15, j = lane / 16;
+    // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t of the tile over
+    // the tiles below, whole tiles below and to the left, and its own tile.
+    float left = 0.f, below = 0.f, dg = 0.f, r0 = 0.f, r1 = 0.f;
+    if (lane < C) {
+        if (j > 0) left = r0 = rows[0][lane];
+        if (j < 1) below += cols[1][lane];
+        if constexpr (TT == 4) {
+            if (j > 1) left += r1 = rows[1][lane];
+            if (j > 2) left += rows[2][lane];
+            if (j < 2) below += cols[2][lane];
+            if (j < 3) below += cols[3][lane];
+        }
+        dg = cols[j][lane];
+    }
+    if (TT == 4) {
+        const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
+        const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
+        dg += j == 1 ? f1 : j == 2 ? f2 : 0.f;
+    }
+    const int turned = lane ^ 15;
+    float up = __shfl(left, turned);
+    row_scan(up);
+    float before = __shfl_up(below, 1), y_before = __shfl_up(y, 1);
+    if (n16 == 0) before = 0.f;
+    row_scan(before);
+    const float x_on = wave_scan_add(__shfl(x, 63 - lane));
+    const float y_sum = wave_scan_add(lane == 0 ? 0.f : y_before);
+    return dg + ((__shfl(up, turned) + before) + (__shfl(x_on, 63 - lane) + y_sum));
 }
 
 // A chunk token by token, taken where the state before or after it is not finite: products over masked
@@ -744,6 +817,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
         sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
         if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, p.vc);
+        if (p.kept) S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + ci) * kept_size(p.ka, p.vc), v, up16(p.ka), up16(p.vc));
         if (n > 1) fetch(ci + 1, true);
         const int64_t token = (int64_t)ci * C + lane;
         float y_now = 0.f;  // of this chunk, for the wave that adds up dg
@@ -826,38 +900,10 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         if (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
         if (DOT && wave == 1) {
-            // Token t of tile j: rows u >= t of the tile over the tiles to their left, columns s < t of the
-            // tile over the tiles below, whole tiles below and to the left, and its own tile.
-            const int j = lane / 16;
-            float left = 0.f, below = 0.f, dg = 0.f, r0 = 0.f, r1 = 0.f;
-            if (lane < C) {
-                if (j > 0) left = r0 = lds.rows[0][lane];
-                if (TT == 4 && j > 1) left += r1 = lds.rows[1][lane];
-                if (TT == 4 && j > 2) left += lds.rows[2][lane];
-                if (j < 1) below += lds.cols[1][lane];
-                if (TT == 4 && j < 2) below += lds.cols[2][lane];
-                if (TT == 4 && j < 3) below += lds.cols[3][lane];
-                dg = lds.cols[j][lane];
-            }
-            if (TT == 4) {
-                const float f1 = wave_sum(lane >= 32 ? r0 : 0.f);
-                const float f2 = wave_sum(lane >= 48 ? r0 + r1 : 0.f);
-                dg += j == 1 ? f1 : j == 2 ? f2 : 0.f;
-            }
-            // Sums from a lane to the end are sums up to it with the lanes turned round: scans add only what
-            // belongs to them, so that a value that is not finite stays with the tokens that see it.
             const bool in = lane < C && token < p.T;
             const float x = sum_dots<C, NW>(lds.red), y = in ? y_now : 0.f;
-            const int turned = lane ^ 15;
-            float up = __shfl(left, turned);
-            row_scan(up);
-            float before = __shfl_up(below, 1), y_before = __shfl_up(y, 1);
-            if (n16 == 0) before = 0.f;
-            row_scan(before);
-            const float x_on = wave_scan_add(__shfl(x, 63 - lane));
-            const float y_sum = wave_scan_add(lane == 0 ? 0.f : y_before);
             const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(x);
-            dg += (__shfl(up, turned) + before) + (__shfl(x_on, 63 - lane) + y_sum) + E;
+            const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + E;
             edge = E + wave_sum(y);
             const bool on = in && gate.seg[lane] >= 0 && gate.step[lane] != 0.f;
             if (in) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
@@ -891,18 +937,23 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         __syncthreads();  // the chunk's tiles are read
         if (++gi == kGates && n > 1) next_gates();
     }
-    if (p.fin && at.nth == p.segments - 1) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
+    if (at.nth != p.segments - 1) return;
+    if (p.fin) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
+    if (p.kept)
+        S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * kept_size(p.ka, p.vc), v, up16(p.ka), up16(p.vc));
 }
 
 // dv and dk, from the last chunk to the first.  A wave owns 16 value columns of the adjoint state [K, V]
 // and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once
 // a chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for
 // dk read three of the four tensors again, and took its pairs' decays and the state's update a second
-// time.)  DOT: y_s = row_s k_s^T S v_s, and the products with the forward's states at segment starts.
-template <typename T, int KP, int VP, bool VEC, bool DOT>
+// time.)  MODE 1: also y_s = row_s k_s^T S v_s and the products with the forward's states at segment starts,
+// for the dq walk.  MODE 2: dq and dg as well, from the forward's states before every chunk (all_in_one).
+template <typename T, int KP, int VP, bool VEC, int MODE>
 __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
     typedef Mat<T> M;
-    typedef BackLds<T, KP, VP> L;
+    constexpr bool ALL = MODE == 2, DOT = MODE >= 1;
+    typedef BackLds<T, KP, VP, ALL> L;
     constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDK = L::LDK, LDV = L::LDV,
                   LDP = L::LDP, BT = RB / 16, NW = L::NW, THREADS = 64 * NW;
     __shared__ L lds;
@@ -980,6 +1031,30 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         if (++gi == kGates) next_gates();
     }
 
+    // ALL: the forward's state before the chunk, transposed: rows = values, the wave's 16 columns = keys.
+    const bool gates_too = ALL && p.dg;
+    const int64_t size = kept_size(p.K, p.V);
+    const float *kept = ALL ? p.kept + (int64_t)at.bh * (p.chunks + 1) * size : nullptr;
+    State<VP / 16> F;
+    float edge = 0.f;  // gates_too: <forward state, adjoint> at the chunk's end
+    if (ALL) {
+        if (gates_too) {
+            State<KT> e;
+            e.load_kept(kept + c_hi * size, v, up16(p.K), up16(p.V));
+            float d = 0.f;
+#pragma unroll
+            for (int m = 0; m < KT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
+            d = wave_sum(v < p.V ? d : 0.f);
+            if (lane == 0) lds.red[wave][0] = d;
+            __syncthreads();
+            for (int w = 0; w < VP / 16; ++w) edge += lds.red[w][0];
+            __syncthreads();
+        }
+        F.load_transposed(kept + ci * size, v, up16(p.V), up16(p.K));
+    }
+
     for (; n > 0; --n, --ci) {
         const GateTile<C> &gate = lds.gate[gi];
         const bool masks = odd || p.T - (int64_t)ci * C < C;
@@ -1001,18 +1076,20 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
 
         // For out token s and source t >= s: pk = Gam k_s.q_t, pv = Gam v_s.do_t, by tiles as in linear_walk
         // but from the other end.
+        constexpr int MINE = TT == 4 ? (12 + NW - 1) / NW : 1;
+        f32x4 W[MINE];
+        int sjs[MINE], tis[MINE];
 #pragma unroll
-        for (int m = 0; m < (TT == 4 ? 12 / NW + (12 % NW > 0) : 1); ++m) {
+        for (int m = 0; m < MINE; ++m) {
             const int id = wave + m * NW;
-            int sj, ti;
-            if (TT == 4) {
-                if (12 % NW && id >= 12) continue;
-                sj = id < 4 ? id >> 1 : id < 8 ? 2 : 3, ti = id < 4 ? id & 1 : id & 3;
-            } else {
-                sj = id >> 1, ti = id & 1;
-                if (id >= 4 || ti > sj) continue;
+            int sj = id >> 1, ti = id & 1;
+            if (TT == 4 && id >= 4) sj = id < 8 ? 2 : 3, ti = id & 3;
+            sjs[m] = TT - 1 - sj, tis[m] = TT - 1 - ti;
+            if ((TT == 4 && 12 % NW && id >= 12) || (TT == 2 && (id >= 4 || ti > sj))) {
+                sjs[m] = -1;
+                continue;
             }
-            sj = TT - 1 - sj, ti = TT - 1 - ti;
+            sj = sjs[m], ti = tis[m];
             f32x4 x = zero4(), y = zero4();
 #pragma unroll
             for (int r = 0; r < KP; r += RB)
@@ -1021,12 +1098,42 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int r = 0; r < VP; r += RB)
                 M::mma(y, M::row(lds.o + 16 * ti * LDV, LDV, r), M::row(lds.v + 16 * sj * LDV, LDV, r));
             const int s = 16 * sj + n16, t = 16 * ti + g4;
-            const f32x4 f = pair_decays<C, true, sizeof(T) == 4>(gate, s, t);
+            const f32x4 f = pair_decays<C, true, ALL || sizeof(T) == 4>(gate, s, t);
             T e[4], g[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] * f[i]), Elem<T>::store(g, i, y[i] * f[i]);
+            for (int i = 0; i < 4; ++i) {
+                const float a = x[i] * f[i];
+                Elem<T>::store(e, i, a), Elem<T>::store(g, i, y[i] * f[i]);
+                if (ALL) W[m][i] = f[i] == 0.f || t + i <= s ? 0.f : a * y[i];
+            }
             __builtin_memcpy(__builtin_assume_aligned(lds.pk + s * LDP + t, 4 * sizeof(T)), e, sizeof e);
             __builtin_memcpy(__builtin_assume_aligned(lds.pv + s * LDP + t, 4 * sizeof(T)), g, sizeof g);
+        }
+        if (gates_too) {
+            // As in linear_walk, with t along the rows: sums over the s of a tile for each t, over its t for each
+            // s, and on the diagonal for each token over the t from it on and the s before it.
+            float q[MINE], a[MINE], b[MINE], c[MINE];
+#pragma unroll
+            for (int m = 0; m < MINE; ++m) q[m] = (W[m][0] + W[m][1]) + (W[m][2] + W[m][3]);
+#pragma unroll
+            for (int m = 0; m < MINE; ++m)
+                a[m] = __shfl_down(q[m], 16), b[m] = __shfl_down(q[m], 32), c[m] = __shfl_down(q[m], 48);
+#pragma unroll
+            for (int m = 0; m < MINE; ++m) {
+                const float post = (g4 < 12 ? a[m] : 0.f) + (g4 < 8 ? b[m] : 0.f) + (g4 < 4 ? c[m] : 0.f);
+                const bool diag = sjs[m] == tis[m];
+                float z[4], from = post;
+#pragma unroll
+                for (int i = 3; i >= 0; --i) {
+                    from += W[m][i];
+                    z[i] = row16_sum(diag ? (n16 < g4 + i ? from : 0.f) : W[m][i]);
+                }
+                if (sjs[m] < 0 || tis[m] < sjs[m]) continue;
+                const float mine = pick(n16, z[0], z[1], z[2], z[3]);
+                const int t = 16 * tis[m] + g4 + n16;
+                if (n16 < 4) (diag ? lds.cols[tis[m]] : lds.rows[sjs[m]])[t] = mine;
+                if (!diag && lane < 16) lds.cols[tis[m]][16 * sjs[m] + n16] = post + q[m];  // the first group: all t
+            }
         }
         // The state's parts: rows = the wave's columns, column = token 16 j + n16.
         f32x4 av[TT], ak[TT];
@@ -1056,19 +1163,69 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
 #pragma unroll
             for (int i = 0; i < 4; ++i) av[j][i] *= f[j], ak[j][i] *= f[j];
         }
-        if (DOT && own_v) dot_rows<T, TT>(av, f, lds.v + 16 * wave, LDV, lds.red[wave]);
+        if (DOT && own_v && (!ALL || gates_too)) dot_rows<T, TT>(av, f, lds.v + 16 * wave, LDV, lds.red[wave]);
+        f32x4 aq[TT];
+        if (ALL) {
+#pragma unroll
+            for (int j = 0; j < TT; ++j) aq[j] = zero4();
+            if (gates_too) state_rows<T, VP, true>(aq, F, lds.o, LDV);
+            else state_rows<T, VP, false>(aq, F, lds.o, LDV);
+#pragma unroll
+            for (int j = 0; j < TT; ++j) {
+                f[j] = gate.col[16 * j + n16];  // of the walk in order
+#pragma unroll
+                for (int i = 0; i < 4; ++i) aq[j][i] *= f[j];
+            }
+            if (gates_too) dot_rows<T, TT>(aq, f, lds.q + 16 * wave, LDK, lds.red_q[wave]);
+            if (n > 1) F.load_transposed(kept + (ci - 1) * size, v, up16(p.V), up16(p.K));
+        }
         if (!good && lane == 0) lds.bad[n & 1] = 1;
         __syncthreads();
         const bool bad = lds.bad[n & 1] != 0;
         if (threadIdx.x == 0) lds.bad[(n & 1) ^ 1] = 0;
-        if (DOT && wave == 1) {
+        if (MODE == 1 && wave == 1) {
             const int64_t t = (int64_t)ci * C + lane;
             const float y = sum_dots<C, VP / 16>(lds.red);
             if (lane < C && t < p.T) p.y[at.bh * p.T + t] = y;
         }
+        if constexpr (ALL)
+            if (gates_too && wave == 1) {
+                const int64_t token = (int64_t)ci * C + lane;
+                const float x = sum_dots<C, KP / 16>(lds.red_q), y = sum_dots<C, VP / 16>(lds.red);
+                const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(y);
+                const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + E;
+                edge = E + wave_sum(x);
+                const bool on = gate.seg[lane & (C - 1)] >= 0 && gate.step[lane & (C - 1)] != 0.f;
+                if (lane < C && token < p.T) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
+            }
         const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
         T *dv = reinterpret_cast<T *>(p.dv), *dk = reinterpret_cast<T *>(p.dk);
+        if (ALL && p.dq) {
+            typename M::Frag kf[C / RB];
+#pragma unroll
+            for (int r = 0; r < C / RB; ++r) kf[r] = M::template across<LDK>(lds.k, r * RB, 16 * wave);
+            float z = 0.f;
+#pragma unroll
+            for (int j = 0; j < TT; ++j) {
+#pragma unroll
+                for (int r = 0; r <= j / BT; ++r)
+                    M::mma(aq[j], kf[r], M::template across<LDP>(lds.pv, r * RB, 16 * j));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z = fmaf(aq[j][i], 0.f, z);
+            }
+            T *dq = reinterpret_cast<T *>(p.dq) + row0 * p.K;
+            if (__builtin_expect(!__any(z != 0.f) && p.T > kFew, 1)) {
+                store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, aq);
+            } else {
+                // k, v or the state before the chunk may not be finite: token by token, from that state again
+                no_loads_left();
+                State<VP / 16> G;
+                G.load_transposed(kept + ci * size, v, up16(p.V), up16(p.K));
+                walk_tokens<T, VP, LDK, false, true>(G, lds.o, lds.v, lds.k, gate, p.V, v, p.K, dq,
+                                                     (int64_t)p.H * p.K, left);
+            }
+        }
         if (__builtin_expect(!bad, 1)) {
             if (dv && own_v) {
 #pragma unroll
@@ -1140,7 +1297,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     }
 
     if (p.fin && own_v && at.seg == 0) S.store(p.fin + (int64_t)at.bh * p.K * p.V, v, p.K, p.V);
-    if (DOT) {
+    if (MODE == 1) {
         float d = 0.f;
         if (own_v) {
             const float *src = reinterpret_cast<const float *>(p.edge_first.data);
@@ -1340,14 +1497,24 @@ Plan plan(const gdn2_shape *s, int dtype) {
 }
 
 struct Layout {
-    size_t state, decay, y, edges, dg, bytes;
+    size_t state, decay, kept, y, edges, dg, bytes;
 };
 
-// Checkpoint: the start states of the segments, and their decays.
-Layout checkpoint_layout(const Plan &p) {
+// Widths for which the backward is one walk, from a state that the forward keeps before every chunk.  Up to 64
+// such a state weighs half of what the chunk's four bf16 tensors do, which a dq walk of its own reads again:
+// forward and backward of 16 x 512 tokens, 8 heads of 64, 60 us against 68.  At 128 it weighs as much as they,
+// and the walk's registers run out: 4 x 8192 tokens, 16 heads of 128, 1253 us against 887.
+bool all_in_one(const gdn2_shape *s) { return s->keys <= 64 && s->values <= 64; }
+
+// Checkpoint: the start states of the segments and their decays, and for a backward in one walk the states
+// before every chunk and after the last.  A forward that no backward follows needs it only to carry states.
+Layout checkpoint_layout(const Plan &p, const gdn2_shape *s, bool train) {
     Layout l{};
     l.decay = p.segments > 1 ? round16(4 * p.BH * p.segments * p.KV) : 0;
-    l.bytes = l.decay + round16(4 * p.BH * p.segments);
+    l.kept = l.decay + round16(4 * p.BH * p.segments);
+    l.bytes = l.kept;
+    if (!train && (p.segments == 1 || p.prewalk)) l.bytes = 16;
+    if (train && all_in_one(s)) l.bytes += 4 * p.BH * (p.chunks + 1) * kept_size((int)s->keys, (int)s->values);
     return l;
 }
 
@@ -1437,8 +1604,9 @@ void launch_walk(const Forward &w, bool vec, unsigned grid, hipStream_t st) {
 
 template <typename T, bool REV, bool OUT, bool DOT>
 void size_walk(const Forward &w, bool vec, unsigned grid, hipStream_t st) {
-    if (w.ka <= 64 && w.vc <= 64) launch_walk<T, 64, 64, REV, OUT, DOT>(w, vec, grid, st);
-    else if (w.ka <= 64) launch_walk<T, 64, 128, REV, OUT, DOT>(w, vec, grid, st);
+    if constexpr (!DOT)  // with it, such widths are linear_back's
+        if (w.ka <= 64 && w.vc <= 64) return launch_walk<T, 64, 64, REV, OUT, DOT>(w, vec, grid, st);
+    if (w.ka <= 64) launch_walk<T, 64, 128, REV, OUT, DOT>(w, vec, grid, st);
     else if (w.vc <= 64) launch_walk<T, 128, 64, REV, OUT, DOT>(w, vec, grid, st);
     else launch_walk<T, 128, 128, REV, OUT, DOT>(w, vec, grid, st);
 }
@@ -1451,26 +1619,29 @@ hipError_t run_walk(const Forward &w, const Plan &p, int dtype, bool vec, hipStr
     return hipGetLastError();
 }
 
-template <typename T, int KP, int VP, bool DOT>
+template <typename T, int KP, int VP, int MODE>
 void launch_back(const Back &w, bool vec, unsigned grid, hipStream_t st) {
     const dim3 block(4 * std::max(KP, VP));
-    if (vec) hipLaunchKernelGGL((linear_back<T, KP, VP, true, DOT>), dim3(grid), block, 0, st, w);
-    else hipLaunchKernelGGL((linear_back<T, KP, VP, false, DOT>), dim3(grid), block, 0, st, w);
+    if (vec) hipLaunchKernelGGL((linear_back<T, KP, VP, true, MODE>), dim3(grid), block, 0, st, w);
+    else hipLaunchKernelGGL((linear_back<T, KP, VP, false, MODE>), dim3(grid), block, 0, st, w);
 }
 
-template <typename T, bool DOT>
+template <typename T, int MODE>
 void size_back(const Back &w, bool vec, unsigned grid, hipStream_t st) {
-    if (w.K <= 64 && w.V <= 64) launch_back<T, 64, 64, DOT>(w, vec, grid, st);
-    else if (w.K <= 64) launch_back<T, 64, 128, DOT>(w, vec, grid, st);
-    else if (w.V <= 64) launch_back<T, 128, 64, DOT>(w, vec, grid, st);
-    else launch_back<T, 128, 128, DOT>(w, vec, grid, st);
+    if constexpr (MODE == 2) {
+        launch_back<T, 64, 64, 2>(w, vec, grid, st);
+    } else {
+        if (w.K <= 64) launch_back<T, 64, 128, MODE>(w, vec, grid, st);
+        else if (w.V <= 64) launch_back<T, 128, 64, MODE>(w, vec, grid, st);
+        else launch_back<T, 128, 128, MODE>(w, vec, grid, st);
+    }
 }
 
-template <bool DOT>
+template <int MODE>
 hipError_t run_back(const Back &w, const Plan &p, int dtype, bool vec, hipStream_t st) {
     const unsigned grid = (unsigned)(p.BH * p.segments);
-    if (dtype == GDN2_BF16) size_back<bf16_t, DOT>(w, vec, grid, st);
-    else size_back<float, DOT>(w, vec, grid, st);
+    if (dtype == GDN2_BF16) size_back<bf16_t, MODE>(w, vec, grid, st);
+    else size_back<float, MODE>(w, vec, grid, st);
     return hipGetLastError();
 }
 
@@ -1512,21 +1683,22 @@ using namespace gdn2;
 
 extern "C" {
 
-size_t gdn2_linear_checkpoint_bytes(const gdn2_shape *shape, int32_t dtype) {
+size_t gdn2_linear_checkpoint_bytes(const gdn2_shape *shape, int32_t dtype, int train) {
     if (check_linear(shape, dtype) != GDN2_OK) return 0;
-    return checkpoint_layout(plan(shape, dtype)).bytes;
+    return checkpoint_layout(plan(shape, dtype), shape, train != 0).bytes;
 }
 
 int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
                      const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
                      const gdn2_view *reset, const gdn2_view *initial, void *output,
-                     float *final_state, void *checkpoint, size_t checkpoint_bytes, void *stream) {
+                     float *final_state, int train, void *checkpoint, size_t checkpoint_bytes,
+                     void *stream) {
     GDN2_TRY(check_inputs(shape, q, k, v, g, valid, reset));
     if (initial) GDN2_TRY(check_state(initial, "initial"));
     if (!output || !final_state)
         return fail(GDN2_ERR_ARGUMENT, "output and final_state must be non-null");
     const Plan p = plan(shape, q->dtype);
-    const Layout l = checkpoint_layout(p);
+    const Layout l = checkpoint_layout(p, shape, train != 0);
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, l.bytes, "checkpoint"));
     if (initial && !initial->data) initial = nullptr;
     const int64_t K = shape->keys, V = shape->values;
@@ -1540,7 +1712,8 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_scan");
         w.starts = state;
     }
-    if (p.segments > 1 && p.prewalk) w.starts_out = state;
+    if (train && all_in_one(shape)) w.kept = (float *)((char *)checkpoint + l.kept);
+    else if (train && p.segments > 1 && p.prewalk) w.starts_out = state;
     set_triple(&w, q, k, v, K, V);
     w.first = first;
     w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
@@ -1565,7 +1738,8 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     if (initial) GDN2_TRY(check_state(initial, "initial"));
     GDN2_TRY(check_view(d_output, "d_output", q->dtype, false));
     const Plan p = plan(shape, q->dtype);
-    const Layout lc = checkpoint_layout(p), l = workspace_layout(p, shape->time);
+    const bool all = all_in_one(shape);
+    const Layout lc = checkpoint_layout(p, shape, true), l = workspace_layout(p, shape->time);
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, lc.bytes, "checkpoint"));
     GDN2_TRY(check_buffer(workspace, workspace_bytes, l.bytes, "workspace"));
     if (initial && !initial->data) initial = nullptr;
@@ -1580,7 +1754,7 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     const View first = make_view(initial), d_final{d_final_state, shape->heads * p.KV, p.KV, V, 1};
     const bool many = p.segments > 1;
     hipError_t e = hipSuccess;
-    if (dk || dv || gates || d_initial) {
+    if (dk || dv || gates || d_initial || (all && dq)) {
         Back w = base_walk<Back>(shape, p, g, valid, reset);
         if (many && !p.prewalk) {
             float *adj = at(l.state);
@@ -1594,16 +1768,21 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
         w.first = d_final;
         w.s_bh = p.segments * p.KV, w.s_row = (int)V, w.s_col = 1;
         w.fin = d_initial;
-        if (gates) {
+        if (all) {
+            w.kept = (float *)((char *)const_cast<void *>(checkpoint) + lc.kept);
+            w.dq = dq;
+            w.dg = !gates ? nullptr : dg ? dg : at(l.dg);
+            e = run_back<2>(w, p, dtype, vec, st);
+        } else if (gates) {
             w.y = at(l.y), w.edges = at(l.edges);
             w.edge = states, w.edge_first = first;
-            e = run_back<true>(w, p, dtype, vec, st);
+            e = run_back<1>(w, p, dtype, vec, st);
         } else {
-            e = run_back<false>(w, p, dtype, vec, st);
+            e = run_back<0>(w, p, dtype, vec, st);
         }
         if (e != hipSuccess) return launch_status(e, "gdn2_linear_backward");
     }
-    if (dq || gates) {
+    if (!all && (dq || gates)) {
         Forward w = base;
         set_triple(&w, d_output, v, k, V, K);  // the state transposed: rows V, columns K
         w.out = dq;

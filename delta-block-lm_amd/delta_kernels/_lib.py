@@ -154,9 +154,9 @@ SIGNATURES = {
     "gdn2_lm_mixer_out_backward": (_I, [_M] + [_P] * 9 + [_Z, _P]),
     "gdn2_lm_swiglu_forward": (_I, [_L, _L, _P, _P, _P]),
     "gdn2_lm_swiglu_backward": (_I, [_L, _L, _P, _P, _P, _P]),
-    "gdn2_linear_checkpoint_bytes": (_Z, [_S, ctypes.c_int32]),
+    "gdn2_linear_checkpoint_bytes": (_Z, [_S, ctypes.c_int32, _I]),
     # Shapes and views of these go as packed bytes, hence as plain pointers.
-    "gdn2_linear_scan": (_I, [_P] * 8 + [_P, _F, _P, _Z, _P]),
+    "gdn2_linear_scan": (_I, [_P] * 8 + [_P, _F, _I, _P, _Z, _P]),
     "gdn2_linear_workspace_bytes": (_Z, [_S, ctypes.c_int32]),
     "gdn2_linear_backward": (_I, [_P] * 8 + [_P, _Z, _P, _F] + [_P] * 3 + [_F] * 3 + [_P, _Z, _P]),
     "gdn2_linear_step": (_I, [_P] * 7 + [_F, _P, _P]),

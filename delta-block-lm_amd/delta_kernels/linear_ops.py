@@ -121,28 +121,29 @@ def _attention_inputs(q, k, v, g, valid, reset, state=None, state_name="initial"
     return code, (B, T, H, K, V), views, (g, valid, reset)
 
 
-def _bytes(query: str, q, v, code: int) -> int:
+def _bytes(query: str, q, v, *args) -> int:
     """A buffer's size, remembered by shape."""
-    n = _size(query, _shape(q, v), code)
+    n = _size(query, _shape(q, v), *args)
     if n == 0:
         check(query, 2)
     return n
 
 
-def linear_attention_forward(q, k, v, g, valid=None, reset=None, initial=None):
+def linear_attention_forward(q, k, v, g, valid=None, reset=None, initial=None,
+                             train: bool = True):
     """Raw forward.  Returns (output, final_state, checkpoint); the checkpoint is
-    private storage for linear_attention_backward."""
+    private storage for linear_attention_backward, without train scratch alone."""
     code, shape, views, held = _attention_inputs(q, k, v, g, valid, reset, initial)
     if initial is not None and initial.dtype != F32:
         initial = initial.float()
     B, T, H, K, V = shape
     dev = q.device
-    n = _bytes("gdn2_linear_checkpoint_bytes", q, v, code)
+    n = _bytes("gdn2_linear_checkpoint_bytes", q, v, code, 1 if train else 0)
     out = torch.empty((B, T, H, V), dtype=q.dtype, device=dev)
     final = torch.empty((B, H, K, V), dtype=F32, device=dev)
     ck = torch.empty((n,), dtype=torch.uint8, device=dev)
     _call("gdn2_linear_scan", dev, _SHAPE(*shape), *views, _view(initial), out.data_ptr(),
-          final.data_ptr(), ck.data_ptr(), n)
+          final.data_ptr(), 1 if train else 0, ck.data_ptr(), n)
     return out, final, ck
 
 
@@ -214,7 +215,7 @@ def linear_attention(q, k, v, g, valid=None, reset=None, initial=None):
         if m is not None and m.requires_grad:
             raise ValueError(f"{name} is nondifferentiable metadata")
     if not _wants_grad(q, k, v, g, initial):
-        return linear_attention_forward(q, k, v, g, valid, reset, initial)[:2]
+        return linear_attention_forward(q, k, v, g, valid, reset, initial, False)[:2]
     return _LinearAttention.apply(q, k, v, g, valid, reset, initial)
 
 

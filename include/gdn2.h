@@ -533,17 +533,19 @@ GDN2_API int gdn2_hola_backward(const gdn2_hola_shape *shape, const gdn2_view *q
  * NULL (all valid, no reset); initial F32 [B,H,keys,values], a view or NULL.
  * Any element strides; rows of 16-byte aligned unit-stride channels are read
  * fastest.  batch * heads * ceil(time / 32) is at most 2^21.  A value that is not
- * finite reaches the tokens that see it and no others.
+ * finite reaches the outputs of the tokens that see it and no others, and no
+ * gradient outside its document.
  *
  * output is dense in q's dtype, final_state F32 dense.  The checkpoint (16-byte
- * aligned, sized by the query for the dtype) holds start states of segments of
- * the sequence for the backward; the forward needs it also where none follows. */
-GDN2_API size_t gdn2_linear_checkpoint_bytes(const gdn2_shape *shape, int32_t dtype);
+ * aligned, sized by the query for the dtype) holds states along the sequence for
+ * the backward if train is nonzero (for widths up to 64 one every 64 tokens, 32 in
+ * F32), and is scratch, and smaller, if it is zero. */
+GDN2_API size_t gdn2_linear_checkpoint_bytes(const gdn2_shape *shape, int32_t dtype, int train);
 GDN2_API int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
                               const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
                               const gdn2_view *reset, const gdn2_view *initial, void *output,
-                              float *final_state, void *checkpoint, size_t checkpoint_bytes,
-                              void *stream);
+                              float *final_state, int train, void *checkpoint,
+                              size_t checkpoint_bytes, void *stream);
 
 /* VJP.  d_output ([B,T,H,values], q's dtype, strided); d_final_state F32 dense or
  * NULL (zero).  dq, dk, dv dense in q's dtype; dg [B,T,H] and its sums over batch

@@ -28,13 +28,14 @@ def message(L):
 
 def size(L, query, s, dtype):
     from delta_kernels._lib import Gdn2Shape
-    return getattr(L, query)(Gdn2Shape.from_buffer_copy(s), dtype)
+    more = (1,) if "checkpoint" in query else ()
+    return getattr(L, query)(Gdn2Shape.from_buffer_copy(s), dtype, *more)
 
 
 def scan(L, s=None, q=None, k=None, v=None, g=None, valid=None, initial=None, out=0x2000, final=0x3000,
          ck=0x4000, n=1 << 40):
     return L.gdn2_linear_scan(s or shape(), q or view(), k or view(), v or view(), g or view(), valid,
-                              None, initial, out, final, ck, n, None)
+                              None, initial, out, final, 1, ck, n, None)
 
 
 @pytest.mark.parametrize("sizes,text", [
