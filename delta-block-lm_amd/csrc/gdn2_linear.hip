@@ -10,16 +10,22 @@
 //   dq_t = sum_{s<=t} Gam_ts (do_t.v_s) k_s + gam_t S0 do_t      the forward on  (do, v, k)
 //   dv_s = sum_{t>=s} Gam_ts (k_s.q_t) do_t + lam_s R^T k_s      time reversed on (k, q, do)
 //   dk_s = sum_{t>=s} Gam_ts (v_s.do_t) q_t + lam_s R v_s        time reversed on (v, do, q)
-// The forward and dq are one walk over the chunks in order (linear_walk), from a triple (a, b, c):
+// The forward and dq are a walk over the chunks in order (linear_walk), from a triple (a, b, c):
 //   out_t = sum_s Gam (a_t.b_s) c_s + row_t (a_t S),   S' = tot S + sum_s col_s b_s c_s^T;
 // dv and dk share a walk in the other direction (linear_back), with the pairs' decays and the adjoint
-// state of both.  The gate's gradient is a sum over the pairs that span a token,
+// state of both; for widths up to 64 it has dq and the gate's gradient as well.  The gate's gradient is a sum over the pairs that span a token,
 //   dg_t = sum_{u>=t,s<t} W_us,  W_us = Gam_us (q_u.k_s)(do_u.v_s),
 // cut at the chunk's bounds, with x_u = gam_u q_u^T S0 do_u, y_s = lam_s k_s^T R v_s and E = gam <S0, R>:
 //   dg_t = sum_{u>=t,s<t inside the chunk} W_us + sum_{u>=t} x_u + sum_{s<t} y_s + E.
-// linear_back gives y and the products <S0, R> at segment starts; the dq walk has the rest and steps
-// E from chunk to chunk (less x, plus y; 0 at a cut).  Nothing is subtracted over more than one segment,
-// so it keeps float32 accuracy for long memories.
+// Where dq has a walk of its own, linear_back gives y and the products <S0, R> at segment starts, and the
+// dq walk has the rest and steps E from chunk to chunk (less x, plus y; 0 at a cut); in one walk E steps the
+// other way.  Nothing is subtracted over more than one segment, so it keeps float32 accuracy for long memories.
+//
+// A sequence is cut into segments for parallel work; their start states come from a walk over (b, c) alone,
+// a launch of its own for all segments (carry) and a join over them, or, in short sequences, by each
+// segment from the sequence's start.  Operands of matrix products are the inputs' type.  In bf16 the pair
+// weights and, for the output, the state are rounded once, as the result is; the state itself, its update
+// and the sums of the gate's gradient keep float32 accuracy (three bf16 terms).
 #include <math.h>
 
 #include <algorithm>
@@ -33,7 +39,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGates = 8;       // chunks whose gates are made at a time
-constexpr int kFew = 4;         // sequences of up to so many tokens are taken token by token
+// Sequences of up to so many tokens are taken token by token, with nothing rounded but the result, as a call
+// of a token or two is expected to be: a chunk rounds its weights and the state too.  That is paid for: 256
+// x 8 heads of 64 on a state, bf16, take 36 us forward for one token and 45 for four (as a chunk 25), and
+// 99 and 165 backward (66).  The same line at 8 tokens would cost 57 and 251 in place of 25 and 66.
+constexpr int kFew = 4;
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
@@ -274,8 +284,9 @@ struct Staged {
 // are the tokens 16 j + n16; out is at the chunk's first row, stride the elements between two rows.
 //
 // Whole chunks of whole columns are stored without conditions.  Otherwise the compiler cannot count the
-// stores behind the next chunk's loads, and the wait for those loads becomes one for the stores too (a
-// tenth of a step); on the other way it is told that none are left.
+// stores behind the next chunk's loads, and the wait for those loads becomes one for the stores too; on
+// the other way it is told that none are left (4 x 8192 tokens, 16 heads of 128, both directions: 861 us,
+// 888 before).
 template <typename T, int TT, bool VEC>
 __device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int width, int left, bool whole,
                                            const f32x4 (&x)[TT]) {
@@ -718,6 +729,12 @@ struct MakeGates {
 // last chunk to the first).
 // DOT: the gate's gradient too, with (a, b, c, d) = (do, v, k, q): the products of the state's part with d
 // are its x, and W_us = Gam_us (a_u.b_s)(d_u.c_s).
+//
+// Bound by latency at 64 columns (two waves on each SIMD, which wait for LDS and for each other's tiles) and
+// by LDS at 128 (500 KB read a chunk).  bf16: 16 x 512 tokens, 8 heads of 64, forward 24.8 us (52 MB with the
+// kept states, 2.1 TB/s); 4 x 8192 tokens, 16 heads of 128, forward 175 us (3.1 TB/s), dq and dg 270 us (2.5
+// TB/s), a carry 80 us (3.3 TB/s; 57 us without the update).  The carry at 128 columns has four waves a SIMD:
+// with two it took 87 us, then 73.
 template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
 __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_walk(Forward p) {
     static_assert(!(OUT && REV), "");
@@ -943,12 +960,16 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * kept_size(p.ka, p.vc), v, up16(p.ka), up16(p.vc));
 }
 
-// dv and dk, from the last chunk to the first.  A wave owns 16 value columns of the adjoint state [K, V]
+// dv and dk, from the last chunk to the first, and more by MODE.  A wave owns 16 value columns of the adjoint state [K, V]
 // and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once
 // a chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for
 // dk read three of the four tensors again, and took its pairs' decays and the state's update a second
 // time.)  MODE 1: also y_s = row_s k_s^T S v_s and the products with the forward's states at segment starts,
 // for the dq walk.  MODE 2: dq and dg as well, from the forward's states before every chunk (all_in_one).
+//
+// Bound like linear_walk: bf16, 16 x 512 tokens, 8 heads of 64, all in one 39.6 us (78 MB, 2.0 TB/s); 4 x 8192
+// tokens, 16 heads of 128, without dq 325 us (2.5 TB/s), one workgroup of eight waves a unit for its 138 KB of
+// LDS and 256 registers.
 template <typename T, int KP, int VP, bool VEC, int MODE>
 __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
     typedef Mat<T> M;
@@ -1329,7 +1350,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
 }
 
 // Segments' additions -> start states, in place: state[s] = what the segments walked before s left.
-// One thread an element; carry over the segments in the walk's order.
+// One thread an element; carry over the segments in the walk's order.  Bound by memory: 64 heads of 128 x 128
+// and 8 segments 12 us (67 MB, 5.6 TB/s).
 struct JoinArgs {
     float *state;        // [BH, segments, K V]
     const float *decay;  // [BH, segments]
@@ -1369,7 +1391,8 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
     }
 }
 
-// out[h] = sum over b, t of x[b, t, h]: one workgroup a head, a fixed order.
+// out[h] = sum over b, t of x[b, t, h]: one workgroup a head, a fixed order.  For 8 x 509 tokens the launch
+// alone (3.9 us).
 __global__ void __launch_bounds__(1024) linear_head_sum(const float *x, int64_t rows, int64_t H, float *out) {
     __shared__ float red[16];
     float s = 0.f;
@@ -1395,7 +1418,8 @@ struct StepArgs {
 };
 
 // One workgroup a (batch, head): CG column groups of four values by 256 / CG rows, each thread four
-// rows at a time.  The state is read and written once; bound by that.
+// rows at a time.  The state is read and written once; bound by that: 2048 states of 64 x 64 14.3 us (4.8
+// TB/s), 8192 of 128 x 128 218 us (4.9 TB/s).
 template <typename T, int CG>
 __global__ void __launch_bounds__(kThreads) linear_step(StepArgs p) {
     constexpr int RG = kThreads / CG, U = 4;
@@ -1476,7 +1500,10 @@ struct Plan {
     bool prewalk;  // start states are walked to, instead of carried by a launch of their own
 };
 
-constexpr int64_t kWantGroups = 512;  // workgroups that fill the card
+// Workgroups that fill the card: two a unit.  Forward and backward of 16 x 512 tokens, 8 heads of 64 / 4 x 8192
+// tokens, 16 heads of 128 / 8 x 509 f32 tokens, 8 heads of 64: 60 / 882 / 80 us; with 1024 60 / 957 / 81, with
+// 256 64 / 883 / 92.
+constexpr int64_t kWantGroups = 512;
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
@@ -1487,11 +1514,14 @@ Plan plan(const gdn2_shape *s, int dtype) {
     p.BH = s->batch * s->heads;
     p.KV = s->keys * s->values;
     // Segments of at least two chunks, as many as fill the card, and of at most 16 (the gate's gradient adds
-    // up what happens in a segment).
+    // up what happens in a segment).  With single chunks a prompt of 3001 tokens, 8 heads of 64, takes 24.8 us
+    // in place of 23.8: more to join.
     int64_t want = std::max<int64_t>(kWantGroups / p.BH, (p.chunks + 15) / 16);
     want = std::max<int64_t>(1, std::min<int64_t>(want, p.chunks / 2));
     p.seg_chunks = (int)((p.chunks + want - 1) / want);
     p.segments = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
+    // Walked to where that costs at most a few chunks: 512 tokens (8 chunks) 60 us in both directions, 74 carried;
+    // 509 f32 tokens (16 chunks) 80 us carried, 103 walked to.
     p.prewalk = p.chunks <= 8;
     return p;
 }
