@@ -47,37 +47,55 @@ constexpr int kFew = 4;
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
-// order() reads a row in the order in which two accumulator tiles hold their 32 rows.
+// Lane group g of a fragment has entries 8 g .. 8 g + 7 of a row of bf16 (4 g .. in float32).
+//
+// place(m, g4): the first of the four rows of a state that a lane (g4 = 4 g) has in accumulator tile m, and the
+// columns of tile m of the pair weights.  In bf16 tiles 2 m and 2 m + 1 share 32 rows, eight to each lane
+// group, so that a group's accumulators are entries 8 g .. 8 g + 7 at once: a product's other operand is then
+// read in 16-byte pieces.  across() reads a tile the other way round, with the rows 4 g .. and 16 + 4 g .. of
+// each 32 in group g (a wave's eight rows at a time lie in different banks), which is what the columns of the
+// pair weights and the rows of BackLds::D are laid out for; across_place() the same of place()'s columns.
 template <typename T> struct Mat;
 template <> struct Mat<bf16_t> {
-    static constexpr int C = 64, RB = 32, PAD = 8, N = 8;  // N: elements of 16 bytes
+    static constexpr int C = 64, RB = 32, N = 8;  // N: elements of 16 bytes
     typedef bf16x8_t Frag;
+    // Elements from row to row in LDS: rows of 64 and of 128 start in banks that 16-byte reads of 16 rows
+    // share at most twice, and not at all.
+    static __host__ __device__ constexpr int ld(int width) { return width + (width == 128 ? 16 : 8); }
     static __device__ __forceinline__ Frag row(const bf16_t *x, int ld, int r0) {
         return frag(x, ld, r0);
     }
-    static __device__ __forceinline__ Frag order(const bf16_t *x, int ld, int r0) {
-        const int l = lane_id();
-        const bf16_t *p = x + (l & 15) * ld + r0 + 4 * (l >> 4);
-        const uint2 u = *reinterpret_cast<const uint2 *>(p), v = *reinterpret_cast<const uint2 *>(p + 16);
-        return __builtin_bit_cast(Frag, make_uint4(u.x, u.y, v.x, v.y));
+    static __device__ __forceinline__ Frag read_tr(const bf16_t *p, int ld16) {
+        const v4s x = lds_tr16(p), y = lds_tr16(p + ld16);
+        typedef short v8s __attribute__((ext_vector_type(8)));
+        const v8s v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return __builtin_bit_cast(Frag, v);
     }
     template <int LD>
     static __device__ __forceinline__ Frag across(const bf16_t *z, int r0, int c0) {
-        return frag_tr<LD>(z, r0, c0);
+        const int l = lane_id(), i = l & 15;
+        return read_tr(z + (r0 + 4 * (l >> 4) + (i >> 2)) * LD + c0 + 4 * (i & 3), 16 * LD);
     }
+    template <int LD>
+    static __device__ __forceinline__ Frag across_place(const bf16_t *z, int r0, int m) {
+        const int l = lane_id(), i = l & 15;
+        return read_tr(z + (r0 + 4 * (l >> 4) + (i >> 2)) * LD + place(m, 4 * (i & 3)), 16 * LD);
+    }
+    static __device__ __forceinline__ constexpr int place(int m, int g4) { return 32 * (m >> 1) + 4 * (m & 1) + 2 * g4; }
+    // Entry e of a fragment of across() is row r0 + 4 g + past(e); row_for(i): the row of which it is entry i.
+    static __device__ __forceinline__ constexpr int past(int e) { return e + 3 * (e & 4); }
+    static __device__ __forceinline__ int row_for(int i) { return (i & ~31) + 4 * ((i >> 3) & 3) + (i & 3) + 4 * (i & 4); }
     static __device__ __forceinline__ void mma(f32x4 &acc, const Frag &x, const Frag &y) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
     }
 };
 template <> struct Mat<float> {
-    static constexpr int C = 32, RB = 16, PAD = 4, N = 4;
+    static constexpr int C = 32, RB = 16, N = 4;
     typedef f32x4 Frag;
+    static __host__ __device__ constexpr int ld(int width) { return width + 4; }
     static __device__ __forceinline__ Frag row(const float *x, int ld, int r0) {
         const int l = lane_id();
         return *reinterpret_cast<const f32x4 *>(x + (l & 15) * ld + r0 + 4 * (l >> 4));
-    }
-    static __device__ __forceinline__ Frag order(const float *x, int ld, int r0) {
-        return row(x, ld, r0);
     }
     template <int LD>
     static __device__ __forceinline__ Frag across(const float *z, int r0, int c0) {
@@ -85,6 +103,11 @@ template <> struct Mat<float> {
         const float *p = z + (r0 + 4 * (l >> 4)) * LD + c0 + (l & 15);
         return Frag{p[0], p[LD], p[2 * LD], p[3 * LD]};
     }
+    template <int LD>
+    static __device__ __forceinline__ Frag across_place(const float *z, int r0, int m) { return across<LD>(z, r0, 16 * m); }
+    static __device__ __forceinline__ constexpr int place(int m, int g4) { return 16 * m + g4; }
+    static __device__ __forceinline__ constexpr int past(int e) { return e; }
+    static __device__ __forceinline__ int row_for(int i) { return i; }
     static __device__ __forceinline__ void mma(f32x4 &acc, const Frag &x, const Frag &y) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -362,8 +385,7 @@ __device__ __forceinline__ float groups_sum(float x) {
 
 template <typename T, int KP, int CP, bool OUT, bool DOT>
 struct WalkLds {
-    static constexpr int C = Mat<T>::C, LDA = KP + Mat<T>::PAD, LDC = CP + Mat<T>::PAD,
-                         LDP = C + Mat<T>::PAD;
+    static constexpr int C = Mat<T>::C, LDA = Mat<T>::ld(KP), LDC = Mat<T>::ld(CP), LDP = Mat<T>::ld(C);
     T b[C * LDA], c[C * LDC];
     T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
     GateTile<C> gate[kGates];
@@ -373,11 +395,11 @@ struct WalkLds {
 
 template <typename T, int KP, int VP, bool ALL>
 struct BackLds {
-    static constexpr int C = Mat<T>::C, LDK = KP + Mat<T>::PAD, LDV = VP + Mat<T>::PAD,
-                         LDP = C + Mat<T>::PAD, NW = (KP > VP ? KP : VP) / 16;
+    static constexpr int C = Mat<T>::C, LDK = Mat<T>::ld(KP), LDV = Mat<T>::ld(VP), LDP = Mat<T>::ld(C),
+                         NW = (KP > VP ? KP : VP) / 16;
     T q[C * LDK], k[C * LDK], v[C * LDV], o[C * LDV];
     T pk[C * LDP], pv[C * LDP];  // Gam k.q and Gam v.do; the token-by-token form keeps float sums in pk
-    T D[VP * LDK];               // the adjoint state transposed, [value][key]
+    T D[VP * LDK];               // the adjoint state transposed, [row_for(value)][key]
     GateTile<C> gate[kGates];
     float red[NW][C], red_q[ALL ? NW : 1][C];
     float rows[ALL ? C / 16 : 1][C], cols[ALL ? C / 16 : 1][C];  // parts of the pair sums, as in WalkLds
@@ -388,12 +410,13 @@ struct BackLds {
 // selects it, one after the other, and waits for every one.
 __device__ __forceinline__ void keep(float &x) { asm volatile("" : "+v"(x)); }
 
-__host__ __device__ inline int up16(int n) { return (n + 15) & ~15; }
-__host__ __device__ inline int64_t kept_size(int rows, int cols) { return (int64_t)up16(rows) * up16(cols); }
+__host__ __device__ inline int up32(int n) { return (n + 31) & ~31; }
+__host__ __device__ inline int64_t kept_size(int rows, int cols) { return (int64_t)up32(rows) * up32(cols); }
 
-// State of one wave: 16 columns, accumulator tiles of 16 rows.
-template <int KT>
+// State of one wave: 16 columns, accumulator tiles of 16 rows (place()).
+template <typename T, int KT>
 struct State {
+    typedef Mat<T> M;
     f32x4 t[KT];
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -416,7 +439,7 @@ struct State {
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[m][i] = src[col + (uint32_t)(min(16 * m + g4 + i, ka - 1) * rs)];
+            for (int i = 0; i < 4; ++i) t[m][i] = src[col + (uint32_t)(min(M::place(m, g4) + i, ka - 1) * rs)];
     }
     __device__ __forceinline__ void settle(int v, int ka, int vc) {
         const int g4 = 4 * (lane_id() >> 4);
@@ -426,78 +449,78 @@ struct State {
             for (int i = 0; i < 4; ++i) {
                 float x = t[m][i];
                 keep(x);
-                t[m][i] = 16 * m + g4 + i < ka && v < vc ? x : 0.f;
+                t[m][i] = M::place(m, g4) + i < ka && v < vc ? x : 0.f;
             }
     }
-    // The kept form of a whole state: [columns][rows], both rounded up to 16.
+    // The kept form of a whole state: [columns][rows], both rounded up to 32.
     __device__ __forceinline__ void keep_at(float *dst, int v, int rows, int cols) const {
         if ((v & ~15) >= cols) return;
-        dst += v * rows + 4 * (lane_id() >> 4);
+        dst += v * rows + M::place(0, 4 * (lane_id() >> 4));
 #pragma unroll
         for (int m = 0; m < KT; ++m)
-            if (16 * m < rows) *reinterpret_cast<f32x4 *>(dst + 16 * m) = t[m];
+            if (M::place(m, 0) < rows) *reinterpret_cast<f32x4 *>(dst + M::place(m, 0)) = t[m];
     }
     // A kept state as it was (the loads are only issued), or its transpose: columns and rows change places.
     __device__ __forceinline__ void load_kept(const float *src, int v, int rows, int cols) {
         zero();
         if ((v & ~15) >= cols) return;
-        src += v * rows + 4 * (lane_id() >> 4);
+        src += v * rows + M::place(0, 4 * (lane_id() >> 4));
 #pragma unroll
         for (int m = 0; m < KT; ++m)
-            if (16 * m < rows) t[m] = *reinterpret_cast<const f32x4 *>(src + 16 * m);
+            if (M::place(m, 0) < rows) t[m] = *reinterpret_cast<const f32x4 *>(src + M::place(m, 0));
     }
     __device__ __forceinline__ void load_transposed(const float *src, int v, int rows, int cols) {
         zero();
         if ((v & ~15) >= cols) return;
-        src += 4 * (lane_id() >> 4) * cols + v;
+        src += M::place(0, 4 * (lane_id() >> 4)) * cols + v;
 #pragma unroll
         for (int m = 0; m < KT; ++m)
-            if (16 * m < rows)
+            if (M::place(m, 0) < rows)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) t[m][i] = src[(uint32_t)((16 * m + i) * cols)];
+                for (int i = 0; i < 4; ++i) t[m][i] = src[(uint32_t)((M::place(m, 0) + i) * cols)];
     }
     // Dense rows of vc columns.
     __device__ __forceinline__ void store(float *dst, int v, int ka, int vc) const {
         const int g4 = 4 * (lane_id() >> 4);
         if (v >= vc) return;
-        dst += g4 * vc + v;
+        dst += M::place(0, g4) * vc + v;
         if (ka == 16 * KT) {
 #pragma unroll
             for (int m = 0; m < KT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dst[(uint32_t)((16 * m + i) * vc)] = t[m][i];
+                for (int i = 0; i < 4; ++i) dst[(uint32_t)((M::place(m, 0) + i) * vc)] = t[m][i];
             return;
         }
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (16 * m + g4 + i < ka) dst[(uint32_t)((16 * m + i) * vc)] = t[m][i];
+                if (M::place(m, g4) + i < ka) dst[(uint32_t)((M::place(m, 0) + i) * vc)] = t[m][i];
     }
 };
 
 // The state after the chunk, tot S + sum_s col_s b_s c_s^T, and whether all of it is finite.
 template <typename T, int KP>
-__device__ __forceinline__ bool update(State<KP / 16> &U, const State<KP / 16> &S, float tot,
+__device__ __forceinline__ bool update(State<T, KP / 16> &U, const State<T, KP / 16> &S, float tot,
                                        const typename Mat<T>::Frag (&cf)[Mat<T>::C / Mat<T>::RB],
                                        const T *b, const float *col) {
     typedef Mat<T> M;
-    constexpr int KT = KP / 16, RB = M::RB, LDA = KP + M::PAD;
+    constexpr int KT = KP / 16, RB = M::RB, LDA = M::ld(KP);
     U.zero();
 #pragma unroll
     for (int r = 0; r < M::C / RB; ++r) {
-        const float *f = col + r * RB + (RB / 4) * (lane_id() >> 4);
+        const float *f = col + r * RB + 4 * (lane_id() >> 4);
         // Four tiles one after the other: a product waits for none of the others.
         Split3 s3;
         float x[8];
 #pragma unroll
-        for (int e = 0; e < RB / 4; ++e) x[e] = static_cast<float>(cf[r][e]) * f[e];
+        for (int e = 0; e < RB / 4; ++e) x[e] = static_cast<float>(cf[r][e]) * f[M::past(e)];
         if constexpr (sizeof(T) == 2) s3 = split3(x);
 #pragma unroll
         for (int m0 = 0; m0 < KT; m0 += 4) {
             typename M::Frag y[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) y[m] = M::template across<LDA>(b, r * RB, 16 * (m0 + m));
+            for (int m = 0; m < 4; ++m) y[m] = M::template across_place<LDA>(b, r * RB, m0 + m);
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int q = 0; q < 3; ++q)
@@ -522,7 +545,7 @@ __device__ __forceinline__ bool update(State<KP / 16> &U, const State<KP / 16> &
 // acc[j] += (row t of x) S for the tokens t of tile j: rows = the wave's columns, column = t.  THREE
 // terms of the state give float32 accuracy; with one, the state is rounded to bf16, as the result is.
 template <typename T, int KP, bool THREE>
-__device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const State<KP / 16> &S, const T *x, int ld) {
+__device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const State<T, KP / 16> &S, const T *x, int ld) {
     typedef Mat<T> M;
 #pragma unroll
     for (int r = 0; r < KP / M::RB; ++r) {
@@ -531,14 +554,14 @@ __device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const S
             const Split3 s3 = split3({u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]});
             typename M::Frag y[M::C / 16];
 #pragma unroll
-            for (int j = 0; j < M::C / 16; ++j) y[j] = M::order(x + 16 * j * ld, ld, r * M::RB);
+            for (int j = 0; j < M::C / 16; ++j) y[j] = M::row(x + 16 * j * ld, ld, r * M::RB);
 #pragma unroll
             for (int q = 0; q < (THREE ? 3 : 1); ++q)
 #pragma unroll
                 for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], s3.t[q], y[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], S.t[r], M::order(x + 16 * j * ld, ld, r * M::RB));
+            for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], S.t[r], M::row(x + 16 * j * ld, ld, r * M::RB));
         }
     }
 }
@@ -631,10 +654,10 @@ __device__ __forceinline__ float gate_sums(const float (&rows)[C / 16][C], const
 // A chunk token by token, taken where the state before or after it is not finite: products over masked
 // tokens, and with factors that are 0, would spread such a value to tokens that do not see it.
 template <typename T, int KP, int LDC, bool REV, bool OUT>
-__device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const T *b, const T *c,
+__device__ __forceinline__ void walk_tokens(State<T, KP / 16> &S, const T *a, const T *b, const T *c,
                                             const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
                                             T *out, int64_t stride, int tokens) {
-    constexpr int KT = KP / 16, C = Mat<T>::C, LDA = KP + Mat<T>::PAD;
+    constexpr int KT = KP / 16, C = Mat<T>::C, LDA = Mat<T>::ld(KP);
     const int g4 = 4 * (lane_id() >> 4);
 #pragma unroll 1
     for (int n = 0; n < C; ++n) {
@@ -648,7 +671,7 @@ __device__ __forceinline__ void walk_tokens(State<KP / 16> &S, const T *a, const
             for (int m = 0; m < KT; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int k = 16 * m + g4 + i;
+                    const int k = Mat<T>::place(m, g4) + i;
                     if (k >= ka) continue;  // 0 there, whatever x is
                     if (!REV) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
                     S.t[m][i] += Elem<T>::load(b, t * LDA + k) * x;
@@ -684,8 +707,8 @@ __device__ __forceinline__ const T *head_rows(const View &x, const Place &at) {
 }
 
 // The state before a walk's segment: at hand (stored), or the walk's first.
-template <int KT>
-__device__ __forceinline__ void start_state(State<KT> &S, const Walk &p, const Place &at, bool stored, int v,
+template <typename T, int KT>
+__device__ __forceinline__ void start_state(State<T, KT> &S, const Walk &p, const Place &at, bool stored, int v,
                                             int ka, int vc) {
     const float *src = reinterpret_cast<const float *>(p.first.data);
     int rs = (int)p.first.s2, cs = (int)p.first.s3;
@@ -730,11 +753,13 @@ struct MakeGates {
 // DOT: the gate's gradient too, with (a, b, c, d) = (do, v, k, q): the products of the state's part with d
 // are its x, and W_us = Gam_us (a_u.b_s)(d_u.c_s).
 //
-// Bound by latency at 64 columns (two waves on each SIMD, which wait for LDS and for each other's tiles) and
-// by LDS at 128 (500 KB read a chunk).  bf16: 16 x 512 tokens, 8 heads of 64, forward 24.8 us (52 MB with the
-// kept states, 2.1 TB/s); 4 x 8192 tokens, 16 heads of 128, forward 175 us (3.1 TB/s), dq and dg 270 us (2.5
-// TB/s), a carry 80 us (3.3 TB/s; 57 us without the update).  The carry at 128 columns has four waves a SIMD:
-// with two it took 87 us, then 73.
+// Bound by latency: a chunk's tiles, weights, products and state wait for each other with two to four waves on
+// each SIMD, whose vector units issue in a third (forward) to a half (DOT) of the cycles.  bf16: 16 x 512
+// tokens, 8 heads of 64, forward 24.3 us (52 MB with the kept states, 2.1 TB/s); 4 x 8192 tokens, 16 heads of
+// 128, forward 156 us (3.4 TB/s), dq and dg 270 us (2.5 TB/s), a carry 73 us (3.7 TB/s).  With a state laid out
+// by 16 rows a tile and rows of 136 in LDS, the forward's LDS was busy for half of its time, two fifths of that
+// in bank conflicts, and it took 175 us, a carry 81.  The carry at 128 columns has four waves a SIMD: 73 us
+// where two took 87, both before that.
 template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
 __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_walk(Forward p) {
     static_assert(!(OUT && REV), "");
@@ -774,7 +799,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     // All first loads are on their way before the first is waited for.
     MakeGates<C, REV, NW> gates;
     gates.load(p, at, ci, n);
-    State<KT> S;
+    State<T, KT> S;
     S.zero();
     if (OUT) start_state(S, p, at, !walked, v, p.ka, p.vc);
     fetch(ci, n <= out);
@@ -805,7 +830,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         __syncthreads();
         typename M::Frag cf[C / RB];
         across_c(cf);
-        State<KT> U;
+        State<T, KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
         decay *= gate.tot;
         if (__builtin_expect(fine && next, 1)) {
@@ -834,7 +859,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
         sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
         if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, p.vc);
-        if (p.kept) S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + ci) * kept_size(p.ka, p.vc), v, up16(p.ka), up16(p.vc));
+        if (p.kept) S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + ci) * kept_size(p.ka, p.vc), v, up32(p.ka), up32(p.vc));
         if (n > 1) fetch(ci + 1, true);
         const int64_t token = (int64_t)ci * C + lane;
         float y_now = 0.f;  // of this chunk, for the wave that adds up dg
@@ -866,7 +891,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             T e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
-            __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + s, 4 * sizeof(T)), e, sizeof e);
+            __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + M::place(si, g4), 4 * sizeof(T)), e, sizeof e);
             if (DOT) {
                 y[m] = zero4();
 #pragma unroll
@@ -928,7 +953,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
 
         typename M::Frag cf[C / RB];
         across_c(cf);
-        State<KT> U;
+        State<T, KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
         T *o = reinterpret_cast<T *>(p.out);
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
@@ -957,7 +982,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     if (at.nth != p.segments - 1) return;
     if (p.fin) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
     if (p.kept)
-        S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * kept_size(p.ka, p.vc), v, up16(p.ka), up16(p.vc));
+        S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * kept_size(p.ka, p.vc), v, up32(p.ka), up32(p.vc));
 }
 
 // dv and dk, from the last chunk to the first, and more by MODE.  A wave owns 16 value columns of the adjoint state [K, V]
@@ -968,7 +993,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
 // for the dq walk.  MODE 2: dq and dg as well, from the forward's states before every chunk (all_in_one).
 //
 // Bound like linear_walk: bf16, 16 x 512 tokens, 8 heads of 64, all in one 39.6 us (78 MB, 2.0 TB/s); 4 x 8192
-// tokens, 16 heads of 128, without dq 325 us (2.5 TB/s), one workgroup of eight waves a unit for its 138 KB of
+// tokens, 16 heads of 128, without dq 320 us (2.5 TB/s), one workgroup of eight waves a unit for its 144 KB of
 // LDS and 256 registers.
 template <typename T, int KP, int VP, bool VEC, int MODE>
 __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
@@ -1005,7 +1030,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     };
     MakeGates<C, true, NW> gates;
     gates.load(p, at, ci, n);
-    State<KT> S;
+    State<T, KT> S;
     S.zero();
     if (own_v) start_state(S, p, at, !walked, v, p.K, p.V);
     fetch(ci, n <= out);
@@ -1038,7 +1063,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         if (own_v) {
             typename M::Frag of[C / RB];
             across_o(of);
-            State<KT> U;
+            State<T, KT> U;
             const bool next = update<T, KP>(U, S, gate.tot, of, lds.q, gate.col);
             if (__builtin_expect(fine && next, 1)) {
                 S = U;
@@ -1056,12 +1081,12 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     const bool gates_too = ALL && p.dg;
     const int64_t size = kept_size(p.K, p.V);
     const float *kept = ALL ? p.kept + (int64_t)at.bh * (p.chunks + 1) * size : nullptr;
-    State<VP / 16> F;
+    State<T, VP / 16> F;
     float edge = 0.f;  // gates_too: <forward state, adjoint> at the chunk's end
     if (ALL) {
         if (gates_too) {
-            State<KT> e;
-            e.load_kept(kept + c_hi * size, v, up16(p.K), up16(p.V));
+            State<T, KT> e;
+            e.load_kept(kept + c_hi * size, v, up32(p.K), up32(p.V));
             float d = 0.f;
 #pragma unroll
             for (int m = 0; m < KT; ++m)
@@ -1073,7 +1098,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int w = 0; w < VP / 16; ++w) edge += lds.red[w][0];
             __syncthreads();
         }
-        F.load_transposed(kept + ci * size, v, up16(p.V), up16(p.K));
+        F.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
     }
 
     for (; n > 0; --n, --ci) {
@@ -1089,7 +1114,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 T e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, S.t[m][i]);
-                __builtin_memcpy(__builtin_assume_aligned(lds.D + v * LDK + 16 * m + g4, 4 * sizeof(T)), e, sizeof e);
+                __builtin_memcpy(__builtin_assume_aligned(lds.D + M::row_for(v) * LDK + M::place(m, g4), 4 * sizeof(T)), e, sizeof e);
             }
         }
         if (n > 1) fetch(ci - 1, true);
@@ -1127,8 +1152,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 Elem<T>::store(e, i, a), Elem<T>::store(g, i, y[i] * f[i]);
                 if (ALL) W[m][i] = f[i] == 0.f || t + i <= s ? 0.f : a * y[i];
             }
-            __builtin_memcpy(__builtin_assume_aligned(lds.pk + s * LDP + t, 4 * sizeof(T)), e, sizeof e);
-            __builtin_memcpy(__builtin_assume_aligned(lds.pv + s * LDP + t, 4 * sizeof(T)), g, sizeof g);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pk + s * LDP + M::place(ti, g4), 4 * sizeof(T)), e, sizeof e);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pv + s * LDP + M::place(ti, g4), 4 * sizeof(T)), g, sizeof g);
         }
         if (gates_too) {
             // As in linear_walk, with t along the rows: sums over the s of a tile for each t, over its t for each
@@ -1160,7 +1185,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         f32x4 av[TT], ak[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) av[j] = ak[j] = zero4();
-        State<KT> U;
+        State<T, KT> U;
         U.zero();
         typename M::Frag of[C / RB];
         bool good = fine;
@@ -1198,7 +1223,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 for (int i = 0; i < 4; ++i) aq[j][i] *= f[j];
             }
             if (gates_too) dot_rows<T, TT>(aq, f, lds.q + 16 * wave, LDK, lds.red_q[wave]);
-            if (n > 1) F.load_transposed(kept + (ci - 1) * size, v, up16(p.V), up16(p.K));
+            if (n > 1) F.load_transposed(kept + (ci - 1) * size, v, up32(p.V), up32(p.K));
         }
         if (!good && lane == 0) lds.bad[n & 1] = 1;
         __syncthreads();
@@ -1231,7 +1256,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int j = 0; j < TT; ++j) {
 #pragma unroll
                 for (int r = 0; r <= j / BT; ++r)
-                    M::mma(aq[j], kf[r], M::template across<LDP>(lds.pv, r * RB, 16 * j));
+                    M::mma(aq[j], kf[r], M::template across_place<LDP>(lds.pv, r * RB, j));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) z = fmaf(aq[j][i], 0.f, z);
             }
@@ -1241,8 +1266,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             } else {
                 // k, v or the state before the chunk may not be finite: token by token, from that state again
                 no_loads_left();
-                State<VP / 16> G;
-                G.load_transposed(kept + ci * size, v, up16(p.V), up16(p.K));
+                State<T, VP / 16> G;
+                G.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
                 walk_tokens<T, VP, LDK, false, true>(G, lds.o, lds.v, lds.k, gate, p.V, v, p.K, dq,
                                                      (int64_t)p.H * p.K, left);
             }
@@ -1290,7 +1315,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                     for (int m = 0; m < KT; ++m)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int k = 16 * m + g4 + i;
+                            const int k = Mat<T>::place(m, g4) + i;
                             if (k < p.K) {
                                 S.t[m][i] += Elem<T>::load(lds.q, t * LDK + k) * x;
                                 o += Elem<T>::load(lds.k, t * LDK + k) * S.t[m][i];
@@ -1329,7 +1354,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 off = ((int64_t)at.bh * p.segments + at.seg) * p.K * p.V;
             }
             if (src) {
-                State<KT> e;
+                State<T, KT> e;
                 e.load(src + off, rs, cs, v, p.K, p.V);
                 e.settle(v, p.K, p.V);
 #pragma unroll
