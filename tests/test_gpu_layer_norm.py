@@ -90,6 +90,25 @@ def test_rows(dk, rows, W):
     check(x, w, b, dy, 1e-5, torch.bfloat16, *run(dk, x, w, b, dy, 1e-5, torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,W", [(200, 8193), (130, 10000), (70, 40001), (33000, 33), (33000, 40)])
+def test_rows_beyond_the_partial_sums(dk, rows, W, dtype):
+    """More rows than rows of partial sums: wide ones, odd widths and others."""
+    x, w, b, dy = inputs(rows, (rows, W), dtype)
+    check(x, w, b, dy, 1e-5, dtype, *run(dk, x, w, b, dy, 1e-5, dtype))
+
+
+@pytest.mark.parametrize("W", [40, 9000, 33000])
+def test_gradients_that_nobody_wants(dk, W):
+    x, w, b, dy = inputs(3, (70, W), torch.float32)
+    x, w, b, dy = dev(x), dev(w), dev(b), dev(dy)
+    _, mean, inv = dk.layer_norm_forward(x, w, b)
+    dx, dw, db = dk.layer_norm_backward(x, w, mean, inv, dy)
+    assert torch.equal(dk.layer_norm_backward(x, w, mean, inv, dy, want_bias=False, want_weight=False)[0], dx)
+    only = dk.layer_norm_backward(x, w, mean, inv, dy, want_x=False)
+    assert only[0] is None and torch.equal(only[1], dw) and torch.equal(only[2], db)
+
+
 def test_no_rows(dk):
     for dtype in (torch.float32, torch.bfloat16):
         x = torch.empty((0, 64), dtype=dtype, device="cuda", requires_grad=True)

@@ -132,9 +132,10 @@ def test_widths(dk, K, V, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("head_decay", [False, True])
 @pytest.mark.parametrize("masks", [False, True])
-def test_segments_of_long_sequences(dk, masks, head_decay, dtype):
+@pytest.mark.parametrize("K,V", [(12, 9), (70, 9)])
+def test_segments_of_long_sequences(dk, K, V, masks, head_decay, dtype):
     """One sequence is cut into many segments; memories longer than a segment."""
-    p = problem(5, 1, 1100, 1, 12, 9, dtype, masks=masks, head_decay=head_decay, initial=True,
+    p = problem(5, 1, 1100, 1, K, V, dtype, masks=masks, head_decay=head_decay, initial=True,
                 final=True, slow=True)
     compare(run(dk, p, dtype), p, dtype)
 
@@ -145,9 +146,10 @@ def test_many_sequences_in_one_segment(dk):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
-def test_gates_at_their_limits(dk, dtype):
+@pytest.mark.parametrize("V", [8, 72])
+def test_gates_at_their_limits(dk, V, dtype):
     """Decays of 0 (-inf, and far below what exp holds), of 1, growth, and a reset at every token."""
-    p = problem(7, 1, 140, 2, 8, 8, dtype, masks=True, initial=True, final=True)
+    p = problem(7, 1, 140, 2, 8, V, dtype, masks=True, initial=True, final=True)
     g = p["g"]
     g[0, 10, 0], g[0, 70, 1], g[0, 100, 0] = -np.inf, -500.0, -104.0
     g[0, 20:60, 1] = 0.0
@@ -213,10 +215,11 @@ def test_padding_may_hold_anything(dk, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("name", ["q", "k", "v", "g", "do"])
-def test_a_value_that_is_not_finite_stays_with_those_that_see_it(dk, name, dtype):
+@pytest.mark.parametrize("V", [16, 80])
+def test_a_value_that_is_not_finite_stays_with_those_that_see_it(dk, V, name, dtype):
     """A NaN at one token of one document reaches that document's later outputs (and the gradients of
     what they depend on), but no earlier token's output, no other document and no other sequence."""
-    p = problem(11, 2, 200, 2, 16, 16, dtype, masks=False)
+    p = problem(11, 2, 200, 2, 16, V, dtype, masks=False)
     p["reset"] = np.zeros((2, 200))
     p["reset"][0, [40, 150]] = 1
     p["valid"] = np.ones((2, 200))
@@ -314,8 +317,26 @@ def test_gradient_is_that_of_differences(dk):
         assert abs(want - have) <= 2e-3 * scale, n
 
 
-def test_gradients_that_nobody_wants(dk):
-    p = problem(14, 1, 100, 2, 16, 16, torch.float32, initial=True)
+@pytest.mark.parametrize("K", [16, 66])
+@pytest.mark.parametrize("T", [40, 400, 1100])
+def test_a_forward_that_no_backward_follows(dk, T, K):
+    """The same output and state, from a checkpoint that a backward refuses where it holds too little."""
+    from delta_kernels._lib import Gdn2Error
+    p = problem(16, 1, T, 2, K, 16, torch.bfloat16, masks=True, initial=True)
+    x = [dev(p[n], torch.bfloat16) for n in ("q", "k", "v")]
+    x += [dev(p[n]) for n in ("g", "valid", "reset", "initial")]
+    out, fin, ck = dk.linear_attention_forward(*x)
+    o2, f2, scratch = dk.linear_attention_forward(*x, train=False)
+    assert torch.equal(out, o2) and torch.equal(fin, f2)
+    assert scratch.numel() <= ck.numel()
+    if scratch.numel() < ck.numel():
+        with pytest.raises(Gdn2Error, match="checkpoint"):
+            dk.linear_attention_backward(*x, scratch, out)
+
+
+@pytest.mark.parametrize("K", [16, 66])
+def test_gradients_that_nobody_wants(dk, K):
+    p = problem(14, 1, 100, 2, K, 16, torch.float32, initial=True)
     ref = run(dk, p, torch.float32)
     x = {n: dev(p[n]) for n in ("q", "k", "v", "g", "initial")}
     names = dict(q="dq", k="dk", v="dv", g="dg", initial="dinitial")

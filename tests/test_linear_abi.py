@@ -76,6 +76,16 @@ def test_bad_buffers(L):
     assert "workspace" in message(L)
 
 
+@pytest.mark.parametrize("T", [1, 64, 512, 5000])
+@pytest.mark.parametrize("K", [16, 100])
+def test_a_forward_alone_needs_less(L, K, T):
+    from delta_kernels._lib import Gdn2Shape
+    s = Gdn2Shape.from_buffer_copy(shape(T=T, K=K))
+    sizes = [L.gdn2_linear_checkpoint_bytes(s, 0, train) for train in (0, 1)]
+    assert 0 < sizes[0] <= sizes[1]
+    assert K > 64 or sizes[0] < sizes[1]
+
+
 def test_step_takes_one_token(L):
     assert L.gdn2_linear_step(shape(), *[view()] * 4, None, None, 0x2000, 0x3000, None) == 2
     assert "time == 1" in message(L)
