@@ -23,9 +23,10 @@
 //
 // A sequence is cut into segments for parallel work; their start states come from a walk over (b, c) alone,
 // a launch of its own for all segments (carry) and a join over them, or, in short sequences, by each
-// segment from the sequence's start.  Operands of matrix products are the inputs' type.  In bf16 the pair
-// weights and, for the output, the state are rounded once, as the result is; the state itself, its update
-// and the sums of the gate's gradient keep float32 accuracy (three bf16 terms).
+// segment from the sequence's start.  Operands of matrix products are the inputs' type.  In bf16 a float32
+// operand goes in as several bf16 terms, so that only the result is rounded: a state has three (float32
+// accuracy), a pair weight, and the adjoint state where it makes dk, two.  Those are off by 2^-16, next to a result
+// that is rounded to 2^-8 in its turn.
 #include <math.h>
 
 #include <algorithm>
@@ -116,12 +117,28 @@ template <> struct Mat<float> {
     }
 };
 
+// Two bf16 terms hold a float32 to 2^-16 of its value.  The remainder is that of the rounded float32, whatever
+// product it came from: the terms are the same bits in every kernel that makes them.
+__device__ __forceinline__ void split2(const f32x4 &x, bf16_t (&hi)[4], bf16_t (&lo)[4]) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        hi[i] = f32_to_bf16(x[i]);
+        lo[i] = f32_to_bf16(x[i] - bf16_to_f32(hi[i]));
+    }
+}
+__device__ __forceinline__ void split2(const f32x4 &x, float (&hi)[4], float (&)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = x[i];
+}
+
 // Three bf16 terms hold a float32 to its last bit or two, so a product over them with an exact bf16
 // operand keeps float32 accuracy: the state and its update are float32 results.
 struct Split3 {
     bf16x8_t t[3];
 };
 __device__ __forceinline__ Split3 split3(const float (&x)[8]) {
+#pragma clang fp contract(off)
     Split3 s;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -133,6 +150,15 @@ __device__ __forceinline__ Split3 split3(const float (&x)[8]) {
         s.t[2][e] = static_cast<__bf16>(r - static_cast<float>(b));
     }
     return s;
+}
+
+// The same number, of which the compiler does not know it: what follows from it (addresses, conditions) is made
+// where it is used, and not kept in registers through the loop over chunks.  Without it linear_back spilled 39
+// registers at 64 x 64, whose reloads wait for the loads of the next chunk before them: 74 us in place of 65 for 16 x
+// 512 tokens, 8 heads of 64, both directions.
+__device__ __forceinline__ int hidden(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // The chunks, gates and states of a walk.  Tensor views are [B, T, H, channels].
@@ -314,7 +340,7 @@ struct Staged {
 template <typename T, int TT, bool VEC>
 __device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int width, int left, bool whole,
                                            const f32x4 (&x)[TT]) {
-    const int n16 = lane_id() & 15;
+    const int n16 = hidden(lane_id()) & 15;
     T *p = out + n16 * stride + col;
     if (VEC && whole && left >= 16 * TT) {
 #pragma unroll
@@ -343,10 +369,8 @@ __device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int 
     }
 }
 
-// Gam of the pairs of out token t with the sources s .. s + 3, 0 for those that t does not see.  EXACT
-// adds the sums' lower parts; without them a decay is off by 2^-24 of the sum since the last cut, at
-// most 2^-11 where the pair still counts, which a bf16 weight does not show.
-template <int C, bool REV, bool EXACT>
+// Gam of the pairs of out token t with the sources s .. s + 3, 0 for those that t does not see.
+template <int C, bool REV>
 __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s) {
     const float ht = gt.hi[t];
     const int st = gt.seg[t];
@@ -356,12 +380,10 @@ __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s
     f32x4 f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = REV ? hs[i] - ht : ht - hs[i];
-    if (EXACT) {
-        const float lt = gt.lo[t];
-        const f32x4 ls = *reinterpret_cast<const f32x4 *>(gt.lo + s);
+    const float lt = gt.lo[t];
+    const f32x4 ls = *reinterpret_cast<const f32x4 *>(gt.lo + s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] += REV ? ls[i] - lt : lt - ls[i];
-    }
+    for (int i = 0; i < 4; ++i) f[i] += REV ? ls[i] - lt : lt - ls[i];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const bool on = seg[i] == st && (REV ? s + i >= t : s + i <= t);
@@ -388,7 +410,11 @@ template <typename T, int KP, int CP, bool OUT, bool DOT>
 struct WalkLds {
     static constexpr int C = Mat<T>::C, LDA = Mat<T>::ld(KP), LDC = Mat<T>::ld(CP), LDP = Mat<T>::ld(C);
     T b[C * LDA], c[C * LDC];
-    T a[OUT ? C * LDA : 8], p[OUT ? C * LDP : 8], d[DOT ? C * LDC : 8];
+    // Terms of the pair weights: the second behind the first, with DOT in the place of d once that is read (two
+    // workgroups share a unit at 128 x 64).
+    static constexpr int TERMS = sizeof(T) == 2 ? 2 : 1, ROOM = DOT ? 1 : TERMS;
+    static_assert(LDC >= LDP, "");
+    T a[OUT ? C * LDA : 8], p[OUT ? ROOM * C * LDP : 8], d[DOT ? C * LDC : 8];
     GateTile<C> gate[kGates];
     float red[CP / 16][C];
     float rows[C / 16][C], cols[C / 16][C];  // parts of the pair sums, by tiles of 16 tokens
@@ -399,8 +425,10 @@ struct BackLds {
     static constexpr int C = Mat<T>::C, LDK = Mat<T>::ld(KP), LDV = Mat<T>::ld(VP), LDP = Mat<T>::ld(C),
                          NW = (KP > VP ? KP : VP) / 16;
     T q[C * LDK], k[C * LDK], v[C * LDV], o[C * LDV];
-    T pk[C * LDP], pv[C * LDP];  // Gam k.q and Gam v.do; the token-by-token form keeps float sums in pk
-    T D[VP * LDK];               // the adjoint state transposed, [row_for(value)][key]
+    // First terms of Gam k.q and Gam v.do (the token-by-token form keeps float sums in pk), and of the adjoint state
+    // transposed, [row_for(value)][key].  The second terms take the places of o, k and D once those are read.
+    T pk[C * LDP], pv[C * LDP];
+    T D[VP * LDK];
     GateTile<C> gate[kGates];
     float red[NW][C], red_q[ALL ? NW : 1][C];
     float rows[ALL ? C / 16 : 1][C], cols[ALL ? C / 16 : 1][C];  // parts of the pair sums, as in WalkLds
@@ -473,7 +501,8 @@ struct State {
     __device__ __forceinline__ void load_transposed(const float *src, int v, int rows, int cols) {
         zero();
         if ((v & ~15) >= cols) return;
-        src += M::place(0, 4 * (lane_id() >> 4)) * cols + v;
+        v = hidden(v);
+        src += M::place(0, 4 * (hidden(lane_id()) >> 4)) * cols + v;
 #pragma unroll
         for (int m = 0; m < KT; ++m)
             if (M::place(m, 0) < rows)
@@ -543,9 +572,8 @@ __device__ __forceinline__ bool update(State<T, KP / 16> &U, const State<T, KP /
     return U.finite();
 }
 
-// acc[j] += (row t of x) S for the tokens t of tile j: rows = the wave's columns, column = t.  THREE
-// terms of the state give float32 accuracy; with one, the state is rounded to bf16, as the result is.
-template <typename T, int KP, bool THREE>
+// acc[j] += (row t of x) S for the tokens t of tile j: rows = the wave's columns, column = t.
+template <typename T, int KP>
 __device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const State<T, KP / 16> &S, const T *x, int ld) {
     typedef Mat<T> M;
 #pragma unroll
@@ -557,7 +585,7 @@ __device__ __forceinline__ void state_rows(f32x4 (&acc)[Mat<T>::C / 16], const S
 #pragma unroll
             for (int j = 0; j < M::C / 16; ++j) y[j] = M::row(x + 16 * j * ld, ld, r * M::RB);
 #pragma unroll
-            for (int q = 0; q < (THREE ? 3 : 1); ++q)
+            for (int q = 0; q < 3; ++q)
 #pragma unroll
                 for (int j = 0; j < M::C / 16; ++j) M::mma(acc[j], s3.t[q], y[j]);
         } else {
@@ -577,7 +605,7 @@ __device__ __forceinline__ float pick(int i, float a, float b, float c, float d)
 // with factor 0 gives 0, also where the state is not finite.
 template <typename T, int TT>
 __device__ __forceinline__ void dot_rows(const f32x4 (&acc)[TT], const float (&f)[TT], const T *d, int ld, float *red) {
-    const int lane = lane_id(), n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int lane = hidden(lane_id()), n16 = lane & 15, g4 = 4 * (lane >> 4);
     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
@@ -659,7 +687,8 @@ __device__ __forceinline__ void walk_tokens(State<T, KP / 16> &S, const T *a, co
                                             const GateTile<Mat<T>::C> &gate, int ka, int v, int vc,
                                             T *out, int64_t stride, int tokens) {
     constexpr int KT = KP / 16, C = Mat<T>::C, LDA = Mat<T>::ld(KP);
-    const int g4 = 4 * (lane_id() >> 4);
+    const int g4 = hidden(4 * (lane_id() >> 4));
+    v = hidden(v);
 #pragma unroll 1
     for (int n = 0; n < C; ++n) {
         const int t = REV ? C - 1 - n : n;
@@ -770,7 +799,8 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
                   LDP = L::LDP, BT = RB / 16;  // BT: accumulator tiles of one fragment
     constexpr int NW = CP / 16;
     __shared__ L lds;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int lane = lane_id(), n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int v = 16 * wave + n16;
     const int segs = p.segments - (OUT ? 0 : 1);
     const Place at = place(p, segs, REV, OUT);
@@ -871,6 +901,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         // bf16, three in float32.
         constexpr int MINE = TT == 4 ? (12 + NW - 1) / NW : 1;
         f32x4 y[MINE];
+        T lo[MINE][4];
         int tjs[MINE], sis[MINE];
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
@@ -888,11 +919,15 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             for (int r = 0; r < KP; r += RB)
                 M::mma(x, M::row(lds.b + 16 * si * LDA, LDA, r), M::row(lds.a + 16 * tj * LDA, LDA, r));
             const int t = 16 * tj + n16, s = 16 * si + g4;
-            const f32x4 f = pair_decays<C, false, DOT || sizeof(T) == 4>(gate, t, s);
-            T e[4];
+            const f32x4 f = pair_decays<C, false>(gate, t, s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[i] *= f[i]);
-            __builtin_memcpy(__builtin_assume_aligned(lds.p + t * LDP + M::place(si, g4), 4 * sizeof(T)), e, sizeof e);
+            for (int i = 0; i < 4; ++i) x[i] *= f[i];
+            T hi[4];
+            split2(x, hi, lo[m]);
+            T *at_p = lds.p + t * LDP + M::place(si, g4);
+            __builtin_memcpy(__builtin_assume_aligned(at_p, 4 * sizeof(T)), hi, sizeof hi);
+            if (L::ROOM == 2)
+                __builtin_memcpy(__builtin_assume_aligned(at_p + C * LDP, 4 * sizeof(T)), lo[m], sizeof hi);
             if (DOT) {
                 y[m] = zero4();
 #pragma unroll
@@ -932,7 +967,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         f32x4 acc[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) acc[j] = zero4();
-        state_rows<T, KP, DOT>(acc, S, lds.a, LDA);
+        state_rows<T, KP>(acc, S, lds.a, LDA);
         float f[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
@@ -952,10 +987,20 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             if (in) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
         }
 
+        constexpr bool LATE = DOT && L::TERMS == 2;
+        if constexpr (LATE)
+#pragma unroll
+            for (int m = 0; m < MINE; ++m)
+                if (tjs[m] >= 0)
+                    __builtin_memcpy(__builtin_assume_aligned(
+                                         lds.d + (16 * tjs[m] + n16) * LDP + M::place(sis[m], g4), 4 * sizeof(T)),
+                                     lo[m], sizeof lo[m]);
         typename M::Frag cf[C / RB];
         across_c(cf);
         State<T, KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
+        if (LATE) __syncthreads();
+        const T *const terms[2] = {lds.p, DOT ? lds.d : lds.p + C * LDP};
         T *o = reinterpret_cast<T *>(p.out);
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
         const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
@@ -964,7 +1009,9 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             for (int j = 0; j < TT; ++j)
 #pragma unroll
                 for (int r = 0; r <= j / BT; ++r)
-                    M::mma(acc[j], cf[r], M::row(lds.p + 16 * j * LDP, LDP, r * RB));
+#pragma unroll
+                    for (int q = 0; q < L::TERMS; ++q)
+                        M::mma(acc[j], cf[r], M::row(terms[q] + 16 * j * LDP, LDP, r * RB));
             if (o)
                 store_rows<T, TT, VEC>(o + row0 * p.vc, (int64_t)p.H * p.vc, 16 * wave + g4, p.vc, left,
                                        p.vc == CP, acc);
@@ -1004,7 +1051,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     constexpr int C = M::C, TT = C / 16, KT = KP / 16, RB = M::RB, LDK = L::LDK, LDV = L::LDV,
                   LDP = L::LDP, BT = RB / 16, NW = L::NW, THREADS = 64 * NW;
     __shared__ L lds;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int lane = lane_id(), n16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int v = 16 * wave + n16;
     const bool own_v = 16 * wave < VP, own_k = 16 * wave < KP;
     const Place at = place(p, p.segments, true, true);
@@ -1099,7 +1147,6 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int w = 0; w < VP / 16; ++w) edge += lds.red[w][0];
             __syncthreads();
         }
-        F.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
     }
 
     for (; n > 0; --n, --ci) {
@@ -1109,15 +1156,17 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         sk.template store<LDK>(lds.k, gate.seg, masks, p.K);
         sv.template store<LDV>(lds.v, gate.seg, masks, p.V);
         so.template store<LDV>(lds.o, gate.seg, masks, p.V);
-        if (own_v) {
+        const auto put_D = [&](int term) {
 #pragma unroll
             for (int m = 0; m < KT; ++m) {
-                T e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, S.t[m][i]);
-                __builtin_memcpy(__builtin_assume_aligned(lds.D + M::row_for(v) * LDK + M::place(m, g4), 4 * sizeof(T)), e, sizeof e);
+                T e[2][4];
+                split2(S.t[m], e[0], e[1]);
+                __builtin_memcpy(__builtin_assume_aligned(lds.D + M::row_for(v) * LDK + M::place(m, g4), 4 * sizeof(T)),
+                                 e[term], sizeof e[0]);
             }
-        }
+        };
+        if (own_v) put_D(0);
+        if (ALL) F.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
         if (n > 1) fetch(ci - 1, true);
         __syncthreads();
 
@@ -1125,6 +1174,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         // but from the other end.
         constexpr int MINE = TT == 4 ? (12 + NW - 1) / NW : 1;
         f32x4 W[MINE];
+        T pk_lo[MINE][4], pv_lo[MINE][4];
         int sjs[MINE], tis[MINE];
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
@@ -1132,6 +1182,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             int sj = id >> 1, ti = id & 1;
             if (TT == 4 && id >= 4) sj = id < 8 ? 2 : 3, ti = id & 3;
             sjs[m] = TT - 1 - sj, tis[m] = TT - 1 - ti;
+            const int lane = hidden(lane_id()), n16 = lane & 15, g4 = 4 * (lane >> 4);
             if ((TT == 4 && 12 % NW && id >= 12) || (TT == 2 && (id >= 4 || ti > sj))) {
                 sjs[m] = -1;
                 continue;
@@ -1145,20 +1196,24 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int r = 0; r < VP; r += RB)
                 M::mma(y, M::row(lds.o + 16 * ti * LDV, LDV, r), M::row(lds.v + 16 * sj * LDV, LDV, r));
             const int s = 16 * sj + n16, t = 16 * ti + g4;
-            const f32x4 f = pair_decays<C, true, ALL || sizeof(T) == 4>(gate, s, t);
-            T e[4], g[4];
+            const f32x4 f = pair_decays<C, true>(gate, s, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float a = x[i] * f[i];
-                Elem<T>::store(e, i, a), Elem<T>::store(g, i, y[i] * f[i]);
-                if (ALL) W[m][i] = f[i] == 0.f || t + i <= s ? 0.f : a * y[i];
+                x[i] *= f[i];
+                if (ALL) W[m][i] = f[i] == 0.f || t + i <= s ? 0.f : x[i] * y[i];
+                y[i] *= f[i];
             }
-            __builtin_memcpy(__builtin_assume_aligned(lds.pk + s * LDP + M::place(ti, g4), 4 * sizeof(T)), e, sizeof e);
-            __builtin_memcpy(__builtin_assume_aligned(lds.pv + s * LDP + M::place(ti, g4), 4 * sizeof(T)), g, sizeof g);
+            T e[4], g[4];
+            split2(x, e, pk_lo[m]);
+            split2(y, g, pv_lo[m]);
+            const int at_p = s * LDP + M::place(ti, g4);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pk + at_p, 4 * sizeof(T)), e, sizeof e);
+            __builtin_memcpy(__builtin_assume_aligned(lds.pv + at_p, 4 * sizeof(T)), g, sizeof g);
         }
         if (gates_too) {
             // As in linear_walk, with t along the rows: sums over the s of a tile for each t, over its t for each
             // s, and on the diagonal for each token over the t from it on and the s before it.
+            const int lane = hidden(lane_id()), n16 = lane & 15, g4 = 4 * (lane >> 4);
             float q[MINE], a[MINE], b[MINE], c[MINE];
 #pragma unroll
             for (int m = 0; m < MINE; ++m) q[m] = (W[m][0] + W[m][1]) + (W[m][2] + W[m][3]);
@@ -1186,22 +1241,42 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         f32x4 av[TT], ak[TT];
 #pragma unroll
         for (int j = 0; j < TT; ++j) av[j] = ak[j] = zero4();
-        State<T, KT> U;
-        U.zero();
-        typename M::Frag of[C / RB];
-        bool good = fine;
-        if (own_v) {
-            state_rows<T, KP, DOT>(av, S, lds.k, LDK);
-            across_o(of);
-            good = update<T, KP>(U, S, gate.tot, of, lds.q, gate.col) && fine;
-        }
-        if (own_k) {
+        const auto dk_state = [&](f32x4 (&acc)[TT]) {  // with the term of the state that is in LDS
 #pragma unroll
             for (int r = 0; r < VP; r += RB) {
                 const typename M::Frag x = M::template across<LDK>(lds.D, r, 16 * wave);
 #pragma unroll
-                for (int j = 0; j < TT; ++j) M::mma(ak[j], x, M::row(lds.v + 16 * j * LDV, LDV, r));
+                for (int j = 0; j < TT; ++j) M::mma(acc[j], x, M::row(lds.v + 16 * j * LDV, LDV, r));
             }
+        };
+        State<T, KT> U;
+        U.zero();
+        typename M::Frag of[C / RB], kf[ALL ? C / RB : 1];
+        bool good = fine;
+        if (own_v) {
+            state_rows<T, KP>(av, S, lds.k, LDK);
+            across_o(of);
+            good = update<T, KP>(U, S, gate.tot, of, lds.q, gate.col) && fine;
+        }
+        if (own_k) {
+            dk_state(ak);
+            if constexpr (ALL)
+#pragma unroll
+                for (int r = 0; r < C / RB; ++r) kf[r] = M::template across<LDK>(lds.k, r * RB, 16 * wave);
+        }
+        f32x4 aq[TT];
+        if (ALL) {
+#pragma unroll
+            for (int j = 0; j < TT; ++j) aq[j] = zero4();
+            state_rows<T, VP>(aq, F, lds.o, LDV);
+            // A value of k or v that is not finite shows in these products, whatever the state: then dq, too, is
+            // taken token by token.
+            float z = 0.f;
+#pragma unroll
+            for (int j = 0; j < TT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z = fmaf(aq[j][i], 0.f, fmaf(av[j][i], 0.f, fmaf(ak[j][i], 0.f, z)));
+            good = good && !__any(z != 0.f);
         }
         float f[TT];
 #pragma unroll
@@ -1211,20 +1286,15 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int i = 0; i < 4; ++i) av[j][i] *= f[j], ak[j][i] *= f[j];
         }
         if (DOT && own_v && (!ALL || gates_too)) dot_rows<T, TT>(av, f, lds.v + 16 * wave, LDV, lds.red[wave]);
-        f32x4 aq[TT];
         if (ALL) {
-#pragma unroll
-            for (int j = 0; j < TT; ++j) aq[j] = zero4();
-            if (gates_too) state_rows<T, VP, true>(aq, F, lds.o, LDV);
-            else state_rows<T, VP, false>(aq, F, lds.o, LDV);
+            float c[TT];
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
-                f[j] = gate.col[16 * j + n16];  // of the walk in order
+                c[j] = gate.col[16 * j + n16];  // of the walk in order
 #pragma unroll
-                for (int i = 0; i < 4; ++i) aq[j][i] *= f[j];
+                for (int i = 0; i < 4; ++i) aq[j][i] *= c[j];
             }
-            if (gates_too) dot_rows<T, TT>(aq, f, lds.q + 16 * wave, LDK, lds.red_q[wave]);
-            if (n > 1) F.load_transposed(kept + (ci - 1) * size, v, up32(p.V), up32(p.K));
+            if (gates_too) dot_rows<T, TT>(aq, c, lds.q + 16 * wave, LDK, lds.red_q[wave]);
         }
         if (!good && lane == 0) lds.bad[n & 1] = 1;
         __syncthreads();
@@ -1248,59 +1318,81 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         const int left = (int)min(p.T - (int64_t)ci * C, (int64_t)C);
         const int64_t row0 = (at.b * p.T + (int64_t)ci * C) * p.H + at.h;
         T *dv = reinterpret_cast<T *>(p.dv), *dk = reinterpret_cast<T *>(p.dk);
-        if (ALL && p.dq) {
-            typename M::Frag kf[C / RB];
+        T *dq = ALL && p.dq ? reinterpret_cast<T *>(p.dq) + row0 * p.K : nullptr;
+        if (__builtin_expect(!bad, 1)) {
+            T *const pk_of[2] = {lds.pk, lds.o}, *const pv_of[2] = {lds.pv, lds.k};
+            constexpr int TERMS = sizeof(T) == 2 ? 2 : 1;
+            if constexpr (TERMS == 2) {
 #pragma unroll
-            for (int r = 0; r < C / RB; ++r) kf[r] = M::template across<LDK>(lds.k, r * RB, 16 * wave);
-            float z = 0.f;
-#pragma unroll
-            for (int j = 0; j < TT; ++j) {
-#pragma unroll
-                for (int r = 0; r <= j / BT; ++r)
-                    M::mma(aq[j], kf[r], M::template across_place<LDP>(lds.pv, r * RB, j));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z = fmaf(aq[j][i], 0.f, z);
+                for (int m = 0; m < MINE; ++m) {
+                    if (sjs[m] < 0) continue;
+                    const int at_p = (16 * sjs[m] + n16) * LDP + M::place(tis[m], g4);
+                    __builtin_memcpy(__builtin_assume_aligned(lds.o + at_p, 8), pk_lo[m], 8);
+                    __builtin_memcpy(__builtin_assume_aligned(lds.k + at_p, 8), pv_lo[m], 8);
+                }
+                if (own_v) put_D(1);
             }
-            T *dq = reinterpret_cast<T *>(p.dq) + row0 * p.K;
-            if (__builtin_expect(!__any(z != 0.f) && p.T > kFew, 1)) {
-                store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, aq);
-            } else {
-                // k, v or the state before the chunk may not be finite: token by token, from that state again
-                no_loads_left();
+            static_assert(LDV >= LDP && LDK >= LDP, "");
+#pragma unroll
+            for (int q = 0; q < TERMS; ++q) {
+                if (q == 1) {
+                    __syncthreads();
+                    if (dk && own_k) {
+                        f32x4 x[TT];
+#pragma unroll
+                        for (int j = 0; j < TT; ++j) x[j] = zero4();
+                        dk_state(x);
+#pragma unroll
+                        for (int j = 0; j < TT; ++j) {
+                            const float row = gate.row[16 * j + n16];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) ak[j][i] = fmaf(row, x[j][i], ak[j][i]);
+                        }
+                    }
+                }
+                if (dv && own_v) {
+#pragma unroll
+                    for (int j = 0; j < TT; ++j)
+#pragma unroll
+                        for (int r = j / BT; r < C / RB; ++r)
+                            M::mma(av[j], of[r], M::row(pk_of[q] + 16 * j * LDP, LDP, r * RB));
+                }
+                if (dk && own_k) {
+                    typename M::Frag qf[C / RB];
+#pragma unroll
+                    for (int r = 0; r < C / RB; ++r) qf[r] = M::template across<LDK>(lds.q, r * RB, 16 * wave);
+#pragma unroll
+                    for (int j = 0; j < TT; ++j)
+#pragma unroll
+                        for (int r = j / BT; r < C / RB; ++r)
+                            M::mma(ak[j], qf[r], M::row(pv_of[q] + 16 * j * LDP, LDP, r * RB));
+                }
+                if constexpr (ALL)
+                    if (dq) {
+#pragma unroll
+                        for (int j = 0; j < TT; ++j)
+#pragma unroll
+                            for (int r = 0; r <= j / BT; ++r)
+                                M::mma(aq[j], kf[r], M::template across_place<LDP>(pv_of[q], r * RB, j));
+                    }
+            }
+            if (ALL && dq) store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, aq);
+            else no_loads_left();
+            if (dv && own_v) store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, p.V == VP, av);
+            else no_loads_left();
+            if (dk && own_k) store_rows<T, TT, VEC>(dk + row0 * p.K, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, ak);
+            else no_loads_left();
+            S = U;
+        } else {
+            no_loads_left();
+            if (ALL && dq) {  // from the state before the chunk again
                 State<T, VP / 16> G;
                 G.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
                 walk_tokens<T, VP, LDK, false, true>(G, lds.o, lds.v, lds.k, gate, p.V, v, p.K, dq,
                                                      (int64_t)p.H * p.K, left);
             }
-        }
-        if (__builtin_expect(!bad, 1)) {
-            if (dv && own_v) {
-#pragma unroll
-                for (int j = 0; j < TT; ++j)
-#pragma unroll
-                    for (int r = j / BT; r < C / RB; ++r)
-                        M::mma(av[j], of[r], M::row(lds.pk + 16 * j * LDP, LDP, r * RB));
-                store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, p.V == VP, av);
-            } else {
-                no_loads_left();
-            }
-            if (dk && own_k) {
-                typename M::Frag qf[C / RB];
-#pragma unroll
-                for (int r = 0; r < C / RB; ++r) qf[r] = M::template across<LDK>(lds.q, r * RB, 16 * wave);
-#pragma unroll
-                for (int j = 0; j < TT; ++j)
-#pragma unroll
-                    for (int r = j / BT; r < C / RB; ++r)
-                        M::mma(ak[j], qf[r], M::row(lds.pv + 16 * j * LDP, LDP, r * RB));
-                store_rows<T, TT, VEC>(dk + row0 * p.K, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, ak);
-            } else {
-                no_loads_left();
-            }
-            S = U;
-        } else {
-            no_loads_left();
             // Token by token, all waves together: see walk_tokens.
+            const int v = hidden(16 * wave + n16), g4 = hidden(4 * (lane >> 4));
             float *part = reinterpret_cast<float *>(lds.pk);  // [NW][KP]: dk's sums over a wave's columns
             static_assert(sizeof(lds.pk) >= sizeof(float) * NW * KP, "");
 #pragma unroll 1
