@@ -40,12 +40,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGates = 8;       // chunks whose gates are made at a time
-// Sequences of up to so many tokens are taken token by token, with nothing rounded but the result: they have a
-// few pair weights, each of which a whole row of the result hangs on, and a rounding of one to bf16 shows there
-// undiminished (in the mean of many the result is off by 1.7e-3 of its norm, as a chunk by 2.3e-3).  That is
-// paid for: 256 x 8 heads of 64 on a state, bf16, take 36 us forward for one token and 45 for four (as a chunk
-// 25), and 99 and 165 backward (66).  The same line at 8 tokens would cost 57 and 251 in place of 25 and 66.
-constexpr int kFew = 4;
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
@@ -840,7 +834,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     __syncthreads();
 
     const bool odd = p.valid.data || p.ka < KP || p.vc < CP;
-    bool fine = S.finite() && p.T > kFew;  // products take a chunk only where the state before it is finite
+    bool fine = S.finite();  // products take a chunk only where the state before it is finite
     const auto across_c = [&](typename M::Frag (&cf)[C / RB]) {
 #pragma unroll
         for (int r = 0; r < C / RB; ++r) cf[r] = M::template across<LDC>(lds.c, r * RB, 16 * wave);
@@ -1090,7 +1084,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     __syncthreads();
 
     const bool odd = p.valid.data || p.K < KP || p.V < VP;
-    bool fine = S.finite() && p.T > kFew;
+    bool fine = S.finite();
     const auto across_o = [&](typename M::Frag (&of)[C / RB]) {
 #pragma unroll
         for (int r = 0; r < C / RB; ++r) of[r] = M::template across<LDV>(lds.o, r * RB, 16 * wave);
