@@ -39,7 +39,6 @@ namespace gdn2 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGates = 8;       // chunks whose gates are made at a time
 constexpr float kCut = -110.f;  // exp(g) is 0 in float32 below: such a gate cuts like a reset
 
 // Matrix operations of one element type: a fragment holds RB entries of the reduction for 16 rows.
@@ -409,9 +408,12 @@ struct WalkLds {
     static constexpr int TERMS = sizeof(T) == 2 ? 2 : 1, ROOM = DOT ? 1 : TERMS;
     static_assert(LDC >= LDP, "");
     T a[OUT ? C * LDA : 8], p[OUT ? ROOM * C * LDP : 8], d[DOT ? C * LDC : 8];
-    GateTile<C> gate[kGates];
-    float red[CP / 16][C];
-    float rows[C / 16][C], cols[C / 16][C];  // parts of the pair sums, by tiles of 16 tokens
+    // Chunks whose gates are made at a time.  With four and without the sums of DOT three forward workgroups share
+    // a unit at 64 x 64 (2048 heads of 8 tokens, bf16: 31.7 us by twos).
+    static constexpr int GATES = OUT && !DOT && CP == 64 ? 4 : 8;
+    GateTile<C> gate[GATES];
+    float red[DOT ? CP / 16 : 1][C];
+    float rows[DOT ? C / 16 : 1][C], cols[DOT ? C / 16 : 1][C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
 template <typename T, int KP, int VP, bool ALL>
@@ -423,7 +425,8 @@ struct BackLds {
     // transposed, [row_for(value)][key].  The second terms take the places of o, k and D once those are read.
     T pk[C * LDP], pv[C * LDP];
     T D[VP * LDK];
-    GateTile<C> gate[kGates];
+    static constexpr int GATES = 8;  // as in WalkLds
+    GateTile<C> gate[GATES];
     float red[NW][C], red_q[ALL ? NW : 1][C];
     float rows[ALL ? C / 16 : 1][C], cols[ALL ? C / 16 : 1][C];  // parts of the pair sums, as in WalkLds
     int bad[2];                  // whether any wave's state is not finite, in turn for even and odd chunks
@@ -745,9 +748,9 @@ __device__ __forceinline__ void start_state(State<T, KT> &S, const Walk &p, cons
 }
 
 // Gates of the next chunks of a walk with n left, from chunk ci on.
-template <int C, bool REV, int NW>
+template <int C, bool REV, int NW, int GATES>
 struct MakeGates {
-    static constexpr int EACH = kGates / NW;  // chunks of each wave
+    static constexpr int EACH = GATES / NW;  // chunks of each wave
     GateIn x[EACH];
     int ci, n;
     __device__ __forceinline__ void load(const Walk &p, const Place &at, int chunk, int left) {
@@ -822,7 +825,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         }
     };
     // All first loads are on their way before the first is waited for.
-    MakeGates<C, REV, NW> gates;
+    MakeGates<C, REV, NW, L::GATES> gates;
     gates.load(p, at, ci, n);
     State<T, KT> S;
     S.zero();
@@ -866,7 +869,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             fine = S.finite();
         }
         __syncthreads();  // the chunk's tiles are read
-        if (++gi == kGates && n > 1) next_gates();
+        if (++gi == L::GATES && n > 1) next_gates();
     }
     if (!OUT) {
         S.store(p.seg_state + ((int64_t)at.bh * p.segments + at.seg) * p.ka * p.vc, v, p.ka, p.vc);
@@ -931,7 +934,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
                 for (int i = 0; i < 4; ++i) y[m][i] = f[i] == 0.f || s + i >= t ? 0.f : x[i] * y[m][i];
             }
         }
-        if (DOT) {
+        if constexpr (DOT) {
             // By tiles: the sums over s for each row, and over the rows for each s; of a tile on the diagonal, for
             // each of its tokens, the sum over the rows from it on and the s before it.  All tiles of the wave
             // side by side.
@@ -969,9 +972,9 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] *= f[j];
         }
-        if (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
+        if constexpr (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
-        if (DOT && wave == 1) {
+        if constexpr (DOT) if (wave == 1) {
             const bool in = lane < C && token < p.T;
             const float x = sum_dots<C, NW>(lds.red), y = in ? y_now : 0.f;
             const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(x);
@@ -1019,7 +1022,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             fine = S.finite();
         }
         __syncthreads();  // the chunk's tiles are read
-        if (++gi == kGates && n > 1) next_gates();
+        if (++gi == L::GATES && n > 1) next_gates();
     }
     if (at.nth != p.segments - 1) return;
     if (p.fin) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
@@ -1071,7 +1074,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             sv.load(pv, p.v.s1, p.v.s3, t0, left, p.V);
         }
     };
-    MakeGates<C, true, NW> gates;
+    MakeGates<C, true, NW, L::GATES> gates;
     gates.load(p, at, ci, n);
     State<T, KT> S;
     S.zero();
@@ -1117,7 +1120,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             }
         }
         __syncthreads();
-        if (++gi == kGates) next_gates();
+        if (++gi == L::GATES) next_gates();
     }
 
     // ALL: the forward's state before the chunk, transposed: rows = values, the wave's 16 columns = keys.
@@ -1426,7 +1429,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             fine = S.finite();
         }
         __syncthreads();  // the chunk's tiles are read
-        if (++gi == kGates && n > 1) next_gates();
+        if (++gi == L::GATES && n > 1) next_gates();
     }
 
     if (p.fin && own_v && at.seg == 0) S.store(p.fin + (int64_t)at.bh * p.K * p.V, v, p.K, p.V);
