@@ -860,7 +860,8 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         across_c(cf);
         State<T, KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
-        decay *= gate.tot;
+        // A cut leaves nothing of the start, whatever the gates before and after it are.
+        decay = decay == 0.f || gate.tot == 0.f ? 0.f : decay * gate.tot;
         if (__builtin_expect(fine && next, 1)) {
             S = U;
         } else {

@@ -1,0 +1,58 @@
+"""What is not finite in linear attention stays in its document, across the segments of a long sequence too.
+
+Bounds as in test_gpu_linear, with u = 2^-8, e = 2^-24 and A the same result of magnitudes: 2.1 u A for bf16
+results, 128 e A for float32 ones, and for dg 256 e max A over the sequence."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_linear import dk, oracle, problem, run, sizes, E, U  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def packed(seed, dtype, starts, T, V=16):
+    p = problem(seed, 1, T, 1, 16, V, dtype, initial=True, final=True)
+    p["reset"] = np.zeros((1, T))
+    p["reset"][0, list(starts)] = 1
+    return p
+
+
+def same_elsewhere(got, p, dtype, inside):
+    """got is the oracle's result of the clean problem p outside the document `inside`."""
+    ref, A = oracle(p), sizes(p)
+    T = p["q"].shape[1]
+    out = np.ones(T, bool)
+    out[inside] = False
+    for n in ("out", "dq", "dk", "dv", "dg"):
+        bound = 256 * E * A[n].max() if n == "dg" else \
+            (2.1 * U if dtype == torch.bfloat16 else 128 * E) * A[n][:, out] + 1e-30
+        err = np.abs(got[n] - ref[n])[:, out]
+        assert np.all(err <= bound), f"{n}: first at {np.argwhere(~(err <= bound))[0]}"
+    for n in ("fin", "dinitial"):
+        assert np.all(np.abs(got[n] - ref[n]) <= 128 * E * A[n] + 1e-30), n
+
+
+@DTYPES
+@pytest.mark.parametrize("V", [16, 80])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 200.0], ids=["nan", "inf", "overflow"])
+@pytest.mark.parametrize("forwards", [True, False], ids=["forward", "backward"])
+def test_a_gate_in_a_carried_segment(dk, forwards, bad, V, dtype):  # noqa: F811
+    """A gate that is not finite, or grows past float32, in one chunk of a segment of two, and a reset in the
+    other: the document behind the reset (forwards), and that before it (backwards), see nothing of it."""
+    C = 64 if dtype == torch.bfloat16 else 32
+    # segments are two chunks: 4 and 5 are one
+    starts = (3 * C + 5, 5 * C + 20, 8 * C + 5) if forwards else (4 * C + 20, 6 * C + 30, 8 * C + 5)
+    p = packed(1, dtype, starts, 33 * C - 7, V)
+    dirty = dict(p, g=p["g"].copy())
+    at = 4 * C + 30 if forwards else 5 * C + 20
+    dirty["g"][0, at, 0] = bad
+    if bad == 200.0:
+        dirty["g"][0, at - 1, 0] = bad  # states of the document, too, pass what float32 holds
+    got = run(dk, dirty, dtype)
+    first = max(s for s in starts if s <= at)
+    last = min(s for s in starts if s > at)
+    same_elsewhere(got, p, dtype, np.s_[first:last])
