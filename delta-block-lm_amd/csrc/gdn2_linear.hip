@@ -13,13 +13,15 @@
 // The forward and dq are a walk over the chunks in order (linear_walk), from a triple (a, b, c):
 //   out_t = sum_s Gam (a_t.b_s) c_s + row_t (a_t S),   S' = tot S + sum_s col_s b_s c_s^T;
 // dv and dk share a walk in the other direction (linear_back), with the pairs' decays and the adjoint
-// state of both; for widths up to 64 it has dq and the gate's gradient as well.  The gate's gradient is a sum over the pairs that span a token,
+// state of both; for widths up to 64 it has dq and the gate's gradient as well.  The gate's gradient is a sum over
+// the pairs that span a token,
 //   dg_t = sum_{u>=t,s<t} W_us,  W_us = Gam_us (q_u.k_s)(do_u.v_s),
 // cut at the chunk's bounds, with x_u = gam_u q_u^T S0 do_u, y_s = lam_s k_s^T R v_s and E = gam <S0, R>:
 //   dg_t = sum_{u>=t,s<t inside the chunk} W_us + sum_{u>=t} x_u + sum_{s<t} y_s + E.
-// Where dq has a walk of its own, linear_back gives y and the products <S0, R> at segment starts, and the
-// dq walk has the rest and steps E from chunk to chunk (less x, plus y; 0 at a cut); in one walk E steps the
-// other way.  Nothing is subtracted over more than one segment, so it keeps float32 accuracy for long memories.
+// Every chunk has E from its two states (as a sum stepped from chunk to chunk, less x and plus y, it would be what is
+// left of much larger numbers after a strong decay).  Where dq has a walk of its own, linear_back leaves it y and
+// the adjoint state R of every chunk; in one walk the forward's kept states are S0.  No part is subtracted from
+// another, so what spans a token has float32 accuracy, whatever lies around it.
 //
 // A sequence is cut into segments for parallel work; their start states come from a walk over (b, c) alone,
 // a launch of its own for all segments (carry) and a join over them, or, in short sequences, by each
@@ -174,7 +176,8 @@ struct Forward : Walk {
     View a, b, c, d;        // d: see DOT
     int ka, vc;             // widths of a and b, and of c, d and out
     void *out;              // dense [B, T, H, vc], or null
-    const float *y, *edges; // [B H, T], [B H, segments], from linear_back
+    const float *y;         // [B H, T], from linear_back
+    const float *adj;       // and the adjoint state behind every chunk, [B H, chunks] kept forms
     float *dg;              // dense [B, T, H]
     float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
     float *seg_decay;       // [B H, segments]
@@ -186,10 +189,7 @@ struct Back : Walk {
     int K, V;
     void *dq, *dk, *dv;     // dense, or null (dq: all in one)
     float *dg;              // dense [B, T, H], or null (all in one)
-    View edge_first;        // with DOT: the forward's states, its first one
-    const float *edge;      // and those before the other segments
-    float *y;               // [B H, T]: see DOT
-    float *edges;           // [B H, segments]: <forward state, adjoint> at each segment's start
+    float *y, *adj;         // MODE 1: as in Forward
 };
 
 // DPP moves of 64 bits; lanes without a source read 0.
@@ -412,7 +412,7 @@ struct WalkLds {
     // a unit at 64 x 64 (2048 heads of 8 tokens, bf16: 31.7 us by twos).
     static constexpr int GATES = OUT && !DOT && CP == 64 ? 4 : 8;
     GateTile<C> gate[GATES];
-    float red[DOT ? CP / 16 : 1][C];
+    float red[DOT ? CP / 16 : 1][C], edge[CP / 16];
     float rows[DOT ? C / 16 : 1][C], cols[DOT ? C / 16 : 1][C];  // parts of the pair sums, by tiles of 16 tokens
 };
 
@@ -427,7 +427,7 @@ struct BackLds {
     T D[VP * LDK];
     static constexpr int GATES = 8;  // as in WalkLds
     GateTile<C> gate[GATES];
-    float red[NW][C], red_q[ALL ? NW : 1][C];
+    float red[NW][C], red_q[ALL ? NW : 1][C], edge[VP / 16];
     float rows[ALL ? C / 16 : 1][C], cols[ALL ? C / 16 : 1][C];  // parts of the pair sums, as in WalkLds
     int bad[2];                  // whether any wave's state is not finite, in turn for even and odd chunks
 };
@@ -505,6 +505,15 @@ struct State {
             if (M::place(m, 0) < rows)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) t[m][i] = src[(uint32_t)((M::place(m, 0) + i) * cols)];
+    }
+    // The wave's part of the sum of products with another state of the same form, without the columns past the width.
+    __device__ __forceinline__ float dot(const State &x, bool column) const {
+        float d = 0.f;
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d = fmaf(t[m][i], x.t[m][i], d);
+        return wave_sum(column ? d : 0.f);
     }
     // Dense rows of vc columns.
     __device__ __forceinline__ void store(float *dst, int v, int ka, int vc) const {
@@ -635,6 +644,15 @@ __device__ __forceinline__ float sum_dots(const float (&red)[ALL][C]) {
         for (int w = 1; w < NW; ++w) d += red[w][lane];
     }
     return d;
+}
+
+// E from the waves' parts of <S0, R>; 0 at a cut, whatever the states hold.
+template <int NW>
+__device__ __forceinline__ float between(const float (&edge)[NW], float tot) {
+    float e = edge[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) e += edge[w];
+    return tot == 0.f ? 0.f : tot * e;
 }
 
 // The pair sums of a chunk from the parts by tiles, rows[si][t] (over the s of tile si, t of a later tile) and
@@ -880,7 +898,11 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     if (p.starts_out && at.nth > 0)
         S.store(p.starts_out + at.bh * p.s_bh + at.seg * (int64_t)p.ka * p.vc, v, p.ka, p.vc);
 
-    float edge = DOT ? p.edges[at.bh * p.segments + at.seg] : 0.f;  // <S0, R> at the chunk's start
+    // DOT: the adjoint state behind the chunk, in the form of S.
+    const int64_t size = kept_size(p.ka, p.vc);
+    const float *adj = DOT ? p.adj + (int64_t)at.bh * p.chunks * size : nullptr;
+    State<T, KT> R;
+    if constexpr (DOT) R.load_transposed(adj + ci * size, v, up32(p.ka), up32(p.vc));
     for (; n > 0; --n, ++ci) {
         const GateTile<C> &gate = lds.gate[gi];
         const bool masks = odd || p.T - (int64_t)ci * C < C;
@@ -888,11 +910,15 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         sb.template store<LDA>(lds.b, gate.seg, masks, p.ka);
         sc.template store<LDC>(lds.c, gate.seg, masks, p.vc);
         if (DOT) sd.template store<LDC>(lds.d, gate.seg, masks, p.vc);
-        if (p.kept) S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + ci) * kept_size(p.ka, p.vc), v, up32(p.ka), up32(p.vc));
+        if (p.kept) S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + ci) * size, v, up32(p.ka), up32(p.vc));
         if (n > 1) fetch(ci + 1, true);
         const int64_t token = (int64_t)ci * C + lane;
         float y_now = 0.f;  // of this chunk, for the wave that adds up dg
         if (DOT && wave == 1) y_now = p.y[at.bh * p.T + min(token, p.T - 1)];
+        if constexpr (DOT) {
+            const float e = S.dot(R, v < p.vc);
+            if (lane == 0) lds.edge[wave] = e;
+        }
         __syncthreads();
 
         // P_ts = Gam_ts a_t.b_s for the tiles whose block of RB sources is seen from the rows: twelve in
@@ -978,9 +1004,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         if constexpr (DOT) if (wave == 1) {
             const bool in = lane < C && token < p.T;
             const float x = sum_dots<C, NW>(lds.red), y = in ? y_now : 0.f;
-            const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(x);
-            const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + E;
-            edge = E + wave_sum(y);
+            const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<NW>(lds.edge, gate.tot);
             const bool on = in && gate.seg[lane] >= 0 && gate.step[lane] != 0.f;
             if (in) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
         }
@@ -1022,21 +1046,22 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
                                                  o ? o + row0 * p.vc : nullptr, (int64_t)p.H * p.vc, left);
             fine = S.finite();
         }
+        if (DOT && n > 1) R.load_transposed(adj + (ci + 1) * size, v, up32(p.ka), up32(p.vc));
         __syncthreads();  // the chunk's tiles are read
         if (++gi == L::GATES && n > 1) next_gates();
     }
     if (at.nth != p.segments - 1) return;
     if (p.fin) S.store(p.fin + (int64_t)at.bh * p.ka * p.vc, v, p.ka, p.vc);
     if (p.kept)
-        S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * kept_size(p.ka, p.vc), v, up32(p.ka), up32(p.vc));
+        S.keep_at(p.kept + ((int64_t)at.bh * (p.chunks + 1) + p.chunks) * size, v, up32(p.ka), up32(p.vc));
 }
 
-// dv and dk, from the last chunk to the first, and more by MODE.  A wave owns 16 value columns of the adjoint state [K, V]
-// and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once
-// a chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for
-// dk read three of the four tensors again, and took its pairs' decays and the state's update a second
-// time.)  MODE 1: also y_s = row_s k_s^T S v_s and the products with the forward's states at segment starts,
-// for the dq walk.  MODE 2: dq and dg as well, from the forward's states before every chunk (all_in_one).
+// dv and dk, from the last chunk to the first, and more by MODE.  A wave owns 16 value columns of the adjoint state
+// [K, V] and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once a
+// chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for dk read
+// three of the four tensors again, and took its pairs' decays and the state's update a second time.)  MODE 1: also
+// y_s = row_s k_s^T S v_s and the adjoint state behind every chunk, for the dq walk.  MODE 2: dq and dg as well,
+// from the forward's states before every chunk (all_in_one).
 //
 // Bound like linear_walk: bf16, 16 x 512 tokens, 8 heads of 64, all in one 39.6 us (78 MB, 2.0 TB/s); 4 x 8192
 // tokens, 16 heads of 128, without dq 320 us (2.5 TB/s), one workgroup of eight waves a unit for its 144 KB of
@@ -1129,23 +1154,8 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
     const int64_t size = kept_size(p.K, p.V);
     const float *kept = ALL ? p.kept + (int64_t)at.bh * (p.chunks + 1) * size : nullptr;
     State<T, VP / 16> F;
-    float edge = 0.f;  // gates_too: <forward state, adjoint> at the chunk's end
-    if (ALL) {
-        if (gates_too) {
-            State<T, KT> e;
-            e.load_kept(kept + c_hi * size, v, up32(p.K), up32(p.V));
-            float d = 0.f;
-#pragma unroll
-            for (int m = 0; m < KT; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
-            d = wave_sum(v < p.V ? d : 0.f);
-            if (lane == 0) lds.red[wave][0] = d;
-            __syncthreads();
-            for (int w = 0; w < VP / 16; ++w) edge += lds.red[w][0];
-            __syncthreads();
-        }
-    }
+    State<T, KT> S0;  // gates_too: the same as it is
+    if (gates_too) S0.load_kept(kept + ci * size, v, up32(p.K), up32(p.V));
 
     for (; n > 0; --n, --ci) {
         const GateTile<C> &gate = lds.gate[gi];
@@ -1164,8 +1174,14 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             }
         };
         if (own_v) put_D(0);
+        if (MODE == 1 && own_v)
+            S.keep_at(p.adj + ((int64_t)at.bh * p.chunks + ci) * size, v, up32(p.K), up32(p.V));
         if (ALL) F.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
         if (n > 1) fetch(ci - 1, true);
+        if (gates_too) {
+            const float e = S.dot(S0, v < p.V);
+            if (lane == 0) lds.edge[wave] = e;
+        }
         __syncthreads();
 
         // For out token s and source t >= s: pk = Gam k_s.q_t, pv = Gam v_s.do_t, by tiles as in linear_walk
@@ -1307,9 +1323,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             if (gates_too && wave == 1) {
                 const int64_t token = (int64_t)ci * C + lane;
                 const float x = sum_dots<C, KP / 16>(lds.red_q), y = sum_dots<C, VP / 16>(lds.red);
-                const float E = gate.tot == 0.f ? 0.f : edge - wave_sum(y);
-                const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + E;
-                edge = E + wave_sum(x);
+                const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<VP / 16>(lds.edge, gate.tot);
                 const bool on = gate.seg[lane & (C - 1)] >= 0 && gate.step[lane & (C - 1)] != 0.f;
                 if (lane < C && token < p.T) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
             }
@@ -1374,6 +1388,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                                 M::mma(aq[j], kf[r], M::template across_place<LDP>(pv_of[q], r * RB, j));
                     }
             }
+            if (gates_too && n > 1) S0.load_kept(kept + (ci - 1) * size, v, up32(p.K), up32(p.V));
             if (ALL && dq) store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, aq);
             else no_loads_left();
             if (dv && own_v) store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, p.V == VP, av);
@@ -1428,41 +1443,13 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                 }
             }
             fine = S.finite();
+            if (gates_too && n > 1) S0.load_kept(kept + (ci - 1) * size, v, up32(p.K), up32(p.V));
         }
         __syncthreads();  // the chunk's tiles are read
         if (++gi == L::GATES && n > 1) next_gates();
     }
 
     if (p.fin && own_v && at.seg == 0) S.store(p.fin + (int64_t)at.bh * p.K * p.V, v, p.K, p.V);
-    if (MODE == 1) {
-        float d = 0.f;
-        if (own_v) {
-            const float *src = reinterpret_cast<const float *>(p.edge_first.data);
-            int rs = (int)p.edge_first.s2, cs = (int)p.edge_first.s3;
-            int64_t off = at.b * p.edge_first.s0 + at.h * p.edge_first.s1;
-            if (at.seg > 0) {
-                src = p.edge, rs = p.V, cs = 1;
-                off = ((int64_t)at.bh * p.segments + at.seg) * p.K * p.V;
-            }
-            if (src) {
-                State<T, KT> e;
-                e.load(src + off, rs, cs, v, p.K, p.V);
-                e.settle(v, p.K, p.V);
-#pragma unroll
-                for (int m = 0; m < KT; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d += S.t[m][i] * e.t[m][i];
-                d = wave_sum(v < p.V ? d : 0.f);
-            }
-            if (lane == 0) lds.red[wave][0] = d;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            d = lds.red[0][0];
-            for (int w = 1; w < VP / 16; ++w) d += lds.red[w][0];
-            p.edges[(int64_t)at.bh * p.segments + at.seg] = d;
-        }
-    }
 }
 
 // Segments' additions -> start states, in place: state[s] = what the segments walked before s left.
@@ -1644,7 +1631,7 @@ Plan plan(const gdn2_shape *s, int dtype) {
 }
 
 struct Layout {
-    size_t state, decay, kept, y, edges, dg, bytes;
+    size_t state, decay, kept, y, adj, dg, bytes;
 };
 
 // Widths for which the backward is one walk, from a state that the forward keeps before every chunk.  Up to 64
@@ -1665,7 +1652,7 @@ Layout checkpoint_layout(const Plan &p, const gdn2_shape *s, bool train) {
     return l;
 }
 
-Layout workspace_layout(const Plan &p, int64_t T) {
+Layout workspace_layout(const Plan &p, const gdn2_shape *s) {
     Layout l{};
     size_t n = 0;
     const auto take = [&](int64_t floats) {
@@ -1675,9 +1662,10 @@ Layout workspace_layout(const Plan &p, int64_t T) {
     };
     l.state = take(p.segments > 1 && !p.prewalk ? p.BH * p.segments * p.KV : 0);
     l.decay = take(p.BH * p.segments);
-    l.y = take(p.BH * T);
-    l.edges = take(p.BH * p.segments);
-    l.dg = take(p.BH * T);
+    const bool all = all_in_one(s);
+    l.y = take(all ? 0 : p.BH * s->time);
+    l.adj = take(all ? 0 : p.BH * p.chunks * kept_size((int)s->keys, (int)s->values));
+    l.dg = take(p.BH * s->time);
     l.bytes = n;
     return l;
 }
@@ -1871,7 +1859,7 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
 
 size_t gdn2_linear_workspace_bytes(const gdn2_shape *shape, int32_t dtype) {
     if (check_linear(shape, dtype) != GDN2_OK) return 0;
-    return workspace_layout(plan(shape, dtype), shape->time).bytes;
+    return workspace_layout(plan(shape, dtype), shape).bytes;
 }
 
 int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
@@ -1886,7 +1874,7 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     GDN2_TRY(check_view(d_output, "d_output", q->dtype, false));
     const Plan p = plan(shape, q->dtype);
     const bool all = all_in_one(shape);
-    const Layout lc = checkpoint_layout(p, shape, true), l = workspace_layout(p, shape->time);
+    const Layout lc = checkpoint_layout(p, shape, true), l = workspace_layout(p, shape);
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, lc.bytes, "checkpoint"));
     GDN2_TRY(check_buffer(workspace, workspace_bytes, l.bytes, "workspace"));
     if (initial && !initial->data) initial = nullptr;
@@ -1921,8 +1909,7 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
             w.dg = !gates ? nullptr : dg ? dg : at(l.dg);
             e = run_back<2>(w, p, dtype, vec, st);
         } else if (gates) {
-            w.y = at(l.y), w.edges = at(l.edges);
-            w.edge = states, w.edge_first = first;
+            w.y = at(l.y), w.adj = at(l.adj);
             e = run_back<1>(w, p, dtype, vec, st);
         } else {
             e = run_back<0>(w, p, dtype, vec, st);
@@ -1937,7 +1924,7 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
         w.starts = many ? states : nullptr, w.s_bh = p.segments * p.KV, w.s_row = 1, w.s_col = (int)V;
         if (gates) {
             w.d = make_view(q);
-            w.y = at(l.y), w.edges = at(l.edges);
+            w.y = at(l.y), w.adj = at(l.adj);
             w.dg = dg ? dg : at(l.dg);
             e = run_walk<false, true, true>(w, p, dtype, vec, st);
         } else {

@@ -551,7 +551,8 @@ GDN2_API int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const
  * NULL (zero).  dq, dk, dv dense in q's dtype; dg [B,T,H] and its sums over batch
  * and time dg_heads [H], d_initial [B,H,keys,values], F32 dense; any of them may
  * be NULL, and what only it needs is then not computed.  dg is 0 at padding, at
- * resets and where exp(g) is 0. */
+ * resets and where exp(g) is 0.  For widths above 64 the workspace holds a state
+ * for every chunk of 64 tokens, 32 in F32. */
 GDN2_API size_t gdn2_linear_workspace_bytes(const gdn2_shape *shape, int32_t dtype);
 GDN2_API int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,
                                   const gdn2_view *v, const gdn2_view *g, const gdn2_view *valid,
