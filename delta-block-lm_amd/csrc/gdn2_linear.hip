@@ -385,6 +385,9 @@ __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s
     return f;
 }
 
+// A product times its decay.  Where that is 0 the product is not seen, and may have overflowed.
+__device__ __forceinline__ float seen(float x, float f) { return f == 0.f ? 0.f : x * f; }
+
 // Inclusive sums over the lanes of each 16-lane group.
 __device__ __forceinline__ void row_scan(float &x) {
     x += dpp<0x111>(x);
@@ -945,7 +948,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
             const int t = 16 * tj + n16, s = 16 * si + g4;
             const f32x4 f = pair_decays<C, false>(gate, t, s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] *= f[i];
+            for (int i = 0; i < 4; ++i) x[i] = seen(x[i], f[i]);
             T hi[4];
             split2(x, hi, lo[m]);
             T *at_p = lds.p + t * LDP + M::place(si, g4);
@@ -997,7 +1000,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         for (int j = 0; j < TT; ++j) {
             f[j] = gate.row[16 * j + n16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] *= f[j];
+            for (int i = 0; i < 4; ++i) acc[j][i] = seen(acc[j][i], f[j]);
         }
         if constexpr (DOT) dot_rows<T, TT>(acc, f, lds.d + 16 * wave, LDC, lds.red[wave]);
         __syncthreads();
@@ -1213,9 +1216,9 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             const f32x4 f = pair_decays<C, true>(gate, s, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] *= f[i];
+                x[i] = seen(x[i], f[i]);
                 if (ALL) W[m][i] = f[i] == 0.f || t + i <= s ? 0.f : x[i] * y[i];
-                y[i] *= f[i];
+                y[i] = seen(y[i], f[i]);
             }
             T e[4], g[4];
             split2(x, e, pk_lo[m]);
@@ -1297,7 +1300,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
         for (int j = 0; j < TT; ++j) {
             f[j] = gate.row[16 * j + n16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) av[j][i] *= f[j], ak[j][i] *= f[j];
+            for (int i = 0; i < 4; ++i) av[j][i] = seen(av[j][i], f[j]), ak[j][i] = seen(ak[j][i], f[j]);
         }
         if (DOT && own_v && (!ALL || gates_too)) dot_rows<T, TT>(av, f, lds.v + 16 * wave, LDV, lds.red[wave]);
         if (ALL) {
@@ -1306,7 +1309,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             for (int j = 0; j < TT; ++j) {
                 c[j] = gate.col[16 * j + n16];  // of the walk in order
 #pragma unroll
-                for (int i = 0; i < 4; ++i) aq[j][i] *= c[j];
+                for (int i = 0; i < 4; ++i) aq[j][i] = seen(aq[j][i], c[j]);
             }
             if (gates_too) dot_rows<T, TT>(aq, c, lds.q + 16 * wave, LDK, lds.red_q[wave]);
         }
@@ -1358,7 +1361,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                         for (int j = 0; j < TT; ++j) {
                             const float row = gate.row[16 * j + n16];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) ak[j][i] = fmaf(row, x[j][i], ak[j][i]);
+                            for (int i = 0; i < 4; ++i) ak[j][i] += seen(x[j][i], row);
                         }
                     }
                 }

@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_linear import dk, oracle, problem, run, sizes, E, U  # noqa: E402,F401
+from test_gpu_linear import compare, dk, oracle, problem, run, sizes, E, U  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,38 @@ def test_a_gate_in_a_carried_segment(dk, forwards, bad, V, dtype):  # noqa: F811
     first = max(s for s in starts if s <= at)
     last = min(s for s in starts if s > at)
     same_elsewhere(got, p, dtype, np.s_[first:last])
+
+
+@DTYPES
+@pytest.mark.parametrize("V", [16, 80])
+def test_pairs_that_overflow_unseen(dk, V, dtype):  # noqa: F811
+    """Large values whose product no token sees, since the one comes later than the other or lies in another
+    document: it is infinite, and reaches nothing."""
+    p = packed(3, dtype, (0, 20, 50), 64, V)
+    big = 2.0 ** 70
+    for a, b in (("q", "k"), ("do", "v")):
+        x = {n: p[n].copy() for n in (a, b)}
+        x[a][0, 22], x[b][0, 40] = big * np.sign(p[a][0, 22]), big * np.sign(p[b][0, 40])  # later
+        x[a][0, 52], x[b][0, 10] = big * np.sign(p[a][0, 52]), big * np.sign(p[b][0, 10])  # another document
+        d = dict(p, **x)
+        compare(run(dk, d, dtype), d, dtype)
+
+
+@DTYPES
+@pytest.mark.parametrize("V", [16, 80])
+def test_products_with_states_that_overflow_unseen(dk, V, dtype):  # noqa: F811
+    """The state before a chunk, or its adjoint behind it, against large values behind, or before, a reset in it."""
+    p = packed(4, dtype, (100,), 200, V)
+    p["initial"] = p["df"] = None
+    p["g"][:] = -0.01
+    big = 2.0 ** 70
+    for a, b in (("k", "q"), ("v", "do")):  # 10 is in the state before 64, 120 sees none of it
+        x = {n: p[n].copy() for n in (a, b)}
+        x[a][0, 10], x[b][0, 120] = big * np.sign(p[a][0, 10]), big * np.sign(p[b][0, 120])
+        d = dict(p, **x)
+        compare(run(dk, d, dtype), d, dtype)
+    for a, b in (("q", "k"), ("do", "v")):  # 150 is in the adjoint behind 128, 70 sees none of it
+        x = {n: p[n].copy() for n in (a, b)}
+        x[a][0, 150], x[b][0, 70] = big * np.sign(p[a][0, 150]), big * np.sign(p[b][0, 70])
+        d = dict(p, **x)
+        compare(run(dk, d, dtype), d, dtype)
