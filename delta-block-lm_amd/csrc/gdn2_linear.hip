@@ -180,7 +180,7 @@ struct Forward : Walk {
     const float *adj;       // and the adjoint state behind every chunk, [B H, chunks] kept forms
     float *dg;              // dense [B, T, H]
     float *seg_state;       // carry: state that a segment adds, [B H, segments, ka, vc]
-    float *seg_decay;       // [B H, segments]
+    float *seg_decay;       // its root, [B H, segments]
 };
 
 // The walk of dv and dk in the other direction, over the adjoint state [K, V].
@@ -213,10 +213,23 @@ template <int C>
 struct alignas(16) GateTile {
     float hi[C], lo[C];     // sum of g log2(e) in the token's segment: hi + lo, both float32
     float row[C], col[C];   // factor of the start state and of the token's update (0: none of it)
-    float step[C];          // exp(g), 0 at a cut, 1 at padding
+    float step[C];          // the root of exp(g), 0 at a cut, 1 at padding
     int seg[C];             // cuts up to the token; -1 at padding
-    float tot;              // decay of the chunk
+    float tot;              // decay of the chunk, or NaN if it may grow past float32
+    float span;             // decay of the chunk, up to 2^127
+    double sum;             // its log2, for a chunk without a cut
 };
+
+// Decays can be growth past what float32 holds, which takes a value that is there to infinity, and leaves zero zero.
+// A chunk where that may be is taken token by token: its decay is NaN, which shows in the state after it.  There, and
+// over chunks that are carried, a decay is its root, applied twice (2^127 twice makes any normal number infinite).
+// Only the gate's gradient, which is never made token by token, has growth past 2^127 in a chunk counted as 2^127.
+__device__ __forceinline__ float root_exp2(float x) {
+    x *= 0.5f;
+    return __builtin_amdgcn_exp2f(x > 127.f ? 127.f : x);  // NaN stays
+}
+// A value times a decay given by its root: what was there may be infinite or NaN where a cut leaves nothing of it.
+__device__ __forceinline__ float decayed(float x, float root) { return root == 0.f ? 0.f : x * root * root; }
 
 struct GateIn {
     float g, valid, reset;
@@ -235,6 +248,7 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
     const int l = lane_id();
     const bool val = l < left && l < C && x.valid != 0.f;
     float g = val ? x.g : 0.f;
+    if (g == INFINITY) g = NAN;  // it makes NaN of a state of zero
     const bool cut = val && (x.reset != 0.f || g < kCut);
     if (cut) g = 0.f;
     const int seg = wave_scan_add((int)cut);
@@ -249,16 +263,22 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
     seg_step<0x143, 0xC>(G, seg + 1);
     const double last = __shfl(G, 63);
     const int end = __builtin_amdgcn_readlane(seg, 63);
+    const float growth = wave_sum(g < 0.f ? 0.f : g);  // NaN if any gate is
     if (l < C) {
-        const float gam = seg == 0 && val ? __builtin_amdgcn_exp2f((float)G) : 0.f;
-        const float lam = seg == end && val ? __builtin_amdgcn_exp2f((float)(last - G)) : 0.f;
+        const auto factor = [](float x) { return __builtin_amdgcn_exp2f(x > 127.f ? 127.f : x); };
+        const float gam = seg == 0 && val ? factor((float)G) : 0.f;
+        const float lam = seg == end && val ? factor((float)(last - G)) : 0.f;
         o->hi[l] = (float)G;
         o->lo[l] = (float)(G - (double)(float)G);
         o->row[l] = REV ? lam : gam;
         o->col[l] = REV ? gam : lam;
-        o->step[l] = cut ? 0.f : val ? __builtin_amdgcn_exp2f(g * 1.44269504f) : 1.f;
+        o->step[l] = cut ? 0.f : val ? root_exp2(g * 1.44269504f) : 1.f;
         o->seg[l] = val ? seg : -1;
-        if (l == 0) o->tot = end == 0 ? __builtin_amdgcn_exp2f((float)last) : 0.f;
+        if (l == 0) {
+            const float span = end == 0 ? factor((float)last) : 0.f;
+            o->span = span, o->tot = growth <= 88.f ? span : NAN;  // e^88 is 2^127
+            o->sum = last;
+        }
     }
 }
 
@@ -380,7 +400,7 @@ __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const bool on = seg[i] == st && (REV ? s + i >= t : s + i <= t);
-        f[i] = __builtin_amdgcn_exp2f(on ? f[i] : -1000.f);
+        f[i] = __builtin_amdgcn_exp2f(on ? fminf(f[i], 127.f) : -1000.f);
     }
     return f;
 }
@@ -721,10 +741,10 @@ __device__ __forceinline__ void walk_tokens(State<T, KP / 16> &S, const T *a, co
                 for (int i = 0; i < 4; ++i) {
                     const int k = Mat<T>::place(m, g4) + i;
                     if (k >= ka) continue;  // 0 there, whatever x is
-                    if (!REV) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
+                    if (!REV) S.t[m][i] = decayed(S.t[m][i], f);
                     S.t[m][i] += Elem<T>::load(b, t * LDA + k) * x;
                     if (OUT) o += Elem<T>::load(a, t * LDA + k) * S.t[m][i];
-                    if (REV) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
+                    if (REV) S.t[m][i] = decayed(S.t[m][i], f);
                 }
             o = groups_sum(o);
         }
@@ -828,7 +848,8 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     const int out = OUT ? n : 0;
     const bool walked = OUT && !(at.nth > 0 && p.starts);  // from the sequence's start
     if (walked) n = c_hi;
-    float decay = 1.f;
+    double sum = 0.;  // carry: log2 of the segment's decay
+    bool cut = false;
     int ci = REV ? c_lo + n - 1 : c_hi - n;
 
     Staged<T, KP, 64 * NW, VEC> sa, sb;
@@ -882,7 +903,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         State<T, KT> U;
         const bool next = update<T, KP>(U, S, gate.tot, cf, lds.b, gate.col);
         // A cut leaves nothing of the start, whatever the gates before and after it are.
-        decay = decay == 0.f || gate.tot == 0.f ? 0.f : decay * gate.tot;
+        sum += gate.sum, cut = cut || gate.span == 0.f;
         if (__builtin_expect(fine && next, 1)) {
             S = U;
         } else {
@@ -895,7 +916,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
     }
     if (!OUT) {
         S.store(p.seg_state + ((int64_t)at.bh * p.segments + at.seg) * p.ka * p.vc, v, p.ka, p.vc);
-        if (threadIdx.x == 0) p.seg_decay[(int64_t)at.bh * p.segments + at.seg] = decay;
+        if (threadIdx.x == 0) p.seg_decay[(int64_t)at.bh * p.segments + at.seg] = cut ? 0.f : root_exp2((float)sum);
         return;
     }
     if (p.starts_out && at.nth > 0)
@@ -1007,7 +1028,7 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
         if constexpr (DOT) if (wave == 1) {
             const bool in = lane < C && token < p.T;
             const float x = sum_dots<C, NW>(lds.red), y = in ? y_now : 0.f;
-            const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<NW>(lds.edge, gate.tot);
+            const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<NW>(lds.edge, gate.span);
             const bool on = in && gate.seg[lane] >= 0 && gate.step[lane] != 0.f;
             if (in) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
         }
@@ -1326,7 +1347,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
             if (gates_too && wave == 1) {
                 const int64_t token = (int64_t)ci * C + lane;
                 const float x = sum_dots<C, KP / 16>(lds.red_q), y = sum_dots<C, VP / 16>(lds.red);
-                const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<VP / 16>(lds.edge, gate.tot);
+                const float dg = gate_sums<C>(lds.rows, lds.cols, x, y) + between<VP / 16>(lds.edge, gate.span);
                 const bool on = gate.seg[lane & (C - 1)] >= 0 && gate.step[lane & (C - 1)] != 0.f;
                 if (lane < C && token < p.T) p.dg[(at.b * p.T + token) * p.H + at.h] = on ? dg : 0.f;
             }
@@ -1431,7 +1452,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                             }
                             const float d = row16_sum(v < p.V ? S.t[m][i] * y : 0.f);
                             if (n16 == 0) part[wave * KP + k] = d;
-                            if (k < p.K) S.t[m][i] = f == 0.f ? 0.f : S.t[m][i] * f;
+                            if (k < p.K) S.t[m][i] = decayed(S.t[m][i], f);
                         }
                     o = groups_sum(o);
                 }
@@ -1460,7 +1481,7 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
 // and 8 segments 12 us (67 MB, 5.6 TB/s).
 struct JoinArgs {
     float *state;        // [BH, segments, K V]
-    const float *decay;  // [BH, segments]
+    const float *decay;  // their roots, [BH, segments]
     const float *first;  // start state of the walk, or null
     int64_t f_b, f_h, f_row, f_col;
     int64_t H, KV, V;
@@ -1492,7 +1513,7 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
         for (int k = 0; k < N; ++k) {
             if (k >= n) break;
             st[(s + step * k) * p.KV] = x;
-            x = (f[k] == 0.f ? 0.f : f[k] * x) + add[k];
+            x = decayed(x, f[k]) + add[k];
         }
     }
 }
@@ -1538,7 +1559,8 @@ __global__ void __launch_bounds__(kThreads) linear_step(StepArgs p) {
         if ((int)threadIdx.x < p.V) Elem<T>::store(p.out, (int64_t)blockIdx.x * p.V + threadIdx.x, 0.f);
         return;
     }
-    float a = expf(ld4<float>(p.g, b, 0, h, 0));
+    const float g = ld4<float>(p.g, b, 0, h, 0);
+    float a = g == INFINITY ? NAN : g < kCut ? 0.f : expf(0.5f * (g > 176.f ? 176.f : g));  // a root, as in the chunks
     if (p.reset.data && ld4<float>(p.reset, b, 0, 0, 0) != 0.f) a = 0.f;
     if ((int)threadIdx.x < p.K) {
         qs[threadIdx.x] = ld4<T>(p.q, b, 0, h, threadIdx.x);
@@ -1575,7 +1597,7 @@ __global__ void __launch_bounds__(kThreads) linear_step(StepArgs p) {
             float x[4] = {s[u].x, s[u].y, s[u].z, s[u].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = (a == 0.f ? 0.f : a * x[i]) + kk * vv[i];
+                x[i] = decayed(x[i], a) + kk * vv[i];
                 o[i] += qq * x[i];
             }
             float *dst = S + k * p.V + v0;

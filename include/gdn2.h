@@ -532,7 +532,8 @@ GDN2_API int gdn2_hola_backward(const gdn2_hola_shape *shape, const gdn2_view *q
  * head; -inf empties the state like a reset); valid, reset F32 [B,T], views or
  * NULL (all valid, no reset); initial F32 [B,H,keys,values], a view or NULL.
  * Any element strides; rows of 16-byte aligned unit-stride channels are read
- * fastest.  batch * heads * ceil(time / 32) is at most 2^21.  A value that is not
+ * fastest.  Gates above 0 may multiply to more than F32 holds: zero stays zero.
+ * batch * heads * ceil(time / 32) is at most 2^21.  A value that is not
  * finite reaches the outputs of the tokens that see it and no others, and no
  * gradient outside its document.
  *
@@ -551,7 +552,8 @@ GDN2_API int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const
  * NULL (zero).  dq, dk, dv dense in q's dtype; dg [B,T,H] and its sums over batch
  * and time dg_heads [H], d_initial [B,H,keys,values], F32 dense; any of them may
  * be NULL, and what only it needs is then not computed.  dg is 0 at padding, at
- * resets and where exp(g) is 0.  For widths above 64 the workspace holds a state
+ * resets and where exp(g) is 0; growth past 2^127 within a chunk (64 tokens, 32 in
+ * F32) counts as 2^127 in it.  For widths above 64 the workspace holds a state
  * for every chunk of 64 tokens, 32 in F32. */
 GDN2_API size_t gdn2_linear_workspace_bytes(const gdn2_shape *shape, int32_t dtype);
 GDN2_API int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2_view *k,

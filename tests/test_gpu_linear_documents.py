@@ -1,4 +1,5 @@
-"""What is not finite in linear attention stays in its document, across the segments of a long sequence too.
+"""What is not finite in linear attention stays in its document, across the segments of a long sequence too,
+and decays that overflow do no harm to a state that is zero.
 
 Bounds as in test_gpu_linear, with u = 2^-8, e = 2^-24 and A the same result of magnitudes: 2.1 u A for bf16
 results, 128 e A for float32 ones, and for dg 256 e max A over the sequence."""
@@ -56,6 +57,24 @@ def test_a_gate_in_a_carried_segment(dk, forwards, bad, V, dtype):  # noqa: F811
     first = max(s for s in starts if s <= at)
     last = min(s for s in starts if s > at)
     same_elsewhere(got, p, dtype, np.s_[first:last])
+
+
+@DTYPES
+@pytest.mark.parametrize("V", [16, 80])
+@pytest.mark.parametrize("T", [200, 1500])
+@pytest.mark.parametrize("cut", [False, True])
+def test_growth_of_nothing(dk, cut, T, V, dtype):  # noqa: F811
+    """Gates that multiply to more than float32 holds, over tokens where neither a state nor its adjoint is
+    there yet: each factor is finite, and zero stays zero."""
+    lo_, hi = T // 2 - 60, T // 2 + 60
+    p = problem(2, 1, T, 1, 16, V, dtype)
+    p["g"][0, lo_:hi, 0] = 2.0
+    p["k"][0, :hi] = 0
+    p["do"][0, lo_:] = 0
+    if cut:
+        p["reset"] = np.zeros((1, T))
+        p["reset"][0, hi + 3] = 1
+    compare(run(dk, p, dtype), p, dtype)
 
 
 @DTYPES
