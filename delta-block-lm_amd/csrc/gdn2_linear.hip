@@ -222,11 +222,11 @@ struct alignas(16) GateTile {
 
 // Decays can be growth past what float32 holds, which takes a value that is there to infinity, and leaves zero zero.
 // A chunk where that may be is taken token by token: its decay is NaN, which shows in the state after it.  There, and
-// over chunks that are carried, a decay is its root, applied twice (2^127 twice makes any normal number infinite).
+// over chunks that are carried, a decay is its root, applied twice (the largest makes any normal number infinite).
 // Only the gate's gradient, which is never made token by token, has growth past 2^127 in a chunk counted as 2^127.
 __device__ __forceinline__ float root_exp2(float x) {
     x *= 0.5f;
-    return __builtin_amdgcn_exp2f(x > 127.f ? 127.f : x);  // NaN stays
+    return __builtin_amdgcn_exp2f(x > 127.99f ? 127.99f : x);  // NaN stays
 }
 // A value times a decay given by its root: what was there may be infinite or NaN where a cut leaves nothing of it.
 __device__ __forceinline__ float decayed(float x, float root) { return root == 0.f ? 0.f : x * root * root; }
@@ -1560,7 +1560,7 @@ __global__ void __launch_bounds__(kThreads) linear_step(StepArgs p) {
         return;
     }
     const float g = ld4<float>(p.g, b, 0, h, 0);
-    float a = g == INFINITY ? NAN : g < kCut ? 0.f : expf(0.5f * (g > 176.f ? 176.f : g));  // a root, as in the chunks
+    float a = g == INFINITY ? NAN : g < kCut ? 0.f : expf(0.5f * (g > 177.4f ? 177.4f : g));  // a root, as in the chunks
     if (p.reset.data && ld4<float>(p.reset, b, 0, 0, 0) != 0.f) a = 0.f;
     if ((int)threadIdx.x < p.K) {
         qs[threadIdx.x] = ld4<T>(p.q, b, 0, h, threadIdx.x);

@@ -8,6 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from gpu_util import host  # noqa: E402
 from test_gpu_linear import compare, dk, oracle, problem, run, sizes, E, U  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +111,22 @@ def test_products_with_states_that_overflow_unseen(dk, V, dtype):  # noqa: F811
         x[a][0, 150], x[b][0, 70] = big * np.sign(p[a][0, 150]), big * np.sign(p[b][0, 70])
         d = dict(p, **x)
         compare(run(dk, d, dtype), d, dtype)
+
+
+@pytest.mark.parametrize("g,want", [(100.0, "zero"), (300.0, "zero"), (np.inf, "nan"), (np.nan, "nan")])
+def test_a_step_that_grows(dk, g, want):  # noqa: F811
+    """The step takes gates as the sequence does: a state of zero stays so under a finite gate, one that is there
+    grows as far as float32 goes."""
+    q = torch.ones((1, 1, 1, 4), device="cuda")
+    k = torch.zeros_like(q)
+    gate = torch.full((1, 1, 1), g, device="cuda")
+    state = torch.zeros((1, 1, 4, 4), device="cuda")
+    state[0, 0, 0, 0] = 1e-38
+    out = host(dk.linear_attention_step(state, q, k, q, gate))
+    seq, fin = dk.linear_attention(q, k, q, gate, None, None, torch.zeros_like(state))
+    if want == "nan":
+        assert np.isnan(out).all() and torch.isnan(seq).all() and torch.isnan(fin).all()
+        return
+    assert np.all(out[..., 1:] == 0) and torch.all(seq == 0) and torch.all(fin == 0)
+    grown = 1e-38 * np.exp(min(g, 700.0))
+    assert out[0, 0, 0, 0] == np.inf if grown > 3.4e38 else abs(out[0, 0, 0, 0] - grown) <= 1e-4 * grown
