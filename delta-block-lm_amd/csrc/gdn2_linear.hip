@@ -1518,19 +1518,20 @@ __global__ void __launch_bounds__(kThreads) linear_join(JoinArgs p) {
     }
 }
 
-// out[h] = sum over b, t of x[b, t, h]: one workgroup a head, a fixed order.  For 8 x 509 tokens the launch
-// alone (3.9 us).
+// out[h] = sum over b, t of x[b, t, h]: one workgroup a head, a fixed order, in 64 bits, since a thread adds up to
+// 2^16 values one after the other.  For 8 x 509 tokens the launch alone (3.9 us).
 __global__ void __launch_bounds__(1024) linear_head_sum(const float *x, int64_t rows, int64_t H, float *out) {
-    __shared__ float red[16];
-    float s = 0.f;
+    __shared__ double red[16];
+    double s = 0.;
     for (int64_t r = threadIdx.x; r < rows; r += 1024) s += x[r * H + blockIdx.x];
-    s = wave_sum(s);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     if (lane_id() == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        float t = red[0];
+        double t = red[0];
         for (int i = 1; i < 16; ++i) t += red[i];
-        out[blockIdx.x] = t;
+        out[blockIdx.x] = (float)t;
     }
 }
 
