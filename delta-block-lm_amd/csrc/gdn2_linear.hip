@@ -1642,12 +1642,12 @@ Plan plan(const gdn2_shape *s, int dtype) {
     p.chunks = (int)((s->time + p.C - 1) / p.C);
     p.BH = s->batch * s->heads;
     p.KV = s->keys * s->values;
-    // Segments of at least two chunks (the last one of an odd number has one), as many as fill the card, and of at
-    // most 16 (the gate's gradient adds up what happens in a segment).  With single chunks a prompt of 3001
+    // Segments of at least two chunks (the last one of an odd number has one), as many as fill the card.  (Cut at 16
+    // chunks, too, 32 x 2048 bf16 tokens, 16 heads of 64, take 258 and 509 us forward and backward in place of 211 and
+    // 472, 8 x 8192 tokens, 16 heads of 128, 541 and 1703 in place of 508 and 1639.)  With single chunks a prompt of 3001
     // tokens, 8 heads of 64, takes 24.8 us in place of 22.3, more to join; with three for two where their number
     // is odd 23.9, and 700 tokens in both directions 59 in place of 48 (5000 forward 26.5 in place of 27.6).
-    int64_t want = std::max<int64_t>(kWantGroups / p.BH, (p.chunks + 15) / 16);
-    want = std::max<int64_t>(1, std::min<int64_t>(want, (p.chunks + 1) / 2));
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kWantGroups / p.BH, (p.chunks + 1) / 2));
     p.seg_chunks = (int)((p.chunks + want - 1) / want);
     p.segments = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
     // Walked to where that costs at most a few chunks: 512 tokens (8 chunks) 60 us in both directions, 74 carried;
