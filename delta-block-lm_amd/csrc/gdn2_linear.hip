@@ -263,7 +263,7 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
     seg_step<0x143, 0xC>(G, seg + 1);
     const double last = __shfl(G, 63);
     const int end = __builtin_amdgcn_readlane(seg, 63);
-    const float growth = wave_sum(g < 0.f ? 0.f : g);  // NaN if any gate is
+    const bool grows = __any(!(g <= 88.f / C));  // e^88 is 2^127; a gate that is NaN, too
     if (l < C) {
         const auto factor = [](float x) { return __builtin_amdgcn_exp2f(x > 127.f ? 127.f : x); };
         const float gam = seg == 0 && val ? factor((float)G) : 0.f;
@@ -276,7 +276,7 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
         o->seg[l] = val ? seg : -1;
         if (l == 0) {
             const float span = end == 0 ? factor((float)last) : 0.f;
-            o->span = span, o->tot = growth <= 88.f ? span : NAN;  // e^88 is 2^127
+            o->span = span, o->tot = grows ? NAN : span;
             o->sum = last;
         }
     }
