@@ -1721,6 +1721,9 @@ bool vec_rows(const gdn2_view *v, int64_t width) {
     return v->stride[1] * es * 64 < ((int64_t)1 << 31);
 }
 
+// And results written so: null, or dense at a 16-byte address (rows of whole pieces then all are).
+bool vec_out(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 int check_inputs(const gdn2_shape *s, const gdn2_view *q, const gdn2_view *k, const gdn2_view *v,
                  const gdn2_view *g, const gdn2_view *valid, const gdn2_view *reset) {
     GDN2_TRY(check_view(q, "q", -1, false));
@@ -1863,7 +1866,7 @@ int gdn2_linear_scan(const gdn2_shape *shape, const gdn2_view *q, const gdn2_vie
     GDN2_TRY(check_buffer(checkpoint, checkpoint_bytes, l.bytes, "checkpoint"));
     if (initial && !initial->data) initial = nullptr;
     const int64_t K = shape->keys, V = shape->values;
-    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V);
+    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V) && vec_out(output);
     hipStream_t st = (hipStream_t)stream;
     Forward w = base_walk<Forward>(shape, p, g, valid, reset);
     const View first = make_view(initial);
@@ -1907,7 +1910,8 @@ int gdn2_linear_backward(const gdn2_shape *shape, const gdn2_view *q, const gdn2
     const int64_t K = shape->keys, V = shape->values;
     const int dtype = q->dtype;
     const bool gates = dg || dg_heads;
-    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V) && vec_rows(d_output, V);
+    const bool vec = vec_rows(q, K) && vec_rows(k, K) && vec_rows(v, V) && vec_rows(d_output, V) && vec_out(dq) &&
+                     vec_out(dk) && vec_out(dv);
     hipStream_t st = (hipStream_t)stream;
     const Forward base = base_walk<Forward>(shape, p, g, valid, reset);
     const auto at = [&](size_t off) { return (float *)((char *)workspace + off); };
