@@ -6,7 +6,8 @@
   layer_norm(x, weight, bias)          layer norm over the last axis
   swiglu_q8(h)                         SwiGLU that keeps its input in 8 bits for the backward
 
-They have no counterpart in the reference.  The first form of each is differentiable;
+They have no counterpart in the reference.  The first form of each is differentiable, once and in
+reverse mode (anything else is refused);
 *_forward and *_backward are the raw calls, for a block that writes its backward out
 (delta_mixers.linear).  All run only on the GPU: there is no CPU fallback.
 """
@@ -15,6 +16,8 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _size, _shape
 from ._lib import GDN2_BF16, GDN2_F32, check, lib, on_device
@@ -81,6 +84,12 @@ def _same_device(like: torch.Tensor, names: str, *tensors) -> None:
 
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _differentiates(*tensors) -> bool:
+    """Whether a call goes through its autograd function: for gradients, and inside forward-mode
+    differentiation, which the function refuses for inputs with a tangent."""
+    return forward_ad._current_level >= 0 or _wants_grad(*tensors)
 
 
 # ---- linear attention ------------------------------------------------------------------
@@ -190,6 +199,7 @@ class _LinearAttention(torch.autograd.Function):
         return out, final
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out, d_final):
         q, k, v, g, valid, reset, initial, ck = ctx.saved_tensors
         if d_out is None and d_final is None:
@@ -214,7 +224,7 @@ def linear_attention(q, k, v, g, valid=None, reset=None, initial=None):
     for name, m in (("valid", valid), ("reset", reset)):
         if m is not None and m.requires_grad:
             raise ValueError(f"{name} is nondifferentiable metadata")
-    if not _wants_grad(q, k, v, g, initial):
+    if not _differentiates(q, k, v, g, initial):
         return linear_attention_forward(q, k, v, g, valid, reset, initial, False)[:2]
     return _LinearAttention.apply(q, k, v, g, valid, reset, initial)
 
@@ -320,6 +330,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, inv = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -331,7 +342,7 @@ def layer_norm(x, weight, bias=None, epsilon: float = 1e-5):
     """Layer norm over the last axis: weight (x - mean) / sqrt(var + epsilon) + bias, x [..., W]
     float32 or bfloat16, weight and bias [W] float32 (bias may be None).  The output has x's shape and
     dtype; statistics and sums are float32.  Differentiable in x, weight and bias."""
-    if not _wants_grad(x, weight, bias):
+    if not _differentiates(x, weight, bias):
         return _ln_forward(x, weight, bias, epsilon, False)[0]
     return _LayerNorm.apply(x, weight, bias, float(epsilon))
 
@@ -402,6 +413,7 @@ class _SwigluQ8(torch.autograd.Function):
         return a
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, da):
         codes, exps = ctx.saved_tensors
         return swiglu_q8_backward(codes, exps, da.contiguous(), False)[0]
@@ -414,5 +426,5 @@ def swiglu_q8(h: torch.Tensor) -> torch.Tensor:
     if h.dim() < 1 or h.shape[-1] % 2 or h.shape[-1] < 2:
         raise ValueError("h must be [..., 2 M]")
     rows = h.reshape(-1, h.shape[-1]).contiguous()
-    a = _SwigluQ8.apply(rows) if _wants_grad(h) else swiglu_q8_forward(rows)[0]
+    a = _SwigluQ8.apply(rows) if _differentiates(h) else swiglu_q8_forward(rows)[0]
     return a.view(h.shape[:-1] + (h.shape[-1] // 2,))

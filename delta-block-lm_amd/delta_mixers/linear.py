@@ -21,6 +21,7 @@ from typing import List, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 import delta_kernels as dk
 
@@ -103,6 +104,7 @@ class _Q8Mlp(torch.autograd.Function):
         return torch.mm(a, w2.t())
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dr):
         x, codes, exps, w13, w2 = ctx.saved_tensors
         dr = dr.contiguous()
