@@ -18,6 +18,7 @@ import struct
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _size, _shape
 from ._lib import GDN2_BF16, GDN2_F32, check, lib, on_device
@@ -84,6 +85,11 @@ def _same_device(like: torch.Tensor, names: str, *tensors) -> None:
 
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _has_tangent(*tensors) -> bool:
+    return forward_ad._current_level >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _differentiates(*tensors) -> bool:
@@ -232,12 +238,17 @@ def linear_attention(q, k, v, g, valid=None, reset=None, initial=None):
 def linear_attention_step(state, q, k, v, g, valid=None, reset=None):
     """One token per sequence on a carried state, updated in place: state [B, H, K, V] float32
     contiguous; q, k [B, 1, H, K], v [B, 1, H, V], g [B, 1, H] or [H], valid, reset [B, 1] or None.
-    Returns the output [B, 1, H, V] in q's dtype.  Without gradients."""
+    Returns the output [B, 1, H, V] in q's dtype.  It has no gradient: where one is recorded, inputs
+    that require one are refused, and autograd is told that the state has changed."""
     if state.dtype != F32 or not state.is_contiguous():
         raise ValueError("state must be a contiguous float32 [B, H, K, V] tensor")
+    if _wants_grad(state, q, k, v, g) or _has_tangent(state, q, k, v, g):
+        raise ValueError("linear_attention_step has no gradient: call it under torch.no_grad(), or on "
+                         "detached inputs")
     _, shape, views, held = _attention_inputs(q, k, v, g, valid, reset, state, "state")
     out = torch.empty(v.shape, dtype=q.dtype, device=q.device)
     _call("gdn2_linear_step", q.device, _SHAPE(*shape), *views, state.data_ptr(), out.data_ptr())
+    increment_version(state)
     return out
 
 

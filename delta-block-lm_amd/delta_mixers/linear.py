@@ -88,7 +88,7 @@ class LinearMixer(torch.nn.Module):
         return self._join(o, gate), state
 
     def step(self, x, state):
-        """One token a sequence, x [B, 1, d_model]; the state is updated in place."""
+        """One token a sequence, x [B, 1, d_model]; the state is updated in place.  Without gradients."""
         q, k, v, gate = self._split(x)
         return self._join(dk.linear_attention_step(state, q, k, v, -F.softplus(self.decay)), gate)
 

@@ -1,4 +1,5 @@
-"""Derivatives that the linear-attention block's operators do not have are refused, not dropped."""
+"""Derivatives that the linear-attention block's operators do not have are refused, not dropped, and a state that
+a step changes in place is known to have changed."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -57,3 +58,43 @@ def test_second_derivatives_of_the_mlp_are_refused(dk):  # noqa: F811
     loss = penalty(mlp(x), x)
     with pytest.raises(RuntimeError, match="twice"):
         loss.backward()
+
+
+def test_a_step_on_a_state_that_a_backward_needs(dk):  # noqa: F811
+    q, k, v, g = inputs(K=100)
+    state = torch.randn((2, 3, 100, 8), device="cuda")
+    q.requires_grad_(True)
+    out, _ = dk.linear_attention(q, k, v, g, None, None, state)
+    with torch.no_grad():
+        dk.linear_attention_step(state, q[:, :1], k[:, :1], v[:, :1], g[:, :1])
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("which", ["state", "q", "k", "v", "g"])
+def test_a_step_has_no_gradient(dk, which):  # noqa: F811
+    q, k, v, g = (x[:, :1].clone() for x in inputs())
+    x = dict(state=torch.zeros((2, 3, 16, 8), device="cuda"), q=q, k=k, v=v, g=g)
+    x[which].requires_grad_(True)
+    with pytest.raises(ValueError, match="no gradient"):
+        dk.linear_attention_step(**x)
+    with torch.no_grad():
+        dk.linear_attention_step(**x)
+
+
+def test_a_step_in_inference_mode(dk):  # noqa: F811
+    with torch.inference_mode():
+        q, k, v, g = (x[:, :1].clone() for x in inputs())
+        a, b = torch.zeros((2, 2, 3, 16, 8), device="cuda").unbind()
+        out = dk.linear_attention_step(a, q, k, v, g)
+        seq, fin = dk.linear_attention(q, k, v, g, None, None, b)
+    assert torch.allclose(out, seq, rtol=1e-5, atol=1e-6) and torch.allclose(a, fin, rtol=1e-5, atol=1e-6)
+
+
+def test_a_step_in_forward_mode(dk):  # noqa: F811
+    q, k, v, g = (x[:, :1].clone() for x in inputs())
+    state = torch.zeros((2, 3, 16, 8), device="cuda")
+    with fwAD.dual_level():
+        dk.linear_attention_step(state, q, k, v, g)  # without a tangent it runs
+        with pytest.raises(ValueError, match="no gradient"):
+            dk.linear_attention_step(state, fwAD.make_dual(q, torch.ones_like(q)), k, v, g)
