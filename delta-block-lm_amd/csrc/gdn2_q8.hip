@@ -7,8 +7,8 @@
 //
 // A block's scale is 2^e with the smallest e for which its largest magnitude is at most 127 2^e, and a
 // code is h 2^-e rounded to the nearest whole number, ties to even: both steps are exact in float32
-// apart from that rounding, and a kept value is exact in bf16 (7 bits).  The error is at most 2^(e-1),
-// so below 1/127 of the block's largest magnitude.  Between the passes a token of width M holds
+// apart from that rounding, and a kept value is exact in bf16 (7 bits).  The error is at most 2^(e-1), or 2^e at
+// the largest of all values, so below 1/127 of the block's largest magnitude.  Between the passes a token of width M holds
 // 2.06 M bytes, where h and a in bf16 hold 6 M.
 //
 // Bound by memory: eight columns of both halves a thread, 16 bytes of bf16 at a time; the four threads
@@ -102,18 +102,19 @@ __device__ __forceinline__ int block_exponent(const float (&v)[8]) {
     if (m >= 0x7F800000u) return kNan;
     // m = 1.f 2^x <= 127 2^e = 1.984375 2^(e + 6)
     const int x = (int)(m >> 23) - 127 - 6 + ((m & 0x7FFFFFu) > 0x7E0000u);
-    return max(x, -126) + 127;
+    return min(max(x, -126), 121) + 127;
 }
 __device__ __forceinline__ float power(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
 __device__ __forceinline__ void put_codes(int8_t *p, uint32_t c, uint32_t M, int vec,
                                           const float (&v)[8], int ex) {
-    // 2^-e = 2^(127 - biased); e <= 121, so it is a normal number
+    // 2^-e = 2^(127 - biased); e <= 121, so it is a normal number.  There values above 127 2^121 take code 127
+    // too: with e = 122 they would round to 2^128.
     const float s = ex == kNan ? 0.f : power(254 - ex);
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int q = ex == kNan ? 0 : (int)rintf(v[i] * s);
+        const int q = ex == kNan ? 0 : (int)fminf(fmaxf(rintf(v[i] * s), -127.f), 127.f);
         w[i / 4] |= (uint32_t)(q & 255) << (8 * (i % 4));
     }
     if (vec) {

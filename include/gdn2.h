@@ -596,9 +596,9 @@ GDN2_API int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_v
  * width] = silu(gate) up, rounded once, and what the backward reads instead of h:
  * codes [rows, 2 width] and, for each block of 32 columns of a half (the last may
  * be short), one exponent: exponents [rows, 2 ceil(width / 32)], e + 127.  2^e is
- * the smallest power of two with max |h| <= 127 2^e in the block (e >= -126), a
- * code is h 2^-e to the nearest whole number, ties to even, and the kept value is
- * code 2^e.  A block with a value that is not finite has exponent 255 and reads
+ * the smallest power of two with max |h| <= 127 2^e in the block (-126 <= e <= 121),
+ * a code is h 2^-e to the nearest whole number, ties to even, at most 127 in
+ * magnitude, and the kept value is code 2^e.  A block with a value that is not finite has exponent 255 and reads
  * back as NaN.  The backward takes the VJP at the kept values: dh [rows, 2 width],
  * and a at the kept values again (may be NULL).  Dense, F32 or BF16 (one dtype);
  * widths that are a multiple of 8 in 16-byte aligned buffers run fastest. */

@@ -89,10 +89,11 @@ def q8(h, block=32):
                     e[r] = 128
                     continue
                 e[r] = -126
-                while top > 127 * 2.0 ** e[r]:
+                while top > 127 * 2.0 ** e[r] and e[r] < 121:  # at 122 a value could round to 2^128
                     e[r] += 1
             ok = e < 128
-            codes[at] = np.where(ok[:, None], np.rint(np.where(ok[:, None], x, 0) * 2.0 ** -e[:, None]), 0)
+            code = np.rint(np.where(ok[:, None], x, 0) * 2.0 ** -e[:, None])
+            codes[at] = np.where(ok[:, None], np.clip(code, -127, 127), 0)
             exps.append((e + 127).astype(np.uint8))
     return codes, np.stack(exps, 1)
 
