@@ -39,13 +39,16 @@ struct Q8Args {
     int vec;
 };
 
-// 16 sigmoid(x), with v_exp_f32 and v_rcp_f32 (about 1 ulp each).  Sixteen times, because v_rcp_f32
-// gives 0 for a result below the normal numbers: x sigmoid(x) still is one where sigmoid(x) is not.
-__device__ __forceinline__ float sigm16(float x) {
-    const float d = 1.f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f);
-    return __builtin_amdgcn_rcpf(d * 0.0625f);
+// 128 sigmoid(x), with v_exp_f32 and v_rcp_f32 (about 1 ulp each).  128 times, because v_rcp_f32 gives 0 for a
+// result below the normal numbers, and x sigmoid(x) still is a normal number down to x = -91.8, where sigmoid(x) is
+// 2^-132.5.
+__device__ __forceinline__ float sigm128(float x) {
+    return __builtin_amdgcn_rcpf(0.0078125f + __builtin_amdgcn_exp2f(fmaf(x, -1.4426950408889634f, -7.f)));
 }
-__device__ __forceinline__ float silu(float x, float s16) { return (x * 0.0625f) * s16; }
+// The scale goes to the larger factor: a small x would lose bits to it.
+__device__ __forceinline__ float silu(float x, float s128) {
+    return x < -1.f ? (x * 0.0078125f) * s128 : x * (s128 * 0.0078125f);
+}
 
 // Columns [c, c + 8) of a row that starts at p, zero past M.
 template <typename T>
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) q8_forward_kernel(Q8Args p) {
     if (!in) return;
     float a[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = silu(g[i], sigm16(g[i])) * u[i];
+    for (int i = 0; i < 8; ++i) a[i] = silu(g[i], sigm128(g[i])) * u[i];
     store8<T>(reinterpret_cast<T *>(p.a) + (int64_t)r * p.M, c, p.M, vec, a);
     int8_t *q = p.codes + (int64_t)r * 2 * p.M;
     put_codes(q, c, p.M, vec, g, eg);
@@ -189,9 +192,9 @@ __global__ void __launch_bounds__(kThreads) q8_backward_kernel(Q8Args p) {
     load8<T>(reinterpret_cast<const T *>(p.da) + (int64_t)r * p.M, c, p.M, p.vec, d);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float s16 = sigm16(g[i]), x = silu(g[i], s16);
+        const float s128 = sigm128(g[i]), x = silu(g[i], s128);
         a[i] = x * u[i];
-        u[i] = d[i] * u[i] * (s16 * (0.0625f * fmaf(g[i], fmaf(s16, -0.0625f, 1.f), 1.f)));
+        u[i] = d[i] * u[i] * (s128 * (0.0078125f * fmaf(g[i], fmaf(s128, -0.0078125f, 1.f), 1.f)));
         g[i] = d[i] * x;
     }
     T *dh = reinterpret_cast<T *>(p.dh) + (int64_t)r * 2 * p.M;
