@@ -409,7 +409,7 @@ def q8_values(codes: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor:
     does not form them)."""
     rows, width = codes.shape
     M = width // 2
-    blocks = exponents.view(rows, 2, -1).to(torch.int32)
+    blocks = exponents.view(rows, 2, -(-M // Q8_BLOCK)).to(torch.int32)
     scale = (blocks << 23).view(F32)  # 2^e from its exponent bits
     scale = torch.where(blocks == 255, torch.full_like(scale, float("nan")), scale)
     scale = scale.repeat_interleave(Q8_BLOCK, 2)[:, :, :M]

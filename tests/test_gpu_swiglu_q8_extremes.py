@@ -56,3 +56,8 @@ def test_gates_whose_sigmoid_is_not_a_normal_number(dk, x):  # noqa: F811
     s = 1 / (1 + np.exp(-kept[:, :32]))
     terms = np.concatenate([s * (1 + np.abs(kept[:, :32])), s * np.abs(kept[:, :32])], 1)
     assert np.all(np.abs(host(dh) - want) <= 16 * E * size * terms + TINY)
+
+
+def test_values_of_no_rows(dk):  # noqa: F811
+    _, codes, exps = dk.swiglu_q8_forward(torch.empty((0, 64), device="cuda"))
+    assert dk.q8_values(codes, exps).shape == (0, 64)
