@@ -504,13 +504,12 @@ void launch_ln(const LnArgs &a, int dtype, bool vec, int64_t partials, hipStream
     else launch_width<float, BWD, false>(a, partials, st);
 }
 
-// Workgroups of the backward, each of which writes a row of column sums: by the sizes alone, as the order
-// of the sums goes by them.  512 (1024: 65536 bf16 rows of 1024 88 us in place of 81, 8192 of 8192 130 in place
-// of 100); 1024 for many rows of widths whose rows start off 16 bytes, which have no row ahead on its way
-// (65536 of 999 118 us, with 512 174); of wide rows fewer, whose sums would weigh as much as they (2000 of
-// 32768 165 us, with 128 178).
-int64_t partial_rows(int64_t rows, int64_t W) {
-    return std::max<int64_t>(1, std::min<int64_t>(rows, W > kSums ? 64 : rows >= 32768 && W % 8 ? 1024 : 512));
+// Workgroups of the backward, each of which writes a row of column sums, at most.  512 (1024: 65536 bf16 rows of 1024
+// 88 us in place of 81, 8192 of 8192 130 in place of 100); 1024 for many rows off 16 bytes, which have no row ahead
+// on its way (65536 of 999 118 us, with 512 174); of wide rows fewer, whose sums would weigh as much as they
+// (2000 of 32768 165 us, with 128 178).  The order of the sums goes by it.
+int64_t partial_rows(int64_t rows, int64_t W, bool vec) {
+    return std::max<int64_t>(1, std::min<int64_t>(rows, W > kSums ? 64 : rows >= 32768 && !vec ? 1024 : 512));
 }
 
 }  // namespace
@@ -547,7 +546,7 @@ int gdn2_layer_norm_forward(const gdn2_rows_shape *shape, float epsilon, const g
 
 size_t gdn2_layer_norm_workspace_bytes(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1) return 0;
-    return (size_t)(2 * 4 * partial_rows(rows, width) * width);
+    return (size_t)(2 * 4 * partial_rows(rows, width, false) * width);
 }
 
 int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, const float *weight,
@@ -560,7 +559,6 @@ int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, c
     GDN2_TRY(check_view(dy, "dy", x->dtype, a.rows == 0));
     if (a.rows && (!mean || !inverse)) return fail(GDN2_ERR_ARGUMENT, "mean and inverse must be non-null");
     a.W = (int)shape->width;
-    const int64_t n = partial_rows(a.rows, a.W);
     const bool params = dweight || dbias;
     if (params) {
         if (!workspace || workspace_bytes < gdn2_layer_norm_workspace_bytes(a.rows, a.W))
@@ -573,24 +571,26 @@ int gdn2_layer_norm_backward(const gdn2_rows_shape *shape, const gdn2_view *x, c
     a.weight = weight;
     a.mean = const_cast<float *>(mean), a.inverse = const_cast<float *>(inverse);
     a.y = dx;
+    const bool bf = x->dtype == GDN2_BF16, views = vec_rows(x, a.W) && vec_rows(dy, a.W);
+    const bool vec = views && aligned(dx) && aligned(weight);
+    const int64_t n = partial_rows(a.rows, a.W, vec);
     if (params) {
         float *ws = (float *)workspace;
         a.part_w = dweight ? ws : nullptr;
         a.part_b = dbias ? ws + n * a.W : nullptr;
     }
     hipStream_t st = (hipStream_t)stream;
-    const bool bf = x->dtype == GDN2_BF16, vec = vec_rows(x, a.W) && vec_rows(dy, a.W);
     if (a.rows && a.W > kWide) {
         if (dx) {
             if (bf) hipLaunchKernelGGL((ln_backward_long<bf16_t>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
             else hipLaunchKernelGGL((ln_backward_long<float>), dim3((unsigned)a.rows), dim3(kLong), 0, st, a);
         }
     } else if (a.rows && (dx || params)) {
-        launch_ln<true>(a, x->dtype, vec && aligned(dx) && aligned(weight), n, st);
+        launch_ln<true>(a, x->dtype, vec, n, st);
     }
     if (a.rows && params && a.W > kSums) {
-        if (bf) launch_columns<bf16_t>(a, vec, n, st);
-        else launch_columns<float>(a, vec, n, st);
+        if (bf) launch_columns<bf16_t>(a, views, n, st);
+        else launch_columns<float>(a, views, n, st);
     }
     if (params)
         hipLaunchKernelGGL(ln_sum_kernel, dim3((unsigned)((a.W + (int64_t)15) / 16), 2), dim3(1024), 0, st,
