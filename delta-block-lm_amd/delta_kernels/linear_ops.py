@@ -136,6 +136,19 @@ def _attention_inputs(q, k, v, g, valid, reset, state=None, state_name="initial"
     return code, (B, T, H, K, V), views, (g, valid, reset)
 
 
+def _initial(state):
+    """The initial state as the library reads it: float32, and copied where rows or columns lie further
+    apart than its 32-bit offsets reach."""
+    if state is None:
+        return None
+    if state.dtype != F32:
+        state = state.float()
+    st = state.stride()
+    if st[2] >= 1 << 22 or st[3] >= 1 << 22:
+        return state.clone(memory_format=torch.contiguous_format)
+    return state
+
+
 def _bytes(query: str, q, v, *args) -> int:
     """A buffer's size, remembered by shape."""
     n = _size(query, _shape(q, v), *args)
@@ -149,8 +162,7 @@ def linear_attention_forward(q, k, v, g, valid=None, reset=None, initial=None,
     """Raw forward.  Returns (output, final_state, checkpoint); the checkpoint is
     private storage for linear_attention_backward, without train scratch alone."""
     code, shape, views, held = _attention_inputs(q, k, v, g, valid, reset, initial)
-    if initial is not None and initial.dtype != F32:
-        initial = initial.float()
+    initial = _initial(initial)
     B, T, H, K, V = shape
     dev = q.device
     n = _bytes("gdn2_linear_checkpoint_bytes", q, v, code, 1 if train else 0)
@@ -168,8 +180,7 @@ def linear_attention_backward(q, k, v, g, valid, reset, initial, checkpoint, d_o
     d_initial): dg in g's shape, d_initial None without an initial state.  wanted
     (dq, dk, dv, dg, d_initial): those that are False are None, and not computed."""
     code, shape, views, held = _attention_inputs(q, k, v, g, valid, reset, initial)
-    if initial is not None and initial.dtype != F32:
-        initial = initial.float()
+    initial = _initial(initial)
     B, T, H, K, V = shape
     dev = q.device
     if d_output.shape != v.shape:
