@@ -282,9 +282,6 @@ __device__ __forceinline__ void gate_store(const GateIn &x, int left, GateTile<C
     }
 }
 
-// Waits for the wave's memory operations (vmcnt(0), the other counters free).
-__device__ __forceinline__ void no_loads_left() { __builtin_amdgcn_s_waitcnt(0x0F70); }
-
 // A tile of C rows and W columns on its way from memory to LDS: 16 bytes a thread and turn.  Rows past
 // the end and columns past the width read others in their place, and become zero on the way to LDS,
 // as do the rows of padding: what they hold is not used.  VEC: unit channel stride, 16-byte aligned
@@ -345,27 +342,10 @@ struct Staged {
 
 // A chunk's rows of a dense output, from tiles whose rows are four columns from col on and whose columns
 // are the tokens 16 j + n16; out is at the chunk's first row, stride the elements between two rows.
-//
-// Whole chunks of whole columns are stored without conditions.  Otherwise the compiler cannot count the
-// stores behind the next chunk's loads, and the wait for those loads becomes one for the stores too; on
-// the other way it is told that none are left (4 x 8192 tokens, 16 heads of 128, both directions: 861 us,
-// 888 before).
 template <typename T, int TT, bool VEC>
-__device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int width, int left, bool whole,
-                                           const f32x4 (&x)[TT]) {
+__device__ __forceinline__ void store_rows(T *out, int64_t stride, int col, int width, int left, const f32x4 (&x)[TT]) {
     const int n16 = hidden(lane_id()) & 15;
     T *p = out + n16 * stride + col;
-    if (VEC && whole && left >= 16 * TT) {
-#pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            T e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Elem<T>::store(e, i, x[j][i]);
-            __builtin_memcpy(__builtin_assume_aligned(p + 16 * j * stride, 4 * sizeof(T)), e, sizeof e);
-        }
-        return;
-    }
-    no_loads_left();
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
         T e[4];
@@ -1059,13 +1039,9 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
                     for (int q = 0; q < L::TERMS; ++q)
                         M::mma(acc[j], cf[r], M::row(terms[q] + 16 * j * LDP, LDP, r * RB));
             if (o)
-                store_rows<T, TT, VEC>(o + row0 * p.vc, (int64_t)p.H * p.vc, 16 * wave + g4, p.vc, left,
-                                       p.vc == CP, acc);
-            else
-                no_loads_left();
+                store_rows<T, TT, VEC>(o + row0 * p.vc, (int64_t)p.H * p.vc, 16 * wave + g4, p.vc, left, acc);
             S = U;
         } else {
-            no_loads_left();
             walk_tokens<T, KP, LDC, false, true>(S, lds.a, lds.b, lds.c, gate, p.ka, v, p.vc,
                                                  o ? o + row0 * p.vc : nullptr, (int64_t)p.H * p.vc, left);
             fine = S.finite();
@@ -1413,15 +1389,13 @@ __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) =
                     }
             }
             if (gates_too && n > 1) S0.load_kept(kept + (ci - 1) * size, v, up32(p.K), up32(p.V));
-            if (ALL && dq) store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, aq);
-            else no_loads_left();
-            if (dv && own_v) store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, p.V == VP, av);
-            else no_loads_left();
-            if (dk && own_k) store_rows<T, TT, VEC>(dk + row0 * p.K, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, p.K == KP, ak);
-            else no_loads_left();
+            if (ALL && dq) store_rows<T, TT, VEC>(dq, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, aq);
+            if (dv && own_v)
+                store_rows<T, TT, VEC>(dv + row0 * p.V, (int64_t)p.H * p.V, 16 * wave + g4, p.V, left, av);
+            if (dk && own_k)
+                store_rows<T, TT, VEC>(dk + row0 * p.K, (int64_t)p.H * p.K, 16 * wave + g4, p.K, left, ak);
             S = U;
         } else {
-            no_loads_left();
             if (ALL && dq) {  // from the state before the chunk again
                 State<T, VP / 16> G;
                 G.load_transposed(kept + ci * size, v, up32(p.V), up32(p.K));
