@@ -148,9 +148,9 @@ __device__ __forceinline__ Split3 split3(const float (&x)[8]) {
 }
 
 // The same number, of which the compiler does not know it: what follows from it (addresses, conditions) is made
-// where it is used, and not kept in registers through the loop over chunks.  Without it linear_back spilled 39
-// registers at 64 x 64, whose reloads wait for the loads of the next chunk before them: 74 us in place of 65 for 16 x
-// 512 tokens, 8 heads of 64, both directions.
+// where it is used, and not kept in registers through the loop over chunks.  Without it linear_back spills at 64 x 64,
+// and its reloads wait for the loads of the next chunk before them: 16 x 512 tokens, 8 heads of 64, both directions
+// 77 us in place of 68.
 __device__ __forceinline__ int hidden(int x) {
     asm volatile("" : "+v"(x));
     return x;
@@ -380,7 +380,7 @@ __device__ __forceinline__ f32x4 pair_decays(const GateTile<C> &gt, int t, int s
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const bool on = seg[i] == st && (REV ? s + i >= t : s + i <= t);
-        f[i] = __builtin_amdgcn_exp2f(on ? fminf(f[i], 127.f) : -1000.f);
+        f[i] = __builtin_amdgcn_exp2f(!on ? -1000.f : f[i] > 127.f ? 127.f : f[i]);  // NaN stays
     }
     return f;
 }
@@ -412,7 +412,7 @@ struct WalkLds {
     static_assert(LDC >= LDP, "");
     T a[OUT ? C * LDA : 8], p[OUT ? ROOM * C * LDP : 8], d[DOT ? C * LDC : 8];
     // Chunks whose gates are made at a time.  With four and without the sums of DOT three forward workgroups share
-    // a unit at 64 x 64 (2048 heads of 8 tokens, bf16: 31.7 us by twos).
+    // a unit at 64 x 64 (2048 heads of 8 tokens, bf16: 26 us, by twos 32; a prompt of 3001 tokens, 8 heads, 23.4, 24.1).
     static constexpr int GATES = OUT && !DOT && CP == 64 ? 4 : 8;
     GateTile<C> gate[GATES];
     float red[DOT ? CP / 16 : 1][C], edge[CP / 16];
@@ -802,12 +802,12 @@ struct MakeGates {
 // are its x, and W_us = Gam_us (a_u.b_s)(d_u.c_s).
 //
 // Bound by latency: a chunk's tiles, weights, products and state wait for each other with two to four waves on
-// each SIMD, whose vector units issue in a third (forward) to a half (DOT) of the cycles.  bf16: 16 x 512
-// tokens, 8 heads of 64, forward 24.3 us (52 MB with the kept states, 2.1 TB/s); 4 x 8192 tokens, 16 heads of
-// 128, forward 156 us (3.4 TB/s), dq and dg 270 us (2.5 TB/s), a carry 73 us (3.7 TB/s).  With a state laid out
-// by 16 rows a tile and rows of 136 in LDS, the forward's LDS was busy for half of its time, two fifths of that
-// in bank conflicts, and it took 175 us, a carry 81.  The carry at 128 columns has four waves a SIMD: 73 us
-// where two took 87, both before that.
+// each SIMD.  bf16: 16 x 512 tokens, 8 heads of 64, forward 26.4 us (52 MB with the kept states, 2.0 TB/s); 4 x 8192
+// tokens, 16 heads of 128, forward 205 us (2.6 TB/s), dq and dg 368 us (1.2 GB with the adjoint states, 3.3 TB/s), a
+// carry 72 us (3.7 TB/s).  The second terms of the pair weights, and the second and third of the state, are a fifth to
+// a quarter of a wide forward.  Rows lie in LDS and states in accumulators as Mat says: with a state by 16 rows a
+// tile and rows of 136 a wide forward took an eighth longer, in bank conflicts.  The carry at 128 columns has four
+// waves a SIMD; with two it took a fifth longer.
 template <typename T, int KP, int CP, bool VEC, bool REV, bool OUT, bool DOT>
 __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_walk(Forward p) {
     static_assert(!(OUT && REV), "");
@@ -1057,15 +1057,15 @@ __global__ void __launch_bounds__(4 * CP, CP == 64 ? 2 : OUT ? 1 : 4) linear_wal
 }
 
 // dv and dk, from the last chunk to the first, and more by MODE.  A wave owns 16 value columns of the adjoint state
-// [K, V] and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS once a
-// chunk, in the type of the inputs, as each of its values meets all key columns.  (A walk of its own for dk read
-// three of the four tensors again, and took its pairs' decays and the state's update a second time.)  MODE 1: also
+// [K, V] and of dv as linear_walk's waves do theirs, and 16 columns of dk; for dk the state goes through LDS, a
+// term in the type of the inputs at a time, as each of its values meets all key columns.  (A walk of its own for dk
+// read three of the four tensors again, and took its pairs' decays and the state's update a second time.)  MODE 1: also
 // y_s = row_s k_s^T S v_s and the adjoint state behind every chunk, for the dq walk.  MODE 2: dq and dg as well,
 // from the forward's states before every chunk (all_in_one).
 //
-// Bound like linear_walk: bf16, 16 x 512 tokens, 8 heads of 64, all in one 39.6 us (78 MB, 2.0 TB/s); 4 x 8192
-// tokens, 16 heads of 128, without dq 320 us (2.5 TB/s), one workgroup of eight waves a unit for its 144 KB of
-// LDS and 256 registers.
+// Bound like linear_walk: bf16, 16 x 512 tokens, 8 heads of 64, all in one 46.6 us (78 MB, 1.7 TB/s); 4 x 8192
+// tokens, 16 heads of 128, without dq 471 us (1.3 GB with the adjoint states that it leaves, 2.9 TB/s; without those,
+// here and in the dq walk, 166 us less), one workgroup of eight waves a unit for its 144 KB of LDS and 256 registers.
 template <typename T, int KP, int VP, bool VEC, int MODE>
 __global__ void __launch_bounds__(4 * (KP > VP ? KP : VP), (KP > VP ? KP : VP) == 64 ? 2 : 1) linear_back(Back p) {
     typedef Mat<T> M;
@@ -1604,8 +1604,8 @@ struct Plan {
 };
 
 // Workgroups that fill the card: two a unit.  Forward and backward of 16 x 512 tokens, 8 heads of 64 / 4 x 8192
-// tokens, 16 heads of 128 / 8 x 509 f32 tokens, 8 heads of 64: 60 / 882 / 80 us; with 1024 60 / 957 / 81, with
-// 256 64 / 883 / 92.
+// tokens, 16 heads of 128 / 8 x 509 f32 tokens, 8 heads of 64: 68 / 1147 / 74 us; with 1024 68 / 1213 / 74, with
+// 256 78 / 1093 / 84.
 constexpr int64_t kWantGroups = 512;
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
@@ -1617,15 +1617,16 @@ Plan plan(const gdn2_shape *s, int dtype) {
     p.BH = s->batch * s->heads;
     p.KV = s->keys * s->values;
     // Segments of at least two chunks (the last one of an odd number has one), as many as fill the card.  (Cut at 16
-    // chunks, too, 32 x 2048 bf16 tokens, 16 heads of 64, take 258 and 509 us forward and backward in place of 211 and
-    // 472, 8 x 8192 tokens, 16 heads of 128, 541 and 1703 in place of 508 and 1639.)  With single chunks a prompt of 3001
-    // tokens, 8 heads of 64, takes 24.8 us in place of 22.3, more to join; with three for two where their number
-    // is odd 23.9, and 700 tokens in both directions 59 in place of 48 (5000 forward 26.5 in place of 27.6).
+    // chunks, too, 32 x 2048 bf16 tokens, 16 heads of 64, take 206 us forward and 538 backward in place of 168 and
+    // 502, 8 x 8192 tokens, 16 heads of 128, 523 and 1666 in place of 500 and 1626.)  With single chunks a prompt of
+    // 3001 tokens, 8 heads of 64, takes 25.9 us in place of 23.6, more to join, but 700 tokens in both directions 45 in
+    // place of 55; with three for two where their number is odd 25.6 and 70 (5000 forward 28.5 in place of 29.6).
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kWantGroups / p.BH, (p.chunks + 1) / 2));
     p.seg_chunks = (int)((p.chunks + want - 1) / want);
     p.segments = (p.chunks + p.seg_chunks - 1) / p.seg_chunks;
-    // Walked to where that costs at most a few chunks: 512 tokens (8 chunks) 60 us in both directions, 74 carried;
-    // 509 f32 tokens (16 chunks) 80 us carried, 103 walked to.
+    // Walked to where that costs at most a few chunks.  Both directions, 8 heads of 64, walked to and carried: 16 x 384
+    // and 16 x 512 bf16 tokens (6 and 8 chunks) 60 and 77, 68 and 82 us; 8 x 250 f32 tokens (8 chunks) 48 and 58; 700
+    // bf16 and 300 f32 tokens (11 and 10) 57 and 55, 51 and 50; 8 x 509 f32 tokens (16) 90 and 74.
     p.prewalk = p.chunks <= 8;
     return p;
 }
@@ -1636,8 +1637,8 @@ struct Layout {
 
 // Widths for which the backward is one walk, from a state that the forward keeps before every chunk.  Up to 64
 // such a state weighs half of what the chunk's four bf16 tensors do, which a dq walk of its own reads again:
-// forward and backward of 16 x 512 tokens, 8 heads of 64, 60 us against 68.  At 128 it weighs as much as they,
-// and the walk's registers run out: 4 x 8192 tokens, 16 heads of 128, 1253 us against 887.
+// forward and backward of 16 x 512 tokens, 8 heads of 64, 68 us against 117, 8 x 509 f32 tokens 74 against 117.  At 128
+// it weighs as much as they, and the walk's registers run out: it took 1.4 times as long as the two.
 bool all_in_one(const gdn2_shape *s) { return s->keys <= 64 && s->values <= 64; }
 
 // Checkpoint: the start states of the segments and their decays, and for a backward in one walk the states

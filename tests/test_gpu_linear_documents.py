@@ -130,3 +130,17 @@ def test_a_step_that_grows(dk, g, want):  # noqa: F811
     assert np.all(out[..., 1:] == 0) and torch.all(seq == 0) and torch.all(fin == 0)
     grown = 1e-38 * np.exp(min(g, 700.0))
     assert out[0, 0, 0, 0] == np.inf if grown > 3.4e38 else abs(out[0, 0, 0, 0] - grown) <= 1e-4 * grown
+
+
+@DTYPES
+@pytest.mark.parametrize("V", [16, 80])
+def test_a_gate_inside_one_chunk(dk, V, dtype):  # noqa: F811
+    """A document inside one chunk, with a gate that is NaN: the gradients of its gates are, and no others."""
+    p = packed(6, dtype, (5, 25), 32, V)
+    p["g"] = p["g"].copy()
+    clean = dict(p, g=p["g"].copy())
+    p["g"][0, 15, 0] = np.nan
+    got = run(dk, p, dtype)
+    same_elsewhere(got, clean, dtype, np.s_[5:25])
+    assert np.isnan(got["dg"][0, 6:25]).all()
+    assert np.isnan(got["out"][0, 15:25]).all()
