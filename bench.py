@@ -63,14 +63,21 @@ def step_bytes(B, T, H, K, V, s_in):
     return fwd + bwd
 
 
+# The sources that the profiled kernels (the scans' chunk kernels and what dispatches to them) are built from.
+PROFILED_SOURCES = ("gdn2_chunk*", "gdn2_seq*", "gdn2_api.hip", "gdn2_common.h", "gdn2_mfma.h",
+                    "gdn2_status.h")
+
+
 def sources_digest():
-    """sha256 (first 16 hex digits) over the kernel sources, file by file in name
-    order: the counter profiles record it, and a profile whose digest differs
-    from the sources being run is stale (its figures are not reported)."""
+    """sha256 (first 16 hex digits) over the sources of the profiled kernels, file by file in
+    name order: the counter profiles record it, and a profile whose digest differs
+    from the sources being run is stale (its figures are not reported).  Other operators'
+    sources do not enter: a change to them leaves these kernels as they were."""
     import glob
     import hashlib
+    csrc = os.path.join(REPO, "delta-block-lm_amd", "csrc")
     h = hashlib.sha256()
-    for path in sorted(glob.glob(os.path.join(REPO, "delta-block-lm_amd", "csrc", "*"))):
+    for path in sorted({p for n in PROFILED_SOURCES for p in glob.glob(os.path.join(csrc, n))}):
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
             h.update(f.read())
