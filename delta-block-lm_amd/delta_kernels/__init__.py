@@ -501,10 +501,13 @@ from .linear_ops import (layer_norm, layer_norm_backward, layer_norm_forward,  #
                          linear_attention, linear_attention_backward, linear_attention_forward,
                          linear_attention_step, q8_values, swiglu_q8, swiglu_q8_backward,
                          swiglu_q8_forward)
+from .recurrence_ops import (gated_recurrence, gated_recurrence_backward,  # noqa: E402
+                             gated_recurrence_forward, gated_recurrence_step)
 
 __all__ += ["causal_conv", "l2_norm", "rms_norm", "decay", "cross_entropy_rows",
             "linear_cross_entropy", "adamw_update", "FusedAdamW", "HolaReadOutput", "hola_read",
             "hola_schedule", "lm_ops", "linear_attention", "linear_attention_forward",
             "linear_attention_backward", "linear_attention_step", "layer_norm",
             "layer_norm_forward", "layer_norm_backward", "swiglu_q8", "swiglu_q8_forward",
-            "swiglu_q8_backward", "q8_values"]
+            "swiglu_q8_backward", "q8_values", "gated_recurrence", "gated_recurrence_forward",
+            "gated_recurrence_backward", "gated_recurrence_step"]

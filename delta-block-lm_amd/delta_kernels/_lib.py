@@ -165,6 +165,11 @@ SIGNATURES = {
     "gdn2_layer_norm_backward": (_I, [_P, _P, _F, _F, _F, _P, _P, _F, _F, _P, _Z, _P]),
     "gdn2_swiglu_q8_forward": (_I, [_L, _L, ctypes.c_int32] + [_P] * 5),
     "gdn2_swiglu_q8_backward": (_I, [_L, _L, ctypes.c_int32] + [_P] * 6),
+    "gdn2_recurrence_checkpoint_bytes": (_Z, [_P, ctypes.c_int32, _I]),
+    "gdn2_recurrence_scan": (_I, [_P] * 8 + [_I, _P, _Z, _P]),
+    "gdn2_recurrence_workspace_bytes": (_Z, [_P, ctypes.c_int32]),
+    "gdn2_recurrence_backward": (_I, [_P] * 6 + [_Z] + [_P] * 6 + [_Z, _P]),
+    "gdn2_recurrence_step": (_I, [_P] * 8),
     "gdn2_stage_timing": (_I, [_I]),
     "gdn2_stage_count": (_I, []),
     "gdn2_stage_name": (ctypes.c_char_p, [_I]),

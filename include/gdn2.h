@@ -608,6 +608,51 @@ GDN2_API int gdn2_swiglu_q8_backward(int64_t rows, int64_t width, int32_t dtype,
                                      const int8_t *codes, const uint8_t *exponents,
                                      const void *da, void *dh, void *a, void *stream);
 
+/* ---- Gated linear recurrence ----------------------------------------------------- */
+/* No counterpart in the reference.  For every channel of [batch, time, width], per
+ * valid token
+ *   h_t = exp(g_t) h_{t-1} + x_t,   output_t = h_t
+ * x and g (the log decay) F32 or BF16 views, each with its own dtype, strides of
+ * [batch, time, channel] (stride[3] unused); valid, reset [batch, time] F32 or NULL:
+ * padding keeps the state and gives zero, a reset on a valid token empties the state
+ * before it, and so does a gate whose exp is below 2^-126; growth past 2^127 in one
+ * token counts as 2^127.  initial [batch, width] F32 strided, or NULL (zero).  output
+ * dense in x's dtype, final_state F32 dense; states and sums are F32.  The checkpoint
+ * (16-byte aligned, sized by the query for x's dtype) holds a state for every block of
+ * 32 to 256 tokens for the backward if train is nonzero, else scratch alone.  batch,
+ * time, width and batch * width up to 2^30. */
+typedef struct gdn2_recurrence_shape {
+    int64_t batch, time, width;
+} gdn2_recurrence_shape;
+
+GDN2_API size_t gdn2_recurrence_checkpoint_bytes(const gdn2_recurrence_shape *shape, int32_t dtype,
+                                                 int train);
+GDN2_API int gdn2_recurrence_scan(const gdn2_recurrence_shape *shape, const gdn2_view *x,
+                                  const gdn2_view *g, const gdn2_view *valid,
+                                  const gdn2_view *reset, const gdn2_view *initial, void *output,
+                                  float *final_state, int train, void *checkpoint,
+                                  size_t checkpoint_bytes, void *stream);
+
+/* VJP, from the inputs and the checkpoint (which holds the initial state).  d_output
+ * [batch, time, width] (x's dtype, strided); d_final_state F32 dense or NULL (zero).
+ * dx, dg dense in x's and g's dtype, d_initial F32 dense; each may be NULL.  dg is 0 at
+ * padding, at resets and where the gate empties the state. */
+GDN2_API size_t gdn2_recurrence_workspace_bytes(const gdn2_recurrence_shape *shape, int32_t dtype);
+GDN2_API int gdn2_recurrence_backward(const gdn2_recurrence_shape *shape, const gdn2_view *x,
+                                      const gdn2_view *g, const gdn2_view *valid,
+                                      const gdn2_view *reset, const void *checkpoint,
+                                      size_t checkpoint_bytes, const gdn2_view *d_output,
+                                      const float *d_final_state, void *dx, void *dg,
+                                      float *d_initial, void *workspace, size_t workspace_bytes,
+                                      void *stream);
+
+/* One token (time == 1) on a carried state [batch, width], F32 dense, updated in place;
+ * output dense in x's dtype. */
+GDN2_API int gdn2_recurrence_step(const gdn2_recurrence_shape *shape, const gdn2_view *x,
+                                  const gdn2_view *g, const gdn2_view *valid,
+                                  const gdn2_view *reset, float *state, void *output,
+                                  void *stream);
+
 /* Measurement hook.  No counterpart in the reference: it serves benchmarks
  * that need the duration of each kernel of the chunked paths, measured on the
  * stream the kernels run on.  After gdn2_stage_timing(1), every chunked

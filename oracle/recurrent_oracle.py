@@ -1,0 +1,59 @@
+"""Float64 oracle of a recurrent language model's operators, from their formulas (numpy).
+
+They have no counterpart in the reference; the definitions are those of include/gdn2.h."""
+from __future__ import annotations
+
+import numpy as np
+
+SMALLEST = 2.0 ** -126  # a gate whose exp is below it empties the state
+
+
+def decays(g, valid=None, reset=None):
+    """exp(g) per token and channel as the recurrence uses it: 1 at padding, 0 at a reset and where it
+    would be below 2^-126, at most 2^127."""
+    with np.errstate(over="ignore"):
+        a = np.exp(g)
+    a = np.where(a < SMALLEST, 0.0, np.minimum(a, 2.0 ** 127))
+    if reset is not None:
+        a = np.where((reset != 0)[..., None], 0.0, a)
+    if valid is not None:
+        a = np.where((valid != 0)[..., None], a, 1.0)
+    return a
+
+
+def _times(a, h):
+    """a h, with 0 where a is."""
+    with np.errstate(invalid="ignore"):
+        return np.where(a == 0, 0.0, a * h)
+
+
+def recurrence(x, g, valid=None, reset=None, initial=None):
+    """x, g [B, T, W] -> (y [B, T, W], final [B, W], carried [B, T, W] = a_t h_{t-1})."""
+    B, T, W = x.shape
+    on = np.ones((B, T), bool) if valid is None else valid != 0
+    a = decays(g, valid, reset)
+    h = np.zeros((B, W)) if initial is None else np.asarray(initial, float)
+    y, carried = np.zeros((B, T, W)), np.zeros((B, T, W))
+    for t in range(T):
+        carried[:, t] = _times(a[:, t], h)
+        h = carried[:, t] + np.where(on[:, t, None], x[:, t], 0.0)
+        y[:, t] = np.where(on[:, t, None], h, 0.0)
+    return y, h, carried
+
+
+def recurrence_backward(x, g, valid, reset, initial, dy, d_final=None):
+    """(dx, dg, d_initial)."""
+    B, T, W = x.shape
+    on = np.ones((B, T), bool) if valid is None else valid != 0
+    a = decays(g, valid, reset)
+    carried = recurrence(x, g, valid, reset, initial)[2]
+    E = np.zeros((B, W)) if d_final is None else np.asarray(d_final, float)
+    dx, dg = np.zeros((B, T, W)), np.zeros((B, T, W))
+    for t in range(T - 1, -1, -1):
+        o = on[:, t, None]
+        e = E + np.where(o, dy[:, t], 0.0)
+        dx[:, t] = np.where(o, e, 0.0)
+        with np.errstate(invalid="ignore"):
+            dg[:, t] = np.where(o & (a[:, t] != 0), carried[:, t] * e, 0.0)
+        E = _times(a[:, t], e)
+    return dx, dg, E
