@@ -13,10 +13,10 @@ from __future__ import annotations
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from ._lib import check, lib
+from ._once import once
 from .linear_ops import (_CODES, F32, _call, _differentiates, _dtype, _has_tangent, _ptr,
                          _same_device, _wants_grad)
 
@@ -124,7 +124,7 @@ class _GatedRecurrence(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy, d_final):
         x, g, valid, reset, initial, ck = ctx.saved_tensors
         if dy is None and d_final is None:

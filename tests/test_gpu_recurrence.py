@@ -460,6 +460,7 @@ def test_other_derivatives_are_refused(dk):
         dk.gated_recurrence(x, x)
     x.requires_grad_(True)
     y, _ = dk.gated_recurrence(x, -x * x)
-    (d,) = torch.autograd.grad((y ** 2).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match="twice"):
-        (d ** 2).sum().backward()
+    for loss in ((y ** 2).sum(), y.sum()):  # an upstream gradient that depends on x, and one that does not
+        (d,) = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            (d ** 2).sum().backward(retain_graph=True)
