@@ -170,6 +170,10 @@ SIGNATURES = {
     "gdn2_recurrence_workspace_bytes": (_Z, [_P, ctypes.c_int32]),
     "gdn2_recurrence_backward": (_I, [_P] * 6 + [_Z] + [_P] * 6 + [_Z, _P]),
     "gdn2_recurrence_step": (_I, [_P] * 8),
+    "gdn2_token_score_forward": (_I, [_L, _L, _P, _P, _L, _P, _L, ctypes.c_float, ctypes.c_int32]
+                                 + [_P] * 6),
+    "gdn2_token_score_backward": (_I, [_L, _L, _P, _P, _L, _P, _L, ctypes.c_float, _P, _P, _L, _P, _L,
+                                       _P, _P]),
     "gdn2_stage_timing": (_I, [_I]),
     "gdn2_stage_count": (_I, []),
     "gdn2_stage_name": (ctypes.c_char_p, [_I]),

@@ -653,6 +653,36 @@ GDN2_API int gdn2_recurrence_step(const gdn2_recurrence_shape *shape, const gdn2
                                   const gdn2_view *reset, float *state, void *output,
                                   void *stream);
 
+/* ---- Scores of given tokens -------------------------------------------------------- */
+/* No counterpart in the reference, whose cross entropy is the negative log probability
+ * alone.  For rows x [rows, width] (F32 or BF16 view, stride[0] and stride[1]) with
+ * z = x / temperature and p = softmax(z):
+ *   log_probs = log p[target],  entropy = -sum p log p          [rows] F32
+ *   the `top` largest x of a row (0 to 64, at most width), largest first, the lower
+ *   index first among equal ones, NaN before all: top_tokens [rows, top] and their
+ *   log p, top_log_probs [rows, top] (both may be NULL where top is 0)
+ * target [rows] int64 and valid [rows] F32 0/1 or NULL, with element strides.  A row that
+ * is not valid is not read and gives zeros.  A target outside [0, width) gives NaN, and
+ * so does a row whose largest value is infinite or that holds a NaN; -inf is probability
+ * 0.  temperature is positive.  stats [rows, 3] F32 is what the backward reads (may be
+ * NULL).  The log probability and the entropy are made from a sum in 64 bits. */
+GDN2_API int gdn2_token_score_forward(int64_t rows, int64_t width, const gdn2_view *x,
+                                      const int64_t *target, int64_t target_stride,
+                                      const float *valid, int64_t valid_stride, float temperature,
+                                      int32_t top, float *log_probs, float *entropy,
+                                      float *top_log_probs, int64_t *top_tokens, float *stats,
+                                      void *stream);
+
+/* VJP of log_probs and entropy: dx dense in x's dtype, zeros for rows that are not valid.
+ * d_log_probs, d_entropy [rows] F32 with element strides; either may be NULL (zero).  A
+ * row with a target outside [0, width) gets NaN unless its d_log_probs is 0. */
+GDN2_API int gdn2_token_score_backward(int64_t rows, int64_t width, const gdn2_view *x,
+                                       const int64_t *target, int64_t target_stride,
+                                       const float *valid, int64_t valid_stride, float temperature,
+                                       const float *stats, const float *d_log_probs,
+                                       int64_t d_log_probs_stride, const float *d_entropy,
+                                       int64_t d_entropy_stride, void *dx, void *stream);
+
 /* Measurement hook.  No counterpart in the reference: it serves benchmarks
  * that need the duration of each kernel of the chunked paths, measured on the
  * stream the kernels run on.  After gdn2_stage_timing(1), every chunked

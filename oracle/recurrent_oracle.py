@@ -57,3 +57,30 @@ def recurrence_backward(x, g, valid, reset, initial, dy, d_final=None):
             dg[:, t] = np.where(o & (a[:, t] != 0), carried[:, t] * e, 0.0)
         E = _times(a[:, t], e)
     return dx, dg, E
+
+
+def scores(x, target, temperature=1.0):
+    """Rows x [R, N] (-inf is probability 0), target [R]: (log p [R, N], log_probs [R], entropy [R])."""
+    with np.errstate(invalid="ignore", divide="ignore"):
+        z = x / temperature
+        z = z - z.max(1, keepdims=True)
+        lp = z - np.log(np.exp(z).sum(1, keepdims=True))
+        p = np.exp(lp)
+        entropy = -np.where(p > 0, p * np.where(p > 0, lp, 0), 0 * lp.max(1, keepdims=True)).sum(1)
+    return lp, lp[np.arange(len(x)), target], entropy
+
+
+def scores_backward(x, target, d_lp, d_entropy, temperature=1.0):
+    lp, _, entropy = scores(x, target, temperature)
+    p = np.exp(lp)
+    dx = -p * (d_lp[:, None] + d_entropy[:, None] * np.where(p > 0, lp + entropy[:, None], 0))
+    dx[np.arange(len(x)), target] += d_lp
+    return dx / temperature
+
+
+def top(x, k):
+    """Indices of the k largest of each row: the lower first among equal ones, NaN before all."""
+    key = np.where(np.isnan(x), np.inf, x)
+    order = [sorted(range(x.shape[1]), key=lambda i: (not np.isnan(row[i]), -k_row[i], i))
+             for row, k_row in zip(x, key)]
+    return np.array(order, dtype=np.int64)[:, :k]

@@ -54,3 +54,32 @@ def test_cuts():
     dy[0, 5, 0] = np.nan
     dx, dg, _ = ro.recurrence_backward(x, g, None, None, None, dy)
     assert np.isfinite(dx[0, :3, 0]).all() and dg[0, 3, 0] == 0
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.6])
+def test_score_gradients_are_the_differences(temperature):
+    r = np.random.default_rng(3)
+    x, t = r.normal(size=(3, 7)), np.array([0, 6, 2])
+    x[1, 3] = -np.inf
+    d, dh = r.normal(size=3), r.normal(size=3)
+
+    def loss(x):
+        _, lp, h = ro.scores(x, t, temperature)
+        return (lp * d + h * dh).sum()
+
+    dx = ro.scores_backward(x, t, d, dh, temperature)
+    for i in np.ndindex(x.shape):
+        if not np.isfinite(x[i]):
+            assert dx[i] == 0
+            continue
+        up, down = x.copy(), x.copy()
+        up[i] += 1e-6
+        down[i] -= 1e-6
+        assert abs((loss(up) - loss(down)) / 2e-6 - dx[i]) < 1e-8
+
+
+def test_scores_of_two():
+    lp, given, h = ro.scores(np.array([[0.0, np.log(3.0)]]), np.array([1]))
+    assert np.allclose(np.exp(lp), [[0.25, 0.75]]) and np.allclose(given, np.log(0.75))
+    assert np.allclose(h, -0.25 * np.log(0.25) - 0.75 * np.log(0.75))
+    assert ro.top(np.array([[1.0, np.nan, 2.0, 2.0, -0.0, 0.0]]), 6).tolist() == [[1, 2, 3, 0, 4, 5]]
