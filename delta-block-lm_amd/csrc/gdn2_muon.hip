@@ -1,0 +1,554 @@
+// Orthogonalised updates on gfx950: Newton-Schulz products of matrices, and the Muon update of
+// parameters with its momentum.
+//
+//   X = U / (|U| + epsilon)                     |U| the root of the sum of squares
+//   A = X X^T,  B = a I + b A + c A A,  X <- B X           `steps` times
+//
+// on the side whose product is the smaller one (X has m = min(rows, cols) rows and n columns).  All
+// products have the form C = L R^T over rows that lie side by side in memory; X is kept in both
+// orientations for that.  A and A A are symmetric: the tiles on and above the diagonal are made and
+// written twice.
+//
+// Precision.  An operand of a product goes in as two float16 terms, x = hi + lo, 22 bits, and a
+// product as hi hi + hi lo + lo hi into float32 accumulators: 2^-22 of the operands, at a third of
+// the matrix cores' float16 rate, where their float32 rate is a sixteenth.  float16's range is met by powers of
+// two: the largest singular values that X, A and B can have follow from the coefficients, no entry
+// is larger, and the powers bring those to 2^14.  What is below 2^-24 there is 2^-38 of the largest.
+#include <float.h>
+#include <math.h>
+
+#include "gdn2_common.h"
+#include "gdn2_mfma.h"
+#include "gdn2_status.h"
+
+namespace gdn2 {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kGroup = 32;    // matrices of one launch
+constexpr int kParts = 64;    // partial sums of a matrix's squares
+constexpr int kChunk = 32;    // columns of a 128-byte piece of a row: 32 hi, 32 lo
+constexpr int64_t kMostBytes = (int64_t)2 << 30;  // of a group's operands
+
+// A matrix of split values: rows of `cols` logical columns (a multiple of the tile), each 128-byte
+// piece 32 columns' first terms, then their second terms.
+struct Split {
+    char *data;
+    int cols;
+};
+
+__device__ __forceinline__ char *piece_of(const Split &s, int64_t row, int col) {
+    return s.data + (row * s.cols + (col & ~(kChunk - 1))) * 4 + (col & (kChunk - 1)) * 2;
+}
+
+// 8 values to the columns col .. col + 7 of a row.
+__device__ __forceinline__ void store_split(const Split &s, int64_t row, int col, const float *v) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi[j] = (_Float16)v[j];
+        lo[j] = (_Float16)(v[j] - (float)hi[j]);
+    }
+    char *p = piece_of(s, row, col);
+    *reinterpret_cast<f16x8 *>(p) = hi;
+    *reinterpret_cast<f16x8 *>(p + 64) = lo;
+}
+
+__device__ __forceinline__ void load_split(const Split &s, int64_t row, int col, float *v) {
+    const char *p = piece_of(s, row, col);
+    const f16x8 hi = *reinterpret_cast<const f16x8 *>(p), lo = *reinterpret_cast<const f16x8 *>(p + 64);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)hi[j] + (float)lo[j];
+}
+
+// ---- the inputs -------------------------------------------------------------------------
+
+struct Tensors {
+    float *param[kGroup];
+    const float *grad[kGroup];
+    float *momentum[kGroup];
+};
+
+struct Source {
+    Tensors t;      // an update's
+    View x;         // [matrix, row, column] otherwise
+    int bf16, update, nesterov;
+    float beta;
+    int first;      // matrix of the view that the group starts with
+    int rows, cols;
+};
+
+__device__ __forceinline__ float source_at(const Source &s, int mat, int64_t r, int64_t c) {
+    if (s.update) {
+        const int64_t i = r * s.cols + c;
+        const float m = s.t.momentum[mat][i];
+        return s.nesterov ? s.t.grad[mat][i] + s.beta * m : m;
+    }
+    const int64_t i = (s.first + mat) * s.x.s0 + r * s.x.s1 + c * s.x.s2;
+    return s.bf16 ? Elem<bf16_t>::load(s.x.data, i) : Elem<float>::load(s.x.data, i);
+}
+
+// Sums of squares of every kParts-th row, in 64 bits; an update's momentum first takes the gradient.
+__global__ void __launch_bounds__(256) ns_squares(Source s, double *partial) {
+    __shared__ double red[4];
+    const int mat = blockIdx.y;
+    double sum = 0;
+    for (int64_t r = blockIdx.x; r < s.rows; r += kParts)
+        for (int64_t c = threadIdx.x; c < s.cols; c += 256) {
+            if (s.update) {
+                const int64_t i = r * s.cols + c;
+                s.t.momentum[mat][i] = s.beta * s.t.momentum[mat][i] + s.t.grad[mat][i];
+            }
+            const double v = source_at(s, mat, r, c);
+            sum += v * v;
+        }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[mat * kParts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// U / (|U| + epsilon) times scale, split, in both orientations.  One workgroup a 64 x 64 tile of U.
+__global__ void __launch_bounds__(256) ns_split(Source s, const double *partial, double epsilon, double scale,
+                                                Split by_rows, Split by_cols, int64_t step) {
+    __shared__ __align__(16) float tile[64][68];
+    const int mat = blockIdx.y, across = by_rows.cols / 64;
+    const int r0 = (int)(blockIdx.x / across) * 64, c0 = (int)(blockIdx.x % across) * 64;
+    by_rows.data += mat * step, by_cols.data += mat * step;
+    double sum = 0;
+    for (int i = 0; i < kParts; ++i) sum += partial[mat * kParts + i];
+    const double by = scale / (sqrt(sum) + epsilon);
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = i >> 6, c = i & 63;
+        tile[r][c] = r0 + r < s.rows && c0 + c < s.cols ? (float)(source_at(s, mat, r0 + r, c0 + c) * by) : 0.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int a = i >> 3, b = (i & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[a][b + j];
+        store_split(by_rows, r0 + a, c0 + b, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[b + j][a];
+        store_split(by_cols, c0 + a, r0 + b, v);
+    }
+}
+
+// ---- products -------------------------------------------------------------------------------
+
+enum Mode { GRAM, POLY, NEXT, LAST };
+
+struct GemmArgs {
+    Split l, r;                // operands: C = L R^T
+    Split out, out_t;          // GRAM, POLY: out; NEXT: both
+    int64_t l_step, r_step, out_step;  // bytes between matrices
+    int tiles_i, tiles_j, tiles, count;  // tiles of a matrix
+    int k;                     // columns of the operands
+    float scale;               // of the accumulators
+    float a, b;                // POLY: of the identity and of A, in the result's scale
+    // LAST
+    int rows, cols, tall, bf16, first;
+    float decay, rate;         // update: param = decay param - rate result
+    int update;
+    void *result;
+    Tensors t;
+};
+
+constexpr int kComputeWaves = 4, kLoadWaves = 2, kThreads = 64 * (kComputeWaves + kLoadWaves);
+
+template <int T> struct Tile {
+    static constexpr int STAGE = 2 * T * 128;  // bytes
+    static constexpr int STAGES = T == 128 ? 3 : 4;
+    static constexpr int LD = T + 4;           // floats of a row of the result's tile
+    static constexpr int OPS = STAGE / 1024 / kLoadWaves;  // loads of a wave and stage
+    static constexpr int BYTES = STAGES * STAGE > T * LD * 4 ? STAGES * STAGE : T * LD * 4;
+    static constexpr int F = T / 32;           // 16-row fragments of a wave, 2 x 2 waves
+    static_assert((STAGES - 1) * OPS <= 63, "loads on their way fit the memory counter");
+    static_assert(BYTES <= 160 * 1024, "LDS");
+};
+
+constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+constexpr int kWaitLds = 15 | (3 << 14) | (7 << 4);
+
+__device__ __forceinline__ void stage_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The stored 16-byte piece of piece x of row r: rows of 128 bytes, 64 banks of 4.
+__device__ __forceinline__ int swizzle(int r, int x) { return x ^ ((r >> 1) & 7); }
+
+// Tile (i, j) of a tile index: all of them, or, for symmetric results, i <= j.
+template <bool SYM> __device__ __forceinline__ void tile_of(int t, int nj, int *i, int *j) {
+    if (!SYM) {
+        *i = t / nj, *j = t % nj;
+        return;
+    }
+    // rows of the triangle from its last: row nj - 1 - q has q + 1 tiles
+    const int n = nj * (nj + 1) / 2 - 1 - t;
+    int q = (int)((sqrtf(8.f * n + 1.f) - 1.f) * 0.5f);
+    while ((q + 1) * (q + 2) / 2 <= n) ++q;
+    while (q * (q + 1) / 2 > n) --q;
+    *i = nj - 1 - q;
+    *j = nj - 1 - (n - q * (q + 1) / 2);
+}
+
+template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_product(GemmArgs p) {
+    using C = Tile<T>;
+    constexpr int F = C::F, LD = C::LD;
+    __shared__ __align__(1024) char lds[C::BYTES];
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    // Neighbouring tiles to one XCD (workgroups go to the eight in turn).
+    const int total = p.tiles * p.count, x = blockIdx.x & 7, full = total >> 3, more = total & 7;
+    const int at = (blockIdx.x >> 3) + x * full + min(x, more);
+    const int mat = at / p.tiles;
+    int ti, tj;
+    tile_of<SYM>(at % p.tiles, p.tiles_j, &ti, &tj);
+    const int I = ti * T, J = tj * T;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+    const int stages = p.k / kChunk;
+    f32x4 acc[F][F];
+
+    if (w >= kComputeWaves) {  // loads
+        typedef __attribute__((address_space(1))) const void *gptr;
+        typedef __attribute__((address_space(3))) void *lptr;
+        const int pw = w - kComputeWaves;
+        // operation i of this wave: rows 8 (kLoadWaves i + pw) .. + 7 of the stacked operands
+        auto issue = [&](int s) {
+            char *slot = lds + (s % C::STAGES) * C::STAGE;
+#pragma unroll
+            for (int i = 0; i < C::OPS; ++i) {
+                const int r0 = 8 * (kLoadWaves * i + pw), r = r0 + (l >> 3);
+                const bool left = r0 < T;
+                const Split &o = left ? p.l : p.r;
+                const int row = left ? r : r - T;
+                const int64_t grow = (left ? I : J) + row;
+                const char *src = o.data + mat * (left ? p.l_step : p.r_step) + grow * o.cols * 4 + s * 128 +
+                                  swizzle(row, l & 7) * 16;
+                __builtin_amdgcn_global_load_lds((gptr)src, (lptr)(slot + r0 * 128), 16, 0, 0);
+            }
+        };
+        for (int s = 0; s < C::STAGES - 1 && s < stages; ++s) issue(s);
+        for (int s = 0; s < stages; ++s) {
+            if (s + C::STAGES - 2 < stages) __builtin_amdgcn_s_waitcnt(wait_vm((C::STAGES - 2) * C::OPS));
+            else __builtin_amdgcn_s_waitcnt(wait_vm(0));
+            stage_barrier();  // stage s has landed, stage s - 1 is read
+            if (s + C::STAGES - 1 < stages) issue(s + C::STAGES - 1);
+        }
+    } else {
+        const int wi = (w >> 1) * (T / 2), wj = (w & 1) * (T / 2);
+        const int n = l & 15, g = l >> 4;
+#pragma unroll
+        for (int a = 0; a < F; ++a)
+#pragma unroll
+            for (int b = 0; b < F; ++b) acc[a][b] = zero4();
+        for (int s = 0; s < stages; ++s) {
+            __builtin_amdgcn_s_waitcnt(kWaitLds);  // stage s - 1 is read
+            stage_barrier();
+            const char *L = lds + (s % C::STAGES) * C::STAGE, *R = L + T * 128;
+            f16x8 rh[F], rl[F];
+#pragma unroll
+            for (int b = 0; b < F; ++b) {
+                const int row = wj + 16 * b + n;
+                rh[b] = *reinterpret_cast<const f16x8 *>(R + row * 128 + swizzle(row, g) * 16);
+                rl[b] = *reinterpret_cast<const f16x8 *>(R + row * 128 + swizzle(row, g + 4) * 16);
+            }
+#pragma unroll
+            for (int a = 0; a < F; ++a) {
+                const int row = wi + 16 * a + n;
+                const f16x8 lh = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g) * 16);
+                const f16x8 ll = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g + 4) * 16);
+#pragma unroll
+                for (int b = 0; b < F; ++b) {
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh[b], acc[a][b], 0, 0, 0);
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[b], acc[a][b], 0, 0, 0);
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[b], acc[a][b], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // The tile through LDS, so that whole pieces are written in either orientation.
+    __syncthreads();
+    float *S = reinterpret_cast<float *>(lds);
+    if (w < kComputeWaves) {
+        const int wi = (w >> 1) * (T / 2), wj = (w & 1) * (T / 2);
+#pragma unroll
+        for (int a = 0; a < F; ++a)
+#pragma unroll
+            for (int b = 0; b < F; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    S[(wi + 16 * a + 4 * (l >> 4) + i) * LD + wj + 16 * b + (l & 15)] = acc[a][b][i] * p.scale;
+    }
+    __syncthreads();
+    if constexpr (MODE == LAST) {
+        const int mr = p.tall ? J : I, mc = p.tall ? I : J;
+        for (int i = threadIdx.x; i < T * T; i += kThreads) {
+            const int a = i / T, b = i % T;
+            const int64_t r = mr + a, c = mc + b;
+            if (r >= p.rows || c >= p.cols) continue;
+            const float v = p.tall ? S[b * LD + a] : S[a * LD + b];
+            const int64_t o = r * p.cols + c;
+            if (p.update) {
+                float *q = p.t.param[mat] + o;
+                *q = p.decay * *q - p.rate * v;
+            } else {
+                store_out(p.result, p.bf16, (int64_t)(p.first + mat) * p.rows * p.cols + o, v);
+            }
+        }
+        return;
+    }
+    Split out = p.out, out_t = MODE == NEXT ? p.out_t : p.out;
+    out.data += mat * p.out_step, out_t.data += mat * p.out_step;
+    if constexpr (MODE == POLY) {
+        Split A = p.l;
+        A.data += mat * p.l_step;
+        for (int i = threadIdx.x; i < T * T / 8; i += kThreads) {
+            const int a = i / (T / 8), b = i % (T / 8) * 8;
+            float v[8];
+            load_split(A, I + a, J + b, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float u = S[a * LD + b + j] + p.b * v[j];
+                if (I + a == J + b + j) u += p.a;
+                S[a * LD + b + j] = u;
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < T * T / 8; i += kThreads) {
+        const int a = i / (T / 8), b = i % (T / 8) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = S[a * LD + b + j];
+        store_split(out, I + a, J + b, v);
+        if (!SYM || ti != tj) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = S[(b + j) * LD + a];
+            store_split(out_t, J + a, I + b, v);
+        }
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+
+struct Plan {
+    int tile;
+    int64_t m, n;                // padded
+    int64_t x_bytes, a_bytes;    // of one matrix: X or its transpose, A or B
+    int64_t matrix_bytes;
+    int group;
+};
+
+int check_matrices(const gdn2_matrices_shape *s) {
+    if (!s) return fail(GDN2_ERR_ARGUMENT, "shape is null");
+    if (s->count < 0 || s->rows < 1 || s->cols < 1)
+        return fail(GDN2_ERR_SHAPE, "count must be >= 0, rows and cols nonempty");
+    if (s->count > 0x7FFFFFFF || s->rows > (1 << 24) || s->cols > (1 << 24) || s->rows * s->cols > (1 << 30))
+        return fail(GDN2_ERR_SHAPE, "too many matrices, rows or columns (2^30 values of a matrix at most)");
+    return ok();
+}
+
+int64_t padded(int64_t n, int64_t t) { return (n + t - 1) / t * t; }
+
+Plan plan_of(const gdn2_matrices_shape *s) {
+    const int64_t m = s->rows < s->cols ? s->rows : s->cols, n = s->rows < s->cols ? s->cols : s->rows;
+    const int64_t ti = (m + 127) / 128;
+    Plan p;
+    const int64_t at_once = s->count < kGroup ? s->count : kGroup;
+    p.tile = m > 64 && at_once * ti * (ti + 1) / 2 >= 256 ? 128 : 64;
+    p.m = padded(m, p.tile), p.n = padded(n, p.tile);
+    p.x_bytes = p.m * p.n * 4, p.a_bytes = p.m * p.m * 4;
+    p.matrix_bytes = 4 * p.x_bytes + 2 * p.a_bytes;
+    int64_t g = kMostBytes / p.matrix_bytes;
+    if (g > kGroup) g = kGroup;
+    if (g > s->count) g = s->count;
+    p.group = g < 1 ? 1 : (int)g;
+    return p;
+}
+
+size_t workspace_of(const Plan &p) {
+    return (size_t)p.group * p.matrix_bytes + (size_t)p.group * kParts * sizeof(double);
+}
+
+// The largest |a t + b t^3 + c t^5| for t in [0, s], and the largest |a + b u + c u^2| for u in [0, s^2].
+struct Bounds {
+    double x, poly;
+};
+
+Bounds bounds_of(const float *k, double s) {
+    const double a = k[0], b = k[1], c = k[2];
+    auto value = [&](double t) { return fabs(t * (a + t * t * (b + c * t * t))); };
+    auto poly = [&](double u) { return fabs(a + u * (b + c * u)); };
+    Bounds r = {value(s), fmax(fabs(a), poly(s * s))};
+    auto turn = [&](double u) {  // where the derivative in t is zero: a + 3 b u + 5 c u^2 = 0, u = t^2
+        if (u > 0 && u < s * s) r.x = fmax(r.x, value(sqrt(u)));
+    };
+    if (c != 0) {
+        const double d = 9 * b * b - 20 * a * c;
+        if (d >= 0) turn((-3 * b + sqrt(d)) / (10 * c)), turn((-3 * b - sqrt(d)) / (10 * c));
+        const double v = -b / (2 * c);
+        if (v > 0 && v < s * s) r.poly = fmax(r.poly, poly(v));
+    } else if (b != 0) {
+        turn(-a / (3 * b));
+    }
+    return r;
+}
+
+// The power of two that brings a bound to 2^13 .. 2^14.
+double power_for(double bound) {
+    int e;
+    frexp(bound > 1e-30 ? bound : 1e-30, &e);  // bound < 2^e
+    return ldexp(1.0, 14 - e);
+}
+
+int check_steps(int steps, const float *k, float epsilon) {
+    if (steps < 1 || steps > 100) return fail(GDN2_ERR_ARGUMENT, "steps must be 1 to 100");
+    if (!k) return fail(GDN2_ERR_ARGUMENT, "coefficients is null");
+    if (!(epsilon >= 0) || !(epsilon <= FLT_MAX)) return fail(GDN2_ERR_ARGUMENT, "epsilon must be >= 0 and finite");
+    double s = 1;
+    for (int i = 0; i < steps; ++i) {
+        const Bounds b = bounds_of(k, s);
+        s = b.x * 1.001;
+        if (!(s < 1e9) || !(b.poly < 1e9))
+            return fail(GDN2_ERR_ARGUMENT, "coefficients make the values grow past 1e9 in step %d", i + 1);
+    }
+    return ok();
+}
+
+template <int T> void launch_mode(Mode mode, const GemmArgs &a, hipStream_t st) {
+    const dim3 grid((unsigned)(a.tiles * a.count)), block(kThreads);
+    switch (mode) {
+        case GRAM: hipLaunchKernelGGL((ns_product<T, GRAM>), grid, block, 0, st, a); break;
+        case POLY: hipLaunchKernelGGL((ns_product<T, POLY>), grid, block, 0, st, a); break;
+        case NEXT: hipLaunchKernelGGL((ns_product<T, NEXT>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((ns_product<T, LAST>), grid, block, 0, st, a);
+    }
+}
+
+// All products of one group of matrices; last holds the fields of the last product's results.
+void run_group(const Plan &p, const Source &src, int count, int steps, const float *k, float epsilon,
+               const GemmArgs &last, char *ws, hipStream_t st) {
+    const bool tall = src.rows > src.cols;
+    double *partial = (double *)(ws + (size_t)p.group * p.matrix_bytes);
+    // of the first matrix; the others follow at matrix_bytes
+    Split X[2], XT[2];
+    for (int i = 0; i < 2; ++i) {
+        X[i] = {ws + 2 * i * p.x_bytes, (int)p.n};
+        XT[i] = {ws + (2 * i + 1) * p.x_bytes, (int)p.m};
+    }
+    const Split A = {ws + 4 * p.x_bytes, (int)p.m}, B = {ws + 4 * p.x_bytes + p.a_bytes, (int)p.m};
+    double s = 1, sx = power_for(s);
+    hipLaunchKernelGGL(ns_squares, dim3(kParts, count), dim3(256), 0, st, src, partial);
+    const int64_t pr = tall ? p.n : p.m, pc = tall ? p.m : p.n;
+    hipLaunchKernelGGL(ns_split, dim3((unsigned)(pr / 64 * (pc / 64)), count), dim3(256), 0, st, src,
+                       partial, (double)epsilon, sx, tall ? XT[0] : X[0], tall ? X[0] : XT[0], p.matrix_bytes);
+    const int ti = (int)(p.m / p.tile), tn = (int)(p.n / p.tile);
+    for (int i = 0; i < steps; ++i) {
+        const Split &x = X[i & 1], &xt = XT[i & 1];
+        const Bounds b = bounds_of(k, s);
+        const double sa = power_for(s * s), sb = power_for(b.poly), next = b.x * 1.001;
+        GemmArgs g = last;
+        g.count = count;
+        g.l_step = g.r_step = g.out_step = p.matrix_bytes;
+        auto run = [&](Mode mode) {
+            if (p.tile == 128) launch_mode<128>(mode, g, st);
+            else launch_mode<64>(mode, g, st);
+        };
+        g.l = g.r = x, g.out = A;
+        g.tiles_i = g.tiles_j = ti, g.tiles = ti * (ti + 1) / 2, g.k = (int)p.n;
+        g.scale = (float)(sa / (sx * sx));
+        run(GRAM);
+        g.l = g.r = A, g.out = B, g.k = (int)p.m;
+        g.scale = (float)(k[2] * sb / (sa * sa)), g.a = (float)(k[0] * sb), g.b = (float)(k[1] * sb / sa);
+        run(POLY);
+        g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
+        g.tiles_j = tn, g.tiles = ti * tn;
+        const double to = i + 1 < steps ? power_for(next) : 1;
+        g.scale = (float)(to / (sb * sx));
+        run(i + 1 < steps ? NEXT : LAST);
+        s = next, sx = to;
+    }
+}
+
+int check_workspace(const void *p, size_t have, size_t need) {
+    if (!p || have < need) return fail(GDN2_ERR_WORKSPACE, "workspace is too small: %zu bytes needed", need);
+    if ((uintptr_t)p & 15) return fail(GDN2_ERR_ARGUMENT, "workspace must be 16-byte aligned");
+    return ok();
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+size_t gdn2_orthogonalize_workspace_bytes(const gdn2_matrices_shape *shape) {
+    if (check_matrices(shape)) return 0;
+    return workspace_of(plan_of(shape));
+}
+
+int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, void *result, int steps,
+                       const float *coefficients, float epsilon, void *workspace, size_t workspace_bytes,
+                       void *stream) {
+    GDN2_TRY(check_matrices(shape));
+    GDN2_TRY(check_view(x, "x", -1, shape->count == 0));
+    GDN2_TRY(check_steps(steps, coefficients, epsilon));
+    if (shape->count == 0) return ok();
+    if (!result) return fail(GDN2_ERR_ARGUMENT, "result must be non-null");
+    const Plan p = plan_of(shape);
+    GDN2_TRY(check_workspace(workspace, workspace_bytes, workspace_of(p)));
+    Source s{};
+    s.x = make_view(x), s.bf16 = x->dtype == GDN2_BF16;
+    s.rows = (int)shape->rows, s.cols = (int)shape->cols;
+    GemmArgs last{};
+    last.rows = s.rows, last.cols = s.cols, last.tall = s.rows > s.cols, last.bf16 = s.bf16;
+    last.result = result;
+    for (int64_t i = 0; i < shape->count; i += p.group) {
+        s.first = last.first = (int)i;
+        const int64_t left = shape->count - i;
+        run_group(p, s, (int)(left < p.group ? left : p.group), steps, coefficients, epsilon, last,
+                  (char *)workspace, (hipStream_t)stream);
+    }
+    return launch_status(hipGetLastError(), "gdn2_orthogonalize");
+}
+
+int gdn2_muon_update(const gdn2_matrices_shape *shape, const gdn2_muon_tensor *tensors, float lr, float beta,
+                     int nesterov, float decay, int steps, const float *coefficients, float epsilon,
+                     void *workspace, size_t workspace_bytes, void *stream) {
+    GDN2_TRY(check_matrices(shape));
+    GDN2_TRY(check_steps(steps, coefficients, epsilon));
+    if (shape->count == 0) return ok();
+    if (!tensors) return fail(GDN2_ERR_ARGUMENT, "tensors is null");
+    for (int64_t i = 0; i < shape->count; ++i)
+        if (!tensors[i].param || !tensors[i].grad || !tensors[i].momentum)
+            return fail(GDN2_ERR_ARGUMENT, "tensor %lld has a null pointer", (long long)i);
+    const Plan p = plan_of(shape);
+    GDN2_TRY(check_workspace(workspace, workspace_bytes, workspace_of(p)));
+    Source s{};
+    s.update = 1, s.nesterov = nesterov != 0, s.beta = beta;
+    s.rows = (int)shape->rows, s.cols = (int)shape->cols;
+    GemmArgs last{};
+    last.rows = s.rows, last.cols = s.cols, last.tall = s.rows > s.cols, last.update = 1;
+    last.decay = 1.f - lr * decay;
+    last.rate = lr * sqrtf(s.rows > s.cols ? (float)s.rows / (float)s.cols : 1.f);
+    for (int64_t i = 0; i < shape->count; i += p.group) {
+        const int64_t left = shape->count - i;
+        const int n = (int)(left < p.group ? left : p.group);
+        for (int j = 0; j < n; ++j) {
+            s.t.param[j] = tensors[i + j].param;
+            s.t.grad[j] = tensors[i + j].grad;
+            s.t.momentum[j] = tensors[i + j].momentum;
+        }
+        last.t = s.t;
+        run_group(p, s, n, steps, coefficients, epsilon, last, (char *)workspace, (hipStream_t)stream);
+    }
+    return launch_status(hipGetLastError(), "gdn2_muon_update");
+}
+
+}  // extern "C"

@@ -505,6 +505,7 @@ from .recurrence_ops import (gated_recurrence, gated_recurrence_backward,  # noq
                              gated_recurrence_forward, gated_recurrence_step)
 from .score_ops import (TokenLogProbs, token_log_probs, token_log_probs_backward,  # noqa: E402
                         token_log_probs_forward)
+from .muon_ops import Muon, muon_update, orthogonalize  # noqa: E402
 
 __all__ += ["causal_conv", "l2_norm", "rms_norm", "decay", "cross_entropy_rows",
             "linear_cross_entropy", "adamw_update", "FusedAdamW", "HolaReadOutput", "hola_read",
@@ -513,4 +514,5 @@ __all__ += ["causal_conv", "l2_norm", "rms_norm", "decay", "cross_entropy_rows",
             "layer_norm_forward", "layer_norm_backward", "swiglu_q8", "swiglu_q8_forward",
             "swiglu_q8_backward", "q8_values", "gated_recurrence", "gated_recurrence_forward",
             "gated_recurrence_backward", "gated_recurrence_step", "TokenLogProbs", "token_log_probs",
-            "token_log_probs_forward", "token_log_probs_backward"]
+            "token_log_probs_forward", "token_log_probs_backward", "orthogonalize", "muon_update",
+            "Muon"]

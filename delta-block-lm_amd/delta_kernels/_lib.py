@@ -174,6 +174,10 @@ SIGNATURES = {
                                  + [_P] * 6),
     "gdn2_token_score_backward": (_I, [_L, _L, _P, _P, _L, _P, _L, ctypes.c_float, _P, _P, _L, _P, _L,
                                        _P, _P]),
+    "gdn2_orthogonalize_workspace_bytes": (_Z, [_P]),
+    "gdn2_orthogonalize": (_I, [_P, _P, _P, _I, _P, ctypes.c_float, _P, _Z, _P]),
+    "gdn2_muon_update": (_I, [_P, _P, ctypes.c_float, ctypes.c_float, _I, ctypes.c_float, _I, _P,
+                              ctypes.c_float, _P, _Z, _P]),
     "gdn2_stage_timing": (_I, [_I]),
     "gdn2_stage_count": (_I, []),
     "gdn2_stage_name": (ctypes.c_char_p, [_I]),

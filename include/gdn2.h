@@ -683,6 +683,42 @@ GDN2_API int gdn2_token_score_backward(int64_t rows, int64_t width, const gdn2_v
                                        int64_t d_log_probs_stride, const float *d_entropy,
                                        int64_t d_entropy_stride, void *dx, void *stream);
 
+/* ---- Orthogonalised updates ----------------------------------------------------------- */
+/* No counterpart in the reference, whose optimizer is AdamW.  Newton-Schulz products of
+ * `count` matrices [rows, cols]:
+ *   X = U / (|U| + epsilon),  then `steps` times
+ *   A = X X^T,  X <- (a I + b A + c A A) X        coefficients {a, b, c}
+ * on the side with fewer rows (a tall matrix's transpose); |U| is the root of its sum of
+ * squares, in 64 bits.  Products are of float16 pairs (22 bits of a value) summed in F32.
+ * steps 1 to 100; coefficients under which values could grow past 1e9 are refused. */
+typedef struct gdn2_matrices_shape {
+    int64_t count, rows, cols;
+} gdn2_matrices_shape;
+
+GDN2_API size_t gdn2_orthogonalize_workspace_bytes(const gdn2_matrices_shape *shape);
+
+/* x: F32 or BF16 view, strides of [matrix, row, column]; result dense in x's dtype. */
+GDN2_API int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, void *result,
+                                int steps, const float *coefficients, float epsilon,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
+/* The Muon update of `count` parameters of one shape (dense F32 each):
+ *   momentum = beta momentum + grad
+ *   U = grad + beta momentum if nesterov is nonzero, else momentum
+ *   param = (1 - lr decay) param - lr sqrt(max(1, rows / cols)) orthogonalised(U)
+ * No two params or momenta may share memory.  The workspace is gdn2_orthogonalize's;
+ * tensors is read during the call. */
+typedef struct gdn2_muon_tensor {
+    float *param;
+    const float *grad;
+    float *momentum;
+} gdn2_muon_tensor;
+
+GDN2_API int gdn2_muon_update(const gdn2_matrices_shape *shape, const gdn2_muon_tensor *tensors,
+                              float lr, float beta, int nesterov, float decay, int steps,
+                              const float *coefficients, float epsilon, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
 /* Measurement hook.  No counterpart in the reference: it serves benchmarks
  * that need the duration of each kernel of the chunked paths, measured on the
  * stream the kernels run on.  After gdn2_stage_timing(1), every chunked

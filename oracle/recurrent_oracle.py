@@ -84,3 +84,44 @@ def top(x, k):
     order = [sorted(range(x.shape[1]), key=lambda i: (not np.isnan(row[i]), -k_row[i], i))
              for row, k_row in zip(x, key)]
     return np.array(order, dtype=np.int64)[:, :k]
+
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(u, steps=5, coefficients=COEFFICIENTS, epsilon=1e-7, product=np.matmul):
+    """One matrix [rows, cols]; product(L, R^T) forms the products."""
+    a, b, c = coefficients
+    tall = u.shape[0] > u.shape[1]
+    x = u.T if tall else u
+    x = x / (np.sqrt((x ** 2).sum()) + epsilon)
+    for _ in range(steps):
+        gram = product(x, x.T)
+        x = product(a * np.eye(len(x)) + b * gram + c * product(gram, gram), x)
+    return x.T if tall else x
+
+
+def split_product(left, right):
+    """A product of float16 pairs that are scaled to 2^13 .. 2^14, summed in float32 by 32 columns: the
+    arithmetic of the library's products."""
+    def split(x):
+        top = np.abs(x).max()
+        by = 2.0 ** (14 - np.frexp(top)[1]) if top > 0 else 1.0
+        hi = (x * by).astype(np.float16).astype(float)
+        return hi, (x * by - hi).astype(np.float16).astype(float), by
+
+    (lh, ll, lb), (rh, rl, rb) = split(left), split(right)
+    total = np.zeros((left.shape[0], right.shape[1]), np.float32)
+    for k in range(0, left.shape[1], 32):
+        s = slice(k, k + 32)
+        for a, b in ((lh, rh), (lh, rl), (ll, rh)):
+            total = (total + (a[:, s] @ b[s])).astype(np.float32)
+    return total.astype(float) / (lb * rb)
+
+
+def muon(x, g, m, lr, beta=0.95, nesterov=True, decay=0.0, steps=5, coefficients=COEFFICIENTS,
+         epsilon=1e-7, product=np.matmul):
+    """(x, m) after one update."""
+    m = beta * m + g
+    o = orthogonalize(g + beta * m if nesterov else m, steps, coefficients, epsilon, product)
+    return (1 - lr * decay) * x - lr * np.sqrt(max(1.0, x.shape[0] / x.shape[1])) * o, m

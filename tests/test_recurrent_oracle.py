@@ -83,3 +83,19 @@ def test_scores_of_two():
     assert np.allclose(np.exp(lp), [[0.25, 0.75]]) and np.allclose(given, np.log(0.75))
     assert np.allclose(h, -0.25 * np.log(0.25) - 0.75 * np.log(0.75))
     assert ro.top(np.array([[1.0, np.nan, 2.0, 2.0, -0.0, 0.0]]), 6).tolist() == [[1, 2, 3, 0, 4, 5]]
+
+
+@pytest.mark.parametrize("shape", [(4, 9), (9, 4), (5, 5)])
+def test_products_change_singular_values_alone(shape):
+    r = np.random.default_rng(2)
+    u = r.normal(size=shape)
+    w, s, vt = np.linalg.svd(u, full_matrices=False)
+    a, b, c = ro.COEFFICIENTS
+    t = s / (np.sqrt((s ** 2).sum()) + 1e-7)
+    for _ in range(5):
+        t = t * (a + b * t ** 2 + c * t ** 4)
+    got = ro.orthogonalize(u)
+    assert np.allclose(got, w @ np.diag(t) @ vt, atol=1e-12)
+    assert np.all((t > 0.6) & (t < 1.3))
+    near = ro.orthogonalize(u, product=ro.split_product)
+    assert 0 < np.abs(near - got).max() < 1e-4
