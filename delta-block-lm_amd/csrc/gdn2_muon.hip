@@ -27,7 +27,7 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kGroup = 32;    // matrices of one launch
-constexpr int kParts = 64;    // partial sums of a matrix's squares
+constexpr int kParts = 256;   // partial sums of a matrix's squares
 constexpr int kChunk = 32;    // columns of a 128-byte piece of a row: 32 hi, 32 lo
 constexpr int64_t kMostBytes = (int64_t)2 << 30;  // of a group's operands
 
@@ -74,6 +74,7 @@ struct Source {
     Tensors t;      // an update's
     View x;         // [matrix, row, column] otherwise
     int bf16, update, nesterov;
+    int dense;      // the view's matrices are rows x cols side by side
     float beta;
     int first;      // matrix of the view that the group starts with
     int rows, cols;
@@ -89,20 +90,61 @@ __device__ __forceinline__ float source_at(const Source &s, int mat, int64_t r, 
     return s.bf16 ? Elem<bf16_t>::load(s.x.data, i) : Elem<float>::load(s.x.data, i);
 }
 
-// Sums of squares of every kParts-th row, in 64 bits; an update's momentum first takes the gradient.
-__global__ void __launch_bounds__(256) ns_squares(Source s, double *partial) {
+// Four values of a dense matrix from element i, zeros behind its end n.
+template <typename T> __device__ __forceinline__ void load4(const T *p, int64_t i, int64_t n, float *v) {
+    if (i + 4 <= n) {
+        T w[4];
+        __builtin_memcpy(w, p + i, sizeof(w));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = Elem<T>::load(w, j);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = i + j < n ? Elem<T>::load(p, i + j) : 0.f;
+}
+
+// Sums of squares in 64 bits: of a part of a dense matrix's values, or of every kParts-th row of
+// another; an update's momentum first takes the gradient.
+template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squares(Source s, double *partial) {
     __shared__ double red[4];
     const int mat = blockIdx.y;
     double sum = 0;
-    for (int64_t r = blockIdx.x; r < s.rows; r += kParts)
-        for (int64_t c = threadIdx.x; c < s.cols; c += 256) {
-            if (s.update) {
-                const int64_t i = r * s.cols + c;
-                s.t.momentum[mat][i] = s.beta * s.t.momentum[mat][i] + s.t.grad[mat][i];
+    if (UPDATE || s.dense) {
+        const int64_t n = (int64_t)s.rows * s.cols, per = ((n + kParts - 1) / kParts + 3) & ~(int64_t)3;
+        const int64_t end = min(n, (blockIdx.x + 1) * per);
+        const T *x = UPDATE ? nullptr : (const T *)s.x.data + (s.first + mat) * s.x.s0;
+        for (int64_t i = blockIdx.x * per + 4 * (int64_t)threadIdx.x; i < end; i += 4 * 256) {
+            float v[4];
+            if constexpr (UPDATE) {
+                float g[4], m[4];
+                load4(s.t.grad[mat], i, end, g);
+                load4(s.t.momentum[mat], i, end, m);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    m[j] = s.beta * m[j] + g[j];
+                    v[j] = s.nesterov ? g[j] + s.beta * m[j] : m[j];
+                }
+                if (i + 4 <= end) {
+                    __builtin_memcpy(s.t.momentum[mat] + i, m, sizeof(m));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j < end) s.t.momentum[mat][i + j] = m[j];
+                        else v[j] = 0.f;
+                }
+            } else {
+                load4(x, i, end, v);
             }
-            const double v = source_at(s, mat, r, c);
-            sum += v * v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += (double)v[j] * v[j];
         }
+    } else {
+        for (int64_t r = blockIdx.x; r < s.rows; r += kParts)
+            for (int64_t c = threadIdx.x; c < s.cols; c += 256) {
+                const double v = source_at(s, mat, r, c);
+                sum += v * v;
+            }
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -117,8 +159,14 @@ __global__ void __launch_bounds__(256) ns_split(Source s, const double *partial,
     const int mat = blockIdx.y, across = by_rows.cols / 64;
     const int r0 = (int)(blockIdx.x / across) * 64, c0 = (int)(blockIdx.x % across) * 64;
     by_rows.data += mat * step, by_cols.data += mat * step;
-    double sum = 0;
-    for (int i = 0; i < kParts; ++i) sum += partial[mat * kParts + i];
+    __shared__ double red[4];
+    static_assert(kParts == 256, "one part a thread");
+    double sum = partial[mat * kParts + threadIdx.x];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = (red[0] + red[1]) + (red[2] + red[3]);
     const double by = scale / (sqrt(sum) + epsilon);
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
         const int r = i >> 6, c = i & 63;
@@ -161,7 +209,13 @@ constexpr int kComputeWaves = 4, kLoadWaves = 2, kThreads = 64 * (kComputeWaves 
 
 template <int T> struct Tile {
     static constexpr int STAGE = 2 * T * 128;  // bytes
-    static constexpr int STAGES = T == 128 ? 3 : 4;
+#ifndef S128
+#define S128 3
+#endif
+#ifndef S64
+#define S64 4
+#endif
+    static constexpr int STAGES = T == 128 ? S128 : S64;
     static constexpr int LD = T + 4;           // floats of a row of the result's tile
     static constexpr int OPS = STAGE / 1024 / kLoadWaves;  // loads of a wave and stage
     static constexpr int BYTES = STAGES * STAGE > T * LD * 4 ? STAGES * STAGE : T * LD * 4;
@@ -360,7 +414,11 @@ Plan plan_of(const gdn2_matrices_shape *s) {
     const int64_t ti = (m + 127) / 128;
     Plan p;
     const int64_t at_once = s->count < kGroup ? s->count : kGroup;
+#ifdef FORCE_TILE
+    p.tile = FORCE_TILE;
+#else
     p.tile = m > 64 && at_once * ti * (ti + 1) / 2 >= 256 ? 128 : 64;
+#endif
     p.m = padded(m, p.tile), p.n = padded(n, p.tile);
     p.x_bytes = p.m * p.n * 4, p.a_bytes = p.m * p.m * 4;
     p.matrix_bytes = 4 * p.x_bytes + 2 * p.a_bytes;
@@ -443,7 +501,10 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
     }
     const Split A = {ws + 4 * p.x_bytes, (int)p.m}, B = {ws + 4 * p.x_bytes + p.a_bytes, (int)p.m};
     double s = 1, sx = power_for(s);
-    hipLaunchKernelGGL(ns_squares, dim3(kParts, count), dim3(256), 0, st, src, partial);
+    const dim3 parts(kParts, count), threads(256);
+    if (src.update) hipLaunchKernelGGL((ns_squares<float, true>), parts, threads, 0, st, src, partial);
+    else if (src.bf16) hipLaunchKernelGGL((ns_squares<bf16_t, false>), parts, threads, 0, st, src, partial);
+    else hipLaunchKernelGGL((ns_squares<float, false>), parts, threads, 0, st, src, partial);
     const int64_t pr = tall ? p.n : p.m, pc = tall ? p.m : p.n;
     hipLaunchKernelGGL(ns_split, dim3((unsigned)(pr / 64 * (pc / 64)), count), dim3(256), 0, st, src,
                        partial, (double)epsilon, sx, tall ? XT[0] : X[0], tall ? X[0] : XT[0], p.matrix_bytes);
@@ -506,6 +567,7 @@ int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, voi
     Source s{};
     s.x = make_view(x), s.bf16 = x->dtype == GDN2_BF16;
     s.rows = (int)shape->rows, s.cols = (int)shape->cols;
+    s.dense = s.x.s2 == 1 && s.x.s1 == s.cols;
     GemmArgs last{};
     last.rows = s.rows, last.cols = s.cols, last.tall = s.rows > s.cols, last.bf16 = s.bf16;
     last.result = result;

@@ -82,32 +82,35 @@ struct Sums {
     float u;
 };
 
-__device__ __forceinline__ Sums merge(const Sums &a, const Sums &b, float inv_t) {
-    const float M = fmaxf(a.m, b.m);
-    const float da = fmaxf((a.m - M) * inv_t, kLowest), db = fmaxf((b.m - M) * inv_t, kLowest);
-    const float ea = __expf(da), eb = __expf(db);
-    return {M, a.s * ea + b.s * eb,
-            ea * (a.u + (float)a.s * da) + eb * (b.u + (float)b.s * db)};
-}
+struct BlockShared {
+    float m[kMaxThreads / 64], u[kMaxThreads / 64];
+    double s[kMaxThreads / 64];
+};
 
-__device__ __forceinline__ Sums merge_lanes(const Sums &a, int d, float inv_t) {
-    const Sums b = {__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.u, d)};
-    // the same order of operands in both lanes
-    const bool low = (threadIdx.x & d) == 0;
-    return merge(low ? a : b, low ? b : a, inv_t);
-}
-
-// The sums of the workgroup, in every thread.
-__device__ Sums merge_block(Sums a, Sums *red, float inv_t) {
+// The sums of the workgroup, in every thread: first the maximum, so that a thread's sums are scaled
+// once, then plain sums in a fixed order.
+__device__ Sums merge_block(const Sums &a, BlockShared &sh, float inv_t) {
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
+    float M = a.m;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) a = merge_lanes(a, d, inv_t);
-    const int waves = blockDim.x >> 6;
-    if (waves == 1) return a;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = red[0];
-    for (int w = 1; w < waves; ++w) a = merge(a, red[w], inv_t);
-    return a;
+    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
+    if (waves > 1) {
+        if ((threadIdx.x & 63) == 0) sh.m[wave] = M;
+        __syncthreads();
+        for (int w = 0; w < waves; ++w) M = fmaxf(M, sh.m[w]);
+    }
+    const float d = fmaxf((a.m - M) * inv_t, kLowest), e = __expf(d);
+    double s = a.s * e;
+    float u = e * (a.u + (float)a.s * d);
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) s += __shfl_xor(s, k), u += __shfl_xor(u, k);
+    if (waves > 1) {
+        if ((threadIdx.x & 63) == 0) sh.s[wave] = s, sh.u[wave] = u;
+        __syncthreads();
+        s = 0, u = 0;
+        for (int w = 0; w < waves; ++w) s += sh.s[w], u += sh.u[w];
+    }
+    return {M, s, u};
 }
 
 template <typename T, bool UNIT>
@@ -158,15 +161,23 @@ __device__ __forceinline__ uint64_t order_of(float v, int64_t i) {
 
 __device__ __forceinline__ int64_t index_of(uint64_t o) { return 0xFFFFFFFFu - (uint32_t)o; }
 
+// The value that was ordered (+0 for -0), of those that are numbers.
+__device__ __forceinline__ float value_of(uint64_t o) {
+    const uint32_t key = (uint32_t)(o >> 32);
+    return __uint_as_float(key ^ ((int32_t)key < 0 ? 0x80000000u : 0xFFFFFFFFu));
+}
+
 __device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t r, int rank, int64_t i, float v,
                                           float m, double log_s) {
     a.top_tokens[r * a.top + rank] = i;
     a.top_log_probs[r * a.top + rank] = (float)((double)(v - m) * a.inv_t - log_s);
 }
 
+constexpr int kGroups = 256;  // of threads, at most, whose maxima give the bound
+
 struct alignas(16) TopShared {
     union {
-        float maxima[kMaxThreads];
+        float maxima[kGroups];
         uint64_t list[kList];
     };
     uint64_t best[kMaxThreads / 64];
@@ -212,29 +223,40 @@ __device__ void find_top(const ScoreArgs &a, const T *row, int64_t r, float mine
         search_top<T, UNIT>(a, row, r, m, log_s, sh);
         return;
     }
-    sh.maxima[i0] = mine;
+    // groups of 1, 2 or 4 neighbours, each thread counting a share of the maxima above its group's
+    const int groups = min(nt, kGroups), each = nt / groups;
+    float top = mine;
+    if (each > 1) top = fmaxf(top, __shfl_xor(top, 1));
+    if (each > 2) top = fmaxf(top, __shfl_xor(top, 2));
+    const int g = i0 / each, share = i0 % each;
+    if (share == 0) sh.maxima[g] = top;
     if (i0 == 0) sh.count = 0;
     __syncthreads();
     int rank = 0;
-    for (int i = 0; i < nt; i += 4) {
+    for (int i = share * (groups / each); i < (share + 1) * (groups / each); i += 4) {
         const float4 o = *reinterpret_cast<const float4 *>(sh.maxima + i);
-        rank += (o.x > mine || (o.x == mine && i < i0)) + (o.y > mine || (o.y == mine && i + 1 < i0)) +
-                (o.z > mine || (o.z == mine && i + 2 < i0)) + (o.w > mine || (o.w == mine && i + 3 < i0));
+        rank += (o.x > top || (o.x == top && i < g)) + (o.y > top || (o.y == top && i + 1 < g)) +
+                (o.z > top || (o.z == top && i + 2 < g)) + (o.w > top || (o.w == top && i + 3 < g));
     }
-    if (rank == a.top - 1) sh.bound = mine;
+    if (each > 1) rank += __shfl_xor(rank, 1);
+    if (each > 2) rank += __shfl_xor(rank, 2);
+    if (share == 0 && rank == a.top - 1) sh.bound = top;
     __syncthreads();  // maxima are read: their place is the list's
     const float bound = sh.bound;
     if (mine >= bound && mine > -FLT_MAX) {
         const int64_t step = (int64_t)nt * N;
-        for (int64_t c = (int64_t)i0 * N; c < a.width; c += step) {
-            float v[N];
-            load_cols<T, UNIT>(a, row, c, v);
+        for (int64_t c = (int64_t)i0 * N; c < a.width; c += kUnroll * step) {
+            float v[kUnroll][N];
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (v[j] >= bound && v[j] > -INFINITY) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kList) sh.list[at] = order_of(v[j], c + j);
-                }
+            for (int i = 0; i < kUnroll; ++i) load_cols<T, UNIT>(a, row, c + i * step, v[i]);
+#pragma unroll
+            for (int i = 0; i < kUnroll; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (v[i][j] >= bound && v[i][j] > -INFINITY) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kList) sh.list[at] = order_of(v[i][j], c + i * step + j);
+                    }
         }
     }
     __syncthreads();
@@ -248,16 +270,13 @@ __device__ void find_top(const ScoreArgs &a, const T *row, int64_t r, float mine
         const uint64_t o = sh.list[i];
         int before = 0;
         for (int k = 0; k < n; ++k) before += sh.list[k] > o;
-        if (before < a.top) {
-            const int64_t c = index_of(o);
-            write_top(a, r, before, c, Elem<T>::load(row, (UNIT ? 1 : a.cs) * c), m, log_s);
-        }
+        if (before < a.top) write_top(a, r, before, index_of(o), value_of(o), m, log_s);
     }
 }
 
 template <typename T, bool UNIT, bool TOP>
 __global__ void __launch_bounds__(kMaxThreads) score_forward(ScoreArgs a) {
-    __shared__ Sums red[kMaxThreads / 64];
+    __shared__ BlockShared red;
     const int64_t r = blockIdx.x;
     if (a.valid && a.valid[r * a.vs] == 0.f) {
         if (threadIdx.x == 0) {
@@ -271,13 +290,13 @@ __global__ void __launch_bounds__(kMaxThreads) score_forward(ScoreArgs a) {
         return;
     }
     const T *row = (const T *)a.x + r * a.rs;
+    const int64_t label = a.target[r * a.ts];
+    const float xl = label >= 0 && label < a.width ? Elem<T>::load(row, (UNIT ? 1 : a.cs) * label)
+                                                   : __builtin_nanf("");
     const Sums mine = sum_row<T, UNIT>(a, row);
     const Sums t = merge_block(mine, red, a.inv_t);
     const double log_s = log(t.s);
     if (threadIdx.x == 0) {
-        const int64_t label = a.target[r * a.ts];
-        const float xl = label >= 0 && label < a.width ? Elem<T>::load(row, (UNIT ? 1 : a.cs) * label)
-                                                       : __builtin_nanf("");
         const float h = (float)(log_s - (double)t.u / t.s);
         a.log_probs[r] = (float)((double)(xl - t.m) * a.inv_t - log_s);
         a.entropy[r] = h;
