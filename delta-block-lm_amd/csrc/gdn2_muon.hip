@@ -27,7 +27,7 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kGroup = 32;    // matrices of one launch
-constexpr int kParts = 256;   // partial sums of a matrix's squares
+constexpr int kParts = 1024;  // partial sums of a matrix's squares, at most
 constexpr int kChunk = 32;    // columns of a 128-byte piece of a row: 32 hi, 32 lo
 constexpr int64_t kMostBytes = (int64_t)2 << 30;  // of a group's operands
 
@@ -38,8 +38,10 @@ struct Split {
     int cols;
 };
 
+__host__ __device__ __forceinline__ int64_t row_bytes(int64_t cols) { return cols * 4; }
+
 __device__ __forceinline__ char *piece_of(const Split &s, int64_t row, int col) {
-    return s.data + (row * s.cols + (col & ~(kChunk - 1))) * 4 + (col & (kChunk - 1)) * 2;
+    return s.data + row * row_bytes(s.cols) + (col & ~(kChunk - 1)) * 4 + (col & (kChunk - 1)) * 2;
 }
 
 // 8 values to the columns col .. col + 7 of a row.
@@ -78,6 +80,7 @@ struct Source {
     float beta;
     int first;      // matrix of the view that the group starts with
     int rows, cols;
+    int parts;      // of the squares
 };
 
 __device__ __forceinline__ float source_at(const Source &s, int mat, int64_t r, int64_t c) {
@@ -103,14 +106,14 @@ template <typename T> __device__ __forceinline__ void load4(const T *p, int64_t 
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? Elem<T>::load(p, i + j) : 0.f;
 }
 
-// Sums of squares in 64 bits: of a part of a dense matrix's values, or of every kParts-th row of
+// Sums of squares in 64 bits: of a part of a dense matrix's values, or of every so-manieth row of
 // another; an update's momentum first takes the gradient.
 template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squares(Source s, double *partial) {
     __shared__ double red[4];
     const int mat = blockIdx.y;
     double sum = 0;
     if (UPDATE || s.dense) {
-        const int64_t n = (int64_t)s.rows * s.cols, per = ((n + kParts - 1) / kParts + 3) & ~(int64_t)3;
+        const int64_t n = (int64_t)s.rows * s.cols, per = ((n + s.parts - 1) / s.parts + 3) & ~(int64_t)3;
         const int64_t end = min(n, (blockIdx.x + 1) * per);
         const T *x = UPDATE ? nullptr : (const T *)s.x.data + (s.first + mat) * s.x.s0;
         for (int64_t i = blockIdx.x * per + 4 * (int64_t)threadIdx.x; i < end; i += 4 * 256) {
@@ -139,7 +142,7 @@ template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squ
             for (int j = 0; j < 4; ++j) sum += (double)v[j] * v[j];
         }
     } else {
-        for (int64_t r = blockIdx.x; r < s.rows; r += kParts)
+        for (int64_t r = blockIdx.x; r < s.rows; r += s.parts)
             for (int64_t c = threadIdx.x; c < s.cols; c += 256) {
                 const double v = source_at(s, mat, r, c);
                 sum += v * v;
@@ -160,8 +163,8 @@ __global__ void __launch_bounds__(256) ns_split(Source s, const double *partial,
     const int r0 = (int)(blockIdx.x / across) * 64, c0 = (int)(blockIdx.x % across) * 64;
     by_rows.data += mat * step, by_cols.data += mat * step;
     __shared__ double red[4];
-    static_assert(kParts == 256, "one part a thread");
-    double sum = partial[mat * kParts + threadIdx.x];
+    double sum = 0;
+    for (int i = threadIdx.x; i < s.parts; i += 256) sum += partial[mat * kParts + i];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -205,23 +208,19 @@ struct GemmArgs {
     Tensors t;
 };
 
-constexpr int kComputeWaves = 4, kLoadWaves = 2, kThreads = 64 * (kComputeWaves + kLoadWaves);
-
+// Tiles of a result.  Four waves multiply, four bring the operands to LDS (two waves do not issue the
+// loads as fast as a stage is used: 4096 x 4096 takes 3 % longer).  At 128 two workgroups share a CU, one
+// multiplies while the other waits: 0.6 us a stage of each, 0.65 alone; more stages and one workgroup are
+// 5 % slower.  At 64 a stage takes 0.2 us, however many workgroups there are: the L2's rate into LDS.
 template <int T> struct Tile {
-    static constexpr int STAGE = 2 * T * 128;  // bytes
-#ifndef S128
-#define S128 3
-#endif
-#ifndef S64
-#define S64 4
-#endif
-    static constexpr int STAGES = T == 128 ? S128 : S64;
-    static constexpr int LD = T + 4;           // floats of a row of the result's tile
-    static constexpr int OPS = STAGE / 1024 / kLoadWaves;  // loads of a wave and stage
-    static constexpr int BYTES = STAGES * STAGE > T * LD * 4 ? STAGES * STAGE : T * LD * 4;
-    static constexpr int F = T / 32;           // 16-row fragments of a wave, 2 x 2 waves
+    static constexpr int WAVES = 4, LOADS = 4, THREADS = 64 * (WAVES + LOADS);
+    static constexpr int STAGE = 2 * T * 128;     // bytes: a chunk of T rows of both operands
+    static constexpr int STAGES = T == 128 ? 2 : 4;
+    static constexpr int OPS = STAGE / 1024 / LOADS;  // loads of a wave and stage
+    static constexpr int BYTES = STAGES * STAGE;
+    static constexpr int F = T / 32;              // 16-row fragments of a wave, 2 x 2 waves
     static_assert((STAGES - 1) * OPS <= 63, "loads on their way fit the memory counter");
-    static_assert(BYTES <= 160 * 1024, "LDS");
+    static_assert(BYTES >= T * T * 4 && BYTES <= 160 * 1024, "the result's tile in the stages' place");
 };
 
 constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
@@ -236,24 +235,46 @@ __device__ __forceinline__ void stage_barrier() {
 // The stored 16-byte piece of piece x of row r: rows of 128 bytes, 64 banks of 4.
 __device__ __forceinline__ int swizzle(int r, int x) { return x ^ ((r >> 1) & 7); }
 
-// Tile (i, j) of a tile index: all of them, or, for symmetric results, i <= j.
-template <bool SYM> __device__ __forceinline__ void tile_of(int t, int nj, int *i, int *j) {
-    if (!SYM) {
-        *i = t / nj, *j = t % nj;
-        return;
-    }
-    // rows of the triangle from its last: row nj - 1 - q has q + 1 tiles
-    const int n = nj * (nj + 1) / 2 - 1 - t;
-    int q = (int)((sqrtf(8.f * n + 1.f) - 1.f) * 0.5f);
-    while ((q + 1) * (q + 2) / 2 <= n) ++q;
-    while (q * (q + 1) / 2 > n) --q;
-    *i = nj - 1 - q;
-    *j = nj - 1 - (n - q * (q + 1) / 2);
+constexpr int kRowsAtOnce = 4;
+
+// Float (i, j) of a result's tile in LDS: the fours of a row are exchanged by the row, so that writes of
+// accumulators (rows 4 apart), reads along rows and reads down columns all spread over the 64 banks.
+template <int T> __device__ __forceinline__ int at_tile(int i, int j) {
+    const int q = i >> 3;
+    const int f = ((q & 1) << 2 | (q & 2) << 2 | (q & 4) >> 2 | (q & 8) >> 2) ^ ((i & 4) << 1);
+    return i * T + (j ^ (f << 2 & (T - 1)));
 }
 
-template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_product(GemmArgs p) {
+// Tile (i, j) of a tile index: all ni x nj, or, for symmetric results, those with i <= j.  Rows of
+// tiles go by kRowsAtOnce, columns inside, so that neighbours share both operands.
+template <bool SYM> __device__ __forceinline__ void tile_of(int t, int ni, int nj, int *i, int *j) {
+    constexpr int R = kRowsAtOnce;
+    if (!SYM) {
+        const int q = t / (R * nj), rows = min(R, ni - q * R), u = t - q * R * nj;
+        *i = q * R + u % rows, *j = u / rows;
+        return;
+    }
+    int q = 0;  // rows q R .. + rows: a triangle of them, then whole columns
+    for (;; ++q) {
+        const int rows = min(R, ni - q * R), n = rows * (rows + 1) / 2 + rows * (ni - q * R - rows);
+        if (t < n) {
+            const int corner = rows * (rows + 1) / 2;
+            if (t < corner) {
+                int c = 0;
+                while ((c + 1) * (c + 2) / 2 <= t) ++c;
+                *j = q * R + c, *i = q * R + t - c * (c + 1) / 2;
+            } else {
+                *i = q * R + (t - corner) % rows, *j = q * R + rows + (t - corner) / rows;
+            }
+            return;
+        }
+        t -= n;
+    }
+}
+
+template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) ns_product(GemmArgs p) {
     using C = Tile<T>;
-    constexpr int F = C::F, LD = C::LD;
+    constexpr int F = C::F, kThreads = C::THREADS;
     __shared__ __align__(1024) char lds[C::BYTES];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     // Neighbouring tiles to one XCD (workgroups go to the eight in turn).
@@ -261,29 +282,31 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
     const int at = (blockIdx.x >> 3) + x * full + min(x, more);
     const int mat = at / p.tiles;
     int ti, tj;
-    tile_of<SYM>(at % p.tiles, p.tiles_j, &ti, &tj);
+    tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
     const int I = ti * T, J = tj * T;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int stages = p.k / kChunk;
     f32x4 acc[F][F];
 
-    if (w >= kComputeWaves) {  // loads
+    if (w >= C::WAVES) {  // loads
         typedef __attribute__((address_space(1))) const void *gptr;
         typedef __attribute__((address_space(3))) void *lptr;
-        const int pw = w - kComputeWaves;
-        // operation i of this wave: rows 8 (kLoadWaves i + pw) .. + 7 of the stacked operands
+        const int pw = w - C::WAVES;
+        // An operation brings 8 rows of a chunk of the stacked operands.  Where it reads is a uniform
+        // address and one of two offsets of the lane.
+        const uint32_t row = (uint32_t)row_bytes(p.k);
+        const uint32_t lane0 = (l >> 3) * row + swizzle(l >> 3, l & 7) * 16;
+        const uint32_t lane8 = (l >> 3) * row + swizzle(8 + (l >> 3), l & 7) * 16;
+        const char *left = p.l.data + mat * p.l_step + (int64_t)I * row;
+        const char *right = p.r.data + mat * p.r_step + (int64_t)J * row;
         auto issue = [&](int s) {
             char *slot = lds + (s % C::STAGES) * C::STAGE;
 #pragma unroll
             for (int i = 0; i < C::OPS; ++i) {
-                const int r0 = 8 * (kLoadWaves * i + pw), r = r0 + (l >> 3);
-                const bool left = r0 < T;
-                const Split &o = left ? p.l : p.r;
-                const int row = left ? r : r - T;
-                const int64_t grow = (left ? I : J) + row;
-                const char *src = o.data + mat * (left ? p.l_step : p.r_step) + grow * o.cols * 4 + s * 128 +
-                                  swizzle(row, l & 7) * 16;
-                __builtin_amdgcn_global_load_lds((gptr)src, (lptr)(slot + r0 * 128), 16, 0, 0);
+                const int at = C::LOADS * i + pw, r0 = 8 * at;
+                const char *src = (r0 < T ? left + (int64_t)r0 * row : right + (int64_t)(r0 - T) * row) + s * 128;
+                __builtin_amdgcn_global_load_lds((gptr)(src + (r0 & 8 ? lane8 : lane0)), (lptr)(slot + at * 1024), 16,
+                                                 0, 0);
             }
         };
         for (int s = 0; s < C::STAGES - 1 && s < stages; ++s) issue(s);
@@ -316,19 +339,23 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
                 const int row = wi + 16 * a + n;
                 const f16x8 lh = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g) * 16);
                 const f16x8 ll = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g + 4) * 16);
+                // sums of different fragments between those of one
 #pragma unroll
-                for (int b = 0; b < F; ++b) {
+                for (int b = 0; b < F; ++b)
                     acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh[b], acc[a][b], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < F; ++b)
                     acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[b], acc[a][b], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < F; ++b)
                     acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[b], acc[a][b], 0, 0, 0);
-                }
             }
         }
     }
     // The tile through LDS, so that whole pieces are written in either orientation.
     __syncthreads();
     float *S = reinterpret_cast<float *>(lds);
-    if (w < kComputeWaves) {
+    if (w < C::WAVES) {
         const int wi = (w >> 1) * (T / 2), wj = (w & 1) * (T / 2);
 #pragma unroll
         for (int a = 0; a < F; ++a)
@@ -336,7 +363,7 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
             for (int b = 0; b < F; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    S[(wi + 16 * a + 4 * (l >> 4) + i) * LD + wj + 16 * b + (l & 15)] = acc[a][b][i] * p.scale;
+                    S[at_tile<T>(wi + 16 * a + 4 * (l >> 4) + i, wj + 16 * b + (l & 15))] = acc[a][b][i] * p.scale;
     }
     __syncthreads();
     if constexpr (MODE == LAST) {
@@ -345,7 +372,7 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
             const int a = i / T, b = i % T;
             const int64_t r = mr + a, c = mc + b;
             if (r >= p.rows || c >= p.cols) continue;
-            const float v = p.tall ? S[b * LD + a] : S[a * LD + b];
+            const float v = S[p.tall ? at_tile<T>(b, a) : at_tile<T>(a, b)];
             const int64_t o = r * p.cols + c;
             if (p.update) {
                 float *q = p.t.param[mat] + o;
@@ -367,9 +394,9 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
             load_split(A, I + a, J + b, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float u = S[a * LD + b + j] + p.b * v[j];
+                float &u = S[at_tile<T>(a, b + j)];
+                u += p.b * v[j];
                 if (I + a == J + b + j) u += p.a;
-                S[a * LD + b + j] = u;
             }
         }
         __syncthreads();
@@ -378,11 +405,11 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
         const int a = i / (T / 8), b = i % (T / 8) * 8;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = S[a * LD + b + j];
+        for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(a, b + j)];
         store_split(out, I + a, J + b, v);
         if (!SYM || ti != tj) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = S[(b + j) * LD + a];
+            for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(b + j, a)];
             store_split(out_t, J + a, I + b, v);
         }
     }
@@ -391,9 +418,9 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(kThreads) ns_produ
 // ---- host -----------------------------------------------------------------------------------------
 
 struct Plan {
-    int tile;
+    int tile[LAST + 1];
     int64_t m, n;                // padded
-    int64_t x_bytes, a_bytes;    // of one matrix: X or its transpose, A or B
+    int64_t x_bytes, xt_bytes, a_bytes;  // of one matrix: X, its transpose, A or B
     int64_t matrix_bytes;
     int group;
 };
@@ -409,24 +436,51 @@ int check_matrices(const gdn2_matrices_shape *s) {
 
 int64_t padded(int64_t n, int64_t t) { return (n + t - 1) / t * t; }
 
+// About the time of a product in us, from the figures at Tile: a CU's tiles one after another, each
+// with its stages and its result, and the launch.
+double time_of(int tile, int64_t tiles, int64_t stages) {
+    const int64_t turns = (tiles + 255) / 256;
+    if (tile == 64) return turns * (0.2 * stages + 1) + 5;
+    return turns == 1 ? 0.65 * stages + 7 : turns * (0.6 * stages + 2) + 5;
+}
+
+// Each product takes the tile that time_of prefers; sizes are padded to the larger of them.
 Plan plan_of(const gdn2_matrices_shape *s) {
     const int64_t m = s->rows < s->cols ? s->rows : s->cols, n = s->rows < s->cols ? s->cols : s->rows;
-    const int64_t ti = (m + 127) / 128;
-    Plan p;
-    const int64_t at_once = s->count < kGroup ? s->count : kGroup;
-#ifdef FORCE_TILE
-    p.tile = FORCE_TILE;
-#else
-    p.tile = m > 64 && at_once * ti * (ti + 1) / 2 >= 256 ? 128 : 64;
-#endif
-    p.m = padded(m, p.tile), p.n = padded(n, p.tile);
-    p.x_bytes = p.m * p.n * 4, p.a_bytes = p.m * p.m * 4;
-    p.matrix_bytes = 4 * p.x_bytes + 2 * p.a_bytes;
-    int64_t g = kMostBytes / p.matrix_bytes;
-    if (g > kGroup) g = kGroup;
-    if (g > s->count) g = s->count;
-    p.group = g < 1 ? 1 : (int)g;
-    return p;
+    const int64_t count = s->count < kGroup ? s->count : kGroup;
+    Plan best{};
+    double least = 0;
+    for (int pad = 64; pad <= 128; pad += 64) {
+        Plan p{};
+        p.m = padded(m, pad), p.n = padded(n, pad);
+        double total = 0;
+        for (int mode = GRAM; mode <= NEXT; ++mode) {
+            double time[2];
+            for (int i = 0; i < 2; ++i) {
+                const int64_t t = 64 << i, ti = p.m / t, tn = p.n / t;
+                time[i] = time_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
+                                  (mode == GRAM ? p.n : p.m) / kChunk);
+            }
+            const bool large = pad == 128 && time[1] < time[0];
+            p.tile[mode] = large ? 128 : 64;
+            total += time[large];
+        }
+        if (pad == 64 || total < least) best = p, least = total;
+    }
+    best.tile[LAST] = best.tile[NEXT];
+    best.x_bytes = best.m * row_bytes(best.n), best.xt_bytes = best.n * row_bytes(best.m);
+    best.a_bytes = best.m * row_bytes(best.m);
+    best.matrix_bytes = 2 * (best.x_bytes + best.xt_bytes + best.a_bytes);
+    int64_t g = kMostBytes / best.matrix_bytes;
+    if (g > count) g = count;
+    best.group = g < 1 ? 1 : (int)g;
+    return best;
+}
+
+// Parts of a matrix's squares: 4096 values each, as far as they go.
+int parts_of(const gdn2_matrices_shape *s) {
+    const int64_t n = (s->rows * s->cols + 4095) / 4096;
+    return n > kParts ? kParts : (int)n;
 }
 
 size_t workspace_of(const Plan &p) {
@@ -479,7 +533,7 @@ int check_steps(int steps, const float *k, float epsilon) {
 }
 
 template <int T> void launch_mode(Mode mode, const GemmArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)(a.tiles * a.count)), block(kThreads);
+    const dim3 grid((unsigned)(a.tiles * a.count)), block(Tile<T>::THREADS);
     switch (mode) {
         case GRAM: hipLaunchKernelGGL((ns_product<T, GRAM>), grid, block, 0, st, a); break;
         case POLY: hipLaunchKernelGGL((ns_product<T, POLY>), grid, block, 0, st, a); break;
@@ -496,19 +550,18 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
     // of the first matrix; the others follow at matrix_bytes
     Split X[2], XT[2];
     for (int i = 0; i < 2; ++i) {
-        X[i] = {ws + 2 * i * p.x_bytes, (int)p.n};
-        XT[i] = {ws + (2 * i + 1) * p.x_bytes, (int)p.m};
+        X[i] = {ws + i * (p.x_bytes + p.xt_bytes), (int)p.n};
+        XT[i] = {X[i].data + p.x_bytes, (int)p.m};
     }
-    const Split A = {ws + 4 * p.x_bytes, (int)p.m}, B = {ws + 4 * p.x_bytes + p.a_bytes, (int)p.m};
+    const Split A = {ws + 2 * (p.x_bytes + p.xt_bytes), (int)p.m}, B = {A.data + p.a_bytes, (int)p.m};
     double s = 1, sx = power_for(s);
-    const dim3 parts(kParts, count), threads(256);
+    const dim3 parts(src.parts, count), threads(256);
     if (src.update) hipLaunchKernelGGL((ns_squares<float, true>), parts, threads, 0, st, src, partial);
     else if (src.bf16) hipLaunchKernelGGL((ns_squares<bf16_t, false>), parts, threads, 0, st, src, partial);
     else hipLaunchKernelGGL((ns_squares<float, false>), parts, threads, 0, st, src, partial);
     const int64_t pr = tall ? p.n : p.m, pc = tall ? p.m : p.n;
     hipLaunchKernelGGL(ns_split, dim3((unsigned)(pr / 64 * (pc / 64)), count), dim3(256), 0, st, src,
                        partial, (double)epsilon, sx, tall ? XT[0] : X[0], tall ? X[0] : XT[0], p.matrix_bytes);
-    const int ti = (int)(p.m / p.tile), tn = (int)(p.n / p.tile);
     for (int i = 0; i < steps; ++i) {
         const Split &x = X[i & 1], &xt = XT[i & 1];
         const Bounds b = bounds_of(k, s);
@@ -517,18 +570,20 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
         g.count = count;
         g.l_step = g.r_step = g.out_step = p.matrix_bytes;
         auto run = [&](Mode mode) {
-            if (p.tile == 128) launch_mode<128>(mode, g, st);
+            const int t = p.tile[mode], ti = (int)(p.m / t), tn = (int)(p.n / t);
+            g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
+            g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
+            if (t == 128) launch_mode<128>(mode, g, st);
             else launch_mode<64>(mode, g, st);
         };
         g.l = g.r = x, g.out = A;
-        g.tiles_i = g.tiles_j = ti, g.tiles = ti * (ti + 1) / 2, g.k = (int)p.n;
+        g.k = (int)p.n;
         g.scale = (float)(sa / (sx * sx));
         run(GRAM);
         g.l = g.r = A, g.out = B, g.k = (int)p.m;
         g.scale = (float)(k[2] * sb / (sa * sa)), g.a = (float)(k[0] * sb), g.b = (float)(k[1] * sb / sa);
         run(POLY);
         g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
-        g.tiles_j = tn, g.tiles = ti * tn;
         const double to = i + 1 < steps ? power_for(next) : 1;
         g.scale = (float)(to / (sb * sx));
         run(i + 1 < steps ? NEXT : LAST);
@@ -571,6 +626,7 @@ int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, voi
     GemmArgs last{};
     last.rows = s.rows, last.cols = s.cols, last.tall = s.rows > s.cols, last.bf16 = s.bf16;
     last.result = result;
+    s.parts = parts_of(shape);
     for (int64_t i = 0; i < shape->count; i += p.group) {
         s.first = last.first = (int)i;
         const int64_t left = shape->count - i;
@@ -598,6 +654,7 @@ int gdn2_muon_update(const gdn2_matrices_shape *shape, const gdn2_muon_tensor *t
     GemmArgs last{};
     last.rows = s.rows, last.cols = s.cols, last.tall = s.rows > s.cols, last.update = 1;
     last.decay = 1.f - lr * decay;
+    s.parts = parts_of(shape);
     last.rate = lr * sqrtf(s.rows > s.cols ? (float)s.rows / (float)s.cols : 1.f);
     for (int64_t i = 0; i < shape->count; i += p.group) {
         const int64_t left = shape->count - i;
