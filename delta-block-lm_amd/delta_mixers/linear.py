@@ -182,6 +182,12 @@ class LinearLM(torch.nn.Module):
                                        self.embed.to(self.cfg.compute_dtype),
                                        tokens[:, 1:].reshape(-1))
 
+    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0) -> dk.TokenLogProbs:
+        """Log probabilities of tokens 1 .. T - 1 after those before them, [B, T - 1], their entropy and
+        the top alternatives; zeros where valid [B, T] is 0."""
+        return dk.token_log_probs(self(tokens[:, :-1]), tokens[:, 1:], top,
+                                  None if valid is None else valid[:, 1:], temperature)
+
     @torch.no_grad()
     def prefill(self, tokens, states=None):
         """A prompt, or its continuation: (logits of the last token [B, vocab], states)."""

@@ -301,6 +301,12 @@ class GdnLM(torch.nn.Module):
         return dk.linear_cross_entropy(h.reshape(-1, self.cfg.d_model), self.embed.to(cd),
                                        tokens[:, 1:].reshape(-1))
 
+    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0) -> dk.TokenLogProbs:
+        """Log probabilities of tokens 1 .. T - 1 after those before them, [B, T - 1], their entropy and
+        the top alternatives; zeros where valid [B, T] is 0.  The reference's models give the loss alone."""
+        return dk.token_log_probs(self(tokens[:, :-1]), tokens[:, 1:], top,
+                                  None if valid is None else valid[:, 1:], temperature)
+
 
 def make_optimizer(model: GdnLM, lr: float = 1e-3, weight_decay: float = 0.01,
                    clip: float = 1.0):
