@@ -6,10 +6,12 @@
 //
 // A run of tokens acts on the state before it as S + A h, and joining two runs needs only their
 // (A, S): the time axis is split over lanes, waves, and, where there are few channels, workgroups.
-//   * A workgroup has 128 bytes of channels (64 bf16, 32 f32: one memory line of a token) and up to
-//     8 waves; a lane has one 16-byte piece of kL tokens in a row, a wave 8 such runs for each of
-//     its 8 pieces, a block is what all waves hold.  Every tensor is read and written once, in
-//     lines, and the next block's loads are on their way while a block is worked on.
+//   * A workgroup has 64 bytes of channels (32 bf16, 16 f32) and up to 8 waves; the two that share a
+//     128-byte line go to one XCD, whose L2 reads it once (halves rather than lines: twice the
+//     workgroups, 306 us against 443 at 4 x 8192 tokens of 2048 channels, where lines have 128).  A lane
+//     has 8 bytes of channels of some tokens in a row, a wave 8 such runs for each of its 8 pieces, a
+//     block is what all waves hold.  Every tensor is read and written once, the next block's loads are on
+//     their way while a block is worked on.
 //   * Inside a block: each lane its own run, the 8 runs of a wave by lane exchanges, the waves
 //     through LDS (one barrier a block); then each lane walks its run again from its true state.
 //   * Segments: if there are too few workgroups the blocks of a sequence go to several.  A first
@@ -17,6 +19,10 @@
 //     the inputs are read twice, by kernels that fill the card.
 // The backward recomputes the states of a block from the state before it, which the forward kept
 // (4 bytes a channel for every block), and walks the blocks from the last.
+//
+// 4 x 8192 tokens of 2048 channels, bf16: forward 120 us, 3.4 TB/s, backward 197.  A block takes 25
+// instructions a value, 10 of them the recurrence's own, at two waves a SIMD that wait for each other once
+// a block: 46 % of the time the vector units work.
 //
 // A is carried as half its log2 and its root applied twice, clamped to [2^-126, 2^127]: a state of
 // any size meets a decay of any size as it would token by token, zero stays zero, and what is not
@@ -26,21 +32,34 @@
 // what is not finite does not pass.
 #include <math.h>
 
+#include <type_traits>
+
 #include "gdn2_common.h"
 #include "gdn2_status.h"
+
+// Sums of products are fused where it says fmaf and nowhere else: a wave that takes the way for gates that
+// need care gives the bits that it would give without them.
+#pragma clang fp contract(off)
 
 namespace gdn2 {
 namespace {
 
-constexpr int kL = 4;         // tokens of a lane's run
-constexpr int kPieces = 8;    // 16-byte pieces of channels in a workgroup
-constexpr int kRuns = 8;      // runs of a wave: 64 / kPieces
 constexpr int kMaxWaves = 8;
+constexpr int kSlabBytes = 64;  // of a token, a workgroup's channels
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNothing = -INFINITY;
 constexpr float kTiny = 0x1p-126f, kHuge = 0x1p127f;
 
-template <typename T> constexpr int kN = 16 / sizeof(T);  // channels of a piece
+// A lane has 8 bytes of 8 tokens in bf16, of 4 in f32: with runs twice as long registers run out, with
+// half as many tokens a block's joining is half of its instructions (4 x 8192 tokens of 2048 channels,
+// bf16, forward and backward: 306 us, with runs of 4 tokens 362, with 4-byte pieces of 16 tokens 321).
+template <typename T> struct Cfg {
+    static constexpr int N = 8 / sizeof(T);               // channels of a lane
+    static constexpr int L = sizeof(T) == 2 ? 8 : 4;      // tokens of a lane's run
+    static constexpr int SLAB = kSlabBytes / sizeof(T);   // channels of a workgroup
+    static constexpr int PIECES = SLAB / N, RUNS = 64 / PIECES;
+    static constexpr int TOKENS = RUNS * L;               // of a wave
+};
 
 struct RecArgs {
     View x, g, dy;         // [batch, time, channel]
@@ -68,86 +87,59 @@ template <typename T, int N> __device__ __forceinline__ float get(const Piece<T,
     else return j & 1 ? __uint_as_float(p.w[j >> 1] & 0xFFFF0000u) : __uint_as_float(p.w[j >> 1] << 16);
 }
 
-// The first n <= N channels at p, zeros behind them.  UNIT: the channels lie side by side, at any
-// address that the type may have.
-template <typename T, int N, bool UNIT>
-__device__ __forceinline__ void load_piece(Piece<T, N> &r, const T *p, int64_t cs, int n) {
-    if (UNIT && n == N) {
-        __builtin_memcpy(&r, p, sizeof(r));
-        return;
+template <typename T, int N> __device__ __forceinline__ void set(Piece<T, N> &p, const float *v) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) p.w[j] = __float_as_uint(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 2)
+            p.w[j >> 1] = (uint32_t)f32_to_bf16(v[j]) | ((uint32_t)f32_to_bf16(v[j + 1]) << 16);
     }
-#pragma unroll
-    for (int i = 0; i < (int)(N * sizeof(T) / 4); ++i) r.w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        if (j < n) {
-            const T v = p[(UNIT ? 1 : cs) * j];
-            if constexpr (sizeof(T) == 4) r.w[j] = __float_as_uint(v);
-            else r.w[j >> 1] |= (uint32_t)v << (16 * (j & 1));
-        }
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store_piece(T *p, const float *v, int n) {
-    if (n == N) {
-        Piece<T, N> r;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) r.w[j] = __float_as_uint(v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; j += 2)
-                r.w[j >> 1] = (uint32_t)f32_to_bf16(v[j]) | ((uint32_t)f32_to_bf16(v[j + 1]) << 16);
-        }
-        __builtin_memcpy(p, &r, sizeof(r));
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        if (j < n) Elem<T>::store(p, j, v[j]);
 }
 
 // ---- joining runs ----------------------------------------------------------------------
 
-// The decay of one token: 0 below 2^-126, at most 2^127; log2g is cut to what it uses.
-__device__ __forceinline__ float decay_of(float &log2g) {
-    log2g = log2g > 127.f ? 127.f : log2g;  // NaN stays
-    const float a = __builtin_amdgcn_exp2f(log2g);
-    return log2g < -126.f ? 0.f : a;
+__device__ __forceinline__ float root_of(float half) {
+    return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(half), kTiny, kHuge);
 }
 
-__device__ __forceinline__ float through(float a, float h) { return a == 0.f ? 0.f : a * h; }
-
-// What a run (half the log2 of its decay, -inf if it lets nothing through, and its sum) makes of the
-// state before it.
-__device__ __forceinline__ float join(float before, float half, float sum) {
-    const float r = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(half), kTiny, kHuge);
-    const float t = (before * r) * r;
-    return (half == kNothing ? 0.f : t) + sum;
+// What a run (the root of its decay, 0 if it lets nothing through, and its sum) makes of the state
+// before it.
+__device__ __forceinline__ float join_root(float before, float r, float sum) {
+    const float t = fmaf(before * r, r, sum);
+    return r == 0.f ? sum : t;
 }
 
-// v of the lane D lanes before (UP) or behind this one, id where there is none.
-template <int D, bool UP> __device__ __forceinline__ float shifted(float v, float id) {
+// The same by half the log2 of the decay, kNothing for 0.  CUT: there may be such runs.
+template <bool CUT> __device__ __forceinline__ float join(float before, float half, float sum) {
+    const float r = root_of(half), t = fmaf(before * r, r, sum);
+    return CUT && half == kNothing ? sum : t;
+}
+
+// v of the lane D lanes before (UP) or behind this one, 0 where there is none.
+template <int D, bool UP> __device__ __forceinline__ float shifted(float v) {
     const float w = UP ? __shfl_up(v, D) : __shfl_down(v, D);
     const int l = threadIdx.x & 63;
-    return (UP ? l >= D : l < 64 - D) ? w : id;
+    return (UP ? l >= D : l < 64 - D) ? w : 0.f;
 }
 
-template <int N, int D, bool UP> __device__ __forceinline__ void scan_level(float *l, float *s) {
+template <int N, int D, bool UP, bool CUT> __device__ __forceinline__ void scan_level(float *l, float *s) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const float l1 = shifted<D, UP>(l[j], 0.f), s1 = shifted<D, UP>(s[j], 0.f);
-        s[j] = join(s1, l[j], s[j]);
+        const float l1 = shifted<D, UP>(l[j]), s1 = shifted<D, UP>(s[j]);
+        s[j] = join<CUT>(s1, l[j], s[j]);
         l[j] += l1;
     }
 }
 
 // Runs of a wave: on return l, s of everything up to and with this lane's run (from the first run
 // on, or, with UP false, from the last one backwards).
-template <int N, bool UP> __device__ __forceinline__ void scan_runs(float *l, float *s) {
-    scan_level<N, 8, UP>(l, s);
-    scan_level<N, 16, UP>(l, s);
-    scan_level<N, 32, UP>(l, s);
+template <typename C, bool UP, bool CUT> __device__ __forceinline__ void scan_runs(float *l, float *s) {
+    if constexpr (C::PIECES <= 4) scan_level<C::N, 4, UP, CUT>(l, s);
+    if constexpr (C::PIECES <= 8) scan_level<C::N, 8, UP, CUT>(l, s);
+    if constexpr (C::PIECES <= 16) scan_level<C::N, 16, UP, CUT>(l, s);
+    if constexpr (C::PIECES <= 32) scan_level<C::N, 32, UP, CUT>(l, s);
 }
 
 // ---- a lane's run ----------------------------------------------------------------------
@@ -155,308 +147,476 @@ template <int N, bool UP> __device__ __forceinline__ void scan_runs(float *l, fl
 struct Place {
     int lane, wave, piece, run;
     int b, seg;
-    int c0, n;   // this lane's channels: c0 .. c0 + n
-    int c;       // the channel that this lane carries across waves and blocks
-    bool owns;   // whether it has one
+    int slab0, c0;  // the slab's channels, and this lane's
+    int own0;    // the first channel that this workgroup answers for
+    int ch, c;   // the channel of the slab, and its number, that this lane carries across waves and blocks
+    bool there;  // whether there is one; lanes beyond the slab's channels carry the same ones again
+    bool owns;   // whether this lane answers for it
 };
 
-template <typename T> __device__ __forceinline__ Place place(const RecArgs &a) {
-    constexpr int N = kN<T>, SLAB = N * kPieces;
+// WHOLE: a slab that would reach past the last channel begins earlier; what it shares with the slab
+// before it is that one's.
+template <typename C, bool WHOLE> __device__ __forceinline__ Place place(const RecArgs &a) {
     Place p;
     p.lane = threadIdx.x & 63;
     p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    p.piece = p.lane & (kPieces - 1);
-    p.run = p.lane / kPieces;
-    const unsigned u = blockIdx.x;
+    p.piece = p.lane & (C::PIECES - 1);
+    p.run = p.lane / C::PIECES;
+    // Slabs that share 128-byte lines to one XCD: workgroups go to the eight in turn.
+    constexpr unsigned G = 128 / kSlabBytes;
+    unsigned u = blockIdx.x;
+    if (G > 1 && u < gridDim.x / (8 * G) * (8 * G)) {
+        const unsigned q = u / (8 * G), r = u % (8 * G);
+        u = (q * 8 + r % 8) * G + r / 8;
+    }
     const int slab = u % (unsigned)a.slabs;
     const unsigned rest = u / (unsigned)a.slabs;
     p.b = rest % (unsigned)a.B;
     p.seg = rest / (unsigned)a.B;
-    p.c0 = slab * SLAB + p.piece * N;
-    p.n = min(max(a.W - p.c0, 0), N);
-    p.c = slab * SLAB + (p.lane & (SLAB - 1));
-    p.owns = p.lane < SLAB && p.c < a.W;
+    p.own0 = slab * C::SLAB;
+    p.slab0 = WHOLE ? min(p.own0, a.W - C::SLAB) : p.own0;
+    p.c0 = p.slab0 + p.piece * C::N;
+    p.ch = p.lane & (C::SLAB - 1);
+    p.c = p.slab0 + p.ch;
+    p.there = p.c < a.W;
+    p.owns = p.lane < C::SLAB && p.c >= p.own0 && p.there;
     return p;
 }
 
-template <typename T, int N, bool UNIT>
+// kL tokens of this lane's channels from token t on, t = wave's first token + run kL.  What lies behind
+// the last token or channel is read as the last: a lane with such tokens leaves them out, and one with
+// such channels writes none.  WHOLE: side by side and near, by a uniform address and a lane's offset.
+template <bool WHOLE, typename T, int N, int kL>
 __device__ __forceinline__ void load_run(Piece<T, N> (&r)[kL], const View &v, const RecArgs &a,
-                                         const Place &p, int64_t t) {
-    const T *q = (const T *)v.data + p.b * v.s0 + t * v.s1 + (UNIT ? (int64_t)p.c0 : p.c0 * v.s2);
+                                         const Place &p, int64_t first, bool inside) {
+    const T *q = (const T *)v.data + p.b * v.s0;
+    if (WHOLE) {
+        const int64_t from = min(first, a.T - 1);
+        const char *base = (const char *)(q + from * v.s1 + p.slab0);
+        const uint32_t row = (uint32_t)v.s1 * sizeof(T), piece = p.piece * (N * sizeof(T));
+        if (inside) {
+            const uint32_t off = p.run * kL * row + piece;
 #pragma unroll
-    for (int i = 0; i < kL; ++i)
-        load_piece<T, N, UNIT>(r[i], q + i * v.s1, v.s2, t + i < a.T ? p.n : 0);
-}
-
-struct Masks {
-    bool on[kL], cut[kL];
-};
-
-__device__ __forceinline__ Masks load_masks(const RecArgs &a, const Place &p, int64_t t) {
-    Masks m;
+            for (int i = 0; i < kL; ++i) __builtin_memcpy(&r[i], base + (int64_t)i * row + off, sizeof(r[i]));
+        } else {
+            const int most = (int)min(a.T - 1 - from, (int64_t)(64 * kL));
+#pragma unroll
+            for (int i = 0; i < kL; ++i) {
+                const uint32_t off = (uint32_t)min(p.run * kL + i, most) * row + piece;
+                __builtin_memcpy(&r[i], base + off, sizeof(r[i]));
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kL; ++i) {
-        m.on[i] = t + i < a.T;
-        m.cut[i] = false;
-        if (m.on[i] && a.valid.data)
-            m.on[i] = ((const float *)a.valid.data)[p.b * a.valid.s0 + (t + i) * a.valid.s1] != 0.f;
-        if (m.on[i] && a.reset.data)
-            m.cut[i] = ((const float *)a.reset.data)[p.b * a.reset.s0 + (t + i) * a.reset.s1] != 0.f;
+        const T *row = q + min(first + p.run * kL + i, a.T - 1) * v.s1;
+#pragma unroll
+        for (int k = 0; k < (int)(N * sizeof(T) / 4); ++k) r[i].w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const T e = row[min(p.c0 + j, a.W - 1) * v.s2];
+            if constexpr (sizeof(T) == 4) r[i].w[j] = __float_as_uint(e);
+            else r[i].w[j >> 1] |= (uint32_t)e << (16 * (j & 1));
+        }
+    }
+}
+
+// Token first + run L + i of a dense result.
+template <bool WHOLE, int L, typename T, int N>
+__device__ __forceinline__ void store_piece(void *out, const RecArgs &a, const Place &p, int64_t first, int i,
+                                            const float *v) {
+    if (WHOLE) {
+        char *base = (char *)((T *)out + (p.b * a.T + first + i) * a.W + p.slab0);
+        T *q = (T *)(base + (uint32_t)((p.run * L * a.W + p.piece * N) * (int)sizeof(T)));
+        if (p.slab0 == p.own0 || p.c0 >= p.own0) {
+            Piece<T, N> r;
+            set(r, v);
+            __builtin_memcpy(q, &r, sizeof(r));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (p.c0 + j >= p.own0) Elem<T>::store(q, j, v[j]);
+        }
+        return;
+    }
+    T *q = (T *)out + (p.b * a.T + first + p.run * L + i) * a.W + p.c0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (p.c0 + j < a.W) Elem<T>::store(q, j, v[j]);
+}
+
+// Bit i: token i of the run counts, and it is a reset.
+struct Masks {
+    uint32_t on, cut;
+};
+
+template <int kL> __device__ __forceinline__ Masks load_masks(const RecArgs &a, const Place &p, int64_t first) {
+    const int64_t t = first + p.run * kL;
+    Masks m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kL; ++i) {
+        const int64_t at = min(t + i, a.T - 1);
+        bool on = t + i < a.T, cut = false;
+        if (a.valid.data) on = on && ((const float *)a.valid.data)[p.b * a.valid.s0 + at * a.valid.s1] != 0.f;
+        if (a.reset.data) cut = ((const float *)a.reset.data)[p.b * a.reset.s0 + at * a.reset.s1] != 0.f;
+        m.on |= (uint32_t)on << i, m.cut |= (uint32_t)(on && cut) << i;
     }
     return m;
 }
 
 // Decays of a run, and half the log2 of their product: finite, or kNothing.  A gate that is NaN
-// counts as 0 there: the sums that it touches are NaN themselves.
-template <typename G, int N>
-__device__ __forceinline__ void decays(const Piece<G, N> (&g)[kL], const Masks &m, float (&a)[kL][N],
+// counts as 0 there: the sums that it touches are NaN themselves.  True if a wave's decays need no
+// care: all tokens count, all gates are numbers, between 2^-126 and 2^127.
+template <bool MASKED, typename G, int N, int kL>
+__device__ __forceinline__ bool decays(const Piece<G, N> (&g)[kL], const Masks &m, float (&d)[kL][N],
                                        float (&half)[N]) {
+    float lo = 0.f, hi = 0.f, all = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        half[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kL; ++i) {
+            const float l = get(g[i], j) * kLog2e;
+            d[i][j] = l;
+            half[j] += l;
+            lo = fminf(lo, l), hi = fmaxf(hi, l);
+        }
+        all += half[j];
+        half[j] *= 0.5f;
+    }
+    const bool care = !(lo >= -126.f && hi <= 127.f && all == all) ||
+                      (MASKED && ((m.on & ((1u << kL) - 1)) != (1u << kL) - 1 || m.cut));
+    if (!__any(care)) {
+#pragma unroll
+        for (int i = 0; i < kL; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) d[i][j] = __builtin_amdgcn_exp2f(d[i][j]);
+        return true;
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         float sum = 0.f;
         bool cut = false;
 #pragma unroll
         for (int i = 0; i < kL; ++i) {
-            float l = get(g[i], j) * kLog2e;
-            float d = decay_of(l);
-            d = m.cut[i] ? 0.f : d;
-            d = m.on[i] ? d : 1.f;
-            l = m.on[i] ? l : 0.f;
-            sum += l;
-            cut = cut || d == 0.f;
-            a[i][j] = d;
+            float l = d[i][j];
+            l = l > 127.f ? 127.f : l;  // NaN stays
+            float v = l < -126.f || (m.cut >> i & 1) ? 0.f : __builtin_amdgcn_exp2f(l);
+            const bool on = m.on >> i & 1;
+            d[i][j] = v = on ? v : 1.f;
+            sum += on ? l : 0.f;
+            cut = cut || v == 0.f;
         }
         half[j] = cut ? kNothing : sum == sum ? 0.5f * sum : 0.f;
     }
+    return false;
 }
 
-// The start state of a segment, in the lanes that own a channel.
+// d h + x, or x where nothing gets through.
+template <bool PLAIN> __device__ __forceinline__ float next_state(float d, float h, float x) {
+    const float t = fmaf(d, h, x);
+    return !PLAIN && d == 0.f ? x : t;
+}
+
+template <bool PLAIN> __device__ __forceinline__ float through(float d, float h) {
+    return !PLAIN && d == 0.f ? 0.f : d * h;
+}
+
+// Value j of token i, 0 if the token does not count.
+template <bool PLAIN, typename T, int N, int kL>
+__device__ __forceinline__ float value(const Piece<T, N> (&x)[kL], const Masks &m, int i, int j) {
+    return PLAIN || (m.on >> i & 1) ? get(x[i], j) : 0.f;
+}
+
+// The start state of a segment.
 __device__ __forceinline__ float start_of(const RecArgs &a, const Place &p, float first, int from,
                                           int to, int step) {
     const int64_t BW = (int64_t)a.B * a.W;
     const int64_t at = (int64_t)p.b * a.W + p.c;
     float st = first;
     for (int s = from; s != to; s += step)
-        st = join(st, a.seg_half[s * BW + at], a.seg_sum[s * BW + at]);
+        st = join<true>(st, a.seg_half[s * BW + at], a.seg_sum[s * BW + at]);
     return st;
 }
 
+// What the waves tell each other of a block, twice: a wave that is a block ahead writes the other half.
+// Waves that the workgroup does not have let everything through and add nothing.
+template <typename C> struct Totals {
+    float half[2][kMaxWaves][C::SLAB], root[2][kMaxWaves][C::SLAB], sum[2][kMaxWaves][C::SLAB];
+    float in[kMaxWaves][C::SLAB];  // the state before each wave's tokens
+
+    __device__ __forceinline__ void clear() {
+        for (int i = threadIdx.x; i < 2 * kMaxWaves * C::SLAB; i += blockDim.x)
+            (&half[0][0][0])[i] = 0.f, (&root[0][0][0])[i] = 1.f, (&sum[0][0][0])[i] = 0.f;
+    }
+    __device__ __forceinline__ void put(int buf, const Place &p, const float *l, const float *s) {
+#pragma unroll
+        for (int j = 0; j < C::N; ++j) {
+            const int c = p.piece * C::N + j;
+            half[buf][p.wave][c] = l[j];
+            root[buf][p.wave][c] = l[j] == kNothing ? 0.f : root_of(l[j]);
+            sum[buf][p.wave][c] = s[j];
+        }
+    }
+    // This lane's channel: the state before its wave's tokens to `in`, and past all waves.  UP: waves in
+    // order, or from the last.  A state goes past a block in one step, by the sum of all logarithms.
+    template <bool UP> __device__ __forceinline__ float pass(int buf, const Place &p, float state, float *all_out) {
+        float r[kMaxWaves], s[kMaxWaves], all = 0.f, total = 0.f, mine = state;
+#pragma unroll
+        for (int k = 0; k < kMaxWaves; ++k) {
+            const int w = UP ? k : kMaxWaves - 1 - k;
+            r[k] = root[buf][w][p.ch], s[k] = sum[buf][w][p.ch], all += half[buf][w][p.ch];
+        }
+#pragma unroll
+        for (int k = 0; k < kMaxWaves; ++k) {
+            const int w = UP ? k : kMaxWaves - 1 - k;
+            const float before = mine;
+            mine = join_root(mine, r[k], s[k]);
+            if (w == p.wave) in[p.wave][p.ch] = before;
+            total = join_root(total, r[k], s[k]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        *all_out = all;
+        return join<true>(state, all, total);
+    }
+};
+
 // ---- forward -----------------------------------------------------------------------------
 
-// CARRY: only the segment's (A, S).
-template <typename T, typename G, bool UNIT, bool CARRY>
-__global__ void __launch_bounds__(64 * kMaxWaves) rec_forward(RecArgs a) {
-    constexpr int N = kN<T>, SLAB = N * kPieces;
-    __shared__ __align__(16) float tot_l[2][kMaxWaves][SLAB], tot_s[2][kMaxWaves][SLAB];
-    __shared__ __align__(16) float in[kMaxWaves][SLAB];
-    const Place p = place<T>(a);
-    const int BT = a.waves * kRuns * kL;
-    const int first = p.seg * a.seg_blocks, last = min(first + a.seg_blocks, a.blocks);
-    const int64_t BW = (int64_t)a.B * a.W, at = (int64_t)p.b * a.W + p.c;
-    const int ch = p.lane & (SLAB - 1);
-    if (CARRY && last == a.blocks) return;  // nothing comes after it
-
-    float state = 0.f, half = 0.f;  // of channel p.c, before the block
-    if (!CARRY && p.owns) {
-        if (a.initial.data)
-            state = ((const float *)a.initial.data)[p.b * a.initial.s0 + p.c * a.initial.s1];
-        state = start_of(a, p, state, 0, p.seg, 1);
-    }
-    int64_t t = (int64_t)first * BT + (p.wave * kRuns + p.run) * kL;
-    Piece<T, N> x[kL], xn[kL];
-    Piece<G, N> g[kL], gn[kL];
-    load_run<T, N, UNIT>(x, a.x, a, p, t);
-    load_run<G, N, UNIT>(g, a.g, a, p, t);
-    for (int blk = first; blk < last; ++blk, t += BT) {
-        const int buf = blk & 1;
-        const Masks m = load_masks(a, p, t);
-        if (blk + 1 < last) {
-            load_run<T, N, UNIT>(xn, a.x, a, p, t + BT);
-            load_run<G, N, UNIT>(gn, a.g, a, p, t + BT);
-        }
-        float d[kL][N], l[N], s[N];
-        decays(g, m, d, l);
+// A block: the runs' sums, what passes from wave to wave, and the states.
+template <typename T, typename G, bool WHOLE, bool CARRY, bool MASKED, typename C>
+__device__ __forceinline__ void forward_block(const RecArgs &a, const Place &p, Totals<C> &tot, int buf, int64_t t,
+                                              const Piece<T, C::N> (&x)[C::L], const Piece<G, C::N> (&g)[C::L],
+                                              const Masks &m, float &state, float &half) {
+    constexpr int N = C::N, L = C::L;
+    float d[L][N], l[N], s[N];
+    const bool plain = decays<MASKED>(g, m, d, l);
+    auto sums = [&](auto flag) {
+        constexpr bool PLAIN = decltype(flag)::value;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             float h = 0.f;
 #pragma unroll
-            for (int i = 0; i < kL; ++i) h = through(d[i][j], h) + (m.on[i] ? get(x[i], j) : 0.f);
+            for (int i = 0; i < L; ++i) h = next_state<PLAIN>(d[i][j], h, value<PLAIN>(x, m, i, j));
             s[j] = h;
         }
-        scan_runs<N, true>(l, s);
-        if (p.run == kRuns - 1) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                tot_l[buf][p.wave][p.piece * N + j] = l[j];
-                tot_s[buf][p.wave][p.piece * N + j] = s[j];
-            }
-        }
-        __syncthreads();
-        if (!CARRY && a.states && p.wave == 0 && p.owns) a.states[blk * BW + at] = state;
-        // The state goes past a block in one step, by the sum of all logarithms.
-        float mine = state, all = 0.f, sum = 0.f;
-        for (int w = 0; w < a.waves; ++w) {
-            const float lw = tot_l[buf][w][ch], sw = tot_s[buf][w][ch];
-            if (!CARRY && w < p.wave) mine = join(mine, lw, sw);
-            sum = join(sum, lw, sw);
-            all += lw;
-        }
-        state = join(state, all, sum);
-        if (CARRY) half += all;
-        if (!CARRY) {
-            if (p.lane < SLAB) in[p.wave][p.lane] = mine;
-            __builtin_amdgcn_wave_barrier();
-            // the runs before this lane's in its wave
-            float h[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float lb = shifted<8, true>(l[j], 0.f), sb = shifted<8, true>(s[j], 0.f);
-                h[j] = join(in[p.wave][p.piece * N + j], lb, sb);
-            }
-            T *y = (T *)a.y + (p.b * a.T + t) * a.W + p.c0;
-#pragma unroll
-            for (int i = 0; i < kL; ++i) {
-                float o[N];
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    h[j] = through(d[i][j], h[j]) + (m.on[i] ? get(x[i], j) : 0.f);
-                    o[j] = m.on[i] ? h[j] : 0.f;
-                }
-                if (t + i < a.T) store_piece<T, N>(y + (int64_t)i * a.W, o, p.n);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kL; ++i) x[i] = xn[i], g[i] = gn[i];
-    }
+        scan_runs<C, true, !PLAIN>(l, s);
+    };
+    if (plain) sums(std::true_type{});
+    else sums(std::false_type{});
+    if (p.run == C::RUNS - 1) tot.put(buf, p, l, s);
+    __syncthreads();
+    float all;
+    state = tot.template pass<true>(buf, p, state, &all);
     if (CARRY) {
-        if (p.wave == 0 && p.owns) {
-            a.seg_half[p.seg * BW + at] = half;
-            a.seg_sum[p.seg * BW + at] = state;
+        half += all;
+        return;
+    }
+    auto states = [&](auto flag) {
+        constexpr bool PLAIN = decltype(flag)::value;
+        float h[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j)  // past the runs before this lane's in its wave
+            h[j] = join<!PLAIN>(tot.in[p.wave][p.piece * N + j], shifted<C::PIECES, true>(l[j]),
+                                shifted<C::PIECES, true>(s[j]));
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            float o[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                h[j] = next_state<PLAIN>(d[i][j], h[j], value<PLAIN>(x, m, i, j));
+                o[j] = PLAIN || (m.on >> i & 1) ? h[j] : 0.f;
+            }
+            if (!MASKED || t + p.run * L + i < a.T) store_piece<WHOLE, L, T, N>(a.y, a, p, t, i, o);
         }
-    } else if (p.wave == 0 && p.owns && last == a.blocks) {
+    };
+    if (plain) states(std::true_type{});
+    else states(std::false_type{});
+}
+
+template <typename T, typename G, bool WHOLE, bool CARRY, typename C>
+__device__ __forceinline__ void forward_walk(const RecArgs &a, const Place &p, Totals<C> &tot) {
+    constexpr int N = C::N, L = C::L;
+    const int BT = a.waves * C::TOKENS;
+    const int first = p.seg * a.seg_blocks, last = min(first + a.seg_blocks, a.blocks);
+    const int64_t BW = (int64_t)a.B * a.W, at = (int64_t)p.b * a.W + p.c;
+    const bool masks = a.valid.data || a.reset.data;
+    float state = 0.f, half = 0.f;  // of channel p.c, before the block
+    if (!CARRY && p.there) {
+        if (a.initial.data)
+            state = ((const float *)a.initial.data)[p.b * a.initial.s0 + p.c * a.initial.s1];
+        state = start_of(a, p, state, 0, p.seg, 1);
+    }
+    int64_t t = (int64_t)first * BT + p.wave * C::TOKENS;  // this wave's first token
+    auto inside = [&](int blk) { return (int64_t)(blk + 1) * BT <= a.T; };
+    Piece<T, N> x[L], xn[L];
+    Piece<G, N> g[L], gn[L];
+    load_run<WHOLE>(x, a.x, a, p, t, inside(first));
+    load_run<WHOLE>(g, a.g, a, p, t, inside(first));
+    for (int blk = first; blk < last; ++blk, t += BT) {
+        if (blk + 1 < last) {
+            load_run<WHOLE>(xn, a.x, a, p, t + BT, inside(blk + 1));
+            load_run<WHOLE>(gn, a.g, a, p, t + BT, inside(blk + 1));
+        }
+        if (!CARRY && a.states && p.wave == 0 && p.owns) a.states[blk * BW + at] = state;
+        if (masks || !inside(blk))
+            forward_block<T, G, WHOLE, CARRY, true>(a, p, tot, blk & 1, t, x, g, load_masks<L>(a, p, t), state, half);
+        else
+            forward_block<T, G, WHOLE, CARRY, false>(a, p, tot, blk & 1, t, x, g, Masks{~0u, 0}, state, half);
+#pragma unroll
+        for (int i = 0; i < L; ++i) x[i] = xn[i], g[i] = gn[i];
+    }
+    if (p.wave != 0 || !p.owns) return;
+    if (CARRY) {
+        a.seg_half[p.seg * BW + at] = half;
+        a.seg_sum[p.seg * BW + at] = state;
+    } else if (last == a.blocks) {
         a.final_state[at] = state;
     }
 }
 
+// CARRY: only the segment's decay and sum.
+template <typename T, typename G, bool WHOLE, bool CARRY>
+__global__ void __launch_bounds__(64 * kMaxWaves) rec_forward(RecArgs a) {
+    using C = Cfg<T>;
+    __shared__ __align__(16) Totals<C> tot;
+    const Place p = place<C, WHOLE>(a);
+    if (CARRY && p.seg == a.segments - 1) return;  // nothing comes after it
+    tot.clear();
+    __syncthreads();
+    forward_walk<T, G, WHOLE, CARRY>(a, p, tot);
+}
+
 // ---- backward ----------------------------------------------------------------------------
 
-template <typename T, typename G, bool UNIT, bool CARRY>
-__global__ void __launch_bounds__(64 * kMaxWaves) rec_backward(RecArgs a) {
-    constexpr int N = kN<T>, SLAB = N * kPieces;
-    __shared__ __align__(16) float tot_l[2][kMaxWaves][SLAB], tot_s[2][kMaxWaves][SLAB],
-        tot_e[2][kMaxWaves][SLAB];
-    __shared__ __align__(16) float in_h[kMaxWaves][SLAB], in_e[kMaxWaves][SLAB];
-    const Place p = place<T>(a);
-    const int BT = a.waves * kRuns * kL;
+template <typename T, typename G, bool WHOLE, bool CARRY, bool MASKED, typename C>
+__device__ __forceinline__ void backward_block(const RecArgs &a, const Place &p, Totals<C> &fwd, Totals<C> &bwd,
+                                               int buf, int64_t t, const Piece<T, C::N> (&x)[C::L],
+                                               const Piece<G, C::N> (&g)[C::L], const Piece<T, C::N> (&dy)[C::L],
+                                               const Masks &m, float state, float &adj, float &half) {
+    constexpr int N = C::N, L = C::L;
+    float d[L][N], l[N], s[N], q[N], e[N];
+    const bool plain = decays<MASKED>(g, m, d, l);
+    auto sums = [&](auto flag) {
+        constexpr bool PLAIN = decltype(flag)::value;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float h = 0.f, u = value<PLAIN>(dy, m, L - 1, j);
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (!CARRY) h = next_state<PLAIN>(d[i][j], h, value<PLAIN>(x, m, i, j));
+                const int k = L - 1 - i;
+                if (k) u = next_state<PLAIN>(d[k][j], u, value<PLAIN>(dy, m, k - 1, j));
+            }
+            const float E = through<PLAIN>(d[0][j], u);
+            s[j] = h, e[j] = E, q[j] = l[j];
+        }
+        scan_runs<C, false, !PLAIN>(q, e);
+        if (!CARRY) scan_runs<C, true, !PLAIN>(l, s);
+    };
+    if (plain) sums(std::true_type{});
+    else sums(std::false_type{});
+    if (p.run == 0) bwd.put(buf, p, q, e);
+    if (!CARRY && p.run == C::RUNS - 1) fwd.put(buf, p, l, s);
+    __syncthreads();
+    float all;
+    if (!CARRY) fwd.template pass<true>(buf, p, state, &all);
+    adj = bwd.template pass<false>(buf, p, adj, &all);
+    if (CARRY) {
+        half += all;
+        return;
+    }
+    auto grads = [&](auto flag) {
+        constexpr bool PLAIN = decltype(flag)::value;
+        float carried[L][N], u[N];  // exp(g_t) h_{t-1}, the adjoint
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float h = join<!PLAIN>(fwd.in[p.wave][p.piece * N + j], shifted<C::PIECES, true>(l[j]),
+                                   shifted<C::PIECES, true>(s[j]));
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                carried[i][j] = through<PLAIN>(d[i][j], h);
+                h = next_state<PLAIN>(d[i][j], h, value<PLAIN>(x, m, i, j));
+            }
+            const float E = join<!PLAIN>(bwd.in[p.wave][p.piece * N + j], shifted<C::PIECES, false>(q[j]),
+                                         shifted<C::PIECES, false>(e[j]));
+            u[j] = E + value<PLAIN>(dy, m, L - 1, j);
+        }
+#pragma unroll
+        for (int i = L - 1; i >= 0; --i) {
+            const bool on = PLAIN || (m.on >> i & 1);
+            float ox[N], og[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                ox[j] = on ? u[j] : 0.f;
+                og[j] = on && (PLAIN || d[i][j] != 0.f) ? carried[i][j] * u[j] : 0.f;
+                if (i) u[j] = next_state<PLAIN>(d[i][j], u[j], value<PLAIN>(dy, m, i - 1, j));
+            }
+            if (!MASKED || t + p.run * L + i < a.T) {
+                if (a.y) store_piece<WHOLE, L, T, N>(a.y, a, p, t, i, ox);
+                if (a.dg) store_piece<WHOLE, L, G, N>(a.dg, a, p, t, i, og);
+            }
+        }
+    };
+    if (plain) grads(std::true_type{});
+    else grads(std::false_type{});
+}
+
+template <typename T, typename G, bool WHOLE, bool CARRY, typename C>
+__device__ __forceinline__ void backward_walk(const RecArgs &a, const Place &p, Totals<C> &fwd, Totals<C> &bwd) {
+    constexpr int N = C::N, L = C::L;
+    const int BT = a.waves * C::TOKENS;
     const int first = p.seg * a.seg_blocks, last = min(first + a.seg_blocks, a.blocks);
     const int64_t BW = (int64_t)a.B * a.W, at = (int64_t)p.b * a.W + p.c;
-    const int ch = p.lane & (SLAB - 1);
-    if (CARRY && first == 0) return;  // nothing comes before it
-
+    const bool masks = a.valid.data || a.reset.data;
     float adj = 0.f, half = 0.f;  // E of channel p.c, behind the block
-    if (!CARRY && p.owns) {
+    if (!CARRY && p.there) {
         if (a.d_final) adj = a.d_final[at];
         adj = start_of(a, p, adj, a.segments - 1, p.seg, -1);
     }
-    int64_t t = (int64_t)(last - 1) * BT + (p.wave * kRuns + p.run) * kL;
-    Piece<T, N> x[kL], xn[kL], dy[kL], dyn[kL];
-    Piece<G, N> g[kL], gn[kL];
-    if (!CARRY) load_run<T, N, UNIT>(x, a.x, a, p, t);
-    load_run<G, N, UNIT>(g, a.g, a, p, t);
-    load_run<T, N, UNIT>(dy, a.dy, a, p, t);
+    int64_t t = (int64_t)(last - 1) * BT + p.wave * C::TOKENS;  // this wave's first token
+    auto inside = [&](int blk) { return (int64_t)(blk + 1) * BT <= a.T; };
+    Piece<T, N> x[L], xn[L], dy[L], dyn[L];
+    Piece<G, N> g[L], gn[L];
+    if (!CARRY) load_run<WHOLE>(x, a.x, a, p, t, inside(last - 1));
+    load_run<WHOLE>(g, a.g, a, p, t, inside(last - 1));
+    load_run<WHOLE>(dy, a.dy, a, p, t, inside(last - 1));
     for (int blk = last - 1; blk >= first; --blk, t -= BT) {
-        const int buf = blk & 1;
-        const Masks m = load_masks(a, p, t);
         float state = 0.f;
-        if (!CARRY && p.owns) state = a.states[blk * BW + at];
+        if (!CARRY && p.there) state = a.states[blk * BW + at];
         if (blk > first) {
-            if (!CARRY) load_run<T, N, UNIT>(xn, a.x, a, p, t - BT);
-            load_run<G, N, UNIT>(gn, a.g, a, p, t - BT);
-            load_run<T, N, UNIT>(dyn, a.dy, a, p, t - BT);
+            if (!CARRY) load_run<WHOLE>(xn, a.x, a, p, t - BT, true);
+            load_run<WHOLE>(gn, a.g, a, p, t - BT, true);
+            load_run<WHOLE>(dyn, a.dy, a, p, t - BT, true);
         }
-        float d[kL][N], l[N], s[N], q[N], e[N];
-        decays(g, m, d, l);
+        if (masks || !inside(blk))
+            backward_block<T, G, WHOLE, CARRY, true>(a, p, fwd, bwd, blk & 1, t, x, g, dy, load_masks<L>(a, p, t),
+                                                     state, adj, half);
+        else
+            backward_block<T, G, WHOLE, CARRY, false>(a, p, fwd, bwd, blk & 1, t, x, g, dy, Masks{~0u, 0}, state,
+                                                      adj, half);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            float h = 0.f, E = 0.f;
-#pragma unroll
-            for (int i = 0; i < kL; ++i) {
-                if (!CARRY) h = through(d[i][j], h) + (m.on[i] ? get(x[i], j) : 0.f);
-                const int k = kL - 1 - i;
-                E = through(d[k][j], E + (m.on[k] ? get(dy[k], j) : 0.f));
-            }
-            s[j] = h, e[j] = E, q[j] = l[j];
-        }
-        scan_runs<N, false>(q, e);
-        if (!CARRY) scan_runs<N, true>(l, s);
-        if (p.run == 0) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                tot_l[buf][p.wave][p.piece * N + j] = q[j];
-                tot_e[buf][p.wave][p.piece * N + j] = e[j];
-            }
-        }
-        if (!CARRY && p.run == kRuns - 1) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) tot_s[buf][p.wave][p.piece * N + j] = s[j];
-        }
-        __syncthreads();
-        float mine_h = state, mine_e = adj, all = 0.f, sum = 0.f;
-        for (int w = 0; w < a.waves; ++w) {
-            const int v = a.waves - 1 - w;
-            const float lv = tot_l[buf][v][ch], ev = tot_e[buf][v][ch];
-            if (!CARRY && v > p.wave) mine_e = join(mine_e, lv, ev);
-            if (!CARRY && w < p.wave) mine_h = join(mine_h, tot_l[buf][w][ch], tot_s[buf][w][ch]);
-            sum = join(sum, lv, ev);
-            all += lv;
-        }
-        adj = join(adj, all, sum);
-        if (CARRY) half += all;
-        if (!CARRY) {
-            if (p.lane < SLAB) in_h[p.wave][p.lane] = mine_h, in_e[p.wave][p.lane] = mine_e;
-            __builtin_amdgcn_wave_barrier();
-            float carried[kL][N];  // exp(g_t) h_{t-1}
-            float E[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                float lb = shifted<8, true>(l[j], 0.f), sb = shifted<8, true>(s[j], 0.f);
-                float h = join(in_h[p.wave][p.piece * N + j], lb, sb);
-#pragma unroll
-                for (int i = 0; i < kL; ++i) {
-                    carried[i][j] = through(d[i][j], h);
-                    h = carried[i][j] + (m.on[i] ? get(x[i], j) : 0.f);
-                }
-                lb = shifted<8, false>(q[j], 0.f), sb = shifted<8, false>(e[j], 0.f);
-                E[j] = join(in_e[p.wave][p.piece * N + j], lb, sb);
-            }
-            const int64_t o = (p.b * a.T + t) * a.W + p.c0;
-#pragma unroll
-            for (int i = kL - 1; i >= 0; --i) {
-                float ox[N], og[N];
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float u = E[j] + (m.on[i] ? get(dy[i], j) : 0.f);
-                    ox[j] = m.on[i] ? u : 0.f;
-                    og[j] = m.on[i] && d[i][j] != 0.f ? carried[i][j] * u : 0.f;
-                    E[j] = through(d[i][j], u);
-                }
-                if (t + i < a.T) {
-                    if (a.y) store_piece<T, N>((T *)a.y + o + (int64_t)i * a.W, ox, p.n);
-                    if (a.dg) store_piece<G, N>((G *)a.dg + o + (int64_t)i * a.W, og, p.n);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kL; ++i) x[i] = xn[i], g[i] = gn[i], dy[i] = dyn[i];
+        for (int i = 0; i < L; ++i) x[i] = xn[i], g[i] = gn[i], dy[i] = dyn[i];
     }
+    if (p.wave != 0 || !p.owns) return;
     if (CARRY) {
-        if (p.wave == 0 && p.owns) {
-            a.seg_half[p.seg * BW + at] = half;
-            a.seg_sum[p.seg * BW + at] = adj;
-        }
-    } else if (p.wave == 0 && p.owns && first == 0 && a.final_state) {
+        a.seg_half[p.seg * BW + at] = half;
+        a.seg_sum[p.seg * BW + at] = adj;
+    } else if (first == 0 && a.final_state) {
         a.final_state[at] = adj;
     }
+}
+
+template <typename T, typename G, bool WHOLE, bool CARRY>
+__global__ void __launch_bounds__(64 * kMaxWaves) rec_backward(RecArgs a) {
+    using C = Cfg<T>;
+    __shared__ __align__(16) Totals<C> fwd, bwd;
+    const Place p = place<C, WHOLE>(a);
+    if (CARRY && p.seg == 0) return;  // nothing comes before it
+    fwd.clear(), bwd.clear();
+    __syncthreads();
+    backward_walk<T, G, WHOLE, CARRY>(a, p, fwd, bwd);
 }
 
 // ---- one token -----------------------------------------------------------------------------
@@ -470,8 +630,9 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) rec_ste
     if (on) {
         const bool cut = a.reset.data && ((const float *)a.reset.data)[b * a.reset.s0] != 0.f;
         float l = Elem<G>::load(a.g.data, b * a.g.s0 + c * a.g.s2) * kLog2e;
-        const float d = cut ? 0.f : decay_of(l);
-        y = through(d, a.final_state[i]) + Elem<T>::load(a.x.data, b * a.x.s0 + c * a.x.s2);
+        l = l > 127.f ? 127.f : l;  // NaN stays
+        const float d = cut || l < -126.f ? 0.f : __builtin_amdgcn_exp2f(l);
+        y = next_state<false>(d, a.final_state[i], Elem<T>::load(a.x.data, b * a.x.s0 + c * a.x.s2));
         a.final_state[i] = y;
     }
     Elem<T>::store(a.y, i, y);
@@ -484,7 +645,10 @@ struct Split {
     int slabs, waves, blocks, seg_blocks, segments;
 };
 
-constexpr int kWantedGroups = 512;
+// Workgroups that fill the card.  Segments read the inputs twice, so they are taken only to come to one
+// workgroup a CU (64 x 2048 tokens of 256 channels, 512 workgroups: 150 us, in two segments 243; 4 x 8192
+// of 2048, 256 workgroups: 306, in two 405).
+constexpr int kWantedGroups = 256;
 
 int check_shape(const gdn2_recurrence_shape *s) {
     if (!s) return fail(GDN2_ERR_ARGUMENT, "shape is null");
@@ -498,11 +662,12 @@ int check_shape(const gdn2_recurrence_shape *s) {
 
 Split split_of(const gdn2_recurrence_shape *s, int32_t dtype) {
     Split k;
-    const int slab = kPieces * (dtype == GDN2_BF16 ? 8 : 4);
+    const bool bf = dtype == GDN2_BF16;
+    const int slab = bf ? Cfg<bf16_t>::SLAB : Cfg<float>::SLAB, run = bf ? Cfg<bf16_t>::TOKENS : Cfg<float>::TOKENS;
     k.slabs = (int)((s->width + slab - 1) / slab);
     k.waves = 1;
-    while (k.waves < kMaxWaves && s->time > (int64_t)k.waves * kRuns * kL) k.waves *= 2;
-    const int64_t bt = (int64_t)k.waves * kRuns * kL;
+    while (k.waves < kMaxWaves && s->time > (int64_t)k.waves * run) k.waves *= 2;
+    const int64_t bt = (int64_t)k.waves * run;
     k.blocks = (int)((s->time + bt - 1) / bt);
     const int64_t units = (int64_t)k.slabs * s->batch;
     int64_t segs = units >= kWantedGroups ? 1 : (kWantedGroups + units - 1) / units;
@@ -560,27 +725,27 @@ int grid_of(const RecArgs &a, int segments, unsigned *out) {
     return ok();
 }
 
-template <typename T, typename G, bool UNIT>
+template <typename T, typename G, bool WHOLE>
 void launch_rec(const RecArgs &a, bool backward, bool carry, unsigned grid, hipStream_t st) {
     const dim3 block(64 * a.waves);
     if (backward) {
-        if (carry) hipLaunchKernelGGL((rec_backward<T, G, UNIT, true>), dim3(grid), block, 0, st, a);
-        else hipLaunchKernelGGL((rec_backward<T, G, UNIT, false>), dim3(grid), block, 0, st, a);
+        if (carry) hipLaunchKernelGGL((rec_backward<T, G, WHOLE, true>), dim3(grid), block, 0, st, a);
+        else hipLaunchKernelGGL((rec_backward<T, G, WHOLE, false>), dim3(grid), block, 0, st, a);
     } else {
-        if (carry) hipLaunchKernelGGL((rec_forward<T, G, UNIT, true>), dim3(grid), block, 0, st, a);
-        else hipLaunchKernelGGL((rec_forward<T, G, UNIT, false>), dim3(grid), block, 0, st, a);
+        if (carry) hipLaunchKernelGGL((rec_forward<T, G, WHOLE, true>), dim3(grid), block, 0, st, a);
+        else hipLaunchKernelGGL((rec_forward<T, G, WHOLE, false>), dim3(grid), block, 0, st, a);
     }
 }
 
-template <bool UNIT>
+template <bool WHOLE>
 void launch_types(const RecArgs &a, int32_t dtype, int32_t gtype, bool backward, bool carry,
                   unsigned grid, hipStream_t st) {
     if (dtype == GDN2_BF16) {
-        if (gtype == GDN2_BF16) launch_rec<bf16_t, bf16_t, UNIT>(a, backward, carry, grid, st);
-        else launch_rec<bf16_t, float, UNIT>(a, backward, carry, grid, st);
+        if (gtype == GDN2_BF16) launch_rec<bf16_t, bf16_t, WHOLE>(a, backward, carry, grid, st);
+        else launch_rec<bf16_t, float, WHOLE>(a, backward, carry, grid, st);
     } else {
-        if (gtype == GDN2_BF16) launch_rec<float, bf16_t, UNIT>(a, backward, carry, grid, st);
-        else launch_rec<float, float, UNIT>(a, backward, carry, grid, st);
+        if (gtype == GDN2_BF16) launch_rec<float, bf16_t, WHOLE>(a, backward, carry, grid, st);
+        else launch_rec<float, float, WHOLE>(a, backward, carry, grid, st);
     }
 }
 
@@ -588,10 +753,16 @@ int launch_all(const RecArgs &a, int32_t dtype, int32_t gtype, bool backward, vo
                const char *what) {
     unsigned grid;
     GDN2_TRY(grid_of(a, a.segments, &grid));
-    const bool unit = a.x.s2 == 1 && a.g.s2 == 1 && (!backward || a.dy.s2 == 1);
+    // whole slabs of channels side by side, a block's offsets, 4 bytes a value at most, in 32 bits
+    constexpr int64_t near = (1 << 29) / (kMaxWaves * (Cfg<float>::TOKENS > Cfg<bf16_t>::TOKENS
+                                                           ? Cfg<float>::TOKENS : Cfg<bf16_t>::TOKENS));
+    auto beside = [&](const View &v) { return v.s2 == 1 && v.s1 <= near; };
+    const int slab = dtype == GDN2_BF16 ? Cfg<bf16_t>::SLAB : Cfg<float>::SLAB;
+    const bool whole = a.W >= slab && a.W <= near && beside(a.x) && beside(a.g) && (!backward || beside(a.dy));
+    hipStream_t st = (hipStream_t)stream;
     for (int carry = a.segments > 1 ? 1 : 0; carry >= 0; --carry) {
-        if (unit) launch_types<true>(a, dtype, gtype, backward, carry, grid, (hipStream_t)stream);
-        else launch_types<false>(a, dtype, gtype, backward, carry, grid, (hipStream_t)stream);
+        if (whole) launch_types<true>(a, dtype, gtype, backward, carry, grid, st);
+        else launch_types<false>(a, dtype, gtype, backward, carry, grid, st);
     }
     return launch_status(hipGetLastError(), what);
 }
