@@ -171,7 +171,8 @@ SIGNATURES = {
     "gdn2_recurrence_backward": (_I, [_P] * 6 + [_Z] + [_P] * 6 + [_Z, _P]),
     "gdn2_recurrence_step": (_I, [_P] * 8),
     "gdn2_token_score_forward": (_I, [_L, _L, _P, _P, _L, _P, _L, ctypes.c_float, ctypes.c_int32]
-                                 + [_P] * 6),
+                                 + [_P] * 6 + [_Z, _P]),
+    "gdn2_token_score_workspace_bytes": (_Z, [_L, _L, ctypes.c_int32]),
     "gdn2_token_score_backward": (_I, [_L, _L, _P, _P, _L, _P, _L, ctypes.c_float, _P, _P, _L, _P, _L,
                                        _P, _P]),
     "gdn2_orthogonalize_workspace_bytes": (_Z, [_P]),

@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from ._lib import lib
 from ._once import once
 from .linear_ops import (_CODES, F32, _VIEW, _call, _differentiates, _dtype, _ptr, _same_device)
 
@@ -67,9 +68,13 @@ def _forward(x, tokens, top, valid, temperature, stats):
         top_lp = torch.empty(lead + (top,), dtype=F32, device=dev)
         top_tokens = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
     stats = torch.empty((rows, 3), dtype=F32, device=dev) if stats else None
+    ws, n = None, 0
+    if rows <= 64 and width >= 65536:  # few wide rows, whose parts are joined
+        n = lib().gdn2_token_score_workspace_bytes(rows, width, top)
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
     _call("gdn2_token_score_forward", dev, rows, width, view, tokens.data_ptr(), _stride(tokens),
           _ptr(valid), _stride(valid), temperature, top, lp.data_ptr(), entropy.data_ptr(),
-          _ptr(top_lp), _ptr(top_tokens), _ptr(stats))
+          _ptr(top_lp), _ptr(top_tokens), _ptr(stats), _ptr(ws), n)
     return TokenLogProbs(lp, entropy, top_lp, top_tokens), stats
 
 

@@ -665,13 +665,16 @@ GDN2_API int gdn2_recurrence_step(const gdn2_recurrence_shape *shape, const gdn2
  * is not valid is not read and gives zeros.  A target outside [0, width) gives NaN, and
  * so does a row whose largest value is infinite or that holds a NaN; -inf is probability
  * 0.  temperature is positive.  stats [rows, 3] F32 is what the backward reads (may be
- * NULL).  The log probability and the entropy are made from a sum in 64 bits. */
+ * NULL).  The log probability and the entropy are made from a sum in 64 bits.  The
+ * workspace (16-byte aligned) is for rows that are few and wide; the query gives 0 where
+ * none is needed. */
+GDN2_API size_t gdn2_token_score_workspace_bytes(int64_t rows, int64_t width, int32_t top);
 GDN2_API int gdn2_token_score_forward(int64_t rows, int64_t width, const gdn2_view *x,
                                       const int64_t *target, int64_t target_stride,
                                       const float *valid, int64_t valid_stride, float temperature,
                                       int32_t top, float *log_probs, float *entropy,
                                       float *top_log_probs, int64_t *top_tokens, float *stats,
-                                      void *stream);
+                                      void *workspace, size_t workspace_bytes, void *stream);
 
 /* VJP of log_probs and entropy: dx dense in x's dtype, zeros for rows that are not valid.
  * d_log_probs, d_entropy [rows] F32 with element strides; either may be NULL (zero).  A

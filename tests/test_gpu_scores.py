@@ -137,6 +137,49 @@ def test_a_wide_row(dk):
 
 
 @BOTH
+@pytest.mark.parametrize("rows,width", [(1, 65536), (1, 65537), (3, 100003), (11, 131072), (64, 70000), (2, 200000),
+                                        (65, 70000)])
+def test_rows_in_parts(dk, rows, width, dtype):
+    """Few rows that are wide: parts, whose sums and alternatives are joined; 65 rows are not split."""
+    c = case(width, rows, width, dtype, 0.8, masked=rows == 3)
+    c["valid"] = np.ones(rows)
+    c["valid"][1:rows:3] = 0
+    r = np.random.default_rng(rows)
+    c["x"][0] = rounded(r.integers(-2, 3, width).astype(float), dtype)  # thousands at the bound
+    check(c, dtype, *run(dk, c, dtype, 20))
+    if rows < 3:
+        check(c, dtype, *run(dk, c, dtype, 64))
+        check(c, dtype, *run(dk, c, dtype, 0))
+
+
+@BOTH
+def test_rows_in_parts_at_the_edges(dk, dtype):
+    """Parts without a finite value, values that are not finite, and alternatives that all lie in one part."""
+    width = 90001
+    c = case(3, 6, width, dtype)
+    nan, inf = np.nan, np.inf
+    c["x"][0, 100:] = -inf
+    c["x"][0, 200] = 1.0
+    c["t"][0] = 5
+    c["x"][1] = -inf
+    c["x"][2, 70000], c["x"][2, 5] = nan, inf
+    c["x"][3, 80000:80030] = np.linspace(20, 30, 30)
+    c["x"][3] = rounded(c["x"][3], dtype)
+    c["x"][4, ::2] = -0.0
+    c["x"][4, 1::2] = 0.0
+    x = dev(c["x"], dtype).requires_grad_(True)
+    r = dk.token_log_probs(x, dev(c["t"], torch.int64), 25)
+    (dx,) = torch.autograd.grad([r.log_probs, r.entropy], [x], [dev(c["d"]), dev(c["dh"])])
+    assert np.array_equal(r.top_tokens.cpu().numpy(), ro.top(c["x"], 25))
+    for row in (1, 2):
+        assert r.log_probs[row].isnan() and r.entropy[row].isnan() and dx[row].isnan().all()
+    for row in (0, 3, 4, 5):
+        keep = slice(row, row + 1)
+        sub = dict(c, x=c["x"][keep], t=c["t"][keep], d=c["d"][keep], dh=c["dh"][keep])
+        check(sub, dtype, dk.TokenLogProbs(*(t[keep] for t in r)), dx[keep])
+
+
+@BOTH
 @pytest.mark.parametrize("top", [1, 2, 31, 32, 63, 64])
 def test_alternatives(dk, top, dtype):
     for width in (64, 65, 3000):

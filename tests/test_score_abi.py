@@ -19,9 +19,9 @@ def view(dtype=0, data=0x1000, strides=(64, 1, 0, 0)):
 
 
 def forward(L, rows=4, width=64, x=None, target=0x2000, ts=1, temperature=1.0, top=0, lp=0x3000, tlp=None,
-            tt=None):
+            tt=None, ws=None, n=0):
     return L.gdn2_token_score_forward(rows, width, x or view(), target, ts, None, 0,
-                                      ctypes.c_float(temperature), top, lp, 0x4000, tlp, tt, None, None)
+                                      ctypes.c_float(temperature), top, lp, 0x4000, tlp, tt, None, ws, n, None)
 
 
 def backward(L, rows=4, width=64, x=None, stats=0x3000, dls=1, dx=0x4000):
@@ -47,3 +47,14 @@ def test_refusals(L):
     assert forward(L, rows=0, x=view(data=0), target=None, lp=None) == 0
     assert backward(L, stats=None) == 1 and backward(L, dx=None) == 1 and backward(L, dls=-1) == 1
     assert backward(L, rows=0) == 0
+
+
+def test_workspace(L):
+    size = L.gdn2_token_score_workspace_bytes
+    assert size(8192, 32768, 8) == 0 and size(8, 32768, 64) == 0 and size(65, 1 << 20, 8) == 0
+    need = size(2, 200000, 8)
+    assert need > size(2, 200000, 0) > 0
+    assert size(-1, 200000, 0) == 0 and size(1, 0, 0) == 0 and size(1, 200000, 65) == 0
+    wide = dict(rows=2, width=200000, x=view(strides=(200000, 1, 0, 0)), top=8, tlp=0x5000, tt=0x6000)
+    assert forward(L, **wide) == 4 and forward(L, **wide, ws=0x7000, n=need - 1) == 4 and "workspace" in message(L)
+    assert forward(L, **wide, ws=0x7008, n=need) == 1
