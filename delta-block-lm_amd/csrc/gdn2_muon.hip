@@ -196,7 +196,9 @@ struct GemmArgs {
     Split l, r;                // operands: C = L R^T
     Split out, out_t;          // GRAM, POLY: out; NEXT: both
     int64_t l_step, r_step, out_step;  // bytes between matrices
-    int tiles_i, tiles_j, tiles, count;  // tiles of a matrix
+    int tiles_i, tiles_j, tiles;  // tiles of a matrix
+    int whole, parts;          // tiles made at once; parts of the others' sums
+    float *partial;            // [tile that is not whole][part][T][T]
     int k;                     // columns of the operands
     float scale;               // of the accumulators
     float a, b;                // POLY: of the identity and of A, in the result's scale
@@ -272,20 +274,83 @@ template <bool SYM> __device__ __forceinline__ void tile_of(int t, int ni, int n
     }
 }
 
+// What a product makes of its tile S at (I, J): the next operand, in both orientations where mirror is
+// set, or the results.
+template <int T, Mode MODE>
+__device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, int J, bool mirror, float *S,
+                                            int threads) {
+    if constexpr (MODE == LAST) {
+        const int mr = p.tall ? J : I, mc = p.tall ? I : J;
+        for (int i = threadIdx.x; i < T * T; i += threads) {
+            const int a = i / T, b = i % T;
+            const int64_t r = mr + a, c = mc + b;
+            if (r >= p.rows || c >= p.cols) continue;
+            const float v = S[p.tall ? at_tile<T>(b, a) : at_tile<T>(a, b)];
+            const int64_t o = r * p.cols + c;
+            if (p.update) {
+                float *q = p.t.param[mat] + o;
+                *q = p.decay * *q - p.rate * v;
+            } else {
+                store_out(p.result, p.bf16, (int64_t)(p.first + mat) * p.rows * p.cols + o, v);
+            }
+        }
+        return;
+    }
+    Split out = p.out, out_t = MODE == NEXT ? p.out_t : p.out;
+    out.data += mat * p.out_step, out_t.data += mat * p.out_step;
+    if constexpr (MODE == POLY) {
+        Split A = p.l;
+        A.data += mat * p.l_step;
+        for (int i = threadIdx.x; i < T * T / 8; i += threads) {
+            const int a = i / (T / 8), b = i % (T / 8) * 8;
+            float v[8];
+            load_split(A, I + a, J + b, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float &u = S[at_tile<T>(a, b + j)];
+                u += p.b * v[j];
+                if (I + a == J + b + j) u += p.a;
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < T * T / 8; i += threads) {
+        const int a = i / (T / 8), b = i % (T / 8) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(a, b + j)];
+        store_split(out, I + a, J + b, v);
+        if (mirror) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(b + j, a)];
+            store_split(out_t, J + a, I + b, v);
+        }
+    }
+}
+
 template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) ns_product(GemmArgs p) {
     using C = Tile<T>;
-    constexpr int F = C::F, kThreads = C::THREADS;
+    constexpr int F = C::F;
     __shared__ __align__(1024) char lds[C::BYTES];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    // Neighbouring tiles to one XCD (workgroups go to the eight in turn).
-    const int total = p.tiles * p.count, x = blockIdx.x & 7, full = total >> 3, more = total & 7;
-    const int at = (blockIdx.x >> 3) + x * full + min(x, more);
+    // Neighbouring tiles to one XCD (workgroups go to the eight in turn): first the whole tiles, behind them
+    // those that are made in parts of the sum.
+    const bool part = (int)blockIdx.x >= p.whole;
+    const int first = part ? p.whole : 0, b = blockIdx.x - first;
+    const int total = part ? (int)gridDim.x - p.whole : p.whole, x = b & 7, full = total >> 3, more = total & 7;
+    const int piece = (b >> 3) + x * full + min(x, more);
+    int at = piece, stages = p.k / kChunk, from = 0;
+    if (part) {
+        const int n = piece % p.parts;
+        at = p.whole + piece / p.parts;
+        from = (int)((int64_t)stages * n / p.parts);
+        stages = (int)((int64_t)stages * (n + 1) / p.parts) - from;
+    }
     const int mat = at / p.tiles;
     int ti, tj;
     tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
     const int I = ti * T, J = tj * T;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
-    const int stages = p.k / kChunk;
     f32x4 acc[F][F];
 
     if (w >= C::WAVES) {  // loads
@@ -297,8 +362,8 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
         const uint32_t row = (uint32_t)row_bytes(p.k);
         const uint32_t lane0 = (l >> 3) * row + swizzle(l >> 3, l & 7) * 16;
         const uint32_t lane8 = (l >> 3) * row + swizzle(8 + (l >> 3), l & 7) * 16;
-        const char *left = p.l.data + mat * p.l_step + (int64_t)I * row;
-        const char *right = p.r.data + mat * p.r_step + (int64_t)J * row;
+        const char *left = p.l.data + mat * p.l_step + (int64_t)I * row + from * 128;
+        const char *right = p.r.data + mat * p.r_step + (int64_t)J * row + from * 128;
         auto issue = [&](int s) {
             char *slot = lds + (s % C::STAGES) * C::STAGE;
 #pragma unroll
@@ -366,53 +431,37 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
                     S[at_tile<T>(wi + 16 * a + 4 * (l >> 4) + i, wj + 16 * b + (l & 15))] = acc[a][b][i] * p.scale;
     }
     __syncthreads();
-    if constexpr (MODE == LAST) {
-        const int mr = p.tall ? J : I, mc = p.tall ? I : J;
-        for (int i = threadIdx.x; i < T * T; i += kThreads) {
-            const int a = i / T, b = i % T;
-            const int64_t r = mr + a, c = mc + b;
-            if (r >= p.rows || c >= p.cols) continue;
-            const float v = S[p.tall ? at_tile<T>(b, a) : at_tile<T>(a, b)];
-            const int64_t o = r * p.cols + c;
-            if (p.update) {
-                float *q = p.t.param[mat] + o;
-                *q = p.decay * *q - p.rate * v;
-            } else {
-                store_out(p.result, p.bf16, (int64_t)(p.first + mat) * p.rows * p.cols + o, v);
-            }
-        }
+    if (part) {
+        float4 *to = reinterpret_cast<float4 *>(p.partial + (int64_t)piece * T * T);
+        for (int i = threadIdx.x; i < T * T / 4; i += C::THREADS)
+            to[i] = *reinterpret_cast<const float4 *>(S + at_tile<T>(i / (T / 4), i % (T / 4) * 4));
         return;
     }
-    Split out = p.out, out_t = MODE == NEXT ? p.out_t : p.out;
-    out.data += mat * p.out_step, out_t.data += mat * p.out_step;
-    if constexpr (MODE == POLY) {
-        Split A = p.l;
-        A.data += mat * p.l_step;
-        for (int i = threadIdx.x; i < T * T / 8; i += kThreads) {
-            const int a = i / (T / 8), b = i % (T / 8) * 8;
-            float v[8];
-            load_split(A, I + a, J + b, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float &u = S[at_tile<T>(a, b + j)];
-                u += p.b * v[j];
-                if (I + a == J + b + j) u += p.a;
-            }
+    finish_tile<T, MODE>(p, mat, I, J, !SYM || ti != tj, S, C::THREADS);
+}
+
+// The sums of the tiles that were made in parts, in order, a quarter of a tile each.
+template <Mode MODE> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) {
+    constexpr int T = 128, Q = 64;
+    __shared__ __align__(16) float S[Q * Q];
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    const int n = blockIdx.x >> 2, qi = (blockIdx.x >> 1 & 1) * Q, qj = (blockIdx.x & 1) * Q;
+    const int at = p.whole + n;
+    int ti, tj;
+    tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
+    const float *from = p.partial + (int64_t)n * p.parts * T * T + qi * T + qj;
+    for (int i = threadIdx.x; i < Q * Q / 4; i += 256) {
+        const int a = i / (Q / 4), b = i % (Q / 4) * 4;
+        float4 sum = *reinterpret_cast<const float4 *>(from + a * T + b);
+#pragma unroll 4
+        for (int k = 1; k < p.parts; ++k) {
+            const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)k * T * T + a * T + b);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-        __syncthreads();
+        *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) = sum;
     }
-    for (int i = threadIdx.x; i < T * T / 8; i += kThreads) {
-        const int a = i / (T / 8), b = i % (T / 8) * 8;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(a, b + j)];
-        store_split(out, I + a, J + b, v);
-        if (!SYM || ti != tj) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(b + j, a)];
-            store_split(out_t, J + a, I + b, v);
-        }
-    }
+    __syncthreads();
+    finish_tile<Q, MODE>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, 256);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -436,15 +485,32 @@ int check_matrices(const gdn2_matrices_shape *s) {
 
 int64_t padded(int64_t n, int64_t t) { return (n + t - 1) / t * t; }
 
-// About the time of a product in us, from the figures at Tile: a CU's tiles one after another, each
-// with its stages and its result, and the launch.
-double time_of(int tile, int64_t tiles, int64_t stages) {
+constexpr int kAtOnce = 512;  // workgroups of large tiles that the card holds
+
+// How the tiles of a product are made: those that fill the card once or more at once, the others, if it
+// pays, in parts of their sums that fill it once more, which another kernel joins.
+struct Way {
+    int tile, parts;
+    int64_t whole;
+    double time;  // about, in us: a CU's tiles one after another, each with its stages and its result, and the
+                  // launch, from the figures at Tile; 16 KB of a part are written and read in 16 ns
+};
+
+Way way_of(int tile, int64_t tiles, int64_t stages) {
     const int64_t turns = (tiles + 255) / 256;
-    if (tile == 64) return turns * (0.2 * stages + 1) + 5;
-    return turns == 1 ? 0.65 * stages + 7 : turns * (0.6 * stages + 2) + 5;
+    if (tile == 64) return {64, 1, tiles, turns * (0.2 * stages + 1) + 5};
+    Way best = {128, 1, tiles, turns == 1 ? 0.65 * stages + 7 : turns * (0.6 * stages + 2) + 5};
+    const int64_t whole = tiles / kAtOnce * kAtOnce, rest = tiles - whole;
+    for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= 4; ++parts) {
+        const int64_t each = (stages + parts - 1) / parts;
+        const double time = whole / 256 * (0.6 * stages + 2) + (rest * parts <= 256 ? 0.65 : 1.2) * each + 13 +
+                            0.016 * rest * parts;
+        if (time < best.time) best = {128, parts, whole, time};
+    }
+    return best;
 }
 
-// Each product takes the tile that time_of prefers; sizes are padded to the larger of them.
+// Each product takes the tile that way_of prefers; sizes are padded to the larger of them.
 Plan plan_of(const gdn2_matrices_shape *s) {
     const int64_t m = s->rows < s->cols ? s->rows : s->cols, n = s->rows < s->cols ? s->cols : s->rows;
     const int64_t count = s->count < kGroup ? s->count : kGroup;
@@ -458,8 +524,8 @@ Plan plan_of(const gdn2_matrices_shape *s) {
             double time[2];
             for (int i = 0; i < 2; ++i) {
                 const int64_t t = 64 << i, ti = p.m / t, tn = p.n / t;
-                time[i] = time_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
-                                  (mode == GRAM ? p.n : p.m) / kChunk);
+                time[i] = way_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
+                                 (mode == GRAM ? p.n : p.m) / kChunk).time;
             }
             const bool large = pad == 128 && time[1] < time[0];
             p.tile[mode] = large ? 128 : 64;
@@ -483,8 +549,11 @@ int parts_of(const gdn2_matrices_shape *s) {
     return n > kParts ? kParts : (int)n;
 }
 
+constexpr size_t kPartialBytes = (size_t)kAtOnce * 128 * 128 * sizeof(float);
+
 size_t workspace_of(const Plan &p) {
-    return (size_t)p.group * p.matrix_bytes + (size_t)p.group * kParts * sizeof(double);
+    const bool large = p.tile[GRAM] == 128 || p.tile[POLY] == 128 || p.tile[NEXT] == 128;
+    return (size_t)p.group * p.matrix_bytes + (size_t)p.group * kParts * sizeof(double) + (large ? kPartialBytes : 0);
 }
 
 // The largest |a t + b t^3 + c t^5| for t in [0, s], and the largest |a + b u + c u^2| for u in [0, s^2].
@@ -532,14 +601,14 @@ int check_steps(int steps, const float *k, float epsilon) {
     return ok();
 }
 
-template <int T> void launch_mode(Mode mode, const GemmArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)(a.tiles * a.count)), block(Tile<T>::THREADS);
-    switch (mode) {
-        case GRAM: hipLaunchKernelGGL((ns_product<T, GRAM>), grid, block, 0, st, a); break;
-        case POLY: hipLaunchKernelGGL((ns_product<T, POLY>), grid, block, 0, st, a); break;
-        case NEXT: hipLaunchKernelGGL((ns_product<T, NEXT>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((ns_product<T, LAST>), grid, block, 0, st, a);
+template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, int64_t rest, hipStream_t st) {
+    const dim3 grid((unsigned)(w.whole + rest * w.parts));
+    if (w.tile == 64) {
+        hipLaunchKernelGGL((ns_product<64, MODE>), grid, dim3(Tile<64>::THREADS), 0, st, a);
+        return;
     }
+    hipLaunchKernelGGL((ns_product<128, MODE>), grid, dim3(Tile<128>::THREADS), 0, st, a);
+    if (rest) hipLaunchKernelGGL((ns_join<MODE>), dim3((unsigned)(4 * rest)), dim3(256), 0, st, a);
 }
 
 // All products of one group of matrices; last holds the fields of the last product's results.
@@ -567,14 +636,21 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
         const Bounds b = bounds_of(k, s);
         const double sa = power_for(s * s), sb = power_for(b.poly), next = b.x * 1.001;
         GemmArgs g = last;
-        g.count = count;
+        g.partial = (float *)(partial + (size_t)p.group * kParts);
         g.l_step = g.r_step = g.out_step = p.matrix_bytes;
         auto run = [&](Mode mode) {
             const int t = p.tile[mode], ti = (int)(p.m / t), tn = (int)(p.n / t);
             g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
             g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
-            if (t == 128) launch_mode<128>(mode, g, st);
-            else launch_mode<64>(mode, g, st);
+            const int64_t tiles = (int64_t)g.tiles * count;
+            const Way w = way_of(t, tiles, g.k / kChunk);
+            g.whole = (int)w.whole, g.parts = w.parts;
+            switch (mode) {
+                case GRAM: launch_product<GRAM>(g, w, tiles - w.whole, st); break;
+                case POLY: launch_product<POLY>(g, w, tiles - w.whole, st); break;
+                case NEXT: launch_product<NEXT>(g, w, tiles - w.whole, st); break;
+                default: launch_product<LAST>(g, w, tiles - w.whole, st);
+            }
         };
         g.l = g.r = x, g.out = A;
         g.k = (int)p.n;
