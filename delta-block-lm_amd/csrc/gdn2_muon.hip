@@ -106,6 +106,20 @@ template <typename T> __device__ __forceinline__ void load4(const T *p, int64_t 
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? Elem<T>::load(p, i + j) : 0.f;
 }
 
+// The first n of four values.
+template <typename T> __device__ __forceinline__ void store4(T *p, int n, const float *v) {
+    if (n == 4) {
+        T w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Elem<T>::store(w, j, v[j]);
+        __builtin_memcpy(p, w, sizeof(w));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < n) Elem<T>::store(p, j, v[j]);
+}
+
 // Sums of squares in 64 bits: of a part of a dense matrix's values, or of every so-manieth row of
 // another; an update's momentum first takes the gradient.
 template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squares(Source s, double *partial) {
@@ -281,17 +295,25 @@ __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, i
                                             int threads) {
     if constexpr (MODE == LAST) {
         const int mr = p.tall ? J : I, mc = p.tall ? I : J;
-        for (int i = threadIdx.x; i < T * T; i += threads) {
-            const int a = i / T, b = i % T;
+        for (int i = threadIdx.x; i < T * T / 4; i += threads) {
+            const int a = i / (T / 4), b = i % (T / 4) * 4;
             const int64_t r = mr + a, c = mc + b;
-            if (r >= p.rows || c >= p.cols) continue;
-            const float v = S[p.tall ? at_tile<T>(b, a) : at_tile<T>(a, b)];
+            const int n = (int)min((int64_t)4, p.cols - c);  // columns that the result has
+            if (r >= p.rows || n <= 0) continue;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = S[p.tall ? at_tile<T>(b + j, a) : at_tile<T>(a, b + j)];
             const int64_t o = r * p.cols + c;
             if (p.update) {
-                float *q = p.t.param[mat] + o;
-                *q = p.decay * *q - p.rate * v;
+                float *q = p.t.param[mat] + o, old[4];
+                load4(q, 0, n, old);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = p.decay * old[j] - p.rate * v[j];
+                store4(q, n, v);
             } else {
-                store_out(p.result, p.bf16, (int64_t)(p.first + mat) * p.rows * p.cols + o, v);
+                const int64_t at = (int64_t)(p.first + mat) * p.rows * p.cols + o;
+                if (p.bf16) store4((bf16_t *)p.result + at, n, v);
+                else store4((float *)p.result + at, n, v);
             }
         }
         return;
@@ -493,7 +515,7 @@ struct Way {
     int tile, parts;
     int64_t whole;
     double time;  // about, in us: a CU's tiles one after another, each with its stages and its result, and the
-                  // launch, from the figures at Tile; 16 KB of a part are written and read in 16 ns
+                  // launch, from the figures at Tile; a part (64 KB) is written and read in 16 ns
 };
 
 Way way_of(int tile, int64_t tiles, int64_t stages) {
@@ -503,7 +525,7 @@ Way way_of(int tile, int64_t tiles, int64_t stages) {
     const int64_t whole = tiles / kAtOnce * kAtOnce, rest = tiles - whole;
     for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= 4; ++parts) {
         const int64_t each = (stages + parts - 1) / parts;
-        const double time = whole / 256 * (0.6 * stages + 2) + (rest * parts <= 256 ? 0.65 : 1.2) * each + 13 +
+        const double time = whole / 256 * (0.6 * stages + 2) + (rest * parts <= 256 ? 0.65 : 1.2) * each + 20 +
                             0.016 * rest * parts;
         if (time < best.time) best = {128, parts, whole, time};
     }
