@@ -9,11 +9,20 @@
 // orientations for that.  A and A A are symmetric: the tiles on and above the diagonal are made and
 // written twice.
 //
-// Precision.  An operand of a product goes in as two float16 terms, x = hi + lo, 22 bits, and a
-// product as hi hi + hi lo + lo hi into float32 accumulators: 2^-22 of the operands, at a third of
-// the matrix cores' float16 rate, where their float32 rate is a sixteenth.  float16's range is met by powers of
-// two: the largest singular values that X, A and B can have follow from the coefficients, no entry
-// is larger, and the powers bring those to 2^14.  What is below 2^-24 there is 2^-38 of the largest.
+// Precision.  An operand of a product goes in as two float16 terms, x = hi + lo, 23 bits, and a
+// product as hi hi + hi lo + lo hi into float32 accumulators, at a third of the matrix cores' float16
+// rate, where their float32 rate is a sixteenth.  float16's range is met by powers of two: the largest
+// singular values that X, A and B can have follow from the coefficients, no entry is larger, and the
+// powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Results are off by
+// half of what float32 products leave (512 x 1408 and larger); sums of a small tile have the small
+// products in accumulators of their own, so that a long sum is not rounded three times as often.  Where
+// the smaller side is at most 64, float32's own rounding of the operands would be the larger part, and
+// the operands are float32 in the same places: 8 products of 4 columns for 3 of 32, 0.45 us a stage for
+// 0.2, hidden by the launches (8 x 8 matrices 73 us for 63).
+//
+// A step is three launches that depend on each other, 7 to 8 us each where the products are small; all
+// of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16 products, where the library's float16 product
+// reaches 1.2 to 1.28.
 #include <float.h>
 #include <math.h>
 
@@ -28,11 +37,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kGroup = 32;    // matrices of one launch
 constexpr int kParts = 1024;  // partial sums of a matrix's squares, at most
-constexpr int kChunk = 32;    // columns of a 128-byte piece of a row: 32 hi, 32 lo
+constexpr int kChunk = 32;    // columns of a 128-byte piece of a row
 constexpr int64_t kMostBytes = (int64_t)2 << 30;  // of a group's operands
 
-// A matrix of split values: rows of `cols` logical columns (a multiple of the tile), each 128-byte
-// piece 32 columns' first terms, then their second terms.
+// An operand: rows of `cols` columns (a multiple of the tile), each 128-byte piece 32 columns, their
+// first terms and then their second terms, or as float32 (F32 below).
 struct Split {
     char *data;
     int cols;
@@ -40,25 +49,31 @@ struct Split {
 
 __host__ __device__ __forceinline__ int64_t row_bytes(int64_t cols) { return cols * 4; }
 
-__device__ __forceinline__ char *piece_of(const Split &s, int64_t row, int col) {
-    return s.data + row * row_bytes(s.cols) + (col & ~(kChunk - 1)) * 4 + (col & (kChunk - 1)) * 2;
-}
-
-// 8 values to the columns col .. col + 7 of a row.
-__device__ __forceinline__ void store_split(const Split &s, int64_t row, int col, const float *v) {
+// 8 values to the columns col .. col + 7 of a row; col is a multiple of 8.
+template <bool F32> __device__ __forceinline__ void store_split(const Split &s, int64_t row, int col, const float *v) {
+    char *p = s.data + row * row_bytes(s.cols) + (col & ~(kChunk - 1)) * 4;
+    if (F32) {
+        __builtin_memcpy(p + (col & (kChunk - 1)) * 4, v, 32);
+        return;
+    }
     f16x8 hi, lo;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         hi[j] = (_Float16)v[j];
         lo[j] = (_Float16)(v[j] - (float)hi[j]);
     }
-    char *p = piece_of(s, row, col);
+    p += (col & (kChunk - 1)) * 2;
     *reinterpret_cast<f16x8 *>(p) = hi;
     *reinterpret_cast<f16x8 *>(p + 64) = lo;
 }
 
-__device__ __forceinline__ void load_split(const Split &s, int64_t row, int col, float *v) {
-    const char *p = piece_of(s, row, col);
+template <bool F32> __device__ __forceinline__ void load_split(const Split &s, int64_t row, int col, float *v) {
+    const char *p = s.data + row * row_bytes(s.cols) + (col & ~(kChunk - 1)) * 4;
+    if (F32) {
+        __builtin_memcpy(v, p + (col & (kChunk - 1)) * 4, 32);
+        return;
+    }
+    p += (col & (kChunk - 1)) * 2;
     const f16x8 hi = *reinterpret_cast<const f16x8 *>(p), lo = *reinterpret_cast<const f16x8 *>(p + 64);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = (float)hi[j] + (float)lo[j];
@@ -170,6 +185,7 @@ template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squ
 }
 
 // U / (|U| + epsilon) times scale, split, in both orientations.  One workgroup a 64 x 64 tile of U.
+template <bool F32>
 __global__ void __launch_bounds__(256) ns_split(Source s, const double *partial, double epsilon, double scale,
                                                 Split by_rows, Split by_cols, int64_t step) {
     __shared__ __align__(16) float tile[64][68];
@@ -195,10 +211,10 @@ __global__ void __launch_bounds__(256) ns_split(Source s, const double *partial,
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[a][b + j];
-        store_split(by_rows, r0 + a, c0 + b, v);
+        store_split<F32>(by_rows, r0 + a, c0 + b, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[b + j][a];
-        store_split(by_cols, c0 + a, r0 + b, v);
+        store_split<F32>(by_cols, c0 + a, r0 + b, v);
     }
 }
 
@@ -248,6 +264,8 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
 }
 
+__device__ __forceinline__ f32x4 four(const f16x8 &v) { return __builtin_bit_cast(f32x4, v); }
+
 // The stored 16-byte piece of piece x of row r: rows of 128 bytes, 64 banks of 4.
 __device__ __forceinline__ int swizzle(int r, int x) { return x ^ ((r >> 1) & 7); }
 
@@ -290,7 +308,7 @@ template <bool SYM> __device__ __forceinline__ void tile_of(int t, int ni, int n
 
 // What a product makes of its tile S at (I, J): the next operand, in both orientations where mirror is
 // set, or the results.
-template <int T, Mode MODE>
+template <int T, Mode MODE, bool F32>
 __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, int J, bool mirror, float *S,
                                             int threads) {
     if constexpr (MODE == LAST) {
@@ -326,7 +344,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, i
         for (int i = threadIdx.x; i < T * T / 8; i += threads) {
             const int a = i / (T / 8), b = i % (T / 8) * 8;
             float v[8];
-            load_split(A, I + a, J + b, v);
+            load_split<F32>(A, I + a, J + b, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float &u = S[at_tile<T>(a, b + j)];
@@ -341,16 +359,16 @@ __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, i
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(a, b + j)];
-        store_split(out, I + a, J + b, v);
+        store_split<F32>(out, I + a, J + b, v);
         if (mirror) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = S[at_tile<T>(b + j, a)];
-            store_split(out_t, J + a, I + b, v);
+            store_split<F32>(out_t, J + a, I + b, v);
         }
     }
 }
 
-template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) ns_product(GemmArgs p) {
+template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>::THREADS) ns_product(GemmArgs p) {
     using C = Tile<T>;
     constexpr int F = C::F;
     __shared__ __align__(1024) char lds[C::BYTES];
@@ -373,7 +391,9 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
     tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
     const int I = ti * T, J = tj * T;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
-    f32x4 acc[F][F];
+    // of the pairs' first terms, and, where registers allow it, of the small products by themselves
+    constexpr bool APART = T == 64 && !F32;
+    f32x4 acc[F][F], low[APART ? F : 1][APART ? F : 1];
 
     if (w >= C::WAVES) {  // loads
         typedef __attribute__((address_space(1))) const void *gptr;
@@ -409,7 +429,10 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
 #pragma unroll
         for (int a = 0; a < F; ++a)
 #pragma unroll
-            for (int b = 0; b < F; ++b) acc[a][b] = zero4();
+            for (int b = 0; b < F; ++b) {
+                acc[a][b] = zero4();
+                if constexpr (APART) low[a][b] = zero4();
+            }
         for (int s = 0; s < stages; ++s) {
             __builtin_amdgcn_s_waitcnt(kWaitLds);  // stage s - 1 is read
             stage_barrier();
@@ -426,16 +449,33 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
                 const int row = wi + 16 * a + n;
                 const f16x8 lh = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g) * 16);
                 const f16x8 ll = *reinterpret_cast<const f16x8 *>(L + row * 128 + swizzle(row, g + 4) * 16);
+                if constexpr (F32) {
+                    // the same pieces hold 4 + 4 columns of float32
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int b = 0; b < F; ++b) {
+                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(four(lh)[e], four(rh[b])[e], acc[a][b],
+                                                                             0, 0, 0);
+                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(four(ll)[e], four(rl[b])[e], acc[a][b],
+                                                                             0, 0, 0);
+                        }
+                    continue;
+                }
                 // sums of different fragments between those of one
 #pragma unroll
                 for (int b = 0; b < F; ++b)
                     acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rh[b], acc[a][b], 0, 0, 0);
 #pragma unroll
-                for (int b = 0; b < F; ++b)
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[b], acc[a][b], 0, 0, 0);
+                for (int b = 0; b < F; ++b) {
+                    f32x4 &to = APART ? low[a][b] : acc[a][b];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(lh, rl[b], to, 0, 0, 0);
+                }
 #pragma unroll
-                for (int b = 0; b < F; ++b)
-                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[b], acc[a][b], 0, 0, 0);
+                for (int b = 0; b < F; ++b) {
+                    f32x4 &to = APART ? low[a][b] : acc[a][b];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(ll, rh[b], to, 0, 0, 0);
+                }
             }
         }
     }
@@ -449,8 +489,11 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
 #pragma unroll
             for (int b = 0; b < F; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    S[at_tile<T>(wi + 16 * a + 4 * (l >> 4) + i, wj + 16 * b + (l & 15))] = acc[a][b][i] * p.scale;
+                for (int i = 0; i < 4; ++i) {
+                    float v = acc[a][b][i];
+                    if constexpr (APART) v += low[a][b][i];
+                    S[at_tile<T>(wi + 16 * a + 4 * (l >> 4) + i, wj + 16 * b + (l & 15))] = v * p.scale;
+                }
     }
     __syncthreads();
     if (part) {
@@ -459,15 +502,15 @@ template <int T, Mode MODE> __global__ void __launch_bounds__(Tile<T>::THREADS) 
             to[i] = *reinterpret_cast<const float4 *>(S + at_tile<T>(i / (T / 4), i % (T / 4) * 4));
         return;
     }
-    finish_tile<T, MODE>(p, mat, I, J, !SYM || ti != tj, S, C::THREADS);
+    finish_tile<T, MODE, F32>(p, mat, I, J, !SYM || ti != tj, S, C::THREADS);
 }
 
-// The sums of the tiles that were made in parts, in order, a quarter of a tile each.
-template <Mode MODE> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) {
-    constexpr int T = 128, Q = 64;
+// The sums of the tiles that were made in parts, in order, 64 x 64 of a tile each.
+template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) {
+    constexpr int Q = 64, N = T / Q;
     __shared__ __align__(16) float S[Q * Q];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    const int n = blockIdx.x >> 2, qi = (blockIdx.x >> 1 & 1) * Q, qj = (blockIdx.x & 1) * Q;
+    const int n = blockIdx.x / (N * N), qi = blockIdx.x / N % N * Q, qj = blockIdx.x % N * Q;
     const int at = p.whole + n;
     int ti, tj;
     tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
@@ -483,13 +526,14 @@ template <Mode MODE> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) 
         *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) = sum;
     }
     __syncthreads();
-    finish_tile<Q, MODE>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, 256);
+    finish_tile<Q, MODE, F32>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, 256);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
 
 struct Plan {
     int tile[LAST + 1];
+    bool f32;                    // operands as float32
     int64_t m, n;                // padded
     int64_t x_bytes, xt_bytes, a_bytes;  // of one matrix: X, its transpose, A or B
     int64_t matrix_bytes;
@@ -518,9 +562,17 @@ struct Way {
                   // launch, from the figures at Tile; a part (64 KB) is written and read in 16 ns
 };
 
-Way way_of(int tile, int64_t tiles, int64_t stages) {
+Way way_of(int tile, int64_t tiles, int64_t stages, bool f32) {
     const int64_t turns = (tiles + 255) / 256;
-    if (tile == 64) return {64, 1, tiles, turns * (0.2 * stages + 1) + 5};
+    if (tile == 64) {
+        const double stage = f32 ? 0.45 : 0.2;
+        Way best = {64, 1, tiles, turns * (stage * stages + 1) + 5};
+        for (int parts = 2; parts <= 16 && tiles * parts <= kAtOnce && stages / parts >= 2; ++parts) {
+            const double time = (tiles * parts + 255) / 256 * (stage * ((stages + parts - 1) / parts) + 1) + 13;
+            if (time < best.time) best = {64, parts, 0, time};
+        }
+        return best;
+    }
     Way best = {128, 1, tiles, turns == 1 ? 0.65 * stages + 7 : turns * (0.6 * stages + 2) + 5};
     const int64_t whole = tiles / kAtOnce * kAtOnce, rest = tiles - whole;
     for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= 4; ++parts) {
@@ -540,6 +592,7 @@ Plan plan_of(const gdn2_matrices_shape *s) {
     double least = 0;
     for (int pad = 64; pad <= 128; pad += 64) {
         Plan p{};
+        p.f32 = m <= 64;
         p.m = padded(m, pad), p.n = padded(n, pad);
         double total = 0;
         for (int mode = GRAM; mode <= NEXT; ++mode) {
@@ -547,9 +600,9 @@ Plan plan_of(const gdn2_matrices_shape *s) {
             for (int i = 0; i < 2; ++i) {
                 const int64_t t = 64 << i, ti = p.m / t, tn = p.n / t;
                 time[i] = way_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
-                                 (mode == GRAM ? p.n : p.m) / kChunk).time;
+                                 (mode == GRAM ? p.n : p.m) / kChunk, p.f32).time;
             }
-            const bool large = pad == 128 && time[1] < time[0];
+            const bool large = pad == 128 && !p.f32 && time[1] < time[0];
             p.tile[mode] = large ? 128 : 64;
             total += time[large];
         }
@@ -575,7 +628,8 @@ constexpr size_t kPartialBytes = (size_t)kAtOnce * 128 * 128 * sizeof(float);
 
 size_t workspace_of(const Plan &p) {
     const bool large = p.tile[GRAM] == 128 || p.tile[POLY] == 128 || p.tile[NEXT] == 128;
-    return (size_t)p.group * p.matrix_bytes + (size_t)p.group * kParts * sizeof(double) + (large ? kPartialBytes : 0);
+    return (size_t)p.group * p.matrix_bytes + (size_t)p.group * kParts * sizeof(double) +
+           (large ? kPartialBytes : kPartialBytes / 4);
 }
 
 // The largest |a t + b t^3 + c t^5| for t in [0, s], and the largest |a + b u + c u^2| for u in [0, s^2].
@@ -623,14 +677,16 @@ int check_steps(int steps, const float *k, float epsilon) {
     return ok();
 }
 
-template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, int64_t rest, hipStream_t st) {
+template <int T, Mode MODE, bool F32> void launch_tiles(const GemmArgs &a, const Way &w, int64_t rest, hipStream_t st) {
     const dim3 grid((unsigned)(w.whole + rest * w.parts));
-    if (w.tile == 64) {
-        hipLaunchKernelGGL((ns_product<64, MODE>), grid, dim3(Tile<64>::THREADS), 0, st, a);
-        return;
-    }
-    hipLaunchKernelGGL((ns_product<128, MODE>), grid, dim3(Tile<128>::THREADS), 0, st, a);
-    if (rest) hipLaunchKernelGGL((ns_join<MODE>), dim3((unsigned)(4 * rest)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((ns_product<T, MODE, F32>), grid, dim3(Tile<T>::THREADS), 0, st, a);
+    if (rest) hipLaunchKernelGGL((ns_join<T, MODE, F32>), dim3((unsigned)(T / 64 * (T / 64) * rest)), dim3(256), 0, st, a);
+}
+
+template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, bool f32, int64_t rest, hipStream_t st) {
+    if (f32) launch_tiles<64, MODE, true>(a, w, rest, st);
+    else if (w.tile == 64) launch_tiles<64, MODE, false>(a, w, rest, st);
+    else launch_tiles<128, MODE, false>(a, w, rest, st);
 }
 
 // All products of one group of matrices; last holds the fields of the last product's results.
@@ -645,18 +701,21 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
         XT[i] = {X[i].data + p.x_bytes, (int)p.m};
     }
     const Split A = {ws + 2 * (p.x_bytes + p.xt_bytes), (int)p.m}, B = {A.data + p.a_bytes, (int)p.m};
-    double s = 1, sx = power_for(s);
+    // float32 operands need no powers
+    auto power = [&](double bound) { return p.f32 ? 1.0 : power_for(bound); };
+    double s = 1, sx = power(s);
     const dim3 parts(src.parts, count), threads(256);
     if (src.update) hipLaunchKernelGGL((ns_squares<float, true>), parts, threads, 0, st, src, partial);
     else if (src.bf16) hipLaunchKernelGGL((ns_squares<bf16_t, false>), parts, threads, 0, st, src, partial);
     else hipLaunchKernelGGL((ns_squares<float, false>), parts, threads, 0, st, src, partial);
     const int64_t pr = tall ? p.n : p.m, pc = tall ? p.m : p.n;
-    hipLaunchKernelGGL(ns_split, dim3((unsigned)(pr / 64 * (pc / 64)), count), dim3(256), 0, st, src,
-                       partial, (double)epsilon, sx, tall ? XT[0] : X[0], tall ? X[0] : XT[0], p.matrix_bytes);
+    hipLaunchKernelGGL((p.f32 ? ns_split<true> : ns_split<false>), dim3((unsigned)(pr / 64 * (pc / 64)), count),
+                       dim3(256), 0, st, src, partial, (double)epsilon, sx, tall ? XT[0] : X[0],
+                       tall ? X[0] : XT[0], p.matrix_bytes);
     for (int i = 0; i < steps; ++i) {
         const Split &x = X[i & 1], &xt = XT[i & 1];
         const Bounds b = bounds_of(k, s);
-        const double sa = power_for(s * s), sb = power_for(b.poly), next = b.x * 1.001;
+        const double sa = power(s * s), sb = power(b.poly), next = b.x * 1.001;
         GemmArgs g = last;
         g.partial = (float *)(partial + (size_t)p.group * kParts);
         g.l_step = g.r_step = g.out_step = p.matrix_bytes;
@@ -665,13 +724,13 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
             g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
             g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
             const int64_t tiles = (int64_t)g.tiles * count;
-            const Way w = way_of(t, tiles, g.k / kChunk);
+            const Way w = way_of(t, tiles, g.k / kChunk, p.f32);
             g.whole = (int)w.whole, g.parts = w.parts;
             switch (mode) {
-                case GRAM: launch_product<GRAM>(g, w, tiles - w.whole, st); break;
-                case POLY: launch_product<POLY>(g, w, tiles - w.whole, st); break;
-                case NEXT: launch_product<NEXT>(g, w, tiles - w.whole, st); break;
-                default: launch_product<LAST>(g, w, tiles - w.whole, st);
+                case GRAM: launch_product<GRAM>(g, w, p.f32, tiles - w.whole, st); break;
+                case POLY: launch_product<POLY>(g, w, p.f32, tiles - w.whole, st); break;
+                case NEXT: launch_product<NEXT>(g, w, p.f32, tiles - w.whole, st); break;
+                default: launch_product<LAST>(g, w, p.f32, tiles - w.whole, st);
             }
         };
         g.l = g.r = x, g.out = A;
@@ -682,7 +741,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
         g.scale = (float)(k[2] * sb / (sa * sa)), g.a = (float)(k[0] * sb), g.b = (float)(k[1] * sb / sa);
         run(POLY);
         g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
-        const double to = i + 1 < steps ? power_for(next) : 1;
+        const double to = i + 1 < steps ? power(next) : 1;
         g.scale = (float)(to / (sb * sx));
         run(i + 1 < steps ? NEXT : LAST);
         s = next, sx = to;

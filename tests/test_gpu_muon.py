@@ -76,6 +76,35 @@ def test_many(dk, count, rows, cols, dtype):
     check(u, dk.orthogonalize(dev(u, dtype)), dtype, every=40)
 
 
+@BOTH
+@pytest.mark.parametrize("count,rows,cols", [(1, 16, 2000), (3, 64, 3001), (2, 2500, 8), (1, 65, 3000), (2, 3000, 120),
+                                             (1, 1, 5000)])
+def test_long_sums(dk, count, rows, cols, dtype):
+    """Few tiles with long sums, which are made in parts; up to 64 rows the operands are float32."""
+    u = matrices(rows + cols, count, rows, cols, dtype)
+    check(u, dk.orthogonalize(dev(u, dtype)), dtype)
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 8), (8, 3000), (16, 2000), (40, 60), (64, 64), (64, 1000)])
+def test_small_matrices_are_float32_s(dk, rows, cols):
+    """Operands and sums of float32: over eight matrices the difference is no larger than that of the formulas in
+    float32 (numpy), whose operands are the same and whose sums are no shorter."""
+    u = matrices(rows, 8, rows, cols)
+    got = host(dk.orthogonalize(dev(u)))
+    own = plain = 0.0
+    for x, y in zip(u, got):
+        ref = ro.orthogonalize(x)
+        z = x.astype(np.float32)
+        z = z / (np.sqrt((z * z).sum()) + np.float32(1e-7))
+        a, b, c = (np.float32(k) for k in ro.COEFFICIENTS)
+        for _ in range(5):
+            gram = z @ z.T
+            z = a * z + (b * gram + c * (gram @ gram)) @ z
+        own += np.linalg.norm(y - ref) ** 2
+        plain += np.linalg.norm(z - ref) ** 2
+    assert own <= plain
+
+
 def test_a_large_matrix(dk):
     """1600 x 2100 has the large tiles' triangle with a rest on both sides."""
     u = matrices(5, 1, 1600, 2100)
