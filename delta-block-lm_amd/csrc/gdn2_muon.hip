@@ -13,12 +13,15 @@
 // product as hi hi + hi lo + lo hi into float32 accumulators, at a third of the matrix cores' float16
 // rate, where their float32 rate is a sixteenth.  float16's range is met by powers of two: the largest
 // singular values that X, A and B can have follow from the coefficients, no entry is larger, and the
-// powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Results are off by
-// half of what float32 products leave (512 x 1408 and larger); sums of a small tile have the small
-// products in accumulators of their own, so that a long sum is not rounded three times as often.  Where
-// the smaller side is at most 64, float32's own rounding of the operands would be the larger part, and
-// the operands are float32 in the same places: 8 products of 4 columns for 3 of 32, 0.45 us a stage for
-// 0.2, hidden by the launches (8 x 8 matrices 73 us for 63).
+// powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Tiles of 64 sum the
+// small products in accumulators of their own, so that a long sum is not rounded three times as often.
+// The polynomial is evaluated and the powers taken in 64 bits and rounded once.  Results are off by 0.4
+// to 0.8 of what float32 products leave, relative to their root mean square: 1.0e-6 for 2.3e-6 at
+// 512 x 512, 1.2e-6 for 3.3e-6 at 512 x 2816, 3.3e-6 for 4.7e-6 at 4096 x 4096.  Where the smaller side
+// is at most 64 the sums are short, and the rounding of operands and accumulators would be the larger
+// part (8.4e-7 for 7.0e-7 at 8 x 8): the operands are float32 in the same places and go through the
+// float64 matrix instructions, which leaves 2e-7 to 3.4e-7.  That takes about 0.85 us a stage for 0.2,
+// most of it hidden by the launches: 8 x 8 matrices 73 us for 63, 16 x 2000 138 us.
 //
 // A step is three launches that depend on each other, 7 to 8 us each where the products are small; all
 // of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16 products, where the library's float16 product
@@ -34,6 +37,7 @@ namespace gdn2 {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kGroup = 32;    // matrices of one launch
 constexpr int kParts = 1024;  // partial sums of a matrix's squares, at most
@@ -229,9 +233,9 @@ struct GemmArgs {
     int tiles_i, tiles_j, tiles;  // tiles of a matrix
     int whole, parts;          // tiles made at once; parts of the others' sums
     float *partial;            // [tile that is not whole][part][T][T]
-    int k;                     // columns of the operands
+    int k, stages;             // columns of the operands, and their chunks that are not padding
     float scale;               // of the accumulators
-    float a, b;                // POLY: of the identity and of A, in the result's scale
+    double a, b, c;            // POLY: of the identity, of A and of the accumulators, in the result's scale
     // LAST
     int rows, cols, tall, bf16, first;
     float decay, rate;         // update: param = decay param - rate result
@@ -346,10 +350,9 @@ __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, i
             float v[8];
             load_split<F32>(A, I + a, J + b, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 8; ++j) {  // rounded once
                 float &u = S[at_tile<T>(a, b + j)];
-                u += p.b * v[j];
-                if (I + a == J + b + j) u += p.a;
+                u = (float)(p.c * u + p.b * v[j] + (I + a == J + b + j ? p.a : 0.0));
             }
         }
         __syncthreads();
@@ -379,7 +382,7 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
     const int first = part ? p.whole : 0, b = blockIdx.x - first;
     const int total = part ? (int)gridDim.x - p.whole : p.whole, x = b & 7, full = total >> 3, more = total & 7;
     const int piece = (b >> 3) + x * full + min(x, more);
-    int at = piece, stages = p.k / kChunk, from = 0;
+    int at = piece, stages = p.stages, from = 0;
     if (part) {
         const int n = piece % p.parts;
         at = p.whole + piece / p.parts;
@@ -391,9 +394,11 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
     tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
     const int I = ti * T, J = tj * T;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
-    // of the pairs' first terms, and, where registers allow it, of the small products by themselves
+    // of the pairs' first terms, and, where registers allow it, of the small products by themselves; a float64
+    // accumulator i of a lane is of row 4 i + lane / 16, a float32 one of row 4 (lane / 16) + i
     constexpr bool APART = T == 64 && !F32;
     f32x4 acc[F][F], low[APART ? F : 1][APART ? F : 1];
+    f64x4 sum[F32 ? F : 1][F32 ? F : 1];
 
     if (w >= C::WAVES) {  // loads
         typedef __attribute__((address_space(1))) const void *gptr;
@@ -432,6 +437,7 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
             for (int b = 0; b < F; ++b) {
                 acc[a][b] = zero4();
                 if constexpr (APART) low[a][b] = zero4();
+                if constexpr (F32) sum[a][b] = f64x4{0., 0., 0., 0.};
             }
         for (int s = 0; s < stages; ++s) {
             __builtin_amdgcn_s_waitcnt(kWaitLds);  // stage s - 1 is read
@@ -455,10 +461,10 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int b = 0; b < F; ++b) {
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(four(lh)[e], four(rh[b])[e], acc[a][b],
-                                                                             0, 0, 0);
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(four(ll)[e], four(rl[b])[e], acc[a][b],
-                                                                             0, 0, 0);
+                            sum[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(lh)[e], (double)four(rh[b])[e],
+                                                                             sum[a][b], 0, 0, 0);
+                            sum[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(ll)[e], (double)four(rl[b])[e],
+                                                                             sum[a][b], 0, 0, 0);
                         }
                     continue;
                 }
@@ -490,9 +496,11 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
             for (int b = 0; b < F; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    int r = 4 * (l >> 4) + i;
                     float v = acc[a][b][i];
                     if constexpr (APART) v += low[a][b][i];
-                    S[at_tile<T>(wi + 16 * a + 4 * (l >> 4) + i, wj + 16 * b + (l & 15))] = v * p.scale;
+                    if constexpr (F32) r = 4 * i + (l >> 4), v = (float)sum[a][b][i];
+                    S[at_tile<T>(wi + 16 * a + r, wj + 16 * b + (l & 15))] = v * p.scale;
                 }
     }
     __syncthreads();
@@ -517,13 +525,14 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(256) ns_
     const float *from = p.partial + (int64_t)n * p.parts * T * T + qi * T + qj;
     for (int i = threadIdx.x; i < Q * Q / 4; i += 256) {
         const int a = i / (Q / 4), b = i % (Q / 4) * 4;
-        float4 sum = *reinterpret_cast<const float4 *>(from + a * T + b);
+        double sum[4] = {0, 0, 0, 0};
 #pragma unroll 4
-        for (int k = 1; k < p.parts; ++k) {
+        for (int k = 0; k < p.parts; ++k) {
             const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)k * T * T + a * T + b);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
         }
-        *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) = sum;
+        *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) =
+            make_float4((float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]);
     }
     __syncthreads();
     finish_tile<Q, MODE, F32>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, 256);
@@ -565,7 +574,7 @@ struct Way {
 Way way_of(int tile, int64_t tiles, int64_t stages, bool f32) {
     const int64_t turns = (tiles + 255) / 256;
     if (tile == 64) {
-        const double stage = f32 ? 0.45 : 0.2;
+        const double stage = f32 ? 0.85 : 0.2;
         Way best = {64, 1, tiles, turns * (stage * stages + 1) + 5};
         for (int parts = 2; parts <= 16 && tiles * parts <= kAtOnce && stages / parts >= 2; ++parts) {
             const double time = (tiles * parts + 255) / 256 * (stage * ((stages + parts - 1) / parts) + 1) + 13;
@@ -600,7 +609,7 @@ Plan plan_of(const gdn2_matrices_shape *s) {
             for (int i = 0; i < 2; ++i) {
                 const int64_t t = 64 << i, ti = p.m / t, tn = p.n / t;
                 time[i] = way_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
-                                 (mode == GRAM ? p.n : p.m) / kChunk, p.f32).time;
+                                 ((mode == GRAM ? n : m) + kChunk - 1) / kChunk, p.f32).time;
             }
             const bool large = pad == 128 && !p.f32 && time[1] < time[0];
             p.tile[mode] = large ? 128 : 64;
@@ -637,7 +646,7 @@ struct Bounds {
     double x, poly;
 };
 
-Bounds bounds_of(const float *k, double s) {
+Bounds bounds_of(const double *k, double s) {
     const double a = k[0], b = k[1], c = k[2];
     auto value = [&](double t) { return fabs(t * (a + t * t * (b + c * t * t))); };
     auto poly = [&](double u) { return fabs(a + u * (b + c * u)); };
@@ -663,7 +672,7 @@ double power_for(double bound) {
     return ldexp(1.0, 14 - e);
 }
 
-int check_steps(int steps, const float *k, float epsilon) {
+int check_steps(int steps, const double *k, float epsilon) {
     if (steps < 1 || steps > 100) return fail(GDN2_ERR_ARGUMENT, "steps must be 1 to 100");
     if (!k) return fail(GDN2_ERR_ARGUMENT, "coefficients is null");
     if (!(epsilon >= 0) || !(epsilon <= FLT_MAX)) return fail(GDN2_ERR_ARGUMENT, "epsilon must be >= 0 and finite");
@@ -690,7 +699,7 @@ template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, bool f
 }
 
 // All products of one group of matrices; last holds the fields of the last product's results.
-void run_group(const Plan &p, const Source &src, int count, int steps, const float *k, float epsilon,
+void run_group(const Plan &p, const Source &src, int count, int steps, const double *k, float epsilon,
                const GemmArgs &last, char *ws, hipStream_t st) {
     const bool tall = src.rows > src.cols;
     double *partial = (double *)(ws + (size_t)p.group * p.matrix_bytes);
@@ -703,6 +712,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
     const Split A = {ws + 2 * (p.x_bytes + p.xt_bytes), (int)p.m}, B = {A.data + p.a_bytes, (int)p.m};
     // float32 operands need no powers
     auto power = [&](double bound) { return p.f32 ? 1.0 : power_for(bound); };
+    auto chunks = [](int columns) { return (columns + kChunk - 1) / kChunk; };
     double s = 1, sx = power(s);
     const dim3 parts(src.parts, count), threads(256);
     if (src.update) hipLaunchKernelGGL((ns_squares<float, true>), parts, threads, 0, st, src, partial);
@@ -724,7 +734,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
             g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
             g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
             const int64_t tiles = (int64_t)g.tiles * count;
-            const Way w = way_of(t, tiles, g.k / kChunk, p.f32);
+            const Way w = way_of(t, tiles, g.stages, p.f32);
             g.whole = (int)w.whole, g.parts = w.parts;
             switch (mode) {
                 case GRAM: launch_product<GRAM>(g, w, p.f32, tiles - w.whole, st); break;
@@ -734,11 +744,11 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const flo
             }
         };
         g.l = g.r = x, g.out = A;
-        g.k = (int)p.n;
+        g.k = (int)p.n, g.stages = chunks(tall ? src.rows : src.cols);
         g.scale = (float)(sa / (sx * sx));
         run(GRAM);
-        g.l = g.r = A, g.out = B, g.k = (int)p.m;
-        g.scale = (float)(k[2] * sb / (sa * sa)), g.a = (float)(k[0] * sb), g.b = (float)(k[1] * sb / sa);
+        g.l = g.r = A, g.out = B, g.k = (int)p.m, g.stages = chunks(tall ? src.cols : src.rows);
+        g.scale = 1, g.a = k[0] * sb, g.b = k[1] * sb / sa, g.c = k[2] * sb / (sa * sa);
         run(POLY);
         g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
         const double to = i + 1 < steps ? power(next) : 1;
@@ -767,7 +777,7 @@ size_t gdn2_orthogonalize_workspace_bytes(const gdn2_matrices_shape *shape) {
 }
 
 int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, void *result, int steps,
-                       const float *coefficients, float epsilon, void *workspace, size_t workspace_bytes,
+                       const double *coefficients, float epsilon, void *workspace, size_t workspace_bytes,
                        void *stream) {
     GDN2_TRY(check_matrices(shape));
     GDN2_TRY(check_view(x, "x", -1, shape->count == 0));
@@ -794,7 +804,7 @@ int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, voi
 }
 
 int gdn2_muon_update(const gdn2_matrices_shape *shape, const gdn2_muon_tensor *tensors, float lr, float beta,
-                     int nesterov, float decay, int steps, const float *coefficients, float epsilon,
+                     int nesterov, float decay, int steps, const double *coefficients, float epsilon,
                      void *workspace, size_t workspace_bytes, void *stream) {
     GDN2_TRY(check_matrices(shape));
     GDN2_TRY(check_steps(steps, coefficients, epsilon));

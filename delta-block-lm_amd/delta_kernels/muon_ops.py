@@ -42,7 +42,7 @@ def _bytes(shape) -> int:
 def _coefficients(c) -> bytes:
     if len(c) != 3:
         raise ValueError("coefficients must be three numbers")
-    return struct.pack("3f", *c)
+    return struct.pack("3d", *c)
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
@@ -50,8 +50,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     """Newton-Schulz products of the matrices x [..., rows, cols], float32 or bfloat16, any strides:
         X = x / (|x| + epsilon), then `steps` times X <- a X + (b A + c A A) X with A = X X^T
     (for tall matrices the same from the right).  Returns the result in x's shape and dtype; products
-    keep 22 bits of their operands and sum in float32.  It has no gradient: where one is recorded, an
-    input that requires one is refused."""
+    keep 22 bits of their operands and sum in float32; of a side of at most 64, all bits and sums in
+    float64.  It has no gradient: where one is recorded, an input that requires one is refused."""
     code = _dtype(x, "x")
     if x.dim() < 2:
         raise ValueError("x must be [..., rows, cols]")

@@ -692,7 +692,8 @@ GDN2_API int gdn2_token_score_backward(int64_t rows, int64_t width, const gdn2_v
  *   X = U / (|U| + epsilon),  then `steps` times
  *   A = X X^T,  X <- (a I + b A + c A A) X        coefficients {a, b, c}
  * on the side with fewer rows (a tall matrix's transpose); |U| is the root of its sum of
- * squares, in 64 bits.  Products are of float16 pairs (22 bits of a value) summed in F32.
+ * squares, in 64 bits.  Products are of float16 pairs (22 bits of a value) summed in F32, or
+ * of F32 values summed in 64 bits where rows or cols is at most 64.
  * steps 1 to 100; coefficients under which values could grow past 1e9 are refused. */
 typedef struct gdn2_matrices_shape {
     int64_t count, rows, cols;
@@ -702,7 +703,7 @@ GDN2_API size_t gdn2_orthogonalize_workspace_bytes(const gdn2_matrices_shape *sh
 
 /* x: F32 or BF16 view, strides of [matrix, row, column]; result dense in x's dtype. */
 GDN2_API int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_view *x, void *result,
-                                int steps, const float *coefficients, float epsilon,
+                                int steps, const double *coefficients, float epsilon,
                                 void *workspace, size_t workspace_bytes, void *stream);
 
 /* The Muon update of `count` parameters of one shape (dense F32 each):
@@ -719,7 +720,7 @@ typedef struct gdn2_muon_tensor {
 
 GDN2_API int gdn2_muon_update(const gdn2_matrices_shape *shape, const gdn2_muon_tensor *tensors,
                               float lr, float beta, int nesterov, float decay, int steps,
-                              const float *coefficients, float epsilon, void *workspace,
+                              const double *coefficients, float epsilon, void *workspace,
                               size_t workspace_bytes, void *stream);
 
 /* Measurement hook.  No counterpart in the reference: it serves benchmarks

@@ -26,14 +26,14 @@ def view(dtype=0, data=0x1000, strides=(2400, 60, 1, 0)):
 
 
 def run(L, s=None, x=None, out=0x2000, steps=5, k=QUINTIC, eps=1e-7, ws=0x4000, n=1 << 40):
-    return L.gdn2_orthogonalize(s or shape(), x or view(), out, steps, None if k is None else struct.pack("3f", *k),
+    return L.gdn2_orthogonalize(s or shape(), x or view(), out, steps, None if k is None else struct.pack("3d", *k),
                                 ctypes.c_float(eps), ws, n, None)
 
 
 def update(L, s=None, table=(0x1000, 0x2000, 0x3000) * 2, steps=5, k=QUINTIC, ws=0x4000, n=1 << 40):
     f = ctypes.c_float
     return L.gdn2_muon_update(s or shape(), None if table is None else struct.pack(f"{len(table)}P", *table),
-                              f(0.1), f(0.95), 1, f(0), steps, struct.pack("3f", *k), f(1e-7), ws, n, None)
+                              f(0.1), f(0.95), 1, f(0), steps, struct.pack("3d", *k), f(1e-7), ws, n, None)
 
 
 def message(L):
