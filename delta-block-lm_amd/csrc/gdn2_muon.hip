@@ -13,19 +13,19 @@
 // product as hi hi + hi lo + lo hi into float32 accumulators, at a third of the matrix cores' float16
 // rate, where their float32 rate is a sixteenth.  float16's range is met by powers of two: the largest
 // singular values that X, A and B can have follow from the coefficients, no entry is larger, and the
-// powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Tiles of 64 sum the
-// small products in accumulators of their own, so that a long sum is not rounded three times as often.
+// powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Tiles up to 64 sum
+// the small products in accumulators of their own, so that a long sum is not rounded three times as often.
 // The polynomial is evaluated and the powers taken in 64 bits and rounded once.  Results are off by 0.4
 // to 0.8 of what float32 products leave, relative to their root mean square: 1.0e-6 for 2.3e-6 at
 // 512 x 512, 1.2e-6 for 3.3e-6 at 512 x 2816, 3.3e-6 for 4.7e-6 at 4096 x 4096.  Where the smaller side
 // is at most 64 the sums are short, and the rounding of operands and accumulators would be the larger
 // part (8.4e-7 for 7.0e-7 at 8 x 8): the operands are float32 in the same places and go through the
-// float64 matrix instructions, which leaves 2e-7 to 3.4e-7.  That takes about 0.85 us a stage for 0.2,
-// most of it hidden by the launches: 8 x 8 matrices 73 us for 63, 16 x 2000 138 us.
+// float64 matrix instructions, which leaves 2e-7 to 3.4e-7; a chunk of a 32 x 32 tile takes 0.25 us for
+// 0.115.
 //
-// A step is three launches that depend on each other, 7 to 8 us each where the products are small; all
-// of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16 products, where the library's float16 product
-// reaches 1.2 to 1.28.
+// A step is three launches that depend on each other: 2.4 to 4 us each for a matrix of 8 x 8 (55 us in
+// all, 5 steps), 6 to 7 at 512 x 512 (102 us); all of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16
+// products, where the library's float16 product reaches 1.2 to 1.28.
 #include <float.h>
 #include <math.h>
 
@@ -41,6 +41,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kGroup = 32;    // matrices of one launch
 constexpr int kParts = 1024;  // partial sums of a matrix's squares, at most
+constexpr int kSplitThreads = 512;
 constexpr int kChunk = 32;    // columns of a 128-byte piece of a row
 constexpr int64_t kMostBytes = (int64_t)2 << 30;  // of a group's operands
 
@@ -103,11 +104,6 @@ struct Source {
 };
 
 __device__ __forceinline__ float source_at(const Source &s, int mat, int64_t r, int64_t c) {
-    if (s.update) {
-        const int64_t i = r * s.cols + c;
-        const float m = s.t.momentum[mat][i];
-        return s.nesterov ? s.t.grad[mat][i] + s.beta * m : m;
-    }
     const int64_t i = (s.first + mat) * s.x.s0 + r * s.x.s1 + c * s.x.s2;
     return s.bf16 ? Elem<bf16_t>::load(s.x.data, i) : Elem<float>::load(s.x.data, i);
 }
@@ -137,6 +133,30 @@ template <typename T> __device__ __forceinline__ void store4(T *p, int n, const 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j < n) Elem<T>::store(p, j, v[j]);
+}
+
+// Values (r, c .. c + 3) of what is made orthogonal, zeros outside.
+__device__ __forceinline__ void source4(const Source &s, int mat, int64_t r, int64_t c, float *v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = 0.f;
+    if (r >= s.rows || c >= s.cols) return;
+    const int64_t i = r * s.cols + c, end = (r + 1) * s.cols;
+    if (s.update) {
+        load4(s.t.momentum[mat], i, end, v);
+        if (!s.nesterov) return;
+        float g[4];
+        load4(s.t.grad[mat], i, end, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = g[j] + s.beta * v[j];
+    } else if (s.dense) {
+        const int64_t at = (s.first + mat) * s.x.s0;
+        if (s.bf16) load4((const bf16_t *)s.x.data + at, i, end, v);
+        else load4((const float *)s.x.data + at, i, end, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < s.cols) v[j] = source_at(s, mat, r, c + j);
+    }
 }
 
 // Sums of squares in 64 bits: of a part of a dense matrix's values, or of every so-manieth row of
@@ -190,35 +210,46 @@ template <typename T, bool UPDATE> __global__ void __launch_bounds__(256) ns_squ
 
 // U / (|U| + epsilon) times scale, split, in both orientations.  One workgroup a 64 x 64 tile of U.
 template <bool F32>
-__global__ void __launch_bounds__(256) ns_split(Source s, const double *partial, double epsilon, double scale,
-                                                Split by_rows, Split by_cols, int64_t step) {
-    __shared__ __align__(16) float tile[64][68];
+__global__ void __launch_bounds__(kSplitThreads) ns_split(Source s, const double *partial, double epsilon,
+                                                          double scale, Split by_rows, Split by_cols, int64_t step) {
+    constexpr int N = 64 * 16 / kSplitThreads;  // fours of a thread
+    __shared__ float tile[64][65];  // by fours, by eights and down columns over all banks
+    __shared__ double red[kSplitThreads / 64];
     const int mat = blockIdx.y, across = by_rows.cols / 64;
     const int r0 = (int)(blockIdx.x / across) * 64, c0 = (int)(blockIdx.x % across) * 64;
     by_rows.data += mat * step, by_cols.data += mat * step;
-    __shared__ double red[4];
+    float v[N][4];  // on their way while the squares are summed
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = threadIdx.x + k * kSplitThreads;
+        source4(s, mat, r0 + (i >> 4), c0 + (i & 15) * 4, v[k]);
+    }
     double sum = 0;
-    for (int i = threadIdx.x; i < s.parts; i += 256) sum += partial[mat * kParts + i];
+    for (int i = threadIdx.x; i < s.parts; i += kSplitThreads) sum += partial[mat * kParts + i];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
     __syncthreads();
-    sum = (red[0] + red[1]) + (red[2] + red[3]);
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSplitThreads / 64; ++w) sum += red[w];
     const double by = scale / (sqrt(sum) + epsilon);
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        tile[r][c] = r0 + r < s.rows && c0 + c < s.cols ? (float)(source_at(s, mat, r0 + r, c0 + c) * by) : 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int i = threadIdx.x + k * kSplitThreads;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tile[i >> 4][(i & 15) * 4 + j] = (float)(v[k][j] * by);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    for (int i = threadIdx.x; i < 64 * 8; i += kSplitThreads) {
         const int a = i >> 3, b = (i & 7) * 8;
-        float v[8];
+        float w[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tile[a][b + j];
-        store_split<F32>(by_rows, r0 + a, c0 + b, v);
+        for (int j = 0; j < 8; ++j) w[j] = tile[a][b + j];
+        store_split<F32>(by_rows, r0 + a, c0 + b, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tile[b + j][a];
-        store_split<F32>(by_cols, c0 + a, r0 + b, v);
+        for (int j = 0; j < 8; ++j) w[j] = tile[b + j][a];
+        store_split<F32>(by_cols, c0 + a, r0 + b, w);
     }
 }
 
@@ -247,11 +278,13 @@ struct GemmArgs {
 // Tiles of a result.  Four waves multiply, four bring the operands to LDS (two waves do not issue the
 // loads as fast as a stage is used: 4096 x 4096 takes 3 % longer).  At 128 two workgroups share a CU, one
 // multiplies while the other waits: 0.6 us a stage of each, 0.65 alone; more stages and one workgroup are
-// 5 % slower.  At 64 a stage takes 0.2 us, however many workgroups there are: the L2's rate into LDS.
+// 5 % slower.  At 64 a stage takes 0.2 us, at 32 0.115: the L2's rate into LDS of a CU.  So where 64 leaves
+// CUs idle 32 spreads the same sums over four times as many: a product of 512 x 512 takes 6 to 7 us for 8,
+// all of it 106 us for 135; 8 of them 284 us for 207.
 template <int T> struct Tile {
     static constexpr int WAVES = 4, LOADS = 4, THREADS = 64 * (WAVES + LOADS);
     static constexpr int STAGE = 2 * T * 128;     // bytes: a chunk of T rows of both operands
-    static constexpr int STAGES = T == 128 ? 2 : 4;
+    static constexpr int STAGES = T == 128 ? 2 : T == 64 ? 4 : 8;
     static constexpr int OPS = STAGE / 1024 / LOADS;  // loads of a wave and stage
     static constexpr int BYTES = STAGES * STAGE;
     static constexpr int F = T / 32;              // 16-row fragments of a wave, 2 x 2 waves
@@ -396,7 +429,7 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     // of the pairs' first terms, and, where registers allow it, of the small products by themselves; a float64
     // accumulator i of a lane is of row 4 i + lane / 16, a float32 one of row 4 (lane / 16) + i
-    constexpr bool APART = T == 64 && !F32;
+    constexpr bool APART = T <= 64 && !F32;
     f32x4 acc[F][F], low[APART ? F : 1][APART ? F : 1];
     f64x4 sum[F32 ? F : 1][F32 ? F : 1];
 
@@ -513,9 +546,9 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
     finish_tile<T, MODE, F32>(p, mat, I, J, !SYM || ti != tj, S, C::THREADS);
 }
 
-// The sums of the tiles that were made in parts, in order, 64 x 64 of a tile each.
+// The sums of the tiles that were made in parts, in order, at most 64 x 64 of a tile each.
 template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) {
-    constexpr int Q = 64, N = T / Q;
+    constexpr int Q = T < 64 ? T : 64, N = T / Q;
     __shared__ __align__(16) float S[Q * Q];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     const int n = blockIdx.x / (N * N), qi = blockIdx.x / N % N * Q, qj = blockIdx.x % N * Q;
@@ -568,17 +601,19 @@ struct Way {
     int tile, parts;
     int64_t whole;
     double time;  // about, in us: a CU's tiles one after another, each with its stages and its result, and the
-                  // launch, from the figures at Tile; a part (64 KB) is written and read in 16 ns
+                  // launch, from the figures at Tile; a part of 64 KB is written and read in 16 ns
 };
 
 Way way_of(int tile, int64_t tiles, int64_t stages, bool f32) {
     const int64_t turns = (tiles + 255) / 256;
-    if (tile == 64) {
-        const double stage = f32 ? 0.85 : 0.2;
-        Way best = {64, 1, tiles, turns * (stage * stages + 1) + 5};
+    if (tile < 128) {
+        const double stage = f32 ? 0.25 : tile == 64 ? 0.2 : 0.115, result = tile == 64 ? 1 : 0.5;
+        const double part = tile == 64 ? 0.004 : 0.001;
+        Way best = {tile, 1, tiles, turns * (stage * stages + result) + 4};
         for (int parts = 2; parts <= 16 && tiles * parts <= kAtOnce && stages / parts >= 2; ++parts) {
-            const double time = (tiles * parts + 255) / 256 * (stage * ((stages + parts - 1) / parts) + 1) + 13;
-            if (time < best.time) best = {64, parts, 0, time};
+            const double time = (tiles * parts + 255) / 256 * (stage * ((stages + parts - 1) / parts) + result) +
+                                8.5 + part * tiles * parts;
+            if (time < best.time) best = {tile, parts, 0, time};
         }
         return best;
     }
@@ -593,7 +628,11 @@ Way way_of(int tile, int64_t tiles, int64_t stages, bool f32) {
     return best;
 }
 
-// Each product takes the tile that way_of prefers; sizes are padded to the larger of them.
+// Tiles of a result that hold rows and columns of the matrices; what lies behind them is never read as a
+// column of an operand.
+int tiles_of(int64_t n, int t) { return (int)((n + t - 1) / t); }
+
+// Each product takes the tile that way_of prefers; sizes are padded to 64 or to the larger tile.
 Plan plan_of(const gdn2_matrices_shape *s) {
     const int64_t m = s->rows < s->cols ? s->rows : s->cols, n = s->rows < s->cols ? s->cols : s->rows;
     const int64_t count = s->count < kGroup ? s->count : kGroup;
@@ -605,15 +644,13 @@ Plan plan_of(const gdn2_matrices_shape *s) {
         p.m = padded(m, pad), p.n = padded(n, pad);
         double total = 0;
         for (int mode = GRAM; mode <= NEXT; ++mode) {
-            double time[2];
-            for (int i = 0; i < 2; ++i) {
-                const int64_t t = 64 << i, ti = p.m / t, tn = p.n / t;
-                time[i] = way_of((int)t, count * (mode == NEXT ? ti * tn : ti * (ti + 1) / 2),
-                                 ((mode == GRAM ? n : m) + kChunk - 1) / kChunk, p.f32).time;
+            double time = 0;
+            for (int t = 32; t <= (p.f32 ? 32 : pad); t *= 2) {
+                const int64_t ti = tiles_of(m, t), tiles = mode == NEXT ? ti * tiles_of(n, t) : ti * (ti + 1) / 2;
+                const Way w = way_of(t, count * tiles, tiles_of(mode == GRAM ? n : m, kChunk), p.f32);
+                if (t == 32 || w.time < time) time = w.time, p.tile[mode] = t;
             }
-            const bool large = pad == 128 && !p.f32 && time[1] < time[0];
-            p.tile[mode] = large ? 128 : 64;
-            total += time[large];
+            total += time;
         }
         if (pad == 64 || total < least) best = p, least = total;
     }
@@ -689,11 +726,13 @@ int check_steps(int steps, const double *k, float epsilon) {
 template <int T, Mode MODE, bool F32> void launch_tiles(const GemmArgs &a, const Way &w, int64_t rest, hipStream_t st) {
     const dim3 grid((unsigned)(w.whole + rest * w.parts));
     hipLaunchKernelGGL((ns_product<T, MODE, F32>), grid, dim3(Tile<T>::THREADS), 0, st, a);
-    if (rest) hipLaunchKernelGGL((ns_join<T, MODE, F32>), dim3((unsigned)(T / 64 * (T / 64) * rest)), dim3(256), 0, st, a);
+    constexpr int N = T <= 64 ? 1 : T / 64;
+    if (rest) hipLaunchKernelGGL((ns_join<T, MODE, F32>), dim3((unsigned)(N * N * rest)), dim3(256), 0, st, a);
 }
 
 template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, bool f32, int64_t rest, hipStream_t st) {
-    if (f32) launch_tiles<64, MODE, true>(a, w, rest, st);
+    if (f32) launch_tiles<32, MODE, true>(a, w, rest, st);
+    else if (w.tile == 32) launch_tiles<32, MODE, false>(a, w, rest, st);
     else if (w.tile == 64) launch_tiles<64, MODE, false>(a, w, rest, st);
     else launch_tiles<128, MODE, false>(a, w, rest, st);
 }
@@ -712,7 +751,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
     const Split A = {ws + 2 * (p.x_bytes + p.xt_bytes), (int)p.m}, B = {A.data + p.a_bytes, (int)p.m};
     // float32 operands need no powers
     auto power = [&](double bound) { return p.f32 ? 1.0 : power_for(bound); };
-    auto chunks = [](int columns) { return (columns + kChunk - 1) / kChunk; };
+    const int m = tall ? src.cols : src.rows, n = tall ? src.rows : src.cols;
     double s = 1, sx = power(s);
     const dim3 parts(src.parts, count), threads(256);
     if (src.update) hipLaunchKernelGGL((ns_squares<float, true>), parts, threads, 0, st, src, partial);
@@ -720,7 +759,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
     else hipLaunchKernelGGL((ns_squares<float, false>), parts, threads, 0, st, src, partial);
     const int64_t pr = tall ? p.n : p.m, pc = tall ? p.m : p.n;
     hipLaunchKernelGGL((p.f32 ? ns_split<true> : ns_split<false>), dim3((unsigned)(pr / 64 * (pc / 64)), count),
-                       dim3(256), 0, st, src, partial, (double)epsilon, sx, tall ? XT[0] : X[0],
+                       dim3(kSplitThreads), 0, st, src, partial, (double)epsilon, sx, tall ? XT[0] : X[0],
                        tall ? X[0] : XT[0], p.matrix_bytes);
     for (int i = 0; i < steps; ++i) {
         const Split &x = X[i & 1], &xt = XT[i & 1];
@@ -730,7 +769,7 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
         g.partial = (float *)(partial + (size_t)p.group * kParts);
         g.l_step = g.r_step = g.out_step = p.matrix_bytes;
         auto run = [&](Mode mode) {
-            const int t = p.tile[mode], ti = (int)(p.m / t), tn = (int)(p.n / t);
+            const int t = p.tile[mode], ti = tiles_of(m, t), tn = tiles_of(n, t);
             g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
             g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
             const int64_t tiles = (int64_t)g.tiles * count;
@@ -744,10 +783,10 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
             }
         };
         g.l = g.r = x, g.out = A;
-        g.k = (int)p.n, g.stages = chunks(tall ? src.rows : src.cols);
+        g.k = (int)p.n, g.stages = tiles_of(n, kChunk);
         g.scale = (float)(sa / (sx * sx));
         run(GRAM);
-        g.l = g.r = A, g.out = B, g.k = (int)p.m, g.stages = chunks(tall ? src.cols : src.rows);
+        g.l = g.r = A, g.out = B, g.k = (int)p.m, g.stages = tiles_of(m, kChunk);
         g.scale = 1, g.a = k[0] * sb, g.b = k[1] * sb / sa, g.c = k[2] * sb / (sa * sa);
         run(POLY);
         g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
