@@ -546,29 +546,31 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
     finish_tile<T, MODE, F32>(p, mat, I, J, !SYM || ti != tj, S, C::THREADS);
 }
 
-// The sums of the tiles that were made in parts, in order, at most 64 x 64 of a tile each.
-template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(256) ns_join(GemmArgs p) {
-    constexpr int Q = T < 64 ? T : 64, N = T / Q;
+// The sums of the tiles that were made in parts, in order, at most 64 x 64 of a tile each, four values a
+// thread: a wave waits for its loads two times, not eight as with a quarter of the threads.
+constexpr int join_side(int tile) { return tile < 64 ? tile : 64; }
+constexpr int join_threads(int tile) { return join_side(tile) * join_side(tile) / 4; }
+
+template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(join_threads(T)) ns_join(GemmArgs p) {
+    constexpr int Q = join_side(T), N = T / Q, THREADS = join_threads(T);
     __shared__ __align__(16) float S[Q * Q];
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     const int n = blockIdx.x / (N * N), qi = blockIdx.x / N % N * Q, qj = blockIdx.x % N * Q;
     const int at = p.whole + n;
     int ti, tj;
     tile_of<SYM>(at % p.tiles, p.tiles_i, p.tiles_j, &ti, &tj);
-    const float *from = p.partial + (int64_t)n * p.parts * T * T + qi * T + qj;
-    for (int i = threadIdx.x; i < Q * Q / 4; i += 256) {
-        const int a = i / (Q / 4), b = i % (Q / 4) * 4;
-        double sum[4] = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int k = 0; k < p.parts; ++k) {
-            const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)k * T * T + a * T + b);
-            sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
-        }
-        *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) =
-            make_float4((float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]);
+    const int a = threadIdx.x / (Q / 4), b = threadIdx.x % (Q / 4) * 4;
+    const float *from = p.partial + (int64_t)n * p.parts * T * T + (qi + a) * T + qj + b;
+    double sum[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int k = 0; k < p.parts; ++k) {
+        const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)k * T * T);
+        sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
     }
+    *reinterpret_cast<float4 *>(S + at_tile<Q>(a, b)) =
+        make_float4((float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]);
     __syncthreads();
-    finish_tile<Q, MODE, F32>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, 256);
+    finish_tile<Q, MODE, F32>(p, at / p.tiles, ti * T + qi, tj * T + qj, !SYM || ti != tj, S, THREADS);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -596,7 +598,8 @@ int64_t padded(int64_t n, int64_t t) { return (n + t - 1) / t * t; }
 constexpr int kAtOnce = 512;  // workgroups of large tiles that the card holds
 
 // How the tiles of a product are made: those that fill the card once or more at once, the others, if it
-// pays, in parts of their sums that fill it once more, which another kernel joins.
+// pays, in parts of their sums that fill it once more, which another kernel joins.  Of several matrices all
+// tiles are made alike, so that equal matrices have equal results.
 struct Way {
     int tile, parts;
     int64_t whole;
@@ -604,28 +607,29 @@ struct Way {
                   // launch, from the figures at Tile; a part of 64 KB is written and read in 16 ns
 };
 
-Way way_of(int tile, int64_t tiles, int64_t stages, bool f32) {
-    const int64_t turns = (tiles + 255) / 256;
-    if (tile < 128) {
-        const double stage = f32 ? 0.25 : tile == 64 ? 0.2 : 0.115, result = tile == 64 ? 1 : 0.5;
-        const double part = tile == 64 ? 0.004 : 0.001;
-        Way best = {tile, 1, tiles, turns * (stage * stages + result) + 4};
-        for (int parts = 2; parts <= 16 && tiles * parts <= kAtOnce && stages / parts >= 2; ++parts) {
-            const double time = (tiles * parts + 255) / 256 * (stage * ((stages + parts - 1) / parts) + result) +
-                                8.5 + part * tiles * parts;
-            if (time < best.time) best = {tile, parts, 0, time};
+Way way_of(int tile, int64_t tiles, int64_t matrices, int64_t stages, bool f32) {
+    const bool small = tile < 128;
+    const double stage = f32 ? 0.25 : tile == 32 ? 0.115 : tile == 64 ? 0.2 : 0.6;
+    const double result = tile == 32 ? 0.5 : tile == 64 ? 1 : 2, part = tile == 32 ? 0.001 : tile == 64 ? 0.004 : 0.016;
+    const double launch = small ? 4 : 5, join = small ? 4.5 : 13;
+    // so many workgroups, one or, at 128, two to a CU at once
+    auto takes = [&](int64_t n, int64_t chunks) {
+        if (!small && n <= 256) return 0.65 * chunks + result;
+        return (double)((n + 255) / 256) * (stage * chunks + result);
+    };
+    tiles *= matrices;
+    Way best = {tile, 1, tiles, takes(tiles, stages) + launch};
+    // Small tiles all in parts or none: with a rest in parts 1600 x 2100 took 537 us for 509.
+    const int64_t most = !small && matrices == 1 ? tiles / kAtOnce * kAtOnce : 0;
+    for (int64_t whole = 0;; whole = most) {
+        const int64_t rest = tiles - whole;
+        for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= (small ? 2 : 4); ++parts) {
+            const double time = (whole ? takes(whole, stages) : 0) + takes(rest * parts, (stages + parts - 1) / parts) +
+                                launch + join + part * (double)(rest * parts);
+            if (time < best.time) best = {tile, parts, whole, time};
         }
-        return best;
+        if (whole == most) return best;
     }
-    Way best = {128, 1, tiles, turns == 1 ? 0.65 * stages + 7 : turns * (0.6 * stages + 2) + 5};
-    const int64_t whole = tiles / kAtOnce * kAtOnce, rest = tiles - whole;
-    for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= 4; ++parts) {
-        const int64_t each = (stages + parts - 1) / parts;
-        const double time = whole / 256 * (0.6 * stages + 2) + (rest * parts <= 256 ? 0.65 : 1.2) * each + 20 +
-                            0.016 * rest * parts;
-        if (time < best.time) best = {128, parts, whole, time};
-    }
-    return best;
 }
 
 // Tiles of a result that hold rows and columns of the matrices; what lies behind them is never read as a
@@ -647,7 +651,7 @@ Plan plan_of(const gdn2_matrices_shape *s) {
             double time = 0;
             for (int t = 32; t <= (p.f32 ? 32 : pad); t *= 2) {
                 const int64_t ti = tiles_of(m, t), tiles = mode == NEXT ? ti * tiles_of(n, t) : ti * (ti + 1) / 2;
-                const Way w = way_of(t, count * tiles, tiles_of(mode == GRAM ? n : m, kChunk), p.f32);
+                const Way w = way_of(t, tiles, count, tiles_of(mode == GRAM ? n : m, kChunk), p.f32);
                 if (t == 32 || w.time < time) time = w.time, p.tile[mode] = t;
             }
             total += time;
@@ -726,8 +730,9 @@ int check_steps(int steps, const double *k, float epsilon) {
 template <int T, Mode MODE, bool F32> void launch_tiles(const GemmArgs &a, const Way &w, int64_t rest, hipStream_t st) {
     const dim3 grid((unsigned)(w.whole + rest * w.parts));
     hipLaunchKernelGGL((ns_product<T, MODE, F32>), grid, dim3(Tile<T>::THREADS), 0, st, a);
-    constexpr int N = T <= 64 ? 1 : T / 64;
-    if (rest) hipLaunchKernelGGL((ns_join<T, MODE, F32>), dim3((unsigned)(N * N * rest)), dim3(256), 0, st, a);
+    constexpr int N = T / join_side(T);
+    if (rest)
+        hipLaunchKernelGGL((ns_join<T, MODE, F32>), dim3((unsigned)(N * N * rest)), dim3(join_threads(T)), 0, st, a);
 }
 
 template <Mode MODE> void launch_product(const GemmArgs &a, const Way &w, bool f32, int64_t rest, hipStream_t st) {
@@ -772,8 +777,10 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
             const int t = p.tile[mode], ti = tiles_of(m, t), tn = tiles_of(n, t);
             g.tiles_i = ti, g.tiles_j = mode >= NEXT ? tn : ti;
             g.tiles = mode >= NEXT ? ti * tn : ti * (ti + 1) / 2;
+            // as for a whole group, also where the last one has fewer matrices
+            Way w = way_of(t, g.tiles, p.group, g.stages, p.f32);
             const int64_t tiles = (int64_t)g.tiles * count;
-            const Way w = way_of(t, tiles, g.stages, p.f32);
+            if (p.group > 1) w.whole = w.parts > 1 ? 0 : tiles;
             g.whole = (int)w.whole, g.parts = w.parts;
             switch (mode) {
                 case GRAM: launch_product<GRAM>(g, w, p.f32, tiles - w.whole, st); break;

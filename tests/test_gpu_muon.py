@@ -116,6 +116,14 @@ def test_a_large_matrix(dk):
     assert torch.equal(out[0], out[3])
 
 
+@pytest.mark.parametrize("count,rows,cols", [(37, 20, 2500), (9, 130, 700), (35, 333, 90), (3, 1200, 1300)])
+def test_equal_matrices_have_equal_results(dk, count, rows, cols):
+    """Wherever they stand in a call, also behind the 32 of a launch, and whether or not sums are made in parts."""
+    u = dev(matrices(rows, 1, rows, cols)).expand(count, rows, cols)
+    out = dk.orthogonalize(u)
+    assert torch.equal(out, out[:1].expand_as(out))
+
+
 def test_spectrum(dk):
     u = matrices(6, 1, 96, 160)
     s = np.linalg.svd(host(dk.orthogonalize(dev(u)))[0], compute_uv=False)
