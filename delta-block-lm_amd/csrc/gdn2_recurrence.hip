@@ -720,7 +720,7 @@ int check_buffer(const char *name, const void *p, size_t have, size_t need) {
 
 int grid_of(const RecArgs &a, int segments, unsigned *out) {
     const int64_t n = (int64_t)a.slabs * a.B * segments;
-    if (n > 0x7FFFFFFF) return fail(GDN2_ERR_SHAPE, "too many sequences or channels");
+    if (n * 64 * a.waves > 0xFFFFFFFFll) return fail(GDN2_ERR_SHAPE, "too many sequences or channels for one launch");
     *out = (unsigned)n;
     return ok();
 }

@@ -477,7 +477,9 @@ int check_score(int64_t rows, int64_t width, const gdn2_view *x, const int64_t *
                 int64_t target_stride, const float *valid, int64_t valid_stride, float temperature,
                 ScoreArgs *a) {
     if (rows < 0 || width < 1) return fail(GDN2_ERR_SHAPE, "rows must be >= 0 and width >= 1");
-    if (rows > 0x7FFFFFFF || width > 0x7FFFFFFF) return fail(GDN2_ERR_SHAPE, "at most 2^31 - 1 rows and columns");
+    // a workgroup of up to 256 threads a row, 2^32 - 1 threads a launch
+    if (rows >= 1 << 24 || width > 0x7FFFFFFF)
+        return fail(GDN2_ERR_SHAPE, "at most 2^24 - 1 rows and 2^31 - 1 columns");
     GDN2_TRY(check_view(x, "x", -1, rows == 0));
     if (rows && !target) return fail(GDN2_ERR_ARGUMENT, "target is null");
     if (target_stride < 0 || valid_stride < 0) return fail(GDN2_ERR_ARGUMENT, "negative stride");

@@ -149,7 +149,7 @@ class Muon(torch.optim.Optimizer):
                     st["momentum"] = torch.zeros_like(p)
                 shapes.setdefault((p.shape, p.device), []).append(p)
             for ps in shapes.values():
-                muon_update(ps, [p.grad for p in ps], [self.state[p]["momentum"] for p in ps],
+                muon_update(ps, [p.grad.contiguous() for p in ps], [self.state[p]["momentum"] for p in ps],
                             group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
                             group["steps"], group["coefficients"], group["epsilon"])
         return loss

@@ -99,6 +99,8 @@ def gated_recurrence_backward(x, g, valid, reset, initial, checkpoint, dy, d_fin
         raise ValueError(f"dy must have shape {shape} (got {tuple(dy.shape)})")
     if d_final_state is not None and d_final_state.shape != (B, W):
         raise ValueError(f"d_final_state must be [batch, width] (got {tuple(d_final_state.shape)})")
+    if checkpoint.dtype != torch.uint8 or not checkpoint.is_contiguous():
+        raise ValueError("checkpoint must be what the forward returned")
     _same_device(x, "dy d_final_state checkpoint", dy, d_final_state, checkpoint)
     if dy.dtype != x.dtype:
         dy = dy.to(x.dtype)

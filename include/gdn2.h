@@ -661,13 +661,13 @@ GDN2_API int gdn2_recurrence_step(const gdn2_recurrence_shape *shape, const gdn2
  *   the `top` largest x of a row (0 to 64, at most width), largest first, the lower
  *   index first among equal ones, NaN before all: top_tokens [rows, top] and their
  *   log p, top_log_probs [rows, top] (both may be NULL where top is 0)
- * target [rows] int64 and valid [rows] F32 0/1 or NULL, with element strides.  A row that
- * is not valid is not read and gives zeros.  A target outside [0, width) gives NaN, and
- * so does a row whose largest value is infinite or that holds a NaN; -inf is probability
- * 0.  temperature is positive.  stats [rows, 3] F32 is what the backward reads (may be
- * NULL).  The log probability and the entropy are made from a sum in 64 bits.  The
- * workspace (16-byte aligned) is for rows that are few and wide; the query gives 0 where
- * none is needed. */
+ * target [rows] int64 and valid [rows] F32 0/1 or NULL, with element strides; at most
+ * 2^24 - 1 rows.  A row that is not valid is not read and gives zeros.  A target outside
+ * [0, width) gives NaN, and so does a row whose largest value is infinite or that holds a
+ * NaN; -inf is probability 0.  temperature is positive.  stats [rows, 3] F32 is what the
+ * backward reads (may be NULL).  The log probability and the entropy are made from a sum
+ * in 64 bits.  The workspace (16-byte aligned) is for rows that are few and wide; the
+ * query gives 0 where none is needed. */
 GDN2_API size_t gdn2_token_score_workspace_bytes(int64_t rows, int64_t width, int32_t top);
 GDN2_API int gdn2_token_score_forward(int64_t rows, int64_t width, const gdn2_view *x,
                                       const int64_t *target, int64_t target_stride,

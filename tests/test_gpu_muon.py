@@ -264,6 +264,15 @@ def test_optimizer(dk):
         dk.Muon([torch.nn.Parameter(torch.zeros(4, device="cuda"))])
 
 
+def test_a_strided_gradient(dk):
+    u = matrices(21, 1, 24, 40)[0]
+    one, two = (torch.nn.Parameter(torch.zeros(24, 40, device="cuda")) for _ in range(2))
+    one.grad, two.grad = dev(u), dev(u.T.copy()).T
+    assert not two.grad.is_contiguous()
+    dk.Muon([one, two]).step()
+    assert torch.equal(one, two) and one.abs().max() > 0
+
+
 def test_same_bits_each_time_and_on_other_streams(dk):
     u = dev(matrices(15, 3, 150, 90, H), H)
     first = dk.orthogonalize(u)

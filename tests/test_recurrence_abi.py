@@ -40,6 +40,14 @@ def test_bad_shapes(L, sizes, text):
     assert L.gdn2_recurrence_workspace_bytes(shape(*sizes), 0) == 0
 
 
+def test_more_workgroups_than_a_launch_has(L):
+    for sizes in ((1 << 27, 1, 1), (1 << 24, 300, 32), (1 << 26, 2, 16)):
+        s = shape(*sizes)
+        assert scan(L, s) == 2 and "one launch" in message(L)
+        assert L.gdn2_recurrence_backward(s, view(), view(), None, None, 0x4000, 1 << 62, view(), None, 0x5000, 0x6000,
+                                          None, 0x7000, 1 << 62, None) == 2
+
+
 def test_bad_types(L):
     assert scan(L, x=view(2)) == 3 and "x:" in message(L)
     assert scan(L, g=view(2)) == 3 and "g:" in message(L)

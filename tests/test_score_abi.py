@@ -49,6 +49,11 @@ def test_refusals(L):
     assert backward(L, rows=0) == 0
 
 
+def test_more_rows_than_a_launch_has(L):
+    assert forward(L, rows=1 << 24, width=8) == 2 and "rows" in message(L)
+    assert backward(L, rows=1 << 24, width=8) == 2 and "rows" in message(L)
+
+
 def test_workspace(L):
     size = L.gdn2_token_score_workspace_bytes
     assert size(8192, 32768, 8) == 0 and size(8, 32768, 64) == 0 and size(65, 1 << 20, 8) == 0
