@@ -6,7 +6,7 @@
 //
 // A run of tokens acts on the state before it as S + A h, and joining two runs needs only their
 // (A, S): the time axis is split over lanes, waves, and, where there are few channels, workgroups.
-//   * A workgroup has 64 bytes of channels (32 bf16, 16 f32) and up to 8 waves; the two that share a
+//   * A workgroup has 64 bytes of channels (32 bf16, 16 f32) and 1 to 8 waves; the two that share a
 //     128-byte line go to one XCD, whose L2 reads it once (halves rather than lines: twice the
 //     workgroups, 306 us against 443 at 4 x 8192 tokens of 2048 channels, where lines have 128).  A lane
 //     has 8 bytes of channels of some tokens in a row, a wave 8 such runs for each of its 8 pieces, a
@@ -53,7 +53,9 @@ constexpr float kTiny = 0x1p-126f, kHuge = 0x1p127f;
 // A lane has 8 bytes of 8 tokens in bf16, of 4 in f32: with runs twice as long registers run out, with
 // half as many tokens a block's joining is half of its instructions (4 x 8192 tokens of 2048 channels,
 // bf16, forward and backward: 306 us, with runs of 4 tokens 362, with 4-byte pieces of 16 tokens 321).
-template <typename T> struct Cfg {
+// WAVES: those of a workgroup, at most.
+template <typename T, int W = kMaxWaves> struct Cfg {
+    static constexpr int WAVES = W;
     static constexpr int N = 8 / sizeof(T);               // channels of a lane
     static constexpr int L = sizeof(T) == 2 ? 8 : 4;      // tokens of a lane's run
     static constexpr int SLAB = kSlabBytes / sizeof(T);   // channels of a workgroup
@@ -343,11 +345,11 @@ __device__ __forceinline__ float start_of(const RecArgs &a, const Place &p, floa
 // What the waves tell each other of a block, twice: a wave that is a block ahead writes the other half.
 // Waves that the workgroup does not have let everything through and add nothing.
 template <typename C> struct Totals {
-    float half[2][kMaxWaves][C::SLAB], root[2][kMaxWaves][C::SLAB], sum[2][kMaxWaves][C::SLAB];
-    float in[kMaxWaves][C::SLAB];  // the state before each wave's tokens
+    float half[2][C::WAVES][C::SLAB], root[2][C::WAVES][C::SLAB], sum[2][C::WAVES][C::SLAB];
+    float in[C::WAVES][C::SLAB];  // the state before each wave's tokens
 
     __device__ __forceinline__ void clear() {
-        for (int i = threadIdx.x; i < 2 * kMaxWaves * C::SLAB; i += blockDim.x)
+        for (int i = threadIdx.x; i < 2 * C::WAVES * C::SLAB; i += blockDim.x)
             (&half[0][0][0])[i] = 0.f, (&root[0][0][0])[i] = 1.f, (&sum[0][0][0])[i] = 0.f;
     }
     __device__ __forceinline__ void put(int buf, const Place &p, const float *l, const float *s) {
@@ -362,15 +364,15 @@ template <typename C> struct Totals {
     // This lane's channel: the state before its wave's tokens to `in`, and past all waves.  UP: waves in
     // order, or from the last.  A state goes past a block in one step, by the sum of all logarithms.
     template <bool UP> __device__ __forceinline__ float pass(int buf, const Place &p, float state, float *all_out) {
-        float r[kMaxWaves], s[kMaxWaves], all = 0.f, total = 0.f, mine = state;
+        float r[C::WAVES], s[C::WAVES], all = 0.f, total = 0.f, mine = state;
 #pragma unroll
-        for (int k = 0; k < kMaxWaves; ++k) {
-            const int w = UP ? k : kMaxWaves - 1 - k;
+        for (int k = 0; k < C::WAVES; ++k) {
+            const int w = UP ? k : C::WAVES - 1 - k;
             r[k] = root[buf][w][p.ch], s[k] = sum[buf][w][p.ch], all += half[buf][w][p.ch];
         }
 #pragma unroll
-        for (int k = 0; k < kMaxWaves; ++k) {
-            const int w = UP ? k : kMaxWaves - 1 - k;
+        for (int k = 0; k < C::WAVES; ++k) {
+            const int w = UP ? k : C::WAVES - 1 - k;
             const float before = mine;
             mine = join_root(mine, r[k], s[k]);
             if (w == p.wave) in[p.wave][p.ch] = before;
@@ -477,9 +479,9 @@ __device__ __forceinline__ void forward_walk(const RecArgs &a, const Place &p, T
 }
 
 // CARRY: only the segment's decay and sum.
-template <typename T, typename G, bool WHOLE, bool CARRY>
-__global__ void __launch_bounds__(64 * kMaxWaves) rec_forward(RecArgs a) {
-    using C = Cfg<T>;
+template <typename T, typename G, bool WHOLE, bool CARRY, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) rec_forward(RecArgs a) {
+    using C = Cfg<T, WAVES>;
     __shared__ __align__(16) Totals<C> tot;
     const Place p = place<C, WHOLE>(a);
     if (CARRY && p.seg == a.segments - 1) return;  // nothing comes after it
@@ -608,9 +610,9 @@ __device__ __forceinline__ void backward_walk(const RecArgs &a, const Place &p, 
     }
 }
 
-template <typename T, typename G, bool WHOLE, bool CARRY>
-__global__ void __launch_bounds__(64 * kMaxWaves) rec_backward(RecArgs a) {
-    using C = Cfg<T>;
+template <typename T, typename G, bool WHOLE, bool CARRY, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) rec_backward(RecArgs a) {
+    using C = Cfg<T, WAVES>;
     __shared__ __align__(16) Totals<C> fwd, bwd;
     const Place p = place<C, WHOLE>(a);
     if (CARRY && p.seg == 0) return;  // nothing comes before it
@@ -648,6 +650,12 @@ struct Split {
 // Workgroups that fill the card.  Segments read the inputs twice, so they are taken only to come to one
 // workgroup a CU (64 x 2048 tokens of 256 channels, 512 workgroups: 150 us, in two segments 243; 4 x 8192
 // of 2048, 256 workgroups: 306, in two 405).
+//
+// Each has 8 waves where it has a CU to itself, 4 and 2 where two and four share one, which do not wait for
+// each other's barriers.  Forward and backward, in us, with 8, 4 and 2 waves: 256 workgroups (4 x 8192 of
+// 2048) 315, 392, 591; 320 (10 x 2048 of 1024) 130, 117, 171; 512 (16 x 4096 of 1024) 345, 291, 390; 1024
+// (64 x 2048 of 512) 364, 319, 304; f32, 504 (8 x 509 of 1001) 52, 44, 48; 1024 (8 x 2048 of 2048) 309, 286,
+// 271.
 constexpr int kWantedGroups = 256;
 
 int check_shape(const gdn2_recurrence_shape *s) {
@@ -665,11 +673,12 @@ Split split_of(const gdn2_recurrence_shape *s, int32_t dtype) {
     const bool bf = dtype == GDN2_BF16;
     const int slab = bf ? Cfg<bf16_t>::SLAB : Cfg<float>::SLAB, run = bf ? Cfg<bf16_t>::TOKENS : Cfg<float>::TOKENS;
     k.slabs = (int)((s->width + slab - 1) / slab);
+    const int64_t units = (int64_t)k.slabs * s->batch;
+    const int most = units <= kWantedGroups ? kMaxWaves : units < 4 * kWantedGroups ? 4 : 2;
     k.waves = 1;
-    while (k.waves < kMaxWaves && s->time > (int64_t)k.waves * run) k.waves *= 2;
+    while (k.waves < most && s->time > (int64_t)k.waves * run) k.waves *= 2;
     const int64_t bt = (int64_t)k.waves * run;
     k.blocks = (int)((s->time + bt - 1) / bt);
-    const int64_t units = (int64_t)k.slabs * s->batch;
     int64_t segs = units >= kWantedGroups ? 1 : (kWantedGroups + units - 1) / units;
     if (segs > k.blocks) segs = k.blocks;
     k.seg_blocks = (int)((k.blocks + segs - 1) / segs);
@@ -725,16 +734,19 @@ int grid_of(const RecArgs &a, int segments, unsigned *out) {
     return ok();
 }
 
+template <typename T, typename G, bool WHOLE, bool CARRY, int WAVES>
+void launch_kind(const RecArgs &a, bool backward, unsigned grid, hipStream_t st) {
+    const dim3 block(64 * a.waves);
+    if (backward) hipLaunchKernelGGL((rec_backward<T, G, WHOLE, CARRY, WAVES>), dim3(grid), block, 0, st, a);
+    else hipLaunchKernelGGL((rec_forward<T, G, WHOLE, CARRY, WAVES>), dim3(grid), block, 0, st, a);
+}
+
 template <typename T, typename G, bool WHOLE>
 void launch_rec(const RecArgs &a, bool backward, bool carry, unsigned grid, hipStream_t st) {
-    const dim3 block(64 * a.waves);
-    if (backward) {
-        if (carry) hipLaunchKernelGGL((rec_backward<T, G, WHOLE, true>), dim3(grid), block, 0, st, a);
-        else hipLaunchKernelGGL((rec_backward<T, G, WHOLE, false>), dim3(grid), block, 0, st, a);
-    } else {
-        if (carry) hipLaunchKernelGGL((rec_forward<T, G, WHOLE, true>), dim3(grid), block, 0, st, a);
-        else hipLaunchKernelGGL((rec_forward<T, G, WHOLE, false>), dim3(grid), block, 0, st, a);
-    }
+    if (carry) launch_kind<T, G, WHOLE, true, kMaxWaves>(a, backward, grid, st);
+    else if (a.waves > 4) launch_kind<T, G, WHOLE, false, kMaxWaves>(a, backward, grid, st);
+    else if (a.waves > 2) launch_kind<T, G, WHOLE, false, 4>(a, backward, grid, st);
+    else launch_kind<T, G, WHOLE, false, 2>(a, backward, grid, st);
 }
 
 template <bool WHOLE>
