@@ -15,6 +15,10 @@
 // bound that at least k values reach; the few that do are collected and ordered, equal ones by their
 // index.  Rows with values that are not finite, with too many values at the bound, or with fewer
 // than k that reach it are ordered by k searches for the next value instead.
+//
+// Both passes are bound by the bytes: 8192 rows of 32768, bf16, forward 99 us (5.4 TB/s), backward 190 (5.6).
+// Of 8 such rows the forward takes 11 us with 8 alternatives: the latency of reading the row, of its sums'
+// join and of the search for the bound.
 #include <float.h>
 #include <math.h>
 
@@ -50,6 +54,7 @@ struct ScoreArgs {
     const float *d_lp, *d_h;
     int64_t d_lp_s, d_h_s;
     void *dx;
+    bool past;     // dx goes past the caches
 };
 
 template <typename T> constexpr int kN = 16 / sizeof(T);
@@ -420,6 +425,13 @@ template <typename T, bool UNIT, bool TOP> __global__ void __launch_bounds__(256
 }
 
 constexpr int kBackThreads = 256;
+// A gradient larger than the last level of cache is written past it, where the logits stay for a while:
+// 8192 rows of 32768, bf16, backward 191 us for 200, forward and backward in turn 282 for 306, with a product
+// that reads the gradient behind it 541 for 541.  Of 64 MB the product finds it in the cache: 170 us, 179
+// if it was written past.
+constexpr int64_t kCache = (int64_t)256 << 20;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
 
 template <typename T, bool UNIT> __global__ void __launch_bounds__(kBackThreads) score_backward(ScoreArgs a) {
     constexpr int N = kN<T>;
@@ -463,7 +475,8 @@ template <typename T, bool UNIT> __global__ void __launch_bounds__(kBackThreads)
                     for (int j = 0; j < 4; ++j)
                         w[j] = (uint32_t)f32_to_bf16(o[2 * j]) | ((uint32_t)f32_to_bf16(o[2 * j + 1]) << 16);
                 }
-                __builtin_memcpy(out + ci, w, 16);
+                if (a.past) __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, (u32x4 *)(out + ci));
+                else __builtin_memcpy(out + ci, w, 16);
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j)
@@ -598,6 +611,7 @@ int gdn2_token_score_backward(int64_t rows, int64_t width, const gdn2_view *x, c
     a.d_lp = d_log_probs, a.d_lp_s = d_log_probs_stride;
     a.d_h = d_entropy, a.d_h_s = d_entropy_stride;
     a.dx = dx;
+    a.past = rows * width * (x->dtype == GDN2_BF16 ? 2 : 4) > kCache;
     const bool unit = a.cs == 1;
     hipStream_t st = (hipStream_t)stream;
     if (x->dtype == GDN2_BF16) unit ? launch_backward<bf16_t, true>(a, st) : launch_backward<bf16_t, false>(a, st);

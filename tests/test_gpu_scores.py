@@ -397,6 +397,21 @@ def test_offsets_beyond_32_bits(dk):
     assert not dx[:-3].any()
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(3000, 50001, H), (1400, 50003, F)])
+def test_a_gradient_larger_than_the_caches(dk, rows, width, dtype):
+    """The same bits as of its rows a hundred at a time."""
+    torch.manual_seed(5)
+    x = torch.randn(rows, width, device="cuda", dtype=dtype)
+    tokens = torch.randint(0, width, (rows,), device="cuda")
+    dl, dh = torch.randn(2, rows, device="cuda")
+    _, stats = dk.token_log_probs_forward(x, tokens)
+    dx = dk.token_log_probs_backward(x, tokens, None, 0.8, stats, dl, dh)
+    for i in range(0, rows, 100):
+        r = slice(i, i + 100)
+        part = dk.token_log_probs_backward(x[r], tokens[r], None, 0.8, stats[r].contiguous(), dl[r], dh[r])
+        assert torch.equal(dx[r], part)
+
+
 def test_same_bits_each_time_and_on_other_streams(dk):
     c = case(19, 9, 5001, H)
     c["x"][1] = 0
