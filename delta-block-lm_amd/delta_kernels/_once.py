@@ -23,11 +23,10 @@ def once(backward):
     """Decorates the backward of a torch.autograd.Function."""
     @functools.wraps(backward)
     def run(ctx, *upstream):
-        recorded = torch.is_grad_enabled()
+        if not torch.is_grad_enabled():
+            return backward(ctx, *upstream)
         with torch.no_grad():
             out = backward(ctx, *upstream)
-        if not recorded:
-            return out
         out = out if isinstance(out, tuple) else (out,)
         there = [g for g in out if g is not None]
         if not there:
