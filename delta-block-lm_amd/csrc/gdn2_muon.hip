@@ -20,11 +20,11 @@
 // 512 x 512, 1.2e-6 for 3.3e-6 at 512 x 2816, 3.3e-6 for 4.7e-6 at 4096 x 4096.  Where the smaller side
 // is at most 64 the sums are short, and the rounding of operands and accumulators would be the larger
 // part (8.4e-7 for 7.0e-7 at 8 x 8): the operands are float32 in the same places and go through the
-// float64 matrix instructions, which leaves 2e-7 to 3.4e-7; a chunk of a 32 x 32 tile takes 0.25 us for
+// float64 matrix instructions, which leaves 1.8e-7 to 2.6e-7; a chunk of a 32 x 32 tile takes 0.25 us for
 // 0.115.
 //
-// A step is three launches that depend on each other: 2.4 to 4 us each for a matrix of 8 x 8 (55 us in
-// all, 5 steps), 6 to 7 at 512 x 512 (102 us); all of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16
+// A step is three launches that depend on each other, two up to 32 rows, whose A is one tile: 2.4 to 4 us
+// each for a matrix of 8 x 8 (40 us in all, 5 steps), 6 to 7 at 512 x 512 (102 us); all of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16
 // products, where the library's float16 product reaches 1.2 to 1.28.
 #include <float.h>
 #include <math.h>
@@ -267,6 +267,7 @@ struct GemmArgs {
     int k, stages;             // columns of the operands, and their chunks that are not padding
     float scale;               // of the accumulators
     double a, b, c;            // POLY: of the identity, of A and of the accumulators, in the result's scale
+    int whole_poly;            // GRAM: A is one tile, whose polynomial is made at once
     // LAST
     int rows, cols, tall, bf16, first;
     float decay, rate;         // update: param = decay param - rate result
@@ -343,6 +344,37 @@ template <bool SYM> __device__ __forceinline__ void tile_of(int t, int ni, int n
     }
 }
 
+// The polynomial of a tile S that is all of A, in its place: sums in 64 bits, rounded once.  This saves a
+// launch of 3 us for 0.3 of work.
+template <int T> __device__ __forceinline__ void tile_poly(const GemmArgs &p, float *S, int threads) {
+    constexpr int MOST = 2;  // pairs of a thread
+    float v[MOST][2];
+#pragma unroll
+    for (int n = 0; n < MOST; ++n) {
+        const int i = threadIdx.x + n * threads, a = i / (T / 2), b = i % (T / 2) * 2;
+        if (i >= T * T / 2) break;
+        double u0 = 0, u1 = 0;
+#pragma unroll 8
+        for (int k = 0; k < T; ++k) {
+            const double l = S[at_tile<T>(a, k)];
+            const float *r = S + at_tile<T>(k, b);
+            u0 = fma(l, (double)r[0], u0), u1 = fma(l, (double)r[1], u1);
+        }
+        const float *m = S + at_tile<T>(a, b);
+        v[n][0] = (float)(p.c * u0 + p.b * m[0] + (a == b ? p.a : 0.0));
+        v[n][1] = (float)(p.c * u1 + p.b * m[1] + (a == b + 1 ? p.a : 0.0));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < MOST; ++n) {
+        const int i = threadIdx.x + n * threads, a = i / (T / 2), b = i % (T / 2) * 2;
+        if (i >= T * T / 2) break;
+        float *m = S + at_tile<T>(a, b);
+        m[0] = v[n][0], m[1] = v[n][1];
+    }
+    __syncthreads();
+}
+
 // What a product makes of its tile S at (I, J): the next operand, in both orientations where mirror is
 // set, or the results.
 template <int T, Mode MODE, bool F32>
@@ -389,6 +421,9 @@ __device__ __forceinline__ void finish_tile(const GemmArgs &p, int mat, int I, i
             }
         }
         __syncthreads();
+    }
+    if constexpr (MODE == GRAM && F32) {
+        if (p.whole_poly) tile_poly<T>(p, S, threads);
     }
     for (int i = threadIdx.x; i < T * T / 8; i += threads) {
         const int a = i / (T / 8), b = i % (T / 8) * 8;
@@ -789,13 +824,16 @@ void run_group(const Plan &p, const Source &src, int count, int steps, const dou
                 default: launch_product<LAST>(g, w, p.f32, tiles - w.whole, st);
             }
         };
-        g.l = g.r = x, g.out = A;
+        // A of one tile: B at once
+        g.whole_poly = p.f32 && m <= 32;
+        g.a = k[0] * sb, g.b = k[1] * sb / sa, g.c = k[2] * sb / (sa * sa);
+        g.l = g.r = x, g.out = g.whole_poly ? B : A;
         g.k = (int)p.n, g.stages = tiles_of(n, kChunk);
         g.scale = (float)(sa / (sx * sx));
         run(GRAM);
         g.l = g.r = A, g.out = B, g.k = (int)p.m, g.stages = tiles_of(m, kChunk);
-        g.scale = 1, g.a = k[0] * sb, g.b = k[1] * sb / sa, g.c = k[2] * sb / (sa * sa);
-        run(POLY);
+        g.scale = 1;
+        if (!g.whole_poly) run(POLY);
         g.l = B, g.r = xt, g.out = X[1 - (i & 1)], g.out_t = XT[1 - (i & 1)];
         const double to = i + 1 < steps ? power(next) : 1;
         g.scale = (float)(to / (sb * sx));
