@@ -108,6 +108,14 @@ def test_segments(dk, B, T, W, types):
 
 
 @pytest.mark.parametrize("types", TYPES, ids=NAMES)
+@pytest.mark.parametrize("B,T,W", [(20, 600, 520), (33, 257, 510), (130, 300, 270), (600, 70, 40), (1100, 130, 5)])
+def test_workgroups_that_share_units(dk, B, T, W, types):
+    """Enough sequences and channels for workgroups of 4 and of 2 waves, over several blocks."""
+    c = inputs(T, B, T, W, types, masks=T != 300, initial=T != 600)
+    check(c, types, *run(dk, c, types))
+
+
+@pytest.mark.parametrize("types", TYPES, ids=NAMES)
 def test_many_channels(dk, types):
     c = inputs(3, 130, 300, 260, types, masks=True)  # one segment a sequence
     check(c, types, *run(dk, c, types))
