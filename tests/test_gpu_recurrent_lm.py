@@ -2,6 +2,7 @@
 import pytest
 
 torch = pytest.importorskip("torch")
+import torch.utils.checkpoint  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +160,42 @@ def test_a_training_step_of_all_operators(lm):
 def test_the_example_runs(lm, capsys):
     lm.main(steps=3)
     assert "the prompt" in capsys.readouterr().out
+
+
+def test_in_inference_mode(lm):
+    dk = lm.dk
+    with torch.inference_mode():
+        x, g = torch.randn(2, 3, 9, 40, device="cuda").unbind()
+        g = -g.abs()
+        y, fin = dk.gated_recurrence(x, g)
+        state = torch.zeros(3, 40, device="cuda")
+        one = torch.cat([dk.gated_recurrence_step(state, x[:, t:t + 1], g[:, t:t + 1]) for t in range(9)], 1)
+        assert torch.allclose(one, y, rtol=1e-5, atol=1e-6) and torch.allclose(state, fin, rtol=1e-5, atol=1e-6)
+        s = dk.token_log_probs(y, torch.zeros(3, 9, device="cuda", dtype=torch.int64), 2)
+        assert torch.allclose(s.log_probs, torch.log_softmax(y, -1)[..., 0], rtol=1e-5, atol=1e-5)
+        p, m = torch.zeros(2, 20, 30, device="cuda").unbind()
+        u = torch.randn(20, 30, device="cuda")
+        dk.muon_update(p, u, m, 1.0, nesterov=False)
+        assert torch.equal(m, u) and torch.equal(p, -dk.orthogonalize(u))
+
+
+def test_saved_tensors_moved_and_blocks_made_again(lm):
+    """The same gradients where autograd keeps what is saved elsewhere, or runs the forward again."""
+    dk = lm.dk
+    torch.manual_seed(2)
+    x, g = torch.randn(2, 3, 600, 40, device="cuda").unbind()
+    x, g = x.requires_grad_(True), (-g.abs()).detach().requires_grad_(True)
+    tokens = torch.randint(0, 40, (3, 600), device="cuda")
+
+    def loss(x, g):
+        y, fin = dk.gated_recurrence(x, g)
+        r = dk.token_log_probs(y, tokens)
+        return r.log_probs.sum() + 0.3 * r.entropy.sum() + fin.sum()
+
+    want = torch.autograd.grad(loss(x, g), (x, g))
+    with torch.autograd.graph.save_on_cpu():
+        moved = loss(x, g)
+    again = torch.utils.checkpoint.checkpoint(loss, x, g, use_reentrant=False)
+    for other in (moved, again):
+        for a, b in zip(want, torch.autograd.grad(other, (x, g))):
+            assert torch.equal(a, b)
