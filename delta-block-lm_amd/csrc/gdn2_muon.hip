@@ -703,9 +703,9 @@ Plan plan_of(const gdn2_matrices_shape *s) {
     return best;
 }
 
-// Parts of a matrix's squares: 4096 values each, as far as they go.
+// Parts of a matrix's squares: 1024 values each, as far as they go.
 int parts_of(const gdn2_matrices_shape *s) {
-    const int64_t n = (s->rows * s->cols + 4095) / 4096;
+    const int64_t n = (s->rows * s->cols + 1023) / 1024;
     return n > kParts ? kParts : (int)n;
 }
 
