@@ -700,6 +700,10 @@ size_t segment_bytes(const gdn2_recurrence_shape *s, const Split &k) {
     return k.segments > 1 ? 2 * k.segments * state_bytes(s) : 0;
 }
 
+size_t checkpoint_bytes_of(const gdn2_recurrence_shape *s, const Split &k, int train) {
+    return segment_bytes(s, k) + (train ? k.blocks * state_bytes(s) : 0);
+}
+
 int check_dtype(int32_t dtype) {
     if (dtype != GDN2_F32 && dtype != GDN2_BF16)
         return fail(GDN2_ERR_DTYPE, "dtype must be F32 or BF16 (got %d)", (int)dtype);
@@ -795,8 +799,7 @@ extern "C" {
 
 size_t gdn2_recurrence_checkpoint_bytes(const gdn2_recurrence_shape *shape, int32_t dtype, int train) {
     if (check_shape(shape) || check_dtype(dtype)) return 0;
-    const Split k = split_of(shape, dtype);
-    const size_t n = segment_bytes(shape, k) + (train ? k.blocks * state_bytes(shape) : 0);
+    const size_t n = checkpoint_bytes_of(shape, split_of(shape, dtype), train);
     return n ? n : 16;
 }
 
@@ -807,9 +810,8 @@ int gdn2_recurrence_scan(const gdn2_recurrence_shape *shape, const gdn2_view *x,
     GDN2_TRY(check_inputs(shape, x, g, valid, reset));
     if (initial) GDN2_TRY(check_view(initial, "initial", GDN2_F32, true));
     if (!output || !final_state) return fail(GDN2_ERR_ARGUMENT, "output and final_state must be non-null");
-    GDN2_TRY(check_buffer("checkpoint", checkpoint, checkpoint_bytes,
-                          gdn2_recurrence_checkpoint_bytes(shape, x->dtype, train)));
     const Split k = split_of(shape, x->dtype);
+    GDN2_TRY(check_buffer("checkpoint", checkpoint, checkpoint_bytes, checkpoint_bytes_of(shape, k, train)));
     RecArgs a = make_args(shape, k, x, g, valid, reset);
     a.initial = make_view(initial);
     a.y = output, a.final_state = final_state;
@@ -836,11 +838,9 @@ int gdn2_recurrence_backward(const gdn2_recurrence_shape *shape, const gdn2_view
                              void *stream) {
     GDN2_TRY(check_inputs(shape, x, g, valid, reset));
     GDN2_TRY(check_view(d_output, "d_output", x->dtype, false));
-    GDN2_TRY(check_buffer("checkpoint", checkpoint, checkpoint_bytes,
-                          gdn2_recurrence_checkpoint_bytes(shape, x->dtype, 1)));
-    GDN2_TRY(check_buffer("workspace", workspace, workspace_bytes,
-                          gdn2_recurrence_workspace_bytes(shape, x->dtype)));
     const Split k = split_of(shape, x->dtype);
+    GDN2_TRY(check_buffer("checkpoint", checkpoint, checkpoint_bytes, checkpoint_bytes_of(shape, k, 1)));
+    GDN2_TRY(check_buffer("workspace", workspace, workspace_bytes, segment_bytes(shape, k)));
     RecArgs a = make_args(shape, k, x, g, valid, reset);
     a.dy = make_view(d_output);
     a.d_final = d_final_state;

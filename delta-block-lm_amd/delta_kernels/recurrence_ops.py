@@ -72,9 +72,17 @@ def _bytes(query: str, shape, *args) -> int:
     return n
 
 
+def _scratch(n: int, shape, dev):
+    """Scratch of a query's n bytes.  16 where none is needed: two segments of a single value need as many,
+    those of more values more."""
+    if n == 16 and shape[0] * shape[2] > 1:
+        return None
+    return torch.empty((n,), dtype=torch.uint8, device=dev)
+
+
 def gated_recurrence_forward(x, g, valid=None, reset=None, initial=None, train: bool = True):
     """Raw forward.  Returns (y, final_state, checkpoint); the checkpoint is private storage for
-    gated_recurrence_backward, without train scratch alone."""
+    gated_recurrence_backward, without train scratch alone, or None where none is needed."""
     code, shape, views, held = _inputs(x, g, valid, reset, initial)
     if initial is not None and initial.dtype != F32:
         initial = initial.float()
@@ -82,9 +90,9 @@ def gated_recurrence_forward(x, g, valid=None, reset=None, initial=None, train: 
     n = _bytes("gdn2_recurrence_checkpoint_bytes", shape, code, train)
     y = torch.empty(shape, dtype=x.dtype, device=dev)
     final = torch.empty((shape[0], shape[2]), dtype=F32, device=dev)
-    ck = torch.empty((n,), dtype=torch.uint8, device=dev)
+    ck = torch.empty((n,), dtype=torch.uint8, device=dev) if train else _scratch(n, shape, dev)
     _call("gdn2_recurrence_scan", dev, _SHAPE(*shape), *views, _view(initial), y.data_ptr(),
-          final.data_ptr(), train, ck.data_ptr(), n)
+          final.data_ptr(), train, _ptr(ck), n)
     return y, final, ck
 
 
@@ -99,7 +107,7 @@ def gated_recurrence_backward(x, g, valid, reset, initial, checkpoint, dy, d_fin
         raise ValueError(f"dy must have shape {shape} (got {tuple(dy.shape)})")
     if d_final_state is not None and d_final_state.shape != (B, W):
         raise ValueError(f"d_final_state must be [batch, width] (got {tuple(d_final_state.shape)})")
-    if checkpoint.dtype != torch.uint8 or not checkpoint.is_contiguous():
+    if checkpoint is None or checkpoint.dtype != torch.uint8 or not checkpoint.is_contiguous():
         raise ValueError("checkpoint must be what the forward returned")
     _same_device(x, "dy d_final_state checkpoint", dy, d_final_state, checkpoint)
     if dy.dtype != x.dtype:
@@ -110,10 +118,10 @@ def gated_recurrence_backward(x, g, valid, reset, initial, checkpoint, dy, d_fin
     dg = torch.empty(shape, dtype=g.dtype, device=dev) if wanted[1] else None
     di = torch.empty((B, W), dtype=F32, device=dev) if wanted[2] and initial is not None else None
     n = _bytes("gdn2_recurrence_workspace_bytes", shape, code)
-    ws = torch.empty((n,), dtype=torch.uint8, device=dev)
+    ws = _scratch(n, shape, dev)
     _call("gdn2_recurrence_backward", dev, _SHAPE(*shape), *views, checkpoint.data_ptr(),
           checkpoint.numel(), _view(dy), _ptr(d_final_state), _ptr(dx), _ptr(dg), _ptr(di),
-          ws.data_ptr(), n)
+          _ptr(ws), n)
     return dx, dg, di
 
 

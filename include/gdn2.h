@@ -619,8 +619,9 @@ GDN2_API int gdn2_swiglu_q8_backward(int64_t rows, int64_t width, int32_t dtype,
  * token counts as 2^127.  initial [batch, width] F32 strided, or NULL (zero).  output
  * dense in x's dtype, final_state F32 dense; states and sums are F32.  The checkpoint
  * (16-byte aligned, sized by the query for x's dtype) holds a state for every block of
- * 32 to 256 tokens for the backward if train is nonzero, else scratch alone.  batch,
- * time, width and batch * width up to 2^30. */
+ * 32 to 512 tokens for the backward if train is nonzero, else scratch alone.  Buffers
+ * for scratch alone may be NULL where sequences are not cut into segments (the query
+ * gives 16).  batch, time, width and batch * width up to 2^30. */
 typedef struct gdn2_recurrence_shape {
     int64_t batch, time, width;
 } gdn2_recurrence_shape;

@@ -115,6 +115,17 @@ def test_workgroups_that_share_units(dk, B, T, W, types):
     check(c, types, *run(dk, c, types))
 
 
+@pytest.mark.parametrize("B,T,W", [(1, 1, 1), (1, 30, 1), (1, 300, 1), (1, 520, 1), (1, 600, 1), (1, 1100, 1),
+                                   (2, 600, 1), (1, 600, 2), (1, 20, 40), (300, 600, 33)])
+def test_smallest_buffers(dk, B, T, W):
+    for types in TYPES:
+        c = inputs(B + T, B, T, W, types, initial=True)
+        args = dev(c["x"], types[0]), dev(c["g"], types[1]), None, None, dev(c["initial"])
+        y, fin, _ = dk.gated_recurrence_forward(*args, train=False)
+        check(c, types, y, fin)
+        check(c, types, *run(dk, c, types))
+
+
 @pytest.mark.parametrize("types", TYPES, ids=NAMES)
 def test_many_channels(dk, types):
     c = inputs(3, 130, 300, 260, types, masks=True)  # one segment a sequence
@@ -457,6 +468,16 @@ def test_refusals(dk):
             dk.gated_recurrence_step(state, x[:, :1], x[:, :1])
     with pytest.raises(dk._lib.Gdn2Error, match="time == 1"):
         dk.gated_recurrence_step(torch.zeros((2, 4), device="cuda"), x, x)
+
+
+def test_other_checkpoints_are_refused(dk):
+    x = torch.zeros(2, 9, 40, device="cuda")
+    _, _, ck = dk.gated_recurrence_forward(x, x)
+    _, _, none = dk.gated_recurrence_forward(x, x, train=False)
+    for other in (none, ck.view(torch.float32), ck.new_zeros(1).expand(ck.numel())):
+        with pytest.raises(ValueError, match="checkpoint"):
+            dk.gated_recurrence_backward(x, x, None, None, None, other, x)
+    dk.gated_recurrence_backward(x, x, None, None, None, ck, x)
 
 
 def test_other_derivatives_are_refused(dk):

@@ -84,6 +84,17 @@ def test_sizes(L, T, W):
         assert 16 <= alone and 4 * W <= train <= alone + 4 * W * (T // 32 + 1)
 
 
+def test_buffers_that_nothing_needs_may_be_null(L):
+    """And are asked for where they are needed: the refusals come before any launch."""
+    for T, W in ((5000, 96), (600, 1)):
+        s, need = shape(2, T, W), L.gdn2_recurrence_workspace_bytes(shape(2, T, W), 0)
+        assert need > 16
+        assert L.gdn2_recurrence_scan(s, view(), view(), None, None, None, 0x2000, 0x3000, 0, None, 0, None) == 4
+    assert L.gdn2_recurrence_workspace_bytes(shape(1, 600, 1), 0) >= 16
+    assert L.gdn2_recurrence_scan(shape(1, 600, 1), view(), view(), None, None, None, 0x2000, 0x3000, 0, None, 0,
+                                  None) == 4
+
+
 def test_step_takes_one_token(L):
     step = L.gdn2_recurrence_step
     assert step(shape(), view(), view(), None, None, 0x2000, 0x3000, None) == 2 and "time == 1" in message(L)
