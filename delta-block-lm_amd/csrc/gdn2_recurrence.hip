@@ -20,7 +20,7 @@
 // The backward recomputes the states of a block from the state before it, which the forward kept
 // (4 bytes a channel for every block), and walks the blocks from the last.
 //
-// 4 x 8192 tokens of 2048 channels, bf16: forward 120 us, 3.4 TB/s, backward 197.  A block takes 25
+// 4 x 8192 tokens of 2048 channels, bf16: forward 122 us, 3.3 TB/s, backward 204.  A block takes 25
 // instructions a value, 10 of them the recurrence's own, at two waves a SIMD that wait for each other once
 // a block: 46 % of the time the vector units work.
 //
@@ -655,8 +655,8 @@ struct Split {
 };
 
 // Workgroups that fill the card.  Segments read the inputs twice, so they are taken only to come to one
-// workgroup a CU (64 x 2048 tokens of 256 channels, 512 workgroups: 150 us, in two segments 243; 4 x 8192
-// of 2048, 256 workgroups: 306, in two 405).
+// workgroup a CU (64 x 2048 tokens of 256 channels, 512 workgroups of 8 waves: 150 us, in two segments 243;
+// 4 x 8192 of 2048, 256 workgroups: 306, in two 405).
 //
 // Each has 8 waves where it has a CU to itself, 4 and 2 where two and four share one, which do not wait for
 // each other's barriers.  Forward and backward, in us, with 8, 4 and 2 waves: 256 workgroups (4 x 8192 of
