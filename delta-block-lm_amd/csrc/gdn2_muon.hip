@@ -24,8 +24,9 @@
 // 0.115.
 //
 // A step is three launches that depend on each other, two up to 32 rows, whose A is one tile: 2.4 to 4 us
-// each for a matrix of 8 x 8 (40 us in all, 5 steps), 6 to 7 at 512 x 512 (102 us); all of 4096 x 4096 is 3.5 ms, 1.17 PFLOP/s of float16
-// products, where the library's float16 product reaches 1.2 to 1.28.
+// each for a matrix of 8 x 8 (40 us in all, 5 steps), 6 to 7 at 512 x 512 (102 us), the same in a captured
+// graph; all of 4096 x 4096 is 3.4 to 3.5 ms, 1.17 to 1.2 PFLOP/s of float16 products, where the library's
+// float16 product reaches 1.2 to 1.28.
 #include <float.h>
 #include <math.h>
 
@@ -529,10 +530,11 @@ template <int T, Mode MODE, bool F32> __global__ void __launch_bounds__(Tile<T>:
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int b = 0; b < F; ++b) {
-                            sum[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(lh)[e], (double)four(rh[b])[e],
-                                                                             sum[a][b], 0, 0, 0);
-                            sum[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(ll)[e], (double)four(rl[b])[e],
-                                                                             sum[a][b], 0, 0, 0);
+                            f64x4 &to = sum[a][b];
+                            to = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(lh)[e], (double)four(rh[b])[e], to,
+                                                                      0, 0, 0);
+                            to = __builtin_amdgcn_mfma_f64_16x16x4f64((double)four(ll)[e], (double)four(rl[b])[e], to,
+                                                                      0, 0, 0);
                         }
                     continue;
                 }
@@ -658,7 +660,8 @@ Way way_of(int tile, int64_t tiles, int64_t matrices, int64_t stages, bool f32) 
     const int64_t most = !small && matrices == 1 ? tiles / kAtOnce * kAtOnce : 0;
     for (int64_t whole = 0;; whole = most) {
         const int64_t rest = tiles - whole;
-        for (int parts = 2; rest && parts <= 16 && rest * parts <= kAtOnce && stages / parts >= (small ? 2 : 4); ++parts) {
+        const int64_t most_parts = rest ? min(min((int64_t)16, kAtOnce / rest), stages / (small ? 2 : 4)) : 0;
+        for (int parts = 2; parts <= most_parts; ++parts) {
             const double time = (whole ? takes(whole, stages) : 0) + takes(rest * parts, (stages + parts - 1) / parts) +
                                 launch + join + part * (double)(rest * parts);
             if (time < best.time) best = {tile, parts, whole, time};

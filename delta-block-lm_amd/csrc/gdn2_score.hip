@@ -318,7 +318,8 @@ __device__ __forceinline__ bool skip_row(const ScoreArgs &a, int64_t r) {
     return true;
 }
 
-template <typename T, bool UNIT> __device__ __forceinline__ float given_logit(const ScoreArgs &a, const T *row, int64_t r) {
+template <typename T, bool UNIT>
+__device__ __forceinline__ float given_logit(const ScoreArgs &a, const T *row, int64_t r) {
     const int64_t label = a.target[r * a.ts];
     return label >= 0 && label < a.width ? Elem<T>::load(row, (UNIT ? 1 : a.cs) * label) : __builtin_nanf("");
 }
