@@ -442,10 +442,9 @@ template <typename T, bool UNIT> __global__ void __launch_bounds__(kBackThreads)
     const bool on = !a.valid || a.valid[r * a.vs] != 0.f;
     const float m = a.stats[3 * r], log_s = a.stats[3 * r + 1], H = a.stats[3 * r + 2];
     float dl = a.d_lp ? a.d_lp[r * a.d_lp_s] : 0.f;
-    const float dh = a.d_h ? a.d_h[r * a.d_h_s] * a.inv_t : 0.f;
+    const float dh = a.d_h ? a.d_h[r * a.d_h_s] : 0.f;
     const int64_t label = a.target[r * a.ts];
     if ((label < 0 || label >= a.width) && dl != 0.f) dl = __builtin_nanf("");
-    dl *= a.inv_t;
     const int64_t step = (int64_t)kBackThreads * N;
     for (int64_t c = ((int64_t)blockIdx.y * kUnroll * kBackThreads + threadIdx.x) * N; c < a.width;
          c += gridDim.y * kUnroll * step) {
@@ -462,9 +461,10 @@ template <typename T, bool UNIT> __global__ void __launch_bounds__(kBackThreads)
             for (int j = 0; j < N; ++j) {
                 const float lp = fmaxf((v[i][j] - m) * a.inv_t, kLowest) - log_s;
                 const float p = __expf(lp);
-                float d = p * (-dl - dh * (lp + H));
+                // p first: p (lp + H) is 0 where p is, and small elsewhere; 1 / temperature may be far larger
+                float d = -p * dl - dh * (p * (lp + H));
                 if (ci + j == label) d += dl;
-                o[j] = on ? d : 0.f;
+                o[j] = on ? d * a.inv_t : 0.f;
             }
             if (ci + N <= a.width) {
                 uint32_t w[4];
