@@ -272,8 +272,10 @@ __device__ void find_top(const ScoreArgs &a, const T *row, int64_t from, int64_t
     for (int d = 1; d < each; d *= 2) rank += __shfl_xor(rank, d);
     if (share == 0 && rank == a.top - 1) sh.bound = top;
     __syncthreads();  // maxima are read: their place is the list's
+    // -FLT_MAX, which a thread without a finite value has too, if fewer groups than that have a larger one: every
+    // thread lists its values then, so that of equal ones the first are found
     const float bound = sh.bound;
-    if (mine >= bound && mine > -FLT_MAX) {
+    if (mine >= bound) {
         const int64_t step = (int64_t)nt * N;
         for (int64_t c = from + (int64_t)i0 * N; c < to; c += kUnroll * step) {
             float v[kUnroll][N];
