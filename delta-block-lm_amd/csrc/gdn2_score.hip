@@ -9,7 +9,9 @@
 // One workgroup reads a row once: every thread keeps the maximum, s and the entropy's sum of its
 // columns, which are joined across the workgroup in a fixed order.  s is held in 64 bits: next to a
 // token of probability near 1 the others' sum is far below it, and their part is all that the log
-// probability and the entropy are made of.  -inf logits have probability 0 and take no part.
+// probability and the entropy are made of.  A thread adds its columns to it by 8 (f32) or 16 (bf16),
+// summed in 32 bits; those around such a token are summed again without it.  -inf logits have
+// probability 0 and take no part.
 //
 // The alternatives need no second sum over the row.  The k-th largest of the threads' maxima is a
 // bound that at least k values reach; the few that do are collected and ordered, equal ones by their
@@ -89,11 +91,14 @@ struct PartSums {
     float m, u;
 };
 
-// m: the maximum so far; s, u: the sums of e and of e (x - m) / temperature, e = exp of that.
+// m: the maximum so far; s, u: the sums of e and of e (x - m) / temperature, e = exp of that.  Of a thread also
+// the columns that brought its maximum, and what they added to s.
 struct Sums {
     float m;
     double s;
     float u;
+    int64_t at;
+    float s_at;
 };
 
 struct BlockShared {
@@ -124,7 +129,7 @@ __device__ Sums merge_block(const Sums &a, BlockShared &sh, float inv_t) {
         s = 0, u = 0;
         for (int w = 0; w < waves; ++w) s += sh.s[w], u += sh.u[w];
     }
-    return {M, s, u};
+    return {M, s, u, 0, 0.f};
 }
 
 // Columns from .. to of a row.
@@ -132,7 +137,7 @@ template <typename T, bool UNIT>
 __device__ __forceinline__ Sums sum_row(const ScoreArgs &a, const T *row, int64_t from, int64_t to) {
     constexpr int N = kN<T>;
     const float c2 = a.inv_t * 1.4426950408889634f;
-    Sums t = {-FLT_MAX, 0.0, 0.f};
+    Sums t = {-FLT_MAX, 0.0, 0.f, from, 0.f};
     float u2 = 0.f;  // the sum of e (x - m), before the temperature
     const int64_t step = (int64_t)blockDim.x * N;
     for (int64_t c = from + (int64_t)threadIdx.x * N; c < to; c += kUnroll * step) {
@@ -144,7 +149,8 @@ __device__ __forceinline__ Sums sum_row(const ScoreArgs &a, const T *row, int64_
         for (int i = 0; i < kUnroll; ++i)
 #pragma unroll
             for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[i][j]);
-        if (cm > t.m) {
+        const bool more = cm > t.m;
+        if (more) {
             const float d = fmaxf(t.m - cm, kLowest), e = __builtin_amdgcn_exp2f(d * c2);
             u2 = e * (u2 + (float)t.s * d);
             t.s *= e;
@@ -160,9 +166,36 @@ __device__ __forceinline__ Sums sum_row(const ScoreArgs &a, const T *row, int64_
                 u2 = fmaf(e, fmaxf(d, kLowest), u2);
             }
         t.s += s;
+        if (more) t.at = c, t.s_at = s;
     }
     t.u = u2 * a.inv_t;
     return t;
+}
+
+// A row, or a part of one, whose largest value is more than half of its sum: it is one value, and log s is
+// made of the others, of which a thread's float, with the 1 of the largest in it, keeps 24 bits of 1.  The same in
+// every thread.
+__device__ __forceinline__ bool is_sure(const Sums &t) { return t.s >= 1.0 && t.s < 2.0 && t.m > -FLT_MAX; }
+
+// The thread that has a sure row's largest value: s with the columns around it summed without the 1.  They are
+// read again, rather than kept by every thread or summed apart in every step.
+template <typename T, bool UNIT>
+__device__ double sure_sum(const ScoreArgs &a, const T *row, int64_t to, const Sums &mine, double s) {
+    constexpr int N = kN<T>;
+    const float c2 = a.inv_t * 1.4426950408889634f;
+    const int64_t step = (int64_t)blockDim.x * N;
+    float others = 0.f;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        float v[N];
+        load_cols<T, UNIT>(a, row, mine.at + i * step, to, v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float d = v[j] - mine.m;
+            others += d < 0.f ? __builtin_amdgcn_exp2f(d * c2) : 0.f;
+        }
+    }
+    return 1.0 + ((s - mine.s_at) + others);
 }
 
 // ---- order of values ------------------------------------------------------------------
@@ -326,14 +359,13 @@ __device__ __forceinline__ float given_logit(const ScoreArgs &a, const T *row, i
     return label >= 0 && label < a.width ? Elem<T>::load(row, (UNIT ? 1 : a.cs) * label) : __builtin_nanf("");
 }
 
-// The results of a row by its first wave; log s for the alternatives is read behind a barrier, or by
-// thread 0.
-template <bool TOP> __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t r, const Sums &t, float xl,
-                                                              TopShared &sh) {
-    if (threadIdx.x >= 64) return;
-    const double log_s = log(t.s);  // in 64 bits: 200 instructions, of one wave
-    if (threadIdx.x == 0) {
-        const float h = (float)(log_s - (double)t.u / t.s);
+// The results of a row by one thread, from its sums and s; log s for the alternatives is read behind a barrier.
+template <bool TOP> __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t r, const Sums &t, double s,
+                                                              float xl, TopShared &sh, bool writes) {
+    if (!__any(writes)) return;
+    const double log_s = log(s);  // in 64 bits: 200 instructions, of one wave
+    if (writes) {
+        const float h = (float)(log_s - (double)t.u / s);
         a.log_probs[r] = (float)((double)(xl - t.m) * a.inv_t - log_s);
         a.entropy[r] = h;
         if (a.stats) a.stats[3 * r] = t.m, a.stats[3 * r + 1] = (float)log_s, a.stats[3 * r + 2] = h;
@@ -351,7 +383,10 @@ __global__ void __launch_bounds__(kMaxThreads) score_forward(ScoreArgs a) {
     const float xl = given_logit<T, UNIT>(a, row, r);
     const Sums mine = sum_row<T, UNIT>(a, row, 0, a.width);
     const Sums t = merge_block(mine, red, a.inv_t);
-    write_row<TOP>(a, r, t, xl, sh);
+    const bool sure = is_sure(t), writes = sure ? mine.m == t.m : threadIdx.x == 0;
+    double s = t.s;
+    if (sure && writes) s = sure_sum<T, UNIT>(a, row, a.width, mine, s);
+    write_row<TOP>(a, r, t, s, xl, sh, writes);
     if constexpr (TOP) find_top<T, UNIT>(a, row, 0, a.width, mine.m, t.s, TopOut{r, t.m, nullptr}, sh);
 }
 
@@ -369,7 +404,9 @@ __global__ void __launch_bounds__(kMaxThreads) score_part(ScoreArgs a) {
     const T *row = (const T *)a.x + r * a.rs;
     const Sums mine = sum_row<T, UNIT>(a, row, from, to);
     const Sums t = merge_block(mine, red, a.inv_t);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = {t.s, t.m, t.u};
+    const bool sure = is_sure(t);
+    if (sure ? mine.m == t.m : threadIdx.x == 0)
+        a.part[blockIdx.x] = {sure ? sure_sum<T, UNIT>(a, row, to, mine, t.s) : t.s, t.m, t.u};
     if constexpr (TOP)
         find_top<T, UNIT>(a, row, from, to, mine.m, t.s, TopOut{r, t.m, a.part_top + (int64_t)blockIdx.x * a.top}, sh);
 }
@@ -398,13 +435,13 @@ template <typename T, bool UNIT, bool TOP> __global__ void __launch_bounds__(256
 #pragma unroll
     for (int k = 1; k < 64; k *= 2) M = fmaxf(M, __shfl_xor(M, k));
     const float d = fmaxf((q.m - M) * a.inv_t, kLowest), e = __expf(d);
-    Sums t = {M, q.s * e, e * (q.u + (float)q.s * d)};
+    Sums t = {M, q.s * e, e * (q.u + (float)q.s * d), 0, 0.f};
 #pragma unroll
     for (int k = 1; k < 64; k *= 2) {
         t.s += __shfl_xor(t.s, k), t.u += __shfl_xor(t.u, k);
         if (TOP) bound = min(bound, (uint64_t)__shfl_xor((unsigned long long)bound, k));
     }
-    write_row<TOP>(a, r, t, xl, sh);
+    write_row<TOP>(a, r, t, t.s, xl, sh, threadIdx.x == 0);
     if constexpr (TOP) {
         const int n = a.splits * a.top;
         if (threadIdx.x == 0) sh.count = 0;

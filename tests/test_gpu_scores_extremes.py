@@ -84,3 +84,42 @@ def test_rows_in_parts_masked_by_the_lowest_value(dk, top, dtype):  # noqa: F811
     c["t"][:4] = (60000, 101, 1, 37)
     c["x"] = rounded(c["x"], dtype)
     check(c, dtype, *run(dk, c, dtype, top))
+
+
+def sure(seed, width, dtype, gap, where):
+    """Two rows of a sure token at `where` and others at a distance of gap to gap + 4."""
+    r = np.random.default_rng(seed)
+    c = case(seed, 2, width, dtype)
+    c["x"] = rounded(-gap - 4 * r.random((2, width)), dtype)
+    c["t"] = np.array([where, where])
+    c["x"][:, where] = 0
+    return c
+
+
+@BOTH
+@pytest.mark.parametrize("gap", [8.0, 15.0, 17.0, 19.0, 25.0])
+@pytest.mark.parametrize("width", [2, 3, 4, 5, 8, 9, 16, 17, 31, 64, 1000, 10007, 70000])
+def test_the_others_of_a_sure_token(dk, width, gap, dtype):  # noqa: F811
+    """Log probability and entropy relative to what the others are, e_j = exp(-d_j) each, with E = 2^-24.  An
+    exponential is off by (2.3 d + 2.1) E of itself: the distance's, the factor log2 e's and the product's roundings,
+    and its own ulp.  A thread's sums of up to 16 floats add 16 E, up to two changes of its maximum and the row's
+    (2.3 d + 2.1) E each, of distances that add up to d: (3 d + 32) E of e_j.  The sums in 64 bits stand beside 1,
+    and have 2^-53 for each of up to 64 steps.  The entropy's own sum has the same terms, up to 32 roundings in a
+    thread and 6 + 16 across the workgroup: (3 d + 80) E of e_j d_j.  A result is rounded once, its sum from two
+    parts before."""
+    for where in sorted({0, width // 2, width - 1}):
+        c = sure(width, width, dtype, gap, where)
+        r, dx = run(dk, c, dtype, 1)
+        check(c, dtype, r, dx)
+        d = np.delete(-c["x"], where, 1)
+        e = np.exp(-d)
+        others = e.sum(1)
+        off = (e * (3 * d + 32)).sum(1) * E + 64 * 2.0 ** -53
+        want = -np.log1p(others)
+        err = np.abs(host(r.log_probs) - want)
+        assert np.all(err <= off + E * np.abs(want)), (where, err / (off + E * np.abs(want)))
+        assert torch.equal(r.top_log_probs[:, 0], r.log_probs)
+        h = np.log1p(others) + (e * d).sum(1) / (1 + others)
+        err = np.abs(host(r.entropy) - h)
+        bound = off + (e * d * (3 * d + 80)).sum(1) * E + 2 * E * h
+        assert np.all(err <= bound), (where, err / bound)
