@@ -15,6 +15,7 @@ reference; delta_mixers.model holds the gated-delta-rule model.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import List, Optional, Tuple
@@ -150,6 +151,18 @@ class LinearBlock(torch.nn.Module):
         return self._mlp(x + y.float())
 
 
+def scored(valid, present, reset):
+    """Which of tokens 1 .. T - 1 have a score, [B, T - 1] or None (all), from the masks [B, T] of score."""
+    if present is None and reset is None:
+        return None if valid is None else valid[:, 1:]
+    on = [] if valid is None else [valid[:, 1:] != 0]
+    if present is not None:
+        on += [present[:, 1:] != 0, present[:, :-1] != 0]
+    if reset is not None:
+        on.append(reset[:, 1:] == 0)
+    return functools.reduce(torch.logical_and, on)
+
+
 class LinearLM(torch.nn.Module):
     def __init__(self, cfg: LinearLMConfig, device=None):
         super().__init__()
@@ -182,11 +195,15 @@ class LinearLM(torch.nn.Module):
                                        self.embed.to(self.cfg.compute_dtype),
                                        tokens[:, 1:].reshape(-1))
 
-    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0) -> dk.TokenLogProbs:
+    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0, present=None,
+              reset=None) -> dk.TokenLogProbs:
         """Log probabilities of tokens 1 .. T - 1 after those before them, [B, T - 1], their entropy and
-        the top alternatives; zeros where valid [B, T] is 0."""
-        return dk.token_log_probs(self(tokens[:, :-1]), tokens[:, 1:], top,
-                                  None if valid is None else valid[:, 1:], temperature)
+        the top alternatives; zeros where valid [B, T] is 0.  valid says which tokens are scored, all are
+        read (a prompt, say); present [B, T], 0 at padding, and reset [B, T], 1 where a document begins,
+        are forward's valid and reset: a token is scored after the one right before it, so padding, what
+        follows it, and a document's first token give zeros."""
+        logits = self(tokens[:, :-1], *(None if m is None else m[:, :-1] for m in (present, reset)))
+        return dk.token_log_probs(logits, tokens[:, 1:], top, scored(valid, present, reset), temperature)
 
     @torch.no_grad()
     def prefill(self, tokens, states=None):

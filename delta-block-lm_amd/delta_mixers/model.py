@@ -303,7 +303,8 @@ class GdnLM(torch.nn.Module):
 
     def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0) -> dk.TokenLogProbs:
         """Log probabilities of tokens 1 .. T - 1 after those before them, [B, T - 1], their entropy and
-        the top alternatives; zeros where valid [B, T] is 0.  The reference's models give the loss alone."""
+        the top alternatives; zeros where valid [B, T] is 0 (which tokens are scored: all are read).  The
+        reference's models give the loss alone."""
         return dk.token_log_probs(self(tokens[:, :-1]), tokens[:, 1:], top,
                                   None if valid is None else valid[:, 1:], temperature)
 

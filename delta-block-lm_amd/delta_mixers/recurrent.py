@@ -23,7 +23,7 @@ import torch.nn.functional as F
 
 import delta_kernels as dk
 
-from .linear import LayerNorm, Q8SwiGLU, _linear, _mm
+from .linear import LayerNorm, Q8SwiGLU, _linear, _mm, scored
 
 
 @dataclass
@@ -119,17 +119,23 @@ class RecurrentLM(torch.nn.Module):
                                        self.embed.to(self.cfg.compute_dtype),
                                        tokens[:, 1:].reshape(-1))
 
-    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0) -> dk.TokenLogProbs:
+    def score(self, tokens, valid=None, top: int = 0, temperature: float = 1.0, present=None,
+              reset=None) -> dk.TokenLogProbs:
         """Log probabilities of tokens 1 .. T - 1 after those before them, [B, T - 1], their entropy and
-        the top alternatives; zeros where valid [B, T] is 0."""
-        return dk.token_log_probs(self(tokens[:, :-1]), tokens[:, 1:], top,
-                                  None if valid is None else valid[:, 1:], temperature)
+        the top alternatives; zeros where valid [B, T] is 0.  valid says which tokens are scored, all are
+        read (a prompt, say); present [B, T], 0 at padding, and reset [B, T], 1 where a document begins,
+        are forward's valid and reset: a token is scored after the one right before it, so padding, what
+        follows it, and a document's first token give zeros."""
+        logits = self(tokens[:, :-1], *(None if m is None else m[:, :-1] for m in (present, reset)))
+        return dk.token_log_probs(logits, tokens[:, 1:], top, scored(valid, present, reset), temperature)
 
-    def policy_loss(self, tokens, advantages, valid=None, entropy_weight: float = 0.0):
-        """Minus the mean over valid tokens 1 .. T - 1 of advantage times log probability, less
-        entropy_weight times their mean entropy; advantages [B, T - 1]."""
-        r = self.score(tokens, valid)
-        n = r.log_probs.numel() if valid is None else valid[:, 1:].sum().clamp(min=1)
+    def policy_loss(self, tokens, advantages, valid=None, entropy_weight: float = 0.0, present=None,
+                    reset=None):
+        """Minus the mean over the scored tokens of advantage times log probability, less entropy_weight
+        times their mean entropy; advantages [B, T - 1], the masks as for score."""
+        r = self.score(tokens, valid, present=present, reset=reset)
+        on = scored(valid, present, reset)
+        n = r.log_probs.numel() if on is None else on.sum().clamp(min=1)
         return -((advantages * r.log_probs).sum() + entropy_weight * r.entropy.sum()) / n
 
     @torch.no_grad()
