@@ -76,8 +76,15 @@ def _list(t: Tensors):
     return [t] if isinstance(t, torch.Tensor) else list(t)
 
 
-def _overlap(spans) -> bool:
-    spans = sorted(spans)
+def _overlap(written, read) -> bool:
+    """Whether of spans (begin, end) one that is written shares memory with another, of either kind."""
+    merged = []
+    for begin, end in sorted(read):  # those that are read may share it with each other
+        if merged and begin < merged[-1][1]:
+            merged[-1] = (merged[-1][0], max(end, merged[-1][1]))
+        else:
+            merged.append((begin, end))
+    spans = sorted(written + merged)
     return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
 
 
@@ -105,8 +112,8 @@ def muon_update(x: Tensors, g: Tensors, m: Tensors, lr: float, beta: float = 0.9
                 raise ValueError(f"{name} must have shape {tuple(shape)} on {dev} (got {tuple(t.shape)} on "
                                  f"{t.device})")
     size = 4 * shape[0] * shape[1]
-    gs = {t.data_ptr() for t in g}  # one gradient may serve several
-    if _overlap([(p, p + size) for p in [t.data_ptr() for t in x + m] + list(gs)]):
+    written, read = ([(t.data_ptr(), t.data_ptr() + size) for t in ts] for ts in (x + m, g))
+    if _overlap(written, read):
         raise ValueError("x and m may not share memory with each other or with g")
     full = (len(x),) + tuple(shape)
     n = _bytes(full)
