@@ -95,7 +95,8 @@ def muon_update(x: Tensors, g: Tensors, m: Tensors, lr: float, beta: float = 0.9
     sequence of them each.  In place:
         m = beta m + g;  u = g + beta m (nesterov), or m
         x = (1 - lr decay) x - lr sqrt(max(1, rows / cols)) orthogonalize(u)
-    x and m may not share memory with each other or with g."""
+    x and m may not share memory with each other or with g.  It has no gradient: where one is recorded, g
+    and m that require one are refused, and x that is not a leaf."""
     x, g, m = _list(x), _list(g), _list(m)
     if not len(x) == len(g) == len(m):
         raise ValueError("x, g and m must be equally many")
@@ -104,6 +105,8 @@ def muon_update(x: Tensors, g: Tensors, m: Tensors, lr: float, beta: float = 0.9
     shape, dev = x[0].shape, x[0].device
     if len(shape) != 2:
         raise ValueError(f"x must be [rows, cols] (got {tuple(shape)})")
+    if _wants_grad(*g, *m) or _wants_grad(*(t for t in x if not t.is_leaf)) or _has_tangent(*x, *g, *m):
+        raise ValueError("muon_update has no gradient: call it under torch.no_grad(), or on detached tensors")
     for name, ts in (("x", x), ("g", g), ("m", m)):
         for t in ts:
             if t.dtype != F32 or not t.is_contiguous() or not t.is_cuda:
