@@ -155,7 +155,8 @@ class RecurrentLM(torch.nn.Module):
 
 def make_optimizers(model, lr: float = 0.02, other_lr: float = 1e-3, weight_decay: float = 0.01):
     """(Muon for the blocks' projections, FusedAdamW for the rest): the embedding, which is the head too,
-    convolutions, norms and gates.  Any of the models here."""
+    convolutions, norms and gates.  Any of the models here.  A packed projection (u, r and gate; q, k, v and
+    what goes with them; w1 and w3) is one matrix, and orthogonalised as one."""
     matrices = [p for n, p in model.named_parameters()
                 if n.startswith("blocks.") and p.dim() == 2 and "conv" not in n]
     own = {id(p) for p in matrices}

@@ -45,3 +45,40 @@ def test_values_are_those_without_care():
     u, g, _ = m._split(x)
     uu = (x @ m.in_proj.t())[..., :40]
     assert torch.equal(u, torch.sqrt(-torch.expm1(2 * g)) * uu)
+
+
+def models(device=None):
+    from delta_mixers.linear import LinearLM, LinearLMConfig
+    from delta_mixers.model import GdnLM, GdnLMConfig
+    from delta_mixers.recurrent import RecurrentLM, RecurrentLMConfig
+    return [RecurrentLM(RecurrentLMConfig(vocab=64, d_model=64, layers=2, width=40, mlp_width=64), device),
+            LinearLM(LinearLMConfig(vocab=64, d_model=64, layers=2, heads=2, key_dim=16, value_dim=16, mlp_width=64),
+                     device),
+            GdnLM(GdnLMConfig(vocab=64, d_model=128, layers=2, heads=2, mlp_width=64), device)]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_what_muon_takes_of_the_models(which):
+    from delta_mixers.recurrent import make_optimizers
+    model = models()[which]
+    names = {id(p): n for n, p in model.named_parameters()}
+    muon, adamw = ({names[id(p)] for g in o.param_groups for p in g["params"]} for o in make_optimizers(model))
+    assert muon == {f"blocks.{i}.{n}" for i in range(2) for n in ("mixer.in_proj", "mixer.out", "mlp.w13", "mlp.w2")}
+    assert adamw == set(names.values()) - muon
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(3))
+def test_both_optimizers_train_each_model(which):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from delta_mixers.recurrent import make_optimizers, train_step
+    torch.manual_seed(0)
+    model = models("cuda")[which]
+    opts = make_optimizers(model)
+    tokens = torch.randint(0, 64, (4, 65), device="cuda")
+    before = {n: p.detach().clone() for n, p in model.named_parameters()}
+    for _ in range(2):
+        assert torch.isfinite(train_step(model, opts, lambda m: m.loss(tokens)))
+    for n, p in model.named_parameters():
+        assert torch.isfinite(p).all() and not torch.equal(p, before[n]), n
