@@ -9,9 +9,10 @@
 // orientations for that.  A and A A are symmetric: the tiles on and above the diagonal are made and
 // written twice.
 //
-// Precision.  An operand of a product goes in as two float16 terms, x = hi + lo, 23 bits, and a
-// product as hi hi + hi lo + lo hi into float32 accumulators, at a third of the matrix cores' float16
-// rate, where their float32 rate is a sixteenth.  float16's range is met by powers of two: the largest
+// Precision.  An operand of a product goes in as two float16 terms, x = hi + lo, 23 bits (off by
+// 2^-23 of itself), and a product as hi hi + hi lo + lo hi into float32 accumulators (lo lo, which is left
+// out, is 2^-22 of it at most), at a third of the matrix cores' float16 rate, where their float32 rate is
+// a sixteenth.  float16's range is met by powers of two: the largest
 // singular values that X, A and B can have follow from the coefficients, no entry is larger, and the
 // powers bring those to 2^14; what is below 2^-24 there is 2^-38 of the largest.  Tiles up to 64 sum
 // the small products in accumulators of their own, so that a long sum is not rounded three times as often.
@@ -641,7 +642,8 @@ struct Way {
     int tile, parts;
     int64_t whole;
     double time;  // about, in us: a CU's tiles one after another, each with its stages and its result, and the
-                  // launch, from the figures at Tile; a part of 64 KB is written and read in 16 ns
+                  // launch, from the figures at Tile; a part of 64 KB is written and read in 16 ns; a join has
+                  // its launch in it, and at 128 more than it takes with the threads it has now (7 to 8 and that)
 };
 
 Way way_of(int tile, int64_t tiles, int64_t matrices, int64_t stages, bool f32) {

@@ -50,8 +50,10 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     """Newton-Schulz products of the matrices x [..., rows, cols], float32 or bfloat16, any strides:
         X = x / (|x| + epsilon), then `steps` times X <- a X + (b A + c A A) X with A = X X^T
     (for tall matrices the same from the right).  Returns the result in x's shape and dtype; products
-    keep 22 bits of their operands and sum in float32; of a side of at most 64, all bits and sums in
-    float64.  It has no gradient: where one is recorded, an input that requires one is refused."""
+    keep 23 bits of their operands (and not the product of the lower halves, 2^-22 of theirs) and sum in
+    float32; of a side of at most 64, all bits and sums in float64.  It works in memory of its own: for each
+    matrix of a launch 16 to 24 bytes a value, the smaller side counted as 64 at least (1 x 2^24: 17 GB).  It
+    has no gradient: where one is recorded, an input that requires one is refused."""
     code = _dtype(x, "x")
     if x.dim() < 2:
         raise ValueError("x must be [..., rows, cols]")

@@ -693,8 +693,11 @@ GDN2_API int gdn2_token_score_backward(int64_t rows, int64_t width, const gdn2_v
  *   X = U / (|U| + epsilon),  then `steps` times
  *   A = X X^T,  X <- (a I + b A + c A A) X        coefficients {a, b, c}
  * on the side with fewer rows (a tall matrix's transpose); |U| is the root of its sum of
- * squares, in 64 bits.  Products are of float16 pairs (22 bits of a value) summed in F32, or
- * of F32 values summed in 64 bits where rows or cols is at most 64.
+ * squares, in 64 bits.  Products are of float16 pairs (23 bits of a value, without the
+ * product of their second terms) summed in F32, or of F32 values summed in 64 bits where rows
+ * or cols is at most 64.  The workspace holds, for each matrix of a launch (up to 32 and 2 GiB
+ * of them, one at least), twice X, its transpose and a matrix of the smaller side squared, 4
+ * bytes a value and both sides rounded up to 64 or 128: 17 GB for one of 1 x 2^24.
  * steps 1 to 100; coefficients under which values could grow past 1e9 are refused. */
 typedef struct gdn2_matrices_shape {
     int64_t count, rows, cols;
@@ -711,7 +714,8 @@ GDN2_API int gdn2_orthogonalize(const gdn2_matrices_shape *shape, const gdn2_vie
  *   momentum = beta momentum + grad
  *   U = grad + beta momentum if nesterov is nonzero, else momentum
  *   param = (1 - lr decay) param - lr sqrt(max(1, rows / cols)) orthogonalised(U)
- * No two params or momenta may share memory.  The workspace is gdn2_orthogonalize's;
+ * No param or momentum may share memory with another or with a grad; grads may with each
+ * other.  The workspace is gdn2_orthogonalize's;
  * tensors is read during the call. */
 typedef struct gdn2_muon_tensor {
     float *param;
