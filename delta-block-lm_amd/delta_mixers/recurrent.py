@@ -51,8 +51,11 @@ class RecurrentMixer(torch.nn.Module):
     def _split(self, x):
         u, r, gate = _mm(x, self.in_proj).chunk(3, -1)
         g = -2 * torch.sigmoid(r.float()) * F.softplus(self.decay)
-        # relu for its gradient: 0 where a gate is closed (g = 0), where the root's is infinite
-        return (torch.sqrt(F.relu(-torch.expm1(2 * g))) * u).to(x.dtype), g, gate
+        rest = -torch.expm1(2 * g)
+        if torch.is_grad_enabled():
+            # for the gradient alone: 0 where a gate is closed (g = 0), where the root's is infinite
+            rest = F.relu(rest)
+        return (torch.sqrt(rest) * u).to(x.dtype), g, gate
 
     def _join(self, h, gate):
         return _mm(h * F.silu(gate), self.out)

@@ -82,3 +82,11 @@ def test_both_optimizers_train_each_model(which):
         assert torch.isfinite(train_step(model, opts, lambda m: m.loss(tokens)))
     for n, p in model.named_parameters():
         assert torch.isfinite(p).all() and not torch.equal(p, before[n]), n
+
+
+def test_the_same_values_without_gradients():
+    m = mixer()
+    x = torch.tensor([-110.0, -3.0, 110.0, 0.0, 1.0, 0.2]).view(1, 6, 1) * torch.ones(3)
+    with torch.no_grad():
+        alone = m._split(x)
+    assert all(torch.equal(a, b) for a, b in zip(alone, m._split(x)))
