@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from gpu_util import dev, host  # noqa: E402
-from test_gpu_scores import BOTH, E, F, H, case, check, dk, rounded, run  # noqa: E402, F401
+from test_gpu_scores import BOTH, E, F, H, case, check, dk, layouts, rounded, run  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,25 @@ def test_the_others_of_a_sure_token(dk, width, gap, dtype):  # noqa: F811
         err = np.abs(host(r.entropy) - h)
         bound = off + (e * d * (3 * d + 80)).sum(1) * E + 2 * E * h
         assert np.all(err <= bound), (where, err / bound)
+
+
+@BOTH
+def test_sure_tokens_in_many_rows_and_other_layouts(dk, dtype):  # noqa: F811
+    """The same bits wherever the row stands, whether its columns lie side by side, and beside ruled-out ones."""
+    c = sure(41, 3000, dtype, 17.0, 1234)
+    two = dev(c["x"], dtype)
+    t = torch.full((514,), 1234, device="cuda")
+    x = torch.randn(514, 3000, device="cuda").to(dtype)
+    x[[0, 513]] = two
+    want = dk.token_log_probs(x, t, 2)
+    assert torch.all(want.log_probs[[0, 513]] < 0) and torch.all(want.log_probs[[0, 513]] > -1e-3)
+    for place in layouts():
+        got = dk.token_log_probs(place(x), t, 2)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    check(c, dtype, dk.TokenLogProbs(*(v[[0, 513]] for v in want)))
+    x[:, 2000:] = -np.inf
+    c["x"][:, 2000:] = -np.inf
+    r = dk.token_log_probs(x, t)
+    others = np.exp(np.delete(c["x"], 1234, 1)).sum(1)
+    # (3 d + 32) E of the others at distances of up to 21, and 64 steps beside 1 in 64 bits
+    assert np.all(np.abs(host(r.log_probs[[0, 513]]) + np.log1p(others)) <= others * 97 * E + 64 * 2.0 ** -53)
